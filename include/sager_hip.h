@@ -491,6 +491,121 @@ int sg_scatter_routed_f16(uint16_t* expert_y, const uint16_t* grouped_out, const
 int sg_scatter_rows_f16(uint16_t* dst, const uint16_t* src, const int* dst_rows, int n_rows,
                         int hidden, void* stream);
 
+/* ---- the verify window between the projections -------------------------
+ * A step of speculative decoding runs, for each of n_seq sequences, a window
+ * of 1..64 tokens: the last token and a chain or a tree of drafts.  The
+ * windows' tokens are the rows of one batch: sequence s has rows
+ * win_off[s] .. win_off[s+1]-1 (win_off: n_seq + 1 device ints, ascending),
+ * and n_tokens is the number of rows of the buffers; rows behind the last
+ * sequence are neither read nor written.  max_window (1..64) is the largest
+ * window; of a longer one, only its first max_window rows are seen.
+ *
+ * parent (n_tokens device ints) makes a window a tree: node i > 0 hangs on
+ * node parent[row] of its window, which must come before it (0 <= parent <
+ * i).  Node 0 is the root, whatever its parent says.  A node whose parent is
+ * anything else, and every node that hangs on it, is absent: it attends to
+ * nothing, nothing attends to it, and no draft of it is accepted.  parent =
+ * NULL: every window is a chain. */
+
+/* Residual addition, RMS norm and Q8_K in one launch, n_rows rows of n
+ * (a multiple of 256, at most 16384):
+ *   r = x + y, rounded to the buffers' type and stored to x_out;
+ *   xn = (r / sqrt(mean(r^2) + eps)) * w, rounded likewise (xn may be NULL);
+ *   xq = Q8_K(xn), as sg_quantize_q8_k / _f16 make it (xq may be NULL).
+ * y and x_out may both be NULL (r = x).  x_out may be x or y, xn may be x or
+ * y where there is no x_out in that place.  The sum of squares is fp32.
+ * These are the xn and moe_xq_in_ of sg_moe_layer_f16: the reference's fused
+ * norm and quantization (mmq.cu; session.cpp:1020-1022, 1129-1131), with the
+ * addition that the several-token output projection leaves to the caller. */
+int sg_add_rmsnorm_q8_k(const float* x, const float* y, float* x_out, const float* w, float eps,
+                        float* xn, sg_block_q8k* xq, int n, int n_rows, void* stream);
+int sg_add_rmsnorm_q8_k_f16(const uint16_t* x, const uint16_t* y, uint16_t* x_out, const float* w,
+                            float eps, uint16_t* xn, sg_block_q8k* xq, int n, int n_rows,
+                            void* stream);
+
+/* A paged fp16 key/value cache (a host struct; the pointers are the
+ * device's).  k and v: [n_layers][n_pages][n_kv_heads][page_size][head_dim],
+ * layer_stride elements from one layer to the next.  pages:
+ * [n_seq][pages_per_seq] page ids, sequence s's token p is slot
+ * p % page_size of page pages[s][p / page_size]; an id outside
+ * 0..n_pages-1 is an absent page, whose tokens are not attended to and not
+ * written.  length: [n_seq] tokens in the cache (more than the page table
+ * holds, or less than 0, counts as that many, or 0).  page_size is a power
+ * of two from 16 on, head_dim 64, 128 or 256. */
+typedef struct sg_kv_cache {
+  uint16_t* k;
+  uint16_t* v;
+  const int* pages;
+  const int* length;
+  long long layer_stride;
+  int n_layers, n_pages, page_size, pages_per_seq, n_kv_heads, head_dim;
+} sg_kv_cache;
+
+/* Attention of the windows' tokens over the cache and their own window:
+ *   out[t][h] = sum_j p_j v_j,  p = softmax over j of scale * q[t][h] . k_j,
+ * j running over the sequence's cached tokens and, in the window, over t's
+ * ancestors and t itself; head h reads kv head h / (n_heads / n_kv_heads).
+ * A node that is absent gets 0.  q [n_tokens][n_heads][head_dim], k and v
+ * [n_tokens][n_kv_heads][head_dim] with q_stride, k_stride and v_stride
+ * elements from one token to the next (slices of one projection's output),
+ * out contiguous.  k, v, the cache's k and v and their strides are 16-B
+ * aligned.  Scores, softmax statistics and sums are fp32; the weights p are
+ * rounded to fp16 for the product with v.  max_len bounds the caches'
+ * lengths for the split of the work; longer caches are right, but slower.
+ * Workspace: sg_attn_tree_workspace_bytes; it belongs to one call at a time.
+ * One launch, or two where the caches are cut into parts. */
+size_t sg_attn_tree_workspace_bytes(int n_seq, int n_tokens, int max_window, int max_len,
+                                    int n_heads, int n_kv_heads, int head_dim);
+int sg_attn_tree_f16(const uint16_t* q, const uint16_t* k, const uint16_t* v, long long q_stride,
+                     long long k_stride, long long v_stride, const sg_kv_cache* cache, int layer,
+                     const int* win_off, const int* parent, uint16_t* out, void* ws,
+                     size_t ws_bytes, int n_seq, int n_tokens, int max_window, int max_len,
+                     int n_heads, float scale, void* stream);
+
+/* The accepted tokens' keys and values written behind the caches, every
+ * layer in one launch: for i < n_path[s] (at most max_window), row
+ * win_off[s] + path[s][i] (path: [n_seq][max_window] nodes) of each layer's
+ * k and v [n_tokens][n_kv_heads][head_dim] becomes token length[s] + i.  A
+ * node outside its window, and a token past the page table or on an absent
+ * page, is left out.  length_out[s] = length[s] + n_path[s] (NULL: not
+ * written; not the cache's own length, which the launch still reads).  Two
+ * sequences must not share the pages that are written. */
+int sg_kv_commit_f16(const uint16_t* k, const uint16_t* v, long long k_stride, long long v_stride,
+                     long long k_layer_stride, long long v_layer_stride, const sg_kv_cache* cache,
+                     const int* win_off, const int* path, const int* n_path, int* length_out,
+                     int n_seq, int n_tokens, int max_window, void* stream);
+
+/* Which drafts the target's probabilities accept, from given random numbers.
+ * logits [n_tokens][vocab] fp32 are the target's after each node, p their
+ * softmax at the sequence's temperature (0, negative or NaN: all on the
+ * largest logit, the lowest index among equals; a NaN logit counts as
+ * -infinity).  tokens [n_tokens]: the node's token.  draft_probs [n_tokens]
+ * [vocab] fp32: the distribution that the node's token was drawn from, NULL:
+ * the token was chosen, q is 1 on it.  From the root on: with R = p of the
+ * node, its children c in index order are tried; c is accepted if
+ *   u_accept[c] * q_c(token_c) < R(token_c),
+ * and after a rejection R = max(R - q_c, 0) over its sum (left as it is
+ * where that sum is below 2^-30).  The first accepted child is the next
+ * node; where there is none, `next` is the first token at which the running
+ * sum of R passes u_sample[s] of its total.  u in [0, 1).
+ * Out: path [n_seq][max_window] (the root and the accepted nodes, then -1),
+ * n_path [n_seq], next [n_seq] (-1 if every logit of the last node is
+ * -infinity or the window is empty), prob [n_tokens] (may be NULL): the
+ * probability that the node is accepted once its parent is and its earlier
+ * siblings are not; 1 for roots, 0 for absent nodes.
+ * With draft_probs, a node's children past the first max_children (1..16)
+ * are absent; without, max_children is not read.  vocab is at most 2^24.
+ * Weights and sums are fp64, so that next does not depend on their order.
+ * Two launches, and one for each of max_children with draft_probs.
+ * Workspace: sg_tree_verify_workspace_bytes (max_children 0: no
+ * draft_probs). */
+size_t sg_tree_verify_workspace_bytes(int n_tokens, int vocab, int max_children);
+int sg_tree_verify(const float* logits, const int* tokens, const int* win_off, const int* parent,
+                   const float* draft_probs, const float* temperature, const float* u_accept,
+                   const float* u_sample, int* path, int* n_path, int* next, float* prob, void* ws,
+                   size_t ws_bytes, int n_seq, int n_tokens, int max_window, int vocab,
+                   int max_children, void* stream);
+
 /* ---- GGUF expert pool (load time, host + HBM) ------------------------
  * Replaces Weights::load_expert_pool (weights.cpp:800-870, over the GGUF v3
  * reader of gguf.hpp/gguf.cpp) and the device pointer table the session

@@ -22,6 +22,15 @@ _VP = ctypes.c_void_p
 _I = ctypes.c_int
 _F = ctypes.c_float
 _SZ = ctypes.c_size_t
+_LL = ctypes.c_longlong
+
+
+class KvCacheDesc(ctypes.Structure):
+    """sg_kv_cache of include/sager_hip.h."""
+    _fields_ = [("k", _VP), ("v", _VP), ("pages", _VP), ("length", _VP), ("layer_stride", _LL),
+                ("n_layers", _I), ("n_pages", _I), ("page_size", _I), ("pages_per_seq", _I),
+                ("n_kv_heads", _I), ("head_dim", _I)]
+
 
 # name -> (restype, argtypes); mirrors include/sager_hip.h
 SIGNATURES = {
@@ -78,6 +87,16 @@ SIGNATURES = {
     "sg_moe_prefill_workspace_bytes": (_SZ, [_I, _I, _I, _I, _I]),
     "sg_moe_prefill": (_I, [_VP, _VP, _VP, _VP, _VP, _VP, _VP, _VP, _VP, _VP, _VP, _VP, _VP,
                             _VP, _SZ, _I, _I, _I, _I, _I, _F, _VP]),
+    "sg_add_rmsnorm_q8_k": (_I, [_VP, _VP, _VP, _VP, _F, _VP, _VP, _I, _I, _VP]),
+    "sg_add_rmsnorm_q8_k_f16": (_I, [_VP, _VP, _VP, _VP, _F, _VP, _VP, _I, _I, _VP]),
+    "sg_attn_tree_workspace_bytes": (_SZ, [_I, _I, _I, _I, _I, _I, _I]),
+    "sg_attn_tree_f16": (_I, [_VP, _VP, _VP, _LL, _LL, _LL, _VP, _I, _VP, _VP, _VP, _VP, _SZ, _I,
+                              _I, _I, _I, _I, _F, _VP]),
+    "sg_kv_commit_f16": (_I, [_VP, _VP, _LL, _LL, _LL, _LL, _VP, _VP, _VP, _VP, _VP, _I, _I, _I,
+                              _VP]),
+    "sg_tree_verify_workspace_bytes": (_SZ, [_I, _I, _I]),
+    "sg_tree_verify": (_I, [_VP, _VP, _VP, _VP, _VP, _VP, _VP, _VP, _VP, _VP, _VP, _VP, _VP, _SZ,
+                            _I, _I, _I, _I, _I, _VP]),
     "sg_gguf_expert_dims": (_I, [ctypes.c_char_p, _VP, _VP, _VP, _VP, _VP]),
     "sg_expert_pool_load_gguf": (_I, [ctypes.c_char_p, _VP]),
     "sg_expert_pool_dims": (_I, [_VP, _VP, _VP, _VP, _VP]),

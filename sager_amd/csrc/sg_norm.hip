@@ -1,0 +1,188 @@
+// sg_norm.hip - residual addition, RMS norm and Q8_K of the result in one
+// launch: what lies between a layer's output projection and the next
+// projections, the router or the MoE layer (which take the fp16 rows and
+// their Q8_K).
+//
+//   r = x + y (rounded to the buffers' type: the residual stream as stored),
+//   s = 1 / sqrt(mean(r^2) + eps),   xn = (r * s) * w (rounded likewise),
+//   Q8_K(xn), the codes of sg_quantize_q8_k{,_f16}.
+//
+// The sum of squares is fp32: per lane in index order, then over the lanes.
+// Squares are summed in 32 bits because 16 would lose the small channels
+// beside the few large ones of a residual stream.
+#include "sg_common.hpp"
+
+namespace sg {
+
+// four consecutive values of a row, at the element's own alignment (buffers
+// may be slices of larger ones)
+typedef float f32x4_u __attribute__((ext_vector_type(4), aligned(4)));
+typedef uint16_t u16x4_u __attribute__((ext_vector_type(4), aligned(2)));
+
+template <typename T>
+struct Act;
+template <>
+struct Act<float> {
+  typedef f32x4_u vec;
+  static __device__ __forceinline__ float val(float v) { return v; }
+  static __device__ __forceinline__ float bits(float v) { return v; }
+};
+template <>
+struct Act<uint16_t> {
+  typedef u16x4_u vec;
+  static __device__ __forceinline__ float val(uint16_t v) { return half_bits_to_float(v); }
+  static __device__ __forceinline__ uint16_t bits(float v) { return f16b(v); }
+};
+
+template <typename T>
+__device__ __forceinline__ void load4(const T* p, float (&v)[4]) {
+  const typename Act<T>::vec q = *reinterpret_cast<const typename Act<T>::vec*>(p);
+#pragma unroll
+  for (int i = 0; i < 4; ++i) v[i] = Act<T>::val(q[i]);
+}
+// stores v rounded to T and leaves in v what was stored
+template <typename T>
+__device__ __forceinline__ void store4(T* p, float (&v)[4]) {
+  typename Act<T>::vec q;
+#pragma unroll
+  for (int i = 0; i < 4; ++i) {
+    q[i] = Act<T>::bits(v[i]);
+    v[i] = Act<T>::val(q[i]);
+  }
+  *reinterpret_cast<typename Act<T>::vec*>(p) = q;
+}
+template <typename T>
+__device__ __forceinline__ void round4(float (&v)[4]) {
+#pragma unroll
+  for (int i = 0; i < 4; ++i) v[i] = Act<T>::val(Act<T>::bits(v[i]));
+}
+
+// Sum over the wave in a fixed order, same value in every lane.
+__device__ __forceinline__ float wave_sum_dpp(float v) {
+  v += dpp_f<kDppXor1>(v);
+  v += dpp_f<kDppXor2>(v);
+  v += dpp_f<kDppHalfMirror>(v);
+  v += dpp_f<kDppMirror>(v);
+  return (readlane_f(v, 0) + readlane_f(v, 16)) + (readlane_f(v, 32) + readlane_f(v, 48));
+}
+
+// kNW waves per row, each up to kB blocks of 256 values held in registers
+// (lane l has values 4l..4l+3 of a block, the layout of the Q8_K quantizer).
+// kNW == 1: four rows per workgroup and no barrier.
+template <typename T, int kNW, int kB>
+__global__ void __launch_bounds__(kNW == 1 ? 256 : 64 * kNW)
+    add_rmsnorm_kernel(const T* x, const T* y, T* x_out, const float* w, T* xn,
+                       unsigned char* xq, int n, int n_rows, float eps) {
+  const int lane = threadIdx.x & 63;
+  const int wave = threadIdx.x >> 6;
+  const int part = kNW == 1 ? 0 : wave;
+  const long long row = kNW == 1 ? static_cast<long long>(blockIdx.x) * 4 + wave : blockIdx.x;
+  if (kNW == 1 && row >= n_rows) return;
+  const int nb = n / kQK;
+  const long long at = row * n + 4 * lane;
+  float v[kB][4], wv[kB][4];
+  float ss = 0.f;
+#pragma unroll
+  for (int i = 0; i < kB; ++i) {
+    const int b = part + kNW * i;
+    if (b < nb) {
+      load4(x + at + b * kQK, v[i]);
+      load4(w + b * kQK + 4 * lane, wv[i]);
+    }
+  }
+  if (y) {
+#pragma unroll
+    for (int i = 0; i < kB; ++i) {
+      const int b = part + kNW * i;
+      if (b < nb) {
+        float a[4];
+        load4(y + at + b * kQK, a);
+#pragma unroll
+        for (int j = 0; j < 4; ++j) v[i][j] += a[j];
+        store4(x_out + at + b * kQK, v[i]);
+      }
+    }
+  }
+#pragma unroll
+  for (int i = 0; i < kB; ++i)
+    if (part + kNW * i < nb)
+#pragma unroll
+      for (int j = 0; j < 4; ++j) ss = __builtin_fmaf(v[i][j], v[i][j], ss);
+  ss = wave_sum_dpp(ss);
+  if (kNW > 1) {
+    __shared__ float part_ss[kNW];
+    if (lane == 0) part_ss[wave] = ss;
+    __syncthreads();
+    ss = part_ss[0];
+#pragma unroll
+    for (int i = 1; i < kNW; ++i) ss += part_ss[i];
+  }
+  const float s = 1.f / sqrtf(ss / static_cast<float>(n) + eps);
+#pragma unroll
+  for (int i = 0; i < kB; ++i) {
+    const int b = part + kNW * i;
+    if (b < nb) {
+#pragma unroll
+      for (int j = 0; j < 4; ++j) v[i][j] = (v[i][j] * s) * wv[i][j];
+      if (xn)
+        store4(xn + at + b * kQK, v[i]);
+      else
+        round4<T>(v[i]);
+      if (xq) quantize_block_wave(v[i], xq + (row * nb + b) * kQ8Bytes, lane);
+    }
+  }
+}
+
+template <typename T, int kNW, int kB>
+static void norm_go(const T* x, const T* y, T* x_out, const float* w, float eps, T* xn,
+                    sg_block_q8k* xq, int n, int n_rows, hipStream_t s) {
+  const int grid = kNW == 1 ? (n_rows + 3) / 4 : n_rows;
+  hipLaunchKernelGGL((add_rmsnorm_kernel<T, kNW, kB>), dim3(grid),
+                     dim3(kNW == 1 ? 256 : 64 * kNW), 0, s, x, y, x_out, w, xn,
+                     reinterpret_cast<unsigned char*>(xq), n, n_rows, eps);
+}
+
+template <typename T>
+static int norm_launch(const T* x, const T* y, T* x_out, const float* w, float eps, T* xn,
+                       sg_block_q8k* xq, int n, int n_rows, void* stream, const char* nm) {
+  if (!x || !w || (!xn && !xq) || (y && !x_out) || (!y && x_out))
+    return set_error(SG_ERR_INVALID_ARGUMENT,
+                     "%s: x, w and xn or xq are needed, x_out exactly when there is y", nm);
+  if (n <= 0 || n % kQK != 0 || n_rows <= 0)
+    return set_error(SG_ERR_GEOMETRY, "%s: n=%d must be a positive multiple of 256, n_rows=%d",
+                     nm, n, n_rows);
+  if (n > 64 * kQK)
+    return set_error(SG_ERR_UNSUPPORTED, "%s: n=%d is over %d", nm, n, 64 * kQK);
+  if (reinterpret_cast<uintptr_t>(xq) % 4 || reinterpret_cast<uintptr_t>(x) % sizeof(T) ||
+      reinterpret_cast<uintptr_t>(y) % sizeof(T) || reinterpret_cast<uintptr_t>(x_out) % sizeof(T) ||
+      reinterpret_cast<uintptr_t>(xn) % sizeof(T) || reinterpret_cast<uintptr_t>(w) % 4)
+    return set_error(SG_ERR_INVALID_ARGUMENT, "%s: a buffer is not aligned to its elements", nm);
+  const hipStream_t s = static_cast<hipStream_t>(stream);
+  const int nb = n / kQK;
+  if (nb <= 8)
+    norm_go<T, 4, 2>(x, y, x_out, w, eps, xn, xq, n, n_rows, s);
+  else if (nb <= 32)
+    norm_go<T, 8, 4>(x, y, x_out, w, eps, xn, xq, n, n_rows, s);
+  else
+    norm_go<T, 16, 4>(x, y, x_out, w, eps, xn, xq, n, n_rows, s);
+  return check_launch(nm);
+}
+
+}  // namespace sg
+
+extern "C" {
+
+int sg_add_rmsnorm_q8_k(const float* x, const float* y, float* x_out, const float* w, float eps,
+                        float* xn, sg_block_q8k* xq, int n, int n_rows, void* stream) {
+  return sg::norm_launch<float>(x, y, x_out, w, eps, xn, xq, n, n_rows, stream,
+                                "sg_add_rmsnorm_q8_k");
+}
+
+int sg_add_rmsnorm_q8_k_f16(const uint16_t* x, const uint16_t* y, uint16_t* x_out, const float* w,
+                            float eps, uint16_t* xn, sg_block_q8k* xq, int n, int n_rows,
+                            void* stream) {
+  return sg::norm_launch<uint16_t>(x, y, x_out, w, eps, xn, xq, n, n_rows, stream,
+                                   "sg_add_rmsnorm_q8_k_f16");
+}
+
+}  // extern "C"
