@@ -1,19 +1,28 @@
 // sg_attn.hip - the windows' attention over a paged fp16 cache, and the
 // accepted tokens' way into it.
 //
-// For a kv head, the rows of a product are (node, query head of the group):
-// S^T = K Q^T and O^T = V^T P^T, 32 keys at a time and wave.  With keys as
-// the first product's rows, a lane of v_mfma_f32_16x16x32_f16 gets four
-// consecutive keys of one query row (keys 4g..4g+3 of each 16, g = lane / 16),
-// and since the order of a product's 32 terms is free, those eight weights
-// are the second product's operand as they are: p never leaves its lane.  V's
-// operand then is, per lane, one column of V at the same eight keys, which
-// ds_read_b64_tr_b16 reads from V's rows as they lie in memory.
+// For a kv head, the rows of a product are (node, query head of the group).
+// A workgroup takes a block of rows and a part of a sequence's keys, 64 keys
+// a step, in rows' groups of four waves:
+//   S^T = K Q^T   wave w has keys 16w..16w+15 and all rows of its group (Q in
+//                 registers);
+//   P             goes through LDS to the group's other waves;
+//   O^T = V^T P^T wave w has columns w D/4 .. of all keys.
+// So K and V are read from LDS once per group, no wave holds more than a
+// quarter of O, and nothing is joined at the end but the rows' sums.  With
+// keys as the first product's rows, a lane of v_mfma_f32_16x16x32_f16 gets
+// four consecutive keys of one query row, 8 B of P; and since the order of a
+// product's 32 terms is free, V's operand is, per lane, one column of V at
+// four and four consecutive keys, which ds_read_b64_tr_b16 reads from V's
+// rows as they lie in memory.
 //
-// The running maximum is a reference point `mref` per row that moves only
-// when a score passes it by 2^15: p = 2^(s - mref) fits fp16 (its largest
-// value is 2^16), and 2^(8+15) below it is still a normal number.  l = sum p
-// is kept per lane and joined at the end.
+// The running maximum is a reference point `mref` per row, common to the
+// group's waves, that moves only when a score passes it by 2^15: p =
+// 2^(s - mref) fits fp16 (its largest value is 2^16), and 2^(8+15) below it
+// is still a normal number.  Until a score does, the waves share nothing but
+// P; then all of them stop for it.  p is rounded to fp16 for the product
+// (2^-11 of each weight, below the output's own rounding to fp16 once a few
+// keys are averaged); l = sum p is fp32, of the unrounded p.
 #include "sg_window.hpp"
 
 namespace sg {
@@ -27,7 +36,7 @@ typedef __attribute__((address_space(3))) s4* lds_s4_p;
 // read through the scalar cache, whatever is stored in between
 typedef const __attribute__((address_space(4))) int* const_int_p;
 
-constexpr int kTile = 32;          // keys of a wave's step
+constexpr int kKeys = 64;          // keys of a step
 constexpr float kRise = 15.f;      // log2 above mref at which mref moves
 constexpr float kBelow = 8.f;      // log2 by which mref lies below the maximum it is set from
 constexpr float kLog2e = 1.44269504088896340736f;
@@ -41,20 +50,18 @@ struct AttnArgs {
   float* part_o;   // [split][token][head][D]
   float2* part_ml; // [split][token][head]: mref (log2), l
   int n_tokens, max_window, n_heads, n_kv, group, n_pages, page_log2, pages_per_seq;
-  int n_split, split_keys, row_blocks;
+  int n_split, split_keys, row_blocks, units;
   float scale_log2;
 };
 
-// The cached tokens of sequence s that the page table can hold.
-__device__ __forceinline__ int cached_len(const int* __restrict__ length, int s, int page_log2,
-                                          int pages_per_seq) {
+// The cached tokens of a sequence that the page table can hold.
+__device__ __forceinline__ int cached_len(int length, int page_log2, int pages_per_seq) {
   const long long cap = static_cast<long long>(pages_per_seq) << page_log2;
-  const long long len = length[s];
-  return static_cast<int>(len < 0 ? 0 : len > cap ? cap : len);
+  return static_cast<int>(length < 0 ? 0 : length > cap ? cap : length);
 }
 
-// Where chunk c (16 B) of key row r lies in its row: rows are a multiple of
-// 128 B apart, so 16 rows read at one chunk would share their banks.
+// Where chunk c (16 B) of row r lies in its row: rows are a multiple of 128 B
+// apart, so 16 rows read at one chunk would share their banks.
 template <int D>
 __device__ __forceinline__ int swz(int r) {
   return D == 64 ? (r >> 1) & 7 : r & 15;
@@ -74,174 +81,147 @@ __device__ __forceinline__ void dma16_ptr(uint32_t lds, const void* src) {
                : "s"(__builtin_amdgcn_readfirstlane(lds)), "v"(src)
                : "memory");
 }
-template <int N>
-__device__ __forceinline__ void wait_vm_upto() {
-  static_assert(N < 64, "the counter's range");
-  __builtin_amdgcn_s_waitcnt(0x0F70 | (N & 15) | (N >> 4 << 14));
-  __builtin_amdgcn_fence(__ATOMIC_ACQUIRE, "wavefront");
-}
 
-__device__ __forceinline__ const uint16_t* shfl_ptr(const uint16_t* p, int src) {
-  const uint64_t v = reinterpret_cast<uintptr_t>(p);
-  const uint32_t lo = __shfl(static_cast<uint32_t>(v), src);
-  const uint32_t hi = __shfl(static_cast<uint32_t>(v >> 32), src);
-  return reinterpret_cast<const uint16_t*>(static_cast<uintptr_t>(hi) << 32 | lo);
-}
-
-// One tile of a wave: which of its keys there are, and whether it needs more
-// than the plain path (a page boundary past 16 keys, an absent page, the
-// window's keys, keys past the end).
-struct TileKind {
-  uint32_t present;  // bit r: key r of the tile exists
-  bool plain;
+// Bytes of LDS: K and V of two steps, P, the rows' maxima and sums of the four
+// waves, the nodes' ancestors, and the flags.
+template <int D, int RT, int RW>
+struct AttnLds {
+  static constexpr uint32_t kStep = kKeys * D * 2;
+  static constexpr uint32_t kRows = 16 * RT * RW;
+  static constexpr uint32_t kP = 4 * kStep;
+  static constexpr uint32_t kMax = kP + kRows * kKeys * 2;
+  static constexpr uint32_t kSeen = kMax + 4 * kRows * 4;
+  static constexpr uint32_t kFlags = kSeen + kMaxWindow * 8;
+  static constexpr uint32_t kBytes = kFlags + 16;
 };
 
-template <int D, int RT>
-struct Attn {
-  static constexpr int CH = D / 8;         // 16-B chunks of a row
-  static constexpr int RPI = 64 / CH;      // rows of a copy instruction
-  static constexpr int NI = kTile / RPI;   // copy instructions of a tile
-  static constexpr int DT = D / 16;        // 16-column tiles of the output
-  static constexpr int KK = D / 32;        // steps of the first product
-  static constexpr uint32_t kTileBytes = kTile * D * 2;
+// RT: tiles of 16 rows of a group; RW: groups of four waves.
+template <int D, int RT, int RW>
+__global__ void __launch_bounds__(256 * RW) attn_tree_kernel(const AttnArgs a) {
+  typedef AttnLds<D, RT, RW> L;
+  constexpr int CH = D / 8;       // 16-B chunks of a row
+  constexpr int RPI = 64 / CH;    // rows of a copy instruction
+  constexpr int NI = 16 / RPI;    // copy instructions of a wave's 16 keys
+  constexpr int KK = D / 32;      // steps of the first product
+  constexpr int DQ = D / 64;      // 16-column tiles of a wave's part of O
+  constexpr int kRows = L::kRows;
+  extern __shared__ __attribute__((aligned(16))) unsigned char lds[];
+  const uint32_t lds0 = static_cast<uint32_t>(
+      reinterpret_cast<uintptr_t>((__attribute__((address_space(3))) unsigned char*)lds));
+  int* flags = reinterpret_cast<int*>(lds + L::kFlags);  // rise[2], odd[2]
+  float* mx = reinterpret_cast<float*>(lds + L::kMax);
+  uint64_t* seen = reinterpret_cast<uint64_t*>(lds + L::kSeen);  // node: whom it sees
+  const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+  const int kw = wave & 3, rg = wave >> 2;
+  const int lane = threadIdx.x & 63, col = lane & 15, grp = lane >> 4;
 
-  const AttnArgs& a;
-  int lane, col, grp;
-  int seq, h, len, total;  // cached keys, cached + window
-  Window win;
-  const int* table;
-  uint32_t kbuf, vbuf;  // LDS byte addresses of this wave's buffers
-  const unsigned char* lds;
+  // The row blocks of a unit (part, kv head, sequence) are 8 workgroups apart:
+  // on one XCD, whose L2 then reads the unit's keys once.
+  const int id = blockIdx.x;
+  const int oct = id / (8 * a.row_blocks), in = id - oct * 8 * a.row_blocks;
+  const int rb = in >> 3;
+  int unit = oct * 8 + (in & 7);
+  if (unit >= a.units) return;
+  const int split = unit % a.n_split;
+  unit /= a.n_split;
+  const int h = unit % a.n_kv, seq = unit / a.n_kv;
+  const Window win = window_of(a.win_off, seq, a.n_tokens, a.max_window);
+  const int rows = win.n * a.group;
+  if (rb * kRows >= rows) return;
+  const int len = cached_len(((const_int_p)a.length)[seq], a.page_log2, a.pages_per_seq);
+  const int total = len + win.n;
+  const const_int_p table = (const_int_p)(a.pages + static_cast<long long>(seq) * a.pages_per_seq);
+  const int steps = (total + kKeys - 1) / kKeys;
+  const int per = a.split_keys / kKeys;
+  const long long first = static_cast<long long>(split) * per;
+  const int s_end = split == a.n_split - 1 || first + per > steps ? steps
+                                                                  : static_cast<int>(first + per);
+  int step = first < s_end ? static_cast<int>(first) : s_end;
 
-  __device__ __forceinline__ const uint16_t* cache_row(const uint16_t* c, int page, int slot) const {
+  // ---- copies: wave kw brings keys 16 kw.. of a step (of two groups, the
+  // first brings K's, the second V's) ----
+  const uint32_t blk = kw * 16 * D * 2;
+  auto page_of = [&](int s) {
+    const int j = s * kKeys + 16 * kw;
+    return j < len ? table[j >> a.page_log2] : -1;
+  };
+  auto page_ok = [&](int p) { return static_cast<uint32_t>(p) < static_cast<uint32_t>(a.n_pages); };
+  auto issue = [&](int s, int page) {
+    const int j = s * kKeys + 16 * kw;
+    const uint32_t buf = lds0 + (s & 1) * 2 * L::kStep + blk;
     const long long at =
-        ((static_cast<long long>(page) * a.n_kv + h) << a.page_log2) + slot;
-    return c + at * D;
-  }
-  __device__ __forceinline__ bool page_ok(int p) const {
-    return static_cast<uint32_t>(p) < static_cast<uint32_t>(a.n_pages);
-  }
-
-  // Issues the copies of a tile's K (or V) rows; returns its kind.
-  template <bool kV>
-  __device__ __forceinline__ TileKind issue(int tile) const {
-    const int j0 = tile * kTile;
-    const uint16_t* c = kV ? a.vc : a.kc;
-    const uint32_t buf = kV ? vbuf : kbuf;
-    TileKind kind{0xFFFFFFFFu, false};
-    if (j0 + kTile <= len) {  // pages of 16 hold half a tile, larger ones all of it
-      const const_int_p ids = (const_int_p)(table);
-      const int p0 = ids[j0 >> a.page_log2];
-      const int p1 = ids[(j0 + 16) >> a.page_log2];
-      if (page_ok(p0) && page_ok(p1)) {
-        kind.plain = true;
-        const int mask = (1 << a.page_log2) - 1;
-        const uint16_t* b0 = uniform_ptr(cache_row(c, p0, j0 & mask));
-        const uint16_t* b1 = uniform_ptr(cache_row(c, p1, (j0 + 16) & mask) - 16 * D);
-        const int sub = lane / CH;
+        (((static_cast<long long>(page) * a.n_kv + h) << a.page_log2) +
+         (j & ((1 << a.page_log2) - 1))) * D;
+    if (j + 16 <= len && page_ok(page)) {
+      const uint16_t* kb = uniform_ptr((RW == 2 && rg ? a.vc : a.kc) + at);
+      const uint16_t* vb = uniform_ptr(a.vc + at);
+      int ln = lane;
+      if (RT >= 3) asm("" : "+v"(ln));  // (the offsets made anew: registers are short)
 #pragma unroll
-        for (int i = 0; i < NI; ++i) {
-          const int row = i * RPI + sub;
-          const uint32_t voff = row * (D * 2) + (((lane % CH) ^ swz<D>(row)) << 4);
-          dma16_base(buf + i * 1024, voff, i * RPI < 16 ? b0 : b1);
+      for (int i = 0; i < NI; ++i) {
+        const int row = i * RPI + ln / CH;
+        const uint32_t voff = row * (D * 2) + (((ln % CH) ^ swz<D>(row)) << 4);
+        if (RW == 1) {
+          dma16_base(buf + i * 1024, voff, kb);
+          dma16_base(buf + L::kStep + i * 1024, voff, vb);
+        } else {
+          dma16_base(buf + (rg ? L::kStep : 0) + i * 1024, voff, kb);
         }
-        return kind;
+      }
+    } else if (j < total) {
+      // rows of the cache, then of the window; what is not there reads a
+      // window row and is masked
+      const int n_cache = page_ok(page) ? min(len - j, 16) : 0;
+      const bool k_too = RW == 1 || rg == 0, v_too = RW == 1 || rg == 1;
+#pragma unroll 1
+      for (int i = 0; i < NI; ++i) {
+        const int row = i * RPI + lane / CH;
+        const int c = ((lane % CH) ^ swz<D>(row)) * 8;
+        const long long w = win.off + min(max(j + row - len, 0), win.n - 1);
+        const bool cached = row < n_cache;
+        if (k_too)
+          dma16_ptr(buf + i * 1024,
+                    (cached ? a.kc + at + row * D : a.k + w * a.k_stride + h * D) + c);
+        if (v_too)
+          dma16_ptr(buf + L::kStep + i * 1024,
+                    (cached ? a.vc + at + row * D : a.v + w * a.v_stride + h * D) + c);
       }
     }
-    // lane r (and r + 32) finds key r
-    const int j = j0 + (lane & 31);
-    const uint16_t* w = kV ? a.v : a.k;
-    const long long ws = kV ? a.v_stride : a.k_stride;
-    const uint16_t* src = w + static_cast<long long>(win.off) * ws + h * D;
-    bool there = false;
-    if (j < len) {
-      const int p = table[j >> a.page_log2];
-      there = page_ok(p);
-      if (there) src = cache_row(c, p, j & ((1 << a.page_log2) - 1));
-    } else if (j < total) {
-      there = true;
-      src += static_cast<long long>(j - len) * ws;
-    }
-    kind.present = static_cast<uint32_t>(__ballot(there));
-#pragma unroll 2
-    for (int i = 0; i < NI; ++i) {
-      const int row = i * RPI + lane / CH;
-      const uint16_t* s = shfl_ptr(src, row);
-      dma16_ptr(buf + i * 1024, s + ((lane % CH) ^ swz<D>(row)) * 8);
-    }
-    return kind;
+  };
+  // bit r: key 16 kw + r of the step is there
+  auto present = [&](int s, int page) {
+    const int j = s * kKeys + 16 * kw;
+    const int nc = min(max(len - j, 0), 16), nw = min(max(total - j, 0), 16);
+    const uint32_t c = (1u << nc) - 1;
+    return ((1u << nw) - 1) & (page_ok(page) ? 0xFFFFu : ~c);
+  };
+
+  int page = page_of(step), page_next = 0;
+  if (step < s_end) {
+    issue(step, page);
+    page_next = page_of(step + 1);
   }
-};
+  if (threadIdx.x < 4) flags[threadIdx.x] = 0;
 
-// One workgroup of four waves: one part of a sequence's keys, one kv head, a
-// block of 16 RT rows.  The waves take the part's tiles in turn, each with
-// its own K and V buffer in LDS, so that no barrier orders them: while a
-// wave multiplies by V, its next K is under way, and the other way round.
-template <int D, int RT>
-__global__ void __launch_bounds__(256) attn_tree_kernel(const AttnArgs a) {
-  typedef Attn<D, RT> A;
-  constexpr int CH = A::CH, RPI = A::RPI, NI = A::NI, DT = A::DT, KK = A::KK;
-  constexpr int kRows = 16 * RT;
-  extern __shared__ __attribute__((aligned(16))) unsigned char lds[];
-  const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
-  A t{a};
-  t.lane = threadIdx.x & 63;
-  t.col = t.lane & 15;
-  t.grp = t.lane >> 4;
-  int id = blockIdx.x;
-  const int split = id % a.n_split;
-  id /= a.n_split;
-  const int rb = id % a.row_blocks;
-  id /= a.row_blocks;
-  t.h = id % a.n_kv;
-  t.seq = id / a.n_kv;
-  t.win = window_of(a.win_off, t.seq, a.n_tokens, a.max_window);
-  const int rows = t.win.n * a.group;
-  if (rb * kRows >= rows) return;
-  t.len = cached_len(a.length, t.seq, a.page_log2, a.pages_per_seq);
-  t.total = t.len + t.win.n;
-  t.table = a.pages + static_cast<long long>(t.seq) * a.pages_per_seq;
-  t.lds = lds;
-  const uint32_t lds0 = static_cast<uint32_t>(reinterpret_cast<uintptr_t>(
-      (__attribute__((address_space(3))) unsigned char*)lds));
-  t.kbuf = lds0 + wave * 2 * A::kTileBytes;
-  t.vbuf = t.kbuf + A::kTileBytes;
-  const unsigned char* kb = lds + wave * 2 * A::kTileBytes;
-  unsigned char* vb = lds + wave * 2 * A::kTileBytes + A::kTileBytes;
-
-  const int tiles = (t.total + kTile - 1) / kTile;
-  const int per = a.split_keys / kTile;
-  const long long first = static_cast<long long>(split) * per;
-  const int t_end = split == a.n_split - 1 ? tiles
-                                           : static_cast<int>(first + per < tiles ? first + per : tiles);
-  int tile = first + wave < t_end ? static_cast<int>(first) + wave : t_end;
-
-  TileKind kind{0, true};
-  if (tile < t_end) {
-    t.template issue<false>(tile);
-    kind = t.template issue<true>(tile);
-  }
-
-  // Q's rows, while the first copies are under way
-  const uint64_t up_all = ancestors(a.parent, t.win, t.lane);
+  // ---- Q's rows, while the first copies are under way ----
+  if (wave == 4 * RW - 1) seen[lane] = ancestors(a.parent, win, lane);
+  const int row0 = rb * kRows + rg * 16 * RT;
+  auto node_of = [&](int rt) { return min(row0 + rt * 16 + col, rows - 1) / a.group; };
   h8 qf[RT][KK];
-  uint64_t up[RT];
 #pragma unroll
   for (int rt = 0; rt < RT; ++rt) {
-    const int r = rb * kRows + rt * 16 + t.col;
+    const int r = min(row0 + rt * 16 + col, rows - 1);  // (a row past the end repeats the last)
     const int node = r / a.group, g = r - node * a.group;
-    up[rt] = __shfl(up_all, r < rows ? node : 0);
-    const uint16_t* qp = a.q + static_cast<long long>(t.win.off + (r < rows ? node : 0)) * a.q_stride +
-                         (t.h * a.group + (r < rows ? g : 0)) * D;
+    const uint16_t* qp = a.q + static_cast<long long>(win.off + node) * a.q_stride +
+                         (h * a.group + g) * D;
 #pragma unroll
     for (int s = 0; s < KK; ++s) {
-      u32x4 w = *reinterpret_cast<const u32x4_u*>(qp + s * 32 + t.grp * 8);
-      if (r >= rows) w = (u32x4){0, 0, 0, 0};
+      const u32x4 w = *reinterpret_cast<const u32x4_u*>(qp + s * 32 + grp * 8);
       qf[rt][s] = __builtin_bit_cast(h8, w);
     }
   }
 
-  f4 acc[RT][DT];
+  f4 acc[RT][DQ];
   float mref[RT], l[RT];
   bool begun[RT];
 #pragma unroll
@@ -250,262 +230,323 @@ __global__ void __launch_bounds__(256) attn_tree_kernel(const AttnArgs a) {
     l[rt] = 0.f;
     begun[rt] = false;
 #pragma unroll
-    for (int d = 0; d < DT; ++d) acc[rt][d] = (f4){0.f, 0.f, 0.f, 0.f};
+    for (int d = 0; d < DQ; ++d) acc[rt][d] = (f4){0.f, 0.f, 0.f, 0.f};
   }
+  // P: [row][two halves of 32 keys][grp][two blocks of 16 keys][4], 16-B pieces
+  // swizzled over the row's eight
+  unsigned char* const pl = lds + L::kP + rg * 16 * RT * 128;
+  const int psw = (col >> 1) & 7;
+  // K's pieces st * 4 + grp of row col, swizzled: four offsets, the rest is added.  V's: columns
+  // kw D/4 + 16 d.. of row 4 grp + col / 4 of a 16-key block.
+  constexpr int KO = KK < 4 ? KK : 4;
+  uint32_t koff[KO], voff[DQ];
+#pragma unroll
+  for (int i = 0; i < KO; ++i)
+    koff[i] = blk + col * (D * 2) + (((i * 4) ^ grp ^ swz<D>(col)) << 4);
+#pragma unroll
+  for (int d = 0; d < DQ; ++d)
+    voff[d] = lds0 + L::kStep + (4 * grp + (col >> 2)) * (D * 2) +
+              (((2 * d) ^ (kw * (CH / 4) + ((col & 3) >> 1)) ^ swz<D>(4 * grp + (col >> 2))) << 4) +
+              (col & 1) * 8;
+  unsigned char* const p_out = pl + col * 128 + ((((kw >> 1) * 4 + grp) ^ psw) << 4) + (kw & 1) * 8;
 
-  while (tile < t_end) {
-    const int next = tile + 4;
-    wait_vm_upto<NI>();  // K is here; V's NI copies may be under way
-    f4 s[2][RT];
-#pragma unroll
-    for (int kt = 0; kt < 2; ++kt)
-#pragma unroll
-      for (int rt = 0; rt < RT; ++rt) s[kt][rt] = (f4){0.f, 0.f, 0.f, 0.f};
-#pragma unroll
-    for (int st = 0; st < KK; ++st)
-#pragma unroll
-      for (int kt = 0; kt < 2; ++kt) {
-        const int row = kt * 16 + t.col;
-        const h8 kf = *reinterpret_cast<const h8*>(kb + row * (D * 2) +
-                                                   (((st * 4 + t.grp) ^ swz<D>(row)) << 4));
-#pragma unroll
-        for (int rt = 0; rt < RT; ++rt)
-          s[kt][rt] = __builtin_amdgcn_mfma_f32_16x16x32_f16(kf, qf[rt][st], s[kt][rt], 0, 0, 0);
-      }
-    const TileKind now = kind;
-    wait_lds();
-    if (next < t_end) t.template issue<false>(next);
+  for (; step < s_end; ++step) {
+    const int par = step & 1;
+    wait_vm();
+    bar();  // everybody's copies of this step are here, and nobody reads the other buffers or P
+    if (step + 1 < s_end) issue(step + 1, page_next);
+    const int page_then = step + 2 < s_end ? page_of(step + 2) : -1;
+    if (threadIdx.x == 0) flags[par ^ 1] = flags[2 + (par ^ 1)] = 0;
+    const unsigned char* kb = lds + par * 2 * L::kStep;
+    unsigned char* vb = lds + par * 2 * L::kStep + L::kStep;
+    const int j0 = step * kKeys + 16 * kw;
+    const uint32_t there = present(step, page);
+    const bool plain = j0 + 16 <= len && there == 0xFFFFu;
 
-    float e[RT][8];
-    bool move = false;
-    float top[RT];
-#pragma unroll
-    for (int rt = 0; rt < RT; ++rt) {
-#pragma unroll
-      for (int i = 0; i < 8; ++i)
-        e[rt][i] = __builtin_fmaf(s[i >> 2][rt][i & 3], a.scale_log2, -mref[rt]);
-      if (!now.plain) {
-        // bit r of `see`: key r is there and this lane's row sees it
-        const int w0 = tile * kTile - t.len;  // key 0's window node, if not negative
-        const uint32_t tree = w0 >= 0    ? static_cast<uint32_t>(up[rt] >> w0)
-                              : w0 > -32 ? static_cast<uint32_t>(up[rt] << -w0) | ((1u << -w0) - 1)
-                                         : 0xFFFFFFFFu;
-        const uint32_t see = (now.present & tree) >> (4 * t.grp);
-#pragma unroll
-        for (int i = 0; i < 8; ++i)
-          e[rt][i] = see & 1u << ((i >> 2) * 16 + (i & 3)) ? e[rt][i] : -INFINITY;
-      }
-      top[rt] = e[rt][0];
-#pragma unroll
-      for (int i = 1; i < 8; ++i) top[rt] = fmaxf(top[rt], e[rt][i]);
-      move |= top[rt] > kRise || (!begun[rt] && top[rt] > -INFINITY);
-    }
-    if (__any(move)) {
-#pragma unroll
-      for (int rt = 0; rt < RT; ++rt) {
-        float m = fmaxf(top[rt], __shfl_xor(top[rt], 16));
-        m = fmaxf(m, __shfl_xor(m, 32));
-        const bool set = m > kRise || (!begun[rt] && m > -INFINITY);
-        const float by = set ? m - kBelow : 0.f;
-        const float f = !set ? 1.f : begun[rt] ? __builtin_amdgcn_exp2f(-by) : 0.f;
-        mref[rt] += by;
-        l[rt] *= f;
-#pragma unroll
-        for (int d = 0; d < DT; ++d) acc[rt][d] *= f;
-#pragma unroll
-        for (int i = 0; i < 8; ++i) e[rt][i] -= by;
-        begun[rt] |= set;
-      }
-    }
-    h8 p[RT];
-#pragma unroll
-    for (int rt = 0; rt < RT; ++rt) {
-#pragma unroll
-      for (int i = 0; i < 8; ++i) {
-        e[rt][i] = __builtin_amdgcn_exp2f(e[rt][i]);
-        p[rt][i] = static_cast<_Float16>(e[rt][i]);
-      }
-      l[rt] += ((e[rt][0] + e[rt][1]) + (e[rt][2] + e[rt][3])) +
-               ((e[rt][4] + e[rt][5]) + (e[rt][6] + e[rt][7]));
-    }
-
-    if (next < t_end)
-      wait_vm_upto<NI>();  // V is here; the next K's copies may be under way
-    else
-      wait_vm_upto<0>();
-    if (!now.plain) {
-      // Rows that no query sees become 0 (0 times what lies there need not
-      // be 0).  A window row that some queries see and others do not is
-      // looked through for infinities and NaN: they are taken out for the
-      // product and added to the queries that see them, one by one.
-      const int j0 = tile * kTile;
+    if (!plain && rg == RW - 1) {
+      // Rows that nobody sees become 0 (0 times what lies there need not be
+      // 0).  Window rows, which some queries see and others do not, are looked
+      // through for infinities and NaN.
       bool odd = false;
-#pragma unroll 2
+#pragma unroll 1
       for (int i = 0; i < NI; ++i) {
-        const int row = i * RPI + t.lane / CH;
-        u32x4* at = reinterpret_cast<u32x4*>(vb + i * 1024 + 16 * t.lane);
-        if (!(now.present >> row & 1)) {
+        const int row = i * RPI + lane / CH;
+        u32x4* at = reinterpret_cast<u32x4*>(vb + blk + i * 1024 + 16 * lane);
+        if (!(there >> row & 1)) {
           *at = (u32x4){0, 0, 0, 0};
-        } else if (j0 + row >= t.len && t.win.n > 1) {
+        } else if (j0 + row >= len && win.n > 1) {
           const u32x4 w = *at;
 #pragma unroll
           for (int c = 0; c < 4; ++c)
             odd |= (w[c] & 0x7C00u) == 0x7C00u || (w[c] & 0x7C000000u) == 0x7C000000u;
         }
       }
-      wait_lds();
-      if (__any(odd)) {
-        for (int r = 0; r < kTile; ++r) {
-          if (!(now.present >> r & 1) || j0 + r < t.len) continue;
-          const int from = t.col + 16 * ((r & 15) >> 2);  // the lane that has key r's weight
-#pragma unroll
-          for (int rt = 0; rt < RT; ++rt) {
-            float mine = 0.f;
-#pragma unroll
-            for (int i = 0; i < 8; ++i)
-              if (i == ((r >> 4) * 4 + (r & 3))) mine = e[rt][i];
-            const float w = __shfl(mine, from);
-            const bool see = up[rt] >> (j0 + r - t.len & 63) & 1;
-#pragma unroll
-            for (int d = 0; d < DT; ++d)
-#pragma unroll
-              for (int i = 0; i < 4; ++i) {
-                const int c = d * 16 + 4 * t.grp + i;
-                const uint16_t b = *reinterpret_cast<const uint16_t*>(
-                    vb + r * (D * 2) + (((c >> 3) ^ swz<D>(r)) << 4) + (c & 7) * 2);
-                acc[rt][d][i] += see && (b & 0x7C00) == 0x7C00 ? w * half_bits_to_float(b) : 0.f;
-              }
-          }
-        }
-        wait_lds();
-        for (int i = 0; i < NI; ++i) {
-          const int row = i * RPI + t.lane / CH;
-          if (j0 + row < t.len) continue;
-          uint16_t* at = reinterpret_cast<uint16_t*>(vb + i * 1024 + 16 * t.lane);
-          for (int c = 0; c < 8; ++c)
-            if ((at[c] & 0x7C00) == 0x7C00) at[c] = 0;
-        }
-        wait_lds();
-      }
+      if (__any(odd) && lane == 0) flags[2 + par] = 1;
     }
+
+    f4 s[RT];
 #pragma unroll
-    for (int d = 0; d < DT; ++d) {
-      h8 vf;
+    for (int rt = 0; rt < RT; ++rt) s[rt] = (f4){0.f, 0.f, 0.f, 0.f};
 #pragma unroll
-      for (int kt = 0; kt < 2; ++kt) {
-        const int row = kt * 16 + 4 * t.grp + (t.col >> 2);
-        const uint32_t off = row * (D * 2) + (((2 * d + ((t.col & 3) >> 1)) ^ swz<D>(row)) << 4) +
-                             (t.col & 1) * 8;
-        const h4 x = __builtin_bit_cast(
-            h4, __builtin_amdgcn_ds_read_tr16_b64_v4i16(
-                    (lds_s4_p)(static_cast<uintptr_t>(t.vbuf + off))));
-#pragma unroll
-        for (int i = 0; i < 4; ++i) vf[kt * 4 + i] = x[i];
-      }
+    for (int st = 0; st < KK; ++st) {
+      const h8 kf = *reinterpret_cast<const h8*>(kb + koff[st % KO] + st / KO * 256);
 #pragma unroll
       for (int rt = 0; rt < RT; ++rt)
-        acc[rt][d] = __builtin_amdgcn_mfma_f32_16x16x32_f16(vf, p[rt], acc[rt][d], 0, 0, 0);
+        s[rt] = __builtin_amdgcn_mfma_f32_16x16x32_f16(kf, qf[rt][st], s[rt], 0, 0, 0);
     }
-    wait_lds();
-    if (next < t_end) kind = t.template issue<true>(next);
-    tile = next;
+
+    float e[RT][4], top[RT], sum[RT];
+    bool rise = false;
+#pragma unroll
+    for (int rt = 0; rt < RT; ++rt) {
+#pragma unroll
+      for (int i = 0; i < 4; ++i) e[rt][i] = __builtin_fmaf(s[rt][i], a.scale_log2, -mref[rt]);
+      if (!plain) {
+        // bit r of `see`: key r is there and this lane's row sees it
+        const uint64_t up = seen[node_of(rt)];
+        const int w0 = j0 - len;  // key 0's window node, if not negative
+        const uint32_t tree = w0 >= 0    ? static_cast<uint32_t>(up >> (w0 & 63))
+                              : w0 > -16 ? static_cast<uint32_t>(up << -w0) | ((1u << -w0) - 1)
+                                         : 0xFFFFu;
+        const uint32_t see = (there & tree) >> (4 * grp);
+#pragma unroll
+        for (int i = 0; i < 4; ++i) e[rt][i] = see & 1u << i ? e[rt][i] : -INFINITY;
+      }
+      top[rt] = fmaxf(fmaxf(e[rt][0], e[rt][1]), fmaxf(e[rt][2], e[rt][3]));
+      rise |= top[rt] > kRise || (!begun[rt] && top[rt] > -INFINITY);
+      float p[4];
+      h4 ph;
+#pragma unroll
+      for (int i = 0; i < 4; ++i) {
+        p[i] = __builtin_amdgcn_exp2f(e[rt][i]);
+        ph[i] = static_cast<_Float16>(p[i]);
+      }
+      sum[rt] = (p[0] + p[1]) + (p[2] + p[3]);
+      *reinterpret_cast<h4*>(p_out + rt * 16 * 128) = ph;
+    }
+    if (__any(rise) && lane == 0) flags[par] = 1;
+    bar();  // P is here
+
+    if (flags[par]) {
+      // The reference points move: the rows' maxima over the group's waves,
+      // then P once more.
+#pragma unroll
+      for (int rt = 0; rt < RT; ++rt) {
+        float m = fmaxf(top[rt], __shfl_xor(top[rt], 16));
+        m = fmaxf(m, __shfl_xor(m, 32));
+        if (grp == 0) mx[kw * kRows + (rg * RT + rt) * 16 + col] = m;
+      }
+      bar();
+#pragma unroll
+      for (int rt = 0; rt < RT; ++rt) {
+        const float* mr = mx + (rg * RT + rt) * 16 + col;
+        const float m = fmaxf(fmaxf(mr[0], mr[kRows]), fmaxf(mr[2 * kRows], mr[3 * kRows]));
+        const bool set = m > kRise || (!begun[rt] && m > -INFINITY);
+        const float by = set ? m - kBelow : 0.f;
+        const float f = !set ? 1.f : begun[rt] ? __builtin_amdgcn_exp2f(-by) : 0.f;
+        mref[rt] += by;
+        l[rt] *= f;
+#pragma unroll
+        for (int d = 0; d < DQ; ++d) acc[rt][d] *= f;
+        begun[rt] |= set;
+        float p[4];
+        h4 ph;
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+          p[i] = __builtin_amdgcn_exp2f(e[rt][i] - by);
+          ph[i] = static_cast<_Float16>(p[i]);
+        }
+        sum[rt] = (p[0] + p[1]) + (p[2] + p[3]);
+        *reinterpret_cast<h4*>(p_out + rt * 16 * 128) = ph;
+      }
+      bar();
+    }
+#pragma unroll
+    for (int rt = 0; rt < RT; ++rt) l[rt] += sum[rt];
+
+    if (flags[2 + par]) {
+      // Infinities and NaN in the window's V: added one by one to the rows
+      // that see them, then taken out for the product.
+#pragma unroll 1
+      for (int r = 0; r < kKeys; ++r) {
+        const int node = step * kKeys + r - len;
+        if (node < 0 || node >= win.n) continue;
+        const int piece = (r >> 5) * 4 + ((r & 15) >> 2);
+#pragma unroll
+        for (int rt = 0; rt < RT; ++rt) {
+          const float w = half_bits_to_float(*reinterpret_cast<const uint16_t*>(
+              pl + (rt * 16 + col) * 128 + ((piece ^ psw) << 4) + (r >> 4 & 1) * 8 + (r & 3) * 2));
+          const bool see = seen[node_of(rt)] >> node & 1;
+#pragma unroll
+          for (int d = 0; d < DQ; ++d)
+#pragma unroll
+            for (int i = 0; i < 4; ++i) {
+              const int c = kw * (D / 4) + d * 16 + 4 * grp + i;
+              const uint16_t b = *reinterpret_cast<const uint16_t*>(
+                  vb + r * (D * 2) + (((c >> 3) ^ swz<D>(r)) << 4) + (c & 7) * 2);
+              acc[rt][d][i] += see && (b & 0x7C00) == 0x7C00 ? w * half_bits_to_float(b) : 0.f;
+            }
+        }
+      }
+      bar();
+      if (rg == RW - 1)
+#pragma unroll 1
+        for (int i = 0; i < NI; ++i) {
+          const int row = i * RPI + lane / CH;
+          uint16_t* at = reinterpret_cast<uint16_t*>(vb + blk + i * 1024 + 16 * lane);
+#pragma unroll 1
+          for (int c = 0; c < 8; ++c)
+            if (j0 + row >= len && (at[c] & 0x7C00) == 0x7C00) at[c] = 0;
+        }
+      bar();
+    }
+
+    const uint32_t vl = par * 2 * L::kStep;
+#pragma unroll
+    for (int st = 0; st < 2; ++st) {
+      h8 pf[RT];
+#pragma unroll
+      for (int rt = 0; rt < RT; ++rt)
+        pf[rt] = *reinterpret_cast<const h8*>(pl + (rt * 16 + col) * 128 +
+                                              (((st * 4 + grp) ^ psw) << 4));
+#pragma unroll
+      for (int d = 0; d < DQ; ++d) {
+        h8 vf;
+#pragma unroll
+        for (int b = 0; b < 2; ++b) {
+          const h4 x = __builtin_bit_cast(
+              h4, __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_s4_p)(static_cast<uintptr_t>(
+                      vl + voff[d] + (st * 2 + b) * 16 * D * 2))));
+#pragma unroll
+          for (int i = 0; i < 4; ++i) vf[b * 4 + i] = x[i];
+        }
+#pragma unroll
+        for (int rt = 0; rt < RT; ++rt)
+          acc[rt][d] = __builtin_amdgcn_mfma_f32_16x16x32_f16(vf, pf[rt], acc[rt][d], 0, 0, 0);
+      }
+    }
+    page = page_next;
+    page_next = page_then;
   }
 
-  // Join the four waves: O = sum over waves of O_w 2^(mref_w - m).  A wave's
-  // 16-B pieces of O lie at piece ^ row, against bank conflicts.
+  // ---- the rows' sums over the group's waves, and out ----
+  bar();
 #pragma unroll
   for (int rt = 0; rt < RT; ++rt) {
     l[rt] += __shfl_xor(l[rt], 16);
     l[rt] += __shfl_xor(l[rt], 32);
+    if (grp == 0) mx[kw * kRows + (rg * RT + rt) * 16 + col] = l[rt];
   }
-  __syncthreads();
-  float* ob = reinterpret_cast<float*>(lds);
-  float* ml = ob + 4 * kRows * D;  // [wave][row]: mref, then [wave][row]: l
+  bar();
 #pragma unroll
   for (int rt = 0; rt < RT; ++rt) {
-    const int r = rt * 16 + t.col;
+    const int r = row0 + rt * 16 + col;
+    const float* lr = mx + (rg * RT + rt) * 16 + col;
+    float lt = (lr[0] + lr[kRows]) + (lr[2 * kRows] + lr[3 * kRows]);
+    if (!seen[node_of(rt)]) lt = 0.f;  // an absent node
+    if (r < rows) {
+      const int node = r / a.group, g = r - node * a.group;
+      const long long at = static_cast<long long>(win.off + node) * a.n_heads + h * a.group + g;
+      const int c0 = kw * (D / 4) + 4 * grp;
+      if (a.n_split == 1) {
+        const float inv = lt != 0.f ? 1.f / lt : 0.f;
 #pragma unroll
-    for (int d = 0; d < DT; ++d)
-      *reinterpret_cast<f4*>(ob + (wave * kRows + r) * D + (((d * 4 + t.grp) ^ t.col) << 2)) =
-          acc[rt][d];
-    if (t.grp == 0) {
-      // (a row whose scores are all NaN has not begun either, but counts)
-      ml[wave * kRows + r] = begun[rt] || l[rt] != l[rt] ? mref[rt] : -INFINITY;
-      ml[(4 + wave) * kRows + r] = up[rt] ? l[rt] : 0.f;
-    }
-  }
-  __syncthreads();
-  constexpr int kPieces = D / 4;
-  for (int x = threadIdx.x; x < kRows * kPieces; x += 256) {
-    const int r = x / kPieces, piece = x % kPieces;
-    const int rr = rb * kRows + r;
-    if (rr >= rows) break;
-    float m = -INFINITY, sum = 0.f;
+        for (int d = 0; d < DQ; ++d) {
+          h4 y;
 #pragma unroll
-    for (int w = 0; w < 4; ++w) m = fmaxf(m, ml[w * kRows + r]);
-    f4 o = (f4){0.f, 0.f, 0.f, 0.f};
+          for (int i = 0; i < 4; ++i)
+            y[i] = lt != 0.f ? static_cast<_Float16>(acc[rt][d][i] * inv) : static_cast<_Float16>(0);
+          *reinterpret_cast<h4*>(a.out + at * D + c0 + d * 16) = y;
+        }
+      } else {
+        const long long pa = static_cast<long long>(split) * a.n_tokens * a.n_heads + at;
 #pragma unroll
-    for (int w = 0; w < 4; ++w) {
-      const float mw = ml[w * kRows + r], lw = ml[(4 + w) * kRows + r];
-      if (mw > -INFINITY && lw != 0.f) {
-        const float f = __builtin_amdgcn_exp2f(mw - m);
-        sum += lw * f;
-        o += *reinterpret_cast<const f4*>(ob + (w * kRows + r) * D + ((piece ^ (r & 15)) << 2)) * f;
+        for (int d = 0; d < DQ; ++d)
+          *reinterpret_cast<f4*>(a.part_o + pa * D + c0 + d * 16) = acc[rt][d];
+        if (kw == 0 && grp == 0) a.part_ml[pa] = make_float2(mref[rt], lt);
       }
-    }
-    const int node = rr / a.group, g = rr - node * a.group;
-    const long long at =
-        static_cast<long long>(t.win.off + node) * a.n_heads + t.h * a.group + g;
-    if (a.n_split == 1) {
-      const float inv = sum != 0.f ? 1.f / sum : 0.f;
-      h4 y;
-#pragma unroll
-      for (int i = 0; i < 4; ++i) y[i] = static_cast<_Float16>(o[i] * inv);
-      *reinterpret_cast<h4*>(a.out + at * D + piece * 4) = y;
-    } else {
-      const long long pa = static_cast<long long>(split) * a.n_tokens * a.n_heads + at;
-      if (sum != 0.f) *reinterpret_cast<f4*>(a.part_o + pa * D + piece * 4) = o;
-      if (piece == 0) a.part_ml[pa] = make_float2(m, sum);
     }
   }
 }
 
-// The parts of a split, joined: one wave per (token, head).
+// The parts of a row's keys, joined: a workgroup per (token, head), each
+// wave's 16-B lanes taking whole parts in turn.  A part whose l is 0 has no
+// key that the row sees, and what its O holds is not read as a number.
 template <int D>
-__global__ void __launch_bounds__(256) attn_join_kernel(const AttnArgs a, int n_seq) {
-  const int lane = threadIdx.x & 63;
-  const long long x = static_cast<long long>(blockIdx.x) * 4 + (threadIdx.x >> 6);
-  const long long per = static_cast<long long>(a.max_window) * a.n_heads;
-  if (x >= per * n_seq) return;
-  const int seq = static_cast<int>(x / per);
-  const int rest = static_cast<int>(x - seq * per);
+__global__ void __launch_bounds__(256) attn_join_kernel(const AttnArgs a) {
+  constexpr int LP = D / 4;        // lanes of a part
+  constexpr int SP = 256 / LP;     // parts at once
+  constexpr int U = 8;             // loads under way per lane
+  const int per = a.max_window * a.n_heads;
+  const int seq = blockIdx.x / per;
+  const int rest = blockIdx.x - seq * per;
   const int node = rest / a.n_heads, head = rest - node * a.n_heads;
   const Window w = window_of(a.win_off, seq, a.n_tokens, a.max_window);
   if (node >= w.n) return;
   const long long at = static_cast<long long>(w.off + node) * a.n_heads + head;
   const long long step = static_cast<long long>(a.n_tokens) * a.n_heads;
-  float m = -INFINITY;
-  for (int s = lane; s < a.n_split; s += 64) {
-    const float2 v = a.part_ml[at + s * step];
-    if (v.y != 0.f) m = fmaxf(m, v.x);
+  const int t = threadIdx.x, sub = t / LP, c = (t % LP) * 4;
+  const float* po = a.part_o + at * D + c;
+  // every lane group joins its parts about a maximum of its own
+  float m = -INFINITY, sum = 0.f;
+  f4 o = (f4){0.f, 0.f, 0.f, 0.f};
+  for (int s0 = sub; s0 < a.n_split; s0 += SP * U) {
+    f4 v[U];
+    float2 ml[U];
+#pragma unroll
+    for (int u = 0; u < U; ++u) {
+      const int s = min(s0 + u * SP, a.n_split - 1);
+      ml[u] = a.part_ml[at + s * step];
+      v[u] = *reinterpret_cast<const f4*>(po + s * step * D);
+    }
+    float top = m;
+#pragma unroll
+    for (int u = 0; u < U; ++u) {
+      if (s0 + u * SP >= a.n_split) ml[u].y = 0.f;
+      top = ml[u].y != 0.f ? fmaxf(top, ml[u].x) : top;
+    }
+    const float f0 = m > -INFINITY ? __builtin_amdgcn_exp2f(m - top) : 0.f;
+    sum *= f0;
+    o *= f0;
+#pragma unroll
+    for (int u = 0; u < U; ++u) {
+      const bool some = ml[u].y != 0.f;
+      const float f = some ? __builtin_amdgcn_exp2f(ml[u].x - top) : 0.f;
+      sum += some ? ml[u].y * f : 0.f;
+#pragma unroll
+      for (int i = 0; i < 4; ++i) o[i] += some ? v[u][i] * f : 0.f;
+    }
+    m = top;
   }
-  m = wave_max_dpp(m);
-  constexpr int E = D / 64;
-  float o[E], sum = 0.f;
-#pragma unroll
-  for (int i = 0; i < E; ++i) o[i] = 0.f;
-  for (int s = 0; s < a.n_split; ++s) {
-    const float2 v = a.part_ml[at + s * step];
-    if (v.y == 0.f) continue;
-    const float f = __builtin_amdgcn_exp2f(v.x - m);
-    sum += v.y * f;
-    const float* p = a.part_o + (at + s * step) * D + lane * E;
-#pragma unroll
-    for (int i = 0; i < E; ++i) o[i] += p[i] * f;
+  __shared__ f4 so[256];
+  __shared__ float sm[SP], ss[SP];
+  so[t] = o;
+  if (t % LP == 0) {
+    sm[sub] = m;
+    ss[sub] = sum;
   }
-  const float inv = sum != 0.f ? 1.f / sum : 0.f;
+  __syncthreads();
+  if (sub == 0) {
+    float top = sm[0];
 #pragma unroll
-  for (int i = 0; i < E; ++i) a.out[at * D + lane * E + i] = f16b(o[i] * inv);
+    for (int i = 1; i < SP; ++i) top = fmaxf(top, sm[i]);
+    float total = 0.f;
+    f4 y = (f4){0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+    for (int i = 0; i < SP; ++i) {
+      const bool some = ss[i] != 0.f;
+      const float f = some ? __builtin_amdgcn_exp2f(sm[i] - top) : 0.f;
+      total += some ? ss[i] * f : 0.f;
+      const f4 x = so[i * LP + t];
+#pragma unroll
+      for (int j = 0; j < 4; ++j) y[j] += some ? x[j] * f : 0.f;
+    }
+    const float inv = total != 0.f ? 1.f / total : 0.f;
+    h4 z;
+#pragma unroll
+    for (int j = 0; j < 4; ++j) z[j] = static_cast<_Float16>(y[j] * inv);
+    *reinterpret_cast<h4*>(a.out + at * D + c) = z;
+  }
 }
 
 // ---- the accepted tokens into the cache --------------------------------------
@@ -586,21 +627,22 @@ static int check_cache(const sg_kv_cache* c, int n_seq, int n_tokens, int max_wi
 
 // How a call is cut: rows of a workgroup, parts of the caches.
 struct Cut {
-  int rt, row_blocks, n_split, split_keys;
+  int rt, rw, row_blocks, n_split, split_keys;
 };
 static Cut attn_cut(int n_seq, int max_window, int max_len, int group, int n_kv, int dim) {
   Cut c;
-  const int rows = max_window * group;
-  c.rt = rows > 16 ? 2 : 1;
-  c.row_blocks = (rows + 16 * c.rt - 1) / (16 * c.rt);
+  const long long rows = static_cast<long long>(max_window) * group;
+  c.rt = rows > 32 ? 4 : rows > 16 ? 2 : 1;
+  c.rw = rows > 64 ? 2 : 1;
+  if (c.rw == 2 && dim == 256) c.rt = 3;
+  c.row_blocks = static_cast<int>((rows + 16 * c.rt * c.rw - 1) / (16 * c.rt * c.rw));
   const long long keys = static_cast<long long>(max_len) + max_window;
-  const long long step = 4 * kTile;
-  const long long most = (keys + step - 1) / step;
-  const long long groups = static_cast<long long>(n_seq) * n_kv * c.row_blocks;
-  const long long slots = 256 * (dim == 256 ? 1 : 2);
-  long long n = groups >= slots ? 1 : slots / groups;
+  const long long most = (keys + kKeys - 1) / kKeys;
+  const long long units = static_cast<long long>(n_seq) * n_kv * c.row_blocks;
+  const long long slots = 256 * (dim == 256 || c.rw == 2 ? 1 : 2);
+  long long n = units >= slots ? 1 : slots / units;
   if (n > most) n = most;
-  c.split_keys = static_cast<int>((most + n - 1) / n * step);
+  c.split_keys = static_cast<int>((most + n - 1) / n * kKeys);
   c.n_split = static_cast<int>((keys + c.split_keys - 1) / c.split_keys);
   return c;
 }
@@ -609,23 +651,26 @@ static size_t part_bytes(const Cut& c, int n_tokens, int n_heads, int dim) {
   return static_cast<size_t>(c.n_split) * n_tokens * n_heads * (dim * 4 + 8);
 }
 
+template <int D, int RT, int RW>
+static void attn_go(const AttnArgs& a, long long grid, hipStream_t s) {
+  hipLaunchKernelGGL((attn_tree_kernel<D, RT, RW>), dim3(static_cast<unsigned>(grid)),
+                     dim3(256 * RW), (AttnLds<D, RT, RW>::kBytes), s, a);
+}
 template <int D>
-static int attn_launch(const AttnArgs& a, const Cut& c, int n_seq, long long grid, hipStream_t s,
-                       const char* nm) {
-  const size_t lds = 4 * 16 * c.rt * D * 4 + 2 * 4 * 16 * c.rt * 4;
-  const size_t bufs = 4 * 2 * Attn<D, 1>::kTileBytes;
-  const size_t bytes = lds > bufs ? lds : bufs;
-  if (c.rt == 1)
-    hipLaunchKernelGGL((attn_tree_kernel<D, 1>), dim3(static_cast<unsigned>(grid)), dim3(256),
-                       bytes, s, a);
+static int attn_launch(const AttnArgs& a, const Cut& c, int n_seq, hipStream_t s, const char* nm) {
+  const long long grid = (a.units + 7LL) / 8 * 8 * c.row_blocks;
+  if (c.rw == 2)
+    attn_go<D, D == 256 ? 3 : 4, 2>(a, grid, s);
+  else if (c.rt == 4)
+    attn_go<D, 4, 1>(a, grid, s);
+  else if (c.rt == 2)
+    attn_go<D, 2, 1>(a, grid, s);
   else
-    hipLaunchKernelGGL((attn_tree_kernel<D, 2>), dim3(static_cast<unsigned>(grid)), dim3(256),
-                       bytes, s, a);
+    attn_go<D, 1, 1>(a, grid, s);
   if (int st = check_launch(nm)) return st;
   if (c.n_split > 1) {
-    const long long waves = static_cast<long long>(n_seq) * a.max_window * a.n_heads;
-    hipLaunchKernelGGL(attn_join_kernel<D>, dim3(static_cast<unsigned>((waves + 3) / 4)),
-                       dim3(256), 0, s, a, n_seq);
+    hipLaunchKernelGGL(attn_join_kernel<D>, dim3(n_seq * a.max_window * a.n_heads), dim3(256), 0, s,
+                       a);
     return check_launch(nm);
   }
   return SG_OK;
@@ -679,9 +724,9 @@ int sg_attn_tree_f16(const uint16_t* q, const uint16_t* k, const uint16_t* v, lo
   if (need && (!ws || ws_bytes < need || reinterpret_cast<uintptr_t>(ws) % 16))
     return set_error(SG_ERR_INVALID_ARGUMENT, "%s: the workspace needs %zu bytes, 16-B aligned", nm,
                      need);
-  const long long grid = static_cast<long long>(n_seq) * n_kv * c.row_blocks * c.n_split;
+  const long long units = static_cast<long long>(n_seq) * n_kv * c.n_split;
   const long long join = static_cast<long long>(n_seq) * max_window * n_heads;
-  if (grid > 0x7FFFFFFF || join > 0x7FFFFFFF)
+  if ((units + 8) * c.row_blocks > 0x7FFFFFFF || join > 0x7FFFFFFF)
     return set_error(SG_ERR_UNSUPPORTED, "%s: too many sequences", nm);
   AttnArgs a;
   a.q = q;
@@ -711,11 +756,12 @@ int sg_attn_tree_f16(const uint16_t* q, const uint16_t* k, const uint16_t* v, lo
   a.n_split = c.n_split;
   a.split_keys = c.split_keys;
   a.row_blocks = c.row_blocks;
+  a.units = static_cast<int>(units);
   a.scale_log2 = scale * kLog2e;
   const hipStream_t s = static_cast<hipStream_t>(stream);
-  if (dim == 64) return attn_launch<64>(a, c, n_seq, grid, s, nm);
-  if (dim == 128) return attn_launch<128>(a, c, n_seq, grid, s, nm);
-  return attn_launch<256>(a, c, n_seq, grid, s, nm);
+  if (dim == 64) return attn_launch<64>(a, c, n_seq, s, nm);
+  if (dim == 128) return attn_launch<128>(a, c, n_seq, s, nm);
+  return attn_launch<256>(a, c, n_seq, s, nm);
 }
 
 int sg_kv_commit_f16(const uint16_t* k, const uint16_t* v, long long k_stride, long long v_stride,

@@ -675,8 +675,8 @@ def test_a_window_step_in_a_graph():
         g.replay()
         eager.run()
         torch.cuda.synchronize()
-        for a, b in zip(st.results(), eager.results()):
-            assert torch.equal(a, b)
+        for a, b in zip(st.results(), eager.results()):  # (bits: a row may hold NaN)
+            assert torch.equal(a.view(torch.uint8), b.view(torch.uint8))
         for s in (st, eager):  # the next step's caches
             s.cache.length.copy_(torch.tensor([33 + i, 60 - i, 5 * i], dtype=torch.int32))
 
