@@ -92,7 +92,7 @@ struct AttnLds {
   static constexpr uint32_t kMax = kP + kRows * kKeys * 2;
   static constexpr uint32_t kSeen = kMax + 4 * kRows * 4;
   static constexpr uint32_t kFlags = kSeen + kMaxWindow * 8;
-  static constexpr uint32_t kBytes = kFlags + 16;
+  static constexpr uint32_t kBytes = kFlags + 32;
 };
 
 // RT: tiles of 16 rows of a group; RW: groups of four waves.
@@ -108,7 +108,7 @@ __global__ void __launch_bounds__(256 * RW) attn_tree_kernel(const AttnArgs a) {
   extern __shared__ __attribute__((aligned(16))) unsigned char lds[];
   const uint32_t lds0 = static_cast<uint32_t>(
       reinterpret_cast<uintptr_t>((__attribute__((address_space(3))) unsigned char*)lds));
-  int* flags = reinterpret_cast<int*>(lds + L::kFlags);  // rise[2], odd[2]
+  int* flags = reinterpret_cast<int*>(lds + L::kFlags);  // by step parity: rise of either group, odd
   float* mx = reinterpret_cast<float*>(lds + L::kMax);
   uint64_t* seen = reinterpret_cast<uint64_t*>(lds + L::kSeen);  // node: whom it sees
   const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
@@ -146,33 +146,28 @@ __global__ void __launch_bounds__(256 * RW) attn_tree_kernel(const AttnArgs a) {
     return j < len ? table[j >> a.page_log2] : -1;
   };
   auto page_ok = [&](int p) { return static_cast<uint32_t>(p) < static_cast<uint32_t>(a.n_pages); };
-  auto issue = [&](int s, int page) {
+  auto issue = [&](int s, int page, bool k_too, bool v_too) {  // (both flags are compile-time)
     const int j = s * kKeys + 16 * kw;
     const uint32_t buf = lds0 + (s & 1) * 2 * L::kStep + blk;
     const long long at =
         (((static_cast<long long>(page) * a.n_kv + h) << a.page_log2) +
          (j & ((1 << a.page_log2) - 1))) * D;
     if (j + 16 <= len && page_ok(page)) {
-      const uint16_t* kb = uniform_ptr((RW == 2 && rg ? a.vc : a.kc) + at);
+      const uint16_t* kb = uniform_ptr(a.kc + at);
       const uint16_t* vb = uniform_ptr(a.vc + at);
       int ln = lane;
       if (RT >= 3) asm("" : "+v"(ln));  // (the offsets made anew: registers are short)
 #pragma unroll
       for (int i = 0; i < NI; ++i) {
         const int row = i * RPI + ln / CH;
-        const uint32_t voff = row * (D * 2) + (((ln % CH) ^ swz<D>(row)) << 4);
-        if (RW == 1) {
-          dma16_base(buf + i * 1024, voff, kb);
-          dma16_base(buf + L::kStep + i * 1024, voff, vb);
-        } else {
-          dma16_base(buf + (rg ? L::kStep : 0) + i * 1024, voff, kb);
-        }
+        const uint32_t off = row * (D * 2) + (((ln % CH) ^ swz<D>(row)) << 4);
+        if (k_too) dma16_base(buf + i * 1024, off, kb);
+        if (v_too) dma16_base(buf + L::kStep + i * 1024, off, vb);
       }
     } else if (j < total) {
       // rows of the cache, then of the window; what is not there reads a
       // window row and is masked
       const int n_cache = page_ok(page) ? min(len - j, 16) : 0;
-      const bool k_too = RW == 1 || rg == 0, v_too = RW == 1 || rg == 1;
 #pragma unroll 1
       for (int i = 0; i < NI; ++i) {
         const int row = i * RPI + lane / CH;
@@ -198,10 +193,15 @@ __global__ void __launch_bounds__(256 * RW) attn_tree_kernel(const AttnArgs a) {
 
   int page = page_of(step), page_next = 0;
   if (step < s_end) {
-    issue(step, page);
+    if (RW == 1)
+      issue(step, page, true, true);
+    else if (rg == 0)
+      issue(step, page, true, false);
+    else
+      issue(step, page, false, true);
     page_next = page_of(step + 1);
   }
-  if (threadIdx.x < 4) flags[threadIdx.x] = 0;
+  if (threadIdx.x < 8) flags[threadIdx.x] = 0;
 
   // ---- Q's rows, while the first copies are under way ----
   if (wave == 4 * RW - 1) seen[lane] = ancestors(a.parent, win, lane);
@@ -250,40 +250,36 @@ __global__ void __launch_bounds__(256 * RW) attn_tree_kernel(const AttnArgs a) {
               (col & 1) * 8;
   unsigned char* const p_out = pl + col * 128 + ((((kw >> 1) * 4 + grp) ^ psw) << 4) + (kw & 1) * 8;
 
-  for (; step < s_end; ++step) {
-    const int par = step & 1;
-    wait_vm();
-    bar();  // everybody's copies of this step are here, and nobody reads the other buffers or P
-    if (step + 1 < s_end) issue(step + 1, page_next);
-    const int page_then = step + 2 < s_end ? page_of(step + 2) : -1;
-    if (threadIdx.x == 0) flags[par ^ 1] = flags[2 + (par ^ 1)] = 0;
-    const unsigned char* kb = lds + par * 2 * L::kStep;
-    unsigned char* vb = lds + par * 2 * L::kStep + L::kStep;
-    const int j0 = step * kKeys + 16 * kw;
-    const uint32_t there = present(step, page);
-    const bool plain = j0 + 16 <= len && there == 0xFFFFu;
-
-    if (!plain && rg == RW - 1) {
-      // Rows that nobody sees become 0 (0 times what lies there need not be
-      // 0).  Window rows, which some queries see and others do not, are looked
-      // through for infinities and NaN.
-      bool odd = false;
+  // Rows of V that nobody sees become 0 (0 times what lies there need not be
+  // 0).  Window rows, which some queries see and others do not, are looked
+  // through for infinities and NaN.  Each wave does the rows it has copied.
+  auto fix_v = [&](int s, uint32_t there) {
+    const int j = s * kKeys + 16 * kw;
+    unsigned char* vb = lds + (s & 1) * 2 * L::kStep + L::kStep + blk;
+    bool odd = false;
 #pragma unroll 1
-      for (int i = 0; i < NI; ++i) {
-        const int row = i * RPI + lane / CH;
-        u32x4* at = reinterpret_cast<u32x4*>(vb + blk + i * 1024 + 16 * lane);
-        if (!(there >> row & 1)) {
-          *at = (u32x4){0, 0, 0, 0};
-        } else if (j0 + row >= len && win.n > 1) {
-          const u32x4 w = *at;
+    for (int i = 0; i < NI; ++i) {
+      const int row = i * RPI + lane / CH;
+      u32x4* at = reinterpret_cast<u32x4*>(vb + i * 1024 + 16 * lane);
+      if (!(there >> row & 1)) {
+        *at = (u32x4){0, 0, 0, 0};
+      } else if (j + row >= len && win.n > 1) {
+        const u32x4 w = *at;
 #pragma unroll
-          for (int c = 0; c < 4; ++c)
-            odd |= (w[c] & 0x7C00u) == 0x7C00u || (w[c] & 0x7C000000u) == 0x7C000000u;
-        }
+        for (int c = 0; c < 4; ++c)
+          odd |= (w[c] & 0x7C00u) == 0x7C00u || (w[c] & 0x7C000000u) == 0x7C000000u;
       }
-      if (__any(odd) && lane == 0) flags[2 + par] = 1;
     }
+    if (__any(odd) && lane == 0) flags[4 + (s & 1)] = 1;
+  };
+  auto plain_step = [&](int s, uint32_t there) {
+    return s * kKeys + 16 * kw + 16 <= len && there == 0xFFFFu;
+  };
 
+  float e[RT][4], top[RT], sum[RT];
+  // e: the scores of a step's keys 16 kw.. above mref, log2; top: their largest per row
+  auto scores = [&](int step_, uint32_t there, bool plain) {
+    const unsigned char* kb = lds + (step_ & 1) * 2 * L::kStep;
     f4 s[RT];
 #pragma unroll
     for (int rt = 0; rt < RT; ++rt) s[rt] = (f4){0.f, 0.f, 0.f, 0.f};
@@ -293,10 +289,8 @@ __global__ void __launch_bounds__(256 * RW) attn_tree_kernel(const AttnArgs a) {
 #pragma unroll
       for (int rt = 0; rt < RT; ++rt)
         s[rt] = __builtin_amdgcn_mfma_f32_16x16x32_f16(kf, qf[rt][st], s[rt], 0, 0, 0);
+      if (RW == 2 && st % 4 == 3) asm volatile("" ::: "memory");  // (no more reads ahead: registers)
     }
-
-    float e[RT][4], top[RT], sum[RT];
-    bool rise = false;
 #pragma unroll
     for (int rt = 0; rt < RT; ++rt) {
 #pragma unroll
@@ -304,7 +298,7 @@ __global__ void __launch_bounds__(256 * RW) attn_tree_kernel(const AttnArgs a) {
       if (!plain) {
         // bit r of `see`: key r is there and this lane's row sees it
         const uint64_t up = seen[node_of(rt)];
-        const int w0 = j0 - len;  // key 0's window node, if not negative
+        const int w0 = step_ * kKeys + 16 * kw - len;  // key 0's window node, if not negative
         const uint32_t tree = w0 >= 0    ? static_cast<uint32_t>(up >> (w0 & 63))
                               : w0 > -16 ? static_cast<uint32_t>(up << -w0) | ((1u << -w0) - 1)
                                          : 0xFFFFu;
@@ -313,30 +307,41 @@ __global__ void __launch_bounds__(256 * RW) attn_tree_kernel(const AttnArgs a) {
         for (int i = 0; i < 4; ++i) e[rt][i] = see & 1u << i ? e[rt][i] : -INFINITY;
       }
       top[rt] = fmaxf(fmaxf(e[rt][0], e[rt][1]), fmaxf(e[rt][2], e[rt][3]));
-      rise |= top[rt] > kRise || (!begun[rt] && top[rt] > -INFINITY);
-      float p[4];
-      h4 ph;
-#pragma unroll
-      for (int i = 0; i < 4; ++i) {
-        p[i] = __builtin_amdgcn_exp2f(e[rt][i]);
-        ph[i] = static_cast<_Float16>(p[i]);
-      }
-      sum[rt] = (p[0] + p[1]) + (p[2] + p[3]);
-      *reinterpret_cast<h4*>(p_out + rt * 16 * 128) = ph;
     }
-    if (__any(rise) && lane == 0) flags[par] = 1;
-    bar();  // P is here
-
-    if (flags[par]) {
-      // The reference points move: the rows' maxima over the group's waves,
-      // then P once more.
+  };
+  auto weigh = [&](int rt, float by) {  // row tile rt's p = 2^(e - by), into LDS
+    float p[4];
+    h4 ph;
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+      p[i] = __builtin_amdgcn_exp2f(e[rt][i] - by);
+      ph[i] = static_cast<_Float16>(p[i]);
+    }
+    sum[rt] = (p[0] + p[1]) + (p[2] + p[3]);
+    *reinterpret_cast<h4*>(p_out + rt * 16 * 128) = ph;
+  };
+  auto first_part = [&](int s, uint32_t there, int* rise_flag) {
+    scores(s, there, plain_step(s, there));
+    bool rise = false;
+#pragma unroll
+    for (int rt = 0; rt < RT; ++rt) {
+      rise |= top[rt] > kRise || (!begun[rt] && top[rt] > -INFINITY);
+      weigh(rt, 0.f);
+    }
+    if (__any(rise) && lane == 0) *rise_flag = 1;
+  };
+  // The reference points move: the rows' maxima over the group's waves, then P
+  // once more.  Every wave of the workgroup comes to the two barriers.
+  auto move_refs = [&](bool mine) {
+    if (mine)
 #pragma unroll
       for (int rt = 0; rt < RT; ++rt) {
         float m = fmaxf(top[rt], __shfl_xor(top[rt], 16));
         m = fmaxf(m, __shfl_xor(m, 32));
         if (grp == 0) mx[kw * kRows + (rg * RT + rt) * 16 + col] = m;
       }
-      bar();
+    bar();
+    if (mine)
 #pragma unroll
       for (int rt = 0; rt < RT; ++rt) {
         const float* mr = mx + (rg * RT + rt) * 16 + col;
@@ -349,27 +354,21 @@ __global__ void __launch_bounds__(256 * RW) attn_tree_kernel(const AttnArgs a) {
 #pragma unroll
         for (int d = 0; d < DQ; ++d) acc[rt][d] *= f;
         begun[rt] |= set;
-        float p[4];
-        h4 ph;
-#pragma unroll
-        for (int i = 0; i < 4; ++i) {
-          p[i] = __builtin_amdgcn_exp2f(e[rt][i] - by);
-          ph[i] = static_cast<_Float16>(p[i]);
-        }
-        sum[rt] = (p[0] + p[1]) + (p[2] + p[3]);
-        *reinterpret_cast<h4*>(p_out + rt * 16 * 128) = ph;
+        weigh(rt, by);
       }
-      bar();
-    }
+    bar();
+  };
+  auto second_part = [&](int s) {
+    const unsigned char* vb = lds + (s & 1) * 2 * L::kStep + L::kStep;
+    const bool odd = flags[4 + (s & 1)] != 0;
 #pragma unroll
     for (int rt = 0; rt < RT; ++rt) l[rt] += sum[rt];
-
-    if (flags[2 + par]) {
+    if (odd) {
       // Infinities and NaN in the window's V: added one by one to the rows
-      // that see them, then taken out for the product.
+      // that see them, and taken as 0 below.
 #pragma unroll 1
       for (int r = 0; r < kKeys; ++r) {
-        const int node = step * kKeys + r - len;
+        const int node = s * kKeys + r - len;
         if (node < 0 || node >= win.n) continue;
         const int piece = (r >> 5) * 4 + ((r & 15) >> 2);
 #pragma unroll
@@ -388,20 +387,8 @@ __global__ void __launch_bounds__(256 * RW) attn_tree_kernel(const AttnArgs a) {
             }
         }
       }
-      bar();
-      if (rg == RW - 1)
-#pragma unroll 1
-        for (int i = 0; i < NI; ++i) {
-          const int row = i * RPI + lane / CH;
-          uint16_t* at = reinterpret_cast<uint16_t*>(vb + blk + i * 1024 + 16 * lane);
-#pragma unroll 1
-          for (int c = 0; c < 8; ++c)
-            if (j0 + row >= len && (at[c] & 0x7C00) == 0x7C00) at[c] = 0;
-        }
-      bar();
     }
-
-    const uint32_t vl = par * 2 * L::kStep;
+    const uint32_t vl = (s & 1) * 2 * L::kStep;
 #pragma unroll
     for (int st = 0; st < 2; ++st) {
       h8 pf[RT];
@@ -411,22 +398,89 @@ __global__ void __launch_bounds__(256 * RW) attn_tree_kernel(const AttnArgs a) {
                                               (((st * 4 + grp) ^ psw) << 4));
 #pragma unroll
       for (int d = 0; d < DQ; ++d) {
-        h8 vf;
+        s4 x[2];
 #pragma unroll
         for (int b = 0; b < 2; ++b) {
-          const h4 x = __builtin_bit_cast(
-              h4, __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_s4_p)(static_cast<uintptr_t>(
-                      vl + voff[d] + (st * 2 + b) * 16 * D * 2))));
+          x[b] = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_s4_p)(static_cast<uintptr_t>(
+              vl + voff[d] + (st * 2 + b) * 16 * D * 2)));
+          if (odd) {
+            const int j = s * kKeys + (st * 2 + b) * 16 + 4 * grp;
 #pragma unroll
-          for (int i = 0; i < 4; ++i) vf[b * 4 + i] = x[i];
+            for (int i = 0; i < 4; ++i)
+              x[b][i] = j + i >= len && (x[b][i] & 0x7C00) == 0x7C00 ? 0 : x[b][i];
+          }
         }
+        const h8 vf = __builtin_bit_cast(
+            h8, __builtin_shufflevector(x[0], x[1], 0, 1, 2, 3, 4, 5, 6, 7));
 #pragma unroll
         for (int rt = 0; rt < RT; ++rt)
           acc[rt][d] = __builtin_amdgcn_mfma_f32_16x16x32_f16(vf, pf[rt], acc[rt][d], 0, 0, 0);
       }
+      if (RW == 2) asm volatile("" ::: "memory");
     }
-    page = page_next;
-    page_next = page_then;
+  };
+
+  bar();  // the flags are cleared
+  if (RW == 1) {
+    for (; step < s_end; ++step) {
+      const int par = step & 1;
+      const uint32_t there = present(step, page);
+      wait_vm();
+      if (!plain_step(step, there)) fix_v(step, there);
+      bar();  // everybody's copies of this step are here, and nobody reads the other buffers or P
+      if (step + 1 < s_end) issue(step + 1, page_next, true, true);
+      const int page_then = step + 2 < s_end ? page_of(step + 2) : -1;
+      if (threadIdx.x == 0) flags[par ^ 1] = flags[4 + (par ^ 1)] = 0;
+      first_part(step, there, flags + par);
+      bar();  // P is here
+      if (flags[par]) move_refs(true);
+      second_part(step);
+      page = page_next;
+      page_next = page_then;
+    }
+  } else {
+    // Two groups half a step apart: while one takes a step's first part
+    // (scores and weights: vector work), the other takes the second part of
+    // the step before (matrix work).  In half t, group t & 1 takes the first
+    // part of step t / 2, the other the second part of step (t - 1) / 2.
+    const int n = s_end - step, begin = step;
+    uint32_t there = 0;
+#pragma unroll 1
+    for (int t = 0; t <= 2 * n; ++t) {
+      const int who = t & 1, s1 = begin + (t >> 1), s2 = begin + ((t - 1) >> 1);
+      const bool lead = who == rg;
+      if (lead && s1 < s_end) {  // K of s1 is needed from its even half on, V from its odd one
+        wait_vm();
+        there = present(s1, page);
+        if (rg == 1 && !plain_step(s1, there)) fix_v(s1, there);
+      }
+      bar();  // and the other group's P is here
+      int* rise = flags + 2 * who;
+      if (t > 0 && flags[2 * (who ^ 1) + (s2 & 1)]) {
+        // (K of s2 is still there)
+        if (!lead) scores(s2, there, false);
+        move_refs(!lead);
+      }
+      if (threadIdx.x == 0) {
+        rise[(s1 & 1) ^ 1] = 0;
+        if (who == 1) flags[4 + ((s1 & 1) ^ 1)] = 0;
+      }
+      if (lead) {
+        if (s1 < s_end) {
+          if (s1 + 1 < s_end) {
+            if (rg == 0)
+              issue(s1 + 1, page_next, true, false);
+            else
+              issue(s1 + 1, page_next, false, true);
+          }
+          page = page_next;
+          if (s1 + 2 < s_end) page_next = page_of(s1 + 2);
+          first_part(s1, there, rise + (s1 & 1));
+        }
+      } else if (t > 0) {
+        second_part(s2);
+      }
+    }
   }
 
   // ---- the rows' sums over the group's waves, and out ----
@@ -634,7 +688,7 @@ static Cut attn_cut(int n_seq, int max_window, int max_len, int group, int n_kv,
   const long long rows = static_cast<long long>(max_window) * group;
   c.rt = rows > 32 ? 4 : rows > 16 ? 2 : 1;
   c.rw = rows > 64 ? 2 : 1;
-  if (c.rw == 2 && dim == 256) c.rt = 3;
+  if (c.rw == 2 && dim == 256) c.rt = 2;
   c.row_blocks = static_cast<int>((rows + 16 * c.rt * c.rw - 1) / (16 * c.rt * c.rw));
   const long long keys = static_cast<long long>(max_len) + max_window;
   const long long most = (keys + kKeys - 1) / kKeys;
@@ -660,7 +714,7 @@ template <int D>
 static int attn_launch(const AttnArgs& a, const Cut& c, int n_seq, hipStream_t s, const char* nm) {
   const long long grid = (a.units + 7LL) / 8 * 8 * c.row_blocks;
   if (c.rw == 2)
-    attn_go<D, D == 256 ? 3 : 4, 2>(a, grid, s);
+    attn_go<D, D == 256 ? 2 : 4, 2>(a, grid, s);
   else if (c.rt == 4)
     attn_go<D, 4, 1>(a, grid, s);
   else if (c.rt == 2)
