@@ -139,45 +139,47 @@ __global__ void __launch_bounds__(256 * RW) attn_tree_kernel(const AttnArgs a) {
   int step = first < s_end ? static_cast<int>(first) : s_end;
 
   // ---- copies: wave kw brings keys 16 kw.. of a step (of two groups, the
-  // first brings K's, the second V's) ----
+  // first brings V's, the second K's) ----
   const uint32_t blk = kw * 16 * D * 2;
   auto page_of = [&](int s) {
     const int j = s * kKeys + 16 * kw;
     return j < len ? table[j >> a.page_log2] : -1;
   };
   auto page_ok = [&](int p) { return static_cast<uint32_t>(p) < static_cast<uint32_t>(a.n_pages); };
-  auto issue = [&](int s, int page, bool k_too, bool v_too) {  // (both flags are compile-time)
+  // Brings a step's K and V; with two groups, V or K.
+  auto issue = [&](int s, int page, bool v) {
     const int j = s * kKeys + 16 * kw;
-    const uint32_t buf = lds0 + (s & 1) * 2 * L::kStep + blk;
+    const uint32_t buf = lds0 + (s & 1) * 2 * L::kStep + blk + (RW == 2 && v ? L::kStep : 0);
     const long long at =
         (((static_cast<long long>(page) * a.n_kv + h) << a.page_log2) +
          (j & ((1 << a.page_log2) - 1))) * D;
+    const uint16_t* const c1 = RW == 2 && v ? a.vc : a.kc;
     if (j + 16 <= len && page_ok(page)) {
-      const uint16_t* kb = uniform_ptr(a.kc + at);
-      const uint16_t* vb = uniform_ptr(a.vc + at);
+      const uint16_t* b1 = uniform_ptr(c1 + at);
+      const uint16_t* b2 = uniform_ptr(a.vc + at);
       int ln = lane;
       if (RT >= 3) asm("" : "+v"(ln));  // (the offsets made anew: registers are short)
 #pragma unroll
       for (int i = 0; i < NI; ++i) {
         const int row = i * RPI + ln / CH;
         const uint32_t off = row * (D * 2) + (((ln % CH) ^ swz<D>(row)) << 4);
-        if (k_too) dma16_base(buf + i * 1024, off, kb);
-        if (v_too) dma16_base(buf + L::kStep + i * 1024, off, vb);
+        dma16_base(buf + i * 1024, off, b1);
+        if (RW == 1) dma16_base(buf + L::kStep + i * 1024, off, b2);
       }
     } else if (j < total) {
       // rows of the cache, then of the window; what is not there reads a
       // window row and is masked
       const int n_cache = page_ok(page) ? min(len - j, 16) : 0;
+      const uint16_t* const w1 = RW == 2 && v ? a.v : a.k;
+      const long long ws1 = RW == 2 && v ? a.v_stride : a.k_stride;
 #pragma unroll 1
       for (int i = 0; i < NI; ++i) {
         const int row = i * RPI + lane / CH;
         const int c = ((lane % CH) ^ swz<D>(row)) * 8;
         const long long w = win.off + min(max(j + row - len, 0), win.n - 1);
         const bool cached = row < n_cache;
-        if (k_too)
-          dma16_ptr(buf + i * 1024,
-                    (cached ? a.kc + at + row * D : a.k + w * a.k_stride + h * D) + c);
-        if (v_too)
+        dma16_ptr(buf + i * 1024, (cached ? c1 + at + row * D : w1 + w * ws1 + h * D) + c);
+        if (RW == 1)
           dma16_ptr(buf + L::kStep + i * 1024,
                     (cached ? a.vc + at + row * D : a.v + w * a.v_stride + h * D) + c);
       }
@@ -193,12 +195,7 @@ __global__ void __launch_bounds__(256 * RW) attn_tree_kernel(const AttnArgs a) {
 
   int page = page_of(step), page_next = 0;
   if (step < s_end) {
-    if (RW == 1)
-      issue(step, page, true, true);
-    else if (rg == 0)
-      issue(step, page, true, false);
-    else
-      issue(step, page, false, true);
+    issue(step, page, rg == 0);
     page_next = page_of(step + 1);
   }
   if (threadIdx.x < 8) flags[threadIdx.x] = 0;
@@ -320,8 +317,7 @@ __global__ void __launch_bounds__(256 * RW) attn_tree_kernel(const AttnArgs a) {
     sum[rt] = (p[0] + p[1]) + (p[2] + p[3]);
     *reinterpret_cast<h4*>(p_out + rt * 16 * 128) = ph;
   };
-  auto first_part = [&](int s, uint32_t there, int* rise_flag) {
-    scores(s, there, plain_step(s, there));
+  auto first_part = [&](int* rise_flag) {  // after scores()
     bool rise = false;
 #pragma unroll
     for (int rt = 0; rt < RT; ++rt) {
@@ -428,10 +424,11 @@ __global__ void __launch_bounds__(256 * RW) attn_tree_kernel(const AttnArgs a) {
       wait_vm();
       if (!plain_step(step, there)) fix_v(step, there);
       bar();  // everybody's copies of this step are here, and nobody reads the other buffers or P
-      if (step + 1 < s_end) issue(step + 1, page_next, true, true);
+      if (step + 1 < s_end) issue(step + 1, page_next, false);
       const int page_then = step + 2 < s_end ? page_of(step + 2) : -1;
       if (threadIdx.x == 0) flags[par ^ 1] = flags[4 + (par ^ 1)] = 0;
-      first_part(step, there, flags + par);
+      scores(step, there, plain_step(step, there));
+      first_part(flags + par);
       bar();  // P is here
       if (flags[par]) move_refs(true);
       second_part(step);
@@ -440,45 +437,46 @@ __global__ void __launch_bounds__(256 * RW) attn_tree_kernel(const AttnArgs a) {
     }
   } else {
     // Two groups half a step apart: while one takes a step's first part
-    // (scores and weights: vector work), the other takes the second part of
-    // the step before (matrix work).  In half t, group t & 1 takes the first
-    // part of step t / 2, the other the second part of step (t - 1) / 2.
+    // (scores and weights), the other takes the second part of the step before
+    // and brings the next step's copies, since the first part is the longer
+    // way: K in even halves (the second group), V in odd ones (the first).  In
+    // half t, group t & 1 takes the first part of step t / 2, the other the
+    // second part of step (t - 1) / 2.
     const int n = s_end - step, begin = step;
-    uint32_t there = 0;
+    uint32_t there = 0, there_before = 0;
 #pragma unroll 1
     for (int t = 0; t <= 2 * n; ++t) {
       const int who = t & 1, s1 = begin + (t >> 1), s2 = begin + ((t - 1) >> 1);
-      const bool lead = who == rg;
-      if (lead && s1 < s_end) {  // K of s1 is needed from its even half on, V from its odd one
-        wait_vm();
+      const bool lead = who == rg, more = s1 < s_end;
+      if (who == 0) {
+        there_before = there;
         there = present(s1, page);
-        if (rg == 1 && !plain_step(s1, there)) fix_v(s1, there);
       }
-      bar();  // and the other group's P is here
-      int* rise = flags + 2 * who;
-      if (t > 0 && flags[2 * (who ^ 1) + (s2 & 1)]) {
-        // (K of s2 is still there)
-        if (!lead) scores(s2, there, false);
-        move_refs(!lead);
+      if (!lead && more) {
+        wait_vm();
+        if (who == 1 && !plain_step(s1, there)) fix_v(s1, there);
+      }
+      bar();  // K (V) of s1 is here, and the other group's P
+      const int moved = t > 0 ? flags[2 * (who ^ 1) + (s2 & 1)] : 0;
+      if (lead) {
+        if (more) scores(s1, there, plain_step(s1, there));
+        if (moved) move_refs(false);
+        if (more) first_part(flags + 2 * who + (s1 & 1));
+      } else {
+        if (moved) {  // (K of s2 is still there)
+          scores(s2, who ? there : there_before, false);
+          move_refs(true);
+        }
+        if (s1 + 1 < s_end) issue(s1 + 1, page_next, who == 1);
+        if (t > 0) second_part(s2);
       }
       if (threadIdx.x == 0) {
-        rise[(s1 & 1) ^ 1] = 0;
+        flags[2 * who + ((s1 & 1) ^ 1)] = 0;
         if (who == 1) flags[4 + ((s1 & 1) ^ 1)] = 0;
       }
-      if (lead) {
-        if (s1 < s_end) {
-          if (s1 + 1 < s_end) {
-            if (rg == 0)
-              issue(s1 + 1, page_next, true, false);
-            else
-              issue(s1 + 1, page_next, false, true);
-          }
-          page = page_next;
-          if (s1 + 2 < s_end) page_next = page_of(s1 + 2);
-          first_part(s1, there, rise + (s1 & 1));
-        }
-      } else if (t > 0) {
-        second_part(s2);
+      if (who == 1) {
+        page = page_next;
+        if (s1 + 2 < s_end) page_next = page_of(s1 + 2);
       }
     }
   }
