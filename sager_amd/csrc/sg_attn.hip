@@ -3,26 +3,27 @@
 //
 // For a kv head, the rows of a product are (node, query head of the group).
 // A workgroup takes a block of rows and a part of a sequence's keys, 64 keys
-// a step, in rows' groups of four waves:
-//   S^T = K Q^T   wave w has keys 16w..16w+15 and all rows of its group (Q in
-//                 registers);
-//   P             goes through LDS to the group's other waves;
-//   O^T = V^T P^T wave w has columns w D/4 .. of all keys.
-// So K and V are read from LDS once per group, no wave holds more than a
-// quarter of O, and nothing is joined at the end but the rows' sums.  With
-// keys as the first product's rows, a lane of v_mfma_f32_16x16x32_f16 gets
-// four consecutive keys of one query row, 8 B of P; and since the order of a
-// product's 32 terms is free, V's operand is, per lane, one column of V at
-// four and four consecutive keys, which ds_read_b64_tr_b16 reads from V's
-// rows as they lie in memory.
+// a step through two LDS buffers: S^T = K Q^T, then O^T = V^T P^T.  With keys
+// as the first product's rows, a lane of v_mfma_f32_16x16x32_f16 gets four
+// consecutive keys of one query row; and since the order of a product's 32
+// terms is free, V's operand is, per lane, one column of V at four and four
+// consecutive keys, which ds_read_b64_tr_b16 reads from V's rows as they lie
+// in memory.  Two kernels:
 //
-// The running maximum is a reference point `mref` per row, common to the
-// group's waves, that moves only when a score passes it by 2^15: p =
-// 2^(s - mref) fits fp16 (its largest value is 2^16), and 2^(8+15) below it
-// is still a normal number.  Until a score does, the waves share nothing but
-// P; then all of them stop for it.  p is rounded to fp16 for the product
-// (2^-11 of each weight, below the output's own rounding to fp16 once a few
-// keys are averaged); l = sum p is fp32, of the unrounded p.
+//   attn_few_kernel   up to 64 rows: the four waves share the keys of the
+//                     first product and the columns of the second, P goes
+//                     through LDS between them.  K and V are read from LDS
+//                     once, no wave holds more than a quarter of O, and
+//                     nothing is joined at the end but the rows' sums.
+//   attn_rows_kernel  more rows: each wave has 32 rows of its own and reads
+//                     all of K and V from LDS; P stays in its lanes, and one
+//                     barrier a step orders the copies.
+//
+// A row's running maximum is a reference point `mref` that moves only when a
+// score passes it by 2^15: p = 2^(s - mref) fits fp16 (its largest value is
+// 2^16), and 2^(8+15) below it is still a normal number.  p is rounded to
+// fp16 for the product (2^-11 of each weight, no more than the output's own
+// rounding to fp16); l = sum p is fp32, of the unrounded p.
 #include "sg_window.hpp"
 
 namespace sg {
@@ -54,6 +55,15 @@ struct AttnArgs {
   float scale_log2;
 };
 
+// The arguments once more from where the launch put them, for paths taken now
+// and then: what only they need then holds no scalar registers between.
+typedef const __attribute__((address_space(4))) AttnArgs* kernarg_p;
+__device__ __forceinline__ kernarg_p cold_args() {
+  kernarg_p p = (kernarg_p)__builtin_amdgcn_kernarg_segment_ptr();
+  asm volatile("" : "+s"(p));
+  return p;
+}
+
 // The cached tokens of a sequence that the page table can hold.
 __device__ __forceinline__ int cached_len(int length, int page_log2, int pages_per_seq) {
   const long long cap = static_cast<long long>(pages_per_seq) << page_log2;
@@ -81,97 +91,107 @@ __device__ __forceinline__ void dma16_ptr(uint32_t lds, const void* src) {
                : "s"(__builtin_amdgcn_readfirstlane(lds)), "v"(src)
                : "memory");
 }
+__device__ __forceinline__ bool fp16_odd(uint32_t b) { return (b & 0x7C00) == 0x7C00; }
 
-// Bytes of LDS: K and V of two steps, P, the rows' maxima and sums of the four
-// waves, the nodes' ancestors, and the flags.
-template <int D, int RT, int RW>
-struct AttnLds {
+// What both kernels know of their part of the work.  K and V of step s lie at
+// (s & 1) * 2 kStep and kStep after it, 64 rows of D values each, their 16-B
+// chunks at chunk ^ swz(row).
+template <int D>
+struct Part {
+  static constexpr int CH = D / 8;       // 16-B chunks of a row
+  static constexpr int RPI = 64 / CH;    // rows of a copy instruction
+  static constexpr int NI = 16 / RPI;    // copy instructions of 16 keys
+  static constexpr int KK = D / 32;      // steps of the first product
+  static constexpr int KO = KK < 4 ? KK : 4;
   static constexpr uint32_t kStep = kKeys * D * 2;
-  static constexpr uint32_t kRows = 16 * RT * RW;
-  static constexpr uint32_t kP = 4 * kStep;
-  static constexpr uint32_t kMax = kP + kRows * kKeys * 2;
-  static constexpr uint32_t kSeen = kMax + 4 * kRows * 4;
-  static constexpr uint32_t kFlags = kSeen + kMaxWindow * 8;
-  static constexpr uint32_t kBytes = kFlags + 32;
-};
 
-// RT: tiles of 16 rows of a group; RW: groups of four waves.
-template <int D, int RT, int RW>
-__global__ void __launch_bounds__(256 * RW) attn_tree_kernel(const AttnArgs a) {
-  typedef AttnLds<D, RT, RW> L;
-  constexpr int CH = D / 8;       // 16-B chunks of a row
-  constexpr int RPI = 64 / CH;    // rows of a copy instruction
-  constexpr int NI = 16 / RPI;    // copy instructions of a wave's 16 keys
-  constexpr int KK = D / 32;      // steps of the first product
-  constexpr int DQ = D / 64;      // 16-column tiles of a wave's part of O
-  constexpr int kRows = L::kRows;
-  extern __shared__ __attribute__((aligned(16))) unsigned char lds[];
-  const uint32_t lds0 = static_cast<uint32_t>(
-      reinterpret_cast<uintptr_t>((__attribute__((address_space(3))) unsigned char*)lds));
-  int* flags = reinterpret_cast<int*>(lds + L::kFlags);  // by step parity: rise of either group, odd
-  float* mx = reinterpret_cast<float*>(lds + L::kMax);
-  uint64_t* seen = reinterpret_cast<uint64_t*>(lds + L::kSeen);  // node: whom it sees
-  const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
-  const int kw = wave & 3, rg = wave >> 2;
-  const int lane = threadIdx.x & 63, col = lane & 15, grp = lane >> 4;
+  const AttnArgs& a;
+  int lane, col, grp;
+  int split, rb, h, seq;
+  Window win;
+  int rows, len, total;  // rows of the window; cached keys, cached and window's
+  int begin, end;        // steps
+  const_int_p table;
+  unsigned char* lds;
+  uint32_t lds0;
 
   // The row blocks of a unit (part, kv head, sequence) are 8 workgroups apart:
   // on one XCD, whose L2 then reads the unit's keys once.
-  const int id = blockIdx.x;
-  const int oct = id / (8 * a.row_blocks), in = id - oct * 8 * a.row_blocks;
-  const int rb = in >> 3;
-  int unit = oct * 8 + (in & 7);
-  if (unit >= a.units) return;
-  const int split = unit % a.n_split;
-  unit /= a.n_split;
-  const int h = unit % a.n_kv, seq = unit / a.n_kv;
-  const Window win = window_of(a.win_off, seq, a.n_tokens, a.max_window);
-  const int rows = win.n * a.group;
-  if (rb * kRows >= rows) return;
-  const int len = cached_len(((const_int_p)a.length)[seq], a.page_log2, a.pages_per_seq);
-  const int total = len + win.n;
-  const const_int_p table = (const_int_p)(a.pages + static_cast<long long>(seq) * a.pages_per_seq);
-  const int steps = (total + kKeys - 1) / kKeys;
-  const int per = a.split_keys / kKeys;
-  const long long first = static_cast<long long>(split) * per;
-  const int s_end = split == a.n_split - 1 || first + per > steps ? steps
-                                                                  : static_cast<int>(first + per);
-  int step = first < s_end ? static_cast<int>(first) : s_end;
-
-  // ---- copies: wave kw brings keys 16 kw.. of a step (of two groups, the
-  // first brings V's, the second K's) ----
-  const uint32_t blk = kw * 16 * D * 2;
-  auto page_of = [&](int s) {
-    const int j = s * kKeys + 16 * kw;
+  __device__ __forceinline__ bool start(unsigned char* l, int block_rows) {
+    lds = l;
+    lds0 = static_cast<uint32_t>(
+        reinterpret_cast<uintptr_t>((__attribute__((address_space(3))) unsigned char*)l));
+    lane = threadIdx.x & 63;
+    col = lane & 15;
+    grp = lane >> 4;
+    const int id = blockIdx.x;
+    const int oct = id / (8 * a.row_blocks), in = id - oct * 8 * a.row_blocks;
+    rb = in >> 3;
+    int unit = oct * 8 + (in & 7);
+    if (unit >= a.units) return false;
+    split = unit % a.n_split;
+    unit /= a.n_split;
+    h = unit % a.n_kv;
+    seq = unit / a.n_kv;
+    win = window_of(a.win_off, seq, a.n_tokens, a.max_window);
+    rows = win.n * a.group;
+    if (rb * block_rows >= rows) return false;
+    len = cached_len(((const_int_p)a.length)[seq], a.page_log2, a.pages_per_seq);
+    total = len + win.n;
+    table = (const_int_p)(a.pages + static_cast<long long>(seq) * a.pages_per_seq);
+    const int steps = (total + kKeys - 1) / kKeys, per = a.split_keys / kKeys;
+    const long long first = static_cast<long long>(split) * per;
+    end = split == a.n_split - 1 || first + per > steps ? steps : static_cast<int>(first + per);
+    begin = first < end ? static_cast<int>(first) : end;
+    return true;
+  }
+  // The page of keys 16 b.. of step s (pages hold a multiple of 16 keys).
+  __device__ __forceinline__ int page_of(int s, int b) const {
+    const int j = s * kKeys + 16 * b;
     return j < len ? table[j >> a.page_log2] : -1;
-  };
-  auto page_ok = [&](int p) { return static_cast<uint32_t>(p) < static_cast<uint32_t>(a.n_pages); };
-  // Brings a step's K and V; with two groups, V or K.
-  auto issue = [&](int s, int page, bool v) {
-    const int j = s * kKeys + 16 * kw;
-    const uint32_t buf = lds0 + (s & 1) * 2 * L::kStep + blk + (RW == 2 && v ? L::kStep : 0);
+  }
+  __device__ __forceinline__ bool page_ok(int p) const {
+    return static_cast<uint32_t>(p) < static_cast<uint32_t>(a.n_pages);
+  }
+  // bit r: key 16 b + r of step s is there
+  __device__ __forceinline__ uint32_t present(int s, int b, int page) const {
+    const int j = s * kKeys + 16 * b;
+    const int nc = min(max(len - j, 0), 16), nw = min(max(total - j, 0), 16);
+    return ((1u << nw) - 1) & (page_ok(page) ? 0xFFFFu : ~((1u << nc) - 1));
+  }
+  // whether all 16 keys are the cache's, and there
+  __device__ __forceinline__ bool plain(int s, int b, int page) const {
+    return s * kKeys + 16 * b + 16 <= len && page_ok(page);
+  }
+  // Brings keys 16 b.. of step s: K (kv 1), V (2) or both (3).
+  template <bool kAnew>
+  __device__ __forceinline__ void issue(int s, int b, int page, int kv) const {
+    const int j = s * kKeys + 16 * b;
+    const uint32_t buf = lds0 + (s & 1) * 2 * kStep + b * 16 * D * 2 + (kv == 2 ? kStep : 0);
     const long long at =
         (((static_cast<long long>(page) * a.n_kv + h) << a.page_log2) +
          (j & ((1 << a.page_log2) - 1))) * D;
-    const uint16_t* const c1 = RW == 2 && v ? a.vc : a.kc;
-    if (j + 16 <= len && page_ok(page)) {
+    const uint16_t* const c1 = kv == 2 ? a.vc : a.kc;
+    if (plain(s, b, page)) {
       const uint16_t* b1 = uniform_ptr(c1 + at);
       const uint16_t* b2 = uniform_ptr(a.vc + at);
       int ln = lane;
-      if (RT >= 3) asm("" : "+v"(ln));  // (the offsets made anew: registers are short)
+      if (kAnew) asm("" : "+v"(ln));  // (the offsets made anew: registers are short)
 #pragma unroll
       for (int i = 0; i < NI; ++i) {
         const int row = i * RPI + ln / CH;
         const uint32_t off = row * (D * 2) + (((ln % CH) ^ swz<D>(row)) << 4);
         dma16_base(buf + i * 1024, off, b1);
-        if (RW == 1) dma16_base(buf + L::kStep + i * 1024, off, b2);
+        if (kv == 3) dma16_base(buf + kStep + i * 1024, off, b2);
       }
     } else if (j < total) {
       // rows of the cache, then of the window; what is not there reads a
       // window row and is masked
       const int n_cache = page_ok(page) ? min(len - j, 16) : 0;
-      const uint16_t* const w1 = RW == 2 && v ? a.v : a.k;
-      const long long ws1 = RW == 2 && v ? a.v_stride : a.k_stride;
+      const kernarg_p ca = cold_args();
+      const uint16_t* const w1 = kv == 2 ? ca->v : ca->k;
+      const uint16_t* const w2 = ca->v;
+      const long long ws1 = kv == 2 ? ca->v_stride : ca->k_stride, ws2 = ca->v_stride;
 #pragma unroll 1
       for (int i = 0; i < NI; ++i) {
         const int row = i * RPI + lane / CH;
@@ -179,80 +199,19 @@ __global__ void __launch_bounds__(256 * RW) attn_tree_kernel(const AttnArgs a) {
         const long long w = win.off + min(max(j + row - len, 0), win.n - 1);
         const bool cached = row < n_cache;
         dma16_ptr(buf + i * 1024, (cached ? c1 + at + row * D : w1 + w * ws1 + h * D) + c);
-        if (RW == 1)
-          dma16_ptr(buf + L::kStep + i * 1024,
-                    (cached ? a.vc + at + row * D : a.v + w * a.v_stride + h * D) + c);
+        if (kv == 3)
+          dma16_ptr(buf + kStep + i * 1024,
+                    (cached ? a.vc + at + row * D : w2 + w * ws2 + h * D) + c);
       }
     }
-  };
-  // bit r: key 16 kw + r of the step is there
-  auto present = [&](int s, int page) {
-    const int j = s * kKeys + 16 * kw;
-    const int nc = min(max(len - j, 0), 16), nw = min(max(total - j, 0), 16);
-    const uint32_t c = (1u << nc) - 1;
-    return ((1u << nw) - 1) & (page_ok(page) ? 0xFFFFu : ~c);
-  };
-
-  int page = page_of(step), page_next = 0;
-  if (step < s_end) {
-    issue(step, page, rg == 0);
-    page_next = page_of(step + 1);
   }
-  if (threadIdx.x < 8) flags[threadIdx.x] = 0;
-
-  // ---- Q's rows, while the first copies are under way ----
-  if (wave == 4 * RW - 1) seen[lane] = ancestors(a.parent, win, lane);
-  const int row0 = rb * kRows + rg * 16 * RT;
-  auto node_of = [&](int rt) { return min(row0 + rt * 16 + col, rows - 1) / a.group; };
-  h8 qf[RT][KK];
-#pragma unroll
-  for (int rt = 0; rt < RT; ++rt) {
-    const int r = min(row0 + rt * 16 + col, rows - 1);  // (a row past the end repeats the last)
-    const int node = r / a.group, g = r - node * a.group;
-    const uint16_t* qp = a.q + static_cast<long long>(win.off + node) * a.q_stride +
-                         (h * a.group + g) * D;
-#pragma unroll
-    for (int s = 0; s < KK; ++s) {
-      const u32x4 w = *reinterpret_cast<const u32x4_u*>(qp + s * 32 + grp * 8);
-      qf[rt][s] = __builtin_bit_cast(h8, w);
-    }
-  }
-
-  f4 acc[RT][DQ];
-  float mref[RT], l[RT];
-  bool begun[RT];
-#pragma unroll
-  for (int rt = 0; rt < RT; ++rt) {
-    mref[rt] = 0.f;
-    l[rt] = 0.f;
-    begun[rt] = false;
-#pragma unroll
-    for (int d = 0; d < DQ; ++d) acc[rt][d] = (f4){0.f, 0.f, 0.f, 0.f};
-  }
-  // P: [row][two halves of 32 keys][grp][two blocks of 16 keys][4], 16-B pieces
-  // swizzled over the row's eight
-  unsigned char* const pl = lds + L::kP + rg * 16 * RT * 128;
-  const int psw = (col >> 1) & 7;
-  // K's pieces st * 4 + grp of row col, swizzled: four offsets, the rest is added.  V's: columns
-  // kw D/4 + 16 d.. of row 4 grp + col / 4 of a 16-key block.
-  constexpr int KO = KK < 4 ? KK : 4;
-  uint32_t koff[KO], voff[DQ];
-#pragma unroll
-  for (int i = 0; i < KO; ++i)
-    koff[i] = blk + col * (D * 2) + (((i * 4) ^ grp ^ swz<D>(col)) << 4);
-#pragma unroll
-  for (int d = 0; d < DQ; ++d)
-    voff[d] = lds0 + L::kStep + (4 * grp + (col >> 2)) * (D * 2) +
-              (((2 * d) ^ (kw * (CH / 4) + ((col & 3) >> 1)) ^ swz<D>(4 * grp + (col >> 2))) << 4) +
-              (col & 1) * 8;
-  unsigned char* const p_out = pl + col * 128 + ((((kw >> 1) * 4 + grp) ^ psw) << 4) + (kw & 1) * 8;
-
   // Rows of V that nobody sees become 0 (0 times what lies there need not be
-  // 0).  Window rows, which some queries see and others do not, are looked
-  // through for infinities and NaN.  Each wave does the rows it has copied.
-  auto fix_v = [&](int s, uint32_t there) {
-    const int j = s * kKeys + 16 * kw;
-    unsigned char* vb = lds + (s & 1) * 2 * L::kStep + L::kStep + blk;
+  // 0), and so do infinities and NaN in the window's rows, which some queries
+  // see and others do not: true if there are any, to be added by odd_v.  For
+  // the 16 keys that the calling wave has brought.
+  __device__ __forceinline__ bool fix_v(int s, int b, uint32_t there) const {
+    const int j = s * kKeys + 16 * b;
+    unsigned char* vb = lds + (s & 1) * 2 * kStep + kStep + b * 16 * D * 2;
     bool odd = false;
 #pragma unroll 1
     for (int i = 0; i < NI; ++i) {
@@ -261,86 +220,233 @@ __global__ void __launch_bounds__(256 * RW) attn_tree_kernel(const AttnArgs a) {
       if (!(there >> row & 1)) {
         *at = (u32x4){0, 0, 0, 0};
       } else if (j + row >= len && win.n > 1) {
-        const u32x4 w = *at;
+        u32x4 w = *at;
+        bool mine = false;
 #pragma unroll
-        for (int c = 0; c < 4; ++c)
-          odd |= (w[c] & 0x7C00u) == 0x7C00u || (w[c] & 0x7C000000u) == 0x7C000000u;
+        for (int c = 0; c < 4; ++c) {
+          const bool lo = fp16_odd(w[c]), hi = fp16_odd(w[c] >> 16);
+          mine |= lo || hi;
+          w[c] &= (lo ? 0u : 0xFFFFu) | (hi ? 0u : 0xFFFF0000u);
+        }
+        if (mine) *at = w;
+        odd |= mine;
       }
     }
-    if (__any(odd) && lane == 0) flags[4 + (s & 1)] = 1;
-  };
-  auto plain_step = [&](int s, uint32_t there) {
-    return s * kKeys + 16 * kw + 16 <= len && there == 0xFFFFu;
-  };
+    return __any(odd);
+  }
+  // bit i: key 16 b + 4 grp + i of step s is there and seen by a node with these ancestors
+  __device__ __forceinline__ uint32_t seen_bits(int s, int b, uint32_t there, uint64_t up) const {
+    const int w0 = s * kKeys + 16 * b - len;  // key 0's window node, if not negative
+    const uint32_t tree = w0 >= 0    ? static_cast<uint32_t>(up >> (w0 & 63))
+                          : w0 > -16 ? static_cast<uint32_t>(up << -w0) | ((1u << -w0) - 1)
+                                     : 0xFFFFu;
+    return (there & tree) >> (4 * grp);
+  }
+  __device__ __forceinline__ int node_of(int r) const {
+    return min(r, rows - 1) / cold_args()->group;
+  }
+  // The 16-B pieces of Q's row r that a lane holds (a row past the end: the last).
+  __device__ __forceinline__ void load_q(int r, h8 (&q)[KK]) const {
+    r = min(r, rows - 1);
+    const int node = r / a.group, g = r - node * a.group;
+    const uint16_t* qp =
+        a.q + static_cast<long long>(win.off + node) * a.q_stride + (h * a.group + g) * D;
+#pragma unroll
+    for (int s = 0; s < KK; ++s) {
+      const u32x4 w = *reinterpret_cast<const u32x4_u*>(qp + s * 32 + grp * 8);
+      q[s] = __builtin_bit_cast(h8, w);
+    }
+  }
+  // Piece st * 4 + grp of K's row col of a 16-key block; at: k_offset plus
+  // the block's place, multiples of 256 B.
+  __device__ __forceinline__ uint32_t k_offset() const {
+    return col * (D * 2) + ((grp ^ swz<D>(col)) << 4);
+  }
+  __device__ __forceinline__ h8 k_frag(uint32_t at, int st) const {
+    return *reinterpret_cast<const h8*>(lds + ((at ^ ((st & 3) << 6)) + (st >> 2) * 256));
+  }
+  // V's columns 0..15 of row 4 grp + col / 4 of a 16-key block; tile c of
+  // columns is at v_tile(that plus the block's place, c).
+  __device__ __forceinline__ uint32_t v_offset() const {
+    const int row = 4 * grp + (col >> 2);
+    return kStep + row * (D * 2) + ((((col & 3) >> 1) ^ swz<D>(row)) << 4) + (col & 1) * 8;
+  }
+  static __device__ __forceinline__ uint32_t v_tile(uint32_t at, int c) {
+    return (at ^ ((c & 7) << 5)) + (c >> 3) * 256;
+  }
+  // V's operand: 16 columns (at: v_tile) at keys 32 st.. of a step
+  __device__ __forceinline__ h8 v_frag(uint32_t at, int st) const {
+    s4 x[2];
+#pragma unroll
+    for (int b = 0; b < 2; ++b)
+      x[b] = __builtin_amdgcn_ds_read_tr16_b64_v4i16(
+          (lds_s4_p)(static_cast<uintptr_t>(lds0 + at + (st * 2 + b) * 16 * D * 2)));
+    return __builtin_bit_cast(h8, __builtin_shufflevector(x[0], x[1], 0, 1, 2, 3, 4, 5, 6, 7));
+  }
+  // What weight w adds at window node `node` and column c for fix_v's infinities and NaN.
+  __device__ __forceinline__ float odd_v(int node, int c, float w) const {
+    const kernarg_p ca = cold_args();
+    const uint16_t b =
+        ca->v[static_cast<long long>(win.off + node) * ca->v_stride + h * D + c];
+    return fp16_odd(b) ? w * half_bits_to_float(b) : 0.f;
+  }
+  // Row r's columns c.. (4), and its sum l about mref.
+  template <int N, int kStride>
+  __device__ __forceinline__ void store(int r, int c, const f4 (&o)[N], float mref, float l,
+                                        bool first) const {
+    if (r >= rows) return;
+    const kernarg_p a = cold_args();
+    const int node = r / a->group, g = r - node * a->group;
+    const long long at = static_cast<long long>(win.off + node) * a->n_heads + h * a->group + g;
+    if (a->n_split == 1) {
+      const float inv = l != 0.f ? 1.f / l : 0.f;
+#pragma unroll
+      for (int d = 0; d < N; ++d) {
+        h4 y;
+#pragma unroll
+        for (int i = 0; i < 4; ++i)
+          y[i] = l != 0.f ? static_cast<_Float16>(o[d][i] * inv) : static_cast<_Float16>(0);
+        *reinterpret_cast<h4*>(a->out + at * D + c + d * kStride) = y;
+      }
+    } else {
+      const long long pa = static_cast<long long>(split) * a->n_tokens * a->n_heads + at;
+#pragma unroll
+      for (int d = 0; d < N; ++d)
+        *reinterpret_cast<f4*>(a->part_o + pa * D + c + d * kStride) = o[d];
+      if (first) a->part_ml[pa] = make_float2(mref, l);
+    }
+  }
+};
 
-  float e[RT][4], top[RT], sum[RT];
-  // e: the scores of a step's keys 16 kw.. above mref, log2; top: their largest per row
-  auto scores = [&](int step_, uint32_t there, bool plain) {
-    const unsigned char* kb = lds + (step_ & 1) * 2 * L::kStep;
+// ---- up to 64 rows ---------------------------------------------------------------
+// LDS: K and V of two steps, P, the rows' maxima and sums of the four waves,
+// the nodes' ancestors, the flags.
+template <int D, int RT>
+struct FewLds {
+  static constexpr uint32_t kRows = 16 * RT;
+  static constexpr uint32_t kP = 4 * Part<D>::kStep;
+  static constexpr uint32_t kMax = kP + kRows * kKeys * 2;
+  static constexpr uint32_t kSeen = kMax + 4 * kRows * 4;
+  static constexpr uint32_t kFlags = kSeen + kMaxWindow * 8;
+  static constexpr uint32_t kBytes = kFlags + 16;
+};
+
+// RT: tiles of 16 rows.  Wave w brings keys 16 w.. of a step, has them in the
+// first product, and has columns w D/4 .. of all keys in the second.
+template <int D, int RT>
+__global__ void __launch_bounds__(256) attn_few_kernel(const AttnArgs a) {
+  typedef Part<D> P;
+  typedef FewLds<D, RT> L;
+  constexpr int DQ = D / 64;  // 16-column tiles of a wave's part of O
+  constexpr int kRows = L::kRows;
+  extern __shared__ __attribute__((aligned(16))) unsigned char lds[];
+  const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+  P t{a};
+  if (!t.start(lds, kRows)) return;
+  const int lane = t.lane, col = t.col, grp = t.grp, row0 = t.rb * kRows;
+  // flags of odd and even steps: 1 + the last step whose reference points move, and the last
+  // with infinities or NaN in its window's V
+  int* rise = reinterpret_cast<int*>(lds + L::kFlags);
+  int* odds = rise + 2;
+  float* mx = reinterpret_cast<float*>(lds + L::kMax);
+  uint64_t* seen = reinterpret_cast<uint64_t*>(lds + L::kSeen);  // node: whom it sees
+
+  int step = t.begin;
+  int page = t.page_of(step, wave), page_next = 0;
+  if (step < t.end) {
+    t.template issue<false>(step, wave, page, 3);
+    page_next = t.page_of(step + 1, wave);
+  }
+  if (threadIdx.x < 4) rise[threadIdx.x] = 0;
+  if (wave == 3) seen[lane] = ancestors(a.parent, t.win, lane);
+
+  h8 qf[RT][P::KK];
+  f4 acc[RT][DQ];
+  float mref[RT], l[RT];
+  bool begun[RT];
+#pragma unroll
+  for (int rt = 0; rt < RT; ++rt) {
+    t.load_q(row0 + rt * 16 + col, qf[rt]);
+    mref[rt] = 0.f;
+    l[rt] = 0.f;
+    begun[rt] = false;
+#pragma unroll
+    for (int d = 0; d < DQ; ++d) acc[rt][d] = (f4){0.f, 0.f, 0.f, 0.f};
+  }
+  const uint32_t koff = t.k_offset() + wave * 16 * D * 2, voff0 = t.v_offset();
+  uint32_t voff[DQ];
+#pragma unroll
+  for (int d = 0; d < DQ; ++d) voff[d] = t.v_tile(voff0, wave * DQ + d);
+  // P: [row][two halves of 32 keys][grp][two blocks of 16 keys][4], 16-B pieces
+  // swizzled over the row's eight
+  unsigned char* const pl = lds + L::kP;
+  const int psw = (col >> 1) & 7;
+  unsigned char* const p_out =
+      pl + col * 128 + ((((wave >> 1) * 4 + grp) ^ psw) << 4) + (wave & 1) * 8;
+
+  bar();  // the flags are cleared
+  for (; step < t.end; ++step) {
+    const int par = step & 1;
+    const uint32_t there = t.present(step, wave, page);
+    const bool plain = t.plain(step, wave, page);
+    wait_vm();
+    if (!plain && t.fix_v(step, wave, there)) odds[par] = step + 1;
+    bar();  // everybody's copies of this step are here, and nobody reads the other buffers or P
+    if (step + 1 < t.end) t.template issue<false>(step + 1, wave, page_next, 3);
+    page = page_next;
+    if (step + 2 < t.end) page_next = t.page_of(step + 2, wave);
+
     f4 s[RT];
 #pragma unroll
     for (int rt = 0; rt < RT; ++rt) s[rt] = (f4){0.f, 0.f, 0.f, 0.f};
 #pragma unroll
-    for (int st = 0; st < KK; ++st) {
-      const h8 kf = *reinterpret_cast<const h8*>(kb + koff[st % KO] + st / KO * 256);
+    for (int st = 0; st < P::KK; ++st) {
+      const h8 kf = t.k_frag(koff + par * 2 * P::kStep, st);
 #pragma unroll
       for (int rt = 0; rt < RT; ++rt)
         s[rt] = __builtin_amdgcn_mfma_f32_16x16x32_f16(kf, qf[rt][st], s[rt], 0, 0, 0);
-      if (RW == 2 && st % 4 == 3) asm volatile("" ::: "memory");  // (no more reads ahead: registers)
     }
+    float e[RT][4], top[RT], sum[RT];
+    auto weigh = [&](int rt, float by) {  // row tile rt's p = 2^(e - by), into LDS
+      float p[4];
+      h4 ph;
+#pragma unroll
+      for (int i = 0; i < 4; ++i) {
+        p[i] = __builtin_amdgcn_exp2f(e[rt][i] - by);
+        ph[i] = static_cast<_Float16>(p[i]);
+      }
+      sum[rt] = (p[0] + p[1]) + (p[2] + p[3]);
+      *reinterpret_cast<h4*>(p_out + rt * 16 * 128) = ph;
+    };
+    bool move = false;
 #pragma unroll
     for (int rt = 0; rt < RT; ++rt) {
 #pragma unroll
       for (int i = 0; i < 4; ++i) e[rt][i] = __builtin_fmaf(s[rt][i], a.scale_log2, -mref[rt]);
       if (!plain) {
-        // bit r of `see`: key r is there and this lane's row sees it
-        const uint64_t up = seen[node_of(rt)];
-        const int w0 = step_ * kKeys + 16 * kw - len;  // key 0's window node, if not negative
-        const uint32_t tree = w0 >= 0    ? static_cast<uint32_t>(up >> (w0 & 63))
-                              : w0 > -16 ? static_cast<uint32_t>(up << -w0) | ((1u << -w0) - 1)
-                                         : 0xFFFFu;
-        const uint32_t see = (there & tree) >> (4 * grp);
+        const uint32_t see = t.seen_bits(step, wave, there, seen[t.node_of(row0 + rt * 16 + col)]);
 #pragma unroll
         for (int i = 0; i < 4; ++i) e[rt][i] = see & 1u << i ? e[rt][i] : -INFINITY;
       }
       top[rt] = fmaxf(fmaxf(e[rt][0], e[rt][1]), fmaxf(e[rt][2], e[rt][3]));
-    }
-  };
-  auto weigh = [&](int rt, float by) {  // row tile rt's p = 2^(e - by), into LDS
-    float p[4];
-    h4 ph;
-#pragma unroll
-    for (int i = 0; i < 4; ++i) {
-      p[i] = __builtin_amdgcn_exp2f(e[rt][i] - by);
-      ph[i] = static_cast<_Float16>(p[i]);
-    }
-    sum[rt] = (p[0] + p[1]) + (p[2] + p[3]);
-    *reinterpret_cast<h4*>(p_out + rt * 16 * 128) = ph;
-  };
-  auto first_part = [&](int* rise_flag) {  // after scores()
-    bool rise = false;
-#pragma unroll
-    for (int rt = 0; rt < RT; ++rt) {
-      rise |= top[rt] > kRise || (!begun[rt] && top[rt] > -INFINITY);
+      move |= top[rt] > kRise || (!begun[rt] && top[rt] > -INFINITY);
       weigh(rt, 0.f);
     }
-    if (__any(rise) && lane == 0) *rise_flag = 1;
-  };
-  // The reference points move: the rows' maxima over the group's waves, then P
-  // once more.  Every wave of the workgroup comes to the two barriers.
-  auto move_refs = [&](bool mine) {
-    if (mine)
+    if (__any(move)) rise[par] = step + 1;
+    bar();  // P is here
+
+    if (rise[par] == step + 1) {
+      // The reference points move: the rows' maxima over the waves, then P once more.
 #pragma unroll
       for (int rt = 0; rt < RT; ++rt) {
         float m = fmaxf(top[rt], __shfl_xor(top[rt], 16));
         m = fmaxf(m, __shfl_xor(m, 32));
-        if (grp == 0) mx[kw * kRows + (rg * RT + rt) * 16 + col] = m;
+        if (grp == 0) mx[wave * kRows + rt * 16 + col] = m;
       }
-    bar();
-    if (mine)
+      bar();
 #pragma unroll
       for (int rt = 0; rt < RT; ++rt) {
-        const float* mr = mx + (rg * RT + rt) * 16 + col;
+        const float* mr = mx + rt * 16 + col;
         const float m = fmaxf(fmaxf(mr[0], mr[kRows]), fmaxf(mr[2 * kRows], mr[3 * kRows]));
         const bool set = m > kRise || (!begun[rt] && m > -INFINITY);
         const float by = set ? m - kBelow : 0.f;
@@ -352,39 +458,32 @@ __global__ void __launch_bounds__(256 * RW) attn_tree_kernel(const AttnArgs a) {
         begun[rt] |= set;
         weigh(rt, by);
       }
-    bar();
-  };
-  auto second_part = [&](int s) {
-    const unsigned char* vb = lds + (s & 1) * 2 * L::kStep + L::kStep;
-    const bool odd = flags[4 + (s & 1)] != 0;
+      bar();
+    }
 #pragma unroll
     for (int rt = 0; rt < RT; ++rt) l[rt] += sum[rt];
-    if (odd) {
-      // Infinities and NaN in the window's V: added one by one to the rows
-      // that see them, and taken as 0 below.
+
+    if (odds[par] == step + 1) {  // one by one, to the rows that see them
 #pragma unroll 1
       for (int r = 0; r < kKeys; ++r) {
-        const int node = s * kKeys + r - len;
-        if (node < 0 || node >= win.n) continue;
+        const int node = step * kKeys + r - t.len;
+        if (node < 0 || node >= t.win.n) continue;
         const int piece = (r >> 5) * 4 + ((r & 15) >> 2);
 #pragma unroll
         for (int rt = 0; rt < RT; ++rt) {
           const float w = half_bits_to_float(*reinterpret_cast<const uint16_t*>(
               pl + (rt * 16 + col) * 128 + ((piece ^ psw) << 4) + (r >> 4 & 1) * 8 + (r & 3) * 2));
-          const bool see = seen[node_of(rt)] >> node & 1;
+          const bool see = seen[t.node_of(row0 + rt * 16 + col)] >> node & 1;
 #pragma unroll
           for (int d = 0; d < DQ; ++d)
 #pragma unroll
             for (int i = 0; i < 4; ++i) {
-              const int c = kw * (D / 4) + d * 16 + 4 * grp + i;
-              const uint16_t b = *reinterpret_cast<const uint16_t*>(
-                  vb + r * (D * 2) + (((c >> 3) ^ swz<D>(r)) << 4) + (c & 7) * 2);
-              acc[rt][d][i] += see && (b & 0x7C00) == 0x7C00 ? w * half_bits_to_float(b) : 0.f;
+              const float v = t.odd_v(node, (wave * DQ + d) * 16 + 4 * grp + i, w);
+              acc[rt][d][i] += see ? v : 0.f;
             }
         }
       }
     }
-    const uint32_t vl = (s & 1) * 2 * L::kStep;
 #pragma unroll
     for (int st = 0; st < 2; ++st) {
       h8 pf[RT];
@@ -394,130 +493,217 @@ __global__ void __launch_bounds__(256 * RW) attn_tree_kernel(const AttnArgs a) {
                                               (((st * 4 + grp) ^ psw) << 4));
 #pragma unroll
       for (int d = 0; d < DQ; ++d) {
-        s4 x[2];
-#pragma unroll
-        for (int b = 0; b < 2; ++b) {
-          x[b] = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_s4_p)(static_cast<uintptr_t>(
-              vl + voff[d] + (st * 2 + b) * 16 * D * 2)));
-          if (odd) {
-            const int j = s * kKeys + (st * 2 + b) * 16 + 4 * grp;
-#pragma unroll
-            for (int i = 0; i < 4; ++i)
-              x[b][i] = j + i >= len && (x[b][i] & 0x7C00) == 0x7C00 ? 0 : x[b][i];
-          }
-        }
-        const h8 vf = __builtin_bit_cast(
-            h8, __builtin_shufflevector(x[0], x[1], 0, 1, 2, 3, 4, 5, 6, 7));
+        const h8 vf = t.v_frag(voff[d] + par * 2 * P::kStep, st);
 #pragma unroll
         for (int rt = 0; rt < RT; ++rt)
           acc[rt][d] = __builtin_amdgcn_mfma_f32_16x16x32_f16(vf, pf[rt], acc[rt][d], 0, 0, 0);
       }
-      if (RW == 2) asm volatile("" ::: "memory");
-    }
-  };
-
-  bar();  // the flags are cleared
-  if (RW == 1) {
-    for (; step < s_end; ++step) {
-      const int par = step & 1;
-      const uint32_t there = present(step, page);
-      wait_vm();
-      if (!plain_step(step, there)) fix_v(step, there);
-      bar();  // everybody's copies of this step are here, and nobody reads the other buffers or P
-      if (step + 1 < s_end) issue(step + 1, page_next, false);
-      const int page_then = step + 2 < s_end ? page_of(step + 2) : -1;
-      if (threadIdx.x == 0) flags[par ^ 1] = flags[4 + (par ^ 1)] = 0;
-      scores(step, there, plain_step(step, there));
-      first_part(flags + par);
-      bar();  // P is here
-      if (flags[par]) move_refs(true);
-      second_part(step);
-      page = page_next;
-      page_next = page_then;
-    }
-  } else {
-    // Two groups half a step apart: while one takes a step's first part
-    // (scores and weights), the other takes the second part of the step before
-    // and brings the next step's copies, since the first part is the longer
-    // way: K in even halves (the second group), V in odd ones (the first).  In
-    // half t, group t & 1 takes the first part of step t / 2, the other the
-    // second part of step (t - 1) / 2.
-    const int n = s_end - step, begin = step;
-    uint32_t there = 0, there_before = 0;
-#pragma unroll 1
-    for (int t = 0; t <= 2 * n; ++t) {
-      const int who = t & 1, s1 = begin + (t >> 1), s2 = begin + ((t - 1) >> 1);
-      const bool lead = who == rg, more = s1 < s_end;
-      if (who == 0) {
-        there_before = there;
-        there = present(s1, page);
-      }
-      if (!lead && more) {
-        wait_vm();
-        if (who == 1 && !plain_step(s1, there)) fix_v(s1, there);
-      }
-      bar();  // K (V) of s1 is here, and the other group's P
-      const int moved = t > 0 ? flags[2 * (who ^ 1) + (s2 & 1)] : 0;
-      if (lead) {
-        if (more) scores(s1, there, plain_step(s1, there));
-        if (moved) move_refs(false);
-        if (more) first_part(flags + 2 * who + (s1 & 1));
-      } else {
-        if (moved) {  // (K of s2 is still there)
-          scores(s2, who ? there : there_before, false);
-          move_refs(true);
-        }
-        if (s1 + 1 < s_end) issue(s1 + 1, page_next, who == 1);
-        if (t > 0) second_part(s2);
-      }
-      if (threadIdx.x == 0) {
-        flags[2 * who + ((s1 & 1) ^ 1)] = 0;
-        if (who == 1) flags[4 + ((s1 & 1) ^ 1)] = 0;
-      }
-      if (who == 1) {
-        page = page_next;
-        if (s1 + 2 < s_end) page_next = page_of(s1 + 2);
-      }
     }
   }
 
-  // ---- the rows' sums over the group's waves, and out ----
+  // the rows' sums over the waves, and out
   bar();
 #pragma unroll
   for (int rt = 0; rt < RT; ++rt) {
     l[rt] += __shfl_xor(l[rt], 16);
     l[rt] += __shfl_xor(l[rt], 32);
-    if (grp == 0) mx[kw * kRows + (rg * RT + rt) * 16 + col] = l[rt];
+    if (grp == 0) mx[wave * kRows + rt * 16 + col] = l[rt];
   }
   bar();
 #pragma unroll
   for (int rt = 0; rt < RT; ++rt) {
     const int r = row0 + rt * 16 + col;
-    const float* lr = mx + (rg * RT + rt) * 16 + col;
+    const float* lr = mx + rt * 16 + col;
     float lt = (lr[0] + lr[kRows]) + (lr[2 * kRows] + lr[3 * kRows]);
-    if (!seen[node_of(rt)]) lt = 0.f;  // an absent node
-    if (r < rows) {
-      const int node = r / a.group, g = r - node * a.group;
-      const long long at = static_cast<long long>(win.off + node) * a.n_heads + h * a.group + g;
-      const int c0 = kw * (D / 4) + 4 * grp;
-      if (a.n_split == 1) {
-        const float inv = lt != 0.f ? 1.f / lt : 0.f;
+    if (!seen[t.node_of(r)]) lt = 0.f;  // an absent node
+    t.template store<DQ, 16>(r, wave * (D / 4) + 4 * grp, acc[rt], mref[rt], lt,
+                             wave == 0 && grp == 0);
+  }
+}
+
+// ---- more rows ---------------------------------------------------------------------
+template <int D, int RT, int NW>
+struct RowsLds {
+  static constexpr uint32_t kSeen = 4 * Part<D>::kStep;
+  static constexpr uint32_t kThere = kSeen + kMaxWindow * 8;
+  static constexpr uint32_t kFlags = kThere + 16;
+  static constexpr uint32_t kBytes = kFlags + 16;
+};
+
+// NW waves of 16 RT rows each.  Four waves bring 16 keys of K and V each,
+// eight 16 keys of K or V.
+template <int D, int RT, int NW>
+__global__ void __launch_bounds__(64 * NW) attn_rows_kernel(const AttnArgs a) {
+  typedef Part<D> P;
+  typedef RowsLds<D, RT, NW> L;
+  constexpr int DT = D / 16;
+  extern __shared__ __attribute__((aligned(16))) unsigned char lds[];
+  const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+  const int blk = wave & 3, kv = NW == 4 ? 3 : 1 + (wave >> 2);
+  P t{a};
+  if (!t.start(lds, 16 * RT * NW)) return;
+  const int lane = t.lane, col = t.col, grp = t.grp;
+  const int row0 = (t.rb * NW + wave) * 16 * RT;
+  int* odds = reinterpret_cast<int*>(lds + L::kFlags);  // 1 + the last odd (even) step with any
+  uint64_t* seen = reinterpret_cast<uint64_t*>(lds + L::kSeen);
+
+  int step = t.begin;
+  int page = t.page_of(step, blk), page_next = 0;
+  if (step < t.end) {
+    t.template issue<true>(step, blk, page, kv);
+    page_next = t.page_of(step + 1, blk);
+  }
+  if (threadIdx.x < 2) odds[threadIdx.x] = 0;
+  if (wave == NW - 1) seen[lane] = ancestors(a.parent, t.win, lane);
+
+  h8 qf[RT][P::KK];
+  f4 acc[RT][DT];
+  float mref[RT], l[RT];
+  bool begun[RT];
 #pragma unroll
-        for (int d = 0; d < DQ; ++d) {
-          h4 y;
+  for (int rt = 0; rt < RT; ++rt) {
+    t.load_q(row0 + rt * 16 + col, qf[rt]);
+    mref[rt] = 0.f;
+    l[rt] = 0.f;
+    begun[rt] = false;
+#pragma unroll
+    for (int d = 0; d < DT; ++d) acc[rt][d] = (f4){0.f, 0.f, 0.f, 0.f};
+  }
+  const uint32_t koff = t.k_offset(), voff = t.v_offset();
+  // which of a step's keys are there, by step parity and block of 16
+  uint16_t* there_of = reinterpret_cast<uint16_t*>(lds + L::kThere);
+
+  bar();  // the flags are cleared
+  for (; step < t.end; ++step) {
+    const int par = step & 1;
+    const uint32_t mine = t.present(step, blk, page);
+    if (wave < 4) there_of[par * 4 + blk] = mine;
+    wait_vm();
+    if (kv != 1 && !t.plain(step, blk, page) && t.fix_v(step, blk, mine)) odds[par] = step + 1;
+    bar();  // everybody's copies of this step are here, and nobody reads the other buffers
+    const uint64_t there = reinterpret_cast<const uint64_t*>(there_of)[par];
+    if (step + 1 < t.end) t.template issue<true>(step + 1, blk, page_next, kv);
+    page = page_next;
+    if (step + 2 < t.end) page_next = t.page_of(step + 2, blk);
+    // (the same in every lane: into scalar registers)
+    const uint32_t there_lo = __builtin_amdgcn_readfirstlane(static_cast<uint32_t>(there));
+    const uint32_t there_hi = __builtin_amdgcn_readfirstlane(static_cast<uint32_t>(there >> 32));
+    const bool plain = (step + 1) * kKeys <= t.len && (there_lo & there_hi) == 0xFFFFFFFFu;
+    const bool odd = !plain && odds[par] == step + 1;
+
+#pragma unroll 1
+    for (int st = 0; st < 2; ++st) {
+      const uint32_t kb = koff + par * 2 * P::kStep + st * 32 * D * 2;
+      f4 s[2][RT];
+#pragma unroll
+      for (int b = 0; b < 2; ++b)
+#pragma unroll
+        for (int rt = 0; rt < RT; ++rt) s[b][rt] = (f4){0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+      for (int ks = 0; ks < P::KK; ++ks) {
+#pragma unroll
+        for (int b = 0; b < 2; ++b) {
+          const h8 kf = t.k_frag(kb + b * 16 * D * 2, ks);
+#pragma unroll
+          for (int rt = 0; rt < RT; ++rt)
+            s[b][rt] = __builtin_amdgcn_mfma_f32_16x16x32_f16(kf, qf[rt][ks], s[b][rt], 0, 0, 0);
+        }
+        if (ks % 2) asm volatile("" ::: "memory");  // (no more reads ahead: registers)
+      }
+      bool move = false;
+      float top[RT];
+#pragma unroll
+      for (int rt = 0; rt < RT; ++rt) {
+#pragma unroll
+        for (int b = 0; b < 2; ++b) {
 #pragma unroll
           for (int i = 0; i < 4; ++i)
-            y[i] = lt != 0.f ? static_cast<_Float16>(acc[rt][d][i] * inv) : static_cast<_Float16>(0);
-          *reinterpret_cast<h4*>(a.out + at * D + c0 + d * 16) = y;
-        }
-      } else {
-        const long long pa = static_cast<long long>(split) * a.n_tokens * a.n_heads + at;
+            s[b][rt][i] = __builtin_fmaf(s[b][rt][i], a.scale_log2, -mref[rt]);
+          if (!plain) {
+            const uint32_t see =
+                t.seen_bits(step, 2 * st + b, (st ? there_hi : there_lo) >> (16 * b) & 0xFFFFu,
+                            seen[t.node_of(row0 + rt * 16 + col)]);
 #pragma unroll
-        for (int d = 0; d < DQ; ++d)
-          *reinterpret_cast<f4*>(a.part_o + pa * D + c0 + d * 16) = acc[rt][d];
-        if (kw == 0 && grp == 0) a.part_ml[pa] = make_float2(mref[rt], lt);
+            for (int i = 0; i < 4; ++i) s[b][rt][i] = see & 1u << i ? s[b][rt][i] : -INFINITY;
+          }
+        }
+        top[rt] = fmaxf(fmaxf(fmaxf(s[0][rt][0], s[0][rt][1]), fmaxf(s[0][rt][2], s[0][rt][3])),
+                        fmaxf(fmaxf(s[1][rt][0], s[1][rt][1]), fmaxf(s[1][rt][2], s[1][rt][3])));
+        move |= top[rt] > kRise || (!begun[rt] && top[rt] > -INFINITY);
+      }
+      if (__any(move)) {
+#pragma unroll
+        for (int rt = 0; rt < RT; ++rt) {
+          float m = fmaxf(top[rt], __shfl_xor(top[rt], 16));
+          m = fmaxf(m, __shfl_xor(m, 32));
+          const bool set = m > kRise || (!begun[rt] && m > -INFINITY);
+          const float by = set ? m - kBelow : 0.f;
+          const float f = !set ? 1.f : begun[rt] ? __builtin_amdgcn_exp2f(-by) : 0.f;
+          mref[rt] += by;
+          l[rt] *= f;
+#pragma unroll
+          for (int d = 0; d < DT; ++d) acc[rt][d] *= f;
+          begun[rt] |= set;
+#pragma unroll
+          for (int b = 0; b < 2; ++b) s[b][rt] -= by;
+        }
+      }
+      h8 pf[RT];
+#pragma unroll
+      for (int rt = 0; rt < RT; ++rt) {
+#pragma unroll
+        for (int b = 0; b < 2; ++b)
+#pragma unroll
+          for (int i = 0; i < 4; ++i) {
+            s[b][rt][i] = __builtin_amdgcn_exp2f(s[b][rt][i]);
+            pf[rt][4 * b + i] = static_cast<_Float16>(s[b][rt][i]);
+          }
+        l[rt] += ((s[0][rt][0] + s[0][rt][1]) + (s[0][rt][2] + s[0][rt][3])) +
+                 ((s[1][rt][0] + s[1][rt][1]) + (s[1][rt][2] + s[1][rt][3]));
+      }
+      if (odd) {
+#pragma unroll 1
+        for (int r = 0; r < 32; ++r) {  // one by one, to the rows that see them
+          const int node = step * kKeys + 32 * st + r - t.len;
+          if (node < 0 || node >= t.win.n) continue;
+          const int from = col + 16 * ((r & 15) >> 2);  // the lane that has key r's weight
+#pragma unroll
+          for (int rt = 0; rt < RT; ++rt) {
+            float mine = 0.f;
+#pragma unroll
+            for (int i = 0; i < 8; ++i)
+              mine = i == (r >> 4) * 4 + (r & 3) ? s[i >> 2][rt][i & 3] : mine;
+            const float w = __shfl(mine, from);
+            const bool see = seen[t.node_of(row0 + rt * 16 + col)] >> node & 1;
+#pragma unroll
+            for (int d = 0; d < DT; ++d)
+#pragma unroll
+              for (int i = 0; i < 4; ++i) {
+                const float v = t.odd_v(node, d * 16 + 4 * grp + i, w);
+                acc[rt][d][i] += see ? v : 0.f;
+              }
+          }
+        }
+      }
+      const uint32_t vl = voff + par * 2 * P::kStep + st * 32 * D * 2;
+#pragma unroll
+      for (int d = 0; d < DT; ++d) {
+        if (d % 4 == 0) asm volatile("" ::: "memory");
+        const h8 vf = t.v_frag(t.v_tile(vl, d), 0);
+#pragma unroll
+        for (int rt = 0; rt < RT; ++rt)
+          acc[rt][d] = __builtin_amdgcn_mfma_f32_16x16x32_f16(vf, pf[rt], acc[rt][d], 0, 0, 0);
       }
     }
+  }
+
+#pragma unroll
+  for (int rt = 0; rt < RT; ++rt) {
+    const int r = row0 + rt * 16 + col;
+    l[rt] += __shfl_xor(l[rt], 16);
+    l[rt] += __shfl_xor(l[rt], 32);
+    const float lt = seen[t.node_of(r)] ? l[rt] : 0.f;  // 0: an absent node
+    t.template store<DT, 16>(r, 4 * grp, acc[rt], mref[rt], lt, grp == 0);
   }
 }
 
@@ -679,19 +865,17 @@ static int check_cache(const sg_kv_cache* c, int n_seq, int n_tokens, int max_wi
 
 // How a call is cut: rows of a workgroup, parts of the caches.
 struct Cut {
-  int rt, rw, row_blocks, n_split, split_keys;
+  int block_rows, row_blocks, n_split, split_keys;
 };
 static Cut attn_cut(int n_seq, int max_window, int max_len, int group, int n_kv, int dim) {
   Cut c;
   const long long rows = static_cast<long long>(max_window) * group;
-  c.rt = rows > 32 ? 4 : rows > 16 ? 2 : 1;
-  c.rw = rows > 64 ? 2 : 1;
-  if (c.rw == 2 && dim == 256) c.rt = 2;
-  c.row_blocks = static_cast<int>((rows + 16 * c.rt * c.rw - 1) / (16 * c.rt * c.rw));
+  c.block_rows = rows > 128 ? 256 : rows > 64 ? 128 : rows > 32 ? 64 : rows > 16 ? 32 : 16;
+  c.row_blocks = static_cast<int>((rows + c.block_rows - 1) / c.block_rows);
   const long long keys = static_cast<long long>(max_len) + max_window;
   const long long most = (keys + kKeys - 1) / kKeys;
   const long long units = static_cast<long long>(n_seq) * n_kv * c.row_blocks;
-  const long long slots = 256 * (dim == 256 || c.rw == 2 ? 1 : 2);
+  const long long slots = 256 * (dim == 256 ? 1 : 2);
   long long n = units >= slots ? 1 : slots / units;
   if (n > most) n = most;
   c.split_keys = static_cast<int>((most + n - 1) / n * kKeys);
@@ -703,22 +887,25 @@ static size_t part_bytes(const Cut& c, int n_tokens, int n_heads, int dim) {
   return static_cast<size_t>(c.n_split) * n_tokens * n_heads * (dim * 4 + 8);
 }
 
-template <int D, int RT, int RW>
-static void attn_go(const AttnArgs& a, long long grid, hipStream_t s) {
-  hipLaunchKernelGGL((attn_tree_kernel<D, RT, RW>), dim3(static_cast<unsigned>(grid)),
-                     dim3(256 * RW), (AttnLds<D, RT, RW>::kBytes), s, a);
+template <int D, int RT>
+static void few_go(const AttnArgs& a, unsigned grid, hipStream_t s) {
+  hipLaunchKernelGGL((attn_few_kernel<D, RT>), dim3(grid), dim3(256), (FewLds<D, RT>::kBytes), s, a);
+}
+template <int D, int RT, int NW>
+static void rows_go(const AttnArgs& a, unsigned grid, hipStream_t s) {
+  hipLaunchKernelGGL((attn_rows_kernel<D, RT, NW>), dim3(grid), dim3(64 * NW),
+                     (RowsLds<D, RT, NW>::kBytes), s, a);
 }
 template <int D>
 static int attn_launch(const AttnArgs& a, const Cut& c, int n_seq, hipStream_t s, const char* nm) {
-  const long long grid = (a.units + 7LL) / 8 * 8 * c.row_blocks;
-  if (c.rw == 2)
-    attn_go<D, D == 256 ? 2 : 4, 2>(a, grid, s);
-  else if (c.rt == 4)
-    attn_go<D, 4, 1>(a, grid, s);
-  else if (c.rt == 2)
-    attn_go<D, 2, 1>(a, grid, s);
-  else
-    attn_go<D, 1, 1>(a, grid, s);
+  const unsigned grid = static_cast<unsigned>((a.units + 7LL) / 8 * 8 * c.row_blocks);
+  switch (c.block_rows) {
+    case 256: rows_go<D, 2, 8>(a, grid, s); break;
+    case 128: rows_go<D, 2, 4>(a, grid, s); break;
+    case 64: few_go<D, 4>(a, grid, s); break;
+    case 32: few_go<D, 2>(a, grid, s); break;
+    default: few_go<D, 1>(a, grid, s); break;
+  }
   if (int st = check_launch(nm)) return st;
   if (c.n_split > 1) {
     hipLaunchKernelGGL(attn_join_kernel<D>, dim3(n_seq * a.max_window * a.n_heads), dim3(256), 0, s,

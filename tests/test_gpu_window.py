@@ -261,10 +261,12 @@ def test_attention_absent_pages_and_lengths_out_of_range():
     check_attn(c)
 
 
-def test_attention_inf_and_nan_in_masked_places():
+@pytest.mark.parametrize("D,group", [(64, 3), (128, 2), (256, 3), (128, 8), (64, 16), (128, 20),
+                                     (256, 16), (256, 40), (64, 50)])
+def test_attention_inf_and_nan_in_masked_places(D, group):
     """What a query does not see does not reach it: the slots behind the cache's end, the siblings in
-    the tree, absent nodes."""
-    c = attn_case(11, [6], [37], 1, 3, 64, 16, branch=2)
+    the tree, absent nodes.  (From 12 to 300 rows a kv head.)"""
+    c = attn_case(11, [6], [37], 1, group, D, 16, branch=2)
     c["parent"][:] = [-1, 0, 0, 1, 2, 77]
     last = c["pages"][0, 2]
     c["kc"][0, last, :, 5:] = np.nan
