@@ -70,11 +70,12 @@ __device__ __forceinline__ int cached_len(int length, int page_log2, int pages_p
   return static_cast<int>(length < 0 ? 0 : length > cap ? cap : length);
 }
 
-// Where chunk c (16 B) of row r lies in its row: rows are a multiple of 128 B
-// apart, so 16 rows read at one chunk would share their banks.
+// Where chunk c (16 B) of row r lies in its row: at c ^ swz(r).  Rows are a
+// multiple of 128 B apart; 16 rows read at one chunk (K) and eight rows read
+// at a pair of chunks (V) then share no bank.
 template <int D>
 __device__ __forceinline__ int swz(int r) {
-  return D == 64 ? (r >> 1) & 7 : r & 15;
+  return D == 64 ? (r & 6) | (r >> 3 & 1) : (r & 7) << 1 | (r >> 3 & 1);
 }
 
 // 16 B per lane from base + voff (bytes) into LDS at lds + 16 * lane.  As
@@ -189,13 +190,15 @@ struct Part {
       // window row and is masked
       const int n_cache = page_ok(page) ? min(len - j, 16) : 0;
       const kernarg_p ca = cold_args();
+      int ln = lane;
+      asm("" : "+v"(ln));
       const uint16_t* const w1 = kv == 2 ? ca->v : ca->k;
       const uint16_t* const w2 = ca->v;
       const long long ws1 = kv == 2 ? ca->v_stride : ca->k_stride, ws2 = ca->v_stride;
 #pragma unroll 1
       for (int i = 0; i < NI; ++i) {
-        const int row = i * RPI + lane / CH;
-        const int c = ((lane % CH) ^ swz<D>(row)) * 8;
+        const int row = i * RPI + ln / CH;
+        const int c = ((ln % CH) ^ swz<D>(row)) * 8;
         const long long w = win.off + min(max(j + row - len, 0), win.n - 1);
         const bool cached = row < n_cache;
         dma16_ptr(buf + i * 1024, (cached ? c1 + at + row * D : w1 + w * ws1 + h * D) + c);
@@ -262,8 +265,10 @@ struct Part {
   __device__ __forceinline__ uint32_t k_offset() const {
     return col * (D * 2) + ((grp ^ swz<D>(col)) << 4);
   }
-  __device__ __forceinline__ h8 k_frag(uint32_t at, int st) const {
-    return *reinterpret_cast<const h8*>(lds + ((at ^ ((st & 3) << 6)) + (st >> 2) * 256));
+  static __device__ __forceinline__ uint32_t k_piece(uint32_t at, int i) { return at ^ (i << 6); }
+  // at: k_piece(.., st % 4)
+  __device__ __forceinline__ h8 k_frag(uint32_t at, int st, int block = 0) const {
+    return *reinterpret_cast<const h8*>(lds + at + (block * 16 * D * 2 + (st >> 2) * 256));
   }
   // V's columns 0..15 of row 4 grp + col / 4 of a 16-key block; tile c of
   // columns is at v_tile(that plus the block's place, c).
@@ -283,12 +288,18 @@ struct Part {
           (lds_s4_p)(static_cast<uintptr_t>(lds0 + at + (st * 2 + b) * 16 * D * 2)));
     return __builtin_bit_cast(h8, __builtin_shufflevector(x[0], x[1], 0, 1, 2, 3, 4, 5, 6, 7));
   }
-  // What weight w adds at window node `node` and column c for fix_v's infinities and NaN.
-  __device__ __forceinline__ float odd_v(int node, int c, float w) const {
+  // Adds what weight w (0: not seen) brings to columns c.. (4) from fix_v's infinities and NaN
+  // of window node `node`.
+  __device__ __forceinline__ void add_odd(f4& o, int node, int c, float w, bool see) const {
     const kernarg_p ca = cold_args();
-    const uint16_t b =
-        ca->v[static_cast<long long>(win.off + node) * ca->v_stride + h * D + c];
-    return fp16_odd(b) ? w * half_bits_to_float(b) : 0.f;
+    const uint64_t b = *reinterpret_cast<const uint64_t*>(
+        ca->v + static_cast<long long>(win.off + node) * ca->v_stride + h * D + c);
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+      const uint32_t x = static_cast<uint32_t>(b >> (16 * i)) & 0xFFFFu;
+      o[i] += see && fp16_odd(x) ? w * half_bits_to_float(x) : 0.f;
+    }
+    asm volatile("" : "+v"(o)::"memory");  // (one after the other: registers)
   }
   // Row r's columns c.. (4), and its sum l about mref.
   template <int N, int kStride>
@@ -373,8 +384,10 @@ __global__ void __launch_bounds__(256) attn_few_kernel(const AttnArgs a) {
 #pragma unroll
     for (int d = 0; d < DQ; ++d) acc[rt][d] = (f4){0.f, 0.f, 0.f, 0.f};
   }
-  const uint32_t koff = t.k_offset() + wave * 16 * D * 2, voff0 = t.v_offset();
-  uint32_t voff[DQ];
+  const uint32_t koff0 = t.k_offset() + wave * 16 * D * 2, voff0 = t.v_offset();
+  uint32_t koff[P::KO], voff[DQ];
+#pragma unroll
+  for (int i = 0; i < P::KO; ++i) koff[i] = P::k_piece(koff0, i);
 #pragma unroll
   for (int d = 0; d < DQ; ++d) voff[d] = t.v_tile(voff0, wave * DQ + d);
   // P: [row][two halves of 32 keys][grp][two blocks of 16 keys][4], 16-B pieces
@@ -401,7 +414,7 @@ __global__ void __launch_bounds__(256) attn_few_kernel(const AttnArgs a) {
     for (int rt = 0; rt < RT; ++rt) s[rt] = (f4){0.f, 0.f, 0.f, 0.f};
 #pragma unroll
     for (int st = 0; st < P::KK; ++st) {
-      const h8 kf = t.k_frag(koff + par * 2 * P::kStep, st);
+      const h8 kf = t.k_frag(koff[st % P::KO] + par * 2 * P::kStep, st);
 #pragma unroll
       for (int rt = 0; rt < RT; ++rt)
         s[rt] = __builtin_amdgcn_mfma_f32_16x16x32_f16(kf, qf[rt][st], s[rt], 0, 0, 0);
@@ -476,11 +489,7 @@ __global__ void __launch_bounds__(256) attn_few_kernel(const AttnArgs a) {
           const bool see = seen[t.node_of(row0 + rt * 16 + col)] >> node & 1;
 #pragma unroll
           for (int d = 0; d < DQ; ++d)
-#pragma unroll
-            for (int i = 0; i < 4; ++i) {
-              const float v = t.odd_v(node, (wave * DQ + d) * 16 + 4 * grp + i, w);
-              acc[rt][d][i] += see ? v : 0.f;
-            }
+            t.add_odd(acc[rt][d], node, (wave * DQ + d) * 16 + 4 * grp, w, see);
         }
       }
     }
@@ -569,7 +578,8 @@ __global__ void __launch_bounds__(64 * NW) attn_rows_kernel(const AttnArgs a) {
 #pragma unroll
     for (int d = 0; d < DT; ++d) acc[rt][d] = (f4){0.f, 0.f, 0.f, 0.f};
   }
-  const uint32_t koff = t.k_offset(), voff = t.v_offset();
+  uint32_t kbase = t.k_offset() + (step & 1) * 2 * P::kStep;  // of the present step's buffer
+  uint32_t vbase = t.v_offset() + (step & 1) * 2 * P::kStep;
   // which of a step's keys are there, by step parity and block of 16
   uint16_t* there_of = reinterpret_cast<uint16_t*>(lds + L::kThere);
 
@@ -593,7 +603,6 @@ __global__ void __launch_bounds__(64 * NW) attn_rows_kernel(const AttnArgs a) {
 
 #pragma unroll 1
     for (int st = 0; st < 2; ++st) {
-      const uint32_t kb = koff + par * 2 * P::kStep + st * 32 * D * 2;
       f4 s[2][RT];
 #pragma unroll
       for (int b = 0; b < 2; ++b)
@@ -603,7 +612,7 @@ __global__ void __launch_bounds__(64 * NW) attn_rows_kernel(const AttnArgs a) {
       for (int ks = 0; ks < P::KK; ++ks) {
 #pragma unroll
         for (int b = 0; b < 2; ++b) {
-          const h8 kf = t.k_frag(kb + b * 16 * D * 2, ks);
+          const h8 kf = t.k_frag(P::k_piece(kbase, ks % P::KO), ks, b);
 #pragma unroll
           for (int rt = 0; rt < RT; ++rt)
             s[b][rt] = __builtin_amdgcn_mfma_f32_16x16x32_f16(kf, qf[rt][ks], s[b][rt], 0, 0, 0);
@@ -676,25 +685,24 @@ __global__ void __launch_bounds__(64 * NW) attn_rows_kernel(const AttnArgs a) {
             const float w = __shfl(mine, from);
             const bool see = seen[t.node_of(row0 + rt * 16 + col)] >> node & 1;
 #pragma unroll
-            for (int d = 0; d < DT; ++d)
-#pragma unroll
-              for (int i = 0; i < 4; ++i) {
-                const float v = t.odd_v(node, d * 16 + 4 * grp + i, w);
-                acc[rt][d][i] += see ? v : 0.f;
-              }
+            for (int d = 0; d < DT; ++d) t.add_odd(acc[rt][d], node, d * 16 + 4 * grp, w, see);
           }
         }
       }
-      const uint32_t vl = voff + par * 2 * P::kStep + st * 32 * D * 2;
 #pragma unroll
       for (int d = 0; d < DT; ++d) {
         if (d % 4 == 0) asm volatile("" ::: "memory");
-        const h8 vf = t.v_frag(t.v_tile(vl, d), 0);
+        const h8 vf = t.v_frag(P::v_tile(vbase, d), 0);
 #pragma unroll
         for (int rt = 0; rt < RT; ++rt)
           acc[rt][d] = __builtin_amdgcn_mfma_f32_16x16x32_f16(vf, pf[rt], acc[rt][d], 0, 0, 0);
       }
+      kbase += 32 * D * 2;
+      vbase += 32 * D * 2;
     }
+    // the other buffer
+    kbase += (par ? -2 : 2) * static_cast<int>(P::kStep) - 64 * D * 2;
+    vbase += (par ? -2 : 2) * static_cast<int>(P::kStep) - 64 * D * 2;
   }
 
 #pragma unroll
