@@ -3,14 +3,15 @@
 //
 // The vocabulary is cut into chunks.  verify_rows_kernel reads every row of
 // logits once and leaves per chunk the largest logit m_c and
-// sum exp((x - m_c) / temperature) (greedy: where m_c lies);
-// verify_walk_kernel, one workgroup a sequence, joins the chunks of each row,
-// goes down the tree and draws the last token: first its chunk, by the
-// chunks' sums, then the token inside it, so that of the last row only one
-// chunk is read again.  With the drafter's distributions, what a rejection
-// leaves, max(R - q, 0), has to be summed over the vocabulary before the next
-// sibling can be tried: verify_rest_kernel does it for all children of one
-// rank of all nodes, as if their earlier siblings had been rejected.
+// sum 2^((x - m_c) log2(e) / temperature) (greedy: where m_c lies), and per
+// node what its tree says of it; verify_walk_kernel, one workgroup a
+// sequence, joins the chunks of each row, goes down the tree and draws the
+// last token: first its chunk, by the chunks' sums, then the token inside it,
+// so that of the last row only one chunk is read again.  With the drafter's
+// distributions, what a rejection leaves, max(R - q, 0), has to be summed over
+// the vocabulary before the next sibling can be tried: verify_rest_kernel does
+// it for all children of one rank of all nodes, as if their earlier siblings
+// had been rejected.
 //
 // Weights and sums are fp64: the last token is found by comparing running
 // sums, and with a vocabulary's worth of borders an fp32 sum would move one
@@ -19,42 +20,50 @@
 
 namespace sg {
 
-constexpr int kChunk = 2048;      // logits of a workgroup of verify_rows_kernel
-constexpr int kWalk = 1024;       // threads of verify_walk_kernel
+constexpr int kChunk = 4096;      // logits of a workgroup of verify_rows_kernel
+constexpr int kWalk = 1024;       // threads of verify_walk_kernel, kChunk / 4
 constexpr int kMaxChildren = 16;
 constexpr double kRest = 0x1p-30; // a smaller share of the mass counts as none
 
 typedef float f32x4_u __attribute__((ext_vector_type(4), aligned(4)));
 
-// e^x for x <= 0, relative error below 1e-12: x = k ln2 + r, |r| <= ln2/2,
-// e^r by its Taylor series to degree 11 (remainder below 7e-15).
-__device__ __forceinline__ double exp_neg(double x) {
-  const double k = __builtin_rint(x * 1.4426950408889634074);
-  double r = __builtin_fma(k, -6.93147180369123816490e-01, x);
-  r = __builtin_fma(k, -1.90821492927058770002e-10, r);
-  double p = 1.0 / 39916800;
-  p = __builtin_fma(p, r, 1.0 / 3628800);
-  p = __builtin_fma(p, r, 1.0 / 362880);
-  p = __builtin_fma(p, r, 1.0 / 40320);
-  p = __builtin_fma(p, r, 1.0 / 5040);
-  p = __builtin_fma(p, r, 1.0 / 720);
-  p = __builtin_fma(p, r, 1.0 / 120);
-  p = __builtin_fma(p, r, 1.0 / 24);
-  p = __builtin_fma(p, r, 1.0 / 6);
-  p = __builtin_fma(p, r, 0.5);
-  p = __builtin_fma(p, r, 1.0);
-  p = __builtin_fma(p, r, 1.0);
-  return x < -700.0 ? 0.0 : __builtin_ldexp(p, static_cast<int>(k));
+// 2^y for y <= 0, relative error below 1e-12: y = k + f, |f| <= 1/2, 2^f by
+// the Taylor series of e^(f ln2) to degree 10 (remainder below 3e-13).  0 from
+// 2^-1075 down, and for NaN.
+__device__ __forceinline__ double exp2_neg(double y) {
+  y = __builtin_fmax(y, -1100.0);
+  const double k = __builtin_rint(y), f = y - k;
+  double p = 7.054911620801123e-09;  // ln2^n / n!, n = 10 .. 1
+  p = __builtin_fma(p, f, 1.01780860092396997e-07);
+  p = __builtin_fma(p, f, 1.32154867901443095e-06);
+  p = __builtin_fma(p, f, 1.52527338040598403e-05);
+  p = __builtin_fma(p, f, 1.54035303933816099e-04);
+  p = __builtin_fma(p, f, 1.33335581464284434e-03);
+  p = __builtin_fma(p, f, 9.61812910762847716e-03);
+  p = __builtin_fma(p, f, 5.55041086648215800e-02);
+  p = __builtin_fma(p, f, 2.40226506959100712e-01);
+  p = __builtin_fma(p, f, 6.93147180559945309e-01);
+  p = __builtin_fma(p, f, 1.0);
+  return __builtin_ldexp(p, static_cast<int>(k));
 }
 
 __device__ __forceinline__ float no_nan(float x) { return x == x ? x : -INFINITY; }
 
 // The weight of logit x under the row's (or chunk's) largest m, which is not
-// -infinity: equal logits get 1 even where both are infinite.
-__device__ __forceinline__ double weight(float x, float m, double inv_t) {
-  const double d = static_cast<double>(x) - static_cast<double>(m);
-  return x == m ? 1.0 : d == -INFINITY ? 0.0 : exp_neg(d * inv_t);  // (0: at any temperature)
+// -infinity; c = log2(e) / temperature.  Equal logits get exactly 1, also
+// where both are infinite; -infinity gets 0 at any temperature.
+__device__ __forceinline__ double weight(float x, float m, double c) {
+  const double w = exp2_neg((static_cast<double>(x) - static_cast<double>(m)) * c);
+  return x == m ? 1.0 : w;
 }
+
+// What the tree says of a node.
+struct Node {
+  int up, rank;        // its parent (-1: the root, or absent), its place among the siblings
+  uint64_t sib, same;  // its earlier siblings; those of them with its token
+  float x, q;          // its token's logit at the parent, and draft probability
+  int tok, pad;        // -1: no token of the vocabulary
+};
 
 struct VerifyArgs {
   const float* logits;
@@ -62,57 +71,103 @@ struct VerifyArgs {
   const float *draft, *temperature, *u_accept, *u_sample;
   int *path, *n_path, *next;
   float* prob;
-  int2* tree;     // [token]: parent node that counts (-1: none), rank among its siblings
-  float* cmax;    // [token][chunk]
+  Node* nodes;    // [token]
   double* csum;   // [token][chunk]: sum of weights; greedy: index of the largest logit
   double* rest;   // [token][chunk]: sum of max(R - q, 0) once the node is rejected
+  float* cmax;    // [token][chunk]
   int n_tokens, max_window, vocab, n_chunks, max_children;
 };
 
-// The windows' trees, with draft distributions without the children past
-// max_children.  One wave; node `lane`.
-__device__ __forceinline__ int2 tree_node(const VerifyArgs& a, Window w, int lane) {
+// Sums over the wave (the same in every lane) and running sums, by DPP; a
+// double goes in two halves.
+template <int CTRL, int ROWS = 0xF>
+__device__ __forceinline__ double dpp_d(double v) {
+  const uint64_t b = __builtin_bit_cast(uint64_t, v);
+  const uint32_t lo = __builtin_amdgcn_update_dpp(0, static_cast<int>(b), CTRL, ROWS, 0xF, false);
+  const uint32_t hi =
+      __builtin_amdgcn_update_dpp(0, static_cast<int>(b >> 32), CTRL, ROWS, 0xF, false);
+  return __builtin_bit_cast(double, static_cast<uint64_t>(hi) << 32 | lo);
+}
+__device__ __forceinline__ double readlane_d(double v, int l) {
+  const uint64_t b = __builtin_bit_cast(uint64_t, v);
+  const uint32_t lo = __builtin_amdgcn_readlane(static_cast<int>(b), l);
+  const uint32_t hi = __builtin_amdgcn_readlane(static_cast<int>(b >> 32), l);
+  return __builtin_bit_cast(double, static_cast<uint64_t>(hi) << 32 | lo);
+}
+__device__ __forceinline__ double wave_run_sum(double v) {  // lane l: of lanes 0..l
+  v += dpp_d<0x111>(v);  // row_shr 1, 2, 4, 8
+  v += dpp_d<0x112>(v);
+  v += dpp_d<0x114>(v);
+  v += dpp_d<0x118>(v);
+  v += dpp_d<0x142, 0xA>(v);  // row_bcast 15 into rows 1 and 3, 31 into 2 and 3
+  v += dpp_d<0x143, 0xC>(v);
+  return v;
+}
+__device__ __forceinline__ double wave_sum(double v) { return readlane_d(wave_run_sum(v), 63); }
+
+// Node `lane` of a window, for the calling wave.
+__device__ __forceinline__ Node tree_node(const VerifyArgs& a, Window w, int lane) {
+  Node n;
+  const bool here = lane < w.n;
+  const int tok = here ? a.tokens[w.off + lane] : -1;
+  n.tok = tok >= 0 && tok < a.vocab ? tok : -1;
   int up = parent_of(a.parent, w, lane);
-  int rank = 0;
+  n.sib = n.same = 0;
   for (int j = 1; j < w.n; ++j) {
-    const int pj = __shfl(up, j);
-    rank += j < lane && pj == up && pj != j && up != lane;
+    const int pj = __builtin_amdgcn_readlane(up, j), tj = __builtin_amdgcn_readlane(n.tok, j);
+    const bool s = j < lane && pj == up && pj != j && up != lane;
+    n.sib |= s ? 1ull << j : 0;
+    n.same |= s && tj == n.tok ? 1ull << j : 0;
   }
-  if (a.draft && rank >= a.max_children) up = lane;
-  const bool in = masks_up(up, w.n, lane) != 0;
-  return make_int2(in && lane > 0 ? up : -1, rank);
+  n.rank = __popcll(n.sib);
+  if (a.draft && n.rank >= a.max_children) up = lane;
+  n.up = masks_up(up, w.n, lane) != 0 && lane > 0 ? up : -1;
+  const bool real = n.up >= 0 && n.tok >= 0;
+  n.x = real ? no_nan(a.logits[static_cast<long long>(w.off + n.up) * a.vocab + n.tok]) : 0.f;
+  n.q = real && a.draft ? a.draft[static_cast<long long>(w.off + lane) * a.vocab + n.tok] : 0.f;
+  n.pad = 0;
+  return n;
 }
 
-// Grid: (chunk, node, sequence).
+// Grid: (chunk, node, sequence); the workgroup past the chunks of node 0
+// does the tree.
 __global__ void __launch_bounds__(256) verify_rows_kernel(const VerifyArgs a) {
   const int s = blockIdx.z, node = blockIdx.y, c = blockIdx.x;
   const Window w = window_of(a.win_off, s, a.n_tokens, a.max_window);
   if (node >= w.n) return;
   const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
+  if (c == a.n_chunks) {
+    if (node == 0 && wave == 0) {
+      const Node n = tree_node(a, w, lane);
+      if (lane < w.n) a.nodes[w.off + lane] = n;
+    }
+    return;
+  }
   const long long row = w.off + node;
   const float* x = a.logits + row * a.vocab;
   const int v0 = c * kChunk + 4 * threadIdx.x;
-  float v[8];
+  constexpr int kLoads = kChunk / 1024;
+  float v[4 * kLoads];
+  if ((c + 1) * kChunk <= a.vocab) {
 #pragma unroll
-  for (int h = 0; h < 2; ++h) {
-    const int at = v0 + h * (kChunk / 2);
-    if (at + 4 <= a.vocab) {
-      const f32x4_u q = *reinterpret_cast<const f32x4_u*>(x + at);
+    for (int h = 0; h < kLoads; ++h) {
+      const f32x4_u q = *reinterpret_cast<const f32x4_u*>(x + v0 + h * 1024);
 #pragma unroll
       for (int i = 0; i < 4; ++i) v[4 * h + i] = no_nan(q[i]);
-    } else {
-#pragma unroll
-      for (int i = 0; i < 4; ++i) v[4 * h + i] = at + i < a.vocab ? no_nan(x[at + i]) : -INFINITY;
     }
+  } else {
+#pragma unroll
+    for (int h = 0; h < kLoads; ++h)
+#pragma unroll
+      for (int i = 0; i < 4; ++i) {
+        const int at = v0 + h * 1024 + i;
+        v[4 * h + i] = at < a.vocab ? no_nan(x[at]) : -INFINITY;
+      }
   }
   const float t = a.temperature[s];
-  if (c == 0 && node == 0 && wave == 3) {
-    const int2 tn = tree_node(a, w, lane);
-    if (lane < w.n) a.tree[w.off + lane] = tn;
-  }
   float m = v[0];
 #pragma unroll
-  for (int i = 1; i < 8; ++i) m = fmaxf(m, v[i]);
+  for (int i = 1; i < 4 * kLoads; ++i) m = fmaxf(m, v[i]);
   m = wave_max_dpp(m);
   __shared__ float sm[4];
   __shared__ double ss[4];
@@ -122,19 +177,22 @@ __global__ void __launch_bounds__(256) verify_rows_kernel(const VerifyArgs a) {
   const bool sampled = t > 0.f;
   double sum = 0.0;
   if (sampled) {
-    const double inv_t = 1.0 / static_cast<double>(t);
-    if (m > -INFINITY)
+    const double k = 1.4426950408889634074 / static_cast<double>(t);
+    if (m == INFINITY) {
 #pragma unroll
-      for (int i = 0; i < 8; ++i) sum += weight(v[i], m, inv_t);
+      for (int i = 0; i < 4 * kLoads; ++i) sum += v[i] == m ? 1.0 : 0.0;
+    } else if (m > -INFINITY) {
 #pragma unroll
-    for (int d = 1; d < 64; d <<= 1) sum += __shfl_xor(sum, d);
+      for (int i = 0; i < 4 * kLoads; ++i)
+        sum += exp2_neg((static_cast<double>(v[i]) - static_cast<double>(m)) * k);
+    }
+    sum = wave_sum(sum);
   } else {  // the lowest index of the largest logit, as a number
-    sum = static_cast<double>(a.vocab);
+    int at = a.vocab;
 #pragma unroll
-    for (int i = 7; i >= 0; --i)
-      if (v[i] == m) sum = fmin(sum, static_cast<double>(v0 + (i >> 2) * (kChunk / 2) + (i & 3)));
-#pragma unroll
-    for (int d = 1; d < 64; d <<= 1) sum = fmin(sum, __shfl_xor(sum, d));
+    for (int i = 0; i < 4 * kLoads; ++i)
+      at = v[i] == m ? min(at, v0 + (i >> 2) * 1024 + (i & 3)) : at;
+    sum = static_cast<double>(-wave_max_i32(-at));
   }
   if (lane == 0) ss[wave] = sum;
   __syncthreads();
@@ -151,29 +209,44 @@ struct RowStat {
   float m;
   double s;
 };
-__device__ __forceinline__ RowStat row_stat(const VerifyArgs& a, long long row, bool sampled,
-                                            double inv_t, int lane) {
+// The first 128 chunks (half a million tokens), so that several rows' loads can be under way.
+struct RowHead {
+  float m[2];
+  double s[2];
+};
+__device__ __forceinline__ RowHead row_head(const VerifyArgs& a, long long row, int lane) {
+  RowHead h;
+#pragma unroll
+  for (int i = 0; i < 2; ++i) {
+    const int c = lane + 64 * i;
+    h.m[i] = c < a.n_chunks ? a.cmax[row * a.n_chunks + c] : -INFINITY;
+    h.s[i] = c < a.n_chunks ? a.csum[row * a.n_chunks + c] : 0.0;
+  }
+  return h;
+}
+__device__ __forceinline__ RowStat row_stat(const VerifyArgs& a, long long row, const RowHead& h,
+                                            bool sampled, double k, int lane) {
   const float* cm = a.cmax + row * a.n_chunks;
   const double* cs = a.csum + row * a.n_chunks;
-  float m = -INFINITY;
-  for (int c = lane; c < a.n_chunks; c += 64) m = fmaxf(m, cm[c]);
-  m = wave_max_dpp(m);
   RowStat r;
-  r.m = m;
+  float m = fmaxf(h.m[0], h.m[1]);
+  for (int c = lane + 128; c < a.n_chunks; c += 64) m = fmaxf(m, cm[c]);
+  r.m = m = wave_max_dpp(m);
   if (sampled) {
     double s = 0.0;
-    for (int c = lane; c < a.n_chunks; c += 64)
-      if (cm[c] > -INFINITY) s += cs[c] * weight(cm[c], m, inv_t);
 #pragma unroll
-    for (int d = 1; d < 64; d <<= 1) s += __shfl_xor(s, d);
-    r.s = s;
+    for (int i = 0; i < 2; ++i) s += h.m[i] > -INFINITY ? h.s[i] * weight(h.m[i], m, k) : 0.0;
+    for (int c = lane + 128; c < a.n_chunks; c += 64)
+      if (cm[c] > -INFINITY) s += cs[c] * weight(cm[c], m, k);
+    r.s = wave_sum(s);
   } else {
-    double s = 1e18;
-    for (int c = lane; c < a.n_chunks; c += 64)
-      if (cm[c] == m) s = fmin(s, cs[c]);
+    int at = 0x7FFFFFFF;
 #pragma unroll
-    for (int d = 1; d < 64; d <<= 1) s = fmin(s, __shfl_xor(s, d));
-    r.s = m > -INFINITY ? s : -1.0;
+    for (int i = 1; i >= 0; --i) at = h.m[i] == m && h.s[i] < at ? static_cast<int>(h.s[i]) : at;
+    for (int c = lane + 128; c < a.n_chunks; c += 64)
+      if (cm[c] == m && cs[c] < at) at = static_cast<int>(cs[c]);
+    at = -wave_max_i32(-at);
+    r.s = m > -INFINITY ? static_cast<double>(at) : -1.0;
   }
   return r;
 }
@@ -181,14 +254,12 @@ __device__ __forceinline__ RowStat row_stat(const VerifyArgs& a, long long row, 
 __device__ __forceinline__ double rest_sum(const VerifyArgs& a, long long row, int lane) {
   double s = 0.0;
   for (int c = lane; c < a.n_chunks; c += 64) s += a.rest[row * a.n_chunks + c];
-#pragma unroll
-  for (int d = 1; d < 64; d <<= 1) s += __shfl_xor(s, d);
-  return s;
+  return wave_sum(s);
 }
-// The target's probability of token v in a row.
-__device__ __forceinline__ double target_p(RowStat r, float x, int v, bool sampled, double inv_t) {
+// The target's probability of token v (logit x) in a row.
+__device__ __forceinline__ double target_p(RowStat r, float x, int v, bool sampled, double k) {
   if (!sampled) return static_cast<double>(v) == r.s ? 1.0 : 0.0;
-  return r.s > 0.0 && r.m > -INFINITY ? weight(no_nan(x), r.m, inv_t) / r.s : 0.0;
+  return r.m > -INFINITY ? weight(no_nan(x), r.m, k) / r.s : 0.0;
 }
 
 // The siblings of rank 0 .. n-1 below a node: rows and the sums of their rests.
@@ -215,91 +286,103 @@ __global__ void __launch_bounds__(256) verify_rest_kernel(const VerifyArgs a, in
   const int s = blockIdx.z, node = blockIdx.y, c = blockIdx.x;
   const Window w = window_of(a.win_off, s, a.n_tokens, a.max_window);
   if (node >= w.n) return;
-  const int2 me = a.tree[w.off + node];
-  if (me.x < 0 || me.y != rank) return;
+  const Node me = a.nodes[w.off + node];
+  if (me.up < 0 || me.rank != rank) return;
   const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
+  const float* x = a.logits + static_cast<long long>(w.off + me.up) * a.vocab;
+  const float* q = a.draft + static_cast<long long>(w.off + node) * a.vocab;
+  constexpr int kEach = kChunk / 256;
+  float xv[kEach], qv[kEach];
+#pragma unroll
+  for (int i = 0; i < kEach; ++i) {
+    const int v = c * kChunk + i * 256 + threadIdx.x;
+    xv[i] = v < a.vocab ? x[v] : -INFINITY;
+    qv[i] = v < a.vocab ? q[v] : 0.f;
+  }
   const float t = a.temperature[s];
   const bool sampled = t > 0.f;
-  const double inv_t = sampled ? 1.0 / static_cast<double>(t) : 1.0;
+  const double k = sampled ? 1.4426950408889634074 / static_cast<double>(t) : 1.0;
   __shared__ Chain ch;
   __shared__ RowStat rs;
   __shared__ double ss[4];
   if (wave == 0) {
-    const RowStat r = row_stat(a, w.off + me.x, sampled, inv_t, lane);
+    const RowStat r =
+        row_stat(a, w.off + me.up, row_head(a, w.off + me.up, lane), sampled, k, lane);
     if (lane == 0) rs = r;
-  } else if (wave == 1) {
-    const int2 other = lane < w.n ? a.tree[w.off + lane] : make_int2(-1, 0);
-    if (other.x == me.x && other.y < rank) ch.row[other.y] = w.off + lane;
+  }
+  if (rank > 0) {
+    uint64_t b = me.sib;
+    for (int i = 0; i < rank; ++i, b &= b - 1)
+      if ((i & 3) == 3 - wave) {  // (the last wave first: wave 0 has the row)
+        const int row = w.off + __builtin_ctzll(b);
+        const double r = rest_sum(a, row, lane);
+        if (lane == 0) {
+          ch.row[i] = row;
+          ch.sum[i] = r;
+        }
+      }
   }
   __syncthreads();
-  for (int i = wave; i < rank; i += 4) {
-    const double r = rest_sum(a, ch.row[i], lane);
-    if (lane == 0) ch.sum[i] = r;
-  }
-  __syncthreads();
-  const float* x = a.logits + static_cast<long long>(w.off + me.x) * a.vocab;
-  const float* q = a.draft + static_cast<long long>(w.off + node) * a.vocab;
   double sum = 0.0;
-#pragma unroll
-  for (int i = 0; i < kChunk / 256; ++i) {
+#pragma unroll 4
+  for (int i = 0; i < kEach; ++i) {
     const int v = c * kChunk + i * 256 + threadIdx.x;
     if (v < a.vocab)
-      sum += fmax(chain_rest(a, ch, rank, target_p(rs, x[v], v, sampled, inv_t), v) -
-                      static_cast<double>(q[v]), 0.0);
+      sum += fmax(chain_rest(a, ch, rank, target_p(rs, xv[i], v, sampled, k), v) -
+                      static_cast<double>(qv[i]), 0.0);
   }
-#pragma unroll
-  for (int d = 1; d < 64; d <<= 1) sum += __shfl_xor(sum, d);
+  sum = wave_sum(sum);
   if (lane == 0) ss[wave] = sum;
   __syncthreads();
   if (threadIdx.x == 0)
     a.rest[static_cast<long long>(w.off + node) * a.n_chunks + c] = (ss[0] + ss[1]) + (ss[2] + ss[3]);
 }
 
-// The first i of the workgroup's values at which their running sum (from
-// `before` on) passes goal and the value is positive; *total: their sum.
-// Values 0..kWalk-1 by thread; -1 if there is none.  *last: the last positive one.
+// The first thread at which the running sum of v over the workgroup's threads,
+// from `before` on, passes goal and v is positive.
 struct Found {
-  int at, last;
-  double before, total;  // the sum in front of `at`, the sum of all
+  int at, last;          // that thread, the last with a positive v; -1: none
+  double before, after;  // the sum in front of thread `at`, the sum behind the last thread
 };
 __device__ __forceinline__ Found find_in(double v, double before, double goal, double* ws, int* wi) {
   const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
-  double run = v;
-#pragma unroll
-  for (int d = 1; d < 64; d <<= 1) {
-    const double o = __shfl_up(run, d);
-    if (lane >= d) run += o;
-  }
-  __syncthreads();
+  const double run = wave_run_sum(v);
+  __syncthreads();  // (ws and wi may still be read)
   if (lane == 63) ws[wave] = run;
-  if (threadIdx.x < 2) wi[threadIdx.x] = threadIdx.x ? -1 : kWalk;
   __syncthreads();
-  double base = before, all = 0.0;
+  double base = before, all = before;
 #pragma unroll
   for (int i = 0; i < kWalk / 64; ++i) {
-    if (i == wave) base = before + all;
+    if (i == wave) base = all;
     all += ws[i];
   }
-  if (v > 0.0) {
-    if (base + run > goal) atomicMin(&wi[0], static_cast<int>(threadIdx.x));
-    atomicMax(&wi[1], static_cast<int>(threadIdx.x));
+  const uint64_t hit = __ballot(v > 0.0 && base + run > goal), some = __ballot(v > 0.0);
+  if (lane == 0) {
+    wi[wave] = hit ? wave * 64 + __builtin_ctzll(hit) : kWalk;
+    wi[kWalk / 64 + wave] = some ? wave * 64 + 63 - __builtin_clzll(some) : -1;
   }
   __syncthreads();
   Found f;
-  f.at = wi[0] < kWalk ? wi[0] : -1;
-  f.last = wi[1];
-  f.total = all;
-  f.before = 0.0;
-  if (f.at == static_cast<int>(threadIdx.x)) ws[kWalk / 64] = base + run - v;
+  f.at = kWalk;
+  f.last = -1;
+#pragma unroll
+  for (int i = 0; i < kWalk / 64; ++i) {
+    f.at = min(f.at, wi[i]);
+    f.last = max(f.last, wi[kWalk / 64 + i]);
+  }
+  if (static_cast<int>(threadIdx.x) == f.at) ws[kWalk / 64] = base + run - v;
   __syncthreads();
-  if (f.at >= 0) f.before = ws[kWalk / 64];
+  f.before = ws[kWalk / 64];
+  f.at = f.at < kWalk ? f.at : -1;
+  f.after = all;
   return f;
 }
 
 // One workgroup a sequence.
 __global__ void __launch_bounds__(kWalk) verify_walk_kernel(const VerifyArgs a) {
   const int s = blockIdx.x;
-  const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
+  const int lane = threadIdx.x & 63;
+  const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
   const Window w = window_of(a.win_off, s, a.n_tokens, a.max_window);
   int* path = a.path + static_cast<long long>(s) * a.max_window;
   if (w.n == 0) {
@@ -311,94 +394,97 @@ __global__ void __launch_bounds__(kWalk) verify_walk_kernel(const VerifyArgs a) 
     return;
   }
   __shared__ RowStat stat[kMaxWindow];
-  __shared__ double left[kMaxWindow];   // a rejected node's rest
-  __shared__ int kids[kMaxWindow][2];   // the end's rejected children: row, token
+  __shared__ double left[kMaxWindow];   // a rejected node's rest; a point mass: 1 if its share is taken
+  __shared__ double mass[kMaxWindow];   // of R at a node, point masses
+  __shared__ int kid_tok[kMaxWindow];   // the end's children whose share is taken
   __shared__ int s_end, s_kids;
-  __shared__ double ws[kWalk / 64 + 1];
-  __shared__ int wi[2];
+  __shared__ double s_total, ws[kWalk / 64 + 1];
+  __shared__ int wi[2 * kWalk / 64];
   __shared__ Chain chain;
   const float t = a.temperature[s];
+  const float us = a.u_sample[s];
   const bool sampled = t > 0.f;
-  const double inv_t = sampled ? 1.0 / static_cast<double>(t) : 1.0;
-  const int2 tn = lane < w.n ? a.tree[w.off + lane] : make_int2(-1, 0);
-  for (int i = wave; i < w.n; i += kWalk / 64) {
-    const RowStat r = row_stat(a, w.off + i, sampled, inv_t, lane);
-    double rest = 0.0;
-    if (a.draft && __shfl(tn.x, i) >= 0) rest = rest_sum(a, w.off + i, lane);
-    if (lane == 0) {
-      stat[i] = r;
-      left[i] = rest;
+  const double k = sampled ? 1.4426950408889634074 / static_cast<double>(t) : 1.0;
+  Node n;
+  n.up = -1;
+  n.rank = 0;
+  n.sib = n.same = 0;
+  n.x = n.q = 0.f;
+  n.tok = -1;
+  float u = 1.f;
+  if (wave == 0 && lane < w.n) {
+    n = a.nodes[w.off + lane];
+    u = a.u_accept[w.off + lane];
+  }
+  constexpr int kRounds = kMaxWindow / (kWalk / 64);
+  RowHead head[kRounds];
+#pragma unroll
+  for (int j = 0; j < kRounds; ++j)
+    head[j] = row_head(a, w.off + min(wave + j * (kWalk / 64), w.n - 1), lane);
+#pragma unroll
+  for (int j = 0; j < kRounds; ++j) {
+    const int i = wave + j * (kWalk / 64);
+    if (i < w.n) {
+      const RowStat r = row_stat(a, w.off + i, head[j], sampled, k, lane);
+      if (lane == 0) {
+        stat[i] = r;
+        mass[i] = r.m > -INFINITY ? 1.0 : 0.0;
+      }
     }
   }
+  if (a.draft)
+    for (int i = wave; i < w.n; i += kWalk / 64) {
+      const double rest = a.nodes[w.off + i].up >= 0 ? rest_sum(a, w.off + i, lane) : 0.0;
+      if (lane == 0) left[i] = rest;
+    }
   __syncthreads();
   if (wave == 0) {
-    // Node `lane`: its token's share of R at its parent, as far as the node
-    // alone tells.
-    const bool in = tn.x >= 0;
-    const int up = in ? tn.x : 0;
-    const int tok = lane < w.n ? a.tokens[w.off + lane] : -1;
-    const bool real = in && tok >= 0 && tok < a.vocab;
-    double r = 0.0, q = 1.0;
-    if (real)
-      r = target_p(stat[up], a.logits[static_cast<long long>(w.off + up) * a.vocab + tok], tok,
-                   sampled, inv_t);
-    const float u = in ? a.u_accept[w.off + lane] : 1.f;
-    const double full = stat[up].m > -INFINITY ? 1.0 : 0.0;
-    uint64_t same = 0, sib = 0;  // earlier siblings with this token, earlier siblings
-    for (int j = 1; j < w.n; ++j) {
-      const int pj = __shfl(tn.x, j), tj = __shfl(tok, j);
-      if (j < lane && in && pj == up && pj >= 0) {
-        sib |= 1ull << j;
-        if (tj == tok) same |= 1ull << j;
-      }
-    }
-    double mass = full;  // sum of R
+    const bool in = n.up >= 0;
+    const int up = in ? n.up : 0;
+    // R of the node's token at its parent, R's mass there, the bar u has to stay under
+    double r = in && n.tok >= 0 ? target_p(stat[up], n.x, n.tok, sampled, k) : 0.0;
+    double m = mass[up], q = 1.0;
     if (a.draft) {
-      q = real ? a.draft[static_cast<long long>(w.off + lane) * a.vocab + tok] : 0.0;
-      double norm = full;
-      for (uint64_t b = sib; b; b &= b - 1) {
+      q = n.q;
+      for (uint64_t b = n.sib; b; b &= b - 1) {
         const int j = __builtin_ctzll(b);
         if (left[j] < kRest) continue;
-        const double qj =
-            real ? a.draft[static_cast<long long>(w.off + j) * a.vocab + tok] : 0.0;
-        r = fmax((norm > 0.0 ? r / norm : 0.0) - qj, 0.0);
-        norm = left[j];
+        const double qj = in && n.tok >= 0
+                              ? a.draft[static_cast<long long>(w.off + j) * a.vocab + n.tok] : 0.0;
+        r = fmax((m > 0.0 ? r / m : 0.0) - qj, 0.0);
+        m = left[j];
       }
-      mass = norm;
     } else {
-      // A point mass: a rejected sibling takes its token's share away.  Node
-      // by node, since each depends on what its earlier siblings left.
-      double m = lane < w.n && stat[lane < w.n ? lane : 0].m > -INFINITY ? 1.0 : 0.0;
-      uint64_t gone = 0;  // rejected nodes whose share is taken
-      for (int j = 1; j < w.n; ++j) {
-        const int p = __shfl(tn.x, j);
-        if (p < 0) continue;
-        const uint64_t sm = __shfl(same, j);
-        const double rj = sm & gone ? 0.0 : __shfl(r, j);
-        const double mp = __shfl(m, p);
-        if (lane == j) {
-          r = rj;
-          mass = mp;
+      // A point mass: a rejected sibling takes its token's share away.  All
+      // children of one rank at once.
+      uint64_t gone = 0;  // the nodes whose share is taken
+      for (int j = 0; __any(in && n.rank >= j); ++j) {
+        const bool now = in && n.rank == j;
+        bool take = false;
+        if (now) {
+          if (n.same & gone) r = 0.0;
+          m = mass[up];
+          take = m - r >= kRest * m;
+          if (take) mass[up] = m - r;
         }
-        if (mp - rj >= kRest * mp) {
-          if (lane == p) m = mp - rj;
-          gone |= 1ull << j;
-        }
+        gone |= __ballot(take);
+        wait_lds();
+        asm volatile("" ::: "memory");  // (mass is other lanes' next)
       }
       if (lane < w.n) left[lane] = gone >> lane & 1 ? 1.0 : 0.0;
     }
-    const double bar = q * mass;
-    const bool take = in && static_cast<double>(u) * bar < r;
+    const double bar = q * m;
+    const bool ok = in && static_cast<double>(u) * bar < r;
     if (a.prob && lane < w.n)
       a.prob[w.off + lane] =
           lane == 0 ? 1.f : !in ? 0.f : r >= bar ? (r > 0.0 ? 1.f : 0.f)
                                                  : static_cast<float>(r / bar);
     // down the tree: the first accepted child of each node
-    const uint64_t yes = __ballot(take);
-    int at = 0, n = 0, mine = -1;
+    const uint64_t yes = __ballot(ok);
+    int at = 0, np = 0, mine = -1;
     while (true) {
-      if (lane == n) mine = at;
-      ++n;
+      if (lane == np) mine = at;
+      ++np;
       const uint64_t kid = __ballot(in && up == at) & yes;
       if (!kid) break;
       at = __builtin_ctzll(kid);
@@ -406,18 +492,17 @@ __global__ void __launch_bounds__(kWalk) verify_walk_kernel(const VerifyArgs a) 
     if (lane < a.max_window) path[lane] = mine;
     const uint64_t kid = __ballot(in && up == at);
     if (in && up == at) {
-      const int k = __popcll(kid & ((1ull << lane) - 1));
-      kids[k][0] = w.off + lane;
-      kids[k][1] = left[lane] > 0.0 ? tok : -1;
+      kid_tok[n.rank] = left[lane] > 0.0 ? n.tok : -1;
       if (a.draft) {
-        chain.row[k] = w.off + lane;
-        chain.sum[k] = left[lane];
+        chain.row[n.rank] = w.off + lane;
+        chain.sum[n.rank] = left[lane];
       }
     }
     if (lane == 0) {
       s_end = at;
       s_kids = __popcll(kid);
-      a.n_path[s] = n;
+      s_total = mass[at];
+      a.n_path[s] = np;
     }
   }
   __syncthreads();
@@ -425,98 +510,108 @@ __global__ void __launch_bounds__(kWalk) verify_walk_kernel(const VerifyArgs a) 
   // The last token: R at the end of the path, in units of the row's weights.
   const int end = s_end, nk = s_kids;
   const RowStat st = stat[end];
-  if (st.m == -INFINITY) {
-    if (threadIdx.x == 0) a.next[s] = -1;
+  if (!sampled || st.m == -INFINITY) {  // all the mass is on one token, rejections or not; or none
+    if (threadIdx.x == 0) a.next[s] = st.m > -INFINITY ? static_cast<int>(st.s) : -1;
     return;
   }
   const long long row = w.off + end;
   const float* x = a.logits + row * a.vocab;
+  double total = st.s * s_total;
   int from = -1;  // the rejected child whose rest is what is left
   if (a.draft)
     for (int i = 0; i < nk; ++i)
-      if (chain.sum[i] >= kRest) from = chain.row[i];
-  if (!sampled) {  // all the mass is on one token, whether or not a rejection left some of it
-    if (threadIdx.x == 0) a.next[s] = static_cast<int>(st.s);
-    return;
-  }
-  // the sum of a chunk
-  auto chunk = [&](int c) {
-    if (c >= a.n_chunks) return 0.0;
-    if (from >= 0) return a.rest[static_cast<long long>(from) * a.n_chunks + c];
-    const float cm = a.cmax[row * a.n_chunks + c];
-    if (!(cm > -INFINITY)) return 0.0;
-    double v = a.csum[row * a.n_chunks + c] * weight(cm, st.m, inv_t);
-    if (!a.draft)
-      for (int i = 0; i < nk; ++i) {
-        const int tok = kids[i][1];
-        bool again = false;
-        for (int j = 0; j < i; ++j) again |= kids[j][1] == tok;
-        if (tok >= 0 && tok < a.vocab && tok / kChunk == c && !again)
-          v -= weight(no_nan(x[tok]), st.m, inv_t);
+      if (chain.sum[i] >= kRest) {
+        from = chain.row[i];
+        total = chain.sum[i];
       }
-    return fmax(v, 0.0);
-  };
-  double total = 0.0;
-  for (int c0 = 0; c0 < a.n_chunks; c0 += kWalk) {
-    const Found f = find_in(chunk(c0 + threadIdx.x), 0.0, 0.0, ws, wi);
-    total += f.total;
-  }
-  const double goal = static_cast<double>(a.u_sample[s]) * total;
+  const double goal = static_cast<double>(us) * total;
+  // its chunk
   int c_at = -1, c_last = 0;
   double before = 0.0, run = 0.0;
   for (int c0 = 0; c0 < a.n_chunks && c_at < 0; c0 += kWalk) {
-    const Found f = find_in(chunk(c0 + threadIdx.x), run, goal, ws, wi);
+    const int c = c0 + threadIdx.x;
+    double v = 0.0;
+    if (c < a.n_chunks) {
+      if (from >= 0) {
+        v = a.rest[static_cast<long long>(from) * a.n_chunks + c];
+      } else {
+        const float cm = a.cmax[row * a.n_chunks + c];
+        const double cs = a.csum[row * a.n_chunks + c];
+        if (cm > -INFINITY) v = cs * weight(cm, st.m, k);
+        if (!a.draft)
+          for (int i = 0; i < nk; ++i) {
+            const int tok = kid_tok[i];
+            if (tok < 0 || tok / kChunk != c) continue;
+            bool again = false;
+            for (int j = 0; j < i; ++j) again |= kid_tok[j] == tok;
+            if (!again) v = fmax(v - weight(no_nan(x[tok]), st.m, k), 0.0);
+          }
+      }
+    }
+    const Found f = find_in(v, run, goal, ws, wi);
     if (f.at >= 0) {
       c_at = c0 + f.at;
       before = f.before;
     }
     if (f.last >= 0) c_last = c0 + f.last;
-    run += f.total;
+    run = f.after;
   }
   const bool past = c_at < 0;  // u_sample is 1 or more, or the sums round so
   if (past) c_at = c_last;
-  int tok = -1, last = 0;
-  run = before;
-  for (int v0 = 0; v0 < kChunk && tok < 0; v0 += kWalk) {
-    const int v = c_at * kChunk + v0 + threadIdx.x;
-    double r = 0.0;
-    if (v < a.vocab) {
-      if (a.draft) {
-        r = chain_rest(a, chain, nk, target_p(st, x[v], v, sampled, inv_t), v);
-        // (chunk sums are of the unnormalized rest, or of the row's weights)
-        if (from >= 0) {
-          double last_sum = 1.0;
-          for (int i = 0; i < nk; ++i)
-            if (chain.sum[i] >= kRest) last_sum = chain.sum[i];
-          r *= last_sum;
-        } else {
-          r *= st.s;
-        }
+  // the token in it: four consecutive ones a thread
+  const int v0 = c_at * kChunk + 4 * threadIdx.x;
+  double r[4], sum = 0.0;
+  if (v0 < a.vocab) {
+    float xv[4];
+#pragma unroll
+    for (int i = 0; i < 4; ++i) xv[i] = v0 + i < a.vocab ? no_nan(x[v0 + i]) : -INFINITY;
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+      const int v = v0 + i;
+      if (a.draft && from >= 0) {  // (the rest as it was summed: not normalized)
+        r[i] = v < a.vocab ? chain_rest(a, chain, nk, target_p(st, xv[i], v, true, k), v) * total
+                           : 0.0;
       } else {
-        r = weight(no_nan(x[v]), st.m, inv_t);
-        for (int i = 0; i < nk; ++i)
-          if (kids[i][1] == v) r = 0.0;
+        r[i] = weight(xv[i], st.m, k);
+        if (!a.draft)
+          for (int j = 0; j < nk; ++j)
+            if (kid_tok[j] == v) r[i] = 0.0;
       }
+      sum += r[i];
     }
-    const Found f = find_in(r, run, past ? INFINITY : goal, ws, wi);
-    if (f.at >= 0) tok = c_at * kChunk + v0 + f.at;
-    if (f.last >= 0) last = c_at * kChunk + v0 + f.last;
-    run += f.total;
+  } else {
+#pragma unroll
+    for (int i = 0; i < 4; ++i) r[i] = 0.0;
   }
-  if (threadIdx.x == 0) a.next[s] = tok >= 0 ? tok : last;
+  const Found f = find_in(sum, before, past ? INFINITY : goal, ws, wi);
+  const int who = f.at >= 0 ? f.at : f.last;
+  if (static_cast<int>(threadIdx.x) == who) {
+    // the first that passes the goal; the last positive one where none does (the sums round so)
+    int tok = -1;
+    bool done = false;
+    double b = f.before;
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+      b += r[i];
+      if (r[i] > 0.0 && !done) tok = v0 + i;
+      done |= r[i] > 0.0 && f.at >= 0 && b > goal;
+    }
+    a.next[s] = tok;
+  }
+  if (who < 0 && threadIdx.x == 0) a.next[s] = -1;  // (a chunk's sum is positive: not reached)
 }
 
 static size_t up16(size_t n) { return (n + 15) / 16 * 16; }
 struct VerifyWs {
-  size_t tree, cmax, csum, rest, bytes;
+  size_t nodes, csum, cmax, rest, bytes;
 };
 static VerifyWs verify_ws(int n_tokens, int vocab, int max_children) {
   const size_t t = n_tokens, c = (vocab + kChunk - 1) / kChunk;
   VerifyWs w;
-  w.tree = 0;
-  w.cmax = w.tree + up16(t * sizeof(int2));
-  w.csum = w.cmax + up16(t * c * sizeof(float));
-  w.rest = w.csum + up16(t * c * sizeof(double));
+  w.nodes = 0;
+  w.csum = w.nodes + up16(t * sizeof(Node));
+  w.cmax = w.csum + up16(t * c * sizeof(double));
+  w.rest = w.cmax + up16(t * c * sizeof(float));
   w.bytes = w.rest + (max_children > 0 ? up16(t * c * sizeof(double)) : 0);
   return w;
 }
@@ -569,7 +664,7 @@ int sg_tree_verify(const float* logits, const int* tokens, const int* win_off, c
   a.next = next;
   a.prob = prob;
   unsigned char* b = static_cast<unsigned char*>(ws);
-  a.tree = reinterpret_cast<int2*>(b + l.tree);
+  a.nodes = reinterpret_cast<Node*>(b + l.nodes);
   a.cmax = reinterpret_cast<float*>(b + l.cmax);
   a.csum = reinterpret_cast<double*>(b + l.csum);
   a.rest = reinterpret_cast<double*>(b + l.rest);
@@ -580,7 +675,7 @@ int sg_tree_verify(const float* logits, const int* tokens, const int* win_off, c
   a.max_children = max_children;
   const hipStream_t s = static_cast<hipStream_t>(stream);
   const dim3 grid(a.n_chunks, max_window, n_seq);
-  hipLaunchKernelGGL(verify_rows_kernel, grid, dim3(256), 0, s, a);
+  hipLaunchKernelGGL(verify_rows_kernel, dim3(a.n_chunks + 1, max_window, n_seq), dim3(256), 0, s, a);
   if (int st = check_launch(nm)) return st;
   if (draft_probs)
     for (int r = 0; r < max_children && r < max_window - 1; ++r) {
