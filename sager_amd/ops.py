@@ -557,68 +557,79 @@ class MoePrefill(MoeLayer):
 # (win_off int32 [n_seq + 1]); parent (int32, one per row, or None for chains)
 # makes a window a tree of drafts.  include/sager_hip.h has the rules.
 
+def _arg(fn, name, t, dtype, shape):
+    """The address of a contiguous GPU tensor of that type and shape."""
+    if t.dtype is not dtype or t.shape != shape or not t.is_cuda or not t.is_contiguous():
+        raise SagerError(f"{fn}: {name} must be {dtype} {tuple(shape)}, contiguous on the GPU, got "
+                         f"{t.dtype} {tuple(t.shape)} on {t.device}")
+    return t.data_ptr()
+
+
+def _current_stream_of(fn, t):
+    """The current stream, of the current device, which has to be t's: the launch goes there."""
+    dev = t.get_device()
+    if dev < 0 or dev != torch._C._cuda_getDevice():
+        raise SagerError(f"{fn}: {t.device} is not the current GPU")
+    return torch._C._cuda_getCurrentRawStream(dev)
+
+
 def add_rmsnorm_q8_k(x, w, eps, y=None, x_out=None, xn=None, xq=None):
     """r = x + y (y may be None), xn = RMS norm of r times w, xq = Q8_K(xn), in
-    one launch (sg_add_rmsnorm_q8_k / _f16): x, y fp16 or fp32 [rows, n], w
+    one launch (sg_add_rmsnorm_q8_k / _f16): x, y fp16 or fp32 [..., n], w
     fp32 [n].  Returns (r, xn, xq).  x_out may be x (in place).  With neither
     xn nor xq given both are made; with one given, only that one (the other
     is None)."""
-    if x.dtype not in (torch.float16, torch.float32):
+    fn, dt, shape = "add_rmsnorm_q8_k", x.dtype, x.shape
+    if dt is torch.float16:
+        entry = load().sg_add_rmsnorm_q8_k_f16
+    elif dt is torch.float32:
+        entry = load().sg_add_rmsnorm_q8_k
+    else:
         raise SagerError("x must be fp32 or fp16")
-    _current("add_rmsnorm_q8_k", x)
-    n = x.shape[-1]
+    stream = _current_stream_of(fn, x)
+    n = shape[-1]
     rows = x.numel() // n if n else 0
-    if w.numel() != n:
-        raise SagerError(f"w must have {n} values")
     if xn is None and xq is None:
         xn, xq = torch.empty_like(x), q8k_empty(rows, n, x.device)
-    if y is None:
-        if x_out is not None:
-            raise SagerError("x_out needs y")
-    elif x_out is None:
-        x_out = torch.empty_like(x)
-    same = {k: v for k, v in (("x", x), ("y", y), ("x_out", x_out), ("xn", xn)) if v is not None}
-    for k, v in same.items():
-        if v.shape != x.shape or v.device != x.device:
-            raise SagerError(f"{k} must have x's shape and device")
-    _dtypes("add_rmsnorm_q8_k", w=(w, torch.float32), **{k: (v, x.dtype) for k, v in same.items()})
+    py = po = pn = pq = None
+    if y is not None:
+        if x_out is None:
+            x_out = torch.empty_like(x)
+        py, po = _arg(fn, "y", y, dt, shape), _arg(fn, "x_out", x_out, dt, shape)
+    elif x_out is not None:
+        raise SagerError("x_out needs y")
+    if xn is not None:
+        pn = _arg(fn, "xn", xn, dt, shape)
     if xq is not None:
-        _dtypes("add_rmsnorm_q8_k", xq=(xq, torch.uint8))
         if xq.numel() != rows * (n // QK) * Q8K_BYTES:
             raise SagerError("xq must hold n/256 Q8_K blocks a row")
-    fn = load().sg_add_rmsnorm_q8_k_f16 if x.dtype == torch.float16 else load().sg_add_rmsnorm_q8_k
-    _check(fn(_ptr(x), _ptr(y), _ptr(x_out), _ptr(w), eps, _ptr(xn), _ptr(xq), n, rows, _stream()))
+        pq = _arg(fn, "xq", xq, torch.uint8, xq.shape)
+    _check(entry(_arg(fn, "x", x, dt, shape), py, po, _arg(fn, "w", w, torch.float32, (n,)), eps, pn,
+                 pq, n, rows, stream))
     return x if y is None else x_out, xn, xq
 
 
-def _rows(name, t, heads, dim):
-    """Element strides (leading dimensions) of a [..., tokens, heads, dim] fp16
-    tensor whose tokens may lie apart."""
-    if t.dtype != torch.float16 or not t.is_cuda:
-        raise SagerError(f"{name} must be fp16 on the GPU")
-    if tuple(t.shape[-2:]) != (heads, dim) or t.stride(-1) != 1 or \
-            (heads > 1 and t.stride(-2) != dim):
-        raise SagerError(f"{name} must be [tokens, {heads}, {dim}], a token's values contiguous")
+def _rows(fn, name, t, shape):
+    """The address and the leading dimensions' strides (elements) of an fp16
+    tensor [..., tokens, heads, dim] whose tokens may lie apart."""
+    st, (heads, dim) = t.stride(), shape[-2:]
+    if t.dtype is not torch.float16 or t.shape != shape or not t.is_cuda or st[-1] != 1 or \
+            (heads > 1 and st[-2] != dim):
+        raise SagerError(f"{fn}: {name} must be fp16 {tuple(shape)} on the GPU, a token's values "
+                         f"contiguous, got {t.dtype} {tuple(t.shape)} strides {st} on {t.device}")
     # (a dimension of one element has any stride)
-    return [max(st, heads * dim) if n == 1 else st for n, st in zip(t.shape[:-2], t.stride()[:-2])]
+    return (t.data_ptr(), *[x if n > 1 else max(x, heads * dim) for n, x in zip(shape[:-2], st)])
 
 
-def _current(name, t):
-    # the launch goes to the current device's current stream
-    if t.is_cuda and t.device.index != torch.cuda.current_device():
-        raise SagerError(f"{name}: {t.device} is not the current device")
-
-
-def _windows(name, win_off, parent, n_tokens):
-    _dtypes(name, win_off=(win_off, torch.int32))
-    _current(name, win_off)
-    if win_off.dim() != 1 or win_off.numel() < 2:
-        raise SagerError(f"{name}: win_off must be [n_seq + 1]")
-    if parent is not None:
-        _dtypes(name, parent=(parent, torch.int32))
-        if parent.numel() != n_tokens:
-            raise SagerError(f"{name}: parent must have one entry a row")
-    return win_off.numel() - 1
+def _windows(fn, win_off, parent, n_tokens):
+    """The number of sequences and the addresses of win_off and parent."""
+    n_seq = win_off.numel() - 1
+    if n_seq < 1:
+        raise SagerError(f"{fn}: win_off must be [n_seq + 1]")
+    off = _arg(fn, "win_off", win_off, torch.int32, (n_seq + 1,))
+    if parent is None:
+        return n_seq, off, None
+    return n_seq, off, _arg(fn, "parent", parent, torch.int32, (n_tokens,))
 
 
 class KvCache:
@@ -627,19 +638,20 @@ class KvCache:
     [n_seq].  Holds the tensors; nothing is copied."""
 
     def __init__(self, k, v, pages, length):
-        _dtypes("KvCache", k=(k, torch.float16), v=(v, torch.float16), pages=(pages, torch.int32),
-                length=(length, torch.int32))
         if k.dim() != 5 or k.shape != v.shape:
             raise SagerError("k and v must be [n_layers, n_pages, n_kv_heads, page_size, head_dim]")
         if pages.dim() != 2 or length.numel() != pages.shape[0]:
             raise SagerError("pages must be [n_seq, pages_per_seq], length [n_seq]")
         if not k.device == v.device == pages.device == length.device:
             raise SagerError("the cache's tensors must be on one device")
+        _dtypes("KvCache", k=(k, torch.float16), v=(v, torch.float16), pages=(pages, torch.int32),
+                length=(length, torch.int32))
         self.k, self.v, self.pages, self.length = k, v, pages, length
-        L, P, H, S, D = k.shape
-        self.n_kv_heads, self.head_dim = H, D
-        self.desc = KvCacheDesc(_ptr(k), _ptr(v), _ptr(pages), _ptr(length), P * H * S * D, L, P, S,
-                                pages.shape[1], H, D)
+        self.n_layers, P, self.n_kv_heads, S, self.head_dim = k.shape
+        self.max_seqs = pages.shape[0]
+        self.desc = KvCacheDesc(_ptr(k), _ptr(v), _ptr(pages), _ptr(length), k[0].numel(),
+                                self.n_layers, P, S, pages.shape[1], self.n_kv_heads, self.head_dim)
+        self._desc = ctypes.byref(self.desc)
 
     def commit(self, k, v, win_off, path, n_path, length_out=None):
         """The accepted tokens' keys and values behind the cache, all layers in
@@ -648,24 +660,23 @@ class KvCache:
         [n_seq] as TreeVerify returns them.  Returns the new lengths (a tensor
         of its own; the cache's own length is left to the caller, since every
         layer of a step still reads it)."""
-        ks, vs = (_rows(n, t, self.n_kv_heads, self.head_dim) for n, t in (("k", k), ("v", v)))
-        if k.dim() != 4 or k.shape != v.shape or k.shape[0] != self.k.shape[0]:
-            raise SagerError("k and v must be [n_layers, n_tokens, n_kv_heads, head_dim]")
-        n_tokens = k.shape[1]
-        n_seq = _windows("commit", win_off, None, n_tokens)
-        _dtypes("commit", path=(path, torch.int32), n_path=(n_path, torch.int32))
-        if path.dim() != 2 or path.shape[0] != n_seq or n_path.numel() != n_seq or \
-                self.pages.shape[0] < n_seq:
-            raise SagerError("path must be [n_seq, max_window], n_path [n_seq]")
+        fn = "KvCache.commit"
+        n_tokens, window = k.shape[1], path.shape[-1]
+        shape = (self.n_layers, n_tokens, self.n_kv_heads, self.head_dim)
+        pk, kl, ks = _rows(fn, "k", k, shape)
+        pv, vl, vs = _rows(fn, "v", v, shape)
+        stream = _current_stream_of(fn, k)
+        n_seq, off, _ = _windows(fn, win_off, None, n_tokens)
+        if n_seq > self.max_seqs:
+            raise SagerError(f"{fn}: {n_seq} sequences, {self.max_seqs} in the cache")
         if length_out is None:
             length_out = torch.empty(n_seq, dtype=torch.int32, device=k.device)
-        _dtypes("commit", length_out=(length_out, torch.int32))
-        if length_out.numel() != n_seq:
-            raise SagerError("length_out must be [n_seq]")
         _check(load().sg_kv_commit_f16(
-            k.data_ptr(), v.data_ptr(), ks[1], vs[1], ks[0], vs[0], ctypes.byref(self.desc),
-            _ptr(win_off), _ptr(path), _ptr(n_path), _ptr(length_out), n_seq, n_tokens,
-            path.shape[1], _stream()))
+            pk, pv, ks, vs, kl, vl, self._desc, off, _arg(fn, "path", path, torch.int32,
+                                                          (n_seq, window)),
+            _arg(fn, "n_path", n_path, torch.int32, (n_seq,)),
+            _arg(fn, "length_out", length_out, torch.int32, (n_seq,)), n_seq, n_tokens, window,
+            stream))
         return length_out
 
 
@@ -691,28 +702,26 @@ class TreeAttention:
         """q fp16 [n_tokens, n_heads, head_dim], k and v [n_tokens, n_kv_heads,
         head_dim] (slices of one projection's output will do) -> out like q,
         contiguous; scale: 1/sqrt(head_dim) if None."""
-        T, D = q.shape[0], self.head_dim
-        (qs,), (ks,), (vs,) = (_rows(n, t, h, D) for n, t, h in (
-            ("q", q, self.n_heads), ("k", k, self.n_kv_heads), ("v", v, self.n_kv_heads)))
-        if k.shape[0] != T or v.shape[0] != T:
-            raise SagerError("q, k and v must have the same tokens")
-        if (cache.n_kv_heads, cache.head_dim) != (self.n_kv_heads, D):
+        fn, T, D = "TreeAttention", q.shape[0], self.head_dim
+        shape, kv_shape = (T, self.n_heads, D), (T, self.n_kv_heads, D)
+        pq, qs = _rows(fn, "q", q, shape)
+        pk, ks = _rows(fn, "k", k, kv_shape)
+        pv, vs = _rows(fn, "v", v, kv_shape)
+        stream = _current_stream_of(fn, q)
+        if cache.n_kv_heads != self.n_kv_heads or cache.head_dim != D:
             raise SagerError("the cache has other heads")
-        n_seq = _windows("TreeAttention", win_off, parent, T)
-        if T > self.max_tokens or n_seq > self.max_seqs or cache.pages.shape[0] < n_seq:
+        n_seq, off, par = _windows(fn, win_off, parent, T)
+        if T > self.max_tokens or n_seq > self.max_seqs or n_seq > cache.max_seqs:
             raise SagerError(f"{n_seq} sequences of {T} tokens: at most {self.max_seqs} of "
-                             f"{self.max_tokens}, {cache.pages.shape[0]} in the cache")
+                             f"{self.max_tokens}, {cache.max_seqs} in the cache")
         if out is None:
-            out = torch.zeros((T, self.n_heads, D), dtype=torch.float16, device=q.device)
-        _dtypes("TreeAttention", out=(out, torch.float16))
-        if out.shape != q.shape:
-            raise SagerError("out must have q's shape")
+            out = torch.zeros(shape, dtype=torch.float16, device=q.device)
         ws = self.workspace if workspace is None else workspace
         _check(load().sg_attn_tree_f16(
-            q.data_ptr(), k.data_ptr(), v.data_ptr(), qs, ks, vs, ctypes.byref(cache.desc), layer,
-            _ptr(win_off), _ptr(parent), _ptr(out), _ptr(ws), ws.numel(), n_seq, T,
-            self.max_window, self.max_len, self.n_heads,
-            D ** -0.5 if scale is None else float(scale), _stream()))
+            pq, pk, pv, qs, ks, vs, cache._desc, layer, off, par,
+            _arg(fn, "out", out, torch.float16, shape), _ptr(ws), ws.numel(), n_seq, T,
+            self.max_window, self.max_len, self.n_heads, D ** -0.5 if scale is None else scale,
+            stream))
         return out
 
 
@@ -735,38 +744,31 @@ class TreeVerify:
         [n_tokens, vocab] or None (drafts that were chosen, not drawn) ->
         (path int32 [n_seq, max_window], n_path int32 [n_seq], next_token
         int32 [n_seq], prob fp32 [n_tokens])."""
-        T = logits.shape[0]
-        n_seq = _windows("TreeVerify", win_off, parent, T)
-        if T > self.max_tokens or n_seq > self.max_seqs or logits.shape != (T, self.vocab):
-            raise SagerError(f"{n_seq} sequences, logits {tuple(logits.shape)}: at most "
-                             f"{self.max_seqs}, {self.max_tokens} rows of {self.vocab}")
-        dev = logits.device
+        fn, T, f32, i32 = "TreeVerify", logits.shape[0], torch.float32, torch.int32
+        stream = _current_stream_of(fn, logits)
+        n_seq, off, par = _windows(fn, win_off, parent, T)
+        if T > self.max_tokens or n_seq > self.max_seqs:
+            raise SagerError(f"{n_seq} sequences of {T} rows: at most {self.max_seqs} of "
+                             f"{self.max_tokens}")
+        dev, rows, seqs = logits.device, (T,), (n_seq,)
+        full, paths = (T, self.vocab), (n_seq, self.max_window)
         if path is None:
-            path = torch.empty((n_seq, self.max_window), dtype=torch.int32, device=dev)
+            path = torch.empty(paths, dtype=i32, device=dev)
         if n_path is None:
-            n_path = torch.empty(n_seq, dtype=torch.int32, device=dev)
+            n_path = torch.empty(n_seq, dtype=i32, device=dev)
         if next_token is None:
-            next_token = torch.empty(n_seq, dtype=torch.int32, device=dev)
+            next_token = torch.empty(n_seq, dtype=i32, device=dev)
         if prob is None:
-            prob = torch.zeros(T, dtype=torch.float32, device=dev)
-        f32, i32 = torch.float32, torch.int32
-        args = dict(logits=(logits, f32, T * self.vocab), tokens=(tokens, i32, T),
-                    temperature=(temperature, f32, n_seq), u_accept=(u_accept, f32, T),
-                    u_sample=(u_sample, f32, n_seq), path=(path, i32, n_seq * self.max_window),
-                    n_path=(n_path, i32, n_seq), next_token=(next_token, i32, n_seq),
-                    prob=(prob, f32, T))
-        if draft_probs is not None:
-            args["draft_probs"] = (draft_probs, f32, T * self.vocab)
-        for name, (t, dt, n) in args.items():
-            if t.numel() != n:
-                raise SagerError(f"TreeVerify: {name} must have {n} values")
-        _dtypes("TreeVerify", **{k: (t, dt) for k, (t, dt, _) in args.items()})
+            prob = torch.zeros(T, dtype=f32, device=dev)
         ws = self.workspace if workspace is None else workspace
         _check(load().sg_tree_verify(
-            _ptr(logits), _ptr(tokens), _ptr(win_off), _ptr(parent), _ptr(draft_probs),
-            _ptr(temperature), _ptr(u_accept), _ptr(u_sample), _ptr(path), _ptr(n_path),
-            _ptr(next_token), _ptr(prob), _ptr(ws), ws.numel(), n_seq, T, self.max_window,
-            self.vocab, self.max_children, _stream()))
+            _arg(fn, "logits", logits, f32, full), _arg(fn, "tokens", tokens, i32, rows), off, par,
+            None if draft_probs is None else _arg(fn, "draft_probs", draft_probs, f32, full),
+            _arg(fn, "temperature", temperature, f32, seqs),
+            _arg(fn, "u_accept", u_accept, f32, rows), _arg(fn, "u_sample", u_sample, f32, seqs),
+            _arg(fn, "path", path, i32, paths), _arg(fn, "n_path", n_path, i32, seqs),
+            _arg(fn, "next_token", next_token, i32, seqs), _arg(fn, "prob", prob, f32, rows),
+            _ptr(ws), ws.numel(), n_seq, T, self.max_window, self.vocab, self.max_children, stream))
         return path, n_path, next_token, prob
 
 
