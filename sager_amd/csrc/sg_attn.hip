@@ -802,22 +802,25 @@ struct CommitArgs {
   uint16_t *kc, *vc;
   const int *pages, *length, *win_off, *path, *n_path;
   int* length_out;
-  int n_tokens, max_window, n_kv, dim, n_pages, page_log2, pages_per_seq;
+  int n_tokens, max_window, n_layers, n_kv, dim, n_pages, page_log2, pages_per_seq;
 };
 
-// Grid: (16-B pieces of a window's K and V rows, sequence, layer).
+// Grid: (16-B pieces of a window's K and V rows, sequence, kCommitLayers
+// layers).  A thread looks its piece's place up once and then copies it in
+// every layer, whose loads are under way together.
+constexpr int kCommitLayers = 8;
 __global__ void __launch_bounds__(256) kv_commit_kernel(const CommitArgs a) {
-  const int s = blockIdx.y, layer = blockIdx.z;
-  const Window w = window_of(a.win_off, s, a.n_tokens, a.max_window);
+  const int s = blockIdx.y, l0 = blockIdx.z * kCommitLayers;
   const int n = min(max(a.n_path[s], 0), a.max_window);
   const int len = a.length[s];
-  if (a.length_out && blockIdx.x == 0 && layer == 0 && threadIdx.x == 0) a.length_out[s] = len + n;
+  if (a.length_out && blockIdx.x == 0 && l0 == 0 && threadIdx.x == 0) a.length_out[s] = len + n;
   const int pieces = a.n_kv * (a.dim / 8);
   int x = blockIdx.x * 256 + threadIdx.x;
-  const bool is_v = x & 1;  // K's and V's piece of one place by neighbours: both tables' pages once
+  const bool is_v = x & 1;  // K's and V's piece of one place by neighbours
   x >>= 1;
   const int i = x / pieces;
   if (i >= n) return;
+  const Window w = window_of(a.win_off, s, a.n_tokens, a.max_window);
   x -= i * pieces;
   const int h = x / (a.dim / 8), c = x - h * (a.dim / 8);
   const int node = a.path[static_cast<long long>(s) * a.max_window + i];
@@ -825,13 +828,23 @@ __global__ void __launch_bounds__(256) kv_commit_kernel(const CommitArgs a) {
   if (len < 0 || node < 0 || node >= w.n || pos >> a.page_log2 >= a.pages_per_seq) return;
   const int page = a.pages[static_cast<long long>(s) * a.pages_per_seq + (pos >> a.page_log2)];
   if (page < 0 || page >= a.n_pages) return;
-  const uint16_t* src = (is_v ? a.v + layer * a.v_layer + (w.off + node) * a.v_stride
-                              : a.k + layer * a.k_layer + (w.off + node) * a.k_stride) +
-                        h * a.dim + c * 8;
+  const long long step = is_v ? a.v_layer : a.k_layer;
+  const uint16_t* src = (is_v ? a.v + (w.off + node) * a.v_stride : a.k + (w.off + node) * a.k_stride) +
+                        h * a.dim + c * 8 + l0 * step;
   const long long slot = ((static_cast<long long>(page) * a.n_kv + h) << a.page_log2) +
                          (pos & ((1 << a.page_log2) - 1));
-  uint16_t* dst = (is_v ? a.vc : a.kc) + layer * a.layer_stride + slot * a.dim + c * 8;
-  *reinterpret_cast<u32x4*>(dst) = *reinterpret_cast<const u32x4_u*>(src);
+  uint16_t* dst = (is_v ? a.vc : a.kc) + l0 * a.layer_stride + slot * a.dim + c * 8;
+  if (l0 + kCommitLayers <= a.n_layers) {
+    u32x4 v[kCommitLayers];
+#pragma unroll
+    for (int l = 0; l < kCommitLayers; ++l) v[l] = *reinterpret_cast<const u32x4_u*>(src + l * step);
+#pragma unroll
+    for (int l = 0; l < kCommitLayers; ++l) *reinterpret_cast<u32x4*>(dst + l * a.layer_stride) = v[l];
+  } else {
+    for (int l = 0; l0 + l < a.n_layers; ++l)
+      *reinterpret_cast<u32x4*>(dst + l * a.layer_stride) =
+          *reinterpret_cast<const u32x4_u*>(src + l * step);
+  }
 }
 
 // ---- host -----------------------------------------------------------------------
@@ -1049,13 +1062,15 @@ int sg_kv_commit_f16(const uint16_t* k, const uint16_t* v, long long k_stride, l
   a.length_out = length_out;
   a.n_tokens = n_tokens;
   a.max_window = max_window;
+  a.n_layers = cache->n_layers;
   a.n_kv = cache->n_kv_heads;
   a.dim = cache->head_dim;
   a.n_pages = cache->n_pages;
   a.page_log2 = log2_of(cache->page_size);
   a.pages_per_seq = cache->pages_per_seq;
   hipLaunchKernelGGL(kv_commit_kernel,
-                     dim3(static_cast<unsigned>((pieces + 255) / 256), n_seq, cache->n_layers),
+                     dim3(static_cast<unsigned>((pieces + 255) / 256), n_seq,
+                          (cache->n_layers + kCommitLayers - 1) / kCommitLayers),
                      dim3(256), 0, static_cast<hipStream_t>(stream), a);
   return check_launch(nm);
 }

@@ -68,23 +68,20 @@ __device__ __forceinline__ float wave_sum_dpp(float v) {
 
 // kNW waves per row, each up to kB blocks of 256 values held in registers
 // (lane l has values 4l..4l+3 of a block, the layout of the Q8_K quantizer).
-// kNW == 1: four rows per workgroup and no barrier.
 template <typename T, int kNW, int kB>
-__global__ void __launch_bounds__(kNW == 1 ? 256 : 64 * kNW)
+__global__ void __launch_bounds__(64 * kNW)
     add_rmsnorm_kernel(const T* x, const T* y, T* x_out, const float* w, T* xn,
                        unsigned char* xq, int n, int n_rows, float eps) {
   const int lane = threadIdx.x & 63;
   const int wave = threadIdx.x >> 6;
-  const int part = kNW == 1 ? 0 : wave;
-  const long long row = kNW == 1 ? static_cast<long long>(blockIdx.x) * 4 + wave : blockIdx.x;
-  if (kNW == 1 && row >= n_rows) return;
+  const long long row = blockIdx.x;
   const int nb = n / kQK;
   const long long at = row * n + 4 * lane;
   float v[kB][4], wv[kB][4];
   float ss = 0.f;
 #pragma unroll
   for (int i = 0; i < kB; ++i) {
-    const int b = part + kNW * i;
+    const int b = wave + kNW * i;
     if (b < nb) {
       load4(x + at + b * kQK, v[i]);
       load4(w + b * kQK + 4 * lane, wv[i]);
@@ -93,7 +90,7 @@ __global__ void __launch_bounds__(kNW == 1 ? 256 : 64 * kNW)
   if (y) {
 #pragma unroll
     for (int i = 0; i < kB; ++i) {
-      const int b = part + kNW * i;
+      const int b = wave + kNW * i;
       if (b < nb) {
         float a[4];
         load4(y + at + b * kQK, a);
@@ -105,22 +102,20 @@ __global__ void __launch_bounds__(kNW == 1 ? 256 : 64 * kNW)
   }
 #pragma unroll
   for (int i = 0; i < kB; ++i)
-    if (part + kNW * i < nb)
+    if (wave + kNW * i < nb)
 #pragma unroll
       for (int j = 0; j < 4; ++j) ss = __builtin_fmaf(v[i][j], v[i][j], ss);
   ss = wave_sum_dpp(ss);
-  if (kNW > 1) {
-    __shared__ float part_ss[kNW];
-    if (lane == 0) part_ss[wave] = ss;
-    __syncthreads();
-    ss = part_ss[0];
+  __shared__ float part_ss[kNW];
+  if (lane == 0) part_ss[wave] = ss;
+  __syncthreads();
+  ss = part_ss[0];
 #pragma unroll
-    for (int i = 1; i < kNW; ++i) ss += part_ss[i];
-  }
+  for (int i = 1; i < kNW; ++i) ss += part_ss[i];
   const float s = 1.f / sqrtf(ss / static_cast<float>(n) + eps);
 #pragma unroll
   for (int i = 0; i < kB; ++i) {
-    const int b = part + kNW * i;
+    const int b = wave + kNW * i;
     if (b < nb) {
 #pragma unroll
       for (int j = 0; j < 4; ++j) v[i][j] = (v[i][j] * s) * wv[i][j];
@@ -136,10 +131,8 @@ __global__ void __launch_bounds__(kNW == 1 ? 256 : 64 * kNW)
 template <typename T, int kNW, int kB>
 static void norm_go(const T* x, const T* y, T* x_out, const float* w, float eps, T* xn,
                     sg_block_q8k* xq, int n, int n_rows, hipStream_t s) {
-  const int grid = kNW == 1 ? (n_rows + 3) / 4 : n_rows;
-  hipLaunchKernelGGL((add_rmsnorm_kernel<T, kNW, kB>), dim3(grid),
-                     dim3(kNW == 1 ? 256 : 64 * kNW), 0, s, x, y, x_out, w, xn,
-                     reinterpret_cast<unsigned char*>(xq), n, n_rows, eps);
+  hipLaunchKernelGGL((add_rmsnorm_kernel<T, kNW, kB>), dim3(n_rows), dim3(64 * kNW), 0, s, x, y,
+                     x_out, w, xn, reinterpret_cast<unsigned char*>(xq), n, n_rows, eps);
 }
 
 template <typename T>
@@ -159,10 +152,15 @@ static int norm_launch(const T* x, const T* y, T* x_out, const float* w, float e
     return set_error(SG_ERR_INVALID_ARGUMENT, "%s: a buffer is not aligned to its elements", nm);
   const hipStream_t s = static_cast<hipStream_t>(stream);
   const int nb = n / kQK;
-  if (nb <= 8)
-    norm_go<T, 4, 2>(x, y, x_out, w, eps, xn, xq, n, n_rows, s);
+  // one block a wave as far as the waves go
+  if (nb <= 4)
+    norm_go<T, 4, 1>(x, y, x_out, w, eps, xn, xq, n, n_rows, s);
+  else if (nb <= 8)
+    norm_go<T, 8, 1>(x, y, x_out, w, eps, xn, xq, n, n_rows, s);
+  else if (nb <= 16)
+    norm_go<T, 16, 1>(x, y, x_out, w, eps, xn, xq, n, n_rows, s);
   else if (nb <= 32)
-    norm_go<T, 8, 4>(x, y, x_out, w, eps, xn, xq, n, n_rows, s);
+    norm_go<T, 16, 2>(x, y, x_out, w, eps, xn, xq, n, n_rows, s);
   else
     norm_go<T, 16, 4>(x, y, x_out, w, eps, xn, xq, n, n_rows, s);
   return check_launch(nm);
