@@ -10,14 +10,14 @@
 // consecutive keys, which ds_read_b64_tr_b16 reads from V's rows as they lie
 // in memory.  Two kernels:
 //
-//   attn_few_kernel   up to 64 rows: the four waves share the keys of the
-//                     first product and the columns of the second, P goes
-//                     through LDS between them.  K and V are read from LDS
-//                     once, no wave holds more than a quarter of O, and
+//   attn_few_kernel   blocks of 16 or 32 rows: the four waves share the keys
+//                     of the first product and the columns of the second, P
+//                     goes through LDS between them.  K and V are read from
+//                     LDS once, no wave holds more than a quarter of O, and
 //                     nothing is joined at the end but the rows' sums.
-//   attn_rows_kernel  more rows: each wave has 32 rows of its own and reads
-//                     all of K and V from LDS; P stays in its lanes, and one
-//                     barrier a step orders the copies.
+//   attn_rows_kernel  blocks of 256 rows: each of eight waves has 32 rows of
+//                     its own and reads all of K and V from LDS; P stays in
+//                     its lanes, and one barrier a step orders the copies.
 //
 // A row's running maximum is a reference point `mref` that moves only when a
 // score passes it by 2^15: p = 2^(s - mref) fits fp16 (its largest value is
@@ -117,7 +117,10 @@ struct Part {
   uint32_t lds0;
 
   // The row blocks of a unit (part, kv head, sequence) are 8 workgroups apart:
-  // on one XCD, whose L2 then reads the unit's keys once.
+  // on one XCD, whose L2 then reads the unit's keys once.  The units of eight
+  // go to the XCDs in turn, each time from another one on, so that no XCD gets
+  // the same part of every sequence (24 ragged sequences in 8 parts: 54 us
+  // with the last, mostly empty parts on one XCD).
   __device__ __forceinline__ bool start(unsigned char* l, int block_rows) {
     lds = l;
     lds0 = static_cast<uint32_t>(
@@ -128,7 +131,7 @@ struct Part {
     const int id = blockIdx.x;
     const int oct = id / (8 * a.row_blocks), in = id - oct * 8 * a.row_blocks;
     rb = in >> 3;
-    int unit = oct * 8 + (in & 7);
+    int unit = oct * 8 + ((in + oct) & 7);
     if (unit >= a.units) return false;
     split = unit % a.n_split;
     unit /= a.n_split;
@@ -329,7 +332,7 @@ struct Part {
   }
 };
 
-// ---- up to 64 rows ---------------------------------------------------------------
+// ---- blocks of 16 or 32 rows ---------------------------------------------------------------
 // LDS: K and V of two steps, P, the rows' maxima and sums of the four waves,
 // the nodes' ancestors, the flags.
 template <int D, int RT>
@@ -530,8 +533,9 @@ __global__ void __launch_bounds__(256) attn_few_kernel(const AttnArgs a) {
   }
 }
 
-// ---- more rows ---------------------------------------------------------------------
-template <int D, int RT, int NW>
+// ---- blocks of 256 rows ---------------------------------------------------------------------
+constexpr int kRowWaves = 8, kRowTiles = 2;  // 16-row tiles of a wave
+template <int D>
 struct RowsLds {
   static constexpr uint32_t kSeen = 4 * Part<D>::kStep;
   static constexpr uint32_t kThere = kSeen + kMaxWindow * 8;
@@ -539,16 +543,15 @@ struct RowsLds {
   static constexpr uint32_t kBytes = kFlags + 16;
 };
 
-// NW waves of 16 RT rows each.  Four waves bring 16 keys of K and V each,
-// eight 16 keys of K or V.
-template <int D, int RT, int NW>
-__global__ void __launch_bounds__(64 * NW) attn_rows_kernel(const AttnArgs a) {
+// Each wave brings 16 keys of K (the first four) or V.
+template <int D>
+__global__ void __launch_bounds__(64 * kRowWaves) attn_rows_kernel(const AttnArgs a) {
   typedef Part<D> P;
-  typedef RowsLds<D, RT, NW> L;
-  constexpr int DT = D / 16;
+  typedef RowsLds<D> L;
+  constexpr int RT = kRowTiles, NW = kRowWaves, DT = D / 16;
   extern __shared__ __attribute__((aligned(16))) unsigned char lds[];
   const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
-  const int blk = wave & 3, kv = NW == 4 ? 3 : 1 + (wave >> 2);
+  const int blk = wave & 3, kv = 1 + (wave >> 2);
   P t{a};
   if (!t.start(lds, 16 * RT * NW)) return;
   const int lane = t.lane, col = t.col, grp = t.grp;
@@ -891,12 +894,12 @@ struct Cut {
 static Cut attn_cut(int n_seq, int max_window, int max_len, int group, int n_kv, int dim) {
   Cut c;
   const long long rows = static_cast<long long>(max_window) * group;
-  c.block_rows = rows > 128 ? 256 : rows > 64 ? 128 : rows > 32 ? 64 : rows > 16 ? 32 : 16;
+  c.block_rows = rows > 128 ? 256 : rows > 16 ? 32 : 16;
   c.row_blocks = static_cast<int>((rows + c.block_rows - 1) / c.block_rows);
   const long long keys = static_cast<long long>(max_len) + max_window;
   const long long most = (keys + kKeys - 1) / kKeys;
   const long long units = static_cast<long long>(n_seq) * n_kv * c.row_blocks;
-  const long long slots = 256 * (dim == 256 ? 1 : 2);
+  const long long slots = 256 * (dim == 256 || c.block_rows == 256 ? 1 : 2) * (n_seq > 1 ? 2 : 1);
   long long n = units >= slots ? 1 : slots / units;
   if (n > most) n = most;
   c.split_keys = static_cast<int>((most + n - 1) / n * kKeys);
@@ -908,25 +911,16 @@ static size_t part_bytes(const Cut& c, int n_tokens, int n_heads, int dim) {
   return static_cast<size_t>(c.n_split) * n_tokens * n_heads * (dim * 4 + 8);
 }
 
-template <int D, int RT>
-static void few_go(const AttnArgs& a, unsigned grid, hipStream_t s) {
-  hipLaunchKernelGGL((attn_few_kernel<D, RT>), dim3(grid), dim3(256), (FewLds<D, RT>::kBytes), s, a);
-}
-template <int D, int RT, int NW>
-static void rows_go(const AttnArgs& a, unsigned grid, hipStream_t s) {
-  hipLaunchKernelGGL((attn_rows_kernel<D, RT, NW>), dim3(grid), dim3(64 * NW),
-                     (RowsLds<D, RT, NW>::kBytes), s, a);
-}
 template <int D>
 static int attn_launch(const AttnArgs& a, const Cut& c, int n_seq, hipStream_t s, const char* nm) {
   const unsigned grid = static_cast<unsigned>((a.units + 7LL) / 8 * 8 * c.row_blocks);
-  switch (c.block_rows) {
-    case 256: rows_go<D, 2, 8>(a, grid, s); break;
-    case 128: rows_go<D, 2, 4>(a, grid, s); break;
-    case 64: few_go<D, 4>(a, grid, s); break;
-    case 32: few_go<D, 2>(a, grid, s); break;
-    default: few_go<D, 1>(a, grid, s); break;
-  }
+  if (c.block_rows == 256)
+    hipLaunchKernelGGL(attn_rows_kernel<D>, dim3(grid), dim3(64 * kRowWaves), RowsLds<D>::kBytes, s,
+                       a);
+  else if (c.block_rows == 32)
+    hipLaunchKernelGGL((attn_few_kernel<D, 2>), dim3(grid), dim3(256), (FewLds<D, 2>::kBytes), s, a);
+  else
+    hipLaunchKernelGGL((attn_few_kernel<D, 1>), dim3(grid), dim3(256), (FewLds<D, 1>::kBytes), s, a);
   if (int st = check_launch(nm)) return st;
   if (c.n_split > 1) {
     hipLaunchKernelGGL(attn_join_kernel<D>, dim3(n_seq * a.max_window * a.n_heads), dim3(256), 0, s,
