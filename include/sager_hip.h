@@ -551,11 +551,12 @@ typedef struct sg_kv_cache {
  * out contiguous.  k, v, the cache's k and v and their strides are 16-B
  * aligned.  Scores, softmax statistics and sums are fp32; the weights p are
  * rounded to fp16 for the product with v.  max_len bounds the caches'
- * lengths for the split of the work; longer caches are right, but slower.
- * Workspace: sg_attn_tree_workspace_bytes; it belongs to one call at a time.
- * One launch, or two where the caches are cut into parts. */
-size_t sg_attn_tree_workspace_bytes(int n_seq, int n_tokens, int max_window, int max_len,
-                                    int n_heads, int n_kv_heads, int head_dim);
+ * lengths for the choice of the launches; longer caches are right, but may
+ * be slower.  Workspace: sg_attn_tree_workspace_bytes of as many sequences or
+ * more (it may be 0 bytes); it belongs to one call at a time.  One launch, or
+ * two where the caches are cut into parts. */
+size_t sg_attn_tree_workspace_bytes(int n_seq, int max_window, int max_len, int n_heads,
+                                    int n_kv_heads, int head_dim);
 int sg_attn_tree_f16(const uint16_t* q, const uint16_t* k, const uint16_t* v, long long q_stride,
                      long long k_stride, long long v_stride, const sg_kv_cache* cache, int layer,
                      const int* win_off, const int* parent, uint16_t* out, void* ws,

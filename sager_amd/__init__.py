@@ -89,7 +89,7 @@ SIGNATURES = {
                             _VP, _SZ, _I, _I, _I, _I, _I, _F, _VP]),
     "sg_add_rmsnorm_q8_k": (_I, [_VP, _VP, _VP, _VP, _F, _VP, _VP, _I, _I, _VP]),
     "sg_add_rmsnorm_q8_k_f16": (_I, [_VP, _VP, _VP, _VP, _F, _VP, _VP, _I, _I, _VP]),
-    "sg_attn_tree_workspace_bytes": (_SZ, [_I, _I, _I, _I, _I, _I, _I]),
+    "sg_attn_tree_workspace_bytes": (_SZ, [_I, _I, _I, _I, _I, _I]),
     "sg_attn_tree_f16": (_I, [_VP, _VP, _VP, _LL, _LL, _LL, _VP, _I, _VP, _VP, _VP, _VP, _SZ, _I,
                               _I, _I, _I, _I, _F, _VP]),
     "sg_kv_commit_f16": (_I, [_VP, _VP, _LL, _LL, _LL, _LL, _VP, _VP, _VP, _VP, _VP, _I, _I, _I,

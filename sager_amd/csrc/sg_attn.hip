@@ -48,10 +48,15 @@ struct AttnArgs {
   const uint16_t *kc, *vc;
   const int *pages, *length, *win_off, *parent;
   uint16_t* out;
-  float* part_o;   // [split][token][head][D]
-  float2* part_ml; // [split][token][head]: mref (log2), l
+  // Parts of cut units, by unit, row block and row: O, and mref (log2) and l.
+  // seq_plan: per sequence its first unit and the parts of its units; then the
+  // steps of a part.
+  float* part_o;
+  float2* part_ml;
+  int2* seq_plan;
   int n_tokens, max_window, n_heads, n_kv, group, n_pages, page_log2, pages_per_seq;
-  int n_split, split_keys, row_blocks, units;
+  int n_seq, row_blocks, block_rows, max_units;
+  bool cut;
   float scale_log2;
 };
 
@@ -68,6 +73,88 @@ __device__ __forceinline__ kernarg_p cold_args() {
 __device__ __forceinline__ int cached_len(int length, int page_log2, int pages_per_seq) {
   const long long cap = static_cast<long long>(pages_per_seq) << page_log2;
   return static_cast<int>(length < 0 ? 0 : length > cap ? cap : length);
+}
+
+// How a batch is cut, from the caches' lengths, which only the device knows.
+// A unit is a part of a sequence's keys for one kv head; a sequence's steps of
+// 64 keys are cut into parts of `part` steps, the least for which the units
+// are no more than max_units, so that the units of a ragged batch are equally
+// long and the launch ends in one round.  Every wave finds this by itself: a
+// sequence a lane, the sum, a few guesses at `part`, the running sum.
+__device__ __forceinline__ int parts_of(int steps, int part) {
+  // (fp32: a part more or less changes nothing, the last one takes what is left)
+  const float inv = __builtin_amdgcn_rcpf(static_cast<float>(part));
+  return steps > 0 ? max(1, static_cast<int>(ceilf(static_cast<float>(steps) * inv))) : 0;
+}
+__device__ __forceinline__ int steps_of(const AttnArgs& a, int seq, int* len, Window* win) {
+  if (seq >= a.n_seq) return 0;
+  *win = window_of(a.win_off, seq, a.n_tokens, a.max_window);
+  *len = cached_len(a.length[seq], a.page_log2, a.pages_per_seq);
+  return win->n > 0 ? (*len + win->n + kKeys - 1) / kKeys : 0;
+}
+__device__ __forceinline__ int wave_run_sum_i(int v) {  // lane l: of lanes 0..l
+  v += __builtin_amdgcn_update_dpp(0, v, 0x111, 0xF, 0xF, false);
+  v += __builtin_amdgcn_update_dpp(0, v, 0x112, 0xF, 0xF, false);
+  v += __builtin_amdgcn_update_dpp(0, v, 0x114, 0xF, 0xF, false);
+  v += __builtin_amdgcn_update_dpp(0, v, 0x118, 0xF, 0xF, false);
+  v += __builtin_amdgcn_update_dpp(0, v, 0x142, 0xA, 0xF, false);
+  v += __builtin_amdgcn_update_dpp(0, v, 0x143, 0xC, 0xF, false);
+  return v;
+}
+struct Unit {
+  int seq, h, k, parts, part;  // part k of `parts`, `part` steps each
+  int len, steps;
+  Window win;
+};
+// Finds unit `unit`; false if there is none.  plan: leaves the plan for the join.
+__device__ __forceinline__ bool find_unit(const AttnArgs& a, int unit, int lane, bool plan, Unit& u) {
+  int len = 0;
+  Window win{0, 0};
+  int steps = steps_of(a, lane, &len, &win);
+  int part = 0x7FFFFFFF;
+  if (a.cut) {
+    long long sum = __builtin_amdgcn_readlane(wave_run_sum_i(steps), 63);
+    if (a.n_seq <= 64) {
+      part = max(1, static_cast<int>((sum * a.n_kv + a.max_units - 1) / a.max_units));
+      while (__builtin_amdgcn_readlane(wave_run_sum_i(parts_of(steps, part)), 63) * a.n_kv >
+             a.max_units)
+        part += max(1, part >> 3);
+    } else {  // (a sequence has at most one part more than its share)
+      for (int s = lane + 64; s - lane < a.n_seq; s += 64) {
+        int l;
+        Window w;
+        sum += __builtin_amdgcn_readlane(wave_run_sum_i(steps_of(a, s, &l, &w)), 63);
+      }
+      const long long free = a.max_units - static_cast<long long>(a.n_seq) * a.n_kv;
+      part = max(1, static_cast<int>(min((sum * a.n_kv + free - 1) / free, 0x7FFFFFFFLL)));
+    }
+  }
+  int base = 0;
+  bool found = false;
+  for (int s0 = 0; s0 < a.n_seq; s0 += 64) {
+    if (s0 > 0) steps = steps_of(a, s0 + lane, &len, &win);
+    const int n = a.cut ? parts_of(steps, part) : steps > 0;
+    const int run = wave_run_sum_i(n) * a.n_kv;  // units up to this sequence's end
+    if (plan && s0 + lane < a.n_seq) a.seq_plan[s0 + lane] = make_int2(base + run - n * a.n_kv, n);
+    const uint64_t past = __ballot(base + run > unit);
+    if (past && !found) {
+      const int l = __builtin_ctzll(past);
+      found = true;
+      u.seq = s0 + l;
+      u.parts = __builtin_amdgcn_readlane(n, l);
+      const int in = unit - (base + __builtin_amdgcn_readlane(run, l) - u.parts * a.n_kv);
+      u.h = in / u.parts;
+      u.k = in - u.h * u.parts;
+      u.part = part;
+      u.len = __builtin_amdgcn_readlane(len, l);
+      u.steps = __builtin_amdgcn_readlane(steps, l);
+      u.win.off = __builtin_amdgcn_readlane(win.off, l);
+      u.win.n = __builtin_amdgcn_readlane(win.n, l);
+      if (!plan) break;
+    }
+    base += __builtin_amdgcn_readlane(run, 63);
+  }
+  return found;
 }
 
 // Where chunk c (16 B) of row r lies in its row: at c ^ swz(r).  Rows are a
@@ -108,7 +195,7 @@ struct Part {
 
   const AttnArgs& a;
   int lane, col, grp;
-  int split, rb, h, seq;
+  int unit, parts, rb, h;
   Window win;
   int rows, len, total;  // rows of the window; cached keys, cached and window's
   int begin, end;        // steps
@@ -116,12 +203,9 @@ struct Part {
   unsigned char* lds;
   uint32_t lds0;
 
-  // The row blocks of a unit (part, kv head, sequence) are 8 workgroups apart:
-  // on one XCD, whose L2 then reads the unit's keys once.  The units of eight
-  // go to the XCDs in turn, each time from another one on, so that no XCD gets
-  // the same part of every sequence (24 ragged sequences in 8 parts: 54 us
-  // with the last, mostly empty parts on one XCD).
-  __device__ __forceinline__ bool start(unsigned char* l, int block_rows) {
+  // The row blocks of a unit are 8 workgroups apart: on one XCD, whose L2 then
+  // reads the unit's keys once.
+  __device__ __forceinline__ bool start(unsigned char* l) {
     lds = l;
     lds0 = static_cast<uint32_t>(
         reinterpret_cast<uintptr_t>((__attribute__((address_space(3))) unsigned char*)l));
@@ -131,22 +215,23 @@ struct Part {
     const int id = blockIdx.x;
     const int oct = id / (8 * a.row_blocks), in = id - oct * 8 * a.row_blocks;
     rb = in >> 3;
-    int unit = oct * 8 + ((in + oct) & 7);
-    if (unit >= a.units) return false;
-    split = unit % a.n_split;
-    unit /= a.n_split;
-    h = unit % a.n_kv;
-    seq = unit / a.n_kv;
-    win = window_of(a.win_off, seq, a.n_tokens, a.max_window);
+    unit = oct * 8 + (in & 7);
+    Unit u;
+    const bool plan = a.cut && id == 0 && __builtin_amdgcn_readfirstlane(threadIdx.x >> 6) == 0;
+    if (!find_unit(a, unit, lane, plan, u)) return false;
+    auto one = [](int v) { return __builtin_amdgcn_readfirstlane(v); };  // (the same in every lane)
+    h = one(u.h);
+    parts = one(u.parts);
+    win = Window{one(u.win.off), one(u.win.n)};
     rows = win.n * a.group;
-    if (rb * block_rows >= rows) return false;
-    len = cached_len(((const_int_p)a.length)[seq], a.page_log2, a.pages_per_seq);
+    if (rb * a.block_rows >= rows) return false;
+    len = one(u.len);
     total = len + win.n;
-    table = (const_int_p)(a.pages + static_cast<long long>(seq) * a.pages_per_seq);
-    const int steps = (total + kKeys - 1) / kKeys, per = a.split_keys / kKeys;
-    const long long first = static_cast<long long>(split) * per;
-    end = split == a.n_split - 1 || first + per > steps ? steps : static_cast<int>(first + per);
-    begin = first < end ? static_cast<int>(first) : end;
+    table = (const_int_p)(a.pages + static_cast<long long>(one(u.seq)) * a.pages_per_seq);
+    const int k = one(u.k), part = one(u.part), steps = one(u.steps);
+    const long long first = static_cast<long long>(k) * part;
+    begin = first < steps ? static_cast<int>(first) : steps;
+    end = k == parts - 1 || first + part > steps ? steps : static_cast<int>(first + part);
     return true;
   }
   // The page of keys 16 b.. of step s (pages hold a multiple of 16 keys).
@@ -310,9 +395,9 @@ struct Part {
                                         bool first) const {
     if (r >= rows) return;
     const kernarg_p a = cold_args();
-    const int node = r / a->group, g = r - node * a->group;
-    const long long at = static_cast<long long>(win.off + node) * a->n_heads + h * a->group + g;
-    if (a->n_split == 1) {
+    if (parts == 1) {
+      const int node = r / a->group, g = r - node * a->group;
+      const long long at = static_cast<long long>(win.off + node) * a->n_heads + h * a->group + g;
       const float inv = l != 0.f ? 1.f / l : 0.f;
 #pragma unroll
       for (int d = 0; d < N; ++d) {
@@ -323,7 +408,8 @@ struct Part {
         *reinterpret_cast<h4*>(a->out + at * D + c + d * kStride) = y;
       }
     } else {
-      const long long pa = static_cast<long long>(split) * a->n_tokens * a->n_heads + at;
+      const long long pa =
+          (static_cast<long long>(unit) * a->row_blocks + rb) * a->block_rows + r - rb * a->block_rows;
 #pragma unroll
       for (int d = 0; d < N; ++d)
         *reinterpret_cast<f4*>(a->part_o + pa * D + c + d * kStride) = o[d];
@@ -356,7 +442,7 @@ __global__ void __launch_bounds__(256) attn_few_kernel(const AttnArgs a) {
   extern __shared__ __attribute__((aligned(16))) unsigned char lds[];
   const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
   P t{a};
-  if (!t.start(lds, kRows)) return;
+  if (!t.start(lds)) return;
   const int lane = t.lane, col = t.col, grp = t.grp, row0 = t.rb * kRows;
   // flags of odd and even steps: 1 + the last step whose reference points move, and the last
   // with infinities or NaN in its window's V
@@ -553,7 +639,7 @@ __global__ void __launch_bounds__(64 * kRowWaves) attn_rows_kernel(const AttnArg
   const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
   const int blk = wave & 3, kv = 1 + (wave >> 2);
   P t{a};
-  if (!t.start(lds, 16 * RT * NW)) return;
+  if (!t.start(lds)) return;
   const int lane = t.lane, col = t.col, grp = t.grp;
   const int row0 = (t.rb * NW + wave) * 16 * RT;
   int* odds = reinterpret_cast<int*>(lds + L::kFlags);  // 1 + the last odd (even) step with any
@@ -731,27 +817,33 @@ __global__ void __launch_bounds__(256) attn_join_kernel(const AttnArgs a) {
   const int rest = blockIdx.x - seq * per;
   const int node = rest / a.n_heads, head = rest - node * a.n_heads;
   const Window w = window_of(a.win_off, seq, a.n_tokens, a.max_window);
-  if (node >= w.n) return;
-  const long long at = static_cast<long long>(w.off + node) * a.n_heads + head;
-  const long long step = static_cast<long long>(a.n_tokens) * a.n_heads;
+  const int2 plan = a.seq_plan[seq];  // the first unit, the parts
+  if (node >= w.n || plan.y <= 1) return;
+  const int h = head / a.group, r = node * a.group + head - h * a.group;
+  const int rb = r / a.block_rows;
+  // the row in the unit's first part; from part to part:
+  const long long at =
+      (static_cast<long long>(plan.x + h * plan.y) * a.row_blocks + rb) * a.block_rows + r -
+      rb * a.block_rows;
+  const long long step = static_cast<long long>(a.row_blocks) * a.block_rows;
   const int t = threadIdx.x, sub = t / LP, c = (t % LP) * 4;
   const float* po = a.part_o + at * D + c;
   // every lane group joins its parts about a maximum of its own
   float m = -INFINITY, sum = 0.f;
   f4 o = (f4){0.f, 0.f, 0.f, 0.f};
-  for (int s0 = sub; s0 < a.n_split; s0 += SP * U) {
+  for (int s0 = sub; s0 < plan.y; s0 += SP * U) {
     f4 v[U];
     float2 ml[U];
 #pragma unroll
     for (int u = 0; u < U; ++u) {
-      const int s = min(s0 + u * SP, a.n_split - 1);
+      const int s = min(s0 + u * SP, plan.y - 1);
       ml[u] = a.part_ml[at + s * step];
       v[u] = *reinterpret_cast<const f4*>(po + s * step * D);
     }
     float top = m;
 #pragma unroll
     for (int u = 0; u < U; ++u) {
-      if (s0 + u * SP >= a.n_split) ml[u].y = 0.f;
+      if (s0 + u * SP >= plan.y) ml[u].y = 0.f;
       top = ml[u].y != 0.f ? fmaxf(top, ml[u].x) : top;
     }
     const float f0 = m > -INFINITY ? __builtin_amdgcn_exp2f(m - top) : 0.f;
@@ -794,7 +886,8 @@ __global__ void __launch_bounds__(256) attn_join_kernel(const AttnArgs a) {
     h4 z;
 #pragma unroll
     for (int j = 0; j < 4; ++j) z[j] = static_cast<_Float16>(y[j] * inv);
-    *reinterpret_cast<h4*>(a.out + at * D + c) = z;
+    const long long row = static_cast<long long>(w.off + node) * a.n_heads + head;
+    *reinterpret_cast<h4*>(a.out + row * D + c) = z;
   }
 }
 
@@ -887,44 +980,52 @@ static int check_cache(const sg_kv_cache* c, int n_seq, int n_tokens, int max_wi
   return SG_OK;
 }
 
-// How a call is cut: rows of a workgroup, parts of the caches.
-struct Cut {
-  int block_rows, row_blocks, n_split, split_keys;
+// How a call is laid out: rows of a workgroup, the most units.
+struct Layout {
+  int block_rows, row_blocks, max_units;
+  bool cut;
+  int least_cut;                      // the most sequences that are cut whatever their lengths
+  size_t plan_bytes, o_bytes, bytes;  // of the workspace
 };
-static Cut attn_cut(int n_seq, int max_window, int max_len, int group, int n_kv, int dim) {
-  Cut c;
+static Layout attn_layout(int n_seq, int max_window, int max_len, int group, int n_kv, int dim) {
+  Layout l;
   const long long rows = static_cast<long long>(max_window) * group;
-  c.block_rows = rows > 128 ? 256 : rows > 16 ? 32 : 16;
-  c.row_blocks = static_cast<int>((rows + c.block_rows - 1) / c.block_rows);
-  const long long keys = static_cast<long long>(max_len) + max_window;
-  const long long most = (keys + kKeys - 1) / kKeys;
-  const long long units = static_cast<long long>(n_seq) * n_kv * c.row_blocks;
-  const long long slots = 256 * (dim == 256 || c.block_rows == 256 ? 1 : 2) * (n_seq > 1 ? 2 : 1);
-  long long n = units >= slots ? 1 : slots / units;
-  if (n > most) n = most;
-  c.split_keys = static_cast<int>((most + n - 1) / n * kKeys);
-  c.n_split = static_cast<int>((keys + c.split_keys - 1) / c.split_keys);
-  return c;
-}
-static size_t part_bytes(const Cut& c, int n_tokens, int n_heads, int dim) {
-  if (c.n_split == 1) return 0;
-  return static_cast<size_t>(c.n_split) * n_tokens * n_heads * (dim * 4 + 8);
+  l.block_rows = rows > 128 ? 256 : rows > 16 ? 32 : 16;
+  l.row_blocks = static_cast<int>((rows + l.block_rows - 1) / l.block_rows);
+  const long long units = static_cast<long long>(n_seq) * n_kv;
+  const long long most = (static_cast<long long>(max_len) + max_window + kKeys - 1) / kKeys;
+  // workgroups that the card holds at once (by their LDS), and units: a unit's
+  // row blocks are on one of the 8 XCDs, and 11 units of three on the 32 CUs of
+  // an XCD would take two rounds
+  const int each = dim == 256 || l.block_rows == 256 ? 1 : dim == 128 ? 2 : 4;
+  const long long slots = 256 * each;
+  const long long per = 32 * each >= l.row_blocks ? 32 * each / l.row_blocks * 8 : 8;
+  l.cut = most > 1 && (units < slots || most > 8);
+  l.least_cut = most > 1 ? static_cast<int>((slots - 1) / n_kv) : 0;
+  long long n = units;
+  if (l.cut) n = (2 * units + per - 1) / per * per;
+  l.max_units = n > 0x7FFFFF00 ? 0x7FFFFF00 : static_cast<int>(n);
+  const size_t part_rows =
+      static_cast<size_t>((l.max_units + 7LL) / 8 * 8) * l.row_blocks * l.block_rows;
+  l.plan_bytes = l.cut ? (static_cast<size_t>(n_seq) * sizeof(int2) + 15) / 16 * 16 : 0;
+  l.o_bytes = l.cut ? part_rows * dim * sizeof(float) : 0;
+  l.bytes = l.plan_bytes + l.o_bytes + (l.cut ? part_rows * sizeof(float2) : 0);
+  return l;
 }
 
 template <int D>
-static int attn_launch(const AttnArgs& a, const Cut& c, int n_seq, hipStream_t s, const char* nm) {
-  const unsigned grid = static_cast<unsigned>((a.units + 7LL) / 8 * 8 * c.row_blocks);
-  if (c.block_rows == 256)
-    hipLaunchKernelGGL(attn_rows_kernel<D>, dim3(grid), dim3(64 * kRowWaves), RowsLds<D>::kBytes, s,
-                       a);
-  else if (c.block_rows == 32)
-    hipLaunchKernelGGL((attn_few_kernel<D, 2>), dim3(grid), dim3(256), (FewLds<D, 2>::kBytes), s, a);
+static int attn_launch(const AttnArgs& a, hipStream_t s, const char* nm) {
+  const dim3 grid(static_cast<unsigned>((a.max_units + 7LL) / 8 * 8 * a.row_blocks));
+  if (a.block_rows == 256)
+    hipLaunchKernelGGL(attn_rows_kernel<D>, grid, dim3(64 * kRowWaves), RowsLds<D>::kBytes, s, a);
+  else if (a.block_rows == 32)
+    hipLaunchKernelGGL((attn_few_kernel<D, 2>), grid, dim3(256), (FewLds<D, 2>::kBytes), s, a);
   else
-    hipLaunchKernelGGL((attn_few_kernel<D, 1>), dim3(grid), dim3(256), (FewLds<D, 1>::kBytes), s, a);
+    hipLaunchKernelGGL((attn_few_kernel<D, 1>), grid, dim3(256), (FewLds<D, 1>::kBytes), s, a);
   if (int st = check_launch(nm)) return st;
-  if (c.n_split > 1) {
-    hipLaunchKernelGGL(attn_join_kernel<D>, dim3(n_seq * a.max_window * a.n_heads), dim3(256), 0, s,
-                       a);
+  if (a.cut) {
+    hipLaunchKernelGGL(attn_join_kernel<D>, dim3(a.n_seq * a.max_window * a.n_heads), dim3(256), 0,
+                       s, a);
     return check_launch(nm);
   }
   return SG_OK;
@@ -934,21 +1035,18 @@ static int attn_launch(const AttnArgs& a, const Cut& c, int n_seq, hipStream_t s
 
 extern "C" {
 
-size_t sg_attn_tree_workspace_bytes(int n_seq, int n_tokens, int max_window, int max_len,
-                                    int n_heads, int n_kv_heads, int head_dim) {
-  if (n_seq <= 0 || n_tokens <= 0 || max_window <= 0 || max_len < 0 || n_kv_heads <= 0 ||
+size_t sg_attn_tree_workspace_bytes(int n_seq, int max_window, int max_len, int n_heads,
+                                    int n_kv_heads, int head_dim) {
+  if (n_seq <= 0 || max_window <= 0 || max_len < 0 || n_kv_heads <= 0 ||
       n_heads <= 0 || n_heads % n_kv_heads != 0)
     return 0;
-  // enough for every smaller batch too: fewer sequences are cut into more parts
-  size_t most = 0;
-  for (int s = 1; s <= n_seq; ++s) {
-    const sg::Cut c =
-        sg::attn_cut(s, max_window, max_len, n_heads / n_kv_heads, n_kv_heads, head_dim);
-    const size_t b = sg::part_bytes(c, n_tokens, n_heads, head_dim);
-    if (b > most) most = b;
-    if (c.n_split == 1) break;
-  }
-  return most;
+  // Enough for every smaller batch too: fewer sequences have no more units, but
+  // may be cut where more are not.
+  const int group = n_heads / n_kv_heads;
+  const sg::Layout l = sg::attn_layout(n_seq, max_window, max_len, group, n_kv_heads, head_dim);
+  if (l.cut || l.least_cut <= 0) return l.bytes;
+  return sg::attn_layout(l.least_cut < n_seq ? l.least_cut : n_seq, max_window, max_len, group,
+                         n_kv_heads, head_dim).bytes;
 }
 
 int sg_attn_tree_f16(const uint16_t* q, const uint16_t* k, const uint16_t* v, long long q_stride,
@@ -973,15 +1071,14 @@ int sg_attn_tree_f16(const uint16_t* q, const uint16_t* k, const uint16_t* v, lo
   if (q_stride < static_cast<long long>(n_heads) * dim ||
       k_stride < static_cast<long long>(n_kv) * dim || v_stride < static_cast<long long>(n_kv) * dim)
     return set_error(SG_ERR_GEOMETRY, "%s: a token stride is less than a token", nm);
-  const Cut c = attn_cut(n_seq, max_window, max_len, n_heads / n_kv, n_kv, dim);
-  const size_t need = part_bytes(c, n_tokens, n_heads, dim);
-  if (need && (!ws || ws_bytes < need || reinterpret_cast<uintptr_t>(ws) % 16))
-    return set_error(SG_ERR_INVALID_ARGUMENT, "%s: the workspace needs %zu bytes, 16-B aligned", nm,
-                     need);
-  const long long units = static_cast<long long>(n_seq) * n_kv * c.n_split;
+  const long long units = static_cast<long long>(n_seq) * n_kv;
   const long long join = static_cast<long long>(n_seq) * max_window * n_heads;
-  if ((units + 8) * c.row_blocks > 0x7FFFFFFF || join > 0x7FFFFFFF)
+  if (units * (max_window * (n_heads / n_kv) / 16 + 1) > 0x7FFFFFF || join > 0x7FFFFFFF)
     return set_error(SG_ERR_UNSUPPORTED, "%s: too many sequences", nm);
+  const Layout l = attn_layout(n_seq, max_window, max_len, n_heads / n_kv, n_kv, dim);
+  if (l.bytes && (!ws || ws_bytes < l.bytes || reinterpret_cast<uintptr_t>(ws) % 16))
+    return set_error(SG_ERR_INVALID_ARGUMENT, "%s: the workspace needs %zu bytes, 16-B aligned", nm,
+                     l.bytes);
   AttnArgs a;
   a.q = q;
   a.k = k;
@@ -996,9 +1093,11 @@ int sg_attn_tree_f16(const uint16_t* q, const uint16_t* k, const uint16_t* v, lo
   a.win_off = win_off;
   a.parent = parent;
   a.out = out;
-  a.part_o = static_cast<float*>(ws);
-  a.part_ml = reinterpret_cast<float2*>(
-      a.part_o + static_cast<size_t>(c.n_split) * n_tokens * n_heads * dim);
+  unsigned char* const w = static_cast<unsigned char*>(ws);
+  a.seq_plan = reinterpret_cast<int2*>(w);
+  a.part_o = reinterpret_cast<float*>(w + l.plan_bytes);
+  a.part_ml = reinterpret_cast<float2*>(w + l.plan_bytes + l.o_bytes);
+  a.n_seq = n_seq;
   a.n_tokens = n_tokens;
   a.max_window = max_window;
   a.n_heads = n_heads;
@@ -1007,15 +1106,15 @@ int sg_attn_tree_f16(const uint16_t* q, const uint16_t* k, const uint16_t* v, lo
   a.n_pages = cache->n_pages;
   a.page_log2 = log2_of(cache->page_size);
   a.pages_per_seq = cache->pages_per_seq;
-  a.n_split = c.n_split;
-  a.split_keys = c.split_keys;
-  a.row_blocks = c.row_blocks;
-  a.units = static_cast<int>(units);
+  a.row_blocks = l.row_blocks;
+  a.block_rows = l.block_rows;
+  a.max_units = l.max_units;
+  a.cut = l.cut;
   a.scale_log2 = scale * kLog2e;
   const hipStream_t s = static_cast<hipStream_t>(stream);
-  if (dim == 64) return attn_launch<64>(a, c, n_seq, s, nm);
-  if (dim == 128) return attn_launch<128>(a, c, n_seq, s, nm);
-  return attn_launch<256>(a, c, n_seq, s, nm);
+  if (dim == 64) return attn_launch<64>(a, s, nm);
+  if (dim == 128) return attn_launch<128>(a, s, nm);
+  return attn_launch<256>(a, s, nm);
 }
 
 int sg_kv_commit_f16(const uint16_t* k, const uint16_t* v, long long k_stride, long long v_stride,

@@ -693,8 +693,8 @@ class TreeAttention:
         self.n_heads, self.n_kv_heads, self.head_dim = n_heads, n_kv_heads, head_dim
         self.max_tokens, self.max_seqs = max_tokens, max_seqs
         self.max_window, self.max_len = max_window, max_len
-        nbytes = load().sg_attn_tree_workspace_bytes(max_seqs, max_tokens, max_window, max_len,
-                                                     n_heads, n_kv_heads, head_dim)
+        nbytes = load().sg_attn_tree_workspace_bytes(max_seqs, max_window, max_len, n_heads,
+                                                     n_kv_heads, head_dim)
         self.workspace = torch.empty(nbytes, dtype=torch.uint8, device=device)
 
     def forward(self, q, k, v, cache, win_off, parent=None, layer=0, scale=None, out=None,

@@ -84,12 +84,13 @@ def test_attention_refusals(lib):
 
 def test_attention_workspace(lib):
     f = lib.sg_attn_tree_workspace_bytes
-    assert f(0, 1, 1, 1, 1, 1, 64) == 0 and f(1, 1, 1, 1, 3, 2, 64) == 0
-    one = f(1, 4, 4, 100000, 16, 2, 256)
-    assert one > 0
+    assert f(0, 1, 1, 1, 1, 64) == 0 and f(1, 1, 1, 3, 2, 64) == 0
+    assert f(1, 4, 100000, 16, 2, 256) > 0
     # what is enough for a batch is enough for a smaller one
-    for n in range(1, 40):
-        assert f(n, 160, 4, 100000, 16, 2, 256) >= f(max(1, n - 1), 160, 4, 100000, 16, 2, 256)
+    for max_len in (0, 100, 500, 100000):
+        for args in ((4, max_len, 16, 2, 256), (1, max_len, 32, 8, 128), (64, max_len, 7, 7, 64)):
+            for n in range(2, 400):
+                assert f(n, *args) >= f(n - 1, *args)
 
 
 def test_commit_refusals(lib):
