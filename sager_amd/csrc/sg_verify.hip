@@ -274,29 +274,29 @@ __device__ __forceinline__ double rest_sum(const VerifyArgs& a, long long row, i
   for (int c = lane; c < a.n_chunks; c += 64) s += a.rest[row * a.n_chunks + c];
   return wave_sum(s);
 }
-// The target's probability of token v (logit x) in a row.
-__device__ __forceinline__ double target_p(RowStat r, float x, int v, bool sampled, double k) {
+// The target's probability of token v (logit x) in a row; inv: 1 / r.s.
+__device__ __forceinline__ double target_p(RowStat r, double inv, float x, int v, bool sampled,
+                                           double k) {
   if (!sampled) return static_cast<double>(v) == r.s ? 1.0 : 0.0;
-  return r.m > -INFINITY ? weight(no_nan(x), r.m, k) / r.s : 0.0;
+  return r.m > -INFINITY ? weight(x, r.m, k) * inv : 0.0;
 }
 
-// The siblings of rank 0 .. n-1 below a node: rows and the sums of their rests.
+// The siblings of rank 0 .. n-1 below a node: rows, and one over the sums of
+// their rests (0: less than kRest, which counts as none).
 struct Chain {
   int row[kMaxChildren];
-  double sum[kMaxChildren];
+  double inv[kMaxChildren];
 };
 // R(v) after the rejection of the first n siblings, normalized by the last
 // rest that counts.  r: the target's probability.
 __device__ __forceinline__ double chain_rest(const VerifyArgs& a, const Chain& ch, int n, double r,
                                              int v) {
-  double s = 1.0;
   for (int i = 0; i < n; ++i) {
-    if (ch.sum[i] < kRest) continue;
+    if (ch.inv[i] == 0.0) continue;
     const double q = a.draft[static_cast<long long>(ch.row[i]) * a.vocab + v];
-    r = fmax(r / s - q, 0.0);
-    s = ch.sum[i];
+    r = fmax(r - q, 0.0) * ch.inv[i];
   }
-  return r / s;
+  return r;
 }
 
 // Grid: (chunk, node, sequence), for the children of rank `rank`.
@@ -336,19 +336,33 @@ __global__ void __launch_bounds__(256) verify_rest_kernel(const VerifyArgs a, in
         const double r = rest_sum(a, row, lane);
         if (lane == 0) {
           ch.row[i] = row;
-          ch.sum[i] = r;
+          ch.inv[i] = r < kRest ? 0.0 : 1.0 / r;
         }
       }
   }
   __syncthreads();
-  double sum = 0.0;
-#pragma unroll 4
-  for (int i = 0; i < kEach; ++i) {
-    const int v = c * kChunk + i * 256 + threadIdx.x;
-    if (v < a.vocab)
-      sum += fmax(chain_rest(a, ch, rank, target_p(rs, xv[i], v, sampled, k), v) -
-                      static_cast<double>(qv[i]), 0.0);
+  const RowStat st = rs;
+  const double inv = 1.0 / st.s;
+  double p[kEach];
+#pragma unroll
+  for (int i = 0; i < kEach; ++i)
+    p[i] = target_p(st, inv, xv[i], c * kChunk + i * 256 + threadIdx.x, sampled, k);
+  for (int j = 0; j < rank; ++j) {  // a sibling's row at a time, its loads together
+    const double jnv = ch.inv[j];
+    if (jnv == 0.0) continue;
+    const float* qj = a.draft + static_cast<long long>(ch.row[j]) * a.vocab;
+    float o[kEach];
+#pragma unroll
+    for (int i = 0; i < kEach; ++i) {
+      const int v = c * kChunk + i * 256 + threadIdx.x;
+      o[i] = v < a.vocab ? qj[v] : 0.f;
+    }
+#pragma unroll
+    for (int i = 0; i < kEach; ++i) p[i] = fmax(p[i] - static_cast<double>(o[i]), 0.0) * jnv;
   }
+  double sum = 0.0;  // (past the vocabulary x is -infinity and q 0)
+#pragma unroll
+  for (int i = 0; i < kEach; ++i) sum += fmax(p[i] - static_cast<double>(qv[i]), 0.0);
   sum = wave_sum(sum);
   if (lane == 0) ss[wave] = sum;
   __syncthreads();
@@ -450,17 +464,22 @@ __global__ void __launch_bounds__(kWalk) verify_walk_kernel(const VerifyArgs a) 
       }
     }
   }
-  if (a.draft)
-    for (int i = wave; i < w.n; i += kWalk / 64) {
-      const double rest = a.nodes[w.off + i].up >= 0 ? rest_sum(a, w.off + i, lane) : 0.0;
-      if (lane == 0) left[i] = rest;
+  if (a.draft)  // (of nodes that are nobody's child, whatever lies there: it is not used)
+#pragma unroll
+    for (int j = 0; j < kRounds; ++j) {
+      const int i = wave + j * (kWalk / 64);
+      if (i < w.n) {
+        const double rest = rest_sum(a, w.off + i, lane);
+        if (lane == 0) left[i] = rest;
+      }
     }
   __syncthreads();
   if (wave == 0) {
     const bool in = n.up >= 0;
     const int up = in ? n.up : 0;
     // R of the node's token at its parent, R's mass there, the bar u has to stay under
-    double r = in && n.tok >= 0 ? target_p(stat[up], n.x, n.tok, sampled, k) : 0.0;
+    double r =
+        in && n.tok >= 0 ? target_p(stat[up], 1.0 / stat[up].s, n.x, n.tok, sampled, k) : 0.0;
     double m = mass[up], q = 1.0;
     if (a.draft) {
       q = n.q;
@@ -513,7 +532,7 @@ __global__ void __launch_bounds__(kWalk) verify_walk_kernel(const VerifyArgs a) 
       kid_tok[n.rank] = left[lane] > 0.0 ? n.tok : -1;
       if (a.draft) {
         chain.row[n.rank] = w.off + lane;
-        chain.sum[n.rank] = left[lane];
+        chain.inv[n.rank] = left[lane] < kRest ? 0.0 : 1.0 / left[lane];
       }
     }
     if (lane == 0) {
@@ -538,9 +557,9 @@ __global__ void __launch_bounds__(kWalk) verify_walk_kernel(const VerifyArgs a) 
   int from = -1;  // the rejected child whose rest is what is left
   if (a.draft)
     for (int i = 0; i < nk; ++i)
-      if (chain.sum[i] >= kRest) {
+      if (chain.inv[i] != 0.0) {
         from = chain.row[i];
-        total = chain.sum[i];
+        total = left[from - w.off];
       }
   const double goal = static_cast<double>(us) * total;
   // its chunk
@@ -587,8 +606,9 @@ __global__ void __launch_bounds__(kWalk) verify_walk_kernel(const VerifyArgs a) 
     for (int i = 0; i < 4; ++i) {
       const int v = v0 + i;
       if (a.draft && from >= 0) {  // (the rest as it was summed: not normalized)
-        r[i] = v < a.vocab ? chain_rest(a, chain, nk, target_p(st, xv[i], v, true, k), v) * total
-                           : 0.0;
+        r[i] = v < a.vocab
+                   ? chain_rest(a, chain, nk, target_p(st, 1.0 / st.s, xv[i], v, true, k), v) * total
+                   : 0.0;
       } else {
         r[i] = weight(xv[i], st.m, k);
         if (!a.draft)
