@@ -348,6 +348,18 @@ struct Part {
       q[s] = __builtin_bit_cast(h8, w);
     }
   }
+  // Waits for Q before the loop: left to the compiler, the waits stand at Q's
+  // uses inside it, where they wait for the copies just issued as well. Over
+  // many steps that costs (a tree of 64 over 131,071 tokens: 194 us against
+  // 189); the small blocks do few steps, and there the first step's start
+  // weighs more (four tokens over 4,096: 15.2 us against 15.8 with it).
+  template <int RT>
+  static __device__ __forceinline__ void settle_q(h8 (&q)[RT][KK]) {
+#pragma unroll
+    for (int rt = 0; rt < RT; ++rt)
+#pragma unroll
+      for (int s = 0; s < KK; ++s) asm volatile("" : "+v"(q[rt][s]));
+  }
   // Piece st * 4 + grp of K's row col of a 16-key block; at: k_offset plus
   // the block's place, multiples of 256 B.
   __device__ __forceinline__ uint32_t k_offset() const {
@@ -672,6 +684,7 @@ __global__ void __launch_bounds__(64 * kRowWaves) attn_rows_kernel(const AttnArg
   // which of a step's keys are there, by step parity and block of 16
   uint16_t* there_of = reinterpret_cast<uint16_t*>(lds + L::kThere);
 
+  P::settle_q(qf);
   bar();  // the flags are cleared
   for (; step < t.end; ++step) {
     const int par = step & 1;
