@@ -508,7 +508,7 @@ int sg_scatter_rows_f16(uint16_t* dst, const uint16_t* src, const int* dst_rows,
  * NULL: every window is a chain. */
 
 /* Residual addition, RMS norm and Q8_K in one launch, n_rows rows of n
- * (a multiple of 256, at most 16384):
+ * (a multiple of 256, at most 16384; n_rows is below 2^22):
  *   r = x + y, rounded to the buffers' type and stored to x_out;
  *   xn = (r / sqrt(mean(r^2) + eps)) * w, rounded likewise (xn may be NULL);
  *   xq = Q8_K(xn), as sg_quantize_q8_k / _f16 make it (xq may be NULL).
@@ -545,7 +545,8 @@ typedef struct sg_kv_cache {
  *   out[t][h] = sum_j p_j v_j,  p = softmax over j of scale * q[t][h] . k_j,
  * j running over the sequence's cached tokens and, in the window, over t's
  * ancestors and t itself; head h reads kv head h / (n_heads / n_kv_heads).
- * A node that is absent gets 0.  q [n_tokens][n_heads][head_dim], k and v
+ * A node that is absent gets 0, and so does one that sees no score above
+ * -infinity.  q [n_tokens][n_heads][head_dim], k and v
  * [n_tokens][n_kv_heads][head_dim] with q_stride, k_stride and v_stride
  * elements from one token to the next (slices of one projection's output),
  * out contiguous.  k, v, the cache's k and v and their strides are 16-B
@@ -579,8 +580,8 @@ int sg_kv_commit_f16(const uint16_t* k, const uint16_t* v, long long k_stride, l
 /* Which drafts the target's probabilities accept, from given random numbers.
  * logits [n_tokens][vocab] fp32 are the target's after each node, p their
  * softmax at the sequence's temperature (0, negative or NaN: all on the
- * largest logit, the lowest index among equals; a NaN logit counts as
- * -infinity).  tokens [n_tokens]: the node's token.  draft_probs [n_tokens]
+ * largest logit, the lowest index among equals; below 2^-126 it counts as
+ * 2^-126; a NaN logit counts as -infinity).  tokens [n_tokens]: the node's token.  draft_probs [n_tokens]
  * [vocab] fp32: the distribution that the node's token was drawn from, NULL:
  * the token was chosen, q is 1 on it.  From the root on: with R = p of the
  * node, its children c in index order are tried; c is accepted if

@@ -125,7 +125,9 @@ __device__ __forceinline__ bool find_unit(const AttnArgs& a, int unit, int lane,
         Window w;
         sum += __builtin_amdgcn_readlane(wave_run_sum_i(steps_of(a, s, &l, &w)), 63);
       }
-      const long long free = a.max_units - static_cast<long long>(a.n_seq) * a.n_kv;
+      // (one in a thousand less than there are: parts_of rounds)
+      long long free = a.max_units - static_cast<long long>(a.n_seq) * a.n_kv;
+      free -= free >> 10;
       part = max(1, static_cast<int>(min((sum * a.n_kv + free - 1) / free, 0x7FFFFFFFLL)));
     }
   }
@@ -1086,7 +1088,9 @@ int sg_attn_tree_f16(const uint16_t* q, const uint16_t* k, const uint16_t* v, lo
     return set_error(SG_ERR_GEOMETRY, "%s: a token stride is less than a token", nm);
   const long long units = static_cast<long long>(n_seq) * n_kv;
   const long long join = static_cast<long long>(n_seq) * max_window * n_heads;
-  if (units * (max_window * (n_heads / n_kv) / 16 + 1) > 0x7FFFFFF || join > 0x7FFFFFFF)
+  const long long rows = static_cast<long long>(max_window) * (n_heads / n_kv);
+  // a launch has less than 2^32 threads, two units to a kv head
+  if (units * (rows / 16 + 1) > 0x1FFFFF || join > 0xFFFFFF)
     return set_error(SG_ERR_UNSUPPORTED, "%s: too many sequences", nm);
   const Layout l = attn_layout(n_seq, max_window, max_len, n_heads / n_kv, n_kv, dim);
   if (l.bytes && (!ws || ws_bytes < l.bytes || reinterpret_cast<uintptr_t>(ws) % 16))

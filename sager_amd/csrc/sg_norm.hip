@@ -144,8 +144,9 @@ static int norm_launch(const T* x, const T* y, T* x_out, const float* w, float e
   if (n <= 0 || n % kQK != 0 || n_rows <= 0)
     return set_error(SG_ERR_GEOMETRY, "%s: n=%d must be a positive multiple of 256, n_rows=%d",
                      nm, n, n_rows);
-  if (n > 64 * kQK)
-    return set_error(SG_ERR_UNSUPPORTED, "%s: n=%d is over %d", nm, n, 64 * kQK);
+  if (n > 64 * kQK || n_rows >= 1 << 22)  // (a launch has less than 2^32 threads)
+    return set_error(SG_ERR_UNSUPPORTED, "%s: n=%d is over %d, or n_rows=%d over 2^22 - 1", nm, n,
+                     64 * kQK, n_rows);
   if (reinterpret_cast<uintptr_t>(xq) % 4 || reinterpret_cast<uintptr_t>(x) % sizeof(T) ||
       reinterpret_cast<uintptr_t>(y) % sizeof(T) || reinterpret_cast<uintptr_t>(x_out) % sizeof(T) ||
       reinterpret_cast<uintptr_t>(xn) % sizeof(T) || reinterpret_cast<uintptr_t>(w) % 4)

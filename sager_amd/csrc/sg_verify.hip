@@ -27,6 +27,11 @@ constexpr double kRest = 0x1p-30; // a smaller share of the mass counts as none
 
 typedef float f32x4_u __attribute__((ext_vector_type(4), aligned(4)));
 
+// log2(e) / t.  A subnormal temperature counts as the least normal one: the
+// factor has to be an fp32 number too.
+__device__ __forceinline__ double per_temperature(float t) {
+  return 1.4426950408889634074 / static_cast<double>(fmaxf(t, 0x1p-126f));
+}
 __device__ __forceinline__ float no_nan(float x) { return x == x ? x : -INFINITY; }
 
 // The weight 2^((x - m) c) of logit x under the row's (or chunk's) largest m,
@@ -177,7 +182,7 @@ __global__ void __launch_bounds__(256) verify_rows_kernel(const VerifyArgs a) {
   }
   const float t = a.temperature[s];
   const bool sampled = t > 0.f;
-  const double k = sampled ? 1.4426950408889634074 / static_cast<double>(t) : 1.0;
+  const double k = sampled ? per_temperature(t) : 1.0;
   __shared__ float sm[4];
   __shared__ double ss[4];
   float m = -INFINITY;  // (fmaxf passes a NaN over)
@@ -300,7 +305,8 @@ __device__ __forceinline__ double chain_rest(const VerifyArgs& a, const Chain& c
 }
 
 // Grid: (chunk, node, sequence), for the children of rank `rank`.
-__global__ void __launch_bounds__(256) verify_rest_kernel(const VerifyArgs a, int rank) {
+// (at most 128 registers: four workgroups a CU.)
+__global__ void __launch_bounds__(256, 4) verify_rest_kernel(const VerifyArgs a, int rank) {
   const int s = blockIdx.z, node = blockIdx.y, c = blockIdx.x;
   const Window w = window_of(a.win_off, s, a.n_tokens, a.max_window);
   if (node >= w.n) return;
@@ -319,7 +325,7 @@ __global__ void __launch_bounds__(256) verify_rest_kernel(const VerifyArgs a, in
   }
   const float t = a.temperature[s];
   const bool sampled = t > 0.f;
-  const double k = sampled ? 1.4426950408889634074 / static_cast<double>(t) : 1.0;
+  const double k = sampled ? per_temperature(t) : 1.0;
   __shared__ Chain ch;
   __shared__ RowStat rs;
   __shared__ double ss[4];
@@ -436,7 +442,7 @@ __global__ void __launch_bounds__(kWalk) verify_walk_kernel(const VerifyArgs a) 
   const float t = a.temperature[s];
   const float us = a.u_sample[s];
   const bool sampled = t > 0.f;
-  const double k = sampled ? 1.4426950408889634074 / static_cast<double>(t) : 1.0;
+  const double k = sampled ? per_temperature(t) : 1.0;
   Node n;
   n.up = -1;
   n.rank = 0;

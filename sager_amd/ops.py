@@ -557,20 +557,27 @@ class MoePrefill(MoeLayer):
 # (win_off int32 [n_seq + 1]); parent (int32, one per row, or None for chains)
 # makes a window a tree of drafts.  include/sager_hip.h has the rules.
 
-def _arg(fn, name, t, dtype, shape):
-    """The address of a contiguous GPU tensor of that type and shape."""
-    if t.dtype is not dtype or t.shape != shape or not t.is_cuda or not t.is_contiguous():
-        raise SagerError(f"{fn}: {name} must be {dtype} {tuple(shape)}, contiguous on the GPU, got "
-                         f"{t.dtype} {tuple(t.shape)} on {t.device}")
+def _arg(fn, name, t, dtype, shape, dev):
+    """The address of a contiguous tensor of that type and shape on GPU dev."""
+    if t.dtype is not dtype or t.shape != shape or t.get_device() != dev or not t.is_contiguous():
+        raise SagerError(f"{fn}: {name} must be {dtype} {tuple(shape)}, contiguous on GPU {dev}, "
+                         f"got {t.dtype} {tuple(t.shape)} on {t.device}")
     return t.data_ptr()
 
 
-def _current_stream_of(fn, t):
-    """The current stream, of the current device, which has to be t's: the launch goes there."""
+def _current_of(fn, t):
+    """The current device, which has to be t's, and its current stream: the launch goes there."""
     dev = t.get_device()
     if dev < 0 or dev != torch._C._cuda_getDevice():
         raise SagerError(f"{fn}: {t.device} is not the current GPU")
-    return torch._C._cuda_getCurrentRawStream(dev)
+    return dev, torch._C._cuda_getCurrentRawStream(dev)
+
+
+def _space(fn, ws, dev):
+    """The address and the bytes of a workspace."""
+    if ws.get_device() != dev or not ws.is_contiguous():
+        raise SagerError(f"{fn}: the workspace must be contiguous on GPU {dev}, is on {ws.device}")
+    return ws.data_ptr(), ws.nbytes
 
 
 def add_rmsnorm_q8_k(x, w, eps, y=None, x_out=None, xn=None, xq=None):
@@ -586,8 +593,8 @@ def add_rmsnorm_q8_k(x, w, eps, y=None, x_out=None, xn=None, xq=None):
         entry = load().sg_add_rmsnorm_q8_k
     else:
         raise SagerError("x must be fp32 or fp16")
-    stream = _current_stream_of(fn, x)
-    n = shape[-1]
+    dev, stream = _current_of(fn, x)
+    n = shape[-1] if shape else 0
     rows = x.numel() // n if n else 0
     if xn is None and xq is None:
         xn, xq = torch.empty_like(x), q8k_empty(rows, n, x.device)
@@ -595,47 +602,48 @@ def add_rmsnorm_q8_k(x, w, eps, y=None, x_out=None, xn=None, xq=None):
     if y is not None:
         if x_out is None:
             x_out = torch.empty_like(x)
-        py, po = _arg(fn, "y", y, dt, shape), _arg(fn, "x_out", x_out, dt, shape)
+        py, po = _arg(fn, "y", y, dt, shape, dev), _arg(fn, "x_out", x_out, dt, shape, dev)
     elif x_out is not None:
         raise SagerError("x_out needs y")
     if xn is not None:
-        pn = _arg(fn, "xn", xn, dt, shape)
+        pn = _arg(fn, "xn", xn, dt, shape, dev)
     if xq is not None:
         if xq.numel() != rows * (n // QK) * Q8K_BYTES:
             raise SagerError("xq must hold n/256 Q8_K blocks a row")
-        pq = _arg(fn, "xq", xq, torch.uint8, xq.shape)
-    _check(entry(_arg(fn, "x", x, dt, shape), py, po, _arg(fn, "w", w, torch.float32, (n,)), eps, pn,
-                 pq, n, rows, stream))
+        pq = _arg(fn, "xq", xq, torch.uint8, xq.shape, dev)
+    _check(entry(_arg(fn, "x", x, dt, shape, dev), py, po,
+                 _arg(fn, "w", w, torch.float32, (n,), dev), eps, pn, pq, n, rows, stream))
     return x if y is None else x_out, xn, xq
 
 
-def _rows(fn, name, t, shape):
+def _rows(fn, name, t, shape, dev):
     """The address and the leading dimensions' strides (elements) of an fp16
     tensor [..., tokens, heads, dim] whose tokens may lie apart."""
     st, (heads, dim) = t.stride(), shape[-2:]
-    if t.dtype is not torch.float16 or t.shape != shape or not t.is_cuda or st[-1] != 1 or \
+    if t.dtype is not torch.float16 or t.shape != shape or t.get_device() != dev or st[-1] != 1 or \
             (heads > 1 and st[-2] != dim):
-        raise SagerError(f"{fn}: {name} must be fp16 {tuple(shape)} on the GPU, a token's values "
+        raise SagerError(f"{fn}: {name} must be fp16 {tuple(shape)} on GPU {dev}, a token's values "
                          f"contiguous, got {t.dtype} {tuple(t.shape)} strides {st} on {t.device}")
     # (a dimension of one element has any stride)
     return (t.data_ptr(), *[x if n > 1 else max(x, heads * dim) for n, x in zip(shape[:-2], st)])
 
 
-def _windows(fn, win_off, parent, n_tokens):
+def _windows(fn, win_off, parent, n_tokens, dev):
     """The number of sequences and the addresses of win_off and parent."""
     n_seq = win_off.numel() - 1
     if n_seq < 1:
         raise SagerError(f"{fn}: win_off must be [n_seq + 1]")
-    off = _arg(fn, "win_off", win_off, torch.int32, (n_seq + 1,))
+    off = _arg(fn, "win_off", win_off, torch.int32, (n_seq + 1,), dev)
     if parent is None:
         return n_seq, off, None
-    return n_seq, off, _arg(fn, "parent", parent, torch.int32, (n_tokens,))
+    return n_seq, off, _arg(fn, "parent", parent, torch.int32, (n_tokens,), dev)
 
 
 class KvCache:
     """A paged fp16 key/value cache: k, v [n_layers, n_pages, n_kv_heads,
     page_size, head_dim], pages int32 [n_seq, pages_per_seq], length int32
-    [n_seq].  Holds the tensors; nothing is copied."""
+    [n_seq].  Holds the tensors; nothing is copied, and what changes between
+    steps changes in place (length.copy_(...), pages[s, i] = ...)."""
 
     def __init__(self, k, v, pages, length):
         if k.dim() != 5 or k.shape != v.shape:
@@ -647,6 +655,7 @@ class KvCache:
         _dtypes("KvCache", k=(k, torch.float16), v=(v, torch.float16), pages=(pages, torch.int32),
                 length=(length, torch.int32))
         self.k, self.v, self.pages, self.length = k, v, pages, length
+        self.device = k.get_device()
         self.n_layers, P, self.n_kv_heads, S, self.head_dim = k.shape
         self.max_seqs = pages.shape[0]
         self.desc = KvCacheDesc(_ptr(k), _ptr(v), _ptr(pages), _ptr(length), k[0].numel(),
@@ -661,21 +670,25 @@ class KvCache:
         of its own; the cache's own length is left to the caller, since every
         layer of a step still reads it)."""
         fn = "KvCache.commit"
-        n_tokens, window = k.shape[1], path.shape[-1]
+        if k.dim() != 4 or path.dim() != 2:
+            raise SagerError(f"{fn}: k must be [n_layers, n_tokens, n_kv_heads, head_dim], path "
+                             "[n_seq, max_window]")
+        n_tokens, window = k.shape[1], path.shape[1]
         shape = (self.n_layers, n_tokens, self.n_kv_heads, self.head_dim)
-        pk, kl, ks = _rows(fn, "k", k, shape)
-        pv, vl, vs = _rows(fn, "v", v, shape)
-        stream = _current_stream_of(fn, k)
-        n_seq, off, _ = _windows(fn, win_off, None, n_tokens)
-        if n_seq > self.max_seqs:
-            raise SagerError(f"{fn}: {n_seq} sequences, {self.max_seqs} in the cache")
+        dev, stream = _current_of(fn, k)
+        pk, kl, ks = _rows(fn, "k", k, shape, dev)
+        pv, vl, vs = _rows(fn, "v", v, shape, dev)
+        n_seq, off, _ = _windows(fn, win_off, None, n_tokens, dev)
+        if n_seq > self.max_seqs or self.device != dev:
+            raise SagerError(f"{fn}: {n_seq} sequences on GPU {dev}, the cache has "
+                             f"{self.max_seqs} on GPU {self.device}")
         if length_out is None:
             length_out = torch.empty(n_seq, dtype=torch.int32, device=k.device)
         _check(load().sg_kv_commit_f16(
-            pk, pv, ks, vs, kl, vl, self._desc, off, _arg(fn, "path", path, torch.int32,
-                                                          (n_seq, window)),
-            _arg(fn, "n_path", n_path, torch.int32, (n_seq,)),
-            _arg(fn, "length_out", length_out, torch.int32, (n_seq,)), n_seq, n_tokens, window,
+            pk, pv, ks, vs, kl, vl, self._desc, off,
+            _arg(fn, "path", path, torch.int32, (n_seq, window), dev),
+            _arg(fn, "n_path", n_path, torch.int32, (n_seq,), dev),
+            _arg(fn, "length_out", length_out, torch.int32, (n_seq,), dev), n_seq, n_tokens, window,
             stream))
         return length_out
 
@@ -704,22 +717,22 @@ class TreeAttention:
         contiguous; scale: 1/sqrt(head_dim) if None."""
         fn, T, D = "TreeAttention", q.shape[0], self.head_dim
         shape, kv_shape = (T, self.n_heads, D), (T, self.n_kv_heads, D)
-        pq, qs = _rows(fn, "q", q, shape)
-        pk, ks = _rows(fn, "k", k, kv_shape)
-        pv, vs = _rows(fn, "v", v, kv_shape)
-        stream = _current_stream_of(fn, q)
-        if cache.n_kv_heads != self.n_kv_heads or cache.head_dim != D:
-            raise SagerError("the cache has other heads")
-        n_seq, off, par = _windows(fn, win_off, parent, T)
+        dev, stream = _current_of(fn, q)
+        pq, qs = _rows(fn, "q", q, shape, dev)
+        pk, ks = _rows(fn, "k", k, kv_shape, dev)
+        pv, vs = _rows(fn, "v", v, kv_shape, dev)
+        if cache.n_kv_heads != self.n_kv_heads or cache.head_dim != D or cache.device != dev:
+            raise SagerError(f"the cache has other heads, or is not on GPU {dev}")
+        n_seq, off, par = _windows(fn, win_off, parent, T, dev)
         if T > self.max_tokens or n_seq > self.max_seqs or n_seq > cache.max_seqs:
             raise SagerError(f"{n_seq} sequences of {T} tokens: at most {self.max_seqs} of "
                              f"{self.max_tokens}, {cache.max_seqs} in the cache")
         if out is None:
             out = torch.zeros(shape, dtype=torch.float16, device=q.device)
-        ws = self.workspace if workspace is None else workspace
+        ws, ws_bytes = _space(fn, self.workspace if workspace is None else workspace, dev)
         _check(load().sg_attn_tree_f16(
             pq, pk, pv, qs, ks, vs, cache._desc, layer, off, par,
-            _arg(fn, "out", out, torch.float16, shape), _ptr(ws), ws.numel(), n_seq, T,
+            _arg(fn, "out", out, torch.float16, shape, dev), ws, ws_bytes, n_seq, T,
             self.max_window, self.max_len, self.n_heads, D ** -0.5 if scale is None else scale,
             stream))
         return out
@@ -745,30 +758,33 @@ class TreeVerify:
         (path int32 [n_seq, max_window], n_path int32 [n_seq], next_token
         int32 [n_seq], prob fp32 [n_tokens])."""
         fn, T, f32, i32 = "TreeVerify", logits.shape[0], torch.float32, torch.int32
-        stream = _current_stream_of(fn, logits)
-        n_seq, off, par = _windows(fn, win_off, parent, T)
+        dev, stream = _current_of(fn, logits)
+        n_seq, off, par = _windows(fn, win_off, parent, T, dev)
         if T > self.max_tokens or n_seq > self.max_seqs:
             raise SagerError(f"{n_seq} sequences of {T} rows: at most {self.max_seqs} of "
                              f"{self.max_tokens}")
-        dev, rows, seqs = logits.device, (T,), (n_seq,)
+        place, rows, seqs = logits.device, (T,), (n_seq,)
         full, paths = (T, self.vocab), (n_seq, self.max_window)
         if path is None:
-            path = torch.empty(paths, dtype=i32, device=dev)
+            path = torch.empty(paths, dtype=i32, device=place)
         if n_path is None:
-            n_path = torch.empty(n_seq, dtype=i32, device=dev)
+            n_path = torch.empty(n_seq, dtype=i32, device=place)
         if next_token is None:
-            next_token = torch.empty(n_seq, dtype=i32, device=dev)
+            next_token = torch.empty(n_seq, dtype=i32, device=place)
         if prob is None:
-            prob = torch.zeros(T, dtype=f32, device=dev)
-        ws = self.workspace if workspace is None else workspace
+            prob = torch.zeros(T, dtype=f32, device=place)
+        ws, ws_bytes = _space(fn, self.workspace if workspace is None else workspace, dev)
         _check(load().sg_tree_verify(
-            _arg(fn, "logits", logits, f32, full), _arg(fn, "tokens", tokens, i32, rows), off, par,
-            None if draft_probs is None else _arg(fn, "draft_probs", draft_probs, f32, full),
-            _arg(fn, "temperature", temperature, f32, seqs),
-            _arg(fn, "u_accept", u_accept, f32, rows), _arg(fn, "u_sample", u_sample, f32, seqs),
-            _arg(fn, "path", path, i32, paths), _arg(fn, "n_path", n_path, i32, seqs),
-            _arg(fn, "next_token", next_token, i32, seqs), _arg(fn, "prob", prob, f32, rows),
-            _ptr(ws), ws.numel(), n_seq, T, self.max_window, self.vocab, self.max_children, stream))
+            _arg(fn, "logits", logits, f32, full, dev), _arg(fn, "tokens", tokens, i32, rows, dev),
+            off, par,
+            None if draft_probs is None else _arg(fn, "draft_probs", draft_probs, f32, full, dev),
+            _arg(fn, "temperature", temperature, f32, seqs, dev),
+            _arg(fn, "u_accept", u_accept, f32, rows, dev),
+            _arg(fn, "u_sample", u_sample, f32, seqs, dev),
+            _arg(fn, "path", path, i32, paths, dev), _arg(fn, "n_path", n_path, i32, seqs, dev),
+            _arg(fn, "next_token", next_token, i32, seqs, dev),
+            _arg(fn, "prob", prob, f32, rows, dev),
+            ws, ws_bytes, n_seq, T, self.max_window, self.vocab, self.max_children, stream))
         return path, n_path, next_token, prob
 
 

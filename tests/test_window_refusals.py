@@ -176,3 +176,14 @@ def test_plain_attention_of_one_key_is_its_value():
                            np.array([-1, 5]), 1.0, 16, np.zeros((2, 1, 64)))
     np.testing.assert_array_equal(out[0], v[0].astype(float))
     assert (out[1] == 0).all()
+
+
+# ---- launches past what a grid holds ---------------------------------------------------
+
+def test_launches_too_large(lib):
+    for fn in (lib.sg_add_rmsnorm_q8_k_f16, lib.sg_add_rmsnorm_q8_k):
+        assert fn(*norm_args(rows=1 << 22)) == UNSUPPORTED
+    c = cache()
+    for kw in (dict(n_seq=1 << 20, max_window=4, n_heads=8), dict(n_seq=1 << 21, max_window=1),
+               dict(n_seq=1 << 15, max_window=64, n_heads=16, qs=2048)):
+        assert lib.sg_attn_tree_f16(*attn_args(c, **kw)) == UNSUPPORTED, kw
