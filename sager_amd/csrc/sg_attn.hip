@@ -34,6 +34,7 @@ typedef float f4 __attribute__((ext_vector_type(4)));
 typedef uint32_t u32x4_u __attribute__((ext_vector_type(4), aligned(2)));
 typedef short s4 __attribute__((ext_vector_type(4)));
 typedef __attribute__((address_space(3))) s4* lds_s4_p;
+typedef __attribute__((address_space(3))) unsigned char* lds_char_p;
 // read through the scalar cache, whatever is stored in between
 typedef const __attribute__((address_space(4))) int* const_int_p;
 
@@ -181,6 +182,13 @@ __device__ __forceinline__ void dma16_ptr(uint32_t lds, const void* src) {
                : "s"(__builtin_amdgcn_readfirstlane(lds)), "v"(src)
                : "memory");
 }
+// The larger of three, a NaN passed over (fmaxf twice, without the
+// canonicalization of its arguments that the compiler adds).
+__device__ __forceinline__ float max3(float a, float b, float c) {
+  float r;
+  asm("v_max3_f32 %0, %1, %2, %3" : "=v"(r) : "v"(a), "v"(b), "v"(c));
+  return r;
+}
 __device__ __forceinline__ bool fp16_odd(uint32_t b) { return (b & 0x7C00) == 0x7C00; }
 
 // What both kernels know of their part of the work.  K and V of step s lie at
@@ -209,8 +217,7 @@ struct Part {
   // reads the unit's keys once.
   __device__ __forceinline__ bool start(unsigned char* l) {
     lds = l;
-    lds0 = static_cast<uint32_t>(
-        reinterpret_cast<uintptr_t>((__attribute__((address_space(3))) unsigned char*)l));
+    lds0 = static_cast<uint32_t>(reinterpret_cast<uintptr_t>((lds_char_p)l));
     lane = threadIdx.x & 63;
     col = lane & 15;
     grp = lane >> 4;
@@ -254,37 +261,38 @@ struct Part {
   __device__ __forceinline__ bool plain(int s, int b, int page) const {
     return s * kKeys + 16 * b + 16 <= len && page_ok(page);
   }
-  // Brings keys 16 b.. of step s: K (kv 1), V (2) or both (3).
-  template <bool kAnew>
+  // Brings keys 16 b.. of step s: K and V (kBoth), or K (kv 1) or V (2).
+  // Row i * RPI + r of a copy (r < RPI: its lane's) has swz(i * RPI) ^ swz(r):
+  // every copy's offset is the first one's, one xor and one sum away.
+  template <bool kBoth>
   __device__ __forceinline__ void issue(int s, int b, int page, int kv) const {
     const int j = s * kKeys + 16 * b;
-    const uint32_t buf = lds0 + (s & 1) * 2 * kStep + b * 16 * D * 2 + (kv == 2 ? kStep : 0);
+    const bool v_only = !kBoth && kv == 2;
+    const uint32_t buf = lds0 + (s & 1) * 2 * kStep + b * 16 * D * 2 + (v_only ? kStep : 0);
     const long long at =
         (((static_cast<long long>(page) * a.n_kv + h) << a.page_log2) +
          (j & ((1 << a.page_log2) - 1))) * D;
-    const uint16_t* const c1 = kv == 2 ? a.vc : a.kc;
+    const uint16_t* const c1 = v_only ? a.vc : a.kc;
+    int ln = lane;
+    asm("" : "+v"(ln));  // (the offsets made anew: registers are short)
     if (plain(s, b, page)) {
       const uint16_t* b1 = uniform_ptr(c1 + at);
       const uint16_t* b2 = uniform_ptr(a.vc + at);
-      int ln = lane;
-      if (kAnew) asm("" : "+v"(ln));  // (the offsets made anew: registers are short)
+      const uint32_t off0 = (ln / CH) * (D * 2) + (((ln % CH) ^ swz<D>(ln / CH)) << 4);
 #pragma unroll
       for (int i = 0; i < NI; ++i) {
-        const int row = i * RPI + ln / CH;
-        const uint32_t off = row * (D * 2) + (((ln % CH) ^ swz<D>(row)) << 4);
+        const uint32_t off = (off0 ^ (swz<D>(i * RPI) << 4)) + i * 1024;
         dma16_base(buf + i * 1024, off, b1);
-        if (kv == 3) dma16_base(buf + kStep + i * 1024, off, b2);
+        if (kBoth) dma16_base(buf + kStep + i * 1024, off, b2);
       }
     } else if (j < total) {
       // rows of the cache, then of the window; what is not there reads a
       // window row and is masked
       const int n_cache = page_ok(page) ? min(len - j, 16) : 0;
       const kernarg_p ca = cold_args();
-      int ln = lane;
-      asm("" : "+v"(ln));
-      const uint16_t* const w1 = kv == 2 ? ca->v : ca->k;
+      const uint16_t* const w1 = v_only ? ca->v : ca->k;
       const uint16_t* const w2 = ca->v;
-      const long long ws1 = kv == 2 ? ca->v_stride : ca->k_stride, ws2 = ca->v_stride;
+      const long long ws1 = v_only ? ca->v_stride : ca->k_stride, ws2 = ca->v_stride;
 #pragma unroll 1
       for (int i = 0; i < NI; ++i) {
         const int row = i * RPI + ln / CH;
@@ -292,7 +300,7 @@ struct Part {
         const long long w = win.off + min(max(j + row - len, 0), win.n - 1);
         const bool cached = row < n_cache;
         dma16_ptr(buf + i * 1024, (cached ? c1 + at + row * D : w1 + w * ws1 + h * D) + c);
-        if (kv == 3)
+        if (kBoth)
           dma16_ptr(buf + kStep + i * 1024,
                     (cached ? a.vc + at + row * D : w2 + w * ws2 + h * D) + c);
       }
@@ -387,7 +395,7 @@ struct Part {
 #pragma unroll
     for (int b = 0; b < 2; ++b)
       x[b] = __builtin_amdgcn_ds_read_tr16_b64_v4i16(
-          (lds_s4_p)(static_cast<uintptr_t>(lds0 + at + (st * 2 + b) * 16 * D * 2)));
+          (lds_s4_p)((lds_char_p)lds + at + (st * 2 + b) * 16 * D * 2));
     return __builtin_bit_cast(h8, __builtin_shufflevector(x[0], x[1], 0, 1, 2, 3, 4, 5, 6, 7));
   }
   // Adds what weight w (0: not seen) brings to columns c.. (4) from fix_v's infinities and NaN
@@ -468,7 +476,7 @@ __global__ void __launch_bounds__(256) attn_few_kernel(const AttnArgs a) {
   int step = t.begin;
   int page = t.page_of(step, wave), page_next = 0;
   if (step < t.end) {
-    t.template issue<false>(step, wave, page, 3);
+    t.template issue<true>(step, wave, page, 0);
     page_next = t.page_of(step + 1, wave);
   }
   if (threadIdx.x < 4) rise[threadIdx.x] = 0;
@@ -476,14 +484,14 @@ __global__ void __launch_bounds__(256) attn_few_kernel(const AttnArgs a) {
 
   h8 qf[RT][P::KK];
   f4 acc[RT][DQ];
-  float mref[RT], l[RT];
-  bool begun[RT];
+  // lim: the score, less mref, above which mref moves: kRise once it is set
+  float mref[RT], l[RT], lim[RT];
 #pragma unroll
   for (int rt = 0; rt < RT; ++rt) {
     t.load_q(row0 + rt * 16 + col, qf[rt]);
     mref[rt] = 0.f;
     l[rt] = 0.f;
-    begun[rt] = false;
+    lim[rt] = -INFINITY;
 #pragma unroll
     for (int d = 0; d < DQ; ++d) acc[rt][d] = (f4){0.f, 0.f, 0.f, 0.f};
   }
@@ -508,7 +516,7 @@ __global__ void __launch_bounds__(256) attn_few_kernel(const AttnArgs a) {
     wait_vm();
     if (!plain && t.fix_v(step, wave, there)) odds[par] = step + 1;
     bar();  // everybody's copies of this step are here, and nobody reads the other buffers or P
-    if (step + 1 < t.end) t.template issue<false>(step + 1, wave, page_next, 3);
+    if (step + 1 < t.end) t.template issue<true>(step + 1, wave, page_next, 0);
     page = page_next;
     if (step + 2 < t.end) page_next = t.page_of(step + 2, wave);
 
@@ -544,8 +552,8 @@ __global__ void __launch_bounds__(256) attn_few_kernel(const AttnArgs a) {
 #pragma unroll
         for (int i = 0; i < 4; ++i) e[rt][i] = see & 1u << i ? e[rt][i] : -INFINITY;
       }
-      top[rt] = fmaxf(fmaxf(e[rt][0], e[rt][1]), fmaxf(e[rt][2], e[rt][3]));
-      move |= top[rt] > kRise || (!begun[rt] && top[rt] > -INFINITY);
+      top[rt] = max3(max3(e[rt][0], e[rt][1], e[rt][2]), e[rt][3], e[rt][3]);
+      move |= top[rt] > lim[rt];
       weigh(rt, 0.f);
     }
     if (__any(move)) rise[par] = step + 1;
@@ -564,14 +572,14 @@ __global__ void __launch_bounds__(256) attn_few_kernel(const AttnArgs a) {
       for (int rt = 0; rt < RT; ++rt) {
         const float* mr = mx + rt * 16 + col;
         const float m = fmaxf(fmaxf(mr[0], mr[kRows]), fmaxf(mr[2 * kRows], mr[3 * kRows]));
-        const bool set = m > kRise || (!begun[rt] && m > -INFINITY);
+        const bool set = m > lim[rt], begun = lim[rt] > 0.f;
         const float by = set ? m - kBelow : 0.f;
-        const float f = !set ? 1.f : begun[rt] ? __builtin_amdgcn_exp2f(-by) : 0.f;
+        const float f = !set ? 1.f : begun ? __builtin_amdgcn_exp2f(-by) : 0.f;
         mref[rt] += by;
         l[rt] *= f;
 #pragma unroll
         for (int d = 0; d < DQ; ++d) acc[rt][d] *= f;
-        begun[rt] |= set;
+        lim[rt] = set ? kRise : lim[rt];
         weigh(rt, by);
       }
       bar();
@@ -662,7 +670,7 @@ __global__ void __launch_bounds__(64 * kRowWaves) attn_rows_kernel(const AttnArg
   int step = t.begin;
   int page = t.page_of(step, blk), page_next = 0;
   if (step < t.end) {
-    t.template issue<true>(step, blk, page, kv);
+    t.template issue<false>(step, blk, page, kv);
     page_next = t.page_of(step + 1, blk);
   }
   if (threadIdx.x < 2) odds[threadIdx.x] = 0;
@@ -670,14 +678,14 @@ __global__ void __launch_bounds__(64 * kRowWaves) attn_rows_kernel(const AttnArg
 
   h8 qf[RT][P::KK];
   f4 acc[RT][DT];
-  float mref[RT], l[RT];
-  bool begun[RT];
+  // lim: the score, less mref, above which mref moves: kRise once it is set
+  float mref[RT], l[RT], lim[RT];
 #pragma unroll
   for (int rt = 0; rt < RT; ++rt) {
     t.load_q(row0 + rt * 16 + col, qf[rt]);
     mref[rt] = 0.f;
     l[rt] = 0.f;
-    begun[rt] = false;
+    lim[rt] = -INFINITY;
 #pragma unroll
     for (int d = 0; d < DT; ++d) acc[rt][d] = (f4){0.f, 0.f, 0.f, 0.f};
   }
@@ -696,7 +704,7 @@ __global__ void __launch_bounds__(64 * kRowWaves) attn_rows_kernel(const AttnArg
     if (kv != 1 && !t.plain(step, blk, page) && t.fix_v(step, blk, mine)) odds[par] = step + 1;
     bar();  // everybody's copies of this step are here, and nobody reads the other buffers
     const uint64_t there = reinterpret_cast<const uint64_t*>(there_of)[par];
-    if (step + 1 < t.end) t.template issue<true>(step + 1, blk, page_next, kv);
+    if (step + 1 < t.end) t.template issue<false>(step + 1, blk, page_next, kv);
     page = page_next;
     if (step + 2 < t.end) page_next = t.page_of(step + 2, blk);
     // (the same in every lane: into scalar registers)
@@ -740,23 +748,24 @@ __global__ void __launch_bounds__(64 * kRowWaves) attn_rows_kernel(const AttnArg
             for (int i = 0; i < 4; ++i) s[b][rt][i] = see & 1u << i ? s[b][rt][i] : -INFINITY;
           }
         }
-        top[rt] = fmaxf(fmaxf(fmaxf(s[0][rt][0], s[0][rt][1]), fmaxf(s[0][rt][2], s[0][rt][3])),
-                        fmaxf(fmaxf(s[1][rt][0], s[1][rt][1]), fmaxf(s[1][rt][2], s[1][rt][3])));
-        move |= top[rt] > kRise || (!begun[rt] && top[rt] > -INFINITY);
+        top[rt] = max3(max3(s[0][rt][0], s[0][rt][1], s[0][rt][2]),
+                       max3(s[0][rt][3], s[1][rt][0], s[1][rt][1]),
+                       max3(s[1][rt][2], s[1][rt][3], s[1][rt][3]));
+        move |= top[rt] > lim[rt];
       }
       if (__any(move)) {
 #pragma unroll
         for (int rt = 0; rt < RT; ++rt) {
           float m = fmaxf(top[rt], __shfl_xor(top[rt], 16));
           m = fmaxf(m, __shfl_xor(m, 32));
-          const bool set = m > kRise || (!begun[rt] && m > -INFINITY);
+          const bool set = m > lim[rt], begun = lim[rt] > 0.f;
           const float by = set ? m - kBelow : 0.f;
-          const float f = !set ? 1.f : begun[rt] ? __builtin_amdgcn_exp2f(-by) : 0.f;
+          const float f = !set ? 1.f : begun ? __builtin_amdgcn_exp2f(-by) : 0.f;
           mref[rt] += by;
           l[rt] *= f;
 #pragma unroll
           for (int d = 0; d < DT; ++d) acc[rt][d] *= f;
-          begun[rt] |= set;
+          lim[rt] = set ? kRise : lim[rt];
 #pragma unroll
           for (int b = 0; b < 2; ++b) s[b][rt] -= by;
         }
@@ -793,10 +802,12 @@ __global__ void __launch_bounds__(64 * kRowWaves) attn_rows_kernel(const AttnArg
           }
         }
       }
+      h8 next = t.v_frag(P::v_tile(vbase, 0), 0);
 #pragma unroll
-      for (int d = 0; d < DT; ++d) {
-        if (d % 4 == 0) asm volatile("" ::: "memory");
-        const h8 vf = t.v_frag(P::v_tile(vbase, d), 0);
+      for (int d = 0; d < DT; ++d) {  // one tile read ahead (and no more: registers)
+        const h8 vf = next;
+        if (d + 1 < DT) next = t.v_frag(P::v_tile(vbase, d + 1), 0);
+        asm volatile("" ::: "memory");
 #pragma unroll
         for (int rt = 0; rt < RT; ++rt)
           acc[rt][d] = __builtin_amdgcn_mfma_f32_16x16x32_f16(vf, pf[rt], acc[rt][d], 0, 0, 0);
