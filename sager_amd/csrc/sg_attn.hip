@@ -720,16 +720,25 @@ __global__ void __launch_bounds__(64 * kRowWaves) attn_rows_kernel(const AttnArg
       for (int b = 0; b < 2; ++b)
 #pragma unroll
         for (int rt = 0; rt < RT; ++rt) s[b][rt] = (f4){0.f, 0.f, 0.f, 0.f};
+      // (the two blocks' pieces one step ahead; the fences keep the compiler from
+      // reading further ahead: registers)
+      h8 kn[2];
+#pragma unroll
+      for (int b = 0; b < 2; ++b) kn[b] = t.k_frag(P::k_piece(kbase, 0), 0, b);
 #pragma unroll
       for (int ks = 0; ks < P::KK; ++ks) {
+        const h8 kf[2] = {kn[0], kn[1]};
+        if (ks + 1 < P::KK) {
 #pragma unroll
-        for (int b = 0; b < 2; ++b) {
-          const h8 kf = t.k_frag(P::k_piece(kbase, ks % P::KO), ks, b);
+          for (int b = 0; b < 2; ++b)
+            kn[b] = t.k_frag(P::k_piece(kbase, (ks + 1) % P::KO), ks + 1, b);
+        }
+        asm volatile("" ::: "memory");
+#pragma unroll
+        for (int b = 0; b < 2; ++b)
 #pragma unroll
           for (int rt = 0; rt < RT; ++rt)
-            s[b][rt] = __builtin_amdgcn_mfma_f32_16x16x32_f16(kf, qf[rt][ks], s[b][rt], 0, 0, 0);
-        }
-        if (ks % 2) asm volatile("" ::: "memory");  // (no more reads ahead: registers)
+            s[b][rt] = __builtin_amdgcn_mfma_f32_16x16x32_f16(kf[b], qf[rt][ks], s[b][rt], 0, 0, 0);
       }
       bool move = false;
       float top[RT];
@@ -802,11 +811,12 @@ __global__ void __launch_bounds__(64 * kRowWaves) attn_rows_kernel(const AttnArg
           }
         }
       }
-      h8 next = t.v_frag(P::v_tile(vbase, 0), 0);
+      h8 next[2] = {t.v_frag(P::v_tile(vbase, 0), 0), t.v_frag(P::v_tile(vbase, 1), 0)};
 #pragma unroll
-      for (int d = 0; d < DT; ++d) {  // one tile read ahead (and no more: registers)
-        const h8 vf = next;
-        if (d + 1 < DT) next = t.v_frag(P::v_tile(vbase, d + 1), 0);
+      for (int d = 0; d < DT; ++d) {  // two tiles read ahead
+        const h8 vf = next[d % 2];
+        asm volatile("" ::: "memory");
+        if (d + 2 < DT) next[d % 2] = t.v_frag(P::v_tile(vbase, d + 2), 0);
         asm volatile("" ::: "memory");
 #pragma unroll
         for (int rt = 0; rt < RT; ++rt)
@@ -831,13 +841,18 @@ __global__ void __launch_bounds__(64 * kRowWaves) attn_rows_kernel(const AttnArg
 }
 
 // The parts of a row's keys, joined: a workgroup per (token, head), each
-// wave's 16-B lanes taking whole parts in turn.  A part whose l is 0 has no
-// key that the row sees, and what its O holds is not read as a number.
+// 16-B lanes taking whole parts in turn.  A part whose l is 0 has no key that
+// the row sees, and what its O holds is not read as a number.  Latency decides
+// for few rows (four tokens of 16 heads in 128 parts: 4.3 us; a tree of 64 in
+// 64 parts: 14 us for 67 MB).  (256 threads of eight loads whatever D: 1 us
+// more at D 64 and 256.)
 template <int D>
-__global__ void __launch_bounds__(256) attn_join_kernel(const AttnArgs a) {
-  constexpr int LP = D / 4;        // lanes of a part
-  constexpr int SP = 256 / LP;     // parts at once
-  constexpr int U = 8;             // loads under way per lane
+constexpr int kJoinThreads = 2 * D;
+template <int D>
+__global__ void __launch_bounds__(kJoinThreads<D>) attn_join_kernel(const AttnArgs a) {
+  constexpr int LP = D / 4;                 // lanes of a part
+  constexpr int SP = kJoinThreads<D> / LP;  // parts at once
+  constexpr int U = 4;                      // loads under way per lane
   const int per = a.max_window * a.n_heads;
   const int seq = blockIdx.x / per;
   const int rest = blockIdx.x - seq * per;
@@ -885,7 +900,7 @@ __global__ void __launch_bounds__(256) attn_join_kernel(const AttnArgs a) {
     }
     m = top;
   }
-  __shared__ f4 so[256];
+  __shared__ f4 so[kJoinThreads<D>];
   __shared__ float sm[SP], ss[SP];
   so[t] = o;
   if (t % LP == 0) {
@@ -1050,8 +1065,8 @@ static int attn_launch(const AttnArgs& a, hipStream_t s, const char* nm) {
     hipLaunchKernelGGL((attn_few_kernel<D, 1>), grid, dim3(256), (FewLds<D, 1>::kBytes), s, a);
   if (int st = check_launch(nm)) return st;
   if (a.cut) {
-    hipLaunchKernelGGL(attn_join_kernel<D>, dim3(a.n_seq * a.max_window * a.n_heads), dim3(256), 0,
-                       s, a);
+    hipLaunchKernelGGL(attn_join_kernel<D>, dim3(a.n_seq * a.max_window * a.n_heads),
+                       dim3(kJoinThreads<D>), 0, s, a);
     return check_launch(nm);
   }
   return SG_OK;
