@@ -305,8 +305,13 @@ __device__ __forceinline__ double chain_rest(const VerifyArgs& a, const Chain& c
 }
 
 // Grid: (chunk, node, sequence), for the children of rank `rank`.
-// (at most 128 registers: four workgroups a CU.)
-__global__ void __launch_bounds__(256, 4) verify_rest_kernel(const VerifyArgs a, int rank) {
+// What its time goes into is one round after the other (the node, its row's
+// chunks, the siblings' sums, the tokens), so the tokens are spread over 1024
+// threads: 42 rows of 50,257 logits 6.2 us for the first children and 8 us for
+// the second ones, 64 rows of 248,320 (three ranks, the other launches with
+// them) 100 us; 256 threads of 16 tokens: 10, 14 and 123.
+constexpr int kRestThreads = 1024;
+__global__ void __launch_bounds__(kRestThreads, 8) verify_rest_kernel(const VerifyArgs a, int rank) {
   const int s = blockIdx.z, node = blockIdx.y, c = blockIdx.x;
   const Window w = window_of(a.win_off, s, a.n_tokens, a.max_window);
   if (node >= w.n) return;
@@ -315,29 +320,36 @@ __global__ void __launch_bounds__(256, 4) verify_rest_kernel(const VerifyArgs a,
   const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
   const float* x = a.logits + static_cast<long long>(w.off + me.up) * a.vocab;
   const float* q = a.draft + static_cast<long long>(w.off + node) * a.vocab;
-  constexpr int kEach = kChunk / 256;
-  float xv[kEach], qv[kEach];
+  constexpr int kEach = kChunk / kRestThreads, kWaves = kRestThreads / 64;
+  float xv[kEach], qv[kEach], next[kEach];
+  auto load = [&](float (&o)[kEach], const float* from, float none) {
 #pragma unroll
-  for (int i = 0; i < kEach; ++i) {
-    const int v = c * kChunk + i * 256 + threadIdx.x;
-    xv[i] = v < a.vocab ? x[v] : -INFINITY;
-    qv[i] = v < a.vocab ? q[v] : 0.f;
-  }
+    for (int i = 0; i < kEach; ++i) {
+      const int v = c * kChunk + i * kRestThreads + threadIdx.x;
+      o[i] = v < a.vocab ? from[v] : none;
+    }
+  };
+  auto sibling = [&](uint64_t b) {
+    return a.draft + static_cast<long long>(w.off + __builtin_ctzll(b)) * a.vocab;
+  };
+  load(xv, x, -INFINITY);
+  load(qv, q, 0.f);
   const float t = a.temperature[s];
   const bool sampled = t > 0.f;
   const double k = sampled ? per_temperature(t) : 1.0;
   __shared__ Chain ch;
   __shared__ RowStat rs;
-  __shared__ double ss[4];
+  __shared__ double ss[kWaves];
   if (wave == 0) {
     const RowStat r =
         row_stat(a, w.off + me.up, row_head(a, w.off + me.up, lane), sampled, k, lane);
     if (lane == 0) rs = r;
   }
   if (rank > 0) {
+    load(next, sibling(me.sib), 0.f);
     uint64_t b = me.sib;
     for (int i = 0; i < rank; ++i, b &= b - 1)
-      if ((i & 3) == 3 - wave) {  // (the last wave first: wave 0 has the row)
+      if (i == kWaves - 1 - wave) {  // (the last wave first: wave 0 has the row)
         const int row = w.off + __builtin_ctzll(b);
         const double r = rest_sum(a, row, lane);
         if (lane == 0) {
@@ -352,17 +364,16 @@ __global__ void __launch_bounds__(256, 4) verify_rest_kernel(const VerifyArgs a,
   double p[kEach];
 #pragma unroll
   for (int i = 0; i < kEach; ++i)
-    p[i] = target_p(st, inv, xv[i], c * kChunk + i * 256 + threadIdx.x, sampled, k);
-  for (int j = 0; j < rank; ++j) {  // a sibling's row at a time, its loads together
+    p[i] = target_p(st, inv, xv[i], c * kChunk + i * kRestThreads + threadIdx.x, sampled, k);
+  uint64_t b = me.sib;
+  for (int j = 0; j < rank; ++j) {  // a sibling's row at a time, the next one's loads under way
     const double jnv = ch.inv[j];
-    if (jnv == 0.0) continue;
-    const float* qj = a.draft + static_cast<long long>(ch.row[j]) * a.vocab;
     float o[kEach];
 #pragma unroll
-    for (int i = 0; i < kEach; ++i) {
-      const int v = c * kChunk + i * 256 + threadIdx.x;
-      o[i] = v < a.vocab ? qj[v] : 0.f;
-    }
+    for (int i = 0; i < kEach; ++i) o[i] = next[i];
+    b &= b - 1;
+    if (b) load(next, sibling(b), 0.f);
+    if (jnv == 0.0) continue;
 #pragma unroll
     for (int i = 0; i < kEach; ++i) p[i] = fmax(p[i] - static_cast<double>(o[i]), 0.0) * jnv;
   }
@@ -372,8 +383,10 @@ __global__ void __launch_bounds__(256, 4) verify_rest_kernel(const VerifyArgs a,
   sum = wave_sum(sum);
   if (lane == 0) ss[wave] = sum;
   __syncthreads();
-  if (threadIdx.x == 0)
-    a.rest[static_cast<long long>(w.off + node) * a.n_chunks + c] = (ss[0] + ss[1]) + (ss[2] + ss[3]);
+  if (wave == 0) {
+    const double all = wave_sum(lane < kWaves ? ss[lane] : 0.0);
+    if (lane == 0) a.rest[static_cast<long long>(w.off + node) * a.n_chunks + c] = all;
+  }
 }
 
 // The first thread at which the running sum of v over the workgroup's threads,
@@ -723,7 +736,7 @@ int sg_tree_verify(const float* logits, const int* tokens, const int* win_off, c
   if (int st = check_launch(nm)) return st;
   if (draft_probs)
     for (int r = 0; r < max_children && r < max_window - 1; ++r) {
-      hipLaunchKernelGGL(verify_rest_kernel, grid, dim3(256), 0, s, a, r);
+      hipLaunchKernelGGL(verify_rest_kernel, grid, dim3(kRestThreads), 0, s, a, r);
       if (int st = check_launch(nm)) return st;
     }
   hipLaunchKernelGGL(verify_walk_kernel, dim3(n_seq), dim3(kWalk), 0, s, a);
