@@ -56,7 +56,7 @@ struct AttnArgs {
   float2* part_ml;
   int2* seq_plan;
   int n_tokens, max_window, n_heads, n_kv, group, n_pages, page_log2, pages_per_seq;
-  int n_seq, row_blocks, block_rows, max_units;
+  int n_seq, row_blocks, block_rows, max_units, goal;
   bool cut;
   float scale_log2;
 };
@@ -78,10 +78,11 @@ __device__ __forceinline__ int cached_len(int length, int page_log2, int pages_p
 
 // How a batch is cut, from the caches' lengths, which only the device knows.
 // A unit is a part of a sequence's keys for one kv head; a sequence's steps of
-// 64 keys are cut into parts of `part` steps, the least for which the units
-// are no more than max_units, so that the units of a ragged batch are equally
-// long and the launch ends in one round.  Every wave finds this by itself: a
-// sequence a lane, the sum, a few guesses at `part`, the running sum.
+// 64 keys are cut into parts of `part` steps: `goal` of them if they came out
+// even, and up to 64 sequences more a part until the units are no more than
+// max_units, so that the units of a ragged batch are equally long and the
+// launch ends in one round.  Every wave finds this by itself: a sequence a
+// lane, the sum, a few guesses at `part`, the running sum.
 __device__ __forceinline__ int parts_of(int steps, int part) {
   // (fp32: a part more or less changes nothing, the last one takes what is left)
   const float inv = __builtin_amdgcn_rcpf(static_cast<float>(part));
@@ -115,22 +116,17 @@ __device__ __forceinline__ bool find_unit(const AttnArgs& a, int unit, int lane,
   int part = 0x7FFFFFFF;
   if (a.cut) {
     long long sum = __builtin_amdgcn_readlane(wave_run_sum_i(steps), 63);
-    if (a.n_seq <= 64) {
-      part = max(1, static_cast<int>((sum * a.n_kv + a.max_units - 1) / a.max_units));
+    const int n_seq = a.n_seq;
+    for (int s = lane + 64; s - lane < n_seq; s += 64) {
+      int l;
+      Window w;
+      sum += __builtin_amdgcn_readlane(wave_run_sum_i(steps_of(a, s, &l, &w)), 63);
+    }
+    part = max(1, static_cast<int>(min((sum * a.n_kv + a.goal - 1) / a.goal, 0x7FFFFFFFLL)));
+    if (n_seq <= 64)
       while (__builtin_amdgcn_readlane(wave_run_sum_i(parts_of(steps, part)), 63) * a.n_kv >
              a.max_units)
         part += max(1, part >> 3);
-    } else {  // (a sequence has at most one part more than its share)
-      for (int s = lane + 64; s - lane < a.n_seq; s += 64) {
-        int l;
-        Window w;
-        sum += __builtin_amdgcn_readlane(wave_run_sum_i(steps_of(a, s, &l, &w)), 63);
-      }
-      // (one in a thousand less than there are: parts_of rounds)
-      long long free = a.max_units - static_cast<long long>(a.n_seq) * a.n_kv;
-      free -= free >> 10;
-      part = max(1, static_cast<int>(min((sum * a.n_kv + free - 1) / free, 0x7FFFFFFFLL)));
-    }
   }
   int base = 0;
   bool found = false;
@@ -455,6 +451,13 @@ struct FewLds {
 
 // RT: tiles of 16 rows.  Wave w brings keys 16 w.. of a step, has them in the
 // first product, and has columns w D/4 .. of all keys in the second.
+// Bound by memory where the caches are long (24 sequences of one token, 77 to
+// 4,001 cached, 8 kv heads of 128: 200 MB in 37 us, 5.4 TB/s within the
+// launch) and by the rounds of latency where they are short: lengths, pages,
+// copies, the two products (4 tokens over 4,099: 10 us for 8.5 MB).  Up to 128
+// rows it is the faster form, though blocks of 32 read the keys again, from
+// the XCD's L2: 64 rows over 32,768 tokens of dimension 256 28.0 us against
+// 32.6, 128 rows 37.8 against 40.9; 200 rows 59.9 against 45.9.
 template <int D, int RT>
 __global__ void __launch_bounds__(256) attn_few_kernel(const AttnArgs a) {
   typedef Part<D> P;
@@ -652,6 +655,13 @@ struct RowsLds {
 };
 
 // Each wave brings 16 keys of K (the first four) or V.
+// Bound by the matrix cores and what feeds them: a fragment of K or V read
+// from LDS serves two products, which is as much of the LDS' bandwidth as of
+// the matrix cores, and a wave's registers (128 of O, 64 of Q at dimension
+// 256) hold no third tile of rows.  64 tokens of 16 heads over 131,071 cached
+// ones, 2 kv heads of 256: 137 GFLOP in 158 us, 870 TFLOP/s (a large matrix
+// product here: 1,190); the matrix cores are busy 45 % of the cycles, vector
+// instructions 25 %.
 template <int D>
 __global__ void __launch_bounds__(64 * kRowWaves) attn_rows_kernel(const AttnArgs a) {
   typedef Part<D> P;
@@ -944,7 +954,10 @@ struct CommitArgs {
 
 // Grid: (16-B pieces of a window's K and V rows, sequence, kCommitLayers
 // layers).  A thread looks its piece's place up once and then copies it in
-// every layer, whose loads are under way together.
+// every layer, whose loads are under way together.  One window of 4 over 10
+// layers takes 3.2 us, four dependent rounds (the path's length, its node, the
+// page, the copy); 32 windows of up to 16 over 40 layers, 65 MB, 19 us, 3.4
+// TB/s (a layer a thread: 26.8 us).
 constexpr int kCommitLayers = 8;
 __global__ void __launch_bounds__(256) kv_commit_kernel(const CommitArgs a) {
   const int s = blockIdx.y, l0 = blockIdx.z * kCommitLayers;
@@ -1023,14 +1036,17 @@ static int check_cache(const sg_kv_cache* c, int n_seq, int n_tokens, int max_wi
 
 // How a call is laid out: rows of a workgroup, the most units.
 struct Layout {
-  int block_rows, row_blocks, max_units;
+  int block_rows, row_blocks, max_units, goal;
   bool cut;
-  int least_cut;                      // the most sequences that are cut whatever their lengths
+  int few[2];                         // the most sequences for less than one round, and two
   size_t plan_bytes, o_bytes, bytes;  // of the workspace
 };
 static Layout attn_layout(int n_seq, int max_window, int max_len, int group, int n_kv, int dim) {
   Layout l;
   const long long rows = static_cast<long long>(max_window) * group;
+  // (one token of 32 heads over 8 kv heads, 16,384 cached: 14.4 us by blocks of
+  // 16, 15.2 by 32; 96 rows of 6 sequences 27.0 by 32, 33.7 by 256; 200 rows
+  // over 32,768 45.9 by 256, 59.9 by 32)
   l.block_rows = rows > 128 ? 256 : rows > 16 ? 32 : 16;
   l.row_blocks = static_cast<int>((rows + l.block_rows - 1) / l.block_rows);
   const long long units = static_cast<long long>(n_seq) * n_kv;
@@ -1041,10 +1057,26 @@ static Layout attn_layout(int n_seq, int max_window, int max_len, int group, int
   const int each = dim == 256 || l.block_rows == 256 ? 1 : dim == 128 ? 2 : 4;
   const long long slots = 256 * each;
   const long long per = 32 * each >= l.row_blocks ? 32 * each / l.row_blocks * 8 : 8;
-  l.cut = most > 1 && (units < slots || most > 8);
-  l.least_cut = most > 1 ? static_cast<int>((slots - 1) / n_kv) : 0;
+  // Heads of sequences for less than two rounds of workgroups: parts of equal
+  // length.  More: only what is longer than a round's share is cut, the others
+  // are written without a join (200 sequences of 1,500 tokens, 8 kv heads of
+  // 128: 244 us, 290 with all in equal parts; of 300 tokens and one of 30,000:
+  // 83 us, 515 without a cut; 75 sequences of 100 to 3,000, which is 1.2
+  // rounds: 102 us in equal parts, 112 with only the longest cut).  A full
+  // round of at most 8 steps is not cut (200 sequences of 10 to 400: 45 us, 66).
+  const bool rounds = units >= 2 * slots;
+  for (int i = 0; i < 2; ++i) l.few[i] = static_cast<int>(((i + 1) * slots - 1) / n_kv);
   long long n = units;
-  if (l.cut) n = (2 * units + per - 1) / per * per;
+  l.cut = most > 1 && (units < slots || most > 8);
+  l.goal = 1;
+  if (l.cut && !rounds) {
+    n = (2 * units + per - 1) / per * per;
+    // (a part a head lost to rounding; one in a thousand less: parts_of rounds)
+    l.goal = static_cast<int>(n_seq <= 64 ? n : n - units - ((n - units) >> 10));
+  } else if (l.cut) {
+    n = units + per;
+    l.goal = static_cast<int>(per - ((per + 1023) >> 10));
+  }
   l.max_units = n > 0x7FFFFF00 ? 0x7FFFFF00 : static_cast<int>(n);
   const size_t part_rows =
       static_cast<size_t>((l.max_units + 7LL) / 8 * 8) * l.row_blocks * l.block_rows;
@@ -1081,13 +1113,18 @@ size_t sg_attn_tree_workspace_bytes(int n_seq, int max_window, int max_len, int 
   if (n_seq <= 0 || max_window <= 0 || max_len < 0 || n_kv_heads <= 0 ||
       n_heads <= 0 || n_heads % n_kv_heads != 0)
     return 0;
-  // Enough for every smaller batch too: fewer sequences have no more units, but
-  // may be cut where more are not.
+  // Enough for every smaller batch too: within a way of cutting fewer sequences
+  // have no more units, but fewer may be cut where more are not.
   const int group = n_heads / n_kv_heads;
   const sg::Layout l = sg::attn_layout(n_seq, max_window, max_len, group, n_kv_heads, head_dim);
-  if (l.cut || l.least_cut <= 0) return l.bytes;
-  return sg::attn_layout(l.least_cut < n_seq ? l.least_cut : n_seq, max_window, max_len, group,
-                         n_kv_heads, head_dim).bytes;
+  size_t bytes = l.bytes;
+  for (int few : l.few)
+    if (few > 0 && few < n_seq) {
+      const size_t b =
+          sg::attn_layout(few, max_window, max_len, group, n_kv_heads, head_dim).bytes;
+      bytes = b > bytes ? b : bytes;
+    }
+  return bytes;
 }
 
 int sg_attn_tree_f16(const uint16_t* q, const uint16_t* k, const uint16_t* v, long long q_stride,
@@ -1152,6 +1189,7 @@ int sg_attn_tree_f16(const uint16_t* q, const uint16_t* k, const uint16_t* v, lo
   a.row_blocks = l.row_blocks;
   a.block_rows = l.block_rows;
   a.max_units = l.max_units;
+  a.goal = l.goal;
   a.cut = l.cut;
   a.scale_log2 = scale * kLog2e;
   const hipStream_t s = static_cast<hipStream_t>(stream);

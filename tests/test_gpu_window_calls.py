@@ -58,6 +58,20 @@ def test_attention_of_many_sequences(n_seq, longest):
     w.check_attn(w.attn_case(7, sizes, lengths, 2, 1, 64, 16, chain=True, pad=2))
 
 
+@pytest.mark.parametrize("n_seq,n_kv,D,longest", [(66, 8, 256, 1500), (60, 18, 128, 2100),
+                                                  (66, 8, 256, 5)])
+def test_attention_of_more_than_two_rounds(n_seq, n_kv, D, longest):
+    """As many heads of sequences as twice the workgroups the card holds: only the longest are cut,
+    and some sequences have neither a window nor a cache."""
+    rng = np.random.default_rng(D + longest)
+    sizes = [int(x) for x in rng.integers(0, 3, n_seq)]
+    lengths = [int(x) for x in rng.integers(0, min(longest, 70), n_seq)]
+    for i in (0, n_seq // 2, n_seq - 1):
+        sizes[i], lengths[i] = 1 + i % 2, longest - i
+        lengths[i] = max(lengths[i], 0)
+    w.check_attn(w.attn_case(19, sizes, lengths, n_kv, 1, D, 16, chain=True, pad=1))
+
+
 def test_attention_with_a_workspace_for_more_sequences():
     """The workspace of a large batch, which is not cut, serves small ones, which are."""
     for sizes, lengths in (([3, 1, 2], [400, 90, 333]), ([64], [500]), ([1] * 9, [450] * 9)):
