@@ -661,7 +661,7 @@ struct RowsLds {
 // 256) hold no third tile of rows.  64 tokens of 16 heads over 131,071 cached
 // ones, 2 kv heads of 256: 137 GFLOP in 158 us, 870 TFLOP/s (a large matrix
 // product here: 1,190); the matrix cores are busy 45 % of the cycles, vector
-// instructions 25 %.
+// instructions 22 %.
 template <int D>
 __global__ void __launch_bounds__(64 * kRowWaves) attn_rows_kernel(const AttnArgs a) {
   typedef Part<D> P;
