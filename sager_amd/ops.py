@@ -565,6 +565,15 @@ def _arg(fn, name, t, dtype, shape, dev):
     return t.data_ptr()
 
 
+def _out(fn, name, t, like, shape, dev):
+    """An output that the caller gave, or a new one of the type and on the
+    device of `like`, and its address."""
+    if t is None:
+        t = like.new_empty(*shape)
+        return t, t.data_ptr()
+    return t, _arg(fn, name, t, like.dtype, shape, dev)
+
+
 def _current_of(fn, t):
     """The current device, which has to be t's, and its current stream: the launch goes there."""
     dev = t.get_device()
@@ -619,13 +628,14 @@ def add_rmsnorm_q8_k(x, w, eps, y=None, x_out=None, xn=None, xq=None):
 def _rows(fn, name, t, shape, dev):
     """The address and the leading dimensions' strides (elements) of an fp16
     tensor [..., tokens, heads, dim] whose tokens may lie apart."""
-    st, (heads, dim) = t.stride(), shape[-2:]
+    st, heads, dim = t.stride(), shape[-2], shape[-1]
     if t.dtype is not torch.float16 or t.shape != shape or t.get_device() != dev or st[-1] != 1 or \
-            (heads > 1 and st[-2] != dim):
+            (st[-2] != dim and heads > 1):
         raise SagerError(f"{fn}: {name} must be fp16 {tuple(shape)} on GPU {dev}, a token's values "
                          f"contiguous, got {t.dtype} {tuple(t.shape)} strides {st} on {t.device}")
-    # (a dimension of one element has any stride)
-    return (t.data_ptr(), *[x if n > 1 else max(x, heads * dim) for n, x in zip(shape[:-2], st)])
+    if 1 in shape:  # (a dimension of one element has any stride)
+        st = [x if n > 1 else max(x, heads * dim) for n, x in zip(shape, st)]
+    return (t.data_ptr(), *st[:-2])
 
 
 def _windows(fn, win_off, parent, n_tokens, dev):
@@ -682,14 +692,11 @@ class KvCache:
         if n_seq > self.max_seqs or self.device != dev:
             raise SagerError(f"{fn}: {n_seq} sequences on GPU {dev}, the cache has "
                              f"{self.max_seqs} on GPU {self.device}")
-        if length_out is None:
-            length_out = torch.empty(n_seq, dtype=torch.int32, device=k.device)
-        _check(load().sg_kv_commit_f16(
-            pk, pv, ks, vs, kl, vl, self._desc, off,
-            _arg(fn, "path", path, torch.int32, (n_seq, window), dev),
-            _arg(fn, "n_path", n_path, torch.int32, (n_seq,), dev),
-            _arg(fn, "length_out", length_out, torch.int32, (n_seq,), dev), n_seq, n_tokens, window,
-            stream))
+        pp = _arg(fn, "path", path, torch.int32, (n_seq, window), dev)
+        pn = _arg(fn, "n_path", n_path, torch.int32, (n_seq,), dev)
+        length_out, po = _out(fn, "length_out", length_out, n_path, (n_seq,), dev)
+        _check(load().sg_kv_commit_f16(pk, pv, ks, vs, kl, vl, self._desc, off, pp, pn, po, n_seq,
+                                       n_tokens, window, stream))
         return length_out
 
 
@@ -763,28 +770,22 @@ class TreeVerify:
         if T > self.max_tokens or n_seq > self.max_seqs:
             raise SagerError(f"{n_seq} sequences of {T} rows: at most {self.max_seqs} of "
                              f"{self.max_tokens}")
-        place, rows, seqs = logits.device, (T,), (n_seq,)
-        full, paths = (T, self.vocab), (n_seq, self.max_window)
-        if path is None:
-            path = torch.empty(paths, dtype=i32, device=place)
-        if n_path is None:
-            n_path = torch.empty(n_seq, dtype=i32, device=place)
-        if next_token is None:
-            next_token = torch.empty(n_seq, dtype=i32, device=place)
-        if prob is None:
-            prob = torch.zeros(T, dtype=f32, device=place)
+        rows, seqs, full = (T,), (n_seq,), (T, self.vocab)
+        px = _arg(fn, "logits", logits, f32, full, dev)
+        pt = _arg(fn, "tokens", tokens, i32, rows, dev)
+        pd = None if draft_probs is None else _arg(fn, "draft_probs", draft_probs, f32, full, dev)
+        path, pp = _out(fn, "path", path, tokens, (n_seq, self.max_window), dev)
+        n_path, pn = _out(fn, "n_path", n_path, tokens, seqs, dev)
+        next_token, pnext = _out(fn, "next_token", next_token, tokens, seqs, dev)
+        if prob is None:  # (rows behind the last sequence are not written)
+            prob = torch.zeros(T, dtype=f32, device=logits.device)
         ws, ws_bytes = _space(fn, self.workspace if workspace is None else workspace, dev)
         _check(load().sg_tree_verify(
-            _arg(fn, "logits", logits, f32, full, dev), _arg(fn, "tokens", tokens, i32, rows, dev),
-            off, par,
-            None if draft_probs is None else _arg(fn, "draft_probs", draft_probs, f32, full, dev),
-            _arg(fn, "temperature", temperature, f32, seqs, dev),
+            px, pt, off, par, pd, _arg(fn, "temperature", temperature, f32, seqs, dev),
             _arg(fn, "u_accept", u_accept, f32, rows, dev),
-            _arg(fn, "u_sample", u_sample, f32, seqs, dev),
-            _arg(fn, "path", path, i32, paths, dev), _arg(fn, "n_path", n_path, i32, seqs, dev),
-            _arg(fn, "next_token", next_token, i32, seqs, dev),
-            _arg(fn, "prob", prob, f32, rows, dev),
-            ws, ws_bytes, n_seq, T, self.max_window, self.vocab, self.max_children, stream))
+            _arg(fn, "u_sample", u_sample, f32, seqs, dev), pp, pn, pnext,
+            _arg(fn, "prob", prob, f32, rows, dev), ws, ws_bytes, n_seq, T, self.max_window,
+            self.vocab, self.max_children, stream))
         return path, n_path, next_token, prob
 
 
