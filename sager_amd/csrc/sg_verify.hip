@@ -306,15 +306,17 @@ __device__ __forceinline__ double chain_rest(const VerifyArgs& a, const Chain& c
   return r;
 }
 
-// Grid: (chunk, node, sequence), for the children of rank `rank`.
+// Grid: (chunk, node, sequence), for the children of rank `rank`; a workgroup
+// takes every gridDim.x-th chunk.
 // What its time goes into is one round after the other (the node, its row's
 // chunks, the siblings' sums, the tokens), so the tokens are spread over 1024
 // threads: 42 rows of 50,257 logits 6.2 us for the first children and 8 us for
 // the second ones, 64 rows of 248,320 (three ranks, the other launches with
-// them) 100 us; 256 threads of 16 tokens: 10, 14 and 123.
+// them) 100 us, a chunk a workgroup; 256 threads of 16 tokens: 10, 14 and 123.
 constexpr int kRestThreads = 1024;
 __global__ void __launch_bounds__(kRestThreads, 8) verify_rest_kernel(const VerifyArgs a, int rank) {
-  const int s = blockIdx.z, node = blockIdx.y, c = blockIdx.x;
+  const int s = blockIdx.z, node = blockIdx.y;
+  int c = blockIdx.x;
   const Window w = window_of(a.win_off, s, a.n_tokens, a.max_window);
   if (node >= w.n) return;
   const Node me = a.nodes[w.off + node];
@@ -363,31 +365,43 @@ __global__ void __launch_bounds__(kRestThreads, 8) verify_rest_kernel(const Veri
   __syncthreads();
   const RowStat st = rs;
   const double inv = 1.0 / st.s;
-  double p[kEach];
+  while (true) {
+    double p[kEach];
 #pragma unroll
-  for (int i = 0; i < kEach; ++i)
-    p[i] = target_p(st, inv, xv[i], c * kChunk + i * kRestThreads + threadIdx.x, sampled, k);
-  uint64_t b = me.sib;
-  for (int j = 0; j < rank; ++j) {  // a sibling's row at a time, the next one's loads under way
-    const double jnv = ch.inv[j];
-    float o[kEach];
+    for (int i = 0; i < kEach; ++i)
+      p[i] = target_p(st, inv, xv[i], c * kChunk + i * kRestThreads + threadIdx.x, sampled, k);
+    uint64_t b = me.sib;
+    for (int j = 0; j < rank; ++j) {  // a sibling's row at a time, the next one's loads under way
+      const double jnv = ch.inv[j];
+      float o[kEach];
 #pragma unroll
-    for (int i = 0; i < kEach; ++i) o[i] = next[i];
-    b &= b - 1;
-    if (b) load(next, sibling(b), 0.f);
-    if (jnv == 0.0) continue;
+      for (int i = 0; i < kEach; ++i) o[i] = next[i];
+      b &= b - 1;
+      if (b) load(next, sibling(b), 0.f);
+      if (jnv == 0.0) continue;
 #pragma unroll
-    for (int i = 0; i < kEach; ++i) p[i] = fmax(p[i] - static_cast<double>(o[i]), 0.0) * jnv;
-  }
-  double sum = 0.0;  // (past the vocabulary x is -infinity and q 0)
+      for (int i = 0; i < kEach; ++i) p[i] = fmax(p[i] - static_cast<double>(o[i]), 0.0) * jnv;
+    }
+    double sum = 0.0;  // (past the vocabulary x is -infinity and q 0)
 #pragma unroll
-  for (int i = 0; i < kEach; ++i) sum += fmax(p[i] - static_cast<double>(qv[i]), 0.0);
-  sum = wave_sum(sum);
-  if (lane == 0) ss[wave] = sum;
-  __syncthreads();
-  if (wave == 0) {
-    const double all = wave_sum(lane < kWaves ? ss[lane] : 0.0);
-    if (lane == 0) a.rest[static_cast<long long>(w.off + node) * a.n_chunks + c] = all;
+    for (int i = 0; i < kEach; ++i) sum += fmax(p[i] - static_cast<double>(qv[i]), 0.0);
+    const int done = c;
+    c += gridDim.x;
+    const bool more = c < a.n_chunks;
+    if (more) {
+      load(xv, x, -INFINITY);
+      load(qv, q, 0.f);
+      if (rank > 0) load(next, sibling(me.sib), 0.f);
+    }
+    sum = wave_sum(sum);
+    if (lane == 0) ss[wave] = sum;
+    __syncthreads();
+    if (wave == 0) {
+      const double all = wave_sum(lane < kWaves ? ss[lane] : 0.0);
+      if (lane == 0) a.rest[static_cast<long long>(w.off + node) * a.n_chunks + done] = all;
+    }
+    if (!more) return;
+    __syncthreads();
   }
 }
 
@@ -736,7 +750,13 @@ int sg_tree_verify(const float* logits, const int* tokens, const int* win_off, c
   a.n_chunks = (vocab + kChunk - 1) / kChunk;
   a.max_children = max_children;
   const hipStream_t s = static_cast<hipStream_t>(stream);
-  const dim3 grid(a.n_chunks, max_window, n_seq);
+  // Two chunks a workgroup where there are several rounds of workgroups: what it
+  // finds out before its first logit then serves both (64 rows of 248,320 with
+  // three children a node 93 us, 100 with one chunk, 97 with four; five rows of
+  // 128,256 26 with one, 31 with two).
+  const long long chunks = static_cast<long long>(a.n_chunks) * max_window * n_seq;
+  const int per = chunks >= 2048 ? 2 : 1;
+  const dim3 grid((a.n_chunks + per - 1) / per, max_window, n_seq);
   hipLaunchKernelGGL(verify_rows_kernel, dim3(a.n_chunks + 1, max_window, n_seq), dim3(256), 0, s, a);
   if (int st = check_launch(nm)) return st;
   if (draft_probs)

@@ -157,6 +157,16 @@ def test_verify_more_chunks_than_threads(sampled):
         w.check_verify(c)
 
 
+@pytest.mark.parametrize("vocab,window,n_seq", [(8200, 12, 57), (4097, 16, 64)])
+def test_verify_of_several_rounds(vocab, window, n_seq):
+    """So many blocks of logits that a workgroup takes two of them, an odd number a row and an even
+    one."""
+    assert -(-vocab // 4096) * window * n_seq >= 2048
+    c = w.verify_case(85, [window - i % 5 for i in range(n_seq)], vocab, branch=3, absent=True,
+                      sampled=True, peak=3.0)
+    w.check_verify(c, 3)
+
+
 def test_verify_in_two_graphs_with_one_workspace():
     cs = [w.verify_case(s, [6, 4], 9001, branch=2, sampled=True) for s in (83, 84)]
     op = ops.TreeVerify(9001, max_tokens=10, max_seqs=2, max_window=6, max_children=2)
