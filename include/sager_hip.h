@@ -549,8 +549,8 @@ typedef struct sg_kv_cache {
  * -infinity.  q [n_tokens][n_heads][head_dim], k and v
  * [n_tokens][n_kv_heads][head_dim] with q_stride, k_stride and v_stride
  * elements from one token to the next (slices of one projection's output),
- * out contiguous.  k, v, the cache's k and v and their strides are 16-B
- * aligned.  Scores, softmax statistics and sums are fp32; the weights p are
+ * out contiguous and apart from them.  k, v, the cache's k and v and their
+ * strides are 16-B aligned.  Scores, softmax statistics and sums are fp32; the weights p are
  * rounded to fp16 for the product with v.  max_len bounds the caches'
  * lengths for the choice of the launches; longer caches are right, but may
  * be slower.  Workspace: sg_attn_tree_workspace_bytes of as many sequences or
@@ -570,8 +570,9 @@ int sg_attn_tree_f16(const uint16_t* q, const uint16_t* k, const uint16_t* v, lo
  * k and v [n_tokens][n_kv_heads][head_dim] becomes token length[s] + i.  A
  * node outside its window, and a token past the page table or on an absent
  * page, is left out.  length_out[s] = length[s] + n_path[s] (NULL: not
- * written; not the cache's own length, which the launch still reads).  Two
- * sequences must not share the pages that are written. */
+ * written; not the cache's own length, which the launch still reads).  k and
+ * v are not the cache's own memory, and two sequences do not share the pages
+ * that are written. */
 int sg_kv_commit_f16(const uint16_t* k, const uint16_t* v, long long k_stride, long long v_stride,
                      long long k_layer_stride, long long v_layer_stride, const sg_kv_cache* cache,
                      const int* win_off, const int* path, const int* n_path, int* length_out,

@@ -857,7 +857,7 @@ __global__ void __launch_bounds__(64 * kRowWaves) attn_rows_kernel(const AttnArg
 // 64 parts: 14 us for 67 MB).  (256 threads of eight loads whatever D: 1 us
 // more at D 64 and 256.)
 template <int D>
-constexpr int kJoinThreads = 2 * D;
+constexpr int kJoinThreads = 2 * D;  // (counted on by the call's limit)
 template <int D>
 __global__ void __launch_bounds__(kJoinThreads<D>) attn_join_kernel(const AttnArgs a) {
   constexpr int LP = D / 4;                 // lanes of a part
@@ -1003,6 +1003,13 @@ static int log2_of(int v) {
   int l = 0;
   while ((1 << l) < v) ++l;
   return l;
+}
+
+// Whether n elements at a and m at b share memory.
+template <typename T>
+static bool overlap(const T* a, long long n, const T* b, long long m) {
+  const uintptr_t x = reinterpret_cast<uintptr_t>(a), y = reinterpret_cast<uintptr_t>(b);
+  return x < y + m * sizeof(T) && y < x + n * sizeof(T);
 }
 
 static int check_cache(const sg_kv_cache* c, int n_seq, int n_tokens, int max_window,
@@ -1153,8 +1160,14 @@ int sg_attn_tree_f16(const uint16_t* q, const uint16_t* k, const uint16_t* v, lo
   const long long join = static_cast<long long>(n_seq) * max_window * n_heads;
   const long long rows = static_cast<long long>(max_window) * (n_heads / n_kv);
   // a launch has less than 2^32 threads, two units to a kv head
-  if (units * (rows / 16 + 1) > 0x1FFFFF || join > 0xFFFFFF)
+  if (units * (rows / 16 + 1) > 0x1FFFFF || join * 2 * dim > 0xFFFFFFFFLL)
     return set_error(SG_ERR_UNSUPPORTED, "%s: too many sequences", nm);
+  // (workgroups read the inputs while others write)
+  const long long last = n_tokens - 1, n_out = static_cast<long long>(n_tokens) * n_heads * dim;
+  if (overlap(out, n_out, q, last * q_stride + n_heads * dim) ||
+      overlap(out, n_out, k, last * k_stride + n_kv * dim) ||
+      overlap(out, n_out, v, last * v_stride + n_kv * dim))
+    return set_error(SG_ERR_INVALID_ARGUMENT, "%s: out overlaps q, k or v", nm);
   const Layout l = attn_layout(n_seq, max_window, max_len, n_heads / n_kv, n_kv, dim);
   if (l.bytes && (!ws || ws_bytes < l.bytes || reinterpret_cast<uintptr_t>(ws) % 16))
     return set_error(SG_ERR_INVALID_ARGUMENT, "%s: the workspace needs %zu bytes, 16-B aligned", nm,
@@ -1207,8 +1220,6 @@ int sg_kv_commit_f16(const uint16_t* k, const uint16_t* v, long long k_stride, l
   if (!k || !v || !win_off || !path || !n_path)
     return set_error(SG_ERR_INVALID_ARGUMENT, "%s: null pointer", nm);
   if (int st = check_cache(cache, n_seq, n_tokens, max_window, nm)) return st;
-  if (length_out == cache->length)
-    return set_error(SG_ERR_INVALID_ARGUMENT, "%s: length_out is the cache's own length", nm);
   const long long row = static_cast<long long>(cache->n_kv_heads) * cache->head_dim;
   if (k_stride < row || v_stride < row)
     return set_error(SG_ERR_GEOMETRY, "%s: a token stride is less than a token", nm);
@@ -1218,6 +1229,8 @@ int sg_kv_commit_f16(const uint16_t* k, const uint16_t* v, long long k_stride, l
   if (n_seq > 65535 || cache->n_layers > 65535 || pieces > 0x7FFFFFFF - 256)
     return set_error(SG_ERR_UNSUPPORTED, "%s: n_seq=%d n_layers=%d n_kv_heads=%d", nm, n_seq,
                      cache->n_layers, cache->n_kv_heads);
+  if (length_out && overlap(length_out, n_seq, cache->length, n_seq))
+    return set_error(SG_ERR_INVALID_ARGUMENT, "%s: length_out is the cache's own length", nm);
   CommitArgs a;
   a.k = k;
   a.v = v;

@@ -178,6 +178,29 @@ def test_plain_attention_of_one_key_is_its_value():
     assert (out[1] == 0).all()
 
 
+# ---- outputs over inputs -----------------------------------------------------------------
+
+def test_attention_output_over_an_input(lib):
+    c = cache()
+    far = dict(q=P(1 << 30), k=P(2 << 30), v=P(3 << 30), ws=None)
+    n = 4 * 8 * 128 * 2  # bytes of out, and of q
+    for at in (1 << 30, (1 << 30) + n - 8, (1 << 30) - n + 8, 2 << 30, (2 << 30) + 4 * 512 - 8,
+               3 << 30, (3 << 30) - 8):
+        assert lib.sg_attn_tree_f16(*attn_args(c, **far, out=P(at))) == INVALID, at
+        assert b"overlaps" in lib.sg_last_error()
+    for at in ((1 << 30) + n, (1 << 30) - n, (2 << 30) + 4 * 512):  # beside: refused for its workspace
+        assert lib.sg_attn_tree_f16(*attn_args(c, **far, out=P(at))) == INVALID, at
+        assert b"workspace" in lib.sg_last_error()
+
+
+def test_commit_lengths_over_the_cache_s(lib):
+    c = cache()
+    for out in (4096, 4096 + 4, 4096 - 4):
+        args = [A, A, 256, 256, 4096, 4096, ctypes.byref(c), A, A, A, P(out), 2, 4, 4, None]
+        assert lib.sg_kv_commit_f16(*args) == INVALID
+        assert b"length_out" in lib.sg_last_error()
+
+
 # ---- launches past what a grid holds ---------------------------------------------------
 
 def test_launches_too_large(lib):
@@ -185,5 +208,6 @@ def test_launches_too_large(lib):
         assert fn(*norm_args(rows=1 << 22)) == UNSUPPORTED
     c = cache()
     for kw in (dict(n_seq=1 << 20, max_window=4, n_heads=8), dict(n_seq=1 << 21, max_window=1),
-               dict(n_seq=1 << 15, max_window=64, n_heads=16, qs=2048)):
+               dict(n_seq=1 << 15, max_window=64, n_heads=16, qs=2048),
+               dict(n_seq=1 << 15, max_window=64, n_heads=8)):
         assert lib.sg_attn_tree_f16(*attn_args(c, **kw)) == UNSUPPORTED, kw
