@@ -617,11 +617,14 @@ def add_rmsnorm_q8_k(x, w, eps, y=None, x_out=None, xn=None, xq=None):
     if xn is not None:
         pn = _arg(fn, "xn", xn, dt, shape, dev)
     if xq is not None:
-        if xq.numel() != rows * (n // QK) * Q8K_BYTES:
-            raise SagerError("xq must hold n/256 Q8_K blocks a row")
-        pq = _arg(fn, "xq", xq, torch.uint8, xq.shape, dev)
-    _check(entry(_arg(fn, "x", x, dt, shape, dev), py, po,
-                 _arg(fn, "w", w, torch.float32, (n,), dev), eps, pn, pq, n, rows, stream))
+        if xq.dtype is not torch.uint8 or xq.numel() != rows * (n // QK) * Q8K_BYTES or \
+                xq.get_device() != dev or not xq.is_contiguous():
+            raise SagerError(f"{fn}: xq must hold n/256 Q8_K blocks a row (uint8) on GPU {dev}")
+        pq = xq.data_ptr()
+    if not x.is_contiguous():
+        raise SagerError(f"{fn}: x must be contiguous")
+    _check(entry(x.data_ptr(), py, po, _arg(fn, "w", w, torch.float32, (n,), dev), eps, pn, pq, n,
+                 rows, stream))
     return x if y is None else x_out, xn, xq
 
 
