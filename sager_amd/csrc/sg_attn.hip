@@ -156,12 +156,16 @@ __device__ __forceinline__ bool find_unit(const AttnArgs& a, int unit, int lane,
   return found;
 }
 
-// Where chunk c (16 B) of row r lies in its row: at c ^ swz(r).  Rows are a
-// multiple of 128 B apart; 16 rows read at one chunk (K) and eight rows read
-// at a pair of chunks (V) then share no bank.
+// Where chunk c (16 B) of row r lies in its row: at c ^ swz(r), linear in r's
+// bits.  Rows are a multiple of 128 B apart; K's reads (16 rows at a chunk,
+// the next four lanes' rows at the next) and V's (eight rows at a pair of
+// chunks) find no bank twice, whichever quarter or half of the wave goes
+// together.  (With rows r and r + 8 in one pair of chunks a third of the LDS'
+// cycles were conflicts.)
 template <int D>
 __device__ __forceinline__ int swz(int r) {
-  return D == 64 ? (r & 6) | (r >> 3 & 1) : (r & 7) << 1 | (r >> 3 & 1);
+  const int up = r >> 3 & 1;
+  return D == 64 ? ((r & 6) ^ up << 2) | up : ((r & 7) << 1 ^ up << 3) | up;
 }
 
 // 16 B per lane from base + voff (bytes) into LDS at lds + 16 * lane.  As
@@ -655,13 +659,13 @@ struct RowsLds {
 };
 
 // Each wave brings 16 keys of K (the first four) or V.
-// Bound by the matrix cores and what feeds them: a fragment of K or V read
-// from LDS serves two products, which is as much of the LDS' bandwidth as of
-// the matrix cores, and a wave's registers (128 of O, 64 of Q at dimension
-// 256) hold no third tile of rows.  64 tokens of 16 heads over 131,071 cached
-// ones, 2 kv heads of 256: 137 GFLOP in 158 us, 870 TFLOP/s (a large matrix
-// product here: 1,190); the matrix cores are busy 45 % of the cycles, vector
-// instructions 22 %.
+// Bound by the matrix cores and the exponentials together: a wave's registers
+// (128 of O, 64 of Q at dimension 256) leave two waves a SIMD, which seldom are
+// in different phases.  64 tokens of 16 heads over 131,071 cached ones, 2 kv
+// heads of 256: 137 GFLOP in 158 us, 870 TFLOP/s (a large matrix product here:
+// 1,190); the matrix cores are busy 45 % of the cycles, vector instructions
+// some 30 %, the LDS 23 %.  (Wave priorities around either phase: 2 to 20 us
+// more.)
 template <int D>
 __global__ void __launch_bounds__(64 * kRowWaves) attn_rows_kernel(const AttnArgs a) {
   typedef Part<D> P;
