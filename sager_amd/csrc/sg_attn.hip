@@ -659,13 +659,13 @@ struct RowsLds {
 };
 
 // Each wave brings 16 keys of K (the first four) or V.
-// Bound by the matrix cores and the exponentials together: a wave's registers
-// (128 of O, 64 of Q at dimension 256) leave two waves a SIMD, which seldom are
-// in different phases.  64 tokens of 16 heads over 131,071 cached ones, 2 kv
-// heads of 256: 137 GFLOP in 158 us, 870 TFLOP/s (a large matrix product here:
-// 1,190); the matrix cores are busy 45 % of the cycles, vector instructions
-// some 30 %, the LDS 23 %.  (Wave priorities around either phase: 2 to 20 us
-// more.)
+// Bound by the matrix cores and the vector instructions between the products:
+// a wave's registers (128 of O, 64 of Q at dimension 256) leave two waves a
+// SIMD.  64 tokens of 16 heads over 131,071 cached ones, 2 kv heads of 256: 137
+// GFLOP in 158 us, 870 TFLOP/s (a large matrix product here: 1,190); the matrix
+// cores are busy 45 % of the cycles, vector instructions some 30 %, the LDS
+// 23 %.  (Wave priorities around either phase: 2 to 20 us more; half of the
+// waves a phase behind the others, with a second barrier a step: 8 more.)
 template <int D>
 __global__ void __launch_bounds__(64 * kRowWaves) attn_rows_kernel(const AttnArgs a) {
   typedef Part<D> P;
