@@ -405,50 +405,11 @@ __global__ void __launch_bounds__(kRestThreads, 8) verify_rest_kernel(const Veri
   }
 }
 
-// The first thread at which the running sum of v over the workgroup's threads,
-// from `before` on, passes goal and v is positive.
-struct Found {
-  int at, last;          // that thread, the last with a positive v; -1: none
-  double before, after;  // the sum in front of thread `at`, the sum behind the last thread
-};
-__device__ __forceinline__ Found find_in(double v, double before, double goal, double* ws, int* wi) {
-  const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
-  const double run = wave_run_sum(v);
-  __syncthreads();  // (ws and wi may still be read)
-  if (lane == 63) ws[wave] = run;
-  __syncthreads();
-  double base = before, all = before;
-#pragma unroll
-  for (int i = 0; i < kWalk / 64; ++i) {
-    if (i == wave) base = all;
-    all += ws[i];
-  }
-  const uint64_t hit = __ballot(v > 0.0 && base + run > goal), some = __ballot(v > 0.0);
-  if (lane == 0) {
-    wi[wave] = hit ? wave * 64 + __builtin_ctzll(hit) : kWalk;
-    wi[kWalk / 64 + wave] = some ? wave * 64 + 63 - __builtin_clzll(some) : -1;
-  }
-  __syncthreads();
-  Found f;
-  f.at = kWalk;
-  f.last = -1;
-#pragma unroll
-  for (int i = 0; i < kWalk / 64; ++i) {
-    f.at = min(f.at, wi[i]);
-    f.last = max(f.last, wi[kWalk / 64 + i]);
-  }
-  if (static_cast<int>(threadIdx.x) == f.at) ws[kWalk / 64] = base + run - v;
-  __syncthreads();
-  f.before = ws[kWalk / 64];
-  f.at = f.at < kWalk ? f.at : -1;
-  f.after = all;
-  return f;
-}
-
 // One workgroup a sequence, 16 waves: rows shared out among them, then the tree
-// in one, then the end's chunks and one chunk's tokens over all threads.  8.7
-// us for a window of 4, 11.5 for one of 64: the dependent rounds (window;
-// chunks and nodes; the end's chunks; its tokens) and the barriers of two scans.
+// in one, the end's chunk in each by itself, and that chunk's tokens over all
+// threads.  7.5 us for a window of 4, 10 for one of 64: the dependent rounds
+// (window; chunks and nodes; the end's chunks; its tokens).  (The chunk found
+// by the workgroup, and the token with four barriers instead of one: 1.3 more.)
 __global__ void __launch_bounds__(kWalk) verify_walk_kernel(const VerifyArgs a) {
   const int s = blockIdx.x;
   const int lane = threadIdx.x & 63;
@@ -468,8 +429,7 @@ __global__ void __launch_bounds__(kWalk) verify_walk_kernel(const VerifyArgs a) 
   __shared__ double mass[kMaxWindow];   // of R at a node, point masses
   __shared__ int kid_tok[kMaxWindow];   // the end's children whose share is taken
   __shared__ int s_end, s_kids;
-  __shared__ double s_total, ws[kWalk / 64 + 1];
-  __shared__ int wi[2 * kWalk / 64];
+  __shared__ double s_total, ws[kWalk / 64];
   __shared__ Chain chain;
   const float t = a.temperature[s];
   const float us = a.u_sample[s];
@@ -600,11 +560,11 @@ __global__ void __launch_bounds__(kWalk) verify_walk_kernel(const VerifyArgs a) 
         total = left[from - w.off];
       }
   const double goal = static_cast<double>(us) * total;
-  // its chunk
+  // its chunk: every wave by itself, without barriers
   int c_at = -1, c_last = 0;
-  double before = 0.0, run = 0.0;
-  for (int c0 = 0; c0 < a.n_chunks && c_at < 0; c0 += kWalk) {
-    const int c = c0 + threadIdx.x;
+  double before = 0.0, passed = 0.0;
+  for (int c0 = 0; c0 < a.n_chunks && c_at < 0; c0 += 64) {
+    const int c = c0 + lane;
     double v = 0.0;
     if (c < a.n_chunks) {
       if (from >= 0) {
@@ -623,13 +583,15 @@ __global__ void __launch_bounds__(kWalk) verify_walk_kernel(const VerifyArgs a) 
           }
       }
     }
-    const Found f = find_in(v, run, goal, ws, wi);
-    if (f.at >= 0) {
-      c_at = c0 + f.at;
-      before = f.before;
+    const double run = wave_run_sum(v);
+    const uint64_t hit = __ballot(v > 0.0 && passed + run > goal), some = __ballot(v > 0.0);
+    if (hit) {
+      const int at = __builtin_ctzll(hit);
+      c_at = c0 + at;
+      before = readlane_d(passed + run - v, at);
     }
-    if (f.last >= 0) c_last = c0 + f.last;
-    run = f.after;
+    if (some) c_last = c0 + 63 - __builtin_clzll(some);
+    passed += readlane_d(run, 63);
   }
   const bool past = c_at < 0;  // u_sample is 1 or more, or the sums round so
   if (past) c_at = c_last;
@@ -659,22 +621,39 @@ __global__ void __launch_bounds__(kWalk) verify_walk_kernel(const VerifyArgs a) 
 #pragma unroll
     for (int i = 0; i < 4; ++i) r[i] = 0.0;
   }
-  const Found f = find_in(sum, before, past ? INFINITY : goal, ws, wi);
-  const int who = f.at >= 0 ? f.at : f.last;
-  if (static_cast<int>(threadIdx.x) == who) {
-    // the first that passes the goal; the last positive one where none does (the sums round so)
-    int tok = -1;
-    bool done = false;
-    double b = f.before;
+  const double run = wave_run_sum(sum);
+  if (lane == 63) ws[wave] = run;
+  __syncthreads();
+  // the wave whose sums pass the goal; the last one with any where none does (the sums round so)
+  int who = -1;
+  double base = before, all = before;
+  bool found = false;
 #pragma unroll
-    for (int i = 0; i < 4; ++i) {
-      b += r[i];
-      if (r[i] > 0.0 && !done) tok = v0 + i;
-      done |= r[i] > 0.0 && f.at >= 0 && b > goal;
+  for (int i = 0; i < kWalk / 64; ++i) {
+    const double w_sum = ws[i];
+    if (!found && w_sum > 0.0) {
+      who = i;
+      base = all;
+      found = !past && all + w_sum > goal;
     }
-    a.next[s] = tok;
+    all += w_sum;
   }
   if (who < 0 && threadIdx.x == 0) a.next[s] = -1;  // (a chunk's sum is positive: not reached)
+  if (wave != who) return;
+  // its lane, and the token there, likewise
+  const uint64_t some = __ballot(sum > 0.0);
+  const uint64_t hit = found ? __ballot(sum > 0.0 && base + run > goal) : 0;
+  if (lane != (hit ? __builtin_ctzll(hit) : 63 - __builtin_clzll(some))) return;
+  int tok = -1;
+  bool done = false;
+  double b = base + run - sum;
+#pragma unroll
+  for (int i = 0; i < 4; ++i) {
+    b += r[i];
+    if (r[i] > 0.0 && !done) tok = v0 + i;
+    done |= r[i] > 0.0 && hit && b > goal;
+  }
+  a.next[s] = tok;
 }
 
 static size_t up16(size_t n) { return (n + 15) / 16 * 16; }
