@@ -24,6 +24,9 @@ constexpr int kChunk = 4096;      // logits of a workgroup of verify_rows_kernel
 constexpr int kWalk = 1024;       // threads of verify_walk_kernel, kChunk / 4
 constexpr int kMaxChildren = 16;
 constexpr double kRest = 0x1p-30; // a smaller share of the mass counts as none
+// What is left of a chunk is found by subtraction down to this share of its rejected tokens: the
+// weights' errors (4e-12) are then 4e-6 of it.
+constexpr double kLittle = 0x1p-20;
 
 typedef float f32x4_u __attribute__((ext_vector_type(4), aligned(4)));
 
@@ -560,12 +563,36 @@ __global__ void __launch_bounds__(kWalk) verify_walk_kernel(const VerifyArgs a) 
         total = left[from - w.off];
       }
   const double goal = static_cast<double>(us) * total;
-  // its chunk: every wave by itself, without barriers
+  // R of chunk c's tokens, four consecutive ones a thread; returns their sum
+  auto tokens_of = [&](int c, double (&r)[4]) {
+    const int v0 = c * kChunk + 4 * threadIdx.x;
+    double sum = 0.0;
+    float xv[4];
+#pragma unroll
+    for (int i = 0; i < 4; ++i) xv[i] = v0 + i < a.vocab ? no_nan(x[v0 + i]) : -INFINITY;
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+      const int v = v0 + i;
+      if (from >= 0) {  // (the rest as it was summed: not normalized)
+        r[i] = v < a.vocab
+                   ? chain_rest(a, chain, nk, target_p(st, 1.0 / st.s, xv[i], v, true, k), v) * total
+                   : 0.0;
+      } else {
+        r[i] = weight(xv[i], st.m, k);
+        if (!a.draft)
+          for (int j = 0; j < nk; ++j)
+            if (kid_tok[j] == v) r[i] = 0.0;
+      }
+      sum += r[i];
+    }
+    return sum;
+  };
+  // its chunk: every wave by itself, with the same numbers
   int c_at = -1, c_last = 0;
   double before = 0.0, passed = 0.0;
   for (int c0 = 0; c0 < a.n_chunks && c_at < 0; c0 += 64) {
     const int c = c0 + lane;
-    double v = 0.0;
+    double v = 0.0, gone = 0.0;  // gone: the chunk's rejected tokens
     if (c < a.n_chunks) {
       if (from >= 0) {
         v = a.rest[static_cast<long long>(from) * a.n_chunks + c];
@@ -579,9 +606,25 @@ __global__ void __launch_bounds__(kWalk) verify_walk_kernel(const VerifyArgs a) 
             if (tok < 0 || tok / kChunk != c) continue;
             bool again = false;
             for (int j = 0; j < i; ++j) again |= kid_tok[j] == tok;
-            if (!again) v = fmax(v - weight(no_nan(x[tok]), st.m, k), 0.0);
+            if (!again) gone += weight(no_nan(x[tok]), st.m, k);
           }
       }
+    }
+    v -= gone;
+    // Where little is left of a chunk, the difference is its sums' rounding: such a chunk is summed
+    // again without the rejected tokens, by all waves (they take the same turns: their numbers are
+    // the same).  Its sum is then 0 exactly where no token of it has a share.
+    for (uint64_t little = __ballot(gone > 0.0 && v < kLittle * gone); little; little &= little - 1) {
+      const int at = __builtin_ctzll(little);
+      double r[4];
+      const double part = wave_sum(tokens_of(c0 + at, r));
+      if (lane == 0) ws[wave] = part;
+      __syncthreads();
+      double all = 0.0;
+#pragma unroll
+      for (int i = 0; i < kWalk / 64; ++i) all += ws[i];
+      if (lane == at) v = all;
+      __syncthreads();
     }
     const double run = wave_run_sum(v);
     const uint64_t hit = __ballot(v > 0.0 && passed + run > goal), some = __ballot(v > 0.0);
@@ -595,32 +638,10 @@ __global__ void __launch_bounds__(kWalk) verify_walk_kernel(const VerifyArgs a) 
   }
   const bool past = c_at < 0;  // u_sample is 1 or more, or the sums round so
   if (past) c_at = c_last;
-  // the token in it: four consecutive ones a thread
+  // the token in it
   const int v0 = c_at * kChunk + 4 * threadIdx.x;
-  double r[4], sum = 0.0;
-  if (v0 < a.vocab) {
-    float xv[4];
-#pragma unroll
-    for (int i = 0; i < 4; ++i) xv[i] = v0 + i < a.vocab ? no_nan(x[v0 + i]) : -INFINITY;
-#pragma unroll
-    for (int i = 0; i < 4; ++i) {
-      const int v = v0 + i;
-      if (a.draft && from >= 0) {  // (the rest as it was summed: not normalized)
-        r[i] = v < a.vocab
-                   ? chain_rest(a, chain, nk, target_p(st, 1.0 / st.s, xv[i], v, true, k), v) * total
-                   : 0.0;
-      } else {
-        r[i] = weight(xv[i], st.m, k);
-        if (!a.draft)
-          for (int j = 0; j < nk; ++j)
-            if (kid_tok[j] == v) r[i] = 0.0;
-      }
-      sum += r[i];
-    }
-  } else {
-#pragma unroll
-    for (int i = 0; i < 4; ++i) r[i] = 0.0;
-  }
+  double r[4];
+  const double sum = tokens_of(c_at, r);
   const double run = wave_run_sum(sum);
   if (lane == 63) ws[wave] = run;
   __syncthreads();
@@ -638,7 +659,8 @@ __global__ void __launch_bounds__(kWalk) verify_walk_kernel(const VerifyArgs a) 
     }
     all += w_sum;
   }
-  if (who < 0 && threadIdx.x == 0) a.next[s] = -1;  // (a chunk's sum is positive: not reached)
+  // (a chunk with a sum has a token with a share; windows that overlap, against the rules, may differ)
+  if (who < 0 && threadIdx.x == 0) a.next[s] = -1;
   if (wave != who) return;
   // its lane, and the token there, likewise
   const uint64_t some = __ballot(sum > 0.0);

@@ -1,0 +1,84 @@
+"""Verification where little is left after a rejection: chunks of the vocabulary whose tokens were
+all rejected, masses that are a small difference of large ones."""
+import numpy as np
+import pytest
+
+import test_gpu_window as w
+import window_ref as ref
+
+pytestmark = pytest.mark.gpu
+
+CHUNK = 4096  # logits that the kernels sum together
+
+
+def struck_case(seed, n_seq, others=None, vocab=2 * CHUNK + 37, first=0, kids=2, temp=1.0):
+    """Windows of a root and `kids` children that no u_accept accepts.  The children's tokens lie in
+    one chunk (number `first`), whose other logits are -infinity, but for one that is `others` below
+    the chunk's largest where given; three tokens of the next chunk have the larger logits."""
+    rng = np.random.default_rng(seed)
+    rows = 1 + kids
+    x = np.full((n_seq * rows, vocab), -np.inf, np.float32)
+    tok = np.zeros(n_seq * rows, np.int32)
+    for s in range(n_seq):
+        own = rng.choice(CHUNK, kids + 1, replace=False) + first * CHUNK
+        later = rng.choice(37, 3, replace=False) + (2 if first else 1) * CHUNK
+        x[s * rows, own[:kids]] = rng.uniform(3, 6, kids)
+        x[s * rows, later] = rng.uniform(5, 7, 3)
+        if others is not None:
+            x[s * rows, own[kids]] = x[s * rows, own[:kids]].max() - others
+        tok[s * rows + 1:(s + 1) * rows] = own[:kids]
+        x[s * rows + 1:(s + 1) * rows, :3] = 0
+    par = np.tile(np.array([-1] + [0] * kids, np.int32), n_seq)
+    return dict(logits=x, tokens=tok, off=(rows * np.arange(n_seq + 1)).astype(np.int32), parent=par,
+                draft=None, temp=np.full(n_seq, temp, np.float32),
+                u_acc=np.full(n_seq * rows, 1 - 2.0 ** -24, np.float32),
+                u_smp=np.zeros(n_seq, np.float32))
+
+
+def next_of(c):
+    """The kernel's and the plain form's next tokens, all paths equal and as long."""
+    got = w.run_verify(c)
+    want = ref.verify(c["logits"], c["tokens"], c["off"], c["parent"], c["temp"], c["u_acc"],
+                      c["u_smp"], None, 16, int(np.diff(c["off"]).max()))
+    np.testing.assert_array_equal(got[0], want[0])
+    np.testing.assert_array_equal(got[1], want[1])
+    return got[2], want[2]
+
+
+def test_plain_form_of_two_rejected_tokens_in_a_chunk():
+    """The example that the tests below vary: two chunks, both tokens of the first one rejected."""
+    x = np.full((3, 2 * CHUNK), -np.inf, np.float32)
+    x[0, 0], x[0, 1], x[0, CHUNK] = 5.75, 5.5, 6
+    x[1:, 0] = 0
+    c = dict(logits=x, tokens=np.array([0, 0, 1], np.int32), off=np.array([0, 3], np.int32),
+             parent=np.array([-1, 0, 0], np.int32), draft=None, temp=np.ones(1, np.float32),
+             u_acc=np.full(3, 0.99, np.float32), u_smp=np.zeros(1, np.float32))
+    for u in (0.0, 0.5, 1 - 2.0 ** -24):
+        c["u_smp"][:] = u
+        got, want = next_of(c)
+        assert want[0] == CHUNK and got[0] == CHUNK
+
+
+@pytest.mark.parametrize("kids", [2, 3, 7])
+@pytest.mark.parametrize("first,vocab", [(0, 2 * CHUNK + 37), (1, 3 * CHUNK - 5),
+                                         (0, 70 * CHUNK + 1), (1, 70 * CHUNK)])
+def test_verify_chunk_of_rejected_tokens_alone(kids, first, vocab):
+    """Nothing is left of the chunk: no rounding makes it the last token's."""
+    n = 60 if vocab < 5 * CHUNK else 6
+    c = struck_case(kids + vocab, n, None, vocab, first, kids)
+    for u in (0.0, 2.0 ** -24, 0.5, 1 - 2.0 ** -24):
+        c["u_smp"][:] = u
+        got, want = next_of(c)
+        np.testing.assert_array_equal(got, want)
+        assert (want >= (first + 1) * CHUNK).all()
+
+
+@pytest.mark.parametrize("temp", [0.25, 1.0])
+@pytest.mark.parametrize("others", [8.0, 30.0, 50.0, 300.0])
+def test_verify_chunk_of_rejected_tokens_and_a_small_one(others, temp):
+    """What is left of the chunk is less than the rounding of its sum, and at u_sample 0 it is still
+    the first token with a share."""
+    c = struck_case(int(others), 60, others * temp, temp=temp)
+    got, want = next_of(c)
+    np.testing.assert_array_equal(got, want)
+    assert (want < CHUNK).all()
