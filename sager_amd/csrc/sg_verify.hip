@@ -25,7 +25,7 @@ constexpr int kWalk = 1024;       // threads of verify_walk_kernel, kChunk / 4
 constexpr int kMaxChildren = 16;
 constexpr double kRest = 0x1p-30; // a smaller share of the mass counts as none
 // What is left of a chunk is found by subtraction down to this share of its rejected tokens: the
-// weights' errors (4e-12) are then 4e-6 of it.
+// sums' errors (2^-47) are then 2^-27 of it.
 constexpr double kLittle = 0x1p-20;
 
 typedef float f32x4_u __attribute__((ext_vector_type(4), aligned(4)));
@@ -38,14 +38,16 @@ __device__ __forceinline__ double per_temperature(float t) {
 __device__ __forceinline__ float no_nan(float x) { return x == x ? x : -INFINITY; }
 
 // The weight 2^((x - m) c) of logit x under the row's (or chunk's) largest m,
-// which is finite; c = log2(e) / temperature.  Relative error below 4e-12:
-// (x - m) c = n + f, |f| a little over 1/2, and 2^f = 1 + f g(f) with g of
-// degree 7 through its Chebyshev nodes on +-0.502 (2.3e-12).  n comes from the
-// same difference in fp32, where its rounding takes no fp64 operation (an
-// fp64 operation takes about 10 cycles a wave, and 19 of them, with rint and
-// ldexp and a Taylor series to degree 10, took 5.5 of 18.3 us for 64 rows of
-// 248,320 logits).  Exactly 1 for x == m; 0 below 2^-1000 and for NaN and
-// -infinity.
+// which is finite; c = log2(e) / temperature.  (x - m) c = n + f, |f| a little
+// over 1/2, and 2^f = 1 + f g(f) with g of degree 10 through its Chebyshev
+// nodes on +-0.502: with the roundings 2^-52.9 of the weight at most, and
+// 2^-53 |(x - m) c| from the exponent.  All of fp64's bits, because what a
+// rejection leaves is a difference of such sums: with g of degree 7 (2e-12) a
+// third sibling's probability was off by 1.6e-5 where the first two had all
+// but 1e-8 of the mass.  n comes from the same difference in fp32, where its
+// rounding takes no fp64 operation (an fp64 operation takes about 10 cycles a
+// wave: 64 rows of 248,320 logits 19.2 us, 17.5 with g of degree 7).  Exactly 1
+// for x == m; 0 below 2^-1000 and for NaN and -infinity.
 struct Scale {
   double c, m;
   float c32, m32;
@@ -53,18 +55,27 @@ struct Scale {
 __device__ __forceinline__ Scale scale_of(double c, float m) {
   return Scale{c, static_cast<double>(m), static_cast<float>(c), m};
 }
+// A constant in scalar registers: an operand of v_fma_f64 as it is, where a literal is first moved
+// into two vector registers.
+__device__ __forceinline__ double in_sgpr(double c) {
+  asm("" : "+s"(c));
+  return c;
+}
 __device__ __forceinline__ double weight_of(float x, const Scale& s) {
   const float y = (x - s.m32) * s.c32;
   const float n = __builtin_rintf(fmaxf(y, -1010.f));
   const double f = __builtin_fma(static_cast<double>(x) - s.m, s.c, -static_cast<double>(n));
-  double g = 1.325108898947928e-06;
-  g = __builtin_fma(g, f, 1.5304109880682482e-05);
-  g = __builtin_fma(g, f, 0.00015403474297172144);
-  g = __builtin_fma(g, f, 0.0013333477189976734);
-  g = __builtin_fma(g, f, 0.009618129135905786);
-  g = __builtin_fma(g, f, 0.05550410907292433);
-  g = __builtin_fma(g, f, 0.240226506958878);
-  g = __builtin_fma(g, f, 0.6931471805567313);
+  double g = in_sgpr(4.455036203781184e-10);
+  g = __builtin_fma(g, f, in_sgpr(7.072727791672384e-09));
+  g = __builtin_fma(g, f, in_sgpr(1.017806206630947e-07));
+  g = __builtin_fma(g, f, in_sgpr(1.3215441875881882e-06));
+  g = __builtin_fma(g, f, in_sgpr(1.525273383046128e-05));
+  g = __builtin_fma(g, f, in_sgpr(0.00015403530442908896));
+  g = __builtin_fma(g, f, in_sgpr(0.0013333558146416563));
+  g = __builtin_fma(g, f, in_sgpr(0.009618129107606187));
+  g = __builtin_fma(g, f, in_sgpr(0.0555041086648216));
+  g = __builtin_fma(g, f, in_sgpr(0.240226506959101));
+  g = __builtin_fma(g, f, in_sgpr(0.6931471805599453));
   g = __builtin_fma(g, f, 1.0);
   const uint64_t b = __builtin_bit_cast(uint64_t, g);
   const uint32_t hi = static_cast<uint32_t>(b >> 32) + (static_cast<uint32_t>(static_cast<int>(n)) << 20);
@@ -152,8 +163,8 @@ __device__ __forceinline__ Node tree_node(const VerifyArgs& a, Window w, int lan
 }
 
 // Grid: (chunk, node, sequence); the workgroup past the chunks of node 0
-// does the tree.  64 rows of 248,320 take 17 us, 3.7 TB/s: memory, with 11
-// fp64 operations a logit close behind it; 4 rows 4 us, one round of loads.
+// does the tree.  64 rows of 248,320 take 19 us, 3.3 TB/s: 14 fp64 operations
+// a logit, with memory close behind them; 4 rows 4 us, one round of loads.
 // (Workgroups of several chunks, with the next one's logits under way: 22 us
 // for the 64 rows; 512 threads of 8 logits: 20.)
 __global__ void __launch_bounds__(256) verify_rows_kernel(const VerifyArgs a) {

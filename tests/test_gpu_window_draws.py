@@ -82,3 +82,63 @@ def test_verify_chunk_of_rejected_tokens_and_a_small_one(others, temp):
     got, want = next_of(c)
     np.testing.assert_array_equal(got, want)
     assert (want < CHUNK).all()
+
+
+# What a child may be off by once its earlier siblings are rejected, where `left` is the share that
+# they leave: a row's sum by at most 31 fp64 additions after the large weight (16 a thread, 6 a
+# wave, 3 a chunk, 6 over the chunks) and the share of a weight by five roundings more (the weight 2,
+# its chunk's scale 1, the division and product 2): 36 2^-53 < 2^-47 of the whole, which is what the
+# difference is off by: 2^-47 / left, relative.  Then prob's fp32 rounding.
+def small_tol(want, left, times=1):
+    return want * (w.U32 + times * 2.0 ** -47 / left) + 1e-12
+
+
+@pytest.mark.parametrize("vocab", [300, 9001, 248320])
+@pytest.mark.parametrize("left", [1e-2, 1e-4, 1e-6, 1e-8])
+def test_verify_siblings_of_nearly_certain_tokens(left, vocab):
+    """The first three children's tokens, two of them beside each other and the largest elsewhere,
+    have all but `left` of the mass: the others' probabilities, given that they are rejected."""
+    rng = np.random.default_rng(vocab)
+    x = rng.normal(0, 1, (6, vocab)).astype(np.float32)
+    big = [7, vocab - 4, vocab - 2]
+    tok = np.array([0, *big, 100, 255], np.int32)
+    x[:, big] = -np.inf
+    for i in range(6):
+        rest = np.log(np.exp(x[i].astype(np.float64)).sum() * (1 / left - 1))
+        x[i, big] = rest + np.log([0.5, 0.3, 0.2])
+    c = dict(logits=x, tokens=tok, off=np.array([0, 6], np.int32),
+             parent=np.array([-1, 0, 0, 0, 0, 0], np.int32), draft=None, temp=np.ones(1, np.float32),
+             u_acc=np.full(6, 1 - 2.0 ** -24, np.float32), u_smp=np.full(1, 0.5, np.float32))
+    got = w.run_verify(c)[3]
+    p, want, tol = ref.weights(x[0], 1.0), np.ones(6), np.zeros(6)
+    p /= p.sum()
+    for i in range(1, 6):  # (sums without what is rejected: no differences)
+        want[i] = p[tok[i]] / p.sum()
+        tol[i] = small_tol(want[i], p.sum())
+        p[tok[i]] = 0
+    assert (np.abs(got - want) <= tol).all(), (got - want) / want
+
+
+@pytest.mark.parametrize("vocab", [300, 9001])
+@pytest.mark.parametrize("near", [1e-2, 1e-4, 1e-6])
+def test_verify_drafter_close_to_the_target(near, vocab):
+    """The drafter's distribution is the target's but for `near` of each probability: what the first
+    sibling's rejection leaves is that small difference."""
+    rng = np.random.default_rng(vocab)
+    x = rng.normal(0, 1, (3, vocab)).astype(np.float32)
+    p = ref.target(x[0], 1.0)
+    q = (p * (1 + near * np.where(np.arange(vocab) % 2, 1, -1))).astype(np.float32)
+    rest = np.maximum(p - q.astype(np.float64), 0)
+    tok = np.array([0, 10, 20], np.int32)  # (even ones have more of the target's mass)
+    c = dict(logits=x, tokens=tok, off=np.array([0, 3], np.int32),
+             parent=np.array([-1, 0, 0], np.int32), draft=np.stack([q, q, q]),
+             temp=np.ones(1, np.float32), u_acc=np.full(3, 1 - 2.0 ** -24, np.float32),
+             u_smp=np.full(1, 0.5, np.float32))
+    # a second sibling that would be accepted with probability 1 says nothing: its own q is larger
+    c["draft"][2] = 0
+    c["draft"][2, 20] = 1
+    got = w.run_verify(c, 2)[3]
+    want = np.array([1.0, min(p[10] / q[10], 1), rest[20] / rest.sum()])
+    # p - q is as small as `near` p, in the token's rest and in the sum of all: twice
+    tol = small_tol(want, rest[20] / p[20], 2)
+    assert (np.abs(got - want) <= tol).all(), (got - want) / want
