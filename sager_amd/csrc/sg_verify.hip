@@ -443,7 +443,7 @@ __global__ void __launch_bounds__(kWalk) verify_walk_kernel(const VerifyArgs a) 
   __shared__ double mass[kMaxWindow];   // of R at a node, point masses
   __shared__ int kid_tok[kMaxWindow];   // the end's children whose share is taken
   __shared__ int s_end, s_kids;
-  __shared__ double s_total, ws[kWalk / 64];
+  __shared__ double ws[kWalk / 64];
   __shared__ Chain chain;
   const float t = a.temperature[s];
   const float us = a.u_sample[s];
@@ -550,7 +550,6 @@ __global__ void __launch_bounds__(kWalk) verify_walk_kernel(const VerifyArgs a) 
     if (lane == 0) {
       s_end = at;
       s_kids = __popcll(kid);
-      s_total = mass[at];
       a.n_path[s] = np;
     }
   }
@@ -565,15 +564,14 @@ __global__ void __launch_bounds__(kWalk) verify_walk_kernel(const VerifyArgs a) 
   }
   const long long row = w.off + end;
   const float* x = a.logits + row * a.vocab;
-  double total = st.s * s_total;
   int from = -1;  // the rejected child whose rest is what is left
+  double unit = 0.0;
   if (a.draft)
     for (int i = 0; i < nk; ++i)
       if (chain.inv[i] != 0.0) {
         from = chain.row[i];
-        total = left[from - w.off];
+        unit = left[from - w.off];
       }
-  const double goal = static_cast<double>(us) * total;
   // R of chunk c's tokens, four consecutive ones a thread; returns their sum
   auto tokens_of = [&](int c, double (&r)[4]) {
     const int v0 = c * kChunk + 4 * threadIdx.x;
@@ -586,7 +584,7 @@ __global__ void __launch_bounds__(kWalk) verify_walk_kernel(const VerifyArgs a) 
       const int v = v0 + i;
       if (from >= 0) {  // (the rest as it was summed: not normalized)
         r[i] = v < a.vocab
-                   ? chain_rest(a, chain, nk, target_p(st, 1.0 / st.s, xv[i], v, true, k), v) * total
+                   ? chain_rest(a, chain, nk, target_p(st, 1.0 / st.s, xv[i], v, true, k), v) * unit
                    : 0.0;
       } else {
         r[i] = weight(xv[i], st.m, k);
@@ -598,11 +596,14 @@ __global__ void __launch_bounds__(kWalk) verify_walk_kernel(const VerifyArgs a) 
     }
     return sum;
   };
-  // its chunk: every wave by itself, with the same numbers
+  // Its chunk: every wave by itself, with the same numbers.  64 chunks at a time, from the last ones
+  // down to the first for the total, then up for the chunk.  (The row's sum less what is rejected
+  // would be that total too, but for the difference's rounding.)
   int c_at = -1, c_last = 0;
-  double before = 0.0, passed = 0.0;
-  for (int c0 = 0; c0 < a.n_chunks && c_at < 0; c0 += 64) {
-    const int c = c0 + lane;
+  double before = 0.0, passed = 0.0, total = 0.0, goal = 0.0;
+  const int blocks = (a.n_chunks + 63) / 64;
+  for (int b = 1 - blocks; b < blocks && c_at < 0; ++b) {
+    const int c0 = 64 * abs(b), c = c0 + lane;
     double v = 0.0, gone = 0.0;  // gone: the chunk's rejected tokens
     if (c < a.n_chunks) {
       if (from >= 0) {
@@ -638,6 +639,9 @@ __global__ void __launch_bounds__(kWalk) verify_walk_kernel(const VerifyArgs a) 
       __syncthreads();
     }
     const double run = wave_run_sum(v);
+    if (b <= 0) total += readlane_d(run, 63);
+    if (b < 0) continue;
+    goal = static_cast<double>(us) * total;
     const uint64_t hit = __ballot(v > 0.0 && passed + run > goal), some = __ballot(v > 0.0);
     if (hit) {
       const int at = __builtin_ctzll(hit);

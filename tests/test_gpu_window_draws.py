@@ -142,3 +142,32 @@ def test_verify_drafter_close_to_the_target(near, vocab):
     # p - q is as small as `near` p, in the token's rest and in the sum of all: twice
     tol = small_tol(want, rest[20] / p[20], 2)
     assert (np.abs(got - want) <= tol).all(), (got - want) / want
+
+
+@pytest.mark.parametrize("vocab", [300, 5000, 65 * CHUNK])
+@pytest.mark.parametrize("left", [1e-2, 1e-5, 1e-9, 1e-11, 1e-13])
+def test_verify_draw_from_what_little_is_left(left, vocab):
+    """Two rejected children have all but `left` of the mass, 256 tokens share that equally: the last
+    token on either side of each border between them, one step of u_sample away."""
+    n = 256
+    k = np.arange(1, n)
+    u = np.float32(k / n)
+    u = np.concatenate([np.nextafter(u, np.float32(0)), np.nextafter(u, np.float32(1))])
+    x = np.full((3, vocab), -np.inf, np.float32)
+    at = np.linspace(0, vocab - 3, n).astype(int) + 2
+    x[0, at] = 1.0
+    x[0, 1] = 1 + np.log(n * (left ** -0.5 - 1))                           # all but left ** 0.5
+    x[0, 0] = 1 + np.log(n * left ** -0.5 * (left ** -0.5 - 1))            # of what it leaves too
+    x[1:, 0] = 0
+    got = []
+    for some in np.array_split(u, 1 if vocab < 10000 else 16):
+        m = len(some)
+        c = dict(logits=np.tile(x, (m, 1)), tokens=np.tile(np.array([0, 0, 1], np.int32), m),
+                 off=(3 * np.arange(m + 1)).astype(np.int32),
+                 parent=np.tile(np.array([-1, 0, 0], np.int32), m), draft=None,
+                 temp=np.ones(m, np.float32), u_acc=np.full(3 * m, 1 - 2.0 ** -24, np.float32),
+                 u_smp=some)
+        path, n_path, nxt, _ = w.run_verify(c)
+        assert (n_path == 1).all()
+        got.append(nxt)
+    np.testing.assert_array_equal(np.concatenate(got), np.concatenate([at[k - 1], at[k]]))
