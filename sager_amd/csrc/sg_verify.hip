@@ -3,8 +3,8 @@
 //
 // The vocabulary is cut into chunks.  verify_rows_kernel reads every row of
 // logits once and leaves per chunk the largest logit m_c and
-// sum 2^((x - m_c) log2(e) / temperature) (greedy: where m_c lies), and per
-// node what its tree says of it; verify_walk_kernel, one workgroup a
+// sum 2^((x - m_c) log2(e) / temperature) less the largest logit's own 1
+// (greedy: where m_c lies), and per node what its tree says of it; verify_walk_kernel, one workgroup a
 // sequence, joins the chunks of each row, goes down the tree and draws the
 // last token: first its chunk, by the chunks' sums, then the token inside it,
 // so that of the last row only one chunk is read again.  With the drafter's
@@ -15,7 +15,9 @@
 //
 // Weights and sums are fp64: the last token is found by comparing running
 // sums, and with a vocabulary's worth of borders an fp32 sum would move one
-// over the random number now and then.
+// over the random number now and then.  The largest logit's weight stays apart
+// from its chunk's and its row's sum, for it may be nearly all of them: what
+// its rejection leaves is then no difference.
 #include "sg_window.hpp"
 
 namespace sg {
@@ -24,8 +26,8 @@ constexpr int kChunk = 4096;      // logits of a workgroup of verify_rows_kernel
 constexpr int kWalk = 1024;       // threads of verify_walk_kernel, kChunk / 4
 constexpr int kMaxChildren = 16;
 constexpr double kRest = 0x1p-30; // a smaller share of the mass counts as none
-// What is left of a chunk is found by subtraction down to this share of its rejected tokens: the
-// sums' errors (2^-47) are then 2^-27 of it.
+// What other rejected tokens leave of a sum is found by subtraction down to this share of it: the
+// sums' errors (2^-47) are then 2^-27 of what is left.
 constexpr double kLittle = 0x1p-20;
 
 typedef float f32x4_u __attribute__((ext_vector_type(4), aligned(4)));
@@ -105,7 +107,7 @@ struct VerifyArgs {
   int *path, *n_path, *next;
   float* prob;
   Node* nodes;    // [token]
-  double* csum;   // [token][chunk]: sum of weights; greedy: index of the largest logit
+  double* csum;   // [token][chunk]: sum of weights less 1; greedy: index of the largest logit
   double* rest;   // [token][chunk]: sum of max(R - q, 0) once the node is rejected
   float* cmax;    // [token][chunk]
   int n_tokens, max_window, vocab, n_chunks, max_children;
@@ -163,8 +165,8 @@ __device__ __forceinline__ Node tree_node(const VerifyArgs& a, Window w, int lan
 }
 
 // Grid: (chunk, node, sequence); the workgroup past the chunks of node 0
-// does the tree.  64 rows of 248,320 take 19 us, 3.3 TB/s: 14 fp64 operations
-// a logit, with memory close behind them; 4 rows 4 us, one round of loads.
+// does the tree.  64 rows of 248,320 take 19.7 us, 3.2 TB/s: 14 fp64 operations
+// a logit, with memory close behind them; 4 rows 4.8 us, one round of loads.
 // (Workgroups of several chunks, with the next one's logits under way: 22 us
 // for the 64 rows; 512 threads of 8 logits: 20.)
 __global__ void __launch_bounds__(256) verify_rows_kernel(const VerifyArgs a) {
@@ -201,17 +203,31 @@ __global__ void __launch_bounds__(256) verify_rows_kernel(const VerifyArgs a) {
   const double k = sampled ? per_temperature(t) : 1.0;
   __shared__ float sm[4];
   __shared__ double ss[4];
+  __shared__ int sn[4];  // whether the wave has one of the largest
   float m = -INFINITY;  // (fmaxf passes a NaN over)
 #pragma unroll
   for (int h = 0; h < kLoads; ++h)
 #pragma unroll
     for (int i = 0; i < 4; ++i) m = fmaxf(m, v[h][i]);
+  const float mine = m;
   m = wave_max_dpp(m);
   if (lane == 0) sm[wave] = m;
   __syncthreads();
   m = fmaxf(fmaxf(sm[0], sm[1]), fmaxf(sm[2], sm[3]));
   double sum = 0.0;
+  const uint64_t has = __ballot(mine == m);
   if (sampled) {
+    if (has) {  // one of the largest stays apart from the wave's sum
+      bool out = lane == __builtin_ctzll(has);
+#pragma unroll
+      for (int h = 0; h < kLoads; ++h)
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+          const bool it = out && v[h][i] == m;
+          v[h][i] = it ? -INFINITY : v[h][i];
+          out = out && !it;
+        }
+    }
     if (m == INFINITY) {
 #pragma unroll
       for (int h = 0; h < kLoads; ++h)
@@ -233,20 +249,25 @@ __global__ void __launch_bounds__(256) verify_rows_kernel(const VerifyArgs a) {
       for (int i = 0; i < 4; ++i) at = v[h][i] == m ? min(at, v0 + h * 1024 + i) : at;
     sum = static_cast<double>(-wave_max_i32(-at));
   }
-  if (lane == 0) ss[wave] = sum;
+  if (lane == 0) {
+    ss[wave] = sum;
+    sn[wave] = has != 0;
+  }
   __syncthreads();
   if (threadIdx.x == 0) {
     a.cmax[row * a.n_chunks + c] = m;
-    a.csum[row * a.n_chunks + c] = sampled ? (ss[0] + ss[1]) + (ss[2] + ss[3])
-                                           : fmin(fmin(ss[0], ss[1]), fmin(ss[2], ss[3]));
+    a.csum[row * a.n_chunks + c] =
+        sampled ? ((ss[0] + ss[1]) + (ss[2] + ss[3])) + (sn[0] + sn[1] + sn[2] + sn[3] - 1)
+                : fmin(fmin(ss[0], ss[1]), fmin(ss[2], ss[3]));
   }
 }
 
-// A row's largest logit and its sum of weights (greedy: the lowest index of
-// the largest logit; -1 if all are -infinity), by one wave.
+// A row's largest logit, its sum of weights, and that less the largest logit's
+// 1 (greedy: s is the lowest index of the largest logit; -1 if all are
+// -infinity), by one wave.
 struct RowStat {
   float m;
-  double s;
+  double s, others;
 };
 // The first 128 chunks (half a million tokens), so that several rows' loads can be under way.
 struct RowHead {
@@ -271,13 +292,25 @@ __device__ __forceinline__ RowStat row_stat(const VerifyArgs& a, long long row, 
   float m = fmaxf(h.m[0], h.m[1]);
   for (int c = lane + 128; c < a.n_chunks; c += 64) m = fmaxf(m, cm[c]);
   r.m = m = wave_max_dpp(m);
+  r.others = 0.0;
   if (sampled) {
+    // all chunks' sums, but of one that has the largest logit without its 1
     double s = 0.0;
+    bool apart = false;
+    auto add = [&](float mc, double sc) {
+      const uint64_t has = __ballot(mc == m);
+      const bool one = !apart && has && lane == __builtin_ctzll(has);
+      apart |= has != 0;
+      if (mc > -INFINITY) s += one ? sc : (sc + 1.0) * weight(mc, m, k);
+    };
 #pragma unroll
-    for (int i = 0; i < 2; ++i) s += h.m[i] > -INFINITY ? h.s[i] * weight(h.m[i], m, k) : 0.0;
-    for (int c = lane + 128; c < a.n_chunks; c += 64)
-      if (cm[c] > -INFINITY) s += cs[c] * weight(cm[c], m, k);
-    r.s = wave_sum(s);
+    for (int i = 0; i < 2; ++i) add(h.m[i], h.s[i]);
+    for (int c0 = 128; c0 < a.n_chunks; c0 += 64) {
+      const int c = min(c0 + lane, a.n_chunks - 1);
+      add(c == c0 + lane ? cm[c] : -INFINITY, cs[c]);
+    }
+    r.others = wave_sum(s);
+    r.s = m > -INFINITY ? r.others + 1.0 : 0.0;
   } else {
     int at = 0x7FFFFFFF;
 #pragma unroll
@@ -293,6 +326,43 @@ __device__ __forceinline__ RowStat row_stat(const VerifyArgs& a, long long row, 
 __device__ __forceinline__ double rest_sum(const VerifyArgs& a, long long row, int lane) {
   double s = 0.0;
   for (int c = lane; c < a.n_chunks; c += 64) s += a.rest[row * a.n_chunks + c];
+  return wave_sum(s);
+}
+// The row's sum of weights without the tokens of the lanes of `out`, by one wave: the chunks' sums
+// as they are, and a chunk with such a token weight by weight.
+__device__ __forceinline__ double row_without(const VerifyArgs& a, long long row, RowStat r, int tok,
+                                              uint64_t out, double k, int lane) {
+  const float* x = a.logits + row * a.vocab;
+  auto of = [&](uint64_t b) { return __builtin_amdgcn_readlane(tok, __builtin_ctzll(b)); };
+  double s = 0.0;
+  for (int c = lane; c < a.n_chunks; c += 64) {
+    const float cm = a.cmax[row * a.n_chunks + c];
+    bool has = false;
+    for (uint64_t b = out; b; b &= b - 1) has |= of(b) / kChunk == c;
+    if (!has && cm > -INFINITY) s += (a.csum[row * a.n_chunks + c] + 1.0) * weight(cm, r.m, k);
+  }
+  for (uint64_t b = out; b; b &= b - 1) {
+    const int c = of(b) / kChunk;
+    bool again = false;  // (of several in a chunk, the last one's turn)
+    for (uint64_t o = b & (b - 1); o; o &= o - 1) again |= of(o) / kChunk == c;
+    if (again) continue;
+    constexpr int kLoads = 16;  // under way at once
+#pragma unroll 1
+    for (int v0 = c * kChunk + lane; v0 < a.vocab && v0 < (c + 1) * kChunk; v0 += 64 * kLoads) {
+      float xv[kLoads];
+#pragma unroll
+      for (int i = 0; i < kLoads; ++i) {
+        const int v = v0 + 64 * i;
+        xv[i] = v < a.vocab ? no_nan(x[v]) : -INFINITY;
+      }
+#pragma unroll
+      for (int i = 0; i < kLoads; ++i) {
+        bool is = false;
+        for (uint64_t o = out; o; o &= o - 1) is |= of(o) == v0 + 64 * i;
+        if (!is) s += weight(xv[i], r.m, k);
+      }
+    }
+  }
   return wave_sum(s);
 }
 // The target's probability of token v (logit x) in a row; inv: 1 / r.s.
@@ -421,7 +491,7 @@ __global__ void __launch_bounds__(kRestThreads, 8) verify_rest_kernel(const Veri
 
 // One workgroup a sequence, 16 waves: rows shared out among them, then the tree
 // in one, the end's chunk in each by itself, and that chunk's tokens over all
-// threads.  7.5 us for a window of 4, 10 for one of 64: the dependent rounds
+// threads.  8.5 us for a window of 4, 12 for one of 64: the dependent rounds
 // (window; chunks and nodes; the end's chunks; its tokens).  (The chunk found
 // by the workgroup, and the token with four barriers instead of one: 1.3 more.)
 __global__ void __launch_bounds__(kWalk) verify_walk_kernel(const VerifyArgs a) {
@@ -440,7 +510,8 @@ __global__ void __launch_bounds__(kWalk) verify_walk_kernel(const VerifyArgs a) 
   }
   __shared__ RowStat stat[kMaxWindow];
   __shared__ double left[kMaxWindow];   // a rejected node's rest; a point mass: 1 if its share is taken
-  __shared__ double mass[kMaxWindow];   // of R at a node, point masses
+  __shared__ double whole[kMaxWindow];  // of R at a node, point masses: a sum, less the shares
+  __shared__ double taken[kMaxWindow];  // that were taken away since it was one
   __shared__ int kid_tok[kMaxWindow];   // the end's children whose share is taken
   __shared__ int s_end, s_kids;
   __shared__ double ws[kWalk / 64];
@@ -472,7 +543,8 @@ __global__ void __launch_bounds__(kWalk) verify_walk_kernel(const VerifyArgs a) 
       const RowStat r = row_stat(a, w.off + i, head[j], sampled, k, lane);
       if (lane == 0) {
         stat[i] = r;
-        mass[i] = r.m > -INFINITY ? 1.0 : 0.0;
+        whole[i] = r.m > -INFINITY ? 1.0 : 0.0;
+        taken[i] = 0.0;
       }
     }
   }
@@ -490,9 +562,9 @@ __global__ void __launch_bounds__(kWalk) verify_walk_kernel(const VerifyArgs a) 
     const bool in = n.up >= 0;
     const int up = in ? n.up : 0;
     // R of the node's token at its parent, R's mass there, the bar u has to stay under
-    double r =
-        in && n.tok >= 0 ? target_p(stat[up], 1.0 / stat[up].s, n.x, n.tok, sampled, k) : 0.0;
-    double m = mass[up], q = 1.0;
+    const double inv = 1.0 / stat[up].s;
+    double r = in && n.tok >= 0 ? target_p(stat[up], inv, n.x, n.tok, sampled, k) : 0.0;
+    double m = whole[up], q = 1.0;
     if (a.draft) {
       q = n.q;
       for (uint64_t b = n.sib; b; b &= b - 1) {
@@ -505,20 +577,50 @@ __global__ void __launch_bounds__(kWalk) verify_walk_kernel(const VerifyArgs a) 
       }
     } else {
       // A point mass: a rejected sibling takes its token's share away.  All
-      // children of one rank at once.
+      // children of one rank at once.  The largest logit's leaves the others'
+      // sum, another one a difference, down to kLittle; then what is left is
+      // summed anew, if there are later siblings or it may be none.
       uint64_t gone = 0;  // the nodes whose share is taken
+      const uint64_t largest = __ballot(in && sampled && n.tok >= 0 && n.x == stat[up].m);
+      const double others = stat[up].others * inv;
       for (int j = 0; __any(in && n.rank >= j); ++j) {
         const bool now = in && n.rank == j;
-        bool take = false;
+        double all = 0.0, less = 0.0;
+        bool little = false;
         if (now) {
           if (n.same & gone) r = 0.0;
-          m = mass[up];
-          take = m - r >= kRest * m;
-          if (take) mass[up] = m - r;
+          all = whole[up];
+          less = taken[up];
+          m = all - less;
+          if ((largest >> lane & 1) && !(n.sib & gone & largest))
+            all = others;
+          else
+            less += r;
+          little = sampled && all - less < kLittle * all;
+        }
+        if (__any(little)) {
+          uint64_t later = in ? n.sib : 0;
+          for (int o = 1; o < 64; o <<= 1) later |= __shfl_xor(later, o);
+          little = little && ((later >> lane & 1) || m < 0x1p-10 * whole[up]);
+          for (uint64_t b = __ballot(little); b; b &= b - 1) {
+            const int l = __builtin_ctzll(b);
+            const uint64_t out = (__shfl(n.sib, l) & gone) | 1ull << l;
+            const int at = __builtin_amdgcn_readlane(up, l);
+            const double sum = row_without(a, w.off + at, stat[at], n.tok, out, k, lane);
+            if (lane == l) {
+              all = sum / stat[at].s;
+              less = 0.0;
+            }
+          }
+        }
+        const bool take = now && all - less >= kRest * m;
+        if (take) {
+          whole[up] = all;
+          taken[up] = less;
         }
         gone |= __ballot(take);
         wait_lds();
-        asm volatile("" ::: "memory");  // (mass is other lanes' next)
+        asm volatile("" ::: "memory");  // (whole and taken are other lanes' next)
       }
       if (lane < w.n) left[lane] = gone >> lane & 1 ? 1.0 : 0.0;
     }
@@ -604,29 +706,41 @@ __global__ void __launch_bounds__(kWalk) verify_walk_kernel(const VerifyArgs a) 
   const int blocks = (a.n_chunks + 63) / 64;
   for (int b = 1 - blocks; b < blocks && c_at < 0; ++b) {
     const int c0 = 64 * abs(b), c = c0 + lane;
-    double v = 0.0, gone = 0.0;  // gone: the chunk's rejected tokens
+    // v: the chunk's sum; gone: its rejected tokens' weights, but for the largest logit's, which is
+    // left out of v
+    double v = 0.0, gone = 0.0;
+    bool struck = false;
     if (c < a.n_chunks) {
       if (from >= 0) {
         v = a.rest[static_cast<long long>(from) * a.n_chunks + c];
       } else {
         const float cm = a.cmax[row * a.n_chunks + c];
         const double cs = a.csum[row * a.n_chunks + c];
-        if (cm > -INFINITY) v = cs * weight(cm, st.m, k);
+        bool largest = false;
         if (!a.draft)
           for (int i = 0; i < nk; ++i) {
             const int tok = kid_tok[i];
             if (tok < 0 || tok / kChunk != c) continue;
             bool again = false;
             for (int j = 0; j < i; ++j) again |= kid_tok[j] == tok;
-            if (!again) gone += weight(no_nan(x[tok]), st.m, k);
+            if (again) continue;
+            struck = true;
+            const float xt = no_nan(x[tok]);
+            if (xt == cm && !largest)
+              largest = true;
+            else
+              gone += weight(xt, st.m, k);
           }
+        if (cm > -INFINITY) v = (cs + (largest ? 0.0 : 1.0)) * weight(cm, st.m, k);
       }
     }
     v -= gone;
-    // Where little is left of a chunk, the difference is its sums' rounding: such a chunk is summed
-    // again without the rejected tokens, by all waves (they take the same turns: their numbers are
-    // the same).  Its sum is then 0 exactly where no token of it has a share.
-    for (uint64_t little = __ballot(gone > 0.0 && v < kLittle * gone); little; little &= little - 1) {
+    // Where little is left of a chunk, the difference is its sums' rounding, or below what a weight
+    // can be: such a chunk is summed again without the rejected tokens, by all waves (they take the
+    // same turns: their numbers are the same).  Its sum is then 0 exactly where no token of it has a
+    // share.
+    for (uint64_t little = __ballot(struck && (v < kLittle * gone || (v > 0.0 && v < 0x1p-900)));
+         little; little &= little - 1) {
       const int at = __builtin_ctzll(little);
       double r[4];
       const double part = wave_sum(tokens_of(c0 + at, r));

@@ -171,3 +171,39 @@ def test_verify_draw_from_what_little_is_left(left, vocab):
         assert (n_path == 1).all()
         got.append(nxt)
     np.testing.assert_array_equal(np.concatenate(got), np.concatenate([at[k - 1], at[k]]))
+
+
+@pytest.mark.parametrize("vocab", [300, 9001, 248320])
+@pytest.mark.parametrize("lefts", [(1e-7,), (1e-7, 1e-7), (1e-3, 1e-7, 1e-8), (1e-8, 1e-4, 1e-8, 1e-7),
+                                   (1e-9, 0.5), (0.5, 1e-9, 1e-9)])
+def test_verify_siblings_after_nearly_certain_ones(lefts, vocab):
+    """One sibling after the other leaves next to nothing of what there is: the later ones'
+    probabilities are good to fp32 all the same (a difference is kept above 2^-20 of a sum that is
+    good to 2^-47: 2^-26 with the token's own), and so is the last draw."""
+    rng = np.random.default_rng(vocab + len(lefts))
+    n = len(lefts) + 2
+    e = np.exp(rng.normal(0, 1, vocab))          # weights
+    own = rng.choice(np.arange(50, vocab), n, replace=False)
+    if len(lefts) > 1:
+        own[1] = own[0] - 1 if own[0] - 1 not in own else own[1]
+    e[own[:-2]] = 0
+    for i, left in reversed(list(enumerate(lefts))):
+        e[own[i]] = e.sum() * (1 / left - 1)
+    x = np.tile(np.log(e + (e == 0)).astype(np.float32), (n + 1, 1))
+    c = dict(logits=x, tokens=np.concatenate([[0], own]).astype(np.int32),
+             off=np.array([0, n + 1], np.int32), parent=np.array([-1] + [0] * n, np.int32), draft=None,
+             temp=np.ones(1, np.float32), u_acc=np.full(n + 1, 1 - 2.0 ** -24, np.float32),
+             u_smp=np.full(1, 0.5, np.float32))
+    p, want = ref.weights(x[0], 1.0), [1.0]
+    for t in own:  # (sums without what is rejected: no differences)
+        want.append(p[t] / p.sum())
+        p[t] = 0
+    path, n_path, nxt, got = w.run_verify(c)
+    want = np.array(want)
+    assert (np.abs(got - want) <= want * (w.U32 + 2.0 ** -26)).all(), (got - want) / want
+    accepted = want[1:] > 1 - 2.0 ** -24
+    assert n_path[0] == 1 + accepted.any()
+    if accepted.any():
+        return
+    cdf = np.cumsum(p)
+    assert nxt[0] == np.nonzero(cdf > 0.5 * cdf[-1])[0][0]
