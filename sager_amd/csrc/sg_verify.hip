@@ -164,6 +164,14 @@ __device__ __forceinline__ Node tree_node(const VerifyArgs& a, Window w, int lan
   return n;
 }
 
+// Whether what lies at node i of a window can be its own: a window that shares
+// rows with another one (win_off not ascending) may find the other's nodes
+// there, or half of them.  Such a node counts as absent, so that every row that
+// a node names is one of its window's.
+__device__ __forceinline__ bool node_ok(const Node& n, int i) {
+  return n.up >= 0 && n.up < i && n.sib >> i == 0 && n.rank == __popcll(n.sib);
+}
+
 // Grid: (chunk, node, sequence); the workgroup past the chunks of node 0
 // does the tree.  64 rows of 248,320 take 19.7 us, 3.2 TB/s: 14 fp64 operations
 // a logit, with memory close behind them; 4 rows 4.8 us, one round of loads.
@@ -404,7 +412,7 @@ __global__ void __launch_bounds__(kRestThreads, 8) verify_rest_kernel(const Veri
   const Window w = window_of(a.win_off, s, a.n_tokens, a.max_window);
   if (node >= w.n) return;
   const Node me = a.nodes[w.off + node];
-  if (me.up < 0 || me.rank != rank) return;
+  if (!node_ok(me, node) || me.rank != rank) return;
   const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
   const float* x = a.logits + static_cast<long long>(w.off + me.up) * a.vocab;
   const float* q = a.draft + static_cast<long long>(w.off + node) * a.vocab;
@@ -559,7 +567,7 @@ __global__ void __launch_bounds__(kWalk) verify_walk_kernel(const VerifyArgs a) 
     }
   __syncthreads();
   if (wave == 0) {
-    const bool in = n.up >= 0;
+    const bool in = node_ok(n, lane) && (!a.draft || n.rank < a.max_children);
     const int up = in ? n.up : 0;
     // R of the node's token at its parent, R's mass there, the bar u has to stay under
     const double inv = 1.0 / stat[up].s;
@@ -567,10 +575,10 @@ __global__ void __launch_bounds__(kWalk) verify_walk_kernel(const VerifyArgs a) 
     double m = whole[up], q = 1.0;
     if (a.draft) {
       q = n.q;
-      for (uint64_t b = n.sib; b; b &= b - 1) {
+      for (uint64_t b = in ? n.sib : 0; b; b &= b - 1) {
         const int j = __builtin_ctzll(b);
         if (left[j] < kRest) continue;
-        const double qj = in && n.tok >= 0
+        const double qj = n.tok >= 0
                               ? a.draft[static_cast<long long>(w.off + j) * a.vocab + n.tok] : 0.0;
         r = fmax((m > 0.0 ? r / m : 0.0) - qj, 0.0);
         m = left[j];
@@ -641,17 +649,19 @@ __global__ void __launch_bounds__(kWalk) verify_walk_kernel(const VerifyArgs a) 
       at = __builtin_ctzll(kid);
     }
     if (lane < a.max_window) path[lane] = mine;
+    const int most = a.draft ? a.max_children : kMaxWindow;
     const uint64_t kid = __ballot(in && up == at);
-    if (in && up == at) {
-      kid_tok[n.rank] = left[lane] > 0.0 ? n.tok : -1;
+    const int place = __popcll(kid & ((1ull << lane) - 1));  // (the rank)
+    if (in && up == at && place < most) {
+      kid_tok[place] = left[lane] > 0.0 ? n.tok : -1;
       if (a.draft) {
-        chain.row[n.rank] = w.off + lane;
-        chain.inv[n.rank] = left[lane] < kRest ? 0.0 : 1.0 / left[lane];
+        chain.row[place] = w.off + lane;
+        chain.inv[place] = left[lane] < kRest ? 0.0 : 1.0 / left[lane];
       }
     }
     if (lane == 0) {
       s_end = at;
-      s_kids = __popcll(kid);
+      s_kids = min(__popcll(kid), most);
       a.n_path[s] = np;
     }
   }

@@ -207,3 +207,25 @@ def test_verify_siblings_after_nearly_certain_ones(lefts, vocab):
         return
     cdf = np.cumsum(p)
     assert nxt[0] == np.nonzero(cdf > 0.5 * cdf[-1])[0][0]
+
+
+@pytest.mark.parametrize("sampled", [False, True])
+@pytest.mark.parametrize("off", [[6, 12, 0, 9, 3, 12], [0, 64, 10, 74, 5, 70], [-3, 5, 2, 1 << 30, 7]])
+def test_verify_windows_that_share_rows(off, sampled):
+    """Offsets that do not ascend: what the windows get is not defined, but it is their own tokens
+    and paths, and the next call is what it was."""
+    T = 80
+    c = w.verify_case(sum(off[:3]), [T // 4] * 4, 311, branch=4, absent=True, sampled=sampled)
+    base = w.run_verify(c)
+    bad = dict(c, off=np.array(off, np.int32), temp=np.ones(len(off) - 1, np.float32),
+               u_smp=np.full(len(off) - 1, 0.4, np.float32))
+    for u in (0.0, 0.6):
+        bad["u_acc"] = np.full(T, u, np.float32)
+        path, n_path, nxt, _ = w.run_verify(bad, max_window=64)
+        size = np.clip(np.minimum(np.array(off[1:]), T) - np.array(off[:-1]), 0, 64)
+        size[(np.array(off[:-1]) < 0) | (np.array(off[:-1]) >= T)] = 0
+        assert (n_path <= np.maximum(size, 0)).all() and ((n_path > 0) == (size > 0)).all()
+        assert (path < np.maximum(size, 1)[:, None]).all() and (path >= -1).all()
+        assert (nxt >= -1).all() and (nxt < 311).all()
+    for a, b in zip(base, w.run_verify(c)):
+        np.testing.assert_array_equal(a, b)
