@@ -569,10 +569,11 @@ int sg_attn_tree_f16(const uint16_t* q, const uint16_t* k, const uint16_t* v, lo
  * win_off[s] + path[s][i] (path: [n_seq][max_window] nodes) of each layer's
  * k and v [n_tokens][n_kv_heads][head_dim] becomes token length[s] + i.  A
  * node outside its window, and a token past the page table or on an absent
- * page, is left out.  length_out[s] = length[s] + n_path[s] (NULL: not
- * written; not the cache's own length, which the launch still reads).  k and
- * v are not the cache's own memory, and two sequences do not share the pages
- * that are written. */
+ * page, is left out, and so is every token of a cache whose length is less
+ * than 0.  length_out[s] = length[s] + n_path[s] (NULL: not written; apart from
+ * the cache's lengths and pages, n_path, path and win_off, which the launch
+ * still reads).  k and v are not the cache's own memory, and two sequences do
+ * not share the pages that are written. */
 int sg_kv_commit_f16(const uint16_t* k, const uint16_t* v, long long k_stride, long long v_stride,
                      long long k_layer_stride, long long v_layer_stride, const sg_kv_cache* cache,
                      const int* win_off, const int* path, const int* n_path, int* length_out,

@@ -1009,13 +1009,6 @@ static int log2_of(int v) {
   return l;
 }
 
-// Whether n elements at a and m at b share memory.
-template <typename T>
-static bool overlap(const T* a, long long n, const T* b, long long m) {
-  const uintptr_t x = reinterpret_cast<uintptr_t>(a), y = reinterpret_cast<uintptr_t>(b);
-  return x < y + m * sizeof(T) && y < x + n * sizeof(T);
-}
-
 static int check_cache(const sg_kv_cache* c, int n_seq, int n_tokens, int max_window,
                        const char* nm) {
   if (!c || !c->k || !c->v || !c->pages || !c->length)
@@ -1233,8 +1226,16 @@ int sg_kv_commit_f16(const uint16_t* k, const uint16_t* v, long long k_stride, l
   if (n_seq > 65535 || cache->n_layers > 65535 || pieces > 0x7FFFFFFF - 256)
     return set_error(SG_ERR_UNSUPPORTED, "%s: n_seq=%d n_layers=%d n_kv_heads=%d", nm, n_seq,
                      cache->n_layers, cache->n_kv_heads);
-  if (length_out && overlap(length_out, n_seq, cache->length, n_seq))
-    return set_error(SG_ERR_INVALID_ARGUMENT, "%s: length_out is the cache's own length", nm);
+  // (a sequence's first workgroup writes its new length, the others read on)
+  const long long paths = static_cast<long long>(n_seq) * max_window;
+  const long long pages = static_cast<long long>(n_seq) * cache->pages_per_seq;
+  if (length_out &&
+      (overlap(length_out, n_seq, cache->length, n_seq) || overlap(length_out, n_seq, n_path, n_seq) ||
+       overlap(length_out, n_seq, path, paths) || overlap(length_out, n_seq, win_off, n_seq + 1LL) ||
+       overlap(length_out, n_seq, cache->pages, pages)))
+    return set_error(SG_ERR_INVALID_ARGUMENT,
+                     "%s: length_out overlaps the cache's lengths or pages, n_path, path or win_off",
+                     nm);
   CommitArgs a;
   a.k = k;
   a.v = v;

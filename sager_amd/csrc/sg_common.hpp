@@ -21,6 +21,12 @@ constexpr int kWave = 64;
 
 // ---- status plumbing (host) -------------------------------------------
 int set_error(int code, const char* fmt, ...);
+// Whether n elements at a and m at b share memory (either may be null).
+template <typename A, typename B>
+static inline bool overlap(const A* a, long long n, const B* b, long long m) {
+  const uintptr_t x = reinterpret_cast<uintptr_t>(a), y = reinterpret_cast<uintptr_t>(b);
+  return a && b && x < y + m * sizeof(B) && y < x + n * sizeof(A);
+}
 int check_launch(const char* what);
 
 // ---- exact fp16 -> fp32 --------------------------------------------------
