@@ -513,7 +513,8 @@ int sg_scatter_rows_f16(uint16_t* dst, const uint16_t* src, const int* dst_rows,
  *   xn = (r / sqrt(mean(r^2) + eps)) * w, rounded likewise (xn may be NULL);
  *   xq = Q8_K(xn), as sg_quantize_q8_k / _f16 make it (xq may be NULL).
  * y and x_out may both be NULL (r = x).  x_out may be x or y, xn may be x or
- * y where there is no x_out in that place.  The sum of squares is fp32.
+ * y where there is no x_out in that place; an output that overlaps another
+ * buffer in any other way is refused.  The sum of squares is fp32.
  * These are the xn and moe_xq_in_ of sg_moe_layer_f16: the reference's fused
  * norm and quantization (mmq.cu; session.cpp:1020-1022, 1129-1131), with the
  * addition that the several-token output projection leaves to the caller. */

@@ -159,6 +159,18 @@ static int norm_launch(const T* x, const T* y, T* x_out, const float* w, float e
       reinterpret_cast<uintptr_t>(y) % sizeof(T) || reinterpret_cast<uintptr_t>(x_out) % sizeof(T) ||
       reinterpret_cast<uintptr_t>(xn) % sizeof(T) || reinterpret_cast<uintptr_t>(w) % 4)
     return set_error(SG_ERR_INVALID_ARGUMENT, "%s: a buffer is not aligned to its elements", nm);
+  // (a row's values are read before they are written, other rows' at any time)
+  const long long all = static_cast<long long>(n_rows) * n;
+  const long long q = all / kQK * kQ8Bytes;
+  const unsigned char* const codes = reinterpret_cast<const unsigned char*>(xq);
+  auto over = [&](const T* out, const T* in) { return out != in && overlap(out, all, in, all); };
+  if (over(x_out, x) || over(x_out, y) || over(xn, x) || over(xn, y) ||
+      overlap(xn, all, x_out, all) || overlap(x_out, all, w, n) || overlap(xn, all, w, n) ||
+      overlap(codes, q, x, all) || overlap(codes, q, y, all) || overlap(codes, q, w, n) ||
+      overlap(codes, q, x_out, all) || overlap(codes, q, xn, all))
+    return set_error(SG_ERR_INVALID_ARGUMENT,
+                     "%s: an output overlaps another buffer (x_out and xn may each be x or y, "
+                     "not both the same)", nm);
   const hipStream_t s = static_cast<hipStream_t>(stream);
   const int nb = n / kQK;
   // one block a wave as far as the waves go

@@ -38,3 +38,32 @@ def test_commit_lengths_over_what_is_read(lib):
             args = [P(a["k"]), P(a["v"]), 256, 256, 4096, 4096, ctypes.byref(c), P(a["off"]),
                     P(a["path"]), P(a["n_path"]), P(at), n_seq, 4, W, None]
             refused(lambda: lib.sg_kv_commit_f16(*args), (name, at), lib)
+
+
+@pytest.mark.parametrize("f16", [False, True])
+def test_norm_outputs_over_other_rows(lib, f16):
+    """x_out and xn may be x or y; shifted against them they are other rows' inputs, and in one place
+    they are not two outputs."""
+    fn, size = (lib.sg_add_rmsnorm_q8_k_f16, 2) if f16 else (lib.sg_add_rmsnorm_q8_k, 4)
+    n, rows = 512, 5
+    row, q8 = n * size, 2 * 276
+    a = apart("x", "y", "x_out", "w", "xn", "xq")
+    end = {"x": rows * row, "y": rows * row, "x_out": rows * row, "w": n * 4, "xn": rows * row,
+           "xq": rows * q8}
+
+    def call(**kw):
+        b = dict(a, **kw)
+        return fn(P(b["x"]), P(b["y"]), P(b["x_out"]), P(b["w"]), 1e-6, P(b["xn"]), P(b["xq"]), n,
+                  rows, None)
+    for out in ("x_out", "xn", "xq"):
+        for other in set(a) - {out}:
+            places = [a[other] + end[other] - 4, a[other] - end[out] + 4, a[other] + row]
+            if out == "xq" or other in ("w", "xq") or {out, other} == {"x_out", "xn"}:
+                places.append(a[other])
+            for at in places:
+                if a[other] - end[out] < at < a[other] + end[other]:
+                    refused(lambda: call(**{out: at}), (out, other, at), lib)
+    # both in x's place, and without the addition xq in x's
+    refused(lambda: call(x_out=a["x"], xn=a["x"]), "one place", lib)
+    assert fn(P(a["x"]), None, None, P(a["w"]), 1e-6, None, P(a["x"]), n, rows, None) == INVALID
+    assert b"overlap" in lib.sg_last_error()
