@@ -597,7 +597,8 @@ int sg_kv_commit_f16(const uint16_t* k, const uint16_t* v, long long k_stride, l
  * n_path [n_seq], next [n_seq] (-1 if every logit of the last node is
  * -infinity or the window is empty), prob [n_tokens] (may be NULL): the
  * probability that the node is accepted once its parent is and its earlier
- * siblings are not; 1 for roots, 0 for absent nodes.
+ * siblings are not; 1 for roots, 0 for absent nodes.  The outputs are apart
+ * from each other, from the inputs and from the workspace.
  * With draft_probs, a node's children past the first max_children (1..16)
  * are absent; without, max_children is not read.  vocab is at most 2^24.
  * Weights and sums are fp64, so that next does not depend on their order.

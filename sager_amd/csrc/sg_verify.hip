@@ -866,6 +866,21 @@ int sg_tree_verify(const float* logits, const int* tokens, const int* win_off, c
   if (ws_bytes < l.bytes || reinterpret_cast<uintptr_t>(ws) % 16)
     return set_error(SG_ERR_INVALID_ARGUMENT, "%s: the workspace needs %zu bytes, 16-B aligned", nm,
                      l.bytes);
+  // (a sequence's results are written while others' are found)
+  const long long full = static_cast<long long>(n_tokens) * vocab;
+  auto clear = [&](const auto* out, long long n) {
+    return !(overlap(out, n, logits, full) || overlap(out, n, tokens, n_tokens) ||
+             overlap(out, n, win_off, n_seq + 1LL) || overlap(out, n, parent, n_tokens) ||
+             overlap(out, n, draft_probs, full) || overlap(out, n, temperature, n_seq) ||
+             overlap(out, n, u_accept, n_tokens) || overlap(out, n, u_sample, n_seq) ||
+             overlap(out, n, static_cast<unsigned char*>(ws), static_cast<long long>(l.bytes)));
+  };
+  const long long paths = static_cast<long long>(n_seq) * max_window;
+  if (!clear(path, paths) || !clear(n_path, n_seq) || !clear(next, n_seq) || !clear(prob, n_tokens) ||
+      overlap(path, paths, n_path, n_seq) || overlap(path, paths, next, n_seq) ||
+      overlap(path, paths, prob, n_tokens) || overlap(n_path, n_seq, next, n_seq) ||
+      overlap(n_path, n_seq, prob, n_tokens) || overlap(next, n_seq, prob, n_tokens))
+    return set_error(SG_ERR_INVALID_ARGUMENT, "%s: an output overlaps another buffer", nm);
   VerifyArgs a;
   a.logits = logits;
   a.tokens = tokens;

@@ -67,3 +67,20 @@ def test_norm_outputs_over_other_rows(lib, f16):
     refused(lambda: call(x_out=a["x"], xn=a["x"]), "one place", lib)
     assert fn(P(a["x"]), None, None, P(a["w"]), 1e-6, None, P(a["x"]), n, rows, None) == INVALID
     assert b"overlap" in lib.sg_last_error()
+
+
+def test_verify_outputs_over_what_is_read(lib):
+    n_seq, T, W, V = 3, 7, 4, 5000
+    need = lib.sg_tree_verify_workspace_bytes(T, V, 2)
+    size = dict(logits=T * V * 4, tokens=T * 4, off=(n_seq + 1) * 4, parent=T * 4, draft=T * V * 4,
+                temp=n_seq * 4, ua=T * 4, us=n_seq * 4, path=n_seq * W * 4, n_path=n_seq * 4,
+                next=n_seq * 4, prob=T * 4, ws=need)
+    a = apart(*size)
+
+    def call(**kw):
+        b = [P(v) for v in dict(a, **kw).values()]
+        return lib.sg_tree_verify(*b, need, n_seq, T, W, V, 2, None)
+    for out in ("path", "n_path", "next", "prob"):
+        for other in set(size) - {out}:
+            for at in (a[other], a[other] + size[other] - 4, a[other] - size[out] + 4):
+                refused(lambda: call(**{out: at}), (out, other, at), lib)
