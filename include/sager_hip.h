@@ -550,7 +550,7 @@ typedef struct sg_kv_cache {
  * -infinity.  q [n_tokens][n_heads][head_dim], k and v
  * [n_tokens][n_kv_heads][head_dim] with q_stride, k_stride and v_stride
  * elements from one token to the next (slices of one projection's output),
- * out contiguous and apart from them.  k, v, the cache's k and v and their
+ * out contiguous and apart from them and from all else that is read.  k, v, the cache's k and v and their
  * strides are 16-B aligned.  Scores, softmax statistics and sums are fp32; the weights p are
  * rounded to fp16 for the product with v.  max_len bounds the caches'
  * lengths for the choice of the launches; longer caches are right, but may

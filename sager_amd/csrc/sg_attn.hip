@@ -1169,6 +1169,16 @@ int sg_attn_tree_f16(const uint16_t* q, const uint16_t* k, const uint16_t* v, lo
   if (l.bytes && (!ws || ws_bytes < l.bytes || reinterpret_cast<uintptr_t>(ws) % 16))
     return set_error(SG_ERR_INVALID_ARGUMENT, "%s: the workspace needs %zu bytes, 16-B aligned", nm,
                      l.bytes);
+  const uint16_t* const kc = cache->k + layer * cache->layer_stride;
+  const uint16_t* const vc = cache->v + layer * cache->layer_stride;
+  const long long cached = static_cast<long long>(cache->n_pages) * n_kv * cache->page_size * dim;
+  if (overlap(out, n_out, kc, cached) || overlap(out, n_out, vc, cached) ||
+      overlap(out, n_out, cache->pages, static_cast<long long>(n_seq) * cache->pages_per_seq) ||
+      overlap(out, n_out, cache->length, n_seq) || overlap(out, n_out, win_off, n_seq + 1LL) ||
+      overlap(out, n_out, parent, n_tokens) ||
+      overlap(out, n_out, static_cast<unsigned char*>(ws), static_cast<long long>(l.bytes)))
+    return set_error(SG_ERR_INVALID_ARGUMENT,
+                     "%s: out overlaps the cache, win_off, parent or the workspace", nm);
   AttnArgs a;
   a.q = q;
   a.k = k;
@@ -1176,8 +1186,8 @@ int sg_attn_tree_f16(const uint16_t* q, const uint16_t* k, const uint16_t* v, lo
   a.q_stride = q_stride;
   a.k_stride = k_stride;
   a.v_stride = v_stride;
-  a.kc = cache->k + layer * cache->layer_stride;
-  a.vc = cache->v + layer * cache->layer_stride;
+  a.kc = kc;
+  a.vc = vc;
   a.pages = cache->pages;
   a.length = cache->length;
   a.win_off = win_off;

@@ -84,3 +84,21 @@ def test_verify_outputs_over_what_is_read(lib):
         for other in set(size) - {out}:
             for at in (a[other], a[other] + size[other] - 4, a[other] - size[out] + 4):
                 refused(lambda: call(**{out: at}), (out, other, at), lib)
+
+
+def test_attention_output_over_cache_and_workspace(lib):
+    n_seq, T, W, heads, kv, D, n_pages, page, per = 3, 7, 4, 8, 2, 128, 9, 16, 4
+    need = lib.sg_attn_tree_workspace_bytes(n_seq, W, 4000, heads, kv, D)
+    assert need > 0
+    layer = n_pages * kv * page * D
+    size = dict(q=T * heads * D * 2, k=T * kv * D * 2, v=T * kv * D * 2, kc=layer * 2, vc=layer * 2,
+                pages=n_seq * per * 4, length=n_seq * 4, off=(n_seq + 1) * 4, parent=T * 4, ws=need)
+    a, n_out = apart(*size), T * heads * D * 2
+    c = sager_amd.KvCacheDesc(a["kc"] - 2 * layer, a["vc"] - 2 * layer, a["pages"], a["length"],
+                              layer, 2, n_pages, page, per, kv, D)
+    for other in size:
+        for at in (a[other], a[other] + (size[other] - 2) // 8 * 8, a[other] - n_out + 8):
+            refused(lambda: lib.sg_attn_tree_f16(
+                P(a["q"]), P(a["k"]), P(a["v"]), heads * D, kv * D, kv * D, ctypes.byref(c), 1,
+                P(a["off"]), P(a["parent"]), P(at), P(a["ws"]), need, n_seq, T, W, 4000, heads, 0.1,
+                None), (other, at), lib)
