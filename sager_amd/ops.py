@@ -656,7 +656,11 @@ class KvCache:
     """A paged fp16 key/value cache: k, v [n_layers, n_pages, n_kv_heads,
     page_size, head_dim], pages int32 [n_seq, pages_per_seq], length int32
     [n_seq].  Holds the tensors; nothing is copied, and what changes between
-    steps changes in place (length.copy_(...), pages[s, i] = ...)."""
+    steps changes in place (length.copy_(...), pages[s, i] = ...).  The library
+    has the tensors' addresses: none of the four can be replaced by another."""
+
+    k, v, pages, length = (property(lambda self, n=n: self._tensors[n])
+                           for n in ("k", "v", "pages", "length"))
 
     def __init__(self, k, v, pages, length):
         if k.dim() != 5 or k.shape != v.shape:
@@ -667,7 +671,7 @@ class KvCache:
             raise SagerError("the cache's tensors must be on one device")
         _dtypes("KvCache", k=(k, torch.float16), v=(v, torch.float16), pages=(pages, torch.int32),
                 length=(length, torch.int32))
-        self.k, self.v, self.pages, self.length = k, v, pages, length
+        self._tensors = dict(k=k, v=v, pages=pages, length=length)
         self.device = k.get_device()
         self.n_layers, P, self.n_kv_heads, S, self.head_dim = k.shape
         self.max_seqs = pages.shape[0]
