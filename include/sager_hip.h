@@ -552,7 +552,8 @@ typedef struct sg_kv_cache {
  * elements from one token to the next (slices of one projection's output),
  * out contiguous and apart from them and from all else that is read.  k, v, the cache's k and v and their
  * strides are 16-B aligned.  Scores, softmax statistics and sums are fp32; the weights p are
- * rounded to fp16 for the product with v.  max_len bounds the caches'
+ * rounded to fp16 for the product with v (one of less than 2^-33 of the row's largest adds to
+ * their sum only).  max_len bounds the caches'
  * lengths for the choice of the launches; longer caches are right, but may
  * be slower.  Workspace: sg_attn_tree_workspace_bytes of as many sequences or
  * more (it may be 0 bytes); it belongs to one call at a time.  One launch, or

@@ -19,11 +19,13 @@
 //                     its own and reads all of K and V from LDS; P stays in
 //                     its lanes, and one barrier a step orders the copies.
 //
-// A row's running maximum is a reference point `mref` that moves only when a
-// score passes it by 2^15: p = 2^(s - mref) fits fp16 (its largest value is
-// 2^16), and 2^(8+15) below it is still a normal number.  p is rounded to
-// fp16 for the product (2^-11 of each weight, no more than the output's own
-// rounding to fp16); l = sum p is fp32, of the unrounded p.
+// A row's running maximum is a reference point `mref`, set 8 (in powers of 2)
+// below the largest score of its step, that moves only when a score passes it
+// by 15: p = 2^(s - mref) is at most 2^15, which fits fp16.  p is rounded to
+// fp16 for the product: 2^-11 of a weight, no more than the output's own
+// rounding, down to 2^-22 of the largest; below it 2^-33 of the largest, so
+// that smaller weights bring nothing (131,072 keys that all have just that
+// little together 2^-16).  l = sum p is fp32, of the unrounded p.
 #include "sg_window.hpp"
 
 namespace sg {
