@@ -392,13 +392,18 @@ def traffic_run(torch, np, ops, gen, layers, n_steps=32):
     return 0
 
 
+# the sources of the kernels below, with what they include: other operators
+# beside them change nothing of what was counted
+TRAFFIC_SOURCES = ("sg_common.hpp", "sg_gemv.hip", "sg_layer.hip", "sg_prefill.hip", "sg_router.hpp")
+
+
 def source_hash():
-    """sha256 of the kernel sources (sager_amd/csrc), to tie a committed
-    counter summary to the build it describes."""
+    """sha256 of the sources of the counted kernels (of sager_amd/csrc), to tie
+    a committed counter summary to the build it describes."""
     import hashlib
     h = hashlib.sha256()
     d = os.path.join(ROOT, "sager_amd", "csrc")
-    for f in sorted(os.listdir(d)):
+    for f in TRAFFIC_SOURCES:
         h.update(f.encode())
         with open(os.path.join(d, f), "rb") as fh:
             h.update(fh.read())
