@@ -362,9 +362,9 @@ struct Part {
   }
   // Waits for Q before the loop: left to the compiler, the waits stand at Q's
   // uses inside it, where they wait for the copies just issued as well. Over
-  // many steps that costs (a tree of 64 over 131,071 tokens: 194 us against
-  // 189); the small blocks do few steps, and there the first step's start
-  // weighs more (four tokens over 4,096: 15.2 us against 15.8 with it).
+  // many steps that costs (a pass of a tree of 64 over 131,071 tokens: 167 us
+  // against 162); the small blocks do few steps, and there the first step's
+  // start weighs more (four tokens over 4,099: 14.1 us against 14.6 with it).
   template <int RT>
   static __device__ __forceinline__ void settle_q(h8 (&q)[RT][KK]) {
 #pragma unroll
@@ -664,7 +664,8 @@ struct RowsLds {
 // Bound by the matrix cores and the vector instructions between the products:
 // a wave's registers (128 of O, 64 of Q at dimension 256) leave two waves a
 // SIMD.  64 tokens of 16 heads over 131,071 cached ones, 2 kv heads of 256: 137
-// GFLOP in 158 us, 870 TFLOP/s (a large matrix product here: 1,190); the matrix
+// GFLOP in 166 us under the profiler, 830 TFLOP/s (a large matrix product here:
+// 1,190; a pass of this launch and the join among others 162 us); the matrix
 // cores are busy 45 % of the cycles, vector instructions some 30 %, the LDS
 // 23 %.  (Wave priorities around either phase: 2 to 20 us more; half of the
 // waves a phase behind the others, with a second barrier a step: 8 more.)

@@ -175,8 +175,9 @@ __device__ __forceinline__ bool node_ok(const Node& n, int i) {
 // Grid: (chunk, node, sequence); the workgroup past the chunks of node 0
 // does the tree.  64 rows of 248,320 take 19.7 us, 3.2 TB/s: 14 fp64 operations
 // a logit, with memory close behind them; 4 rows 4.8 us, one round of loads.
-// (Workgroups of several chunks, with the next one's logits under way: 22 us
-// for the 64 rows; 512 threads of 8 logits: 20.)
+// (When the 64 rows took 17 us, with weights of fewer bits: workgroups of
+// several chunks, the next one's logits under way, 22; 512 threads of 8 logits
+// 20.)
 __global__ void __launch_bounds__(256) verify_rows_kernel(const VerifyArgs a) {
   const int s = blockIdx.z, node = blockIdx.y, c = blockIdx.x;
   const Window w = window_of(a.win_off, s, a.n_tokens, a.max_window);
@@ -907,8 +908,8 @@ int sg_tree_verify(const float* logits, const int* tokens, const int* win_off, c
   const hipStream_t s = static_cast<hipStream_t>(stream);
   // Two chunks a workgroup where there are several rounds of workgroups: what it
   // finds out before its first logit then serves both (64 rows of 248,320 with
-  // three children a node 93 us, 100 with one chunk, 97 with four; five rows of
-  // 128,256 26 with one, 31 with two).
+  // three children a node 96 us, 100 with one chunk, 98 with four; five rows of
+  // 128,256 25 with one, 29 with two).
   const long long chunks = static_cast<long long>(a.n_chunks) * max_window * n_seq;
   const int per = chunks >= 2048 ? 2 : 1;
   const dim3 grid((a.n_chunks + per - 1) / per, max_window, n_seq);
