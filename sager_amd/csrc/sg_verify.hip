@@ -337,40 +337,32 @@ __device__ __forceinline__ double rest_sum(const VerifyArgs& a, long long row, i
   for (int c = lane; c < a.n_chunks; c += 64) s += a.rest[row * a.n_chunks + c];
   return wave_sum(s);
 }
-// The row's sum of weights without the tokens of the lanes of `out`, by one wave: the chunks' sums
-// as they are, and a chunk with such a token weight by weight.
-__device__ __forceinline__ double row_without(const VerifyArgs& a, long long row, RowStat r, int tok,
-                                              uint64_t out, double k, int lane) {
+// The row's sum of weights without n tokens, this wave's part of it: the chunks' sums as they are, and
+// a chunk with such a token weight by weight.
+__device__ __forceinline__ double part_without(const VerifyArgs& a, long long row, float m,
+                                               const int* toks, int n, double k) {
   const float* x = a.logits + row * a.vocab;
-  auto of = [&](uint64_t b) { return __builtin_amdgcn_readlane(tok, __builtin_ctzll(b)); };
   double s = 0.0;
-  for (int c = lane; c < a.n_chunks; c += 64) {
+  for (int c = threadIdx.x; c < a.n_chunks; c += kWalk) {
     const float cm = a.cmax[row * a.n_chunks + c];
     bool has = false;
-    for (uint64_t b = out; b; b &= b - 1) has |= of(b) / kChunk == c;
-    if (!has && cm > -INFINITY) s += (a.csum[row * a.n_chunks + c] + 1.0) * weight(cm, r.m, k);
+    for (int i = 0; i < n; ++i) has |= toks[i] / kChunk == c;
+    if (!has && cm > -INFINITY) s += (a.csum[row * a.n_chunks + c] + 1.0) * weight(cm, m, k);
   }
-  for (uint64_t b = out; b; b &= b - 1) {
-    const int c = of(b) / kChunk;
-    bool again = false;  // (of several in a chunk, the last one's turn)
-    for (uint64_t o = b & (b - 1); o; o &= o - 1) again |= of(o) / kChunk == c;
+  for (int i = 0; i < n; ++i) {
+    const int c = toks[i] / kChunk;
+    bool again = false;
+    for (int j = 0; j < i; ++j) again |= toks[j] / kChunk == c;
     if (again) continue;
-    constexpr int kLoads = 16;  // under way at once
-#pragma unroll 1
-    for (int v0 = c * kChunk + lane; v0 < a.vocab && v0 < (c + 1) * kChunk; v0 += 64 * kLoads) {
-      float xv[kLoads];
+    const int v0 = c * kChunk + 4 * threadIdx.x;
+    float xv[4];
 #pragma unroll
-      for (int i = 0; i < kLoads; ++i) {
-        const int v = v0 + 64 * i;
-        xv[i] = v < a.vocab ? no_nan(x[v]) : -INFINITY;
-      }
+    for (int h = 0; h < 4; ++h) xv[h] = v0 + h < a.vocab ? no_nan(x[v0 + h]) : -INFINITY;
+    for (int j = 0; j < n; ++j)
 #pragma unroll
-      for (int i = 0; i < kLoads; ++i) {
-        bool is = false;
-        for (uint64_t o = out; o; o &= o - 1) is |= of(o) == v0 + 64 * i;
-        if (!is) s += weight(xv[i], r.m, k);
-      }
-    }
+      for (int h = 0; h < 4; ++h) xv[h] = toks[j] == v0 + h ? -INFINITY : xv[h];
+#pragma unroll
+    for (int h = 0; h < 4; ++h) s += weight(xv[h], m, k);
   }
   return wave_sum(s);
 }
@@ -524,6 +516,8 @@ __global__ void __launch_bounds__(kWalk) verify_walk_kernel(const VerifyArgs a) 
   __shared__ int kid_tok[kMaxWindow];   // the end's children whose share is taken
   __shared__ int s_end, s_kids;
   __shared__ double ws[kWalk / 64];
+  // What all waves sum for the one that goes down the tree: a node's row (-1: no more) without tokens
+  __shared__ int job, job_n, job_tok[kMaxWindow];
   __shared__ Chain chain;
   const float t = a.temperature[s];
   const float us = a.u_sample[s];
@@ -615,7 +609,19 @@ __global__ void __launch_bounds__(kWalk) verify_walk_kernel(const VerifyArgs a) 
             const int l = __builtin_ctzll(b);
             const uint64_t out = (__shfl(n.sib, l) & gone) | 1ull << l;
             const int at = __builtin_amdgcn_readlane(up, l);
-            const double sum = row_without(a, w.off + at, stat[at], n.tok, out, k, lane);
+            if (out >> lane & 1) job_tok[__popcll(out & ((1ull << lane) - 1))] = n.tok;
+            if (lane == 0) {
+              job = at;
+              job_n = __popcll(out);
+            }
+            bar();
+            const double part =
+                part_without(a, w.off + at, stat[at].m, job_tok, __popcll(out), k);
+            if (lane == 0) ws[0] = part;
+            bar();
+            double sum = 0.0;
+#pragma unroll
+            for (int i = 0; i < kWalk / 64; ++i) sum += ws[i];
             if (lane == l) {
               all = sum / stat[at].s;
               less = 0.0;
@@ -632,6 +638,8 @@ __global__ void __launch_bounds__(kWalk) verify_walk_kernel(const VerifyArgs a) 
         asm volatile("" ::: "memory");  // (whole and taken are other lanes' next)
       }
       if (lane < w.n) left[lane] = gone >> lane & 1 ? 1.0 : 0.0;
+      if (lane == 0) job = -1;
+      bar();
     }
     const double bar = q * m;
     const bool ok = in && static_cast<double>(u) * bar < r;
@@ -664,6 +672,15 @@ __global__ void __launch_bounds__(kWalk) verify_walk_kernel(const VerifyArgs a) 
       s_end = at;
       s_kids = min(__popcll(kid), most);
       a.n_path[s] = np;
+    }
+  } else if (!a.draft) {
+    while (true) {
+      bar();
+      const int at = job;
+      if (at < 0) break;
+      const double part = part_without(a, w.off + at, stat[at].m, job_tok, job_n, k);
+      if (lane == 0) ws[wave] = part;
+      bar();
     }
   }
   __syncthreads();

@@ -229,3 +229,34 @@ def test_verify_windows_that_share_rows(off, sampled):
         assert (nxt >= -1).all() and (nxt < 311).all()
     for a, b in zip(base, w.run_verify(c)):
         np.testing.assert_array_equal(a, b)
+
+
+@pytest.mark.parametrize("vocab", [2000, 20011])
+def test_verify_nearly_certain_pairs_at_every_node(vocab):
+    """Three windows, in whose trees every node's first two children of four have all but 1e-8."""
+    rng = np.random.default_rng(vocab)
+    n, n_seq = 64, 3
+    par = np.array([-1] + [(i - 1) // 4 for i in range(1, n)], np.int32)
+    x = rng.normal(0, 1, (n_seq * n, vocab)).astype(np.float32)
+    tok = rng.integers(0, vocab, n_seq * n).astype(np.int32)
+    want = np.ones(n_seq * n)
+    for s in range(n_seq):
+        for i in range(n):
+            kids = [s * n + c for c in range(n) if par[c] == i]
+            while len({tok[c] for c in kids}) < len(kids):
+                tok[kids] = rng.integers(0, vocab, len(kids))
+            row = x[s * n + i]
+            if len(kids) > 1:
+                row[tok[kids[:2]]] = -np.inf
+                top = np.log(np.exp(row.astype(np.float64)).sum() * (1e8 - 1))
+                row[tok[kids[:2]]] = top + np.log([0.9, 0.1])
+            p = ref.weights(row, 1.0)
+            for c in kids:  # (sums without what is rejected: no differences)
+                want[c] = p[tok[c]] / p.sum()
+                p[tok[c]] = 0
+    c = dict(logits=x, tokens=tok, off=(n * np.arange(n_seq + 1)).astype(np.int32),
+             parent=np.tile(par, n_seq), draft=None, temp=np.ones(n_seq, np.float32),
+             u_acc=np.full(n_seq * n, 1 - 2.0 ** -24, np.float32),
+             u_smp=np.full(n_seq, 0.5, np.float32))
+    got = w.run_verify(c)[3]
+    assert (np.abs(got - want) <= want * (w.U32 + 2.0 ** -26)).all(), np.abs(got / want - 1).max()
