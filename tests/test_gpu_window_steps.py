@@ -23,9 +23,9 @@ U16, U32 = w.U16, w.U32
 FORMS = [(3, 4), (13, 3), (40, 5), (64, 8)]
 
 
-def uncut_case(seed, window, group, D, lengths, n_kv=2, page=16, absent=True):
+def uncut_case(seed, window, group, D, lengths, n_kv=2, page=16, absent=True, sharp=1.0):
     return w.attn_case(seed, [window, max(1, window - 5)][:len(lengths)], lengths, n_kv, group, D,
-                       page, branch=2, absent=absent, pad=2)
+                       page, branch=2, absent=absent, pad=2, sharp=sharp)
 
 
 def run(c, max_len):
@@ -165,8 +165,7 @@ def test_attention_reference_point_moves(D, window, group, max_len):
 @pytest.mark.parametrize("D", [64, 128, 256])
 def test_attention_of_sharp_scores(D, window, group):
     """Scores of a spread of 8, so that the reference point moves now and then; pages absent."""
-    c = uncut_case(D - window, window, group, D, [905, 64])
-    c["q"] = (c["q"].astype(np.float32) * 8).astype(np.float16)
+    c = uncut_case(D - window, window, group, D, [905, 64], sharp=8.0)
     c["pages"][0, 5::9] = -1
     check(c)
 
