@@ -581,6 +581,101 @@ int sg_kv_commit_f16(const uint16_t* k, const uint16_t* v, long long k_stride, l
                      const int* win_off, const int* path, const int* n_path, int* length_out,
                      int n_seq, int n_tokens, int max_window, void* stream);
 
+/* The same for whole windows, chains of any length (a prompt's chunk): row
+ * win_off[s] + i becomes token length[s] + i. */
+int sg_kv_append_f16(const uint16_t* k, const uint16_t* v, long long k_stride, long long v_stride,
+                     long long k_layer_stride, long long v_layer_stride, const sg_kv_cache* cache,
+                     const int* win_off, int* length_out, int n_seq, int n_tokens, int max_window,
+                     void* stream);
+
+/* ---- rotary positions, a quantised cache, sliding attention ---------------
+ * The windows are those of the verify window's calls; without a parent they
+ * may be longer than 64 (a prompt's chunk). */
+
+/* The heads' norms and rotary positions of q and k, in one launch:
+ *   y = (x / sqrt(mean(x^2) + eps)) * w   over each head's head_dim values
+ * (q_norm, k_norm: w, fp32 [head_dim]; NULL: y = x), then each pair (a, b) of
+ * the head's first rot_dim values turned by its angle:
+ *   (a c - b s, b c + a s),  c, s = mscale * cos, sin(2 pi turns[i] position).
+ * Pair i is (i, i + rot_dim / 2), or (2 i, 2 i + 1) with neighbours.  turns:
+ * fp64 [rot_dim / 2] on the device, as sg_rope_turns makes them.  Angles are
+ * reduced in fp64, all else is fp32, the result rounded once.
+ * A row's position is positions[row], or without positions that of its window:
+ * length[s] + its depth in the tree (parent) or its place in the chain.  Then
+ * rows behind the last sequence and absent nodes are neither read nor written.
+ * q [n_tokens][n_heads][head_dim], k [n_tokens][n_kv_heads][head_dim] (k may
+ * be left out, n_kv_heads 0), strides in elements from token to token; each
+ * output may be its own input (in place), any other overlap is refused.
+ * head_dim is a multiple of 8, at most 512.  (Norms and RoPE of the reference:
+ * norm_rotary.cu.) */
+int sg_rope(const float* q, const float* k, float* q_out, float* k_out, long long q_stride,
+            long long k_stride, long long qo_stride, long long ko_stride, const float* q_norm,
+            const float* k_norm, float eps, const double* turns, float mscale,
+            const int* positions, const int* win_off, const int* parent, const int* length,
+            int n_tokens, int n_seq, int n_heads, int n_kv_heads, int head_dim, int rot_dim,
+            int neighbours, void* stream);
+int sg_rope_f16(const uint16_t* q, const uint16_t* k, uint16_t* q_out, uint16_t* k_out,
+                long long q_stride, long long k_stride, long long qo_stride, long long ko_stride,
+                const float* q_norm, const float* k_norm, float eps, const double* turns,
+                float mscale, const int* positions, const int* win_off, const int* parent,
+                const int* length, int n_tokens, int n_seq, int n_heads, int n_kv_heads,
+                int head_dim, int rot_dim, int neighbours, void* stream);
+
+/* The table of sg_rope, on the host: turns[i] = f_i / (2 pi) with f_i =
+ * base^(-2 i / rot_dim), stretched for contexts `factor` times longer than
+ * the trained one (`trained` tokens):
+ *   SG_ROPE_PLAIN     not at all;
+ *   SG_ROPE_LINEAR    f / factor;
+ *   SG_ROPE_BY_INDEX  f / factor * r + f * (1 - r), r rising from 0 to 1
+ *                     between the indices (down and up to whole ones) of the
+ *                     pairs that turn `fast` and `slow` times in a trained
+ *                     context (YaRN as GGUF files mean it);
+ *   SG_ROPE_BY_TURNS  the same with 1 - r rising from 0 to 1 between `slow`
+ *                     and `fast` turns in a trained context. */
+enum { SG_ROPE_PLAIN = 0, SG_ROPE_LINEAR = 1, SG_ROPE_BY_INDEX = 2, SG_ROPE_BY_TURNS = 3 };
+int sg_rope_turns(double* turns, int rot_dim, double base, int scaling, double factor,
+                  double trained, double slow, double fast);
+
+/* The paged cache with 8 bits a value: as sg_kv_cache, k and v int8 codes
+ * [n_layers][n_pages][n_kv_heads][page_size][head_dim] and for each group of
+ * 32 values of a head an fp16 scale, [n_layers][n_pages][n_kv_heads]
+ * [page_size][head_dim / 32]; a value is code * scale.  layer_stride: codes
+ * from one layer to the next, a multiple of 512 (scales: layer_stride / 32).
+ * All four are 16-B aligned. */
+typedef struct sg_kv_cache_q8 {
+  int8_t* k;
+  int8_t* v;
+  uint16_t* k_scale;
+  uint16_t* v_scale;
+  const int* pages;
+  const int* length;
+  long long layer_stride;
+  int n_layers, n_pages, page_size, pages_per_seq, n_kv_heads, head_dim;
+} sg_kv_cache_q8;
+
+/* sg_kv_commit_f16 and sg_kv_append_f16 into it, quantised on the way:
+ * scale = fp16(largest |x| / 127), at most 515.5 (127 of which are still
+ * finite), code = x / scale to the nearest whole number, ties to even, within
+ * +-127.  A group with an infinity or a NaN reads back as NaN. */
+int sg_kv_commit_q8(const uint16_t* k, const uint16_t* v, long long k_stride, long long v_stride,
+                    long long k_layer_stride, long long v_layer_stride, const sg_kv_cache_q8* cache,
+                    const int* win_off, const int* path, const int* n_path, int* length_out,
+                    int n_seq, int n_tokens, int max_window, void* stream);
+int sg_kv_append_q8(const uint16_t* k, const uint16_t* v, long long k_stride, long long v_stride,
+                    long long k_layer_stride, long long v_layer_stride, const sg_kv_cache_q8* cache,
+                    const int* win_off, int* length_out, int n_seq, int n_tokens, int max_window,
+                    void* stream);
+
+/* Tokens read back as fp16 rows, every layer in one launch: row row_off[s] + i
+ * of k and v ([n_rows][n_kv_heads][head_dim] a layer) becomes token first[s] +
+ * i, code * scale rounded once; 0 for a token on an absent page or past the
+ * page table.  What is read does not depend on the cache's lengths.  row_off:
+ * n_seq + 1 device ints, ascending; rows behind the last are left as they
+ * were.  k and v are apart from each other and from all that is read. */
+int sg_kv_read_q8(const sg_kv_cache_q8* cache, const int* first, const int* row_off, uint16_t* k,
+                  uint16_t* v, long long k_stride, long long v_stride, long long k_layer_stride,
+                  long long v_layer_stride, int n_seq, int n_rows, void* stream);
+
 /* Which drafts the target's probabilities accept, from given random numbers.
  * logits [n_tokens][vocab] fp32 are the target's after each node, p their
  * softmax at the sequence's temperature (0, negative or NaN: all on the

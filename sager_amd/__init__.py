@@ -23,6 +23,7 @@ _I = ctypes.c_int
 _F = ctypes.c_float
 _SZ = ctypes.c_size_t
 _LL = ctypes.c_longlong
+_D = ctypes.c_double
 
 
 class KvCacheDesc(ctypes.Structure):
@@ -30,6 +31,13 @@ class KvCacheDesc(ctypes.Structure):
     _fields_ = [("k", _VP), ("v", _VP), ("pages", _VP), ("length", _VP), ("layer_stride", _LL),
                 ("n_layers", _I), ("n_pages", _I), ("page_size", _I), ("pages_per_seq", _I),
                 ("n_kv_heads", _I), ("head_dim", _I)]
+
+
+class KvCacheQ8Desc(ctypes.Structure):
+    """sg_kv_cache_q8 of include/sager_hip.h."""
+    _fields_ = [("k", _VP), ("v", _VP), ("k_scale", _VP), ("v_scale", _VP), ("pages", _VP),
+                ("length", _VP), ("layer_stride", _LL), ("n_layers", _I), ("n_pages", _I),
+                ("page_size", _I), ("pages_per_seq", _I), ("n_kv_heads", _I), ("head_dim", _I)]
 
 
 # name -> (restype, argtypes); mirrors include/sager_hip.h
@@ -94,6 +102,16 @@ SIGNATURES = {
                               _I, _I, _I, _I, _F, _VP]),
     "sg_kv_commit_f16": (_I, [_VP, _VP, _LL, _LL, _LL, _LL, _VP, _VP, _VP, _VP, _VP, _I, _I, _I,
                               _VP]),
+    "sg_kv_append_f16": (_I, [_VP, _VP, _LL, _LL, _LL, _LL, _VP, _VP, _VP, _I, _I, _I, _VP]),
+    "sg_rope": (_I, [_VP, _VP, _VP, _VP, _LL, _LL, _LL, _LL, _VP, _VP, _F, _VP, _F, _VP, _VP, _VP,
+                     _VP, _I, _I, _I, _I, _I, _I, _I, _VP]),
+    "sg_rope_f16": (_I, [_VP, _VP, _VP, _VP, _LL, _LL, _LL, _LL, _VP, _VP, _F, _VP, _F, _VP, _VP,
+                         _VP, _VP, _I, _I, _I, _I, _I, _I, _I, _VP]),
+    "sg_rope_turns": (_I, [_VP, _I, _D, _I, _D, _D, _D, _D]),
+    "sg_kv_commit_q8": (_I, [_VP, _VP, _LL, _LL, _LL, _LL, _VP, _VP, _VP, _VP, _VP, _I, _I, _I,
+                             _VP]),
+    "sg_kv_append_q8": (_I, [_VP, _VP, _LL, _LL, _LL, _LL, _VP, _VP, _VP, _I, _I, _I, _VP]),
+    "sg_kv_read_q8": (_I, [_VP, _VP, _VP, _VP, _VP, _LL, _LL, _LL, _LL, _I, _I, _VP]),
     "sg_tree_verify_workspace_bytes": (_SZ, [_I, _I, _I]),
     "sg_tree_verify": (_I, [_VP, _VP, _VP, _VP, _VP, _VP, _VP, _VP, _VP, _VP, _VP, _VP, _VP, _SZ,
                             _I, _I, _I, _I, _I, _VP]),

@@ -26,14 +26,13 @@
 // rounding, down to 2^-22 of the largest; below it 2^-33 of the largest, so
 // that smaller weights bring nothing (131,072 keys that all have just that
 // little together 2^-16).  l = sum p is fp32, of the unrounded p.
-#include "sg_window.hpp"
+#include "sg_cache.hpp"
 
 namespace sg {
 
 typedef _Float16 h4 __attribute__((ext_vector_type(4)));
 typedef _Float16 h8 __attribute__((ext_vector_type(8)));
 typedef float f4 __attribute__((ext_vector_type(4)));
-typedef uint32_t u32x4_u __attribute__((ext_vector_type(4), aligned(2)));
 typedef short s4 __attribute__((ext_vector_type(4)));
 typedef __attribute__((address_space(3))) s4* lds_s4_p;
 typedef __attribute__((address_space(3))) unsigned char* lds_char_p;
@@ -949,7 +948,7 @@ __global__ void __launch_bounds__(kJoinThreads<D>) attn_join_kernel(const AttnAr
   }
 }
 
-// ---- the accepted tokens into the cache --------------------------------------
+// ---- the accepted tokens into the cache, or whole windows (no path) -----------
 struct CommitArgs {
   const uint16_t *k, *v;
   long long k_stride, v_stride, k_layer, v_layer, layer_stride;
@@ -968,7 +967,8 @@ struct CommitArgs {
 constexpr int kCommitLayers = 8;
 __global__ void __launch_bounds__(256) kv_commit_kernel(const CommitArgs a) {
   const int s = blockIdx.y, l0 = blockIdx.z * kCommitLayers;
-  const int n = min(max(a.n_path[s], 0), a.max_window);
+  const Window w = window_of(a.win_off, s, a.n_tokens, a.max_window);
+  const int n = a.path ? min(max(a.n_path[s], 0), a.max_window) : w.n;
   const int len = a.length[s];
   if (a.length_out && blockIdx.x == 0 && l0 == 0 && threadIdx.x == 0) a.length_out[s] = len + n;
   const int pieces = a.n_kv * (a.dim / 8);
@@ -977,10 +977,9 @@ __global__ void __launch_bounds__(256) kv_commit_kernel(const CommitArgs a) {
   x >>= 1;
   const int i = x / pieces;
   if (i >= n) return;
-  const Window w = window_of(a.win_off, s, a.n_tokens, a.max_window);
   x -= i * pieces;
   const int h = x / (a.dim / 8), c = x - h * (a.dim / 8);
-  const int node = a.path[static_cast<long long>(s) * a.max_window + i];
+  const int node = a.path ? a.path[static_cast<long long>(s) * a.max_window + i] : i;
   const long long pos = static_cast<long long>(len) + i;
   if (len < 0 || node < 0 || node >= w.n || pos >> a.page_log2 >= a.pages_per_seq) return;
   const int page = a.pages[static_cast<long long>(s) * a.pages_per_seq + (pos >> a.page_log2)];
@@ -1005,41 +1004,6 @@ __global__ void __launch_bounds__(256) kv_commit_kernel(const CommitArgs a) {
 }
 
 // ---- host -----------------------------------------------------------------------
-
-static int log2_of(int v) {
-  int l = 0;
-  while ((1 << l) < v) ++l;
-  return l;
-}
-
-static int check_cache(const sg_kv_cache* c, int n_seq, int n_tokens, int max_window,
-                       const char* nm) {
-  if (!c || !c->k || !c->v || !c->pages || !c->length)
-    return set_error(SG_ERR_INVALID_ARGUMENT, "%s: null cache", nm);
-  if (n_seq <= 0 || n_tokens <= 0 || max_window <= 0 || c->n_layers <= 0 || c->n_pages <= 0 ||
-      c->pages_per_seq <= 0 || c->n_kv_heads <= 0)
-    return set_error(SG_ERR_GEOMETRY,
-                     "%s: n_seq=%d n_tokens=%d max_window=%d n_layers=%d n_pages=%d "
-                     "pages_per_seq=%d n_kv_heads=%d must be positive",
-                     nm, n_seq, n_tokens, max_window, c->n_layers, c->n_pages, c->pages_per_seq,
-                     c->n_kv_heads);
-  if (max_window > kMaxWindow)
-    return set_error(SG_ERR_UNSUPPORTED, "%s: max_window=%d is over %d", nm, max_window,
-                     kMaxWindow);
-  if (c->head_dim != 64 && c->head_dim != 128 && c->head_dim != 256)
-    return set_error(SG_ERR_UNSUPPORTED, "%s: head_dim=%d is not 64, 128 or 256", nm, c->head_dim);
-  if (c->page_size < 16 || (c->page_size & (c->page_size - 1)) != 0)
-    return set_error(SG_ERR_UNSUPPORTED, "%s: page_size=%d is no power of two from 16 on", nm,
-                     c->page_size);
-  // token positions are 32-bit
-  if ((static_cast<long long>(c->pages_per_seq) << log2_of(c->page_size)) > 0x7FFFF000LL)
-    return set_error(SG_ERR_UNSUPPORTED, "%s: a sequence of %d pages of %d tokens is too long", nm,
-                     c->pages_per_seq, c->page_size);
-  if ((reinterpret_cast<uintptr_t>(c->k) | reinterpret_cast<uintptr_t>(c->v)) % 16 ||
-      c->layer_stride % 8)
-    return set_error(SG_ERR_INVALID_ARGUMENT, "%s: the cache is not 16-B aligned", nm);
-  return SG_OK;
-}
 
 // How a call is laid out: rows of a workgroup, the most units.
 struct Layout {
@@ -1109,6 +1073,62 @@ static int attn_launch(const AttnArgs& a, hipStream_t s, const char* nm) {
     return check_launch(nm);
   }
   return SG_OK;
+}
+
+static int commit(const uint16_t* k, const uint16_t* v, long long k_stride, long long v_stride,
+                  long long k_layer_stride, long long v_layer_stride, const sg_kv_cache* cache,
+                  const int* win_off, const int* path, const int* n_path, int* length_out,
+                  int n_seq, int n_tokens, int max_window, int most, void* stream, const char* nm) {
+  if (!k || !v || !win_off) return set_error(SG_ERR_INVALID_ARGUMENT, "%s: null pointer", nm);
+  if (int st = check_cache(cache, n_seq, n_tokens, max_window, nm, most)) return st;
+  const long long row = static_cast<long long>(cache->n_kv_heads) * cache->head_dim;
+  if (k_stride < row || v_stride < row)
+    return set_error(SG_ERR_GEOMETRY, "%s: a token stride is less than a token", nm);
+  if (reinterpret_cast<uintptr_t>(k) % 2 || reinterpret_cast<uintptr_t>(v) % 2)
+    return set_error(SG_ERR_INVALID_ARGUMENT, "%s: k and v must be 2-B aligned", nm);
+  const long long pieces = 2LL * max_window * (row / 8);
+  if (n_seq > 65535 || cache->n_layers > 65535 || pieces > 0x7FFFFFFF - 256)
+    return set_error(SG_ERR_UNSUPPORTED, "%s: n_seq=%d n_layers=%d n_kv_heads=%d", nm, n_seq,
+                     cache->n_layers, cache->n_kv_heads);
+  // (a sequence's first workgroup writes its new length, the others read on)
+  const long long paths = static_cast<long long>(n_seq) * max_window;
+  const long long pages = static_cast<long long>(n_seq) * cache->pages_per_seq;
+  if (length_out &&
+      (overlap(length_out, n_seq, cache->length, n_seq) || overlap(length_out, n_seq, n_path, n_seq) ||
+       overlap(length_out, n_seq, path, paths) || overlap(length_out, n_seq, win_off, n_seq + 1LL) ||
+       overlap(length_out, n_seq, cache->pages, pages)))
+    return set_error(SG_ERR_INVALID_ARGUMENT,
+                     "%s: length_out overlaps the cache's lengths or pages, n_path, path or win_off",
+                     nm);
+  CommitArgs a;
+  a.k = k;
+  a.v = v;
+  a.k_stride = k_stride;
+  a.v_stride = v_stride;
+  a.k_layer = k_layer_stride;
+  a.v_layer = v_layer_stride;
+  a.layer_stride = cache->layer_stride;
+  a.kc = cache->k;
+  a.vc = cache->v;
+  a.pages = cache->pages;
+  a.length = cache->length;
+  a.win_off = win_off;
+  a.path = path;
+  a.n_path = n_path;
+  a.length_out = length_out;
+  a.n_tokens = n_tokens;
+  a.max_window = max_window;
+  a.n_layers = cache->n_layers;
+  a.n_kv = cache->n_kv_heads;
+  a.dim = cache->head_dim;
+  a.n_pages = cache->n_pages;
+  a.page_log2 = log2_of(cache->page_size);
+  a.pages_per_seq = cache->pages_per_seq;
+  hipLaunchKernelGGL(kv_commit_kernel,
+                     dim3(static_cast<unsigned>((pieces + 255) / 256), n_seq,
+                          (cache->n_layers + kCommitLayers - 1) / kCommitLayers),
+                     dim3(256), 0, static_cast<hipStream_t>(stream), a);
+  return check_launch(nm);
 }
 
 }  // namespace sg
@@ -1226,58 +1246,18 @@ int sg_kv_commit_f16(const uint16_t* k, const uint16_t* v, long long k_stride, l
                      const int* win_off, const int* path, const int* n_path, int* length_out,
                      int n_seq, int n_tokens, int max_window, void* stream) {
   const char* nm = "sg_kv_commit_f16";
-  using namespace sg;
-  if (!k || !v || !win_off || !path || !n_path)
-    return set_error(SG_ERR_INVALID_ARGUMENT, "%s: null pointer", nm);
-  if (int st = check_cache(cache, n_seq, n_tokens, max_window, nm)) return st;
-  const long long row = static_cast<long long>(cache->n_kv_heads) * cache->head_dim;
-  if (k_stride < row || v_stride < row)
-    return set_error(SG_ERR_GEOMETRY, "%s: a token stride is less than a token", nm);
-  if (reinterpret_cast<uintptr_t>(k) % 2 || reinterpret_cast<uintptr_t>(v) % 2)
-    return set_error(SG_ERR_INVALID_ARGUMENT, "%s: k and v must be 2-B aligned", nm);
-  const long long pieces = 2LL * max_window * (row / 8);
-  if (n_seq > 65535 || cache->n_layers > 65535 || pieces > 0x7FFFFFFF - 256)
-    return set_error(SG_ERR_UNSUPPORTED, "%s: n_seq=%d n_layers=%d n_kv_heads=%d", nm, n_seq,
-                     cache->n_layers, cache->n_kv_heads);
-  // (a sequence's first workgroup writes its new length, the others read on)
-  const long long paths = static_cast<long long>(n_seq) * max_window;
-  const long long pages = static_cast<long long>(n_seq) * cache->pages_per_seq;
-  if (length_out &&
-      (overlap(length_out, n_seq, cache->length, n_seq) || overlap(length_out, n_seq, n_path, n_seq) ||
-       overlap(length_out, n_seq, path, paths) || overlap(length_out, n_seq, win_off, n_seq + 1LL) ||
-       overlap(length_out, n_seq, cache->pages, pages)))
-    return set_error(SG_ERR_INVALID_ARGUMENT,
-                     "%s: length_out overlaps the cache's lengths or pages, n_path, path or win_off",
-                     nm);
-  CommitArgs a;
-  a.k = k;
-  a.v = v;
-  a.k_stride = k_stride;
-  a.v_stride = v_stride;
-  a.k_layer = k_layer_stride;
-  a.v_layer = v_layer_stride;
-  a.layer_stride = cache->layer_stride;
-  a.kc = cache->k;
-  a.vc = cache->v;
-  a.pages = cache->pages;
-  a.length = cache->length;
-  a.win_off = win_off;
-  a.path = path;
-  a.n_path = n_path;
-  a.length_out = length_out;
-  a.n_tokens = n_tokens;
-  a.max_window = max_window;
-  a.n_layers = cache->n_layers;
-  a.n_kv = cache->n_kv_heads;
-  a.dim = cache->head_dim;
-  a.n_pages = cache->n_pages;
-  a.page_log2 = log2_of(cache->page_size);
-  a.pages_per_seq = cache->pages_per_seq;
-  hipLaunchKernelGGL(kv_commit_kernel,
-                     dim3(static_cast<unsigned>((pieces + 255) / 256), n_seq,
-                          (cache->n_layers + kCommitLayers - 1) / kCommitLayers),
-                     dim3(256), 0, static_cast<hipStream_t>(stream), a);
-  return check_launch(nm);
+  if (!path || !n_path) return sg::set_error(SG_ERR_INVALID_ARGUMENT, "%s: null pointer", nm);
+  return sg::commit(k, v, k_stride, v_stride, k_layer_stride, v_layer_stride, cache, win_off, path,
+                    n_path, length_out, n_seq, n_tokens, max_window, sg::kMaxWindow, stream, nm);
+}
+
+int sg_kv_append_f16(const uint16_t* k, const uint16_t* v, long long k_stride, long long v_stride,
+                     long long k_layer_stride, long long v_layer_stride, const sg_kv_cache* cache,
+                     const int* win_off, int* length_out, int n_seq, int n_tokens, int max_window,
+                     void* stream) {
+  return sg::commit(k, v, k_stride, v_stride, k_layer_stride, v_layer_stride, cache, win_off,
+                    nullptr, nullptr, length_out, n_seq, n_tokens, max_window, 0x7FFFF000, stream,
+                    "sg_kv_append_f16");
 }
 
 }  // extern "C"

@@ -21,6 +21,19 @@ __device__ __forceinline__ Window window_of(const int* __restrict__ win_off, int
   return w;
 }
 
+// The sequence that row t lies in (the last one, if it lies behind them all), for the calling wave.
+__device__ __forceinline__ int seq_of_row(const int* __restrict__ win_off, int n_seq, int t,
+                                          int lane) {
+  int lo = 0, n = n_seq;
+  while (n > 0) {  // the windows that end before t, counted 64 blocks of them at a time
+    const int step = (n + 63) / 64, i = lane * step + step - 1;
+    const int c = __popcll(__ballot(i < n && win_off[lo + i + 1] <= t));
+    lo += c * step;
+    n = step == 1 ? 0 : min(step - 1, n - c * step);
+  }
+  return min(lo, n_seq - 1);
+}
+
 // The ancestors of node `lane` and itself as a mask of nodes, for the calling
 // wave; 0 for a node that does not hang on the root (node 0).  `up` is the
 // node's parent, or the node itself where it has none that counts.

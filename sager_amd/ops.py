@@ -13,7 +13,7 @@ import ctypes
 import numpy as np
 import torch
 
-from . import Q4K_BYTES, Q8K_BYTES, QK, KvCacheDesc, load
+from . import Q4K_BYTES, Q8K_BYTES, QK, KvCacheDesc, KvCacheQ8Desc, load
 
 
 class SagerError(RuntimeError):
@@ -628,13 +628,13 @@ def add_rmsnorm_q8_k(x, w, eps, y=None, x_out=None, xn=None, xq=None):
     return x if y is None else x_out, xn, xq
 
 
-def _rows(fn, name, t, shape, dev):
-    """The address and the leading dimensions' strides (elements) of an fp16
+def _rows(fn, name, t, shape, dev, dtype=torch.float16):
+    """The address and the leading dimensions' strides (elements) of a
     tensor [..., tokens, heads, dim] whose tokens may lie apart."""
     st, heads, dim = t.stride(), shape[-2], shape[-1]
-    if t.dtype is not torch.float16 or t.shape != shape or t.get_device() != dev or st[-1] != 1 or \
+    if t.dtype is not dtype or t.shape != shape or t.get_device() != dev or st[-1] != 1 or \
             (st[-2] != dim and heads > 1):
-        raise SagerError(f"{fn}: {name} must be fp16 {tuple(shape)} on GPU {dev}, a token's values "
+        raise SagerError(f"{fn}: {name} must be {dtype} {tuple(shape)} on GPU {dev}, a token's values "
                          f"contiguous, got {t.dtype} {tuple(t.shape)} strides {st} on {t.device}")
     if 1 in shape:  # (a dimension of one element has any stride)
         st = [x if n > 1 else max(x, heads * dim) for n, x in zip(shape, st)]
@@ -679,9 +679,23 @@ class KvCache:
                                 self.n_layers, P, S, pages.shape[1], self.n_kv_heads, self.head_dim)
         self._desc = ctypes.byref(self.desc)
 
+    _COMMIT, _APPEND = "sg_kv_commit_f16", "sg_kv_append_f16"
+
+    def _new_rows(self, fn, k, v, win_off):
+        """What commit and append check alike: the device and stream, addresses and strides."""
+        shape = (self.n_layers, k.shape[1], self.n_kv_heads, self.head_dim)
+        dev, stream = _current_of(fn, k)
+        pk, kl, ks = _rows(fn, "k", k, shape, dev)
+        pv, vl, vs = _rows(fn, "v", v, shape, dev)
+        n_seq, off, _ = _windows(fn, win_off, None, k.shape[1], dev)
+        if n_seq > self.max_seqs or self.device != dev:
+            raise SagerError(f"{fn}: {n_seq} sequences on GPU {dev}, the cache has "
+                             f"{self.max_seqs} on GPU {self.device}")
+        return dev, stream, n_seq, (pk, pv, ks, vs, kl, vl, self._desc, off)
+
     def commit(self, k, v, win_off, path, n_path, length_out=None):
         """The accepted tokens' keys and values behind the cache, all layers in
-        one launch (sg_kv_commit_f16): k, v fp16 [n_layers, n_tokens,
+        one launch (sg_kv_commit_f16 / _q8): k, v fp16 [n_layers, n_tokens,
         n_kv_heads, head_dim], path int32 [n_seq, max_window] and n_path int32
         [n_seq] as TreeVerify returns them.  Returns the new lengths (a tensor
         of its own; the cache's own length is left to the caller, since every
@@ -691,20 +705,174 @@ class KvCache:
             raise SagerError(f"{fn}: k must be [n_layers, n_tokens, n_kv_heads, head_dim], path "
                              "[n_seq, max_window]")
         n_tokens, window = k.shape[1], path.shape[1]
-        shape = (self.n_layers, n_tokens, self.n_kv_heads, self.head_dim)
-        dev, stream = _current_of(fn, k)
-        pk, kl, ks = _rows(fn, "k", k, shape, dev)
-        pv, vl, vs = _rows(fn, "v", v, shape, dev)
-        n_seq, off, _ = _windows(fn, win_off, None, n_tokens, dev)
-        if n_seq > self.max_seqs or self.device != dev:
-            raise SagerError(f"{fn}: {n_seq} sequences on GPU {dev}, the cache has "
-                             f"{self.max_seqs} on GPU {self.device}")
+        dev, stream, n_seq, args = self._new_rows(fn, k, v, win_off)
         pp = _arg(fn, "path", path, torch.int32, (n_seq, window), dev)
         pn = _arg(fn, "n_path", n_path, torch.int32, (n_seq,), dev)
         length_out, po = _out(fn, "length_out", length_out, n_path, (n_seq,), dev)
-        _check(load().sg_kv_commit_f16(pk, pv, ks, vs, kl, vl, self._desc, off, pp, pn, po, n_seq,
-                                       n_tokens, window, stream))
+        _check(getattr(load(), self._COMMIT)(*args, pp, pn, po, n_seq, n_tokens, window, stream))
         return length_out
+
+    def append(self, k, v, win_off, max_window=None, length_out=None):
+        """Whole windows behind the cache (sg_kv_append_f16 / _q8): as commit,
+        of every token in its order.  max_window bounds the windows' sizes
+        (None: the number of rows); of a longer one the rest is left out."""
+        fn = "KvCache.append"
+        if k.dim() != 4:
+            raise SagerError(f"{fn}: k must be [n_layers, n_tokens, n_kv_heads, head_dim]")
+        dev, stream, n_seq, args = self._new_rows(fn, k, v, win_off)
+        length_out, po = _out(fn, "length_out", length_out, win_off, (n_seq,), dev)
+        n = k.shape[1]
+        _check(getattr(load(), self._APPEND)(*args, po, n_seq, n,
+                                             n if max_window is None else max_window, stream))
+        return length_out
+
+
+class KvCacheQ8(KvCache):
+    """The paged cache with 8 bits a value: k, v int8 codes [n_layers, n_pages,
+    n_kv_heads, page_size, head_dim], k_scale, v_scale fp16 [..., head_dim /
+    32], pages and length as KvCache's.  commit and append quantise what they
+    write (include/sager_hip.h has the rule), read brings tokens back."""
+
+    _COMMIT, _APPEND = "sg_kv_commit_q8", "sg_kv_append_q8"
+    k_scale, v_scale = (property(lambda self, n=n: self._tensors[n])
+                        for n in ("k_scale", "v_scale"))
+
+    def __init__(self, k, v, k_scale, v_scale, pages, length):
+        if k.dim() != 5 or k.shape != v.shape or k.shape[-1] % 32 != 0:
+            raise SagerError("k and v must be [n_layers, n_pages, n_kv_heads, page_size, head_dim]")
+        if k_scale.shape != (*k.shape[:4], k.shape[4] // 32) or v_scale.shape != k_scale.shape:
+            raise SagerError("k_scale and v_scale must be [n_layers, n_pages, n_kv_heads, "
+                             "page_size, head_dim / 32]")
+        if pages.dim() != 2 or length.numel() != pages.shape[0]:
+            raise SagerError("pages must be [n_seq, pages_per_seq], length [n_seq]")
+        tensors = dict(k=k, v=v, k_scale=k_scale, v_scale=v_scale, pages=pages, length=length)
+        if len({t.device for t in tensors.values()}) != 1:
+            raise SagerError("the cache's tensors must be on one device")
+        f16, i8, i32 = torch.float16, torch.int8, torch.int32
+        _dtypes("KvCacheQ8", k=(k, i8), v=(v, i8), k_scale=(k_scale, f16), v_scale=(v_scale, f16),
+                pages=(pages, i32), length=(length, i32))
+        self._tensors = tensors
+        self.device = k.get_device()
+        self.n_layers, P, self.n_kv_heads, S, self.head_dim = k.shape
+        self.max_seqs = pages.shape[0]
+        self.desc = KvCacheQ8Desc(*(_ptr(t) for t in tensors.values()), k[0].numel(), self.n_layers,
+                                  P, S, pages.shape[1], self.n_kv_heads, self.head_dim)
+        self._desc = ctypes.byref(self.desc)
+
+    @classmethod
+    def empty(cls, n_layers, n_pages, n_kv_heads, page_size, head_dim, pages, length):
+        """A cache of zeros on the device of pages."""
+        shape, dev = (n_layers, n_pages, n_kv_heads, page_size), pages.device
+        k, v = (torch.zeros((*shape, head_dim), dtype=torch.int8, device=dev) for _ in range(2))
+        ks, vs = (torch.zeros((*shape, head_dim // 32), dtype=torch.float16, device=dev)
+                  for _ in range(2))
+        return cls(k, v, ks, vs, pages, length)
+
+    def read(self, first, row_off, n_rows=None, k_out=None, v_out=None):
+        """Tokens first[s] + i of sequence s as rows row_off[s] + i of k_out and
+        v_out, fp16 [n_layers, n_rows, n_kv_heads, head_dim] (sg_kv_read_q8):
+        first int32 [n_seq], row_off int32 [n_seq + 1].  n_rows is needed
+        without outputs; rows of those behind the last sequence are left as
+        they are (0 in new ones).  Returns (k_out, v_out)."""
+        fn = "KvCacheQ8.read"
+        given = v_out if k_out is None else k_out
+        if n_rows is None and given is None or given is not None and given.dim() != 4:
+            raise SagerError(f"{fn}: n_rows, or an output [n_layers, n_rows, n_kv_heads, head_dim], "
+                             "is needed")
+        n_rows = n_rows if given is None else given.shape[1]
+        dev, stream = _current_of(fn, first)
+        if self.device != dev:
+            raise SagerError(f"{fn}: the cache is on GPU {self.device}, not {dev}")
+        shape = (self.n_layers, n_rows, self.n_kv_heads, self.head_dim)
+        if k_out is None:
+            k_out = torch.zeros(shape, dtype=torch.float16, device=first.device)
+        if v_out is None:
+            v_out = torch.zeros(shape, dtype=torch.float16, device=first.device)
+        pk, kl, ks = _rows(fn, "k_out", k_out, shape, dev)
+        pv, vl, vs = _rows(fn, "v_out", v_out, shape, dev)
+        n_seq, off, _ = _windows(fn, row_off, None, n_rows, dev)
+        if n_seq > self.max_seqs:
+            raise SagerError(f"{fn}: {n_seq} sequences, the cache has {self.max_seqs}")
+        _check(load().sg_kv_read_q8(self._desc, _arg(fn, "first", first, torch.int32, (n_seq,), dev),
+                                    off, pk, pv, ks, vs, kl, vl, n_seq, n_rows, stream))
+        return k_out, v_out
+
+
+ROPE_SCALINGS = {None: 0, "linear": 1, "yarn": 2, "by_turns": 3}
+
+
+def rope_frequencies(rot_dim, base=10000.0, scaling=None, factor=1.0, trained=0, slow=1.0,
+                     fast=None, device="cuda"):
+    """The table that rope takes (sg_rope_turns): turns a position of each of
+    the rot_dim / 2 pairs, fp64 on `device`.  scaling: None, "linear", "yarn"
+    (a ramp over the pairs' indices) or "by_turns" (a ramp over their turns in
+    a trained context), for contexts `factor` times longer than `trained`
+    tokens; slow and fast (32, "by_turns" 4) are the ramp's ends in turns.
+    rope's mscale goes with "yarn": 0.1 ln(factor) + 1 is usual."""
+    if scaling not in ROPE_SCALINGS:
+        raise SagerError(f"rope_frequencies: scaling {scaling!r} is none of {list(ROPE_SCALINGS)}")
+    if fast is None:
+        fast = 4.0 if scaling == "by_turns" else 32.0
+    t = torch.empty(max(rot_dim // 2, 1), dtype=torch.float64)
+    _check(load().sg_rope_turns(t.data_ptr(), rot_dim, base, ROPE_SCALINGS[scaling], factor,
+                                trained, slow, fast))
+    return t.to(device)
+
+
+def rope(q, k, table, positions=None, win_off=None, parent=None, length=None, interleaved=False,
+         mscale=1.0, q_norm=None, k_norm=None, eps=1e-6, q_out=None, k_out=None):
+    """The heads' norms (q_norm, k_norm fp32 [head_dim] or None) and rotary
+    positions of q [n_tokens, n_heads, head_dim] and k [n_tokens, n_kv_heads,
+    head_dim] (or None), fp16 or fp32, slices of one projection's output or
+    not, in one launch (sg_rope / _f16).  table: rope_frequencies(...), of as
+    many values of a head as are turned.  A row's position: positions int32
+    [n_tokens], or length[s] + its depth in its window (win_off, parent,
+    length int32 [n_seq]: the cache's).  In place unless q_out and k_out are
+    given; returns (q_out, k_out)."""
+    fn, dt = "rope", q.dtype
+    if q.dim() != 3 or (k is not None and k.dim() != 3):
+        raise SagerError(f"{fn}: q must be [n_tokens, n_heads, head_dim], k likewise")
+    if dt is torch.float16:
+        entry = load().sg_rope_f16
+    elif dt is torch.float32:
+        entry = load().sg_rope
+    else:
+        raise SagerError(f"{fn}: q must be fp32 or fp16")
+    dev, stream = _current_of(fn, q)
+    T, H, D = shape = q.shape
+    K, i32 = 0, torch.int32
+    q_out = q if q_out is None else q_out
+    pq, qs = _rows(fn, "q", q, shape, dev, dt)
+    pqo, qos = (pq, qs) if q_out is q else _rows(fn, "q_out", q_out, shape, dev, dt)
+    pk = pko = None
+    ks = kos = 0
+    if k is not None:
+        K = k.shape[1]
+        k_out = k if k_out is None else k_out
+        pk, ks = _rows(fn, "k", k, (T, K, D), dev, dt)
+        pko, kos = (pk, ks) if k_out is k else _rows(fn, "k_out", k_out, (T, K, D), dev, dt)
+    elif k_out is not None:
+        raise SagerError(f"{fn}: k_out needs k")
+    half = table.numel()
+    pos = off = par = pl = None
+    n_seq = 0
+    if positions is not None:
+        if win_off is not None or parent is not None or length is not None:
+            raise SagerError(f"{fn}: either positions or windows")
+        pos = _arg(fn, "positions", positions, i32, (T,), dev)
+    elif win_off is None or length is None:
+        raise SagerError(f"{fn}: positions, or win_off and length, are needed")
+    else:
+        n_seq, off, par = _windows(fn, win_off, parent, T, dev)
+        if length.dim() != 1 or length.numel() < n_seq:
+            raise SagerError(f"{fn}: length must be [n_seq]")
+        pl = _arg(fn, "length", length, i32, length.shape, dev)
+    _check(entry(pq, pk, pqo, pko, qs, ks, qos, kos,
+                 None if q_norm is None else _arg(fn, "q_norm", q_norm, torch.float32, (D,), dev),
+                 None if k_norm is None else _arg(fn, "k_norm", k_norm, torch.float32, (D,), dev),
+                 eps, _arg(fn, "table", table, torch.float64, (half,), dev), mscale, pos, off, par,
+                 pl, T, n_seq, H, K, D, 2 * half, interleaved, stream))
+    return q_out, k_out
 
 
 class TreeAttention:
