@@ -676,6 +676,29 @@ int sg_kv_read_q8(const sg_kv_cache_q8* cache, const int* first, const int* row_
                   uint16_t* v, long long k_stride, long long v_stride, long long k_layer_stride,
                   long long v_layer_stride, int n_seq, int n_rows, void* stream);
 
+/* sg_attn_tree_f16 over a sliding window of positions and the first tokens,
+ * over either cache: a token at position p (the cache's length plus its depth
+ * in the tree, or its place in the chain) sees of what it would see there the
+ * keys of positions above p - reach (its own among them) and below sinks.
+ * reach 0: all of them.  Pages that nobody sees any more may be absent.
+ * With a parent a window has at most 64 nodes; without one (chains) it may
+ * have any number, a prompt's whole chunk.  A quantised value is rounded to
+ * fp16 once, as code * scale; the rest is as for sg_attn_tree_f16.
+ * Workspace: sg_attn_sliding_workspace_bytes of as many sequences or more, of
+ * the same reach and sinks. */
+size_t sg_attn_sliding_workspace_bytes(int n_seq, int max_window, int max_len, int n_heads,
+                                       int n_kv_heads, int head_dim, int reach, int sinks);
+int sg_attn_sliding_f16(const uint16_t* q, const uint16_t* k, const uint16_t* v, long long q_stride,
+                        long long k_stride, long long v_stride, const sg_kv_cache* cache, int layer,
+                        const int* win_off, const int* parent, uint16_t* out, void* ws,
+                        size_t ws_bytes, int n_seq, int n_tokens, int max_window, int max_len,
+                        int n_heads, float scale, int reach, int sinks, void* stream);
+int sg_attn_sliding_q8(const uint16_t* q, const uint16_t* k, const uint16_t* v, long long q_stride,
+                       long long k_stride, long long v_stride, const sg_kv_cache_q8* cache, int layer,
+                       const int* win_off, const int* parent, uint16_t* out, void* ws,
+                       size_t ws_bytes, int n_seq, int n_tokens, int max_window, int max_len,
+                       int n_heads, float scale, int reach, int sinks, void* stream);
+
 /* Which drafts the target's probabilities accept, from given random numbers.
  * logits [n_tokens][vocab] fp32 are the target's after each node, p their
  * softmax at the sequence's temperature (0, negative or NaN: all on the

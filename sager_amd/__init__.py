@@ -112,6 +112,11 @@ SIGNATURES = {
                              _VP]),
     "sg_kv_append_q8": (_I, [_VP, _VP, _LL, _LL, _LL, _LL, _VP, _VP, _VP, _I, _I, _I, _VP]),
     "sg_kv_read_q8": (_I, [_VP, _VP, _VP, _VP, _VP, _LL, _LL, _LL, _LL, _I, _I, _VP]),
+    "sg_attn_sliding_workspace_bytes": (_SZ, [_I, _I, _I, _I, _I, _I, _I, _I]),
+    "sg_attn_sliding_f16": (_I, [_VP, _VP, _VP, _LL, _LL, _LL, _VP, _I, _VP, _VP, _VP, _VP, _SZ,
+                                 _I, _I, _I, _I, _I, _F, _I, _I, _VP]),
+    "sg_attn_sliding_q8": (_I, [_VP, _VP, _VP, _LL, _LL, _LL, _VP, _I, _VP, _VP, _VP, _VP, _SZ,
+                                _I, _I, _I, _I, _I, _F, _I, _I, _VP]),
     "sg_tree_verify_workspace_bytes": (_SZ, [_I, _I, _I]),
     "sg_tree_verify": (_I, [_VP, _VP, _VP, _VP, _VP, _VP, _VP, _VP, _VP, _VP, _VP, _VP, _VP, _SZ,
                             _I, _I, _I, _I, _I, _VP]),

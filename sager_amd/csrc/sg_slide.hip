@@ -1,0 +1,769 @@
+// sg_slide.hip - attention over a 16-bit or a quantised cache, over all of it
+// or over a sliding window and the first tokens (the sinks).
+//
+// A token at position p sees its ancestors (in a chain: all before it) and
+// itself, as far as they are less than `reach` positions back or among the
+// first `sinks` positions.  The keys come in steps of 64: the cache's steps,
+// then the window's own, so that a step is all of one kind; the steps that no
+// row of a block sees are passed over.  The two products, the running
+// reference point of a row's weights and the cut of a batch into units are
+// those of sg_attn.hip.
+//
+// slide_few_kernel: blocks of 16 or 32 rows.  Four waves share the keys of the
+// first product and the columns of the second, as there, but K and V come
+// through registers: a wave's keys are nobody else's, so K needs no LDS at
+// all, and V's columns go through a corner of LDS that is the wave's own,
+// where ds_read_b64_tr_b16 turns them.  Codes become 16-bit numbers on that
+// way (their product with the scale is rounded once, 2^-12 of the value at the
+// most, as a 16-bit cache's own values are).  Only P is exchanged, so a step
+// has one barrier, and a step's loads are under way during the one before.
+//
+// V at infinity or NaN where some rows see it and others do not: a product
+// with a weight of 0 would spread it.  Weights that are 0 because the key is
+// not seen are written as -0; in a step with such a V the second product is
+// made one by one, without those.
+#include <type_traits>
+
+#include "sg_attn.hpp"
+
+namespace sg {
+
+struct SlideArgs : AttnArgs {
+  const uint16_t *ks, *vs;  // scales of the quantised cache (kc, vc: its codes)
+  int reach, sinks;
+};
+
+// The steps that a sequence's nodes first .. last see: [0, sink) and [low,
+// high), the window's steps from `cached` on.
+struct Steps {
+  int cached, sink, low, high;
+  __device__ __forceinline__ int count() const { return low > sink ? sink + high - low : high; }
+  __device__ __forceinline__ int at(int v) const {  // the v-th of them
+    return low > sink && v >= sink ? v - sink + low : v;
+  }
+  __device__ __forceinline__ int skip(int s) const {  // s, or the next that is seen
+    return s >= sink && s < low ? low : s;
+  }
+};
+__device__ __forceinline__ Steps steps_seen(int len, int n, int first, int last, int reach,
+                                            int sinks) {
+  Steps t;
+  t.cached = (len + kKeys - 1) / kKeys;
+  t.high = t.cached + last / kKeys + 1;
+  const int s = min(sinks, len + n);
+  t.sink = min(s <= len ? (s + kKeys - 1) / kKeys : t.cached + (s - len + kKeys - 1) / kKeys, t.high);
+  const long long l = static_cast<long long>(len) + first - reach + 1;  // the first position seen
+  t.low = l <= 0 ? 0
+                 : static_cast<int>(l < len ? l / kKeys : t.cached + (l - len) / kKeys);
+  return t;
+}
+__device__ __forceinline__ int steps_of(const SlideArgs& a, int seq, int* len, Window* win) {
+  if (seq >= a.n_seq) return 0;
+  *win = window_of(a.win_off, seq, a.n_tokens, a.max_window);
+  *len = cached_len(a.length[seq], a.page_log2, a.pages_per_seq);
+  return win->n > 0 ? steps_seen(*len, win->n, 0, win->n - 1, a.reach, a.sinks).count() : 0;
+}
+
+template <int D>
+struct SlidePart : Part<D> {
+  typedef Part<D> B;
+  const SlideArgs& sa;
+  Steps steps;
+  int first, last;  // nodes of the block
+
+  __device__ __forceinline__ explicit SlidePart(const SlideArgs& s) : B{s}, sa(s) {}
+
+  // Finds the block's work; its steps are steps.skip(begin) .. end - 1.
+  __device__ __forceinline__ bool start(unsigned char* l) {
+    this->lds = l;
+    this->lds0 = static_cast<uint32_t>(reinterpret_cast<uintptr_t>((lds_char_p)l));
+    const int lane = threadIdx.x & 63;
+    this->lane = lane;
+    this->col = lane & 15;
+    this->grp = lane >> 4;
+    const int id = blockIdx.x;
+    // The row blocks of a unit are 8 workgroups apart: on one XCD, whose L2 then
+    // reads the unit's keys once.
+    const int oct = id / (8 * sa.row_blocks), in = id - oct * 8 * sa.row_blocks;
+    this->rb = in >> 3;
+    this->unit = oct * 8 + (in & 7);
+    Unit u;
+    const bool plan = sa.cut && id == 0 && __builtin_amdgcn_readfirstlane(threadIdx.x >> 6) == 0;
+    if (!find_unit(sa, this->unit, lane, plan, u)) return false;
+    auto one = [](int v) { return __builtin_amdgcn_readfirstlane(v); };  // (the same in every lane)
+    this->h = one(u.h);
+    this->parts = one(u.parts);
+    this->win = Window{one(u.win.off), one(u.win.n)};
+    this->rows = this->win.n * sa.group;
+    if (this->rb * sa.block_rows >= this->rows) return false;
+    this->len = one(u.len);
+    this->total = this->len + this->win.n;
+    this->table =
+        (const_int_p)(sa.pages + static_cast<long long>(one(u.seq)) * sa.pages_per_seq);
+    const int n = this->win.n;
+    first = sa.parent ? 0 : this->rb * sa.block_rows / sa.group;
+    last = sa.parent ? n - 1 : min((this->rb + 1) * sa.block_rows - 1, this->rows - 1) / sa.group;
+    const Steps all = steps_seen(this->len, n, 0, n - 1, sa.reach, sa.sinks);
+    steps = steps_seen(this->len, n, first, last, sa.reach, sa.sinks);
+    const int k = one(u.k), part = one(u.part), count = one(u.steps);
+    const long long from = static_cast<long long>(k) * part;
+    const int v0 = from < count ? static_cast<int>(from) : count;
+    const int v1 = k == this->parts - 1 || from + part > count ? count : static_cast<int>(from + part);
+    this->begin = v0 < v1 ? steps.skip(all.at(v0)) : 0;
+    this->end = v0 < v1 ? min(all.at(v1 - 1) + 1, steps.high) : 0;
+    return true;
+  }
+  // The pages of a cached step's four blocks of 16 keys; -1: absent, or behind the cache.
+  __device__ __forceinline__ void pages_of(int s, int (&p)[4]) const {
+#pragma unroll
+    for (int b = 0; b < 4; ++b) {
+      const int j = s * kKeys + 16 * b;
+      p[b] = s < steps.cached && j < this->len ? this->table[j >> sa.page_log2] : -1;
+      if (!this->page_ok(p[b])) p[b] = -1;
+    }
+  }
+  // Whether every row of the block sees every key of step s.
+  __device__ __forceinline__ bool full(int s, const int (&p)[4]) const {
+    const int len = this->len;
+    if (s < steps.cached)
+      return (p[0] | p[1] | p[2] | p[3]) >= 0 && (s + 1) * kKeys <= len &&
+             ((s + 1) * kKeys <= sa.sinks ||
+              s * kKeys > static_cast<long long>(len) + last - sa.reach);
+    const int w = (s - steps.cached) * kKeys;
+    return !sa.parent && w + kKeys - 1 <= first &&
+           (len + w + kKeys <= sa.sinks || w > static_cast<long long>(last) - sa.reach);
+  }
+  // Which of step s's keys are there.
+  __device__ __forceinline__ uint64_t present(int s, const int (&p)[4]) const {
+    const int n = s < steps.cached ? this->len - s * kKeys
+                                   : this->win.n - (s - steps.cached) * kKeys;
+    uint64_t m = n >= kKeys ? ~0ull : (1ull << n) - 1;
+    if (s < steps.cached) {
+#pragma unroll
+      for (int b = 0; b < 4; ++b)
+        if (p[b] < 0) m &= ~(0xFFFFull << (16 * b));
+    }
+    return m;
+  }
+  // bit i: key k + i of step s (i < 4) is there and seen by a row of node `node`
+  // at position pos; up: whom of the window's tree it sees (with a parent).
+  __device__ __forceinline__ uint32_t seen4(int s, int k, uint64_t there, int node, int pos,
+                                            uint64_t up) const {
+    uint32_t m = static_cast<uint32_t>(there >> k) & 15u;
+    const bool cached = s < steps.cached;
+    if (!cached && sa.parent) return m & static_cast<uint32_t>(up >> k);
+    const int p0 = (cached ? s * kKeys : this->len + (s - steps.cached) * kKeys) + k;
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+      const int p = p0 + i;
+      const bool see = p < sa.sinks ? p <= pos : p <= pos && pos - p < sa.reach;
+      m &= see ? ~0u : ~(1u << i);
+    }
+    return m;
+  }
+  // Where the cache's row of head h and slot j of page p begins, in values.
+  __device__ __forceinline__ long long row_at(int p, int j) const {
+    return ((static_cast<long long>(max(p, 0)) * sa.n_kv + this->h) << sa.page_log2) +
+           (j & ((1 << sa.page_log2) - 1));
+  }
+};
+
+// The nodes' positions, and whom of their window each sees, by one wave.
+__device__ __forceinline__ void see_tree(const SlideArgs& a, Window w, int len, int lane, int* pos,
+                                         uint64_t* seen) {
+  uint64_t up = ancestors(a.parent, w, lane);
+  const int depth = __popcll(up) - 1;
+  pos[lane] = len + max(depth, 0);
+  if (a.reach < w.n) {
+    uint64_t near = 0;
+    for (int j = 0; j < w.n; ++j) {
+      const int d = __builtin_amdgcn_readlane(depth, j);
+      if (depth - d < a.reach || len + d < a.sinks) near |= 1ull << j;
+    }
+    up &= near;
+  }
+  seen[lane] = up;
+}
+
+// LDS: V of the four waves, P of two steps, the rows' maxima and sums of the
+// four waves, the nodes' positions and what they see, the flags.
+template <int D, int RT>
+struct SlideFewLds {
+  static constexpr uint32_t kRows = 16 * RT;
+  // A wave's row of V, an odd multiple of 32 B: what a quarter or half of a
+  // wave reads transposed (4 or 8 rows' 32 B) then lies in different banks.
+  static constexpr uint32_t kRow = D == 64 ? 32 : D / 2 + 32;
+  static constexpr uint32_t kWave = kKeys * kRow;
+  static constexpr uint32_t kP = 4 * kWave;
+  static constexpr uint32_t kStepP = kRows * kKeys * 2;
+  static constexpr uint32_t kMax = kP + 2 * kStepP;
+  static constexpr uint32_t kSeen = kMax + 4 * kRows * 4;
+  static constexpr uint32_t kPos = kSeen + kMaxWindow * 8;
+  static constexpr uint32_t kFlags = kPos + kMaxWindow * 4;
+  static constexpr uint32_t kBytes = kFlags + 16;
+};
+
+// RT: tiles of 16 rows.  Wave w has keys 16 w.. of a step in the first product,
+// and columns w D/4 .. of all keys in the second.
+template <int D, int RT, bool Q8>
+__global__ void __launch_bounds__(256) slide_few_kernel(const SlideArgs a) {
+  typedef SlidePart<D> P;
+  typedef SlideFewLds<D, RT> L;
+  constexpr int KK = D / 32, DQ = D / 64, kRows = L::kRows;
+  // A wave's columns of V: LP lanes of 8 values a row, RP rows at once; of
+  // codes, 16 a lane.
+  constexpr int LP = D / 32, RP = 64 / LP, LQ = D / 64, RQ = 64 / LQ;
+  extern __shared__ __attribute__((aligned(16))) unsigned char lds[];
+  const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+  P t(a);
+  if (!t.start(lds)) return;
+  const int lane = t.lane, col = t.col, grp = t.grp, row0 = t.rb * kRows;
+  int* rise = reinterpret_cast<int*>(lds + L::kFlags);  // odd and even: 1 + the last step that moves
+  float* mx = reinterpret_cast<float*>(lds + L::kMax);
+  uint64_t* seen = reinterpret_cast<uint64_t*>(lds + L::kSeen);
+  int* place = reinterpret_cast<int*>(lds + L::kPos);
+  unsigned char* const vl = lds + wave * L::kWave;
+
+  // K: lane (col, grp) has key 16 wave + col; its pieces of 8 values lie at
+  // 32 i + 8 grp, of a quantised cache at 64 (i / 2) + 16 grp + 8 (i % 2).
+  auto piece = [&](int i) {
+    return Q8 ? 64 * (i / 2) + 16 * grp + 8 * (i % 2) : 32 * i + 8 * grp;
+  };
+  u32x4 kr[KK], vr[KK];
+  uint32_t kscale[KK / 2], vscale[LQ];
+  int page[4];
+
+  auto load_k = [&](int s, const int (&pg)[4]) {
+    if (s < t.steps.cached) {
+      const int p = wave == 0 ? pg[0] : wave == 1 ? pg[1] : wave == 2 ? pg[2] : pg[3];
+      const long long at = t.row_at(p, s * kKeys + 16 * wave);
+      if (Q8) {
+        const unsigned char* src = uniform_ptr(reinterpret_cast<const unsigned char*>(a.kc) + at * D);
+        const uint16_t* sc = uniform_ptr(a.ks + at * (D / kKvGroup));
+#pragma unroll
+        for (int i = 0; i < KK / 2; ++i) {
+          kr[i] = *reinterpret_cast<const u32x4*>(src + (col * D + 64 * i + 16 * grp));
+          kscale[i] = sc[col * (D / kKvGroup) + 2 * i + (grp >> 1)];
+        }
+      } else {
+        const uint16_t* src = uniform_ptr(a.kc + at * D);
+#pragma unroll
+        for (int i = 0; i < KK; ++i)
+          kr[i] = *reinterpret_cast<const u32x4*>(src + (col * D + piece(i)));
+      }
+    } else {
+      const int w = min((s - t.steps.cached) * kKeys + 16 * wave + col, t.win.n - 1);
+      const uint16_t* src = a.k + static_cast<long long>(t.win.off + w) * a.k_stride + t.h * D;
+#pragma unroll
+      for (int i = 0; i < KK; ++i) kr[i] = *reinterpret_cast<const u32x4*>(src + piece(i));
+    }
+  };
+  auto load_v = [&](int s, const int (&pg)[4]) {
+    if (s < t.steps.cached) {
+      if (Q8) {
+#pragma unroll
+        for (int i = 0; i < LQ; ++i) {
+          const int r = i * RQ + lane / LQ, b = r >> 4;
+          const int p = b == 0 ? pg[0] : b == 1 ? pg[1] : b == 2 ? pg[2] : pg[3];
+          const long long at =
+              t.row_at(p, s * kKeys + r) * D + wave * (D / 4) + (lane % LQ) * 16;
+          vr[i] = *reinterpret_cast<const u32x4*>(reinterpret_cast<const unsigned char*>(a.vc) + at);
+          vscale[i] = a.vs[at / kKvGroup];
+        }
+      } else {
+#pragma unroll
+        for (int i = 0; i < KK; ++i) {
+          const int r = i * RP + lane / LP, b = r >> 4;
+          const int p = b == 0 ? pg[0] : b == 1 ? pg[1] : b == 2 ? pg[2] : pg[3];
+          const long long at = t.row_at(p, s * kKeys + r) * D + wave * (D / 4) + (lane % LP) * 8;
+          vr[i] = *reinterpret_cast<const u32x4*>(a.vc + at);
+        }
+      }
+    } else {
+#pragma unroll
+      for (int i = 0; i < KK; ++i) {
+        const int w = min((s - t.steps.cached) * kKeys + i * RP + lane / LP, t.win.n - 1);
+        vr[i] = *reinterpret_cast<const u32x4*>(
+            a.v + static_cast<long long>(t.win.off + w) * a.v_stride + t.h * D + wave * (D / 4) +
+            (lane % LP) * 8);
+      }
+    }
+  };
+
+  int step = t.begin;
+  if (step < t.end) {
+    t.pages_of(step, page);
+    load_k(step, page);
+    load_v(step, page);
+  }
+  if (threadIdx.x < 2) rise[threadIdx.x] = 0;
+  if (wave == 3 && a.parent) see_tree(a, t.win, t.len, lane, place, seen);
+
+  h8 qf[RT][KK];
+  f4 acc[RT][DQ];
+  // lim: the score, less mref, above which mref moves: kRise once it is set
+  float mref[RT], l[RT], lim[RT];
+  int node[RT];
+#pragma unroll
+  for (int rt = 0; rt < RT; ++rt) {
+    const int r = min(row0 + rt * 16 + col, t.rows - 1);
+    node[rt] = r / a.group;
+    const uint16_t* qp = a.q + static_cast<long long>(t.win.off + node[rt]) * a.q_stride +
+                         (t.h * a.group + r - node[rt] * a.group) * D;
+#pragma unroll
+    for (int i = 0; i < KK; ++i)
+      qf[rt][i] = __builtin_bit_cast(h8, static_cast<u32x4>(*reinterpret_cast<const u32x4_u*>(qp + piece(i))));
+    mref[rt] = 0.f;
+    l[rt] = 0.f;
+    lim[rt] = -INFINITY;
+#pragma unroll
+    for (int d = 0; d < DQ; ++d) acc[rt][d] = (f4){0.f, 0.f, 0.f, 0.f};
+  }
+  // P: [row][two halves of 32 keys][grp][two blocks of 16 keys][4], 16-B pieces
+  // swizzled over the row's eight
+  const int psw = (col >> 1) & 7;
+  const uint32_t p_out =
+      L::kP + col * 128 + ((((wave >> 1) * 4 + grp) ^ psw) << 4) + (wave & 1) * 8;
+  // V's columns 0..15 of row 4 grp + col / 4 of a 16-key block
+  const uint32_t v_in = wave * L::kWave + (4 * grp + (col >> 2)) * L::kRow + (col & 3) * 8;
+
+  bar();  // the flags are cleared, the tree is there
+  for (int it = 0; step < t.end; ++it) {
+    const int par = it & 1;
+    const bool cached = step < t.steps.cached;
+    const bool full = t.full(step, page);
+    const uint64_t there = full ? ~0ull : t.present(step, page);
+    const int next = t.steps.skip(step + 1);
+    int page_next[4] = {-1, -1, -1, -1};
+    if (next < t.end) t.pages_of(next, page_next);
+
+    f4 s[RT];
+#pragma unroll
+    for (int rt = 0; rt < RT; ++rt) s[rt] = (f4){0.f, 0.f, 0.f, 0.f};
+    if (Q8 && cached) {
+#pragma unroll
+      for (int i = 0; i < KK / 2; ++i) {
+        const h2 d = scale2(kscale[i]);
+#pragma unroll
+        for (int j = 0; j < 2; ++j) {
+          uint32_t w[4];
+          decode4(kr[i][2 * j], d, *reinterpret_cast<uint32_t(*)[2]>(w));
+          decode4(kr[i][2 * j + 1], d, *reinterpret_cast<uint32_t(*)[2]>(w + 2));
+          const h8 kf = __builtin_bit_cast(h8, (u32x4){w[0], w[1], w[2], w[3]});
+#pragma unroll
+          for (int rt = 0; rt < RT; ++rt)
+            s[rt] = __builtin_amdgcn_mfma_f32_16x16x32_f16(kf, qf[rt][2 * i + j], s[rt], 0, 0, 0);
+        }
+      }
+    } else {
+#pragma unroll
+      for (int i = 0; i < KK; ++i)
+#pragma unroll
+        for (int rt = 0; rt < RT; ++rt)
+          s[rt] = __builtin_amdgcn_mfma_f32_16x16x32_f16(__builtin_bit_cast(h8, kr[i]), qf[rt][i],
+                                                         s[rt], 0, 0, 0);
+    }
+    if (next < t.end) load_k(next, page_next);
+
+    float e[RT][4], top[RT], sum[RT];
+    uint32_t see[RT];
+    auto weigh = [&](int rt, float by) {  // row tile rt's p = 2^(e - by), into LDS
+      float p[4];
+      h4 ph;
+#pragma unroll
+      for (int i = 0; i < 4; ++i) {
+        p[i] = __builtin_amdgcn_exp2f(e[rt][i] - by);
+        ph[i] = static_cast<_Float16>(p[i]);
+      }
+      if (!full) {
+#pragma unroll
+        for (int i = 0; i < 4; ++i)
+          if (!(see[rt] >> i & 1)) ph[i] = static_cast<_Float16>(-0.f);
+      }
+      sum[rt] = (p[0] + p[1]) + (p[2] + p[3]);
+      *reinterpret_cast<h4*>(lds + p_out + par * L::kStepP + rt * 16 * 128) = ph;
+    };
+    bool move = false;
+#pragma unroll
+    for (int rt = 0; rt < RT; ++rt) {
+#pragma unroll
+      for (int i = 0; i < 4; ++i) e[rt][i] = __builtin_fmaf(s[rt][i], a.scale_log2, -mref[rt]);
+      see[rt] = 15u;
+      if (!full) {
+        see[rt] = t.seen4(step, 16 * wave + 4 * grp, there, node[rt],
+                          a.parent ? place[node[rt]] : t.len + node[rt],
+                          a.parent ? seen[node[rt]] : 0);
+#pragma unroll
+        for (int i = 0; i < 4; ++i) e[rt][i] = see[rt] >> i & 1 ? e[rt][i] : -INFINITY;
+      }
+      top[rt] = max3(max3(e[rt][0], e[rt][1], e[rt][2]), e[rt][3], e[rt][3]);
+      move |= top[rt] > lim[rt];
+      weigh(rt, 0.f);
+    }
+    if (__any(move)) rise[par] = step + 1;
+
+    // V into the wave's corner; rows that are not there as 0
+    bool odd = false;
+    if (Q8 && cached) {
+#pragma unroll
+      for (int i = 0; i < LQ; ++i) {
+        const int r = i * RQ + lane / LQ;
+        const h2 d = scale2(vscale[i]);
+        const bool some = full || (there >> r & 1);
+        uint32_t w[8];
+#pragma unroll
+        for (int j = 0; j < 4; ++j) decode4(vr[i][j], d, *reinterpret_cast<uint32_t(*)[2]>(w + 2 * j));
+        if (!some) {
+#pragma unroll
+          for (int j = 0; j < 8; ++j) w[j] = 0;
+        }
+        if (!full) odd |= some && fp16_odd(vscale[i]);
+        u32x4* to = reinterpret_cast<u32x4*>(vl + r * L::kRow + (lane % LQ) * 32);
+        to[0] = (u32x4){w[0], w[1], w[2], w[3]};
+        to[1] = (u32x4){w[4], w[5], w[6], w[7]};
+      }
+    } else {
+#pragma unroll
+      for (int i = 0; i < KK; ++i) {
+        const int r = i * RP + lane / LP;
+        u32x4 w = vr[i];
+        if (!full) {
+          const bool some = there >> r & 1;
+#pragma unroll
+          for (int j = 0; j < 4; ++j) {
+            w[j] = some ? w[j] : 0u;
+            odd |= fp16_odd(w[j]) || fp16_odd(w[j] >> 16);
+          }
+        }
+        *reinterpret_cast<u32x4*>(vl + r * L::kRow + (lane % LP) * 16) = w;
+      }
+    }
+    if (next < t.end) load_v(next, page_next);
+    const bool by_one = !full && __any(odd);
+    bar();  // P is here
+
+    if (rise[par] == step + 1) {
+      // The reference points move: the rows' maxima over the waves, then P once more.
+#pragma unroll
+      for (int rt = 0; rt < RT; ++rt) {
+        float m = fmaxf(top[rt], __shfl_xor(top[rt], 16));
+        m = fmaxf(m, __shfl_xor(m, 32));
+        if (grp == 0) mx[wave * kRows + rt * 16 + col] = m;
+      }
+      bar();
+#pragma unroll
+      for (int rt = 0; rt < RT; ++rt) {
+        const float* mr = mx + rt * 16 + col;
+        const float m = fmaxf(fmaxf(mr[0], mr[kRows]), fmaxf(mr[2 * kRows], mr[3 * kRows]));
+        const bool set = m > lim[rt], begun = lim[rt] > 0.f;
+        const float by = set ? m - kBelow : 0.f;
+        const float f = !set ? 1.f : begun ? __builtin_amdgcn_exp2f(-by) : 0.f;
+        mref[rt] += by;
+        l[rt] *= f;
+#pragma unroll
+        for (int d = 0; d < DQ; ++d) acc[rt][d] *= f;
+        lim[rt] = set ? kRise : lim[rt];
+        weigh(rt, by);
+      }
+      bar();
+    }
+#pragma unroll
+    for (int rt = 0; rt < RT; ++rt) l[rt] += sum[rt];
+
+    const unsigned char* const pl = lds + L::kP + par * L::kStepP;
+    if (by_one) {
+#pragma unroll 1
+      for (int r = 0; r < kKeys; ++r) {
+        const int at = (r >> 5) * 4 + ((r & 15) >> 2);
+#pragma unroll
+        for (int rt = 0; rt < RT; ++rt) {
+          const uint32_t w = *reinterpret_cast<const uint16_t*>(
+              pl + (rt * 16 + col) * 128 + ((at ^ psw) << 4) + (r >> 4 & 1) * 8 + (r & 3) * 2);
+          const float p = half_bits_to_float(w);
+#pragma unroll
+          for (int d = 0; d < DQ; ++d) {
+            const h4 v = *reinterpret_cast<const h4*>(vl + r * L::kRow + d * 32 + grp * 8);
+#pragma unroll
+            for (int i = 0; i < 4; ++i)
+              acc[rt][d][i] += w == 0x8000u ? 0.f : p * static_cast<float>(v[i]);
+          }
+        }
+      }
+    } else {
+#pragma unroll
+      for (int st = 0; st < 2; ++st) {
+        h8 pf[RT];
+#pragma unroll
+        for (int rt = 0; rt < RT; ++rt)
+          pf[rt] = *reinterpret_cast<const h8*>(pl + (rt * 16 + col) * 128 +
+                                                (((st * 4 + grp) ^ psw) << 4));
+#pragma unroll
+        for (int d = 0; d < DQ; ++d) {
+          s4 x[2];
+#pragma unroll
+          for (int b = 0; b < 2; ++b)
+            x[b] = __builtin_amdgcn_ds_read_tr16_b64_v4i16(
+                (lds_s4_p)((lds_char_p)lds + v_in + (st * 2 + b) * 16 * L::kRow + d * 32));
+          const h8 vf = __builtin_bit_cast(
+              h8, __builtin_shufflevector(x[0], x[1], 0, 1, 2, 3, 4, 5, 6, 7));
+#pragma unroll
+          for (int rt = 0; rt < RT; ++rt)
+            acc[rt][d] = __builtin_amdgcn_mfma_f32_16x16x32_f16(vf, pf[rt], acc[rt][d], 0, 0, 0);
+        }
+      }
+    }
+    step = next;
+#pragma unroll
+    for (int b = 0; b < 4; ++b) page[b] = page_next[b];
+  }
+
+  // the rows' sums over the waves, and out
+  bar();
+#pragma unroll
+  for (int rt = 0; rt < RT; ++rt) {
+    l[rt] += __shfl_xor(l[rt], 16);
+    l[rt] += __shfl_xor(l[rt], 32);
+    if (grp == 0) mx[wave * kRows + rt * 16 + col] = l[rt];
+  }
+  bar();
+#pragma unroll
+  for (int rt = 0; rt < RT; ++rt) {
+    const int r = row0 + rt * 16 + col;
+    const float* lr = mx + rt * 16 + col;
+    float lt = (lr[0] + lr[kRows]) + (lr[2 * kRows] + lr[3 * kRows]);
+    if (a.parent && !seen[node[rt]]) lt = 0.f;  // an absent node
+    t.template store<DQ, 16>(r, wave * (D / 4) + 4 * grp, acc[rt], mref[rt], lt,
+                             wave == 0 && grp == 0);
+  }
+}
+
+// ---- host -----------------------------------------------------------------------
+
+// How a call is laid out: rows of a workgroup, the most units.
+struct SlideLayout {
+  int block_rows, row_blocks, max_units, goal;
+  bool cut;
+  int few[2];                         // the most sequences for less than one round, and two
+  size_t plan_bytes, o_bytes, bytes;  // of the workspace
+};
+static SlideLayout slide_layout(int n_seq, int max_window, int max_len, int group, int n_kv, int dim,
+                                int reach, int sinks) {
+  SlideLayout l;
+  const long long rows = static_cast<long long>(max_window) * group;
+  l.block_rows = rows > 16 ? 32 : 16;
+  l.row_blocks = static_cast<int>((rows + l.block_rows - 1) / l.block_rows);
+  const long long units = static_cast<long long>(n_seq) * n_kv;
+  // a sequence's steps at the most
+  const long long keys = static_cast<long long>(max_len) + max_window;
+  const long long near = static_cast<long long>(reach) + max_window + sinks + 2 * kKeys;
+  const long long most = ((keys < near ? keys : near) + kKeys - 1) / kKeys + 1;
+  // workgroups that the card holds at once, and units of them
+  const int each = dim == 256 ? 2 : 4;
+  const long long slots = 256 * each;
+  const long long per = 32 * each >= l.row_blocks ? 32 * each / l.row_blocks * 8 : 8;
+  const bool rounds = units >= 2 * slots;
+  for (int i = 0; i < 2; ++i) l.few[i] = static_cast<int>(((i + 1) * slots - 1) / n_kv);
+  long long n = units;
+  l.cut = most > 1 && (units < slots || most > 8);
+  l.goal = 1;
+  if (l.cut && !rounds) {
+    n = (2 * units + per - 1) / per * per;
+    // (a part a head lost to rounding; one in a thousand less: parts_of rounds)
+    l.goal = static_cast<int>(n_seq <= 64 ? n : n - units - ((n - units) >> 10));
+  } else if (l.cut) {
+    n = units + per;
+    l.goal = static_cast<int>(per - ((per + 1023) >> 10));
+  }
+  l.max_units = n > 0x7FFFFF00 ? 0x7FFFFF00 : static_cast<int>(n);
+  const size_t part_rows =
+      static_cast<size_t>((l.max_units + 7LL) / 8 * 8) * l.row_blocks * l.block_rows;
+  l.plan_bytes = l.cut ? (static_cast<size_t>(n_seq) * sizeof(int2) + 15) / 16 * 16 : 0;
+  l.o_bytes = l.cut ? part_rows * dim * sizeof(float) : 0;
+  l.bytes = l.plan_bytes + l.o_bytes + (l.cut ? part_rows * sizeof(float2) : 0);
+  return l;
+}
+
+template <int D, bool Q8>
+static int slide_launch(const SlideArgs& a, hipStream_t s, const char* nm) {
+  const dim3 grid(static_cast<unsigned>((a.max_units + 7LL) / 8 * 8 * a.row_blocks));
+  if (a.block_rows == 32)
+    hipLaunchKernelGGL((slide_few_kernel<D, 2, Q8>), grid, dim3(256), (SlideFewLds<D, 2>::kBytes), s,
+                       a);
+  else
+    hipLaunchKernelGGL((slide_few_kernel<D, 1, Q8>), grid, dim3(256), (SlideFewLds<D, 1>::kBytes), s,
+                       a);
+  if (int st = check_launch(nm)) return st;
+  if (a.cut) {
+    hipLaunchKernelGGL(attn_join_kernel<D>, dim3(a.n_seq * a.max_window * a.n_heads),
+                       dim3(kJoinThreads<D>), 0, s, static_cast<const AttnArgs&>(a));
+    return check_launch(nm);
+  }
+  return SG_OK;
+}
+
+// What the cache is apart from its tables: whether out lies over it, and its layer.
+static bool over_layer(const uint16_t* out, long long n, const sg_kv_cache* c, long long at,
+                       long long values) {
+  return overlap(out, n, c->k + at, values) || overlap(out, n, c->v + at, values);
+}
+static bool over_layer(const uint16_t* out, long long n, const sg_kv_cache_q8* c, long long at,
+                       long long values) {
+  return overlap(out, n, c->k + at, values) || overlap(out, n, c->v + at, values) ||
+         overlap(out, n, c->k_scale + at / kKvGroup, values / kKvGroup) ||
+         overlap(out, n, c->v_scale + at / kKvGroup, values / kKvGroup);
+}
+static void set_layer(SlideArgs& a, const sg_kv_cache* c, long long at) {
+  a.kc = c->k + at;
+  a.vc = c->v + at;
+  a.ks = a.vs = nullptr;
+}
+static void set_layer(SlideArgs& a, const sg_kv_cache_q8* c, long long at) {
+  a.kc = reinterpret_cast<const uint16_t*>(c->k + at);
+  a.vc = reinterpret_cast<const uint16_t*>(c->v + at);
+  a.ks = c->k_scale + at / kKvGroup;
+  a.vs = c->v_scale + at / kKvGroup;
+}
+
+template <typename C>
+static int attn_slide(const uint16_t* q, const uint16_t* k, const uint16_t* v, long long q_stride,
+                      long long k_stride, long long v_stride, const C* cache, int layer,
+                      const int* win_off, const int* parent, uint16_t* out, void* ws,
+                      size_t ws_bytes, int n_seq, int n_tokens, int max_window, int max_len,
+                      int n_heads, float scale, int reach, int sinks, void* stream,
+                      const char* nm) {
+  constexpr bool kQ8 = std::is_same<C, sg_kv_cache_q8>::value;
+  if (!q || !k || !v || !win_off || !out)
+    return set_error(SG_ERR_INVALID_ARGUMENT, "%s: null pointer", nm);
+  if (int st = check_cache(cache, n_seq, n_tokens, max_window, nm, parent ? kMaxWindow : 1 << 24))
+    return st;
+  const int n_kv = cache->n_kv_heads, dim = cache->head_dim;
+  if (layer < 0 || layer >= cache->n_layers || max_len < 0 || n_heads <= 0 || n_heads % n_kv != 0)
+    return set_error(SG_ERR_GEOMETRY, "%s: layer=%d of %d, max_len=%d, n_heads=%d of %d kv heads",
+                     nm, layer, cache->n_layers, max_len, n_heads, n_kv);
+  if (reach < 0 || sinks < 0)
+    return set_error(SG_ERR_GEOMETRY, "%s: reach=%d or sinks=%d is negative", nm, reach, sinks);
+  if (max_len > 0x7FFFF000)
+    return set_error(SG_ERR_UNSUPPORTED, "%s: max_len=%d is too long", nm, max_len);
+  // token positions are 32-bit, the windows' too
+  if ((static_cast<long long>(cache->pages_per_seq) << log2_of(cache->page_size)) + max_window >
+      0x7FFFF000LL)
+    return set_error(SG_ERR_UNSUPPORTED, "%s: a sequence of %d pages and a window of %d is too long",
+                     nm, cache->pages_per_seq, max_window);
+  // (a row's pieces of 16 B lie anywhere in memory; LDS copies need them aligned)
+  if ((reinterpret_cast<uintptr_t>(k) | reinterpret_cast<uintptr_t>(v)) % 16 || k_stride % 8 ||
+      v_stride % 8 || reinterpret_cast<uintptr_t>(q) % 2 || reinterpret_cast<uintptr_t>(out) % 8)
+    return set_error(SG_ERR_INVALID_ARGUMENT, "%s: k and v must be 16-B aligned, out 8-B", nm);
+  if (q_stride < static_cast<long long>(n_heads) * dim ||
+      k_stride < static_cast<long long>(n_kv) * dim || v_stride < static_cast<long long>(n_kv) * dim)
+    return set_error(SG_ERR_GEOMETRY, "%s: a token stride is less than a token", nm);
+  const long long units = static_cast<long long>(n_seq) * n_kv;
+  const long long join = static_cast<long long>(n_seq) * max_window * n_heads;
+  const long long rows = static_cast<long long>(max_window) * (n_heads / n_kv);
+  // a launch has less than 2^32 threads, two units to a kv head; rows are 32-bit
+  if (rows > 0x7FFFF000LL || units * (rows / 16 + 1) > 0x1FFFFF || join * 2 * dim > 0xFFFFFFFFLL)
+    return set_error(SG_ERR_UNSUPPORTED, "%s: too many sequences, or too long windows", nm);
+  const long long last = n_tokens - 1, n_out = static_cast<long long>(n_tokens) * n_heads * dim;
+  if (overlap(out, n_out, q, last * q_stride + n_heads * dim) ||
+      overlap(out, n_out, k, last * k_stride + n_kv * dim) ||
+      overlap(out, n_out, v, last * v_stride + n_kv * dim))
+    return set_error(SG_ERR_INVALID_ARGUMENT, "%s: out overlaps q, k or v", nm);
+  const int far = reach == 0 ? 0x7FFFFFFF : reach;
+  const SlideLayout l =
+      slide_layout(n_seq, max_window, max_len, n_heads / n_kv, n_kv, dim, far, sinks);
+  if (l.bytes && (!ws || ws_bytes < l.bytes || reinterpret_cast<uintptr_t>(ws) % 16))
+    return set_error(SG_ERR_INVALID_ARGUMENT, "%s: the workspace needs %zu bytes, 16-B aligned", nm,
+                     l.bytes);
+  const long long at = layer * cache->layer_stride;
+  const long long values = static_cast<long long>(cache->n_pages) * n_kv * cache->page_size * dim;
+  if (over_layer(out, n_out, cache, at, values) ||
+      overlap(out, n_out, cache->pages, static_cast<long long>(n_seq) * cache->pages_per_seq) ||
+      overlap(out, n_out, cache->length, n_seq) || overlap(out, n_out, win_off, n_seq + 1LL) ||
+      overlap(out, n_out, parent, n_tokens) ||
+      overlap(out, n_out, static_cast<unsigned char*>(ws), static_cast<long long>(l.bytes)))
+    return set_error(SG_ERR_INVALID_ARGUMENT,
+                     "%s: out overlaps the cache, win_off, parent or the workspace", nm);
+  SlideArgs a;
+  a.q = q;
+  a.k = k;
+  a.v = v;
+  a.q_stride = q_stride;
+  a.k_stride = k_stride;
+  a.v_stride = v_stride;
+  set_layer(a, cache, at);
+  a.pages = cache->pages;
+  a.length = cache->length;
+  a.win_off = win_off;
+  a.parent = parent;
+  a.out = out;
+  unsigned char* const w = static_cast<unsigned char*>(ws);
+  a.seq_plan = reinterpret_cast<int2*>(w);
+  a.part_o = reinterpret_cast<float*>(w + l.plan_bytes);
+  a.part_ml = reinterpret_cast<float2*>(w + l.plan_bytes + l.o_bytes);
+  a.n_seq = n_seq;
+  a.n_tokens = n_tokens;
+  a.max_window = max_window;
+  a.n_heads = n_heads;
+  a.n_kv = n_kv;
+  a.group = n_heads / n_kv;
+  a.n_pages = cache->n_pages;
+  a.page_log2 = log2_of(cache->page_size);
+  a.pages_per_seq = cache->pages_per_seq;
+  a.row_blocks = l.row_blocks;
+  a.block_rows = l.block_rows;
+  a.max_units = l.max_units;
+  a.goal = l.goal;
+  a.cut = l.cut;
+  a.scale_log2 = scale * kLog2e;
+  a.reach = far;
+  a.sinks = sinks;
+  const hipStream_t s = static_cast<hipStream_t>(stream);
+  if (dim == 64) return slide_launch<64, kQ8>(a, s, nm);
+  if (dim == 128) return slide_launch<128, kQ8>(a, s, nm);
+  return slide_launch<256, kQ8>(a, s, nm);
+}
+
+}  // namespace sg
+
+extern "C" {
+
+size_t sg_attn_sliding_workspace_bytes(int n_seq, int max_window, int max_len, int n_heads,
+                                       int n_kv_heads, int head_dim, int reach, int sinks) {
+  if (n_seq <= 0 || max_window <= 0 || max_len < 0 || n_kv_heads <= 0 || n_heads <= 0 ||
+      n_heads % n_kv_heads != 0 || reach < 0 || sinks < 0)
+    return 0;
+  // Enough for every smaller batch too: within a way of cutting fewer sequences
+  // have no more units, but fewer may be cut where more are not.
+  const int group = n_heads / n_kv_heads, far = reach == 0 ? 0x7FFFFFFF : reach;
+  const sg::SlideLayout l =
+      sg::slide_layout(n_seq, max_window, max_len, group, n_kv_heads, head_dim, far, sinks);
+  size_t bytes = l.bytes;
+  for (int few : l.few)
+    if (few > 0 && few < n_seq) {
+      const size_t b =
+          sg::slide_layout(few, max_window, max_len, group, n_kv_heads, head_dim, far, sinks).bytes;
+      bytes = b > bytes ? b : bytes;
+    }
+  return bytes;
+}
+
+int sg_attn_sliding_f16(const uint16_t* q, const uint16_t* k, const uint16_t* v, long long q_stride,
+                        long long k_stride, long long v_stride, const sg_kv_cache* cache, int layer,
+                        const int* win_off, const int* parent, uint16_t* out, void* ws,
+                        size_t ws_bytes, int n_seq, int n_tokens, int max_window, int max_len,
+                        int n_heads, float scale, int reach, int sinks, void* stream) {
+  return sg::attn_slide(q, k, v, q_stride, k_stride, v_stride, cache, layer, win_off, parent, out,
+                        ws, ws_bytes, n_seq, n_tokens, max_window, max_len, n_heads, scale, reach,
+                        sinks, stream, "sg_attn_sliding_f16");
+}
+
+int sg_attn_sliding_q8(const uint16_t* q, const uint16_t* k, const uint16_t* v, long long q_stride,
+                       long long k_stride, long long v_stride, const sg_kv_cache_q8* cache, int layer,
+                       const int* win_off, const int* parent, uint16_t* out, void* ws,
+                       size_t ws_bytes, int n_seq, int n_tokens, int max_window, int max_len,
+                       int n_heads, float scale, int reach, int sinks, void* stream) {
+  return sg::attn_slide(q, k, v, q_stride, k_stride, v_stride, cache, layer, win_off, parent, out,
+                        ws, ws_bytes, n_seq, n_tokens, max_window, max_len, n_heads, scale, reach,
+                        sinks, stream, "sg_attn_sliding_q8");
+}
+
+}  // extern "C"

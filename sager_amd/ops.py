@@ -897,7 +897,7 @@ class TreeAttention:
         """q fp16 [n_tokens, n_heads, head_dim], k and v [n_tokens, n_kv_heads,
         head_dim] (slices of one projection's output will do) -> out like q,
         contiguous; scale: 1/sqrt(head_dim) if None."""
-        fn, T, D = "TreeAttention", q.shape[0], self.head_dim
+        fn, T, D = type(self).__name__, q.shape[0], self.head_dim
         shape, kv_shape = (T, self.n_heads, D), (T, self.n_kv_heads, D)
         dev, stream = _current_of(fn, q)
         pq, qs = _rows(fn, "q", q, shape, dev)
@@ -912,12 +912,45 @@ class TreeAttention:
         if out is None:
             out = torch.zeros(shape, dtype=torch.float16, device=q.device)
         ws, ws_bytes = _space(fn, self.workspace if workspace is None else workspace, dev)
-        _check(load().sg_attn_tree_f16(
+        _check(self._entry(fn, cache)(
             pq, pk, pv, qs, ks, vs, cache._desc, layer, off, par,
             _arg(fn, "out", out, torch.float16, shape, dev), ws, ws_bytes, n_seq, T,
             self.max_window, self.max_len, self.n_heads, D ** -0.5 if scale is None else scale,
-            stream))
+            *self._more, stream))
         return out
+
+    _more = ()
+
+    def _entry(self, fn, cache):
+        if isinstance(cache, KvCacheQ8):
+            raise SagerError(f"{fn}: a quantised cache is SlidingAttention's")
+        return load().sg_attn_tree_f16
+
+
+class SlidingAttention(TreeAttention):
+    """TreeAttention over a sliding window of `reach` positions (0: all) and
+    the first `sinks` tokens, over a KvCache or a KvCacheQ8
+    (sg_attn_sliding_f16 / _q8).  Without a parent (chains) windows may be
+    longer than 64 tokens: a prompt's chunk."""
+
+    def __init__(self, n_heads, n_kv_heads, head_dim, max_tokens, max_seqs=1, max_window=1,
+                 max_len=0, reach=0, sinks=0, device="cuda"):
+        if n_kv_heads <= 0 or n_heads % n_kv_heads != 0:
+            raise SagerError("n_heads must be a multiple of n_kv_heads")
+        if reach < 0 or sinks < 0:
+            raise SagerError("reach and sinks must not be negative")
+        self.n_heads, self.n_kv_heads, self.head_dim = n_heads, n_kv_heads, head_dim
+        self.max_tokens, self.max_seqs = max_tokens, max_seqs
+        self.max_window, self.max_len = max_window, max_len
+        self.reach, self.sinks = reach, sinks
+        self._more = (reach, sinks)
+        nbytes = load().sg_attn_sliding_workspace_bytes(max_seqs, max_window, max_len, n_heads,
+                                                        n_kv_heads, head_dim, reach, sinks)
+        self.workspace = torch.empty(nbytes, dtype=torch.uint8, device=device)
+
+    def _entry(self, fn, cache):
+        return load().sg_attn_sliding_q8 if isinstance(cache, KvCacheQ8) else \
+            load().sg_attn_sliding_f16
 
 
 class TreeVerify:

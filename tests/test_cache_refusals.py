@@ -192,3 +192,92 @@ def test_read_refusals(lib):
             for spot in (ROOM * i, ROOM * i + n - 2, ROOM * i - 4094):
                 assert lib.sg_kv_read_q8(*read_args(c, **{out: P(spot)})) == INVALID, (i, out)
                 assert b"overlap" in lib.sg_last_error()
+
+
+# ---- sliding attention -----------------------------------------------------------------
+
+def attn_args(c, **kw):
+    a = dict(q=at(20), k=at(21), v=at(22), qs=8 * 128, ks=256, vs=256, cache=ctypes.byref(c), layer=0,
+             off=at(23), parent=at(24), out=at(25), ws=at(26), ws_bytes=1 << 40, n_seq=1, n_tokens=4,
+             max_window=4, max_len=4000, n_heads=8, scale=0.1, reach=1000, sinks=4)
+    a.update(kw)
+    return list(a.values()) + [None]
+
+
+def f16_cache(**kw):
+    a = dict(k=ROOM, v=ROOM * 2, pages=ROOM * 5, length=ROOM * 6, layer_stride=1 << 20, n_layers=2,
+             n_pages=8, page_size=16, pages_per_seq=4, n_kv_heads=2, head_dim=128)
+    a.update(kw)
+    return sager_amd.KvCacheDesc(*a.values())
+
+
+@pytest.mark.parametrize("q8", [False, True])
+def test_attention_refusals(lib, q8):
+    fn = lib.sg_attn_sliding_q8 if q8 else lib.sg_attn_sliding_f16
+    new = cache if q8 else f16_cache
+    c = new()
+    for kw, status in ((dict(q=None), INVALID), (dict(v=None), INVALID), (dict(off=None), INVALID),
+                       (dict(out=None), INVALID), (dict(cache=None), INVALID), (dict(n_seq=0), GEOMETRY),
+                       (dict(n_tokens=0), GEOMETRY), (dict(max_window=0), GEOMETRY),
+                       (dict(max_window=65), UNSUPPORTED), (dict(layer=2), GEOMETRY),
+                       (dict(layer=-1), GEOMETRY), (dict(max_len=-1), GEOMETRY),
+                       (dict(max_len=0x7FFFFFFF), UNSUPPORTED), (dict(n_heads=7), GEOMETRY),
+                       (dict(reach=-1), GEOMETRY), (dict(sinks=-1), GEOMETRY), (dict(qs=1023), GEOMETRY),
+                       (dict(ks=255), INVALID), (dict(ks=248), GEOMETRY), (dict(vs=-256), GEOMETRY),
+                       (dict(k=P(4104)), INVALID), (dict(out=P(4100)), INVALID), (dict(q=P(4097)), INVALID),
+                       (dict(ws=None), INVALID), (dict(ws=P(4104)), INVALID), (dict(ws_bytes=64), INVALID),
+                       (dict(n_seq=1 << 30), UNSUPPORTED),
+                       (dict(parent=None, max_window=(1 << 24) + 1), UNSUPPORTED),
+                       (dict(parent=None, max_window=1 << 24, n_heads=256, qs=256 * 128), UNSUPPORTED)):
+        assert fn(*attn_args(c, **kw)) == status, kw
+        assert b"sg_attn_sliding" in lib.sg_last_error()
+    if q8:
+        for kw, status in BAD_CACHES:
+            assert fn(*attn_args(cache(**kw))) == status, kw
+    # a window that ends past 32-bit positions
+    far = new(page_size=1 << 20, pages_per_seq=2047, n_pages=1, layer_stride=1 << 40)
+    assert fn(*attn_args(far)) != UNSUPPORTED
+    assert fn(*attn_args(far, parent=None, max_window=1 << 24)) == UNSUPPORTED
+
+
+@pytest.mark.parametrize("q8", [False, True])
+def test_attention_output_over_what_is_read(lib, q8):
+    fn = lib.sg_attn_sliding_q8 if q8 else lib.sg_attn_sliding_f16
+    n_seq, T, W, heads, kv, D, n_pages, page, per = 3, 7, 4, 8, 2, 128, 9, 16, 4
+    need = lib.sg_attn_sliding_workspace_bytes(n_seq, W, 4000, heads, kv, D, 1000, 4)
+    assert need > 0
+    layer, w = n_pages * kv * page * D, 1 if q8 else 2
+    size = dict(q=T * heads * D * 2, k=T * kv * D * 2, v=T * kv * D * 2, kc=layer * w, vc=layer * w,
+                pages=n_seq * per * 4, length=n_seq * 4, off=(n_seq + 1) * 4, parent=T * 4, ws=need)
+    if q8:
+        size.update(ks=layer // 16, vs=layer // 16)
+    a, n_out = {n: ROOM * (i + 1) for i, n in enumerate(size)}, T * heads * D * 2
+    geo = (layer, 2, n_pages, page, per, kv, D)
+    if q8:  # (the second layer, the first one lies before the addresses)
+        c = sager_amd.KvCacheQ8Desc(a["kc"] - layer, a["vc"] - layer, a["ks"] - layer // 16,
+                                    a["vs"] - layer // 16, a["pages"], a["length"], *geo)
+    else:
+        c = sager_amd.KvCacheDesc(a["kc"] - 2 * layer, a["vc"] - 2 * layer, a["pages"], a["length"], *geo)
+
+    def call(out, **kw):
+        b = dict(a, **kw)
+        return fn(P(b["q"]), P(b["k"]), P(b["v"]), heads * D, kv * D, kv * D, ctypes.byref(c), 1,
+                  P(b["off"]), P(b["parent"]), P(out), P(b["ws"]), need, n_seq, T, W, 4000, heads, 0.1,
+                  1000, 4, None)
+    for other in size:
+        for spot in (a[other], a[other] + (size[other] - 2) // 8 * 8, a[other] - n_out + 8):
+            assert call(spot) == INVALID, (other, spot)
+            assert b"overlaps" in lib.sg_last_error(), other
+
+
+def test_attention_workspace(lib):
+    f = lib.sg_attn_sliding_workspace_bytes
+    assert f(0, 1, 1, 1, 1, 64, 0, 0) == 0 and f(1, 1, 1, 3, 2, 64, 0, 0) == 0
+    assert f(1, 1, 1, 2, 2, 64, -1, 0) == 0 and f(1, 4, 100000, 16, 2, 256, 0, 0) > 0
+    # what is enough for a batch is enough for a smaller one
+    for max_len in (0, 100, 500, 100000):
+        for reach, sinks in ((0, 0), (100, 4), (5000, 70)):
+            for args in ((4, max_len, 16, 2, 256), (1, max_len, 32, 8, 128), (64, max_len, 7, 7, 64),
+                         (1000, max_len, 8, 2, 128), (65, max_len, 4, 1, 256)):
+                for n in range(2, 300):
+                    assert f(n, *args, reach, sinks) >= f(n - 1, *args, reach, sinks)
