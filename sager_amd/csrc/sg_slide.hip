@@ -20,13 +20,31 @@
 //
 // V at infinity or NaN where some rows see it and others do not: a product
 // with a weight of 0 would spread it.  Weights that are 0 because the key is
-// not seen are written as -0; in a step with such a V the second product is
-// made one by one, without those.
+// not seen are written as -0; in a step with such a V these values are added
+// one by one, to the rows that see them, and are 0 in the product.
 #include <type_traits>
 
 #include "sg_attn.hpp"
 
 namespace sg {
+
+// 16 and 4 B of global memory, at any address that the buffers' own alignment allows
+typedef const __attribute__((address_space(1))) unsigned char* gmem;
+typedef uint32_t u32x2 __attribute__((ext_vector_type(2)));
+__device__ __forceinline__ u32x4 load16(gmem p, uint32_t off = 0) {
+  return *reinterpret_cast<const __attribute__((address_space(1))) u32x4*>(p + off);
+}
+__device__ __forceinline__ uint32_t load4(gmem p, uint32_t off = 0) {
+  return *reinterpret_cast<const __attribute__((address_space(1))) uint32_t*>(p + off);
+}
+
+// Here the loads of x are waited for, and not before: left to the compiler, some
+// of what is made of them moves up to where the step before has just issued them.
+template <typename T, int N>
+__device__ __forceinline__ void settle(T (&x)[N]) {
+#pragma unroll
+  for (int i = 0; i < N; ++i) asm volatile("" : "+v"(x[i]));
+}
 
 struct SlideArgs : AttnArgs {
   const uint16_t *ks, *vs;  // scales of the quantised cache (kc, vc: its codes)
@@ -113,36 +131,47 @@ struct SlidePart : Part<D> {
     this->end = v0 < v1 ? min(all.at(v1 - 1) + 1, steps.high) : 0;
     return true;
   }
-  // The pages of a cached step's four blocks of 16 keys; -1: absent, or behind the cache.
-  __device__ __forceinline__ void pages_of(int s, int (&p)[4]) const {
+  // Where the rows of a cached step's blocks of 16 keys begin, in values.
+  struct Rows {
+    long long at[4];
+    uint32_t ok;  // bit b: block b's page is there
+  };
+  __device__ __forceinline__ Rows rows_of(int s) const {
+    Rows r;
+    r.ok = 0;
 #pragma unroll
     for (int b = 0; b < 4; ++b) {
       const int j = s * kKeys + 16 * b;
-      p[b] = s < steps.cached && j < this->len ? this->table[j >> sa.page_log2] : -1;
-      if (!this->page_ok(p[b])) p[b] = -1;
+      int p = j < this->len ? this->table[j >> sa.page_log2] : -1;
+      if (this->page_ok(p))
+        r.ok |= 1u << b;
+      else
+        p = 0;  // (any page: what is read there is not used)
+      r.at[b] = (((static_cast<long long>(p) * sa.n_kv + this->h) << sa.page_log2) +
+                 (j & ((1 << sa.page_log2) - 1))) * D;
     }
+    return r;
   }
-  // Whether every row of the block sees every key of step s.
-  __device__ __forceinline__ bool full(int s, const int (&p)[4]) const {
-    const int len = this->len;
-    if (s < steps.cached)
-      return (p[0] | p[1] | p[2] | p[3]) >= 0 && (s + 1) * kKeys <= len &&
-             ((s + 1) * kKeys <= sa.sinks ||
-              s * kKeys > static_cast<long long>(len) + last - sa.reach);
+  // Whether every row of the block sees every key of step s: of the cache,
+  __device__ __forceinline__ bool full(int s, uint32_t ok) const {
+    return ok == 15u && (s + 1) * kKeys <= this->len &&
+           ((s + 1) * kKeys <= sa.sinks ||
+            s * kKeys > static_cast<long long>(this->len) + last - sa.reach);
+  }
+  // and of a chain's window.
+  __device__ __forceinline__ bool full_window(int s) const {
     const int w = (s - steps.cached) * kKeys;
     return !sa.parent && w + kKeys - 1 <= first &&
-           (len + w + kKeys <= sa.sinks || w > static_cast<long long>(last) - sa.reach);
+           (this->len + w + kKeys <= sa.sinks || w > static_cast<long long>(last) - sa.reach);
   }
   // Which of step s's keys are there.
-  __device__ __forceinline__ uint64_t present(int s, const int (&p)[4]) const {
+  __device__ __forceinline__ uint64_t present(int s, uint32_t ok) const {
     const int n = s < steps.cached ? this->len - s * kKeys
                                    : this->win.n - (s - steps.cached) * kKeys;
     uint64_t m = n >= kKeys ? ~0ull : (1ull << n) - 1;
-    if (s < steps.cached) {
 #pragma unroll
-      for (int b = 0; b < 4; ++b)
-        if (p[b] < 0) m &= ~(0xFFFFull << (16 * b));
-    }
+    for (int b = 0; b < 4; ++b)
+      if (!(ok >> b & 1)) m &= ~(0xFFFFull << (16 * b));
     return m;
   }
   // bit i: key k + i of step s (i < 4) is there and seen by a row of node `node`
@@ -152,19 +181,15 @@ struct SlidePart : Part<D> {
     uint32_t m = static_cast<uint32_t>(there >> k) & 15u;
     const bool cached = s < steps.cached;
     if (!cached && sa.parent) return m & static_cast<uint32_t>(up >> k);
+    // (positions as unsigned differences: no further than pos, and less than reach)
     const int p0 = (cached ? s * kKeys : this->len + (s - steps.cached) * kKeys) + k;
 #pragma unroll
     for (int i = 0; i < 4; ++i) {
-      const int p = p0 + i;
-      const bool see = p < sa.sinks ? p <= pos : p <= pos && pos - p < sa.reach;
-      m &= see ? ~0u : ~(1u << i);
+      const uint32_t back = pos - (p0 + i);
+      const uint32_t most = p0 + i < sa.sinks ? 0x7FFFFFFFu : static_cast<uint32_t>(sa.reach - 1);
+      m &= back <= most ? ~0u : ~(1u << i);
     }
     return m;
-  }
-  // Where the cache's row of head h and slot j of page p begins, in values.
-  __device__ __forceinline__ long long row_at(int p, int j) const {
-    return ((static_cast<long long>(max(p, 0)) * sa.n_kv + this->h) << sa.page_log2) +
-           (j & ((1 << sa.page_log2) - 1));
   }
 };
 
@@ -229,73 +254,88 @@ __global__ void __launch_bounds__(256) slide_few_kernel(const SlideArgs a) {
   auto piece = [&](int i) {
     return Q8 ? 64 * (i / 2) + 16 * grp + 8 * (i % 2) : 32 * i + 8 * grp;
   };
-  u32x4 kr[KK], vr[KK];
-  uint32_t kscale[KK / 2], vscale[LQ];
-  int page[4];
-
-  auto load_k = [&](int s, const int (&pg)[4]) {
-    if (s < t.steps.cached) {
-      const int p = wave == 0 ? pg[0] : wave == 1 ? pg[1] : wave == 2 ? pg[2] : pg[3];
-      const long long at = t.row_at(p, s * kKeys + 16 * wave);
-      if (Q8) {
-        const unsigned char* src = uniform_ptr(reinterpret_cast<const unsigned char*>(a.kc) + at * D);
-        const uint16_t* sc = uniform_ptr(a.ks + at * (D / kKvGroup));
-#pragma unroll
-        for (int i = 0; i < KK / 2; ++i) {
-          kr[i] = *reinterpret_cast<const u32x4*>(src + (col * D + 64 * i + 16 * grp));
-          kscale[i] = sc[col * (D / kKvGroup) + 2 * i + (grp >> 1)];
-        }
-      } else {
-        const uint16_t* src = uniform_ptr(a.kc + at * D);
-#pragma unroll
-        for (int i = 0; i < KK; ++i)
-          kr[i] = *reinterpret_cast<const u32x4*>(src + (col * D + piece(i)));
-      }
-    } else {
-      const int w = min((s - t.steps.cached) * kKeys + 16 * wave + col, t.win.n - 1);
-      const uint16_t* src = a.k + static_cast<long long>(t.win.off + w) * a.k_stride + t.h * D;
-#pragma unroll
-      for (int i = 0; i < KK; ++i) kr[i] = *reinterpret_cast<const u32x4*>(src + piece(i));
-    }
+  // A step's raw K and V, of a window or of the cache: 16 B a register quad.
+  struct Raw {
+    u32x4 k[KK], v[KK];
   };
-  auto load_v = [&](int s, const int (&pg)[4]) {
-    if (s < t.steps.cached) {
-      if (Q8) {
+  struct Codes {
+    u32x4 k[KK / 2], v[LQ];
+    uint32_t ks[KK / 2], vs[LQ];
+  };
+  typedef typename std::conditional<Q8, Codes, Raw>::type Cached;
+  typedef typename P::Rows Rows;
+  const gmem kc = (gmem)a.kc, vc = (gmem)a.vc, ksc = (gmem)a.ks, vsc = (gmem)a.vs;
+  auto load_k = [&](Cached& x, const Rows& rows) {
+    const long long at = wave == 0 ? rows.at[0] : wave == 1 ? rows.at[1] : wave == 2 ? rows.at[2] : rows.at[3];
+    if constexpr (Q8) {
 #pragma unroll
-        for (int i = 0; i < LQ; ++i) {
-          const int r = i * RQ + lane / LQ, b = r >> 4;
-          const int p = b == 0 ? pg[0] : b == 1 ? pg[1] : b == 2 ? pg[2] : pg[3];
-          const long long at =
-              t.row_at(p, s * kKeys + r) * D + wave * (D / 4) + (lane % LQ) * 16;
-          vr[i] = *reinterpret_cast<const u32x4*>(reinterpret_cast<const unsigned char*>(a.vc) + at);
-          vscale[i] = a.vs[at / kKvGroup];
-        }
+      for (int i = 0; i < KK / 2; ++i) x.k[i] = load16(kc + at, col * D + 64 * i + 16 * grp);
+      // the row's scales, two a register
+      const gmem sc = ksc + at / (kKvGroup / 2);
+      if constexpr (KK == 8) {
+        const u32x4 w = load16(sc, col * 16);
+#pragma unroll
+        for (int i = 0; i < 4; ++i) x.ks[i] = w[i];
       } else {
 #pragma unroll
-        for (int i = 0; i < KK; ++i) {
-          const int r = i * RP + lane / LP, b = r >> 4;
-          const int p = b == 0 ? pg[0] : b == 1 ? pg[1] : b == 2 ? pg[2] : pg[3];
-          const long long at = t.row_at(p, s * kKeys + r) * D + wave * (D / 4) + (lane % LP) * 8;
-          vr[i] = *reinterpret_cast<const u32x4*>(a.vc + at);
-        }
+        for (int i = 0; i < KK / 2; ++i) x.ks[i] = load4(sc, col * KK * 2 + 4 * i);
       }
     } else {
 #pragma unroll
-      for (int i = 0; i < KK; ++i) {
-        const int w = min((s - t.steps.cached) * kKeys + i * RP + lane / LP, t.win.n - 1);
-        vr[i] = *reinterpret_cast<const u32x4*>(
-            a.v + static_cast<long long>(t.win.off + w) * a.v_stride + t.h * D + wave * (D / 4) +
-            (lane % LP) * 8);
+      for (int i = 0; i < KK; ++i) x.k[i] = load16(kc + 2 * at, (col * D + piece(i)) * 2);
+    }
+  };
+  auto load_v = [&](Cached& x, const Rows& rows) {
+    // (values of the wave's columns; a block of 16 rows or more at once)
+    constexpr int N = Q8 ? LQ : KK, L1 = Q8 ? LQ : LP, R1 = Q8 ? RQ : RP;
+#pragma unroll
+    for (int i = 0; i < N; ++i) {
+      constexpr int kBlocks = R1 <= 16 ? 1 : R1 / 16;
+      const int b0 = i * R1 / 16, in = lane / L1;
+      long long at = rows.at[b0];
+      if constexpr (kBlocks == 2) at = in < 16 ? at : rows.at[b0 + 1];
+      if constexpr (kBlocks == 4)
+        at = in < 32 ? (in < 16 ? rows.at[0] : rows.at[1]) : (in < 48 ? rows.at[2] : rows.at[3]);
+      const uint32_t row = i * R1 % 16 + in % 16;
+      const uint32_t off = row * D + wave * (D / 4) + (lane % L1) * (Q8 ? 16 : 8);
+      if constexpr (Q8) {
+        x.v[i] = load16(vc + at, off);
+        // (the two scales that the wave's are among)
+        x.vs[i] = load4(vsc + at / (kKvGroup / 2), row * (D / 16) + (wave * D / 4 / 64) * 4);
+      } else {
+        x.v[i] = load16(vc + 2 * at, 2 * off);
       }
     }
   };
+  // which of the two scales of load_v a lane's 16 columns have
+  const int vhalf = 16 * ((wave * (D / 4) + (lane % LQ) * 16) / kKvGroup & 1);
+  auto load_window = [&](Raw& x, int s) {
+    const int w0 = (s - t.steps.cached) * kKeys;
+    const gmem kp =
+        (gmem)(a.k + static_cast<long long>(t.win.off + min(w0 + 16 * wave + col, t.win.n - 1)) * a.k_stride +
+               t.h * D);
+#pragma unroll
+    for (int i = 0; i < KK; ++i) x.k[i] = load16(kp, piece(i) * 2);
+#pragma unroll
+    for (int i = 0; i < KK; ++i) {
+      const int w = min(w0 + i * RP + lane / LP, t.win.n - 1);
+      x.v[i] = load16((gmem)(a.v + static_cast<long long>(t.win.off + w) * a.v_stride + t.h * D +
+                             wave * (D / 4) + (lane % LP) * 8));
+    }
+  };
 
-  int step = t.begin;
-  if (step < t.end) {
-    t.pages_of(step, page);
-    load_k(step, page);
-    load_v(step, page);
+  // The block's steps of the cache and of the window.
+  const int cached_end = min(t.end, t.steps.cached);
+  int step = t.begin, wstep = t.steps.skip(max(t.begin, t.steps.cached));
+  Cached now;
+  Rows rows;
+  if (step < cached_end) {
+    rows = t.rows_of(step);
+    load_k(now, rows);
+    load_v(now, rows);
   }
+  Raw own;
+  if (wstep < t.end) load_window(own, wstep);
   if (threadIdx.x < 2) rise[threadIdx.x] = 0;
   if (wave == 3 && a.parent) see_tree(a, t.win, t.len, lane, place, seen);
 
@@ -327,43 +367,16 @@ __global__ void __launch_bounds__(256) slide_few_kernel(const SlideArgs a) {
   // V's columns 0..15 of row 4 grp + col / 4 of a 16-key block
   const uint32_t v_in = wave * L::kWave + (4 * grp + (col >> 2)) * L::kRow + (col & 3) * 8;
 
-  bar();  // the flags are cleared, the tree is there
-  for (int it = 0; step < t.end; ++it) {
-    const int par = it & 1;
-    const bool cached = step < t.steps.cached;
-    const bool full = t.full(step, page);
-    const uint64_t there = full ? ~0ull : t.present(step, page);
-    const int next = t.steps.skip(step + 1);
-    int page_next[4] = {-1, -1, -1, -1};
-    if (next < t.end) t.pages_of(next, page_next);
-
+  int it = 0;
+  // A step's scores from K, its weights and V into LDS, the second product.
+  // scores(s): the products with K; spread(odd): V into the wave's corner;
+  // each issues the next step's loads once it is through with its own.
+  auto run = [&](int step, bool full, uint64_t there, auto&& scores, auto&& spread) {
+    const int par = it++ & 1;
     f4 s[RT];
 #pragma unroll
     for (int rt = 0; rt < RT; ++rt) s[rt] = (f4){0.f, 0.f, 0.f, 0.f};
-    if (Q8 && cached) {
-#pragma unroll
-      for (int i = 0; i < KK / 2; ++i) {
-        const h2 d = scale2(kscale[i]);
-#pragma unroll
-        for (int j = 0; j < 2; ++j) {
-          uint32_t w[4];
-          decode4(kr[i][2 * j], d, *reinterpret_cast<uint32_t(*)[2]>(w));
-          decode4(kr[i][2 * j + 1], d, *reinterpret_cast<uint32_t(*)[2]>(w + 2));
-          const h8 kf = __builtin_bit_cast(h8, (u32x4){w[0], w[1], w[2], w[3]});
-#pragma unroll
-          for (int rt = 0; rt < RT; ++rt)
-            s[rt] = __builtin_amdgcn_mfma_f32_16x16x32_f16(kf, qf[rt][2 * i + j], s[rt], 0, 0, 0);
-        }
-      }
-    } else {
-#pragma unroll
-      for (int i = 0; i < KK; ++i)
-#pragma unroll
-        for (int rt = 0; rt < RT; ++rt)
-          s[rt] = __builtin_amdgcn_mfma_f32_16x16x32_f16(__builtin_bit_cast(h8, kr[i]), qf[rt][i],
-                                                         s[rt], 0, 0, 0);
-    }
-    if (next < t.end) load_k(next, page_next);
+    scores(s);
 
     float e[RT][4], top[RT], sum[RT];
     uint32_t see[RT];
@@ -401,45 +414,7 @@ __global__ void __launch_bounds__(256) slide_few_kernel(const SlideArgs a) {
       weigh(rt, 0.f);
     }
     if (__any(move)) rise[par] = step + 1;
-
-    // V into the wave's corner; rows that are not there as 0
-    bool odd = false;
-    if (Q8 && cached) {
-#pragma unroll
-      for (int i = 0; i < LQ; ++i) {
-        const int r = i * RQ + lane / LQ;
-        const h2 d = scale2(vscale[i]);
-        const bool some = full || (there >> r & 1);
-        uint32_t w[8];
-#pragma unroll
-        for (int j = 0; j < 4; ++j) decode4(vr[i][j], d, *reinterpret_cast<uint32_t(*)[2]>(w + 2 * j));
-        if (!some) {
-#pragma unroll
-          for (int j = 0; j < 8; ++j) w[j] = 0;
-        }
-        if (!full) odd |= some && fp16_odd(vscale[i]);
-        u32x4* to = reinterpret_cast<u32x4*>(vl + r * L::kRow + (lane % LQ) * 32);
-        to[0] = (u32x4){w[0], w[1], w[2], w[3]};
-        to[1] = (u32x4){w[4], w[5], w[6], w[7]};
-      }
-    } else {
-#pragma unroll
-      for (int i = 0; i < KK; ++i) {
-        const int r = i * RP + lane / LP;
-        u32x4 w = vr[i];
-        if (!full) {
-          const bool some = there >> r & 1;
-#pragma unroll
-          for (int j = 0; j < 4; ++j) {
-            w[j] = some ? w[j] : 0u;
-            odd |= fp16_odd(w[j]) || fp16_odd(w[j] >> 16);
-          }
-        }
-        *reinterpret_cast<u32x4*>(vl + r * L::kRow + (lane % LP) * 16) = w;
-      }
-    }
-    if (next < t.end) load_v(next, page_next);
-    const bool by_one = !full && __any(odd);
+    const bool by_one = spread() && !full;
     bar();  // P is here
 
     if (rise[par] == step + 1) {
@@ -475,46 +450,159 @@ __global__ void __launch_bounds__(256) slide_few_kernel(const SlideArgs a) {
 #pragma unroll 1
       for (int r = 0; r < kKeys; ++r) {
         const int at = (r >> 5) * 4 + ((r & 15) >> 2);
+#pragma unroll 1
+        for (int d = 0; d < DQ; ++d) {
+          h4* const vp = reinterpret_cast<h4*>(vl + r * L::kRow + d * 32 + grp * 8);
+          const u32x2 v = *reinterpret_cast<const u32x2*>(vp);
+          const uint32_t x[4] = {v.x & 0xFFFFu, v.x >> 16, v.y & 0xFFFFu, v.y >> 16};
 #pragma unroll
-        for (int rt = 0; rt < RT; ++rt) {
-          const uint32_t w = *reinterpret_cast<const uint16_t*>(
-              pl + (rt * 16 + col) * 128 + ((at ^ psw) << 4) + (r >> 4 & 1) * 8 + (r & 3) * 2);
-          const float p = half_bits_to_float(w);
-#pragma unroll
-          for (int d = 0; d < DQ; ++d) {
-            const h4 v = *reinterpret_cast<const h4*>(vl + r * L::kRow + d * 32 + grp * 8);
+          for (int rt = 0; rt < RT; ++rt) {
+            const uint32_t w = *reinterpret_cast<const uint16_t*>(
+                pl + (rt * 16 + col) * 128 + ((at ^ psw) << 4) + (r >> 4 & 1) * 8 + (r & 3) * 2);
+            const float p = half_bits_to_float(w);
+            f4 add;
 #pragma unroll
             for (int i = 0; i < 4; ++i)
-              acc[rt][d][i] += w == 0x8000u ? 0.f : p * static_cast<float>(v[i]);
+              add[i] = w != 0x8000u && fp16_odd(x[i]) ? p * half_bits_to_float(x[i]) : 0.f;
+#pragma unroll
+            for (int dd = 0; dd < DQ; ++dd)
+              if (dd == d) acc[rt][dd] += add;
           }
+          // (for the product: 0 in their place; the wave's own corner, all of it read first)
+          wait_lds();
+          const uint32_t y0 = (fp16_odd(x[0]) ? 0u : x[0]) | (fp16_odd(x[1]) ? 0u : x[1]) << 16;
+          const uint32_t y1 = (fp16_odd(x[2]) ? 0u : x[2]) | (fp16_odd(x[3]) ? 0u : x[3]) << 16;
+          *reinterpret_cast<u32x2*>(vp) = (u32x2){y0, y1};
         }
       }
-    } else {
+      wait_lds();
+    }
 #pragma unroll
-      for (int st = 0; st < 2; ++st) {
-        h8 pf[RT];
+    for (int st = 0; st < 2; ++st) {
+      h8 pf[RT];
+#pragma unroll
+      for (int rt = 0; rt < RT; ++rt)
+        pf[rt] = *reinterpret_cast<const h8*>(pl + (rt * 16 + col) * 128 +
+                                              (((st * 4 + grp) ^ psw) << 4));
+#pragma unroll
+      for (int d = 0; d < DQ; ++d) {
+        s4 x[2];
+#pragma unroll
+        for (int b = 0; b < 2; ++b)
+          x[b] = __builtin_amdgcn_ds_read_tr16_b64_v4i16(
+              (lds_s4_p)((lds_char_p)lds + v_in + (st * 2 + b) * 16 * L::kRow + d * 32));
+        const h8 vf =
+            __builtin_bit_cast(h8, __builtin_shufflevector(x[0], x[1], 0, 1, 2, 3, 4, 5, 6, 7));
 #pragma unroll
         for (int rt = 0; rt < RT; ++rt)
-          pf[rt] = *reinterpret_cast<const h8*>(pl + (rt * 16 + col) * 128 +
-                                                (((st * 4 + grp) ^ psw) << 4));
-#pragma unroll
-        for (int d = 0; d < DQ; ++d) {
-          s4 x[2];
-#pragma unroll
-          for (int b = 0; b < 2; ++b)
-            x[b] = __builtin_amdgcn_ds_read_tr16_b64_v4i16(
-                (lds_s4_p)((lds_char_p)lds + v_in + (st * 2 + b) * 16 * L::kRow + d * 32));
-          const h8 vf = __builtin_bit_cast(
-              h8, __builtin_shufflevector(x[0], x[1], 0, 1, 2, 3, 4, 5, 6, 7));
-#pragma unroll
-          for (int rt = 0; rt < RT; ++rt)
-            acc[rt][d] = __builtin_amdgcn_mfma_f32_16x16x32_f16(vf, pf[rt], acc[rt][d], 0, 0, 0);
-        }
+          acc[rt][d] = __builtin_amdgcn_mfma_f32_16x16x32_f16(vf, pf[rt], acc[rt][d], 0, 0, 0);
       }
     }
-    step = next;
+  };
+  // 16-bit K and V of a step as they were loaded
+  auto raw_scores = [&](const Raw& x, f4 (&s)[RT]) {
 #pragma unroll
-    for (int b = 0; b < 4; ++b) page[b] = page_next[b];
+    for (int i = 0; i < KK; ++i)
+#pragma unroll
+      for (int rt = 0; rt < RT; ++rt)
+        s[rt] = __builtin_amdgcn_mfma_f32_16x16x32_f16(__builtin_bit_cast(h8, x.k[i]), qf[rt][i],
+                                                       s[rt], 0, 0, 0);
+  };
+  auto raw_spread = [&](const Raw& x, bool full, uint64_t there) {
+    bool odd = false;
+#pragma unroll
+    for (int i = 0; i < KK; ++i) {
+      const int r = i * RP + lane / LP;
+      u32x4 w = x.v[i];
+      if (!full) {  // rows that are not there as 0
+        const bool some = there >> r & 1;
+#pragma unroll
+        for (int j = 0; j < 4; ++j) {
+          w[j] = some ? w[j] : 0u;
+          odd |= fp16_odd(w[j]) || fp16_odd(w[j] >> 16);
+        }
+      }
+      *reinterpret_cast<u32x4*>(vl + r * L::kRow + (lane % LP) * 16) = w;
+    }
+    return __any(odd);
+  };
+
+  bar();  // the flags are cleared, the tree is there
+  while (wstep < t.end) {  // (one step, but for chains of more than 64 tokens)
+    const bool full = t.full_window(wstep);
+    const uint64_t there = full ? ~0ull : t.present(wstep, 15u);
+    run(wstep, full, there, [&](f4 (&s)[RT]) { raw_scores(own, s); },
+        [&] { return raw_spread(own, full, there); });
+    wstep = t.steps.skip(wstep + 1);
+    if (wstep < t.end) load_window(own, wstep);
+  }
+  // (no load of the window is under way any more: else the loop would wait for all of its own)
+  settle(own.k);
+  settle(own.v);
+  while (step < cached_end) {
+    const bool full = t.full(step, rows.ok);
+    const uint64_t there = full ? ~0ull : t.present(step, rows.ok);
+    // (after the last step, that one once more)
+    const int next = t.steps.skip(step + 1);
+    rows = t.rows_of(next < cached_end ? next : step);
+    run(
+        step, full, there,
+        [&](f4 (&s)[RT]) {
+          settle(now.k);
+          if constexpr (Q8) {
+            settle(now.ks);
+#pragma unroll
+            for (int i = 0; i < KK / 2; ++i) {
+              const h2 d = scale2(now.ks[i] >> (grp & 2) * 8);
+#pragma unroll
+              for (int j = 0; j < 2; ++j) {
+                uint32_t w[2][2];
+                decode4(now.k[i][2 * j], d, w[0]);
+                decode4(now.k[i][2 * j + 1], d, w[1]);
+                const h8 kf = __builtin_bit_cast(h8, (u32x4){w[0][0], w[0][1], w[1][0], w[1][1]});
+#pragma unroll
+                for (int rt = 0; rt < RT; ++rt)
+                  s[rt] = __builtin_amdgcn_mfma_f32_16x16x32_f16(kf, qf[rt][2 * i + j], s[rt], 0, 0, 0);
+              }
+            }
+          } else {
+            raw_scores(now, s);
+          }
+          load_k(now, rows);
+        },
+        [&] {
+          bool odd = false;
+          settle(now.v);
+          if constexpr (Q8) {
+            settle(now.vs);
+#pragma unroll
+            for (int i = 0; i < LQ; ++i) {
+              const int r = i * RQ + lane / LQ;
+              const h2 d = scale2(now.vs[i] >> vhalf);
+              uint32_t w[4][2];
+#pragma unroll
+              for (int j = 0; j < 4; ++j) decode4(now.v[i][j], d, w[j]);
+              if (!full) {
+                const bool some = there >> r & 1;
+#pragma unroll
+                for (int j = 0; j < 4; ++j) {
+                  w[j][0] = some ? w[j][0] : 0u;
+                  w[j][1] = some ? w[j][1] : 0u;
+                }
+                odd |= some && fp16_odd(now.vs[i] >> vhalf);
+              }
+              u32x4* to = reinterpret_cast<u32x4*>(vl + r * L::kRow + (lane % LQ) * 32);
+              to[0] = (u32x4){w[0][0], w[0][1], w[1][0], w[1][1]};
+              to[1] = (u32x4){w[2][0], w[2][1], w[3][0], w[3][1]};
+            }
+            odd = __any(odd);
+          } else {
+            odd = raw_spread(now, full, there);
+          }
+          load_v(now, rows);
+          return odd;
+        });
+    step = next;
   }
 
   // the rows' sums over the waves, and out
