@@ -49,6 +49,7 @@ __device__ __forceinline__ void settle(T (&x)[N]) {
 struct SlideArgs : AttnArgs {
   const uint16_t *ks, *vs;  // scales of the quantised cache (kc, vc: its codes)
   int reach, sinks;
+  bool spread;  // row blocks one after the other, not 8 apart
 };
 
 // The steps that a sequence's nodes first .. last see: [0, sink) and [low,
@@ -100,11 +101,17 @@ struct SlidePart : Part<D> {
     this->col = lane & 15;
     this->grp = lane >> 4;
     const int id = blockIdx.x;
-    // The row blocks of a unit are 8 workgroups apart: on one XCD, whose L2 then
-    // reads the unit's keys once.
-    const int oct = id / (8 * sa.row_blocks), in = id - oct * 8 * sa.row_blocks;
-    this->rb = in >> 3;
-    this->unit = oct * 8 + (in & 7);
+    if (sa.spread) {
+      // Many row blocks: over all XCDs, the last rows, which see most, first.
+      this->unit = id / sa.row_blocks;
+      this->rb = sa.row_blocks - 1 - (id - this->unit * sa.row_blocks);
+    } else {
+      // The row blocks of a unit are 8 workgroups apart: on one XCD, whose L2
+      // then reads the unit's keys once.
+      const int oct = id / (8 * sa.row_blocks), in = id - oct * 8 * sa.row_blocks;
+      this->rb = in >> 3;
+      this->unit = oct * 8 + (in & 7);
+    }
     Unit u;
     const bool plan = sa.cut && id == 0 && __builtin_amdgcn_readfirstlane(threadIdx.x >> 6) == 0;
     if (!find_unit(sa, this->unit, lane, plan, u)) return false;
@@ -656,36 +663,406 @@ __global__ void __launch_bounds__(256, slide_waves(D, RT, Q8)) slide_few_kernel(
   }
 }
 
+// ---- blocks of 256 rows ---------------------------------------------------------------------
+// LDS: K and V of two steps, or of one and the codes of two; the nodes'
+// positions and what they see, the scales of two steps' codes, the flags.
+template <int D>
+struct SlideRowsLds {
+  static constexpr uint32_t kSeen = 4 * Part<D>::kStep;
+  static constexpr uint32_t kPos = kSeen + kMaxWindow * 8;
+  static constexpr uint32_t kScales = kPos + kMaxWindow * 4;
+  static constexpr uint32_t kScaleStep = 2 * kKeys * D / kKvGroup * 2;  // K's and V's
+  static constexpr uint32_t kFlags = kScales + 2 * kScaleStep;
+  static constexpr uint32_t kBytes = kFlags + 16;
+};
+constexpr int kSlideRowWaves = 8, kSlideRowTiles = 2;  // 16-row tiles of a wave
+
+// Eight waves with 32 rows each, as attn_rows_kernel: K and V of a step lie in
+// LDS in 16 bits, each wave brings 16 keys of one of them (blk, kv).  Rows of
+// 16 bits are copied into one of two buffers while the other is computed on; a
+// step of codes lies in half of the second buffer and is turned into the first
+// between two steps.
+template <int D, bool Q8>
+__global__ void __launch_bounds__(64 * kSlideRowWaves) slide_rows_kernel(const SlideArgs a) {
+  typedef SlidePart<D> P;
+  typedef SlideRowsLds<D> L;
+  typedef typename P::Rows Rows;
+  constexpr int RT = kSlideRowTiles, NW = kSlideRowWaves, DT = D / 16, KK = D / 32;
+  constexpr int CH = D / 8, RPI = 64 / CH, NI = 16 / RPI;  // as Part: 16-bit copies
+  constexpr int CQ = D / 16, RQ = 64 / CQ, NQ = 16 / RQ;   // of codes
+  extern __shared__ __attribute__((aligned(16))) unsigned char lds[];
+  const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+  const int blk = wave & 3;
+  const bool is_v = wave >= 4;
+  P t(a);
+  if (!t.start(lds)) return;
+  const int lane = t.lane, col = t.col, grp = t.grp;
+  const int row0 = (t.rb * NW + wave) * 16 * RT;
+  int* odds = reinterpret_cast<int*>(lds + L::kFlags);  // 1 + the last odd (even) step with any
+  uint64_t* seen = reinterpret_cast<uint64_t*>(lds + L::kSeen);
+  int* place = reinterpret_cast<int*>(lds + L::kPos);
+  // where the wave's 16 keys go in a buffer of K and V
+  const uint32_t mine = (is_v ? P::kStep : 0) + blk * 16 * D * 2;
+
+  // 16-bit rows of step s into buffer b (bytes from LDS' start)
+  auto bring = [&](int s, const Rows& rows, uint32_t b) {
+    int ln = lane;
+    asm("" : "+v"(ln));  // (the offsets made anew: registers are short)
+    const uint32_t to = t.lds0 + b + mine;
+    if (!Q8 && s < t.steps.cached) {
+      const long long at =
+          blk == 0 ? rows.at[0] : blk == 1 ? rows.at[1] : blk == 2 ? rows.at[2] : rows.at[3];
+      const uint16_t* src = uniform_ptr((is_v ? a.vc : a.kc) + at);
+      const uint32_t off0 = (ln / CH) * (D * 2) + (((ln % CH) ^ swz<D>(ln / CH)) << 4);
+#pragma unroll
+      for (int i = 0; i < NI; ++i)
+        dma16_base(to + i * 1024, (off0 ^ (swz<D>(i * RPI) << 4)) + i * 1024, src);
+    } else {
+      const int w0 = (s - t.steps.cached) * kKeys + 16 * blk;
+      const uint16_t* const base = is_v ? a.v : a.k;
+      const long long stride = is_v ? a.v_stride : a.k_stride;
+#pragma unroll 1
+      for (int i = 0; i < NI; ++i) {
+        const int row = i * RPI + ln / CH;
+        const int c = ((ln % CH) ^ swz<D>(row)) * 8;
+        const long long w = t.win.off + min(w0 + row, t.win.n - 1);
+        dma16_ptr(to + i * 1024, base + w * stride + t.h * D + c);
+      }
+    }
+  };
+  // codes of cached step s, and their scales, into half `half` of the second buffer
+  auto bring_codes = [&](const Rows& rows, int half) {
+    const long long at =
+        blk == 0 ? rows.at[0] : blk == 1 ? rows.at[1] : blk == 2 ? rows.at[2] : rows.at[3];
+    const unsigned char* src =
+        uniform_ptr(reinterpret_cast<const unsigned char*>(is_v ? a.vc : a.kc) + at);
+    const uint32_t to = t.lds0 + (2 + half) * P::kStep + (is_v ? P::kStep / 2 : 0) + blk * 16 * D;
+#pragma unroll
+    for (int i = 0; i < NQ; ++i) dma16_base(to + i * 1024, lane * 16 + i * 1024, src);
+    if (lane < D / 16) {
+      const unsigned char* sc = uniform_ptr(
+          reinterpret_cast<const unsigned char*>(is_v ? a.vs : a.ks) + at / (kKvGroup / 2));
+      dma16_base(t.lds0 + L::kScales + half * L::kScaleStep + (is_v ? L::kScaleStep / 2 : 0) + blk * D,
+                 lane * 16, sc);
+    }
+  };
+  // the wave's 16 keys of half `half` into the first buffer, as 16 bits; rows that
+  // are not there as 0.  True if one of V's groups is not finite and `full` is not so.
+  auto turn_codes = [&](int half, bool full, uint32_t there) {
+    const unsigned char* const from =
+        lds + (2 + half) * P::kStep + (is_v ? P::kStep / 2 : 0) + blk * 16 * D;
+    const unsigned char* const sc =
+        lds + L::kScales + half * L::kScaleStep + (is_v ? L::kScaleStep / 2 : 0) + blk * D;
+    bool odd = false;
+#pragma unroll
+    for (int i = 0; i < NQ; ++i) {
+      const int row = i * RQ + lane / CQ, c = lane % CQ;
+      const u32x4 x = *reinterpret_cast<const u32x4*>(from + i * 1024 + lane * 16);
+      uint32_t scale =
+          *reinterpret_cast<const uint16_t*>(sc + row * (D / kKvGroup * 2) + (c / 2) * 2);
+      if (!full && is_v) {
+        scale = there >> row & 1 ? scale : 0u;
+        // (taken out, and added by those that see it)
+        odd |= fp16_odd(scale);
+        scale = fp16_odd(scale) ? 0u : scale;
+      }
+      const h2 d = scale2(scale);
+      uint32_t w[4][2];
+#pragma unroll
+      for (int j = 0; j < 4; ++j) decode4(x[j], d, w[j]);
+      unsigned char* const to = lds + mine + row * (D * 2);
+      *reinterpret_cast<u32x4*>(to + (((2 * c) ^ swz<D>(row)) << 4)) =
+          (u32x4){w[0][0], w[0][1], w[1][0], w[1][1]};
+      *reinterpret_cast<u32x4*>(to + (((2 * c + 1) ^ swz<D>(row)) << 4)) =
+          (u32x4){w[2][0], w[2][1], w[3][0], w[3][1]};
+    }
+    return !full && is_v && __any(odd);
+  };
+  // Rows of V that are not there become 0, and so do infinities and NaN: true if
+  // there are any.  For the 16 rows that the calling wave has brought to buffer b.
+  auto clean_v = [&](uint32_t b, uint32_t there) {
+    unsigned char* vb = lds + b + mine;
+    bool odd = false;
+#pragma unroll 1
+    for (int i = 0; i < NI; ++i) {
+      u32x4* at = reinterpret_cast<u32x4*>(vb + i * 1024 + 16 * lane);
+      u32x4 w = *at;
+      const bool some = there >> (i * RPI + lane / CH) & 1;
+#pragma unroll
+      for (int c = 0; c < 4; ++c) {
+        const bool lo = fp16_odd(w[c]), hi = fp16_odd(w[c] >> 16);
+        odd |= some && (lo || hi);
+        w[c] &= some ? (lo ? 0u : 0xFFFFu) | (hi ? 0u : 0xFFFF0000u) : 0u;
+      }
+      *at = w;
+    }
+    return __any(odd);
+  };
+  // V's columns c.. (4) of key r of step s, as they are in memory
+  auto own_v = [&](int s, int r, int c, uint32_t (&x)[4]) {
+    if (s >= t.steps.cached) {
+      const long long w = t.win.off + (s - t.steps.cached) * kKeys + r;
+      const uint16_t* p = a.v + w * a.v_stride + t.h * D + c;
+#pragma unroll
+      for (int i = 0; i < 4; ++i) x[i] = p[i];
+    } else {
+      const long long at = t.rows_of(s).at[r >> 4] + (r & 15) * D + c;
+      if constexpr (Q8) {
+        const float d = half_bits_to_float(a.vs[at / kKvGroup]);
+        const signed char* p = reinterpret_cast<const signed char*>(a.vc) + at;
+#pragma unroll
+        for (int i = 0; i < 4; ++i) x[i] = f16b(p[i] * d);
+      } else {
+#pragma unroll
+        for (int i = 0; i < 4; ++i) x[i] = a.vc[at + i];
+      }
+    }
+  };
+
+  if (threadIdx.x < 2) odds[threadIdx.x] = 0;
+  if (wave == NW - 1 && a.parent) see_tree(a, t.win, t.len, lane, place, seen);
+
+  h8 qf[RT][KK];
+  f4 acc[RT][DT];
+  // lim: the score, less mref, above which mref moves: kRise once it is set
+  float mref[RT], l[RT], lim[RT];
+#pragma unroll
+  for (int rt = 0; rt < RT; ++rt) {
+    t.load_q(row0 + rt * 16 + col, qf[rt]);
+    mref[rt] = 0.f;
+    l[rt] = 0.f;
+    lim[rt] = -INFINITY;
+#pragma unroll
+    for (int d = 0; d < DT; ++d) acc[rt][d] = (f4){0.f, 0.f, 0.f, 0.f};
+  }
+  const uint32_t koff = t.k_offset(), voff = t.v_offset();
+
+  // A step on the buffer at b.
+  auto compute = [&](int step, uint32_t b, bool full, uint64_t there, bool odd) {
+    uint32_t kbase = koff + b, vbase = voff + b;
+#pragma unroll 1
+    for (int st = 0; st < 2; ++st) {
+      f4 s[2][RT];
+#pragma unroll
+      for (int b = 0; b < 2; ++b)
+#pragma unroll
+        for (int rt = 0; rt < RT; ++rt) s[b][rt] = (f4){0.f, 0.f, 0.f, 0.f};
+      // (the two blocks' pieces one step ahead; the fences keep the compiler from
+      // reading further ahead: registers)
+      h8 kn[2];
+#pragma unroll
+      for (int b = 0; b < 2; ++b) kn[b] = t.k_frag(P::k_piece(kbase, 0), 0, b);
+#pragma unroll
+      for (int ks = 0; ks < KK; ++ks) {
+        const h8 kf[2] = {kn[0], kn[1]};
+        if (ks + 1 < KK) {
+#pragma unroll
+          for (int b = 0; b < 2; ++b)
+            kn[b] = t.k_frag(P::k_piece(kbase, (ks + 1) % P::KO), ks + 1, b);
+        }
+        asm volatile("" ::: "memory");
+#pragma unroll
+        for (int b = 0; b < 2; ++b)
+#pragma unroll
+          for (int rt = 0; rt < RT; ++rt)
+            s[b][rt] = __builtin_amdgcn_mfma_f32_16x16x32_f16(kf[b], qf[rt][ks], s[b][rt], 0, 0, 0);
+      }
+      bool move = false;
+      float top[RT];
+#pragma unroll
+      for (int rt = 0; rt < RT; ++rt) {
+#pragma unroll
+        for (int b = 0; b < 2; ++b) {
+#pragma unroll
+          for (int i = 0; i < 4; ++i)
+            s[b][rt][i] = __builtin_fmaf(s[b][rt][i], a.scale_log2, -mref[rt]);
+          if (!full) {
+            const int node = t.node_of(row0 + rt * 16 + col);
+            const uint32_t see =
+                t.seen4(step, 32 * st + 16 * b + 4 * grp, there, node,
+                        a.parent ? place[node] : t.len + node, a.parent ? seen[node] : 0);
+#pragma unroll
+            for (int i = 0; i < 4; ++i) s[b][rt][i] = see >> i & 1 ? s[b][rt][i] : -INFINITY;
+          }
+        }
+        top[rt] = max3(max3(s[0][rt][0], s[0][rt][1], s[0][rt][2]),
+                       max3(s[0][rt][3], s[1][rt][0], s[1][rt][1]),
+                       max3(s[1][rt][2], s[1][rt][3], s[1][rt][3]));
+        move |= top[rt] > lim[rt];
+      }
+      if (__any(move)) {
+#pragma unroll
+        for (int rt = 0; rt < RT; ++rt) {
+          float m = fmaxf(top[rt], __shfl_xor(top[rt], 16));
+          m = fmaxf(m, __shfl_xor(m, 32));
+          const bool set = m > lim[rt], begun = lim[rt] > 0.f;
+          const float by = set ? m - kBelow : 0.f;
+          const float f = !set ? 1.f : begun ? __builtin_amdgcn_exp2f(-by) : 0.f;
+          mref[rt] += by;
+          l[rt] *= f;
+#pragma unroll
+          for (int d = 0; d < DT; ++d) acc[rt][d] *= f;
+          lim[rt] = set ? kRise : lim[rt];
+#pragma unroll
+          for (int b = 0; b < 2; ++b) s[b][rt] -= by;
+        }
+      }
+      h8 pf[RT];
+#pragma unroll
+      for (int rt = 0; rt < RT; ++rt) {
+#pragma unroll
+        for (int b = 0; b < 2; ++b)
+#pragma unroll
+          for (int i = 0; i < 4; ++i) {
+            s[b][rt][i] = __builtin_amdgcn_exp2f(s[b][rt][i]);
+            pf[rt][4 * b + i] = static_cast<_Float16>(s[b][rt][i]);
+          }
+        l[rt] += ((s[0][rt][0] + s[0][rt][1]) + (s[0][rt][2] + s[0][rt][3])) +
+                 ((s[1][rt][0] + s[1][rt][1]) + (s[1][rt][2] + s[1][rt][3]));
+      }
+      if (odd) {
+#pragma unroll 1
+        for (int r = 0; r < 32; ++r) {  // one by one, to the rows that see them
+          if (!(there >> (32 * st + r) & 1)) continue;
+          const int from = col + 16 * ((r & 15) >> 2);  // the lane that has key r's weight
+#pragma unroll
+          for (int rt = 0; rt < RT; ++rt) {
+            float w = 0.f;
+#pragma unroll
+            for (int i = 0; i < 8; ++i)
+              w = i == (r >> 4) * 4 + (r & 3) ? s[i >> 2][rt][i & 3] : w;
+            w = __shfl(w, from);
+            const int node = t.node_of(row0 + rt * 16 + col);
+            const bool see = t.seen4(step, 32 * st + r, there, node,
+                                     a.parent ? place[node] : t.len + node,
+                                     a.parent ? seen[node] : 0) & 1;
+#pragma unroll
+            for (int d = 0; d < DT; ++d) {
+              uint32_t x[4];
+              own_v(step, 32 * st + r, d * 16 + 4 * grp, x);
+#pragma unroll
+              for (int i = 0; i < 4; ++i)
+                acc[rt][d][i] += see && fp16_odd(x[i]) ? w * half_bits_to_float(x[i]) : 0.f;
+              asm volatile("" : "+v"(acc[rt][d])::"memory");  // (one after the other: registers)
+            }
+          }
+        }
+      }
+      h8 next[2] = {t.v_frag(P::v_tile(vbase, 0), 0), t.v_frag(P::v_tile(vbase, 1), 0)};
+#pragma unroll
+      for (int d = 0; d < DT; ++d) {  // two tiles read ahead
+        const h8 vf = next[d % 2];
+        asm volatile("" ::: "memory");
+        if (d + 2 < DT) next[d % 2] = t.v_frag(P::v_tile(vbase, d + 2), 0);
+        asm volatile("" ::: "memory");
+#pragma unroll
+        for (int rt = 0; rt < RT; ++rt)
+          acc[rt][d] = __builtin_amdgcn_mfma_f32_16x16x32_f16(vf, pf[rt], acc[rt][d], 0, 0, 0);
+      }
+      kbase += 32 * D * 2;
+      vbase += 32 * D * 2;
+    }
+  };
+
+  P::settle_q(qf);
+  int step = t.begin, it = 0;
+  const int cached_end = min(t.end, t.steps.cached);
+  if constexpr (Q8) {
+    if (step < cached_end) {
+      Rows rows = t.rows_of(step);
+      bring_codes(rows, 0);
+      for (; step < cached_end; ++it) {
+        const uint32_t ok = rows.ok;
+        const bool full = t.full(step, ok);
+        const uint64_t there = full ? ~0ull : t.present(step, ok);
+        const int next = t.steps.skip(step + 1);
+        wait_vm();
+        bar();  // nobody reads the first buffer any more (and the flags are cleared)
+        if (turn_codes(it & 1, full, static_cast<uint32_t>(there >> (16 * blk)) & 0xFFFFu))
+          odds[it & 1] = step + 1;
+        wait_lds();
+        if (next < cached_end) {
+          rows = t.rows_of(next);
+          bring_codes(rows, (it + 1) & 1);
+        }
+        bar();  // everybody's keys are there
+        compute(step, 0, full, there, !full && odds[it & 1] == step + 1);
+        step = next;
+      }
+    }
+  }
+  if (step < t.end) {
+    // the buffers in turn, the second first: the first may still be read
+    Rows rows;
+    rows.ok = 15u;
+    if (!Q8 && step < t.steps.cached) rows = t.rows_of(step);
+    if (Q8) bar();  // (codes in the second one are read)
+    bring(step, rows, 2 * P::kStep);
+    if (!Q8 || it == 0) bar();  // the flags are cleared, the tree is there
+    for (uint32_t b = 2 * P::kStep; step < t.end; b ^= 2 * P::kStep, ++it) {
+      const bool cached = !Q8 && step < t.steps.cached;
+      const uint32_t ok = rows.ok;
+      const bool full = cached ? t.full(step, ok) : t.full_window(step);
+      const uint64_t there = full ? ~0ull : t.present(step, ok);
+      const int next = t.steps.skip(step + 1);
+      rows.ok = 15u;
+      if (!Q8 && next < cached_end) rows = t.rows_of(next);
+      wait_vm();
+      if (is_v && !full && clean_v(b, static_cast<uint32_t>(there >> (16 * blk)) & 0xFFFFu))
+        odds[it & 1] = step + 1;
+      bar();  // everybody's copies of this step are here, and nobody reads the other buffer
+      if (next < t.end) bring(next, rows, b ^ 2 * P::kStep);
+      compute(step, b, full, there, !full && odds[it & 1] == step + 1);
+      step = next;
+    }
+  }
+
+#pragma unroll
+  for (int rt = 0; rt < RT; ++rt) {
+    const int r = row0 + rt * 16 + col;
+    l[rt] += __shfl_xor(l[rt], 16);
+    l[rt] += __shfl_xor(l[rt], 32);
+    const float lt = a.parent && !seen[t.node_of(r)] ? 0.f : l[rt];  // 0: an absent node
+    t.template store<DT, 16>(r, 4 * grp, acc[rt], mref[rt], lt, grp == 0);
+  }
+}
+
 // ---- host -----------------------------------------------------------------------
 
 // How a call is laid out: rows of a workgroup, the most units.
 struct SlideLayout {
   int block_rows, row_blocks, max_units, goal;
-  bool cut;
-  int few[2];                         // the most sequences for less than one round, and two
+  bool cut, spread;
+  int few[3];  // the most sequences for less than one round, two, and one of many row blocks
   size_t plan_bytes, o_bytes, bytes;  // of the workspace
 };
 static SlideLayout slide_layout(int n_seq, int max_window, int max_len, int group, int n_kv, int dim,
                                 int reach, int sinks) {
   SlideLayout l;
   const long long rows = static_cast<long long>(max_window) * group;
-  l.block_rows = rows > 16 ? 32 : 16;
+  l.block_rows = rows > 128 ? 256 : rows > 16 ? 32 : 16;
   l.row_blocks = static_cast<int>((rows + l.block_rows - 1) / l.block_rows);
+  l.spread = l.row_blocks >= 8;
   const long long units = static_cast<long long>(n_seq) * n_kv;
   // a sequence's steps at the most
   const long long keys = static_cast<long long>(max_len) + max_window;
   const long long near = static_cast<long long>(reach) + max_window + sinks + 2 * kKeys;
   const long long most = ((keys < near ? keys : near) + kKeys - 1) / kKeys + 1;
   // workgroups that the card holds at once, and units of them
-  const int each = dim == 256 ? 2 : 4;
+  const int each = l.block_rows == 256 ? 1 : dim == 256 ? 2 : 4;
   const long long slots = 256 * each;
   const long long per = 32 * each >= l.row_blocks ? 32 * each / l.row_blocks * 8 : 8;
   const bool rounds = units >= 2 * slots;
   for (int i = 0; i < 2; ++i) l.few[i] = static_cast<int>(((i + 1) * slots - 1) / n_kv);
+  l.few[2] = static_cast<int>((slots - 1) / (static_cast<long long>(n_kv) * l.row_blocks));
   long long n = units;
-  l.cut = most > 1 && (units < slots || most > 8);
+  // (many row blocks fill the card without a cut)
+  l.cut = most > 1 && (units < slots || most > 8) && !(l.spread && units * l.row_blocks >= slots);
   l.goal = 1;
-  if (l.cut && !rounds) {
+  if (l.cut && l.spread) {
+    n = units + slots / l.row_blocks;
+    l.goal = static_cast<int>(n_seq <= 64 ? n : n - units);
+  } else if (l.cut && !rounds) {
     n = (2 * units + per - 1) / per * per;
     // (a part a head lost to rounding; one in a thousand less: parts_of rounds)
     l.goal = static_cast<int>(n_seq <= 64 ? n : n - units - ((n - units) >> 10));
@@ -704,8 +1081,12 @@ static SlideLayout slide_layout(int n_seq, int max_window, int max_len, int grou
 
 template <int D, bool Q8>
 static int slide_launch(const SlideArgs& a, hipStream_t s, const char* nm) {
-  const dim3 grid(static_cast<unsigned>((a.max_units + 7LL) / 8 * 8 * a.row_blocks));
-  if (a.block_rows == 32)
+  const long long n = a.spread ? a.max_units : (a.max_units + 7LL) / 8 * 8;
+  const dim3 grid(static_cast<unsigned>(n * a.row_blocks));
+  if (a.block_rows == 256)
+    hipLaunchKernelGGL((slide_rows_kernel<D, Q8>), grid, dim3(64 * kSlideRowWaves),
+                       SlideRowsLds<D>::kBytes, s, a);
+  else if (a.block_rows == 32)
     hipLaunchKernelGGL((slide_few_kernel<D, 2, Q8>), grid, dim3(256), (SlideFewLds<D, 2>::kBytes), s,
                        a);
   else
@@ -832,6 +1213,7 @@ static int attn_slide(const uint16_t* q, const uint16_t* k, const uint16_t* v, l
   a.max_units = l.max_units;
   a.goal = l.goal;
   a.cut = l.cut;
+  a.spread = l.spread;
   a.scale_log2 = scale * kLog2e;
   a.reach = far;
   a.sinks = sinks;
