@@ -49,8 +49,17 @@ __device__ __forceinline__ void settle(T (&x)[N]) {
 struct SlideArgs : AttnArgs {
   const uint16_t *ks, *vs;  // scales of the quantised cache (kc, vc: its codes)
   int reach, sinks;
-  bool spread;  // row blocks one after the other, not 8 apart
+  int spread;  // how workgroups are mapped to row blocks
 };
+enum { kSpreadUnits, kSpreadTurns, kSpreadRuns };
+
+// As cold_args, for paths taken now and then.
+typedef const __attribute__((address_space(4))) SlideArgs* slide_p;
+__device__ __forceinline__ slide_p cold_slide() {
+  slide_p p = (slide_p)__builtin_amdgcn_kernarg_segment_ptr();
+  asm volatile("" : "+s"(p));
+  return p;
+}
 
 // The steps that a sequence's nodes first .. last see: [0, sink) and [low,
 // high), the window's steps from `cached` on.
@@ -101,10 +110,19 @@ struct SlidePart : Part<D> {
     this->col = lane & 15;
     this->grp = lane >> 4;
     const int id = blockIdx.x;
-    if (sa.spread) {
-      // Many row blocks: over all XCDs, the last rows, which see most, first.
+    if (sa.spread == kSpreadTurns) {
+      // Many row blocks that see all before them: over the XCDs in turn, the
+      // last rows, which see most, first.
       this->unit = id / sa.row_blocks;
       this->rb = sa.row_blocks - 1 - (id - this->unit * sa.row_blocks);
+    } else if (sa.spread == kSpreadRuns) {
+      // That see a window: an XCD has neighbours, whose windows are the same keys
+      // but for a few, and reads them once (4,096 tokens of 16 heads of 256 over
+      // windows of 2,048: RUNS_US us, in turn TURNS_US).
+      // (past the last unit there is none)
+      const int at = (id & 7) * (gridDim.x >> 3) + (id >> 3);
+      this->unit = at / sa.row_blocks;
+      this->rb = at - this->unit * sa.row_blocks;
     } else {
       // The row blocks of a unit are 8 workgroups apart: on one XCD, whose L2
       // then reads the unit's keys once.
@@ -112,10 +130,12 @@ struct SlidePart : Part<D> {
       this->rb = in >> 3;
       this->unit = oct * 8 + (in & 7);
     }
+    auto one = [](int v) { return __builtin_amdgcn_readfirstlane(v); };  // (the same in every lane)
+    this->unit = one(this->unit);
+    this->rb = one(this->rb);
     Unit u;
     const bool plan = sa.cut && id == 0 && __builtin_amdgcn_readfirstlane(threadIdx.x >> 6) == 0;
     if (!find_unit(sa, this->unit, lane, plan, u)) return false;
-    auto one = [](int v) { return __builtin_amdgcn_readfirstlane(v); };  // (the same in every lane)
     this->h = one(u.h);
     this->parts = one(u.parts);
     this->win = Window{one(u.win.off), one(u.win.n)};
@@ -126,8 +146,8 @@ struct SlidePart : Part<D> {
     this->table =
         (const_int_p)(sa.pages + static_cast<long long>(one(u.seq)) * sa.pages_per_seq);
     const int n = this->win.n;
-    first = sa.parent ? 0 : this->rb * sa.block_rows / sa.group;
-    last = sa.parent ? n - 1 : min((this->rb + 1) * sa.block_rows - 1, this->rows - 1) / sa.group;
+    first = one(sa.parent ? 0 : this->rb * sa.block_rows / sa.group);
+    last = one(sa.parent ? n - 1 : min((this->rb + 1) * sa.block_rows - 1, this->rows - 1) / sa.group);
     const Steps all = steps_seen(this->len, n, 0, n - 1, sa.reach, sa.sinks);
     steps = steps_seen(this->len, n, first, last, sa.reach, sa.sinks);
     const int k = one(u.k), part = one(u.part), count = one(u.steps);
@@ -187,13 +207,16 @@ struct SlidePart : Part<D> {
                                             uint64_t up) const {
     uint32_t m = static_cast<uint32_t>(there >> k) & 15u;
     const bool cached = s < steps.cached;
-    if (!cached && sa.parent) return m & static_cast<uint32_t>(up >> k);
+    const slide_p ca = cold_slide();
+    const int sinks = ca->sinks;
+    const uint32_t reach = ca->reach;
+    if (!cached && ca->parent) return m & static_cast<uint32_t>(up >> k);
     // (positions as unsigned differences: no further than pos, and less than reach)
     const int p0 = (cached ? s * kKeys : this->len + (s - steps.cached) * kKeys) + k;
 #pragma unroll
     for (int i = 0; i < 4; ++i) {
       const uint32_t back = pos - (p0 + i);
-      const uint32_t most = p0 + i < sa.sinks ? 0x7FFFFFFFu : static_cast<uint32_t>(sa.reach - 1);
+      const uint32_t most = p0 + i < sinks ? 0x7FFFFFFFu : reach - 1;
       m &= back <= most ? ~0u : ~(1u << i);
     }
     return m;
@@ -718,9 +741,10 @@ __global__ void __launch_bounds__(64 * kSlideRowWaves) slide_rows_kernel(const S
       for (int i = 0; i < NI; ++i)
         dma16_base(to + i * 1024, (off0 ^ (swz<D>(i * RPI) << 4)) + i * 1024, src);
     } else {
+      const slide_p ca = cold_slide();
       const int w0 = (s - t.steps.cached) * kKeys + 16 * blk;
-      const uint16_t* const base = is_v ? a.v : a.k;
-      const long long stride = is_v ? a.v_stride : a.k_stride;
+      const uint16_t* const base = is_v ? ca->v : ca->k;
+      const long long stride = is_v ? ca->v_stride : ca->k_stride;
 #pragma unroll 1
       for (int i = 0; i < NI; ++i) {
         const int row = i * RPI + ln / CH;
@@ -798,27 +822,6 @@ __global__ void __launch_bounds__(64 * kSlideRowWaves) slide_rows_kernel(const S
     }
     return __any(odd);
   };
-  // V's columns c.. (4) of key r of step s, as they are in memory
-  auto own_v = [&](int s, int r, int c, uint32_t (&x)[4]) {
-    if (s >= t.steps.cached) {
-      const long long w = t.win.off + (s - t.steps.cached) * kKeys + r;
-      const uint16_t* p = a.v + w * a.v_stride + t.h * D + c;
-#pragma unroll
-      for (int i = 0; i < 4; ++i) x[i] = p[i];
-    } else {
-      const long long at = t.rows_of(s).at[r >> 4] + (r & 15) * D + c;
-      if constexpr (Q8) {
-        const float d = half_bits_to_float(a.vs[at / kKvGroup]);
-        const signed char* p = reinterpret_cast<const signed char*>(a.vc) + at;
-#pragma unroll
-        for (int i = 0; i < 4; ++i) x[i] = f16b(p[i] * d);
-      } else {
-#pragma unroll
-        for (int i = 0; i < 4; ++i) x[i] = a.vc[at + i];
-      }
-    }
-  };
-
   if (threadIdx.x < 2) odds[threadIdx.x] = 0;
   if (wave == NW - 1 && a.parent) see_tree(a, t.win, t.len, lane, place, seen);
 
@@ -877,10 +880,11 @@ __global__ void __launch_bounds__(64 * kSlideRowWaves) slide_rows_kernel(const S
           for (int i = 0; i < 4; ++i)
             s[b][rt][i] = __builtin_fmaf(s[b][rt][i], a.scale_log2, -mref[rt]);
           if (!full) {
+            const bool tree = cold_slide()->parent;
             const int node = t.node_of(row0 + rt * 16 + col);
             const uint32_t see =
                 t.seen4(step, 32 * st + 16 * b + 4 * grp, there, node,
-                        a.parent ? place[node] : t.len + node, a.parent ? seen[node] : 0);
+                        tree ? place[node] : t.len + node, tree ? seen[node] : 0);
 #pragma unroll
             for (int i = 0; i < 4; ++i) s[b][rt][i] = see >> i & 1 ? s[b][rt][i] : -INFINITY;
           }
@@ -923,26 +927,51 @@ __global__ void __launch_bounds__(64 * kSlideRowWaves) slide_rows_kernel(const S
       if (odd) {
 #pragma unroll 1
         for (int r = 0; r < 32; ++r) {  // one by one, to the rows that see them
-          if (!(there >> (32 * st + r) & 1)) continue;
+          const int key = 32 * st + r;
+          if (!(there >> key & 1)) continue;
+          // V's row as it is in memory
+          const slide_p ca = cold_slide();
+          const bool window = step >= t.steps.cached;
+          long long at;
+          if (window) {
+            at = static_cast<long long>(t.win.off + (step - t.steps.cached) * kKeys + key) *
+                     ca->v_stride + t.h * D;
+          } else {
+            const int j = step * kKeys + key;
+            at = (((static_cast<long long>(t.table[j >> ca->page_log2]) * ca->n_kv + t.h)
+                   << ca->page_log2) +
+                  (j & ((1 << ca->page_log2) - 1))) * D;
+          }
+          const uint16_t* const row = (window ? ca->v : ca->vc) + at;
+          const bool codes = Q8 && !window;
           const int from = col + 16 * ((r & 15) >> 2);  // the lane that has key r's weight
+          float w[RT];
 #pragma unroll
           for (int rt = 0; rt < RT; ++rt) {
-            float w = 0.f;
+            float x = 0.f;
 #pragma unroll
             for (int i = 0; i < 8; ++i)
-              w = i == (r >> 4) * 4 + (r & 3) ? s[i >> 2][rt][i & 3] : w;
-            w = __shfl(w, from);
+              x = i == (r >> 4) * 4 + (r & 3) ? s[i >> 2][rt][i & 3] : x;
+            w[rt] = __shfl(x, from);
             const int node = t.node_of(row0 + rt * 16 + col);
-            const bool see = t.seen4(step, 32 * st + r, there, node,
-                                     a.parent ? place[node] : t.len + node,
-                                     a.parent ? seen[node] : 0) & 1;
+            const bool see = t.seen4(step, key, there, node,
+                                     ca->parent ? place[node] : t.len + node,
+                                     ca->parent ? seen[node] : 0) & 1;
+            w[rt] = see ? w[rt] : -1.f;  // (weights are not negative)
+          }
 #pragma unroll
-            for (int d = 0; d < DT; ++d) {
-              uint32_t x[4];
-              own_v(step, 32 * st + r, d * 16 + 4 * grp, x);
+          for (int d = 0; d < DT; ++d) {
+            const int c = d * 16 + 4 * grp;
+            // (a group of codes that is not finite is so throughout)
+            float x[4];
+#pragma unroll
+            for (int i = 0; i < 4; ++i)
+              x[i] = half_bits_to_float(codes ? ca->vs[(at + c) / kKvGroup] : row[c + i]);
+#pragma unroll
+            for (int rt = 0; rt < RT; ++rt) {
 #pragma unroll
               for (int i = 0; i < 4; ++i)
-                acc[rt][d][i] += see && fp16_odd(x[i]) ? w * half_bits_to_float(x[i]) : 0.f;
+                acc[rt][d][i] += w[rt] >= 0.f && !isfinite(x[i]) ? w[rt] * x[i] : 0.f;
               asm volatile("" : "+v"(acc[rt][d])::"memory");  // (one after the other: registers)
             }
           }
@@ -1032,7 +1061,8 @@ __global__ void __launch_bounds__(64 * kSlideRowWaves) slide_rows_kernel(const S
 // How a call is laid out: rows of a workgroup, the most units.
 struct SlideLayout {
   int block_rows, row_blocks, max_units, goal;
-  bool cut, spread;
+  bool cut;
+  int spread;
   int few[3];  // the most sequences for less than one round, two, and one of many row blocks
   size_t plan_bytes, o_bytes, bytes;  // of the workspace
 };
@@ -1042,7 +1072,8 @@ static SlideLayout slide_layout(int n_seq, int max_window, int max_len, int grou
   const long long rows = static_cast<long long>(max_window) * group;
   l.block_rows = rows > 128 ? 256 : rows > 16 ? 32 : 16;
   l.row_blocks = static_cast<int>((rows + l.block_rows - 1) / l.block_rows);
-  l.spread = l.row_blocks >= 8;
+  const bool near_only = reach / 2 < max_len / 2 + max_window / 2;
+  l.spread = l.row_blocks < 8 ? kSpreadUnits : near_only ? kSpreadRuns : kSpreadTurns;
   const long long units = static_cast<long long>(n_seq) * n_kv;
   // a sequence's steps at the most
   const long long keys = static_cast<long long>(max_len) + max_window;
@@ -1081,8 +1112,8 @@ static SlideLayout slide_layout(int n_seq, int max_window, int max_len, int grou
 
 template <int D, bool Q8>
 static int slide_launch(const SlideArgs& a, hipStream_t s, const char* nm) {
-  const long long n = a.spread ? a.max_units : (a.max_units + 7LL) / 8 * 8;
-  const dim3 grid(static_cast<unsigned>(n * a.row_blocks));
+  const long long n = a.spread == kSpreadUnits ? (a.max_units + 7LL) / 8 * 8 : a.max_units;
+  const dim3 grid(static_cast<unsigned>((n * a.row_blocks + 7) / 8 * 8));
   if (a.block_rows == 256)
     hipLaunchKernelGGL((slide_rows_kernel<D, Q8>), grid, dim3(64 * kSlideRowWaves),
                        SlideRowsLds<D>::kBytes, s, a);
