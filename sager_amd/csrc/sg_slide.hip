@@ -201,9 +201,9 @@ struct SlidePart : Part<D> {
       if (!(ok >> b & 1)) m &= ~(0xFFFFull << (16 * b));
     return m;
   }
-  // bit i: key k + i of step s (i < 4) is there and seen by a row of node `node`
-  // at position pos; up: whom of the window's tree it sees (with a parent).
-  __device__ __forceinline__ uint32_t seen4(int s, int k, uint64_t there, int node, int pos,
+  // bit i: key k + i of step s (i < 4) is there and seen by a node at position pos;
+  // up: whom of the window's tree it sees (with a parent).
+  __device__ __forceinline__ uint32_t seen4(int s, int k, uint64_t there, int pos,
                                             uint64_t up) const {
     uint32_t m = static_cast<uint32_t>(there >> k) & 15u;
     const bool cached = s < steps.cached;
@@ -450,7 +450,7 @@ __global__ void __launch_bounds__(256, slide_waves(D, RT, Q8)) slide_few_kernel(
       for (int i = 0; i < 4; ++i) e[rt][i] = __builtin_fmaf(s[rt][i], a.scale_log2, -mref[rt]);
       see[rt] = 15u;
       if (!full) {
-        see[rt] = t.seen4(step, 16 * wave + 4 * grp, there, node[rt],
+        see[rt] = t.seen4(step, 16 * wave + 4 * grp, there,
                           a.parent ? place[node[rt]] : t.len + node[rt],
                           a.parent ? seen[node[rt]] : 0);
 #pragma unroll
@@ -699,6 +699,7 @@ struct SlideRowsLds {
   static constexpr uint32_t kBytes = kFlags + 16;
 };
 constexpr int kSlideRowWaves = 8, kSlideRowTiles = 2;  // 16-row tiles of a wave
+constexpr int kAhead = 4;                              // operands read ahead
 
 // Eight waves with 32 rows each, as attn_rows_kernel: K and V of a step lie in
 // LDS in 16 bits, each wave brings 16 keys of one of them (blk, kv).  Rows of
@@ -743,14 +744,23 @@ __global__ void __launch_bounds__(64 * kSlideRowWaves) slide_rows_kernel(const S
     } else {
       const slide_p ca = cold_slide();
       const int w0 = (s - t.steps.cached) * kKeys + 16 * blk;
-      const uint16_t* const base = is_v ? ca->v : ca->k;
+      const uint16_t* const base = (is_v ? ca->v : ca->k) + t.h * D;
       const long long stride = is_v ? ca->v_stride : ca->k_stride;
+      if (w0 + 16 <= t.win.n) {
+        const uint16_t* src = uniform_ptr(base + (t.win.off + w0) * stride);
+        const uint32_t row0 = (ln / CH) * (static_cast<uint32_t>(stride) * 2);
+        const uint32_t c0 = ((ln % CH) ^ swz<D>(ln / CH)) << 4;
+#pragma unroll
+        for (int i = 0; i < NI; ++i)
+          dma16_base(to + i * 1024, row0 + (c0 ^ (swz<D>(i * RPI) << 4)), src + i * RPI * stride);
+      } else {
 #pragma unroll 1
-      for (int i = 0; i < NI; ++i) {
-        const int row = i * RPI + ln / CH;
-        const int c = ((ln % CH) ^ swz<D>(row)) * 8;
-        const long long w = t.win.off + min(w0 + row, t.win.n - 1);
-        dma16_ptr(to + i * 1024, base + w * stride + t.h * D + c);
+        for (int i = 0; i < NI; ++i) {
+          const int row = i * RPI + ln / CH;
+          const int c = ((ln % CH) ^ swz<D>(row)) * 8;
+          const long long w = t.win.off + min(w0 + row, t.win.n - 1);
+          dma16_ptr(to + i * 1024, base + w * stride + c);
+        }
       }
     }
   };
@@ -850,41 +860,41 @@ __global__ void __launch_bounds__(64 * kSlideRowWaves) slide_rows_kernel(const S
       for (int b = 0; b < 2; ++b)
 #pragma unroll
         for (int rt = 0; rt < RT; ++rt) s[b][rt] = (f4){0.f, 0.f, 0.f, 0.f};
-      // (the two blocks' pieces one step ahead; the fences keep the compiler from
-      // reading further ahead: registers)
-      h8 kn[2];
+      // K's pieces, of the two blocks in turn, kAhead of them under way: what LDS
+      // takes to answer eight waves is longer than the products of one or two
+      h8 kn[kAhead];
+      auto k_read = [&](int f) {
+        return t.k_frag(P::k_piece(kbase, (f >> 1) % P::KO), f >> 1, f & 1);
+      };
 #pragma unroll
-      for (int b = 0; b < 2; ++b) kn[b] = t.k_frag(P::k_piece(kbase, 0), 0, b);
+      for (int f = 0; f < kAhead; ++f) kn[f] = k_read(f);
 #pragma unroll
-      for (int ks = 0; ks < KK; ++ks) {
-        const h8 kf[2] = {kn[0], kn[1]};
-        if (ks + 1 < KK) {
+      for (int f = 0; f < 2 * KK; ++f) {
+        const h8 kf = kn[f % kAhead];
 #pragma unroll
-          for (int b = 0; b < 2; ++b)
-            kn[b] = t.k_frag(P::k_piece(kbase, (ks + 1) % P::KO), ks + 1, b);
-        }
-        asm volatile("" ::: "memory");
-#pragma unroll
-        for (int b = 0; b < 2; ++b)
-#pragma unroll
-          for (int rt = 0; rt < RT; ++rt)
-            s[b][rt] = __builtin_amdgcn_mfma_f32_16x16x32_f16(kf[b], qf[rt][ks], s[b][rt], 0, 0, 0);
+        for (int rt = 0; rt < RT; ++rt)
+          s[f & 1][rt] =
+              __builtin_amdgcn_mfma_f32_16x16x32_f16(kf, qf[rt][f >> 1], s[f & 1][rt], 0, 0, 0);
+        if (f + kAhead < 2 * KK) kn[f % kAhead] = k_read(f + kAhead);
+        __builtin_amdgcn_sched_barrier(0);
       }
       bool move = false;
       float top[RT];
 #pragma unroll
       for (int rt = 0; rt < RT; ++rt) {
 #pragma unroll
-        for (int b = 0; b < 2; ++b) {
+        for (int b = 0; b < 2; ++b)
 #pragma unroll
           for (int i = 0; i < 4; ++i)
             s[b][rt][i] = __builtin_fmaf(s[b][rt][i], a.scale_log2, -mref[rt]);
-          if (!full) {
-            const bool tree = cold_slide()->parent;
-            const int node = t.node_of(row0 + rt * 16 + col);
-            const uint32_t see =
-                t.seen4(step, 32 * st + 16 * b + 4 * grp, there, node,
-                        tree ? place[node] : t.len + node, tree ? seen[node] : 0);
+        if (!full) {
+          const bool tree = cold_slide()->parent;
+          const int node = t.node_of(row0 + rt * 16 + col);
+          const int pos = tree ? place[node] : t.len + node;
+          const uint64_t up = tree ? seen[node] : 0;
+#pragma unroll
+          for (int b = 0; b < 2; ++b) {
+            const uint32_t see = t.seen4(step, 32 * st + 16 * b + 4 * grp, there, pos, up);
 #pragma unroll
             for (int i = 0; i < 4; ++i) s[b][rt][i] = see >> i & 1 ? s[b][rt][i] : -INFINITY;
           }
@@ -954,7 +964,7 @@ __global__ void __launch_bounds__(64 * kSlideRowWaves) slide_rows_kernel(const S
               x = i == (r >> 4) * 4 + (r & 3) ? s[i >> 2][rt][i & 3] : x;
             w[rt] = __shfl(x, from);
             const int node = t.node_of(row0 + rt * 16 + col);
-            const bool see = t.seen4(step, key, there, node,
+            const bool see = t.seen4(step, key, there,
                                      ca->parent ? place[node] : t.len + node,
                                      ca->parent ? seen[node] : 0) & 1;
             w[rt] = see ? w[rt] : -1.f;  // (weights are not negative)
@@ -977,16 +987,18 @@ __global__ void __launch_bounds__(64 * kSlideRowWaves) slide_rows_kernel(const S
           }
         }
       }
-      h8 next[2] = {t.v_frag(P::v_tile(vbase, 0), 0), t.v_frag(P::v_tile(vbase, 1), 0)};
+      h8 vn[kAhead];
 #pragma unroll
-      for (int d = 0; d < DT; ++d) {  // two tiles read ahead
-        const h8 vf = next[d % 2];
-        asm volatile("" ::: "memory");
-        if (d + 2 < DT) next[d % 2] = t.v_frag(P::v_tile(vbase, d + 2), 0);
-        asm volatile("" ::: "memory");
+      for (int d = 0; d < kAhead; ++d) vn[d] = t.v_frag(P::v_tile(vbase, d), 0);
+      __builtin_amdgcn_sched_barrier(0);
+#pragma unroll
+      for (int d = 0; d < DT; ++d) {
+        const h8 vf = vn[d % kAhead];
 #pragma unroll
         for (int rt = 0; rt < RT; ++rt)
           acc[rt][d] = __builtin_amdgcn_mfma_f32_16x16x32_f16(vf, pf[rt], acc[rt][d], 0, 0, 0);
+        if (d + kAhead < DT) vn[d % kAhead] = t.v_frag(P::v_tile(vbase, d + kAhead), 0);
+        __builtin_amdgcn_sched_barrier(0);
       }
       kbase += 32 * D * 2;
       vbase += 32 * D * 2;
@@ -1187,6 +1199,9 @@ static int attn_slide(const uint16_t* q, const uint16_t* k, const uint16_t* v, l
   if (q_stride < static_cast<long long>(n_heads) * dim ||
       k_stride < static_cast<long long>(n_kv) * dim || v_stride < static_cast<long long>(n_kv) * dim)
     return set_error(SG_ERR_GEOMETRY, "%s: a token stride is less than a token", nm);
+  // (a few tokens' rows are reached by 32-bit offsets)
+  if (k_stride >= 1LL << 27 || v_stride >= 1LL << 27)
+    return set_error(SG_ERR_UNSUPPORTED, "%s: a token stride of 2^27 or more", nm);
   const long long units = static_cast<long long>(n_seq) * n_kv;
   const long long join = static_cast<long long>(n_seq) * max_window * n_heads;
   const long long rows = static_cast<long long>(max_window) * (n_heads / n_kv);
