@@ -19,9 +19,10 @@
 // has one barrier, and a step's loads are under way during the one before.
 //
 // V at infinity or NaN where some rows see it and others do not: a product
-// with a weight of 0 would spread it.  Weights that are 0 because the key is
-// not seen are written as -0; in a step with such a V these values are added
-// one by one, to the rows that see them, and are 0 in the product.
+// with a weight of 0 would spread it.  In the steps that not every row sees in
+// full such values are 0 in the product; if there were any, they are added at
+// the end to the rows that see them (what they are multiplied by does not
+// matter any more).
 #include <type_traits>
 
 #include "sg_attn.hpp"
@@ -223,6 +224,68 @@ struct SlidePart : Part<D> {
   }
 };
 
+// Eight 16-bit values, or a group's scale, of which infinities and NaN, and
+// all if they are not there, become 0: whether there were any of those.
+__device__ __forceinline__ bool finite8(u32x4& w, bool there) {
+  bool odd = false;
+#pragma unroll
+  for (int c = 0; c < 4; ++c) {
+    const bool lo = fp16_odd(w[c]), hi = fp16_odd(w[c] >> 16);
+    odd |= there && (lo || hi);
+    w[c] &= there ? (lo ? 0u : 0xFFFFu) | (hi ? 0u : 0xFFFF0000u) : 0u;
+  }
+  return odd;
+}
+__device__ __forceinline__ bool finite_scale(uint32_t& scale, bool there) {
+  const bool odd = there && fp16_odd(scale);
+  scale = there && !odd ? scale : 0u;
+  return odd;
+}
+
+// Adds the infinities and NaN that the products were made without: of each key
+// of a step that not all rows see in full, to columns c + 16 d (4) of the rows
+// that see it, at positions pos and with the tree's up.
+template <int D, bool Q8, int RT, int N>
+__device__ __forceinline__ void add_odds(const SlidePart<D>& t, f4 (&acc)[RT][N], int c,
+                                         const int (&pos)[RT], const uint64_t (&up)[RT]) {
+  const slide_p a = cold_slide();
+  for (int s = t.begin; s < t.end; s = t.steps.skip(s + 1)) {
+    const bool window = s >= t.steps.cached;
+    typename SlidePart<D>::Rows rows;
+    rows.ok = 15u;
+    if (!window) rows = t.rows_of(s);
+    if (window ? t.full_window(s) : t.full(s, rows.ok)) continue;
+    const uint64_t there = t.present(s, rows.ok);
+#pragma unroll 1
+    for (int r = 0; r < kKeys; ++r) {
+      if (!(there >> r & 1)) continue;
+      const int b = r >> 4;
+      const long long at =
+          window ? static_cast<long long>(t.win.off + (s - t.steps.cached) * kKeys + r) * a->v_stride +
+                       t.h * D
+                 : (b == 0 ? rows.at[0] : b == 1 ? rows.at[1] : b == 2 ? rows.at[2] : rows.at[3]) +
+                       (r & 15) * D;
+      const uint16_t* const row = (window ? a->v : a->vc) + at;
+      int c0 = c;
+      asm("" : "+v"(c0));  // (the addresses made anew: registers)
+      bool see[RT];
+#pragma unroll
+      for (int rt = 0; rt < RT; ++rt) see[rt] = t.seen4(s, r, there, pos[rt], up[rt]) & 1;
+#pragma unroll
+      for (int d = 0; d < N; ++d)
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+          const int k = c0 + 16 * d + i;
+          // (a group of codes that is not finite is so throughout)
+          const float x =
+              half_bits_to_float(Q8 && !window ? a->vs[(at + k) / kKvGroup] : row[k]);
+#pragma unroll
+          for (int rt = 0; rt < RT; ++rt) acc[rt][d][i] += see[rt] && !isfinite(x) ? x : 0.f;
+        }
+    }
+  }
+}
+
 // The nodes' positions, and whom of their window each sees, by one wave.
 __device__ __forceinline__ void see_tree(const SlideArgs& a, Window w, int len, int lane, int* pos,
                                          uint64_t* seen) {
@@ -415,6 +478,7 @@ __global__ void __launch_bounds__(256, slide_waves(D, RT, Q8)) slide_few_kernel(
   const uint32_t v_in = wave * L::kWave + (4 * grp + (col >> 2)) * L::kRow + (col & 3) * 8;
 
   int it = 0;
+  bool odd = false;
   // A step's scores from K, its weights and V into LDS, the second product.
   // scores(s): the products with K; spread(odd): V into the wave's corner;
   // each issues the next step's loads once it is through with its own.
@@ -426,7 +490,6 @@ __global__ void __launch_bounds__(256, slide_waves(D, RT, Q8)) slide_few_kernel(
     scores(s);
 
     float e[RT][4], top[RT], sum[RT];
-    uint32_t see[RT];
     auto weigh = [&](int rt, float by) {  // row tile rt's p = 2^(e - by), into LDS
       float p[4];
       h4 ph;
@@ -434,11 +497,6 @@ __global__ void __launch_bounds__(256, slide_waves(D, RT, Q8)) slide_few_kernel(
       for (int i = 0; i < 4; ++i) {
         p[i] = __builtin_amdgcn_exp2f(e[rt][i] - by);
         ph[i] = static_cast<_Float16>(p[i]);
-      }
-      if (!full) {
-#pragma unroll
-        for (int i = 0; i < 4; ++i)
-          if (!(see[rt] >> i & 1)) ph[i] = static_cast<_Float16>(-0.f);
       }
       sum[rt] = (p[0] + p[1]) + (p[2] + p[3]);
       *reinterpret_cast<h4*>(lds + p_out + par * L::kStepP + rt * 16 * 128) = ph;
@@ -448,20 +506,19 @@ __global__ void __launch_bounds__(256, slide_waves(D, RT, Q8)) slide_few_kernel(
     for (int rt = 0; rt < RT; ++rt) {
 #pragma unroll
       for (int i = 0; i < 4; ++i) e[rt][i] = __builtin_fmaf(s[rt][i], a.scale_log2, -mref[rt]);
-      see[rt] = 15u;
       if (!full) {
-        see[rt] = t.seen4(step, 16 * wave + 4 * grp, there,
-                          a.parent ? place[node[rt]] : t.len + node[rt],
-                          a.parent ? seen[node[rt]] : 0);
+        const uint32_t see = t.seen4(step, 16 * wave + 4 * grp, there,
+                                     a.parent ? place[node[rt]] : t.len + node[rt],
+                                     a.parent ? seen[node[rt]] : 0);
 #pragma unroll
-        for (int i = 0; i < 4; ++i) e[rt][i] = see[rt] >> i & 1 ? e[rt][i] : -INFINITY;
+        for (int i = 0; i < 4; ++i) e[rt][i] = see >> i & 1 ? e[rt][i] : -INFINITY;
       }
       top[rt] = max3(max3(e[rt][0], e[rt][1], e[rt][2]), e[rt][3], e[rt][3]);
       move |= top[rt] > lim[rt];
       weigh(rt, 0.f);
     }
     if (__any(move)) rise[par] = step + 1;
-    const bool by_one = spread() && !full;
+    odd |= spread();
     bar();  // P is here
 
     if (rise[par] == step + 1) {
@@ -493,37 +550,6 @@ __global__ void __launch_bounds__(256, slide_waves(D, RT, Q8)) slide_few_kernel(
     for (int rt = 0; rt < RT; ++rt) l[rt] += sum[rt];
 
     const unsigned char* const pl = lds + L::kP + par * L::kStepP;
-    if (by_one) {
-#pragma unroll 1
-      for (int r = 0; r < kKeys; ++r) {
-        const int at = (r >> 5) * 4 + ((r & 15) >> 2);
-#pragma unroll 1
-        for (int d = 0; d < DQ; ++d) {
-          h4* const vp = reinterpret_cast<h4*>(vl + r * L::kRow + d * 32 + grp * 8);
-          const u32x2 v = *reinterpret_cast<const u32x2*>(vp);
-          const uint32_t x[4] = {v.x & 0xFFFFu, v.x >> 16, v.y & 0xFFFFu, v.y >> 16};
-#pragma unroll
-          for (int rt = 0; rt < RT; ++rt) {
-            const uint32_t w = *reinterpret_cast<const uint16_t*>(
-                pl + (rt * 16 + col) * 128 + ((at ^ psw) << 4) + (r >> 4 & 1) * 8 + (r & 3) * 2);
-            const float p = half_bits_to_float(w);
-            f4 add;
-#pragma unroll
-            for (int i = 0; i < 4; ++i)
-              add[i] = w != 0x8000u && fp16_odd(x[i]) ? p * half_bits_to_float(x[i]) : 0.f;
-#pragma unroll
-            for (int dd = 0; dd < DQ; ++dd)
-              if (dd == d) acc[rt][dd] += add;
-          }
-          // (for the product: 0 in their place; the wave's own corner, all of it read first)
-          wait_lds();
-          const uint32_t y0 = (fp16_odd(x[0]) ? 0u : x[0]) | (fp16_odd(x[1]) ? 0u : x[1]) << 16;
-          const uint32_t y1 = (fp16_odd(x[2]) ? 0u : x[2]) | (fp16_odd(x[3]) ? 0u : x[3]) << 16;
-          *reinterpret_cast<u32x2*>(vp) = (u32x2){y0, y1};
-        }
-      }
-      wait_lds();
-    }
 #pragma unroll
     for (int st = 0; st < 2; ++st) {
       h8 pf[RT];
@@ -561,14 +587,7 @@ __global__ void __launch_bounds__(256, slide_waves(D, RT, Q8)) slide_few_kernel(
     for (int i = 0; i < KK; ++i) {
       const int r = i * RP + lane / LP;
       u32x4 w = x.v[i];
-      if (!full) {  // rows that are not there as 0
-        const bool some = there >> r & 1;
-#pragma unroll
-        for (int j = 0; j < 4; ++j) {
-          w[j] = some ? w[j] : 0u;
-          odd |= fp16_odd(w[j]) || fp16_odd(w[j] >> 16);
-        }
-      }
+      if (!full) odd |= finite8(w, there >> r & 1);
       *reinterpret_cast<u32x4*>(vl + r * L::kRow + (lane % LP) * 16) = w;
     }
     return __any(odd);
@@ -632,10 +651,7 @@ __global__ void __launch_bounds__(256, slide_waves(D, RT, Q8)) slide_few_kernel(
             for (int i = 0; i < LQ; ++i) {
               const int r = i * RQ + lane / LQ;
               uint32_t scale = st.x.vs[i] >> vhalf;
-              if (!full) {  // rows that are not there as 0
-                scale = there >> r & 1 ? scale : 0u;
-                odd |= fp16_odd(scale);
-              }
+              if (!full) odd |= finite_scale(scale, there >> r & 1);
               const h2 d = scale2(scale);
               uint32_t w[4][2];
 #pragma unroll
@@ -666,6 +682,16 @@ __global__ void __launch_bounds__(256, slide_waves(D, RT, Q8)) slide_few_kernel(
     }
   }
 
+  if (odd) {
+    int pos[RT];
+    uint64_t up[RT];
+#pragma unroll
+    for (int rt = 0; rt < RT; ++rt) {
+      pos[rt] = a.parent ? place[node[rt]] : t.len + node[rt];
+      up[rt] = a.parent ? seen[node[rt]] : 0;
+    }
+    add_odds<D, Q8>(t, acc, wave * (D / 4) + 4 * grp, pos, up);
+  }
   // the rows' sums over the waves, and out
   bar();
 #pragma unroll
@@ -722,7 +748,7 @@ __global__ void __launch_bounds__(64 * kSlideRowWaves) slide_rows_kernel(const S
   if (!t.start(lds)) return;
   const int lane = t.lane, col = t.col, grp = t.grp;
   const int row0 = (t.rb * NW + wave) * 16 * RT;
-  int* odds = reinterpret_cast<int*>(lds + L::kFlags);  // 1 + the last odd (even) step with any
+  int* odds = reinterpret_cast<int*>(lds + L::kFlags);  // whether V had infinities or NaN
   uint64_t* seen = reinterpret_cast<uint64_t*>(lds + L::kSeen);
   int* place = reinterpret_cast<int*>(lds + L::kPos);
   // where the wave's 16 keys go in a buffer of K and V
@@ -766,18 +792,20 @@ __global__ void __launch_bounds__(64 * kSlideRowWaves) slide_rows_kernel(const S
   };
   // codes of cached step s, and their scales, into half `half` of the second buffer
   auto bring_codes = [&](const Rows& rows, int half) {
+    int ln = lane;
+    asm("" : "+v"(ln));
     const long long at =
         blk == 0 ? rows.at[0] : blk == 1 ? rows.at[1] : blk == 2 ? rows.at[2] : rows.at[3];
     const unsigned char* src =
         uniform_ptr(reinterpret_cast<const unsigned char*>(is_v ? a.vc : a.kc) + at);
     const uint32_t to = t.lds0 + (2 + half) * P::kStep + (is_v ? P::kStep / 2 : 0) + blk * 16 * D;
 #pragma unroll
-    for (int i = 0; i < NQ; ++i) dma16_base(to + i * 1024, lane * 16 + i * 1024, src);
-    if (lane < D / 16) {
+    for (int i = 0; i < NQ; ++i) dma16_base(to + i * 1024, ln * 16 + i * 1024, src);
+    if (ln < D / 16) {
       const unsigned char* sc = uniform_ptr(
           reinterpret_cast<const unsigned char*>(is_v ? a.vs : a.ks) + at / (kKvGroup / 2));
       dma16_base(t.lds0 + L::kScales + half * L::kScaleStep + (is_v ? L::kScaleStep / 2 : 0) + blk * D,
-                 lane * 16, sc);
+                 ln * 16, sc);
     }
   };
   // the wave's 16 keys of half `half` into the first buffer, as 16 bits; rows that
@@ -788,18 +816,15 @@ __global__ void __launch_bounds__(64 * kSlideRowWaves) slide_rows_kernel(const S
     const unsigned char* const sc =
         lds + L::kScales + half * L::kScaleStep + (is_v ? L::kScaleStep / 2 : 0) + blk * D;
     bool odd = false;
+    int ln = lane;
+    asm("" : "+v"(ln));
 #pragma unroll
     for (int i = 0; i < NQ; ++i) {
-      const int row = i * RQ + lane / CQ, c = lane % CQ;
-      const u32x4 x = *reinterpret_cast<const u32x4*>(from + i * 1024 + lane * 16);
+      const int row = i * RQ + ln / CQ, c = ln % CQ;
+      const u32x4 x = *reinterpret_cast<const u32x4*>(from + i * 1024 + ln * 16);
       uint32_t scale =
           *reinterpret_cast<const uint16_t*>(sc + row * (D / kKvGroup * 2) + (c / 2) * 2);
-      if (!full && is_v) {
-        scale = there >> row & 1 ? scale : 0u;
-        // (taken out, and added by those that see it)
-        odd |= fp16_odd(scale);
-        scale = fp16_odd(scale) ? 0u : scale;
-      }
+      if (!full && is_v) odd |= finite_scale(scale, there >> row & 1);
       const h2 d = scale2(scale);
       uint32_t w[4][2];
 #pragma unroll
@@ -821,18 +846,12 @@ __global__ void __launch_bounds__(64 * kSlideRowWaves) slide_rows_kernel(const S
     for (int i = 0; i < NI; ++i) {
       u32x4* at = reinterpret_cast<u32x4*>(vb + i * 1024 + 16 * lane);
       u32x4 w = *at;
-      const bool some = there >> (i * RPI + lane / CH) & 1;
-#pragma unroll
-      for (int c = 0; c < 4; ++c) {
-        const bool lo = fp16_odd(w[c]), hi = fp16_odd(w[c] >> 16);
-        odd |= some && (lo || hi);
-        w[c] &= some ? (lo ? 0u : 0xFFFFu) | (hi ? 0u : 0xFFFF0000u) : 0u;
-      }
+      odd |= finite8(w, there >> (i * RPI + lane / CH) & 1);
       *at = w;
     }
     return __any(odd);
   };
-  if (threadIdx.x < 2) odds[threadIdx.x] = 0;
+  if (threadIdx.x == 0) *odds = 0;
   if (wave == NW - 1 && a.parent) see_tree(a, t.win, t.len, lane, place, seen);
 
   h8 qf[RT][KK];
@@ -851,8 +870,9 @@ __global__ void __launch_bounds__(64 * kSlideRowWaves) slide_rows_kernel(const S
   const uint32_t koff = t.k_offset(), voff = t.v_offset();
 
   // A step on the buffer at b.
-  auto compute = [&](int step, uint32_t b, bool full, uint64_t there, bool odd) {
+  auto compute = [&](int step, uint32_t b, bool full, uint64_t there) {
     uint32_t kbase = koff + b, vbase = voff + b;
+    asm("" : "+v"(kbase), "+v"(vbase));
 #pragma unroll 1
     for (int st = 0; st < 2; ++st) {
       f4 s[2][RT];
@@ -934,59 +954,6 @@ __global__ void __launch_bounds__(64 * kSlideRowWaves) slide_rows_kernel(const S
         l[rt] += ((s[0][rt][0] + s[0][rt][1]) + (s[0][rt][2] + s[0][rt][3])) +
                  ((s[1][rt][0] + s[1][rt][1]) + (s[1][rt][2] + s[1][rt][3]));
       }
-      if (odd) {
-#pragma unroll 1
-        for (int r = 0; r < 32; ++r) {  // one by one, to the rows that see them
-          const int key = 32 * st + r;
-          if (!(there >> key & 1)) continue;
-          // V's row as it is in memory
-          const slide_p ca = cold_slide();
-          const bool window = step >= t.steps.cached;
-          long long at;
-          if (window) {
-            at = static_cast<long long>(t.win.off + (step - t.steps.cached) * kKeys + key) *
-                     ca->v_stride + t.h * D;
-          } else {
-            const int j = step * kKeys + key;
-            at = (((static_cast<long long>(t.table[j >> ca->page_log2]) * ca->n_kv + t.h)
-                   << ca->page_log2) +
-                  (j & ((1 << ca->page_log2) - 1))) * D;
-          }
-          const uint16_t* const row = (window ? ca->v : ca->vc) + at;
-          const bool codes = Q8 && !window;
-          const int from = col + 16 * ((r & 15) >> 2);  // the lane that has key r's weight
-          float w[RT];
-#pragma unroll
-          for (int rt = 0; rt < RT; ++rt) {
-            float x = 0.f;
-#pragma unroll
-            for (int i = 0; i < 8; ++i)
-              x = i == (r >> 4) * 4 + (r & 3) ? s[i >> 2][rt][i & 3] : x;
-            w[rt] = __shfl(x, from);
-            const int node = t.node_of(row0 + rt * 16 + col);
-            const bool see = t.seen4(step, key, there,
-                                     ca->parent ? place[node] : t.len + node,
-                                     ca->parent ? seen[node] : 0) & 1;
-            w[rt] = see ? w[rt] : -1.f;  // (weights are not negative)
-          }
-#pragma unroll
-          for (int d = 0; d < DT; ++d) {
-            const int c = d * 16 + 4 * grp;
-            // (a group of codes that is not finite is so throughout)
-            float x[4];
-#pragma unroll
-            for (int i = 0; i < 4; ++i)
-              x[i] = half_bits_to_float(codes ? ca->vs[(at + c) / kKvGroup] : row[c + i]);
-#pragma unroll
-            for (int rt = 0; rt < RT; ++rt) {
-#pragma unroll
-              for (int i = 0; i < 4; ++i)
-                acc[rt][d][i] += w[rt] >= 0.f && !isfinite(x[i]) ? w[rt] * x[i] : 0.f;
-              asm volatile("" : "+v"(acc[rt][d])::"memory");  // (one after the other: registers)
-            }
-          }
-        }
-      }
       h8 vn[kAhead];
 #pragma unroll
       for (int d = 0; d < kAhead; ++d) vn[d] = t.v_frag(P::v_tile(vbase, d), 0);
@@ -1020,14 +987,14 @@ __global__ void __launch_bounds__(64 * kSlideRowWaves) slide_rows_kernel(const S
         wait_vm();
         bar();  // nobody reads the first buffer any more (and the flags are cleared)
         if (turn_codes(it & 1, full, static_cast<uint32_t>(there >> (16 * blk)) & 0xFFFFu))
-          odds[it & 1] = step + 1;
+          *odds = 1;
         wait_lds();
         if (next < cached_end) {
           rows = t.rows_of(next);
           bring_codes(rows, (it + 1) & 1);
         }
         bar();  // everybody's keys are there
-        compute(step, 0, full, there, !full && odds[it & 1] == step + 1);
+        compute(step, 0, full, there);
         step = next;
       }
     }
@@ -1050,14 +1017,26 @@ __global__ void __launch_bounds__(64 * kSlideRowWaves) slide_rows_kernel(const S
       if (!Q8 && next < cached_end) rows = t.rows_of(next);
       wait_vm();
       if (is_v && !full && clean_v(b, static_cast<uint32_t>(there >> (16 * blk)) & 0xFFFFu))
-        odds[it & 1] = step + 1;
+        *odds = 1;
       bar();  // everybody's copies of this step are here, and nobody reads the other buffer
       if (next < t.end) bring(next, rows, b ^ 2 * P::kStep);
-      compute(step, b, full, there, !full && odds[it & 1] == step + 1);
+      compute(step, b, full, there);
       step = next;
     }
   }
 
+  // (the last step's barrier is behind the last flag)
+  if (t.begin < t.end && *odds) {
+    int pos[RT];
+    uint64_t up[RT];
+#pragma unroll
+    for (int rt = 0; rt < RT; ++rt) {
+      const int node = t.node_of(row0 + rt * 16 + col);
+      pos[rt] = a.parent ? place[node] : t.len + node;
+      up[rt] = a.parent ? seen[node] : 0;
+    }
+    add_odds<D, Q8>(t, acc, 4 * grp, pos, up);
+  }
 #pragma unroll
   for (int rt = 0; rt < RT; ++rt) {
     const int r = row0 + rt * 16 + col;
