@@ -322,24 +322,20 @@ struct SlideFewLds {
 };
 
 // Waves of a SIMD, that is, workgroups of a CU.
-constexpr int slide_waves(int dim, int tiles, bool q8) {
-  return dim == 256 || (dim == 128 && tiles == 2 && !q8) ? 2
-         : dim == 128 && (tiles == 2 || !q8)             ? 3
-                                                         : 4;
+constexpr int slide_waves(int dim, int tiles) {
+  return dim == 256 ? (tiles == 2 ? 2 : 3) : dim == 128 ? (tiles == 2 ? 3 : 4) : tiles == 2 ? 4 : 5;
 }
 
 // RT: tiles of 16 rows.  Wave w has keys 16 w.. of a step in the first product,
 // and columns w D/4 .. of all keys in the second.
 template <int D, int RT, bool Q8>
-__global__ void __launch_bounds__(256, slide_waves(D, RT, Q8)) slide_few_kernel(const SlideArgs a) {
+__global__ void __launch_bounds__(256, slide_waves(D, RT)) slide_few_kernel(const SlideArgs a) {
   typedef SlidePart<D> P;
   typedef SlideFewLds<D, RT> L;
   constexpr int KK = D / 32, DQ = D / 64, kRows = L::kRows;
   // A wave's columns of V: LP lanes of 8 values a row, RP rows at once; of
   // codes, 16 a lane.
   constexpr int LP = D / 32, RP = 64 / LP, LQ = D / 64, RQ = 64 / LQ;
-  // steps under way
-  constexpr int kStages = D < 256 ? 2 : 1;
   extern __shared__ __attribute__((aligned(16))) unsigned char lds[];
   const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
   P t(a);
@@ -429,21 +425,6 @@ __global__ void __launch_bounds__(256, slide_waves(D, RT, Q8)) slide_few_kernel(
   // The block's steps of the cache and of the window.
   const int cached_end = min(t.end, t.steps.cached);
   int step = t.begin, wstep = t.steps.skip(max(t.begin, t.steps.cached));
-  // a stage: a step whose loads are under way
-  struct Stage {
-    Cached x;
-    int step;
-    uint32_t ok;
-  } stage[kStages];
-  // (past the last step, a step of the cache that is not used: a load that is
-  // made or not would be waited for as if it were not, with all before it)
-  auto fill = [&](Stage& st, int s) {
-    st.step = s;
-    const Rows rows = t.rows_of(s < cached_end ? s : step);
-    st.ok = rows.ok;
-    load_k(st.x, rows);
-    load_v(st.x, rows);
-  };
   Raw own;
   if (wstep < t.end) load_window(own, wstep);
   if (threadIdx.x < 2) rise[threadIdx.x] = 0;
@@ -605,80 +586,73 @@ __global__ void __launch_bounds__(256, slide_waves(D, RT, Q8)) slide_few_kernel(
   // (no load of the window is under way any more: else the loop would wait for all of its own)
   settle(own.k);
   settle(own.v);
-  // (only now: the window's K and V have had these registers)
-  fill(stage[0], step);
-  int ahead = t.steps.skip(step + 1);  // the next step to be loaded
-  if constexpr (kStages == 2) {
-    fill(stage[1], ahead);
-    ahead = t.steps.skip(ahead + 1);
-  }
-  auto turn = [&](Stage& st) {
-    const int step = st.step;
-    const bool full = t.full(step, st.ok);
-    const uint64_t there = full ? ~0ull : t.present(step, st.ok);
-    const Rows rows = t.rows_of(ahead < cached_end ? ahead : step);
-    run(
-        step, full, there,
-        [&](f4 (&s)[RT]) {
-          settle(st.x.k);
-          if constexpr (Q8) {
-            settle(st.x.ks);
+  if (step < cached_end) {
+    // A step's loads are under way during the step before, and only one step's:
+    // more workgroups on a CU bring more than a second step's registers (32
+    // sequences of one token over 4,000 quantised ones, 8 kv heads of 128: 62 us,
+    // 71 with two).  (The window's K and V have had these registers before.)
+    Cached now;
+    Rows rows = t.rows_of(step);
+    load_k(now, rows);
+    load_v(now, rows);
+    while (step < cached_end) {
+      const bool full = t.full(step, rows.ok);
+      const uint64_t there = full ? ~0ull : t.present(step, rows.ok);
+      // (after the last step that one once more: a load that is made or not would
+      // be waited for as if it were not, with all before it)
+      const int next = t.steps.skip(step + 1);
+      rows = t.rows_of(next < cached_end ? next : step);
+      run(
+          step, full, there,
+          [&](f4 (&s)[RT]) {
+            settle(now.k);
+            if constexpr (Q8) {
+              settle(now.ks);
 #pragma unroll
-            for (int i = 0; i < KK / 2; ++i) {
-              const h2 d = scale2(st.x.ks[i] >> (grp & 2) * 8);
+              for (int i = 0; i < KK / 2; ++i) {
+                const h2 d = scale2(now.ks[i] >> (grp & 2) * 8);
 #pragma unroll
-              for (int j = 0; j < 2; ++j) {
-                uint32_t w[2][2];
-                decode4(st.x.k[i][2 * j], d, w[0]);
-                decode4(st.x.k[i][2 * j + 1], d, w[1]);
-                const h8 kf = __builtin_bit_cast(h8, (u32x4){w[0][0], w[0][1], w[1][0], w[1][1]});
+                for (int j = 0; j < 2; ++j) {
+                  uint32_t w[2][2];
+                  decode4(now.k[i][2 * j], d, w[0]);
+                  decode4(now.k[i][2 * j + 1], d, w[1]);
+                  const h8 kf = __builtin_bit_cast(h8, (u32x4){w[0][0], w[0][1], w[1][0], w[1][1]});
 #pragma unroll
-                for (int rt = 0; rt < RT; ++rt)
-                  s[rt] = __builtin_amdgcn_mfma_f32_16x16x32_f16(kf, qf[rt][2 * i + j], s[rt], 0, 0, 0);
+                  for (int rt = 0; rt < RT; ++rt)
+                    s[rt] = __builtin_amdgcn_mfma_f32_16x16x32_f16(kf, qf[rt][2 * i + j], s[rt], 0, 0, 0);
+                }
               }
+            } else {
+              raw_scores(now, s);
             }
-          } else {
-            raw_scores(st.x, s);
-          }
-          load_k(st.x, rows);
-        },
-        [&] {
-          bool odd = false;
-          settle(st.x.v);
-          if constexpr (Q8) {
-            settle(st.x.vs);
+            load_k(now, rows);
+          },
+          [&] {
+            bool odd = false;
+            settle(now.v);
+            if constexpr (Q8) {
+              settle(now.vs);
 #pragma unroll
-            for (int i = 0; i < LQ; ++i) {
-              const int r = i * RQ + lane / LQ;
-              uint32_t scale = st.x.vs[i] >> vhalf;
-              if (!full) odd |= finite_scale(scale, there >> r & 1);
-              const h2 d = scale2(scale);
-              uint32_t w[4][2];
+              for (int i = 0; i < LQ; ++i) {
+                const int r = i * RQ + lane / LQ;
+                uint32_t scale = now.vs[i] >> vhalf;
+                if (!full) odd |= finite_scale(scale, there >> r & 1);
+                const h2 d = scale2(scale);
+                uint32_t w[4][2];
 #pragma unroll
-              for (int j = 0; j < 4; ++j) decode4(st.x.v[i][j], d, w[j]);
-              u32x4* to = reinterpret_cast<u32x4*>(vl + r * L::kRow + (lane % LQ) * 32);
-              to[0] = (u32x4){w[0][0], w[0][1], w[1][0], w[1][1]};
-              to[1] = (u32x4){w[2][0], w[2][1], w[3][0], w[3][1]};
+                for (int j = 0; j < 4; ++j) decode4(now.v[i][j], d, w[j]);
+                u32x4* to = reinterpret_cast<u32x4*>(vl + r * L::kRow + (lane % LQ) * 32);
+                to[0] = (u32x4){w[0][0], w[0][1], w[1][0], w[1][1]};
+                to[1] = (u32x4){w[2][0], w[2][1], w[3][0], w[3][1]};
+              }
+              odd = __any(odd);
+            } else {
+              odd = raw_spread(now, full, there);
             }
-            odd = __any(odd);
-          } else {
-            odd = raw_spread(st.x, full, there);
-          }
-          load_v(st.x, rows);
-          return odd;
-        });
-    st.step = ahead;
-    st.ok = rows.ok;
-    ahead = t.steps.skip(ahead + 1);
-  };
-  if (stage[0].step < cached_end) {
-    while (true) {
-      turn(stage[0]);
-      if (!(stage[kStages - 1].step < cached_end)) break;
-      if constexpr (kStages == 2) {
-        turn(stage[1]);
-        if (!(stage[0].step < cached_end)) break;
-      }
+            load_v(now, rows);
+            return odd;
+          });
+      step = next;
     }
   }
 
