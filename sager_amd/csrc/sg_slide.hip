@@ -1044,8 +1044,11 @@ static SlideLayout slide_layout(int n_seq, int max_window, int max_len, int grou
   const long long keys = static_cast<long long>(max_len) + max_window;
   const long long near = static_cast<long long>(reach) + max_window + sinks + 2 * kKeys;
   const long long most = ((keys < near ? keys : near) + kKeys - 1) / kKeys + 1;
-  // workgroups that the card holds at once, and units of them
-  const int each = l.block_rows == 256 ? 1 : dim == 256 ? 2 : 4;
+  // workgroups that the card holds at once, and units of them (32 sequences of
+  // one token and of five over 4,000 quantised ones, 8 kv heads of 128: 59.8 and
+  // 69.4 us by 3 a CU, 62.0 and 80.0 by 4, 58.6 and 72.6 by 2; of 64: 53.6 us by
+  // 4, 67.5 by 2; four tokens over 131,071, 2 kv heads of 256: 43.8 by 2, 58.3 by 4)
+  const int each = l.block_rows == 256 ? 1 : dim == 256 ? 2 : dim == 128 ? 3 : 4;
   const long long slots = 256 * each;
   const long long per = 32 * each >= l.row_blocks ? 32 * each / l.row_blocks * 8 : 8;
   const bool rounds = units >= 2 * slots;
