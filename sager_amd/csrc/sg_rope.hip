@@ -16,8 +16,8 @@
 // is rounded once.
 //
 // A workgroup a token: its first threads make the token's sines and cosines,
-// once for all heads, while the heads' values are already on their way into
-// registers (eight consecutive ones a lane).  The half layout's partners come
+// once for all heads, while the first heads' values are already on their way
+// into registers (eight consecutive ones a lane).  The half layout's partners come
 // through LDS, within the wave.
 #include <algorithm>
 #include <cmath>
@@ -27,8 +27,9 @@
 namespace sg {
 
 constexpr int kRopeDim = 512;      // largest head
-constexpr int kRopeThreads = 256;
-constexpr int kRopeBatch = 3;      // rows of values a thread has under way
+// (4,096 tokens of 40 heads of 128: 22.3 us with 128 threads, 23.1 with 256,
+// 28.8 with 512; with three rows of values a thread 25.5)
+constexpr int kRopeThreads = 128;
 
 struct RopeArgs {
   const void *q, *k;
@@ -115,22 +116,18 @@ __global__ void __launch_bounds__(kRopeThreads) rope_kernel(const RopeArgs a) {
     *out = static_cast<T*>(is_q ? a.q_out : a.k_out) + t * (is_q ? a.qo_stride : a.ko_stride) +
            h * a.dim + e;
   };
-  float v[kRopeBatch][8];
-  auto load = [&](int r0) {
+  float v[8];
+  auto load = [&](int r) {
 #pragma unroll
-    for (int b = 0; b < kRopeBatch; ++b) {
-      const int r = r0 + b * per + (tid >> a.lanes_log2);
-#pragma unroll
-      for (int i = 0; i < 8; ++i) v[b][i] = 0.f;
-      if (r < a.n_rows && e < a.dim) {
-        const T* in;
-        T* out;
-        at(r, &in, &out);
-        rope_load(in, v[b]);
-      }
+    for (int i = 0; i < 8; ++i) v[i] = 0.f;
+    if (r < a.n_rows && e < a.dim) {
+      const T* in;
+      T* out;
+      at(r, &in, &out);
+      rope_load(in, v);
     }
   };
-  load(0);
+  load(tid >> a.lanes_log2);
   if (wave == 0) {
     int pos = 0;
     const bool ok = position_of(a, t, lane, &pos);
@@ -147,81 +144,78 @@ __global__ void __launch_bounds__(kRopeThreads) rope_kernel(const RopeArgs a) {
   __syncthreads();
   if (!there) return;
 
-  for (int r0 = 0; r0 < a.n_rows; r0 += kRopeBatch * per) {
-    if (r0 > 0) load(r0);
+  for (int r0 = 0; r0 < a.n_rows; r0 += per) {
+    const int r = r0 + (tid >> a.lanes_log2);
+    if (r0 > 0) load(r);
+    const bool some = r < a.n_rows && e < a.dim;
+    const float* const w = r < a.n_heads ? a.q_norm : a.k_norm;
+    if (a.q_norm || a.k_norm) {  // (the sum over a row's lanes: all of them take part)
+      float ss = 0.f;
 #pragma unroll
-    for (int b = 0; b < kRopeBatch; ++b) {
-      const int r = r0 + b * per + (tid >> a.lanes_log2);
-      const bool some = r < a.n_rows && e < a.dim;
-      const float* const w = r < a.n_heads ? a.q_norm : a.k_norm;
-      if (a.q_norm || a.k_norm) {  // (the sum over a row's lanes: all of them take part)
-        float ss = 0.f;
+      for (int i = 0; i < 8; ++i) ss = __builtin_fmaf(v[i], v[i], ss);
+      for (int m = 1; m < lanes; m <<= 1) ss += __shfl_xor(ss, m);
+      if (some && w) {
+        const float s = 1.f / sqrtf(ss / static_cast<float>(a.dim) + a.eps);
+        float wv[8];
+        rope_load(w + e, wv);
 #pragma unroll
-        for (int i = 0; i < 8; ++i) ss = __builtin_fmaf(v[b][i], v[b][i], ss);
-        for (int m = 1; m < lanes; m <<= 1) ss += __shfl_xor(ss, m);
-        if (some && w) {
-          const float s = 1.f / sqrtf(ss / static_cast<float>(a.dim) + a.eps);
-          float wv[8];
-          rope_load(w + e, wv);
-#pragma unroll
-          for (int i = 0; i < 8; ++i) v[b][i] = (v[b][i] * s) * wv[i];
-        }
+        for (int i = 0; i < 8; ++i) v[i] = (v[i] * s) * wv[i];
       }
-      float y[8];
-      if (a.pairs) {
+    }
+    float y[8];
+    if (a.pairs) {
 #pragma unroll
-        for (int i = 0; i < 4; ++i) {
-          const int p = min(e / 2 + i, kRopeDim / 2 - 1);
-          const float c = cs[0][p], s = cs[1][p], x0 = v[b][2 * i], x1 = v[b][2 * i + 1];
-          const bool in = e + 2 * i < rot;
-          y[2 * i] = in ? x0 * c - x1 * s : x0;
-          y[2 * i + 1] = in ? x1 * c + x0 * s : x1;
-        }
-      } else {
-        // the partners by way of LDS; a wave's own rows, so no barrier
-        *reinterpret_cast<lds_f4*>(mine + e) = (lds_f4){v[b][0], v[b][1], v[b][2], v[b][3]};
-        *reinterpret_cast<lds_f4*>(mine + e + 4) = (lds_f4){v[b][4], v[b][5], v[b][6], v[b][7]};
-        wait_lds();
+      for (int i = 0; i < 4; ++i) {
+        const int p = min(e / 2 + i, kRopeDim / 2 - 1);
+        const float c = cs[0][p], s = cs[1][p], x0 = v[2 * i], x1 = v[2 * i + 1];
+        const bool in = e + 2 * i < rot;
+        y[2 * i] = in ? x0 * c - x1 * s : x0;
+        y[2 * i + 1] = in ? x1 * c + x0 * s : x1;
+      }
+    } else {
+      // the partners by way of LDS; a wave's own rows, so no barrier
+      *reinterpret_cast<lds_f4*>(mine + e) = (lds_f4){v[0], v[1], v[2], v[3]};
+      *reinterpret_cast<lds_f4*>(mine + e + 4) = (lds_f4){v[4], v[5], v[6], v[7]};
+      wait_lds();
 #pragma unroll
-        for (int j = 0; j < 8; j += 4) {
-          // four values in one half of the pairs, their partners in line: 16-B reads
-          const int x = e + j, to = x < a.half ? x + a.half : x - a.half;
-          if (a.half % 4 == 0) {
-            if (x < rot) {
-              const int p = x < a.half ? x : x - a.half;
-              const lds_f4 o = *reinterpret_cast<const lds_f4*>(mine + to);
-              const lds_f4 c = *reinterpret_cast<const lds_f4*>(cs[0] + p);
-              const lds_f4 s = *reinterpret_cast<const lds_f4*>(cs[1] + p);
+      for (int j = 0; j < 8; j += 4) {
+        // four values in one half of the pairs, their partners in line: 16-B reads
+        const int x = e + j, to = x < a.half ? x + a.half : x - a.half;
+        if (a.half % 4 == 0) {
+          if (x < rot) {
+            const int p = x < a.half ? x : x - a.half;
+            const lds_f4 o = *reinterpret_cast<const lds_f4*>(mine + to);
+            const lds_f4 c = *reinterpret_cast<const lds_f4*>(cs[0] + p);
+            const lds_f4 s = *reinterpret_cast<const lds_f4*>(cs[1] + p);
 #pragma unroll
-              for (int i = 0; i < 4; ++i)
-                y[j + i] = x < a.half ? v[b][j + i] * c[i] - o[i] * s[i]
-                                      : v[b][j + i] * c[i] + o[i] * s[i];
-            } else {
-#pragma unroll
-              for (int i = 0; i < 4; ++i) y[j + i] = v[b][j + i];
-            }
+            for (int i = 0; i < 4; ++i)
+              y[j + i] = x < a.half ? v[j + i] * c[i] - o[i] * s[i]
+                                    : v[j + i] * c[i] + o[i] * s[i];
           } else {
 #pragma unroll
-            for (int i = 0; i < 4; ++i) {
-              const int xi = x + i;
-              const bool low = xi < a.half;
-              y[j + i] = v[b][j + i];
-              if (xi < rot) {
-                const int p = low ? xi : xi - a.half;
-                const float o = mine[low ? xi + a.half : p], c = cs[0][p], s = cs[1][p];
-                y[j + i] = low ? y[j + i] * c - o * s : y[j + i] * c + o * s;
-              }
+            for (int i = 0; i < 4; ++i) y[j + i] = v[j + i];
+          }
+        } else {
+#pragma unroll
+          for (int i = 0; i < 4; ++i) {
+            const int xi = x + i;
+            const bool low = xi < a.half;
+            y[j + i] = v[j + i];
+            if (xi < rot) {
+              const int p = low ? xi : xi - a.half;
+              const float o = mine[low ? xi + a.half : p], c = cs[0][p], s = cs[1][p];
+              y[j + i] = low ? y[j + i] * c - o * s : y[j + i] * c + o * s;
             }
           }
         }
-        wait_lds();  // (read before the next row is written)
       }
-      if (some) {
-        const T* in;
-        T* out;
-        at(r, &in, &out);
-        rope_store(out, y);
-      }
+      wait_lds();  // (read before the next row is written)
+    }
+    if (some) {
+      const T* in;
+      T* out;
+      at(r, &in, &out);
+      rope_store(out, y);
     }
   }
 }
