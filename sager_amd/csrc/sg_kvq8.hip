@@ -20,8 +20,8 @@
 namespace sg {
 
 typedef unsigned short us2 __attribute__((ext_vector_type(2)));
-constexpr int kStoreLayers = 4;  // of a thread, loads under way together
-constexpr int kReadLayers = 4;
+constexpr int kStoreLayers = 2;  // of a thread, loads under way together
+constexpr int kReadLayers = 2;
 
 struct StoreQ8Args {
   const uint16_t *k, *v;
@@ -118,22 +118,22 @@ struct ReadQ8Args {
   int n_seq, n_rows, n_layers, n_kv, dim, n_pages, page_log2, pages_per_seq;
 };
 
-// Grid: (16-value pieces of all rows, K or V, kReadLayers layers).
+// Grid: (waves of all rows, K or V, kReadLayers layers).  A wave has one head's
+// pieces of as many tokens as it has lanes for, whose codes lie in line.
 __global__ void __launch_bounds__(256) kv_read_q8_kernel(const ReadQ8Args a) {
-  const int lanes = a.dim / 16, per = lanes * a.n_kv, l0 = blockIdx.z * kReadLayers;
+  const int lane = threadIdx.x & 63, lanes = a.dim / 16, rows = 64 / lanes;
+  const int wave = __builtin_amdgcn_readfirstlane(blockIdx.x * 4 + (threadIdx.x >> 6));
+  const int block = wave / a.n_kv, h = wave - block * a.n_kv, l0 = blockIdx.z * kReadLayers;
   const bool is_v = blockIdx.y != 0;
-  const long long x = blockIdx.x * 256LL + threadIdx.x;
-  const int lane = threadIdx.x & 63;
   // (one sequence for the wave's first row, then on to the lane's own)
-  const int r0 = static_cast<int>((x - lane) / per);
-  int s = seq_of_row(a.rows, a.n_seq, min(r0, a.n_rows - 1), lane);
-  const int r = r0 + (static_cast<int>((x - lane) - static_cast<long long>(r0) * per) + lane) / per;
+  const long long r0 = static_cast<long long>(block) * rows;
+  if (r0 >= a.n_rows) return;
+  int s = seq_of_row(a.rows, a.n_seq, static_cast<int>(r0), lane);
+  const int r = static_cast<int>(r0) + lane / lanes, c = lane % lanes;
   if (r >= a.n_rows) return;
   while (s + 1 < a.n_seq && a.rows[s + 1] <= r) ++s;
   const int begin = a.rows[s];
   if (r < begin || begin < 0 || r >= a.rows[s + 1]) return;
-  const int in = static_cast<int>(x - static_cast<long long>(r) * per);
-  const int h = in / lanes, c = in - h * lanes;
   const long long pos = static_cast<long long>(a.first[s]) + (r - begin);
   int page = -1;
   if (pos >= 0 && pos >> a.page_log2 < a.pages_per_seq)
@@ -275,10 +275,11 @@ int sg_kv_read_q8(const sg_kv_cache_q8* cache, const int* first, const int* row_
     return set_error(SG_ERR_GEOMETRY, "%s: a layer stride is less than a layer's rows", nm);
   if (reinterpret_cast<uintptr_t>(k) % 2 || reinterpret_cast<uintptr_t>(v) % 2)
     return set_error(SG_ERR_INVALID_ARGUMENT, "%s: k and v must be 2-B aligned", nm);
-  const long long pieces = n_rows * (row / 16);
+  const int rows = 64 / (cache->head_dim / 16);  // of a wave
+  const long long waves = (n_rows + rows - 1LL) / rows * cache->n_kv_heads;
   const int groups = (cache->n_layers + kReadLayers - 1) / kReadLayers;
   // (a launch has less than 2^32 threads in a row)
-  if (cache->n_layers > 65535 || pieces > 0xFFFFFFFFLL - 512)
+  if (cache->n_layers > 65535 || waves > 0xFFFFFFFFLL / 64 - 4)
     return set_error(SG_ERR_UNSUPPORTED, "%s: n_rows=%d n_layers=%d n_kv_heads=%d", nm, n_rows,
                      cache->n_layers, cache->n_kv_heads);
   const long long nk = (cache->n_layers - 1) * k_layer_stride + span_k;
@@ -319,7 +320,7 @@ int sg_kv_read_q8(const sg_kv_cache_q8* cache, const int* first, const int* row_
   a.page_log2 = log2_of(cache->page_size);
   a.pages_per_seq = cache->pages_per_seq;
   hipLaunchKernelGGL(kv_read_q8_kernel,
-                     dim3(static_cast<unsigned>((pieces + 255) / 256), 2, groups), dim3(256), 0,
+                     dim3(static_cast<unsigned>((waves + 3) / 4), 2, groups), dim3(256), 0,
                      static_cast<hipStream_t>(stream), a);
   return check_launch(nm);
 }
