@@ -26,6 +26,20 @@ __device__ __forceinline__ void decode4(uint32_t codes, h2 d, uint32_t (&out)[2]
   out[0] = __builtin_bit_cast(uint32_t, (a - bias) * d);
   out[1] = __builtin_bit_cast(uint32_t, (b - bias) * d);
 }
+// The same in two parts, value rounded and what the rounding took: their sum is
+// code * d without an error (18 bits at the most, and a multiple of 2^-24).
+__device__ __forceinline__ void decode4(uint32_t codes, h2 d, uint32_t (&out)[2],
+                                        uint32_t (&rest)[2]) {
+  const uint32_t u = codes ^ 0x80808080u;
+  const h2 bias = {static_cast<_Float16>(1152.f), static_cast<_Float16>(1152.f)};
+  const h2 a = __builtin_bit_cast(h2, __builtin_amdgcn_perm(0x64646464u, u, 0x04010400u)) - bias;
+  const h2 b = __builtin_bit_cast(h2, __builtin_amdgcn_perm(0x64646464u, u, 0x04030402u)) - bias;
+  const h2 x = a * d, y = b * d;
+  out[0] = __builtin_bit_cast(uint32_t, x);
+  out[1] = __builtin_bit_cast(uint32_t, y);
+  rest[0] = __builtin_bit_cast(uint32_t, __builtin_elementwise_fma(a, d, -x));
+  rest[1] = __builtin_bit_cast(uint32_t, __builtin_elementwise_fma(b, d, -y));
+}
 __device__ __forceinline__ h2 scale2(uint32_t bits) {  // one scale in both halves
   return __builtin_bit_cast(h2, (bits & 0xFFFFu) * 0x10001u);
 }

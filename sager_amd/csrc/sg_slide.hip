@@ -13,10 +13,14 @@
 // first product and the columns of the second, as there, but K and V come
 // through registers: a wave's keys are nobody else's, so K needs no LDS at
 // all, and V's columns go through a corner of LDS that is the wave's own,
-// where ds_read_b64_tr_b16 turns them.  Codes become 16-bit numbers on that
-// way (their product with the scale is rounded once, 2^-12 of the value at the
-// most, as a 16-bit cache's own values are).  Only P is exchanged, so a step
-// has one barrier, and a step's loads are under way during the one before.
+// where ds_read_b64_tr_b16 turns them.  Only P is exchanged, so a step has one
+// barrier, and a step's loads are under way during the one before.
+//
+// A code times its scale has up to 18 bits, and rounding it to a factor of the
+// products costs more than all else: keys of 2^-12 of their size off move
+// scores, and so weights, by several times the output's own rounding.  So a
+// quantised value is two 16-bit numbers, rounded and rest, and each product is
+// made with both; the matrix cores have the time.
 //
 // V at infinity or NaN where some rows see it and others do not: a product
 // with a weight of 0 would spread it.  In the steps that not every row sees in
@@ -305,12 +309,17 @@ __device__ __forceinline__ void see_tree(const SlideArgs& a, Window w, int len, 
 
 // LDS: V of the four waves, P of two steps, the rows' maxima and sums of the
 // four waves, the nodes' positions and what they see, the flags.
-template <int D, int RT>
+template <int D, int RT, bool Q8>
 struct SlideFewLds {
   static constexpr uint32_t kRows = 16 * RT;
-  // A wave's row of V, an odd multiple of 32 B: what a quarter or half of a
-  // wave reads transposed (4 or 8 rows' 32 B) then lies in different banks.
-  static constexpr uint32_t kRow = D == 64 ? 32 : D / 2 + 32;
+  // A wave's row of V: slots of 16 columns, of a quantised cache rounded values
+  // and rests in turn.  Row r has slot i at i ^ swz(r), so that the 32 B of four
+  // or eight rows that are read transposed together lie in different banks.
+  static constexpr uint32_t kSlots = D / 64 * (Q8 ? 2 : 1);
+  static constexpr uint32_t kRow = kSlots * 32;
+  static __device__ __forceinline__ uint32_t swz(uint32_t r) {
+    return r / (8 / kSlots) & (kSlots - 1);
+  }
   static constexpr uint32_t kWave = kKeys * kRow;
   static constexpr uint32_t kP = 4 * kWave;
   static constexpr uint32_t kStepP = kRows * kKeys * 2;
@@ -323,7 +332,7 @@ struct SlideFewLds {
 
 // Waves of a SIMD, that is, workgroups of a CU.
 constexpr int slide_waves(int dim, int tiles) {
-  return dim == 256 ? (tiles == 2 ? 2 : 3) : dim == 128 ? (tiles == 2 ? 3 : 4) : tiles == 2 ? 4 : 5;
+  return dim == 256 ? 2 : dim == 128 ? (tiles == 2 ? 3 : 4) : tiles == 2 ? 4 : 5;
 }
 
 // RT: tiles of 16 rows.  Wave w has keys 16 w.. of a step in the first product,
@@ -331,7 +340,7 @@ constexpr int slide_waves(int dim, int tiles) {
 template <int D, int RT, bool Q8>
 __global__ void __launch_bounds__(256, slide_waves(D, RT)) slide_few_kernel(const SlideArgs a) {
   typedef SlidePart<D> P;
-  typedef SlideFewLds<D, RT> L;
+  typedef SlideFewLds<D, RT, Q8> L;
   constexpr int KK = D / 32, DQ = D / 64, kRows = L::kRows;
   // A wave's columns of V: LP lanes of 8 values a row, RP rows at once; of
   // codes, 16 a lane.
@@ -455,15 +464,18 @@ __global__ void __launch_bounds__(256, slide_waves(D, RT)) slide_few_kernel(cons
   const int psw = (col >> 1) & 7;
   const uint32_t p_out =
       L::kP + col * 128 + ((((wave >> 1) * 4 + grp) ^ psw) << 4) + (wave & 1) * 8;
-  // V's columns 0..15 of row 4 grp + col / 4 of a 16-key block
-  const uint32_t v_in = wave * L::kWave + (4 * grp + (col >> 2)) * L::kRow + (col & 3) * 8;
+  // V's columns 0..15 of row 4 grp + col / 4 of a 16-key block; slot i is at v_in ^ 32 i
+  const uint32_t v_row = 4 * grp + (col >> 2);
+  const uint32_t v_in = wave * L::kWave + v_row * L::kRow + L::swz(v_row) * 32 + (col & 3) * 8;
 
   int it = 0;
   bool odd = false;
   // A step's scores from K, its weights and V into LDS, the second product.
   // scores(s): the products with K; spread(odd): V into the wave's corner;
   // each issues the next step's loads once it is through with its own.
-  auto run = [&](int step, bool full, uint64_t there, auto&& scores, auto&& spread) {
+  auto run = [&](int step, bool full, uint64_t there, auto n_parts, auto&& scores,
+                 auto&& spread) {
+    constexpr int parts = decltype(n_parts)::value;  // of V's values
     const int par = it++ & 1;
     f4 s[RT];
 #pragma unroll
@@ -539,18 +551,21 @@ __global__ void __launch_bounds__(256, slide_waves(D, RT)) slide_few_kernel(cons
         pf[rt] = *reinterpret_cast<const h8*>(pl + (rt * 16 + col) * 128 +
                                               (((st * 4 + grp) ^ psw) << 4));
 #pragma unroll
-      for (int d = 0; d < DQ; ++d) {
-        s4 x[2];
+      for (int d = 0; d < DQ; ++d)
 #pragma unroll
-        for (int b = 0; b < 2; ++b)
-          x[b] = __builtin_amdgcn_ds_read_tr16_b64_v4i16(
-              (lds_s4_p)((lds_char_p)lds + v_in + (st * 2 + b) * 16 * L::kRow + d * 32));
-        const h8 vf =
-            __builtin_bit_cast(h8, __builtin_shufflevector(x[0], x[1], 0, 1, 2, 3, 4, 5, 6, 7));
+        for (int part = 0; part < (parts == 2 ? 2 : 1); ++part) {
+          const uint32_t at = v_in ^ 32 * (Q8 ? 2 * d + part : d);
+          s4 x[2];
 #pragma unroll
-        for (int rt = 0; rt < RT; ++rt)
-          acc[rt][d] = __builtin_amdgcn_mfma_f32_16x16x32_f16(vf, pf[rt], acc[rt][d], 0, 0, 0);
-      }
+          for (int b = 0; b < 2; ++b)
+            x[b] = __builtin_amdgcn_ds_read_tr16_b64_v4i16(
+                (lds_s4_p)((lds_char_p)lds + at + (st * 2 + b) * 16 * L::kRow));
+          const h8 vf = __builtin_bit_cast(
+              h8, __builtin_shufflevector(x[0], x[1], 0, 1, 2, 3, 4, 5, 6, 7));
+#pragma unroll
+          for (int rt = 0; rt < RT; ++rt)
+            acc[rt][d] = __builtin_amdgcn_mfma_f32_16x16x32_f16(vf, pf[rt], acc[rt][d], 0, 0, 0);
+        }
     }
   };
   // 16-bit K and V of a step as they were loaded
@@ -569,7 +584,8 @@ __global__ void __launch_bounds__(256, slide_waves(D, RT)) slide_few_kernel(cons
       const int r = i * RP + lane / LP;
       u32x4 w = x.v[i];
       if (!full) odd |= finite8(w, there >> r & 1);
-      *reinterpret_cast<u32x4*>(vl + r * L::kRow + (lane % LP) * 16) = w;
+      const uint32_t p = lane % LP, slot = (Q8 ? 2 : 1) * (p >> 1);
+      *reinterpret_cast<u32x4*>(vl + r * L::kRow + (slot ^ L::swz(r)) * 32 + (p & 1) * 16) = w;
     }
     return __any(odd);
   };
@@ -578,7 +594,9 @@ __global__ void __launch_bounds__(256, slide_waves(D, RT)) slide_few_kernel(cons
   while (wstep < t.end) {  // (one step, but for chains of more than 64 tokens)
     const bool full = t.full_window(wstep);
     const uint64_t there = full ? ~0ull : t.present(wstep, 15u);
-    run(wstep, full, there, [&](f4 (&s)[RT]) { raw_scores(own, s); },
+    run(
+        wstep, full, there, std::integral_constant<int, 1>(),
+        [&](f4 (&s)[RT]) { raw_scores(own, s); },
         [&] { return raw_spread(own, full, there); });
     wstep = t.steps.skip(wstep + 1);
     if (wstep < t.end) load_window(own, wstep);
@@ -603,7 +621,7 @@ __global__ void __launch_bounds__(256, slide_waves(D, RT)) slide_few_kernel(cons
       const int next = t.steps.skip(step + 1);
       rows = t.rows_of(next < cached_end ? next : step);
       run(
-          step, full, there,
+          step, full, there, std::integral_constant<int, Q8 ? 2 : 1>(),
           [&](f4 (&s)[RT]) {
             settle(now.k);
             if constexpr (Q8) {
@@ -613,13 +631,16 @@ __global__ void __launch_bounds__(256, slide_waves(D, RT)) slide_few_kernel(cons
                 const h2 d = scale2(now.ks[i] >> (grp & 2) * 8);
 #pragma unroll
                 for (int j = 0; j < 2; ++j) {
-                  uint32_t w[2][2];
-                  decode4(now.k[i][2 * j], d, w[0]);
-                  decode4(now.k[i][2 * j + 1], d, w[1]);
+                  uint32_t w[2][2], x[2][2];
+                  decode4(now.k[i][2 * j], d, w[0], x[0]);
+                  decode4(now.k[i][2 * j + 1], d, w[1], x[1]);
                   const h8 kf = __builtin_bit_cast(h8, (u32x4){w[0][0], w[0][1], w[1][0], w[1][1]});
+                  const h8 kx = __builtin_bit_cast(h8, (u32x4){x[0][0], x[0][1], x[1][0], x[1][1]});
 #pragma unroll
-                  for (int rt = 0; rt < RT; ++rt)
+                  for (int rt = 0; rt < RT; ++rt) {
                     s[rt] = __builtin_amdgcn_mfma_f32_16x16x32_f16(kf, qf[rt][2 * i + j], s[rt], 0, 0, 0);
+                    s[rt] = __builtin_amdgcn_mfma_f32_16x16x32_f16(kx, qf[rt][2 * i + j], s[rt], 0, 0, 0);
+                  }
                 }
               }
             } else {
@@ -638,12 +659,17 @@ __global__ void __launch_bounds__(256, slide_waves(D, RT)) slide_few_kernel(cons
                 uint32_t scale = now.vs[i] >> vhalf;
                 if (!full) odd |= finite_scale(scale, there >> r & 1);
                 const h2 d = scale2(scale);
-                uint32_t w[4][2];
+                uint32_t w[4][2], x[4][2];
 #pragma unroll
-                for (int j = 0; j < 4; ++j) decode4(now.v[i][j], d, w[j]);
-                u32x4* to = reinterpret_cast<u32x4*>(vl + r * L::kRow + (lane % LQ) * 32);
+                for (int j = 0; j < 4; ++j) decode4(now.v[i][j], d, w[j], x[j]);
+                unsigned char* const row = vl + r * L::kRow;
+                const uint32_t slot = 2 * (lane % LQ) ^ L::swz(r);
+                u32x4* to = reinterpret_cast<u32x4*>(row + slot * 32);
                 to[0] = (u32x4){w[0][0], w[0][1], w[1][0], w[1][1]};
                 to[1] = (u32x4){w[2][0], w[2][1], w[3][0], w[3][1]};
+                to = reinterpret_cast<u32x4*>(row + (slot ^ 1) * 32);
+                to[0] = (u32x4){x[0][0], x[0][1], x[1][0], x[1][1]};
+                to[1] = (u32x4){x[2][0], x[2][1], x[3][0], x[3][1]};
               }
               odd = __any(odd);
             } else {
@@ -699,13 +725,12 @@ struct SlideRowsLds {
   static constexpr uint32_t kBytes = kFlags + 16;
 };
 constexpr int kSlideRowWaves = 8, kSlideRowTiles = 2;  // 16-row tiles of a wave
-constexpr int kAhead = 4;                              // operands read ahead
 
 // Eight waves with 32 rows each, as attn_rows_kernel: K and V of a step lie in
-// LDS in 16 bits, each wave brings 16 keys of one of them (blk, kv).  Rows of
-// 16 bits are copied into one of two buffers while the other is computed on; a
-// step of codes lies in half of the second buffer and is turned into the first
-// between two steps.
+// LDS in 16 bits, each wave brings 16 keys of one of them.  Rows of 16 bits are
+// copied into one of two buffers while the other is computed on.  A step of
+// codes lies in half of the second buffer; 32 of its keys at a time are turned
+// into rounded values and rests of K and of V, which fill the first.
 template <int D, bool Q8>
 __global__ void __launch_bounds__(64 * kSlideRowWaves) slide_rows_kernel(const SlideArgs a) {
   typedef SlidePart<D> P;
@@ -714,6 +739,7 @@ __global__ void __launch_bounds__(64 * kSlideRowWaves) slide_rows_kernel(const S
   constexpr int RT = kSlideRowTiles, NW = kSlideRowWaves, DT = D / 16, KK = D / 32;
   constexpr int CH = D / 8, RPI = 64 / CH, NI = 16 / RPI;  // as Part: 16-bit copies
   constexpr int CQ = D / 16, RQ = 64 / CQ, NQ = 16 / RQ;   // of codes
+  constexpr int kAhead = 4;  // operands read ahead
   extern __shared__ __attribute__((aligned(16))) unsigned char lds[];
   const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
   const int blk = wave & 3;
@@ -782,32 +808,38 @@ __global__ void __launch_bounds__(64 * kSlideRowWaves) slide_rows_kernel(const S
                  ln * 16, sc);
     }
   };
-  // the wave's 16 keys of half `half` into the first buffer, as 16 bits; rows that
-  // are not there as 0.  True if one of V's groups is not finite and `full` is not so.
-  auto turn_codes = [&](int half, bool full, uint32_t there) {
-    const unsigned char* const from =
-        lds + (2 + half) * P::kStep + (is_v ? P::kStep / 2 : 0) + blk * 16 * D;
-    const unsigned char* const sc =
-        lds + L::kScales + half * L::kScaleStep + (is_v ? L::kScaleStep / 2 : 0) + blk * D;
-    bool odd = false;
+  // Keys 32 st.. of half `half` into the first buffer: rounded K, its rests, V
+  // likewise; rows of V that are not there as 0.  A wave has eight of K's keys or
+  // of V's.  True if one of V's groups is not finite and `full` is not so.
+  constexpr uint32_t kPart = 32 * D * 2;
+  auto turn_codes = [&](int half, int st, bool full, uint64_t there) {
     int ln = lane;
-    asm("" : "+v"(ln));
-#pragma unroll
-    for (int i = 0; i < NQ; ++i) {
-      const int row = i * RQ + ln / CQ, c = ln % CQ;
-      const u32x4 x = *reinterpret_cast<const u32x4*>(from + i * 1024 + ln * 16);
+    asm("" : "+v"(ln));  // (the offsets made anew: registers are short)
+    const int key0 = 32 * st + 8 * blk;
+    const unsigned char* const from =
+        lds + (2 + half) * P::kStep + (is_v ? P::kStep / 2 : 0) + key0 * D;
+    const unsigned char* const sc = lds + L::kScales + half * L::kScaleStep +
+                                    (is_v ? L::kScaleStep / 2 : 0) + key0 * (D / kKvGroup * 2);
+    bool odd = false;
+#pragma unroll 1
+    for (int i = 0; i < (RQ < 8 ? 8 / RQ : 1); ++i) {
+      const int r = i * RQ + ln / CQ, c = ln % CQ;  // of the eight keys
+      if (RQ > 8 && r >= 8) break;
+      const u32x4 x = *reinterpret_cast<const u32x4*>(from + r * D + c * 16);
       uint32_t scale =
-          *reinterpret_cast<const uint16_t*>(sc + row * (D / kKvGroup * 2) + (c / 2) * 2);
-      if (!full && is_v) odd |= finite_scale(scale, there >> row & 1);
+          *reinterpret_cast<const uint16_t*>(sc + r * (D / kKvGroup * 2) + (c / 2) * 2);
+      if (!full && is_v) odd |= finite_scale(scale, there >> (key0 + r) & 1);
       const h2 d = scale2(scale);
-      uint32_t w[4][2];
+      uint32_t w[4][2], y[4][2];
 #pragma unroll
-      for (int j = 0; j < 4; ++j) decode4(x[j], d, w[j]);
-      unsigned char* const to = lds + mine + row * (D * 2);
-      *reinterpret_cast<u32x4*>(to + (((2 * c) ^ swz<D>(row)) << 4)) =
-          (u32x4){w[0][0], w[0][1], w[1][0], w[1][1]};
-      *reinterpret_cast<u32x4*>(to + (((2 * c + 1) ^ swz<D>(row)) << 4)) =
-          (u32x4){w[2][0], w[2][1], w[3][0], w[3][1]};
+      for (int j = 0; j < 4; ++j) decode4(x[j], d, w[j], y[j]);
+      const int row = 8 * blk + r;  // of the 32 keys
+      const uint32_t s0 = ((2 * c) ^ swz<D>(row & 15)) << 4, s1 = ((2 * c + 1) ^ swz<D>(row & 15)) << 4;
+      unsigned char* const to = lds + (is_v ? P::kStep : 0) + row * (D * 2);
+      *reinterpret_cast<u32x4*>(to + s0) = (u32x4){w[0][0], w[0][1], w[1][0], w[1][1]};
+      *reinterpret_cast<u32x4*>(to + s1) = (u32x4){w[2][0], w[2][1], w[3][0], w[3][1]};
+      *reinterpret_cast<u32x4*>(to + kPart + s0) = (u32x4){y[0][0], y[0][1], y[1][0], y[1][1]};
+      *reinterpret_cast<u32x4*>(to + kPart + s1) = (u32x4){y[2][0], y[2][1], y[3][0], y[3][1]};
     }
     return !full && is_v && __any(odd);
   };
@@ -843,12 +875,13 @@ __global__ void __launch_bounds__(64 * kSlideRowWaves) slide_rows_kernel(const S
   }
   const uint32_t koff = t.k_offset(), voff = t.v_offset();
 
-  // A step on the buffer at b.
-  auto compute = [&](int step, uint32_t b, bool full, uint64_t there) {
-    uint32_t kbase = koff + b, vbase = voff + b;
-    asm("" : "+v"(kbase), "+v"(vbase));
-#pragma unroll 1
-    for (int st = 0; st < 2; ++st) {
+  // Keys 32 st.. of a step, K's and V's operands from kbase and vbase on; with
+  // rests, kPart behind the values.
+  auto compute = [&](int step, int st, uint32_t kbase, uint32_t vbase, bool full, uint64_t there,
+                     auto rests) {
+    constexpr int kParts = decltype(rests)::value ? 2 : 1;
+    asm("" : "+v"(kbase), "+v"(vbase));  // (the pieces' places made anew: registers)
+    {
       f4 s[2][RT];
 #pragma unroll
       for (int b = 0; b < 2; ++b)
@@ -857,19 +890,22 @@ __global__ void __launch_bounds__(64 * kSlideRowWaves) slide_rows_kernel(const S
       // K's pieces, of the two blocks in turn, kAhead of them under way: what LDS
       // takes to answer eight waves is longer than the products of one or two
       h8 kn[kAhead];
+      constexpr int kPieces = 2 * KK * kParts;
       auto k_read = [&](int f) {
-        return t.k_frag(P::k_piece(kbase, (f >> 1) % P::KO), f >> 1, f & 1);
+        const int g = f % (2 * KK), part = f / (2 * KK);
+        return t.k_frag(P::k_piece(kbase, (g >> 1) % P::KO) + part * kPart, g >> 1, g & 1);
       };
 #pragma unroll
       for (int f = 0; f < kAhead; ++f) kn[f] = k_read(f);
 #pragma unroll
-      for (int f = 0; f < 2 * KK; ++f) {
+      for (int f = 0; f < kPieces; ++f) {
         const h8 kf = kn[f % kAhead];
+        const int g = f % (2 * KK);
 #pragma unroll
         for (int rt = 0; rt < RT; ++rt)
-          s[f & 1][rt] =
-              __builtin_amdgcn_mfma_f32_16x16x32_f16(kf, qf[rt][f >> 1], s[f & 1][rt], 0, 0, 0);
-        if (f + kAhead < 2 * KK) kn[f % kAhead] = k_read(f + kAhead);
+          s[g & 1][rt] =
+              __builtin_amdgcn_mfma_f32_16x16x32_f16(kf, qf[rt][g >> 1], s[g & 1][rt], 0, 0, 0);
+        if (f + kAhead < kPieces) kn[f % kAhead] = k_read(f + kAhead);
         __builtin_amdgcn_sched_barrier(0);
       }
       bool move = false;
@@ -929,20 +965,22 @@ __global__ void __launch_bounds__(64 * kSlideRowWaves) slide_rows_kernel(const S
                  ((s[1][rt][0] + s[1][rt][1]) + (s[1][rt][2] + s[1][rt][3]));
       }
       h8 vn[kAhead];
+      auto v_read = [&](int f) {  // (tile after tile, a tile's rests behind its values)
+        return t.v_frag(P::v_tile(vbase, f / kParts) + f % kParts * kPart, 0);
+      };
 #pragma unroll
-      for (int d = 0; d < kAhead; ++d) vn[d] = t.v_frag(P::v_tile(vbase, d), 0);
+      for (int f = 0; f < kAhead; ++f) vn[f] = v_read(f);
       __builtin_amdgcn_sched_barrier(0);
 #pragma unroll
-      for (int d = 0; d < DT; ++d) {
-        const h8 vf = vn[d % kAhead];
+      for (int f = 0; f < DT * kParts; ++f) {
+        const h8 vf = vn[f % kAhead];
+        const int d = f / kParts;
 #pragma unroll
         for (int rt = 0; rt < RT; ++rt)
           acc[rt][d] = __builtin_amdgcn_mfma_f32_16x16x32_f16(vf, pf[rt], acc[rt][d], 0, 0, 0);
-        if (d + kAhead < DT) vn[d % kAhead] = t.v_frag(P::v_tile(vbase, d + kAhead), 0);
+        if (f + kAhead < DT * kParts) vn[f % kAhead] = v_read(f + kAhead);
         __builtin_amdgcn_sched_barrier(0);
       }
-      kbase += 32 * D * 2;
-      vbase += 32 * D * 2;
     }
   };
 
@@ -959,16 +997,18 @@ __global__ void __launch_bounds__(64 * kSlideRowWaves) slide_rows_kernel(const S
         const uint64_t there = full ? ~0ull : t.present(step, ok);
         const int next = t.steps.skip(step + 1);
         wait_vm();
-        bar();  // nobody reads the first buffer any more (and the flags are cleared)
-        if (turn_codes(it & 1, full, static_cast<uint32_t>(there >> (16 * blk)) & 0xFFFFu))
-          *odds = 1;
-        wait_lds();
+        bar();  // the codes are here, nobody reads the first buffer (and the flags are cleared)
         if (next < cached_end) {
           rows = t.rows_of(next);
           bring_codes(rows, (it + 1) & 1);
         }
-        bar();  // everybody's keys are there
-        compute(step, 0, full, there);
+#pragma unroll 1
+        for (int st = 0; st < 2; ++st) {
+          if (st > 0) bar();  // nobody reads the first 32 keys any more
+          if (turn_codes(it & 1, st, full, there)) *odds = 1;
+          bar();  // everybody's keys are there
+          compute(step, st, koff, voff, full, there, std::true_type());
+        }
         step = next;
       }
     }
@@ -994,7 +1034,10 @@ __global__ void __launch_bounds__(64 * kSlideRowWaves) slide_rows_kernel(const S
         *odds = 1;
       bar();  // everybody's copies of this step are here, and nobody reads the other buffer
       if (next < t.end) bring(next, rows, b ^ 2 * P::kStep);
-      compute(step, b, full, there);
+#pragma unroll 1
+      for (int st = 0; st < 2; ++st)
+        compute(step, st, koff + b + st * kPart, voff + b + st * kPart, full, there,
+                std::false_type());
       step = next;
     }
   }
@@ -1086,10 +1129,10 @@ static int slide_launch(const SlideArgs& a, hipStream_t s, const char* nm) {
     hipLaunchKernelGGL((slide_rows_kernel<D, Q8>), grid, dim3(64 * kSlideRowWaves),
                        SlideRowsLds<D>::kBytes, s, a);
   else if (a.block_rows == 32)
-    hipLaunchKernelGGL((slide_few_kernel<D, 2, Q8>), grid, dim3(256), (SlideFewLds<D, 2>::kBytes), s,
+    hipLaunchKernelGGL((slide_few_kernel<D, 2, Q8>), grid, dim3(256), (SlideFewLds<D, 2, Q8>::kBytes), s,
                        a);
   else
-    hipLaunchKernelGGL((slide_few_kernel<D, 1, Q8>), grid, dim3(256), (SlideFewLds<D, 1>::kBytes), s,
+    hipLaunchKernelGGL((slide_few_kernel<D, 1, Q8>), grid, dim3(256), (SlideFewLds<D, 1, Q8>::kBytes), s,
                        a);
   if (int st = check_launch(nm)) return st;
   if (a.cut) {
