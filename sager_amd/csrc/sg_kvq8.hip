@@ -276,7 +276,7 @@ int sg_kv_read_q8(const sg_kv_cache_q8* cache, const int* first, const int* row_
   if (reinterpret_cast<uintptr_t>(k) % 2 || reinterpret_cast<uintptr_t>(v) % 2)
     return set_error(SG_ERR_INVALID_ARGUMENT, "%s: k and v must be 2-B aligned", nm);
   const int rows = 64 / (cache->head_dim / 16);  // of a wave
-  const long long waves = (n_rows + rows - 1LL) / rows * cache->n_kv_heads;
+  const long long waves = (n_rows - 1LL + rows) / rows * cache->n_kv_heads;
   const int groups = (cache->n_layers + kReadLayers - 1) / kReadLayers;
   // (a launch has less than 2^32 threads in a row)
   if (cache->n_layers > 65535 || waves > 0xFFFFFFFFLL / 64 - 4)
