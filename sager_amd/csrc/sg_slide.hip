@@ -1071,39 +1071,63 @@ struct SlideLayout {
   int block_rows, row_blocks, max_units, goal;
   bool cut;
   int spread;
-  int few[3];  // the most sequences for less than one round, two, and one of many row blocks
+  int few[3];  // the most sequences that are cut for want of work, for two rounds, in few rows
   size_t plan_bytes, o_bytes, bytes;  // of the workspace
 };
 static SlideLayout slide_layout(int n_seq, int max_window, int max_len, int group, int n_kv, int dim,
                                 int reach, int sinks) {
   SlideLayout l;
   const long long rows = static_cast<long long>(max_window) * group;
-  l.block_rows = rows > 128 ? 256 : rows > 16 ? 32 : 16;
+  const long long units = static_cast<long long>(n_seq) * n_kv;
+  // steps at the most: of a sequence, and of a block of 256 of its rows (a window
+  // that may be a tree lies in every block's reach)
+  auto steps = [&](long long nodes) {
+    const long long keys = static_cast<long long>(max_len) + max_window;
+    const long long near = static_cast<long long>(reach) + nodes + sinks + 2 * kKeys;
+    return ((keys < near ? keys : near) + kKeys - 1) / kKeys + 1;
+  };
+  const long long most = steps(max_window);
+  const long long own = max_window <= kMaxWindow ? most : steps(256 / group + 1);
+  // 256 rows read a step's keys once and keep the matrix cores busy, but 32 rows
+  // spread little work further: by 256 as soon as each CU has two such steps (in
+  // us, 32 rows and 256: 32 sequences of 64 nodes, 32 query heads on 8, over 300
+  // keys of 128 quantised values 70 and 43, 4 of 32 nodes, 64 on 8, over 32,768
+  // 494 and 322; 8 of 64 nodes that reach 128 keys back, 48 on 8, 24 and 32).
+  const long long wide_units = 2 * 256 / ((rows + 255) / 256 * own) + 1;
+  const bool wide = rows > 128 && units >= wide_units;
+  l.block_rows = wide ? 256 : rows > 16 ? 32 : 16;
   l.row_blocks = static_cast<int>((rows + l.block_rows - 1) / l.block_rows);
+  const long long blocks = units * l.row_blocks;
   const bool near_only = reach / 2 < max_len / 2 + max_window / 2;
   l.spread = l.row_blocks < 8 ? kSpreadUnits : near_only ? kSpreadRuns : kSpreadTurns;
-  const long long units = static_cast<long long>(n_seq) * n_kv;
-  // a sequence's steps at the most
-  const long long keys = static_cast<long long>(max_len) + max_window;
-  const long long near = static_cast<long long>(reach) + max_window + sinks + 2 * kKeys;
-  const long long most = ((keys < near ? keys : near) + kKeys - 1) / kKeys + 1;
   // workgroups that the card holds at once, and units of them (32 sequences of
   // one token and of five over 4,000 quantised ones, 8 kv heads of 128: 59.8 and
   // 69.4 us by 3 a CU, 62.0 and 80.0 by 4, 58.6 and 72.6 by 2; of 64: 53.6 us by
   // 4, 67.5 by 2; four tokens over 131,071, 2 kv heads of 256: 43.8 by 2, 58.3 by 4)
-  const int each = l.block_rows == 256 ? 1 : dim == 256 ? 2 : dim == 128 ? 3 : 4;
+  const int each = wide ? 1 : dim == 256 ? 2 : dim == 128 ? 3 : 4;
   const long long slots = 256 * each;
   const long long per = 32 * each >= l.row_blocks ? 32 * each / l.row_blocks * 8 : 8;
-  const bool rounds = units >= 2 * slots;
-  for (int i = 0; i < 2; ++i) l.few[i] = static_cast<int>(((i + 1) * slots - 1) / n_kv);
-  l.few[2] = static_cast<int>((slots - 1) / (static_cast<long long>(n_kv) * l.row_blocks));
+  // Less work than the card holds is cut into parts if that saves more steps than
+  // the parts' way through memory and the join cost, `join` of them; blocks that
+  // see few of their sequence's steps would get empty parts.  More than it holds,
+  // in blocks of few rows, is cut over long caches, so that a ragged batch ends
+  // together.  (28 sequences of up to 210 tokens, 56 query heads on 8 of 128, that
+  // reach 63 keys back: 340 us in parts, 88 whole; 600 batches of mixed shapes:
+  // half and twice `join` cost 2% and 1% more.)
+  const long long join = wide ? dim / 32 + 1 : 8;
+  const long long room = own > join ? slots - slots * join / own : 0;  // of blocks: below it
+  const bool rounds = blocks >= 2 * slots;
+  l.cut = own * 2 >= most && (blocks < room || (!wide && blocks >= slots && most > 8));
+  const long long a_seq = static_cast<long long>(n_kv) * l.row_blocks;
+  l.few[0] = static_cast<int>(room > 0 ? (room - 1) / a_seq : 0);
+  l.few[1] = static_cast<int>((2 * slots - 1) / a_seq);
+  const long long narrow = (wide_units - 1) / n_kv;  // the most sequences in blocks of few rows
+  l.few[2] = static_cast<int>(wide ? narrow : 0);
   long long n = units;
-  // (many row blocks fill the card without a cut)
-  l.cut = most > 1 && (units < slots || most > 8) && !(l.spread && units * l.row_blocks >= slots);
   l.goal = 1;
-  if (l.cut && l.spread) {
-    n = units + slots / l.row_blocks;
-    l.goal = static_cast<int>(n_seq <= 64 ? n : n - units);
+  if (l.cut && wide) {
+    l.goal = static_cast<int>(slots / l.row_blocks);
+    n = l.goal + (n_seq <= 64 ? 0 : units);
   } else if (l.cut && !rounds) {
     n = (2 * units + per - 1) / per * per;
     // (a part a head lost to rounding; one in a thousand less: parts_of rounds)
@@ -1280,15 +1304,20 @@ size_t sg_attn_sliding_workspace_bytes(int n_seq, int max_window, int max_len, i
   // Enough for every smaller batch too: within a way of cutting fewer sequences
   // have no more units, but fewer may be cut where more are not.
   const int group = n_heads / n_kv_heads, far = reach == 0 ? 0x7FFFFFFF : reach;
-  const sg::SlideLayout l =
-      sg::slide_layout(n_seq, max_window, max_len, group, n_kv_heads, head_dim, far, sinks);
-  size_t bytes = l.bytes;
-  for (int few : l.few)
-    if (few > 0 && few < n_seq) {
-      const size_t b =
-          sg::slide_layout(few, max_window, max_len, group, n_kv_heads, head_dim, far, sinks).bytes;
-      bytes = b > bytes ? b : bytes;
-    }
+  auto layout = [&](int n) {
+    return sg::slide_layout(n, max_window, max_len, group, n_kv_heads, head_dim, far, sinks);
+  };
+  size_t bytes = 0;
+  for (int n = n_seq; n > 0;) {
+    const sg::SlideLayout l = layout(n);
+    bytes = l.bytes > bytes ? l.bytes : bytes;
+    for (int i = 0; i < 2; ++i)
+      if (l.few[i] > 0 && l.few[i] < n) {
+        const size_t few = layout(l.few[i]).bytes;
+        bytes = few > bytes ? few : bytes;
+      }
+    n = l.few[2];
+  }
   return bytes;
 }
 
