@@ -682,8 +682,10 @@ int sg_kv_read_q8(const sg_kv_cache_q8* cache, const int* first, const int* row_
  * keys of positions above p - reach (its own among them) and below sinks.
  * reach 0: all of them.  Pages that nobody sees any more may be absent.
  * With a parent a window has at most 64 nodes; without one (chains) it may
- * have any number, a prompt's whole chunk.  A quantised value is rounded to
- * fp16 once, as code * scale; the rest is as for sg_attn_tree_f16.
+ * have any number, a prompt's whole chunk.  A quantised value enters both
+ * products as code * scale, not rounded; it has to be below 65,504, as all are
+ * that commit and append write, or is not a number.  The rest is as for
+ * sg_attn_tree_f16.
  * Workspace: sg_attn_sliding_workspace_bytes of as many sequences or more, of
  * the same reach and sinks. */
 size_t sg_attn_sliding_workspace_bytes(int n_seq, int max_window, int max_len, int n_heads,

@@ -122,8 +122,8 @@ struct SlidePart : Part<D> {
       this->rb = sa.row_blocks - 1 - (id - this->unit * sa.row_blocks);
     } else if (sa.spread == kSpreadRuns) {
       // That see a window: an XCD has neighbours, whose windows are the same keys
-      // but for a few, and reads them once (4,096 tokens of 16 heads of 256 over
-      // windows of 2,048: RUNS_US us, in turn TURNS_US).
+      // but for a few, and reads them once (4,096 tokens of 32 heads on 8 of 128 over
+      // windows of 2,048: 210 us, 255 quantised; in turn 221 and 327).
       // (past the last unit there is none)
       const int at = (id & 7) * (gridDim.x >> 3) + (id >> 3);
       this->unit = at / sa.row_blocks;
@@ -336,7 +336,12 @@ constexpr int slide_waves(int dim, int tiles) {
 }
 
 // RT: tiles of 16 rows.  Wave w has keys 16 w.. of a step in the first product,
-// and columns w D/4 .. of all keys in the second.
+// and columns w D/4 .. of all keys in the second.  Bound by the cache's bytes
+// where batches are large (32 sequences of one token over 4,000, 8 kv heads of
+// 128: 525 MB in 16 bits in 102 us, 5.2 TB/s; quantised 279 MB in 63 us, 4.4
+// TB/s, with vector instructions for the values as the other half of the time),
+// and by the length of a step, some 2 us of loads, exponentials and barriers,
+// where few workgroups have work.
 template <int D, int RT, bool Q8>
 __global__ void __launch_bounds__(256, slide_waves(D, RT)) slide_few_kernel(const SlideArgs a) {
   typedef SlidePart<D> P;
@@ -395,14 +400,21 @@ __global__ void __launch_bounds__(256, slide_waves(D, RT)) slide_few_kernel(cons
   auto load_v = [&](Cached& x, const Rows& rows) {
     // (values of the wave's columns; a block of 16 rows or more at once)
     constexpr int N = Q8 ? LQ : KK, L1 = Q8 ? LQ : LP, R1 = Q8 ? RQ : RP;
+    // (out of their array: a choice among its elements would put it into scratch memory)
+    long long from[4];
+#pragma unroll
+    for (int b = 0; b < 4; ++b) {
+      from[b] = rows.at[b];
+      asm("" : "+s"(from[b]));
+    }
 #pragma unroll
     for (int i = 0; i < N; ++i) {
       constexpr int kBlocks = R1 <= 16 ? 1 : R1 / 16;
       const int b0 = i * R1 / 16, in = lane / L1;
-      long long at = rows.at[b0];
-      if constexpr (kBlocks == 2) at = in < 16 ? at : rows.at[b0 + 1];
+      long long at = from[b0];
+      if constexpr (kBlocks == 2) at = in < 16 ? at : from[b0 + 1];
       if constexpr (kBlocks == 4)
-        at = in < 32 ? (in < 16 ? rows.at[0] : rows.at[1]) : (in < 48 ? rows.at[2] : rows.at[3]);
+        at = in < 32 ? (in < 16 ? from[0] : from[1]) : (in < 48 ? from[2] : from[3]);
       const uint32_t row = i * R1 % 16 + in % 16;
       const uint32_t off = row * D + wave * (D / 4) + (lane % L1) * (Q8 ? 16 : 8);
       if constexpr (Q8) {
@@ -730,7 +742,11 @@ constexpr int kSlideRowWaves = 8, kSlideRowTiles = 2;  // 16-row tiles of a wave
 // LDS in 16 bits, each wave brings 16 keys of one of them.  Rows of 16 bits are
 // copied into one of two buffers while the other is computed on.  A step of
 // codes lies in half of the second buffer; 32 of its keys at a time are turned
-// into rounded values and rests of K and of V, which fill the first.
+// into rounded values and rests of K and of V, which fill the first.  Bound by
+// the matrix cores and the exponentials between their products (4,096 tokens,
+// 16 heads on 2 of 256, windows of 2,048 over 4,099 more: 165 to 190 us, 830 to
+// 700 TFLOP/s; quantised 294 us, as the products with the cache are twice as
+// many; 32 heads on 8 of 128: 210 us and 255).
 template <int D, bool Q8>
 __global__ void __launch_bounds__(64 * kSlideRowWaves) slide_rows_kernel(const SlideArgs a) {
   typedef SlidePart<D> P;

@@ -1,6 +1,5 @@
 """Attention over a sliding window and the first tokens, over a 16-bit and a quantised cache, against
-its plain form in 64 bits (a quantised value enters it as the kernel's contract says: code * scale
-rounded to 16 bits).  The tolerance is that of the tree attention's tests: the output's rounding, the
+its plain form in 64 bits (a quantised value is code * scale there as here).  The tolerance is that of the tree attention's tests: the output's rounding, the
 weights' (2^-11 each), fp32 sums, and what a score's fp32 error moves a weight by."""
 import numpy as np
 import pytest
@@ -19,7 +18,7 @@ def case(seed, sizes, lengths, n_kv, group, D, page, reach=0, sinks=0, q8=False,
     c.update(reach=reach, sinks=sinks, q8=q8)
     if q8:
         c["codes"] = [cref.quantise(c[n]) for n in ("kc", "vc")]
-        c["kc"], c["vc"] = (cref.values(*x).astype(np.float16) for x in c["codes"])
+        c["kc"], c["vc"] = (cref.values(*x) for x in c["codes"])
     if evict:  # whole pages that nobody sees any more have gone to others
         for s, n in enumerate(lengths):
             for p in range((n + page - 1) // page):
@@ -158,7 +157,7 @@ def test_a_group_of_nan_where_it_is_not_seen():
             v[0, c["pages"][0, j // 16], 0, j % 16, :32] = 0
             vs[0, c["pages"][0, j // 16], 0, j % 16, 0] = np.nan
         ks[0, c["pages"][0, 100 // 16], 0, 100 % 16, 1] = np.nan
-        c["kc"], c["vc"] = (cref.values(*x).astype(np.float16) for x in c["codes"])
+        c["kc"], c["vc"] = (cref.values(*x) for x in c["codes"])
         got = check(c)
         assert np.isfinite(got[..., 32:]).all() and not np.isfinite(got[..., :32]).all()
 
@@ -272,13 +271,13 @@ def test_past_two_gib_of_a_pool():
         got = w.run_attn(c, op, cache).cpu().numpy().astype(np.float64)
         d = dict(c)
         if q8:
-            d["kc"], d["vc"] = c["kc"].copy(), c["vc"].copy()
             for n, x in zip(("kc", "vc"), codes):
-                d[n][:, used] = cref.values(*x).astype(np.float16)
+                d[n] = c[n].astype(np.float64)
+                d[n][:, used] = cref.values(*x)
             k, v = cache.read(dev(np.zeros(1, np.int32)), dev(np.array([0, 600], np.int32)), 600)
             for t, x in ((k, d["kc"]), (v, d["vc"])):
                 rows = np.concatenate([x[0, p].transpose(1, 0, 2) for p in used])[:600]
-                assert (t[0].cpu().numpy() == rows).all()
+                assert (t[0].cpu().numpy() == rows.astype(np.float16)).all()
         want, spread = plain(d, np.zeros(c["q"].shape))
         assert (np.abs(got - want) <= w.attn_tol(c, want, spread)).all()
         del ts, cache
