@@ -1118,8 +1118,8 @@ static SlideLayout slide_layout(int n_seq, int max_window, int max_len, int grou
   l.spread = l.row_blocks < 8 ? kSpreadUnits : near_only ? kSpreadRuns : kSpreadTurns;
   // workgroups that the card holds at once, and units of them (32 sequences of
   // one token and of five over 4,000 quantised ones, 8 kv heads of 128: 59.8 and
-  // 69.4 us by 3 a CU, 62.0 and 80.0 by 4, 58.6 and 72.6 by 2; of 64: 53.6 us by
-  // 4, 67.5 by 2; four tokens over 131,071, 2 kv heads of 256: 43.8 by 2, 58.3 by 4)
+  // 69.4 us by 3 a CU, 62.0 and 80.0 by 4, 58.6 and 72.6 by 2; of 64: 41 us by
+  // 4, 48 by 2; four tokens over 131,071, 2 kv heads of 256: 43.8 by 2, 58.3 by 4)
   const int each = wide ? 1 : dim == 256 ? 2 : dim == 128 ? 3 : 4;
   const long long slots = 256 * each;
   const long long per = 32 * each >= l.row_blocks ? 32 * each / l.row_blocks * 8 : 8;

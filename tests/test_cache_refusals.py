@@ -281,3 +281,14 @@ def test_attention_workspace(lib):
                          (1000, max_len, 8, 2, 128), (65, max_len, 4, 1, 256)):
                 for n in range(2, 300):
                     assert f(n, *args, reach, sinks) >= f(n - 1, *args, reach, sinks)
+
+
+@pytest.mark.parametrize("q8", [False, True])
+def test_attention_token_strides(lib, q8):
+    """A few tokens' rows are reached by 32-bit offsets."""
+    fn = lib.sg_attn_sliding_q8 if q8 else lib.sg_attn_sliding_f16
+    c = (cache if q8 else f16_cache)()
+    for name in ("ks", "vs"):
+        for stride in (1 << 27, 1 << 40):
+            assert fn(*attn_args(c, n_tokens=1, max_window=1, **{name: stride})) == UNSUPPORTED
+            assert b"stride" in lib.sg_last_error()

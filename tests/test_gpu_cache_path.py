@@ -211,10 +211,11 @@ def test_a_verify_step_as_a_graph(q8):
             assert torch.equal(t, pair[1].cache._tensors[name]), (turn, name)
 
 
-@pytest.mark.parametrize("heads", [1, 16, 128])
+# (256 heads behind what may be a long cache get blocks of 256 rows)
+@pytest.mark.parametrize("heads,max_len", [(1, 2), (16, 2), (128, 2), (256, 10 ** 6)])
 @pytest.mark.parametrize("D", [64, 128, 256])
 @pytest.mark.parametrize("power", [8, 0, -9, -14])
-def test_quantised_keys_are_not_rounded(power, D, heads):
+def test_quantised_keys_are_not_rounded(power, D, heads, max_len):
     """Keys whose values, 128 1/16 and 128 3/16 times a power of two, lie half a step of 16 bits from
     the next, one below and one above: their scores are 256 and 256 1/4, and 256 1/2 if keys were
     rounded, which moves the weights by 6 %.  A score's sum of 256 is off by 2 D roundings of 2^-24 at
@@ -230,7 +231,7 @@ def test_quantised_keys_are_not_rounded(power, D, heads):
     k, v = np.zeros((1, 1, D), np.float16), np.ones((1, 1, D), np.float16)
     pages, length = np.array([[1]], np.int32), np.array([2], np.int32)
     cache = ops.KvCacheQ8(*(dev(x) for x in (kc, vc, ks, vs, pages, length)))
-    op = ops.SlidingAttention(heads, 1, D, max_tokens=1, max_len=2)
+    op = ops.SlidingAttention(heads, 1, D, max_tokens=1, max_len=max_len)
     by = 256 / (2.0 ** power * 128.0625 * D / 2)
     got = op.forward(dev(q), dev(k), dev(v), cache, dev(np.array([0, 1], np.int32)),
                      scale=by).cpu().numpy().astype(np.float64)
