@@ -51,6 +51,14 @@ __device__ __forceinline__ void settle(T (&x)[N]) {
   for (int i = 0; i < N; ++i) asm volatile("" : "+v"(x[i]));
 }
 
+// Two weights more in a row's sum.  The sum is of the rounded weights, those that
+// the product with V is made with: what rounding a large weight takes from one it
+// then takes from the other.
+__device__ __forceinline__ float weight_sum(h2 p, float sum) {
+  const h2 one = {static_cast<_Float16>(1.f), static_cast<_Float16>(1.f)};
+  return __builtin_amdgcn_fdot2(p, one, sum, false);
+}
+
 struct SlideArgs : AttnArgs {
   const uint16_t *ks, *vs;  // scales of the quantised cache (kc, vc: its codes)
   int reach, sinks;
@@ -496,14 +504,11 @@ __global__ void __launch_bounds__(256, slide_waves(D, RT)) slide_few_kernel(cons
 
     float e[RT][4], top[RT], sum[RT];
     auto weigh = [&](int rt, float by) {  // row tile rt's p = 2^(e - by), into LDS
-      float p[4];
       h4 ph;
 #pragma unroll
-      for (int i = 0; i < 4; ++i) {
-        p[i] = __builtin_amdgcn_exp2f(e[rt][i] - by);
-        ph[i] = static_cast<_Float16>(p[i]);
-      }
-      sum[rt] = (p[0] + p[1]) + (p[2] + p[3]);
+      for (int i = 0; i < 4; ++i)
+        ph[i] = static_cast<_Float16>(__builtin_amdgcn_exp2f(e[rt][i] - by));
+      sum[rt] = weight_sum((h2){ph[0], ph[1]}, weight_sum((h2){ph[2], ph[3]}, 0.f));
       *reinterpret_cast<h4*>(lds + p_out + par * L::kStepP + rt * 16 * 128) = ph;
     };
     bool move = false;
@@ -974,11 +979,12 @@ __global__ void __launch_bounds__(64 * kSlideRowWaves) slide_rows_kernel(const S
         for (int b = 0; b < 2; ++b)
 #pragma unroll
           for (int i = 0; i < 4; ++i) {
-            s[b][rt][i] = __builtin_amdgcn_exp2f(s[b][rt][i]);
-            pf[rt][4 * b + i] = static_cast<_Float16>(s[b][rt][i]);
+            pf[rt][4 * b + i] = static_cast<_Float16>(__builtin_amdgcn_exp2f(s[b][rt][i]));
           }
-        l[rt] += ((s[0][rt][0] + s[0][rt][1]) + (s[0][rt][2] + s[0][rt][3])) +
-                 ((s[1][rt][0] + s[1][rt][1]) + (s[1][rt][2] + s[1][rt][3]));
+        float sum = 0.f;
+#pragma unroll
+        for (int i = 0; i < 8; i += 2) sum = weight_sum((h2){pf[rt][i], pf[rt][i + 1]}, sum);
+        l[rt] += sum;
       }
       h8 vn[kAhead];
       auto v_read = [&](int f) {  // (tile after tile, a tile's rests behind its values)
