@@ -748,10 +748,10 @@ constexpr int kSlideRowWaves = 8, kSlideRowTiles = 2;  // 16-row tiles of a wave
 // copied into one of two buffers while the other is computed on.  A step of
 // codes lies in half of the second buffer; 32 of its keys at a time are turned
 // into rounded values and rests of K and of V, which fill the first.  Bound by
-// the matrix cores and the exponentials between their products (4,096 tokens,
-// 16 heads on 2 of 256, windows of 2,048 over 4,099 more: 165 to 190 us, 830 to
-// 700 TFLOP/s; quantised 294 us, as the products with the cache are twice as
-// many; 32 heads on 8 of 128: 210 us and 255).
+// the matrix cores, whose operands and scores are waited for by no more than two
+// waves a SIMD (4,096 tokens over 4,099 more, windows of 2,048: 16 heads on 2 of
+// 256 155 to 190 us, 890 to 730 TFLOP/s, quantised 280, as the products with the
+// cache are twice as many; 32 heads on 8 of 128 187 us and 250).
 template <int D, bool Q8>
 __global__ void __launch_bounds__(64 * kSlideRowWaves) slide_rows_kernel(const SlideArgs a) {
   typedef SlidePart<D> P;
@@ -761,6 +761,10 @@ __global__ void __launch_bounds__(64 * kSlideRowWaves) slide_rows_kernel(const S
   constexpr int CH = D / 8, RPI = 64 / CH, NI = 16 / RPI;  // as Part: 16-bit copies
   constexpr int CQ = D / 16, RQ = 64 / CQ, NQ = 16 / RQ;   // of codes
   constexpr int kAhead = 4;  // operands read ahead
+  // Halves of a step (32 keys) at once: fewer waits for scores and operands, where
+  // registers allow it (as below, heads of 128 without a window: 524 us, by one 595;
+  // at head dimension 64 two workgroups share a CU as long as they need 128).
+  constexpr int kHalves = D == 128 || (D == 64 && !Q8) ? 2 : 1;
   extern __shared__ __attribute__((aligned(16))) unsigned char lds[];
   const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
   const int blk = wave & 3;
@@ -896,113 +900,117 @@ __global__ void __launch_bounds__(64 * kSlideRowWaves) slide_rows_kernel(const S
   }
   const uint32_t koff = t.k_offset(), voff = t.v_offset();
 
-  // Keys 32 st.. of a step, K's and V's operands from kbase and vbase on; with
-  // rests, kPart behind the values.
+  // Keys 32 st.. of a step, `halves` times 32 of them, K's and V's operands from
+  // kbase and vbase on, kPart between the halves; with rests, kPart behind the values.
   auto compute = [&](int step, int st, uint32_t kbase, uint32_t vbase, bool full, uint64_t there,
-                     auto rests) {
-    constexpr int kParts = decltype(rests)::value ? 2 : 1;
+                     auto rests, auto halves) {
+    constexpr int kParts = decltype(rests)::value ? 2 : 1, H = decltype(halves)::value;
     asm("" : "+v"(kbase), "+v"(vbase));  // (the pieces' places made anew: registers)
-    {
-      f4 s[2][RT];
+    f4 s[2 * H][RT];
 #pragma unroll
-      for (int b = 0; b < 2; ++b)
+    for (int b = 0; b < 2 * H; ++b)
 #pragma unroll
-        for (int rt = 0; rt < RT; ++rt) s[b][rt] = (f4){0.f, 0.f, 0.f, 0.f};
-      // K's pieces, of the two blocks in turn, kAhead of them under way: what LDS
-      // takes to answer eight waves is longer than the products of one or two
-      h8 kn[kAhead];
-      constexpr int kPieces = 2 * KK * kParts;
-      auto k_read = [&](int f) {
-        const int g = f % (2 * KK), part = f / (2 * KK);
-        return t.k_frag(P::k_piece(kbase, (g >> 1) % P::KO) + part * kPart, g >> 1, g & 1);
-      };
+      for (int rt = 0; rt < RT; ++rt) s[b][rt] = (f4){0.f, 0.f, 0.f, 0.f};
+    // K's pieces, of the two blocks in turn, kAhead of them under way: what LDS
+    // takes to answer eight waves is longer than the products of one or two
+    h8 kn[kAhead];
+    constexpr int kPieces = 2 * KK * kParts * H;
+    auto k_read = [&](int f) {
+      const int g = f % (2 * KK), part = f / (2 * KK);  // (a half, or the rests)
+      return t.k_frag(P::k_piece(kbase, (g >> 1) % P::KO) + part * kPart, g >> 1, g & 1);
+    };
 #pragma unroll
-      for (int f = 0; f < kAhead; ++f) kn[f] = k_read(f);
+    for (int f = 0; f < kAhead; ++f) kn[f] = k_read(f);
 #pragma unroll
-      for (int f = 0; f < kPieces; ++f) {
-        const h8 kf = kn[f % kAhead];
-        const int g = f % (2 * KK);
+    for (int f = 0; f < kPieces; ++f) {
+      const h8 kf = kn[f % kAhead];
+      const int g = f % (2 * KK), b = (kParts == 1 ? f / (2 * KK) * 2 : 0) + (g & 1);
 #pragma unroll
-        for (int rt = 0; rt < RT; ++rt)
-          s[g & 1][rt] =
-              __builtin_amdgcn_mfma_f32_16x16x32_f16(kf, qf[rt][g >> 1], s[g & 1][rt], 0, 0, 0);
-        if (f + kAhead < kPieces) kn[f % kAhead] = k_read(f + kAhead);
-        __builtin_amdgcn_sched_barrier(0);
+      for (int rt = 0; rt < RT; ++rt)
+        s[b][rt] = __builtin_amdgcn_mfma_f32_16x16x32_f16(kf, qf[rt][g >> 1], s[b][rt], 0, 0, 0);
+      if (f + kAhead < kPieces) kn[f % kAhead] = k_read(f + kAhead);
+      __builtin_amdgcn_sched_barrier(0);
+    }
+    bool move = false;
+    float top[RT];
+#pragma unroll
+    for (int rt = 0; rt < RT; ++rt) {
+#pragma unroll
+      for (int b = 0; b < 2 * H; ++b)
+#pragma unroll
+        for (int i = 0; i < 4; ++i)
+          s[b][rt][i] = __builtin_fmaf(s[b][rt][i], a.scale_log2, -mref[rt]);
+      if (!full) {
+        const bool tree = cold_slide()->parent;
+        const int node = t.node_of(row0 + rt * 16 + col);
+        const int pos = tree ? place[node] : t.len + node;
+        const uint64_t up = tree ? seen[node] : 0;
+#pragma unroll
+        for (int b = 0; b < 2 * H; ++b) {
+          const uint32_t see = t.seen4(step, 32 * st + 16 * b + 4 * grp, there, pos, up);
+#pragma unroll
+          for (int i = 0; i < 4; ++i) s[b][rt][i] = see >> i & 1 ? s[b][rt][i] : -INFINITY;
+        }
       }
-      bool move = false;
-      float top[RT];
+      top[rt] = s[0][rt][0];
+#pragma unroll
+      for (int b = 0; b < 2 * H; ++b) {
+        top[rt] = max3(top[rt], s[b][rt][0], s[b][rt][1]);
+        top[rt] = max3(top[rt], s[b][rt][2], s[b][rt][3]);
+      }
+      move |= top[rt] > lim[rt];
+    }
+    if (__any(move)) {
 #pragma unroll
       for (int rt = 0; rt < RT; ++rt) {
+        float m = fmaxf(top[rt], __shfl_xor(top[rt], 16));
+        m = fmaxf(m, __shfl_xor(m, 32));
+        const bool set = m > lim[rt], begun = lim[rt] > 0.f;
+        const float by = set ? m - kBelow : 0.f;
+        const float f = !set ? 1.f : begun ? __builtin_amdgcn_exp2f(-by) : 0.f;
+        mref[rt] += by;
+        l[rt] *= f;
+#pragma unroll
+        for (int d = 0; d < DT; ++d) acc[rt][d] *= f;
+        lim[rt] = set ? kRise : lim[rt];
+#pragma unroll
+        for (int b = 0; b < 2 * H; ++b) s[b][rt] -= by;
+      }
+    }
+    h8 pf[H][RT];
+#pragma unroll
+    for (int rt = 0; rt < RT; ++rt) {
+      float sum = 0.f;
+#pragma unroll
+      for (int h = 0; h < H; ++h) {
 #pragma unroll
         for (int b = 0; b < 2; ++b)
 #pragma unroll
           for (int i = 0; i < 4; ++i)
-            s[b][rt][i] = __builtin_fmaf(s[b][rt][i], a.scale_log2, -mref[rt]);
-        if (!full) {
-          const bool tree = cold_slide()->parent;
-          const int node = t.node_of(row0 + rt * 16 + col);
-          const int pos = tree ? place[node] : t.len + node;
-          const uint64_t up = tree ? seen[node] : 0;
+            pf[h][rt][4 * b + i] = static_cast<_Float16>(__builtin_amdgcn_exp2f(s[2 * h + b][rt][i]));
 #pragma unroll
-          for (int b = 0; b < 2; ++b) {
-            const uint32_t see = t.seen4(step, 32 * st + 16 * b + 4 * grp, there, pos, up);
-#pragma unroll
-            for (int i = 0; i < 4; ++i) s[b][rt][i] = see >> i & 1 ? s[b][rt][i] : -INFINITY;
-          }
-        }
-        top[rt] = max3(max3(s[0][rt][0], s[0][rt][1], s[0][rt][2]),
-                       max3(s[0][rt][3], s[1][rt][0], s[1][rt][1]),
-                       max3(s[1][rt][2], s[1][rt][3], s[1][rt][3]));
-        move |= top[rt] > lim[rt];
+        for (int i = 0; i < 8; i += 2) sum = weight_sum((h2){pf[h][rt][i], pf[h][rt][i + 1]}, sum);
       }
-      if (__any(move)) {
+      l[rt] += sum;
+    }
+    h8 vn[kAhead];
+    constexpr int kTiles = DT * kParts * H;
+    auto v_read = [&](int f) {  // (tile after tile, a tile's rests behind its values; a half after the other)
+      const int part = kParts == 2 ? f % 2 : f / DT, d = kParts == 2 ? f / 2 : f % DT;
+      return t.v_frag(P::v_tile(vbase, d) + part * kPart, 0);
+    };
 #pragma unroll
-        for (int rt = 0; rt < RT; ++rt) {
-          float m = fmaxf(top[rt], __shfl_xor(top[rt], 16));
-          m = fmaxf(m, __shfl_xor(m, 32));
-          const bool set = m > lim[rt], begun = lim[rt] > 0.f;
-          const float by = set ? m - kBelow : 0.f;
-          const float f = !set ? 1.f : begun ? __builtin_amdgcn_exp2f(-by) : 0.f;
-          mref[rt] += by;
-          l[rt] *= f;
+    for (int f = 0; f < kAhead; ++f) vn[f] = v_read(f);
+    __builtin_amdgcn_sched_barrier(0);
 #pragma unroll
-          for (int d = 0; d < DT; ++d) acc[rt][d] *= f;
-          lim[rt] = set ? kRise : lim[rt];
+    for (int f = 0; f < kTiles; ++f) {
+      const h8 vf = vn[f % kAhead];
+      const int d = kParts == 2 ? f / 2 : f % DT, h = kParts == 2 ? 0 : f / DT;
 #pragma unroll
-          for (int b = 0; b < 2; ++b) s[b][rt] -= by;
-        }
-      }
-      h8 pf[RT];
-#pragma unroll
-      for (int rt = 0; rt < RT; ++rt) {
-#pragma unroll
-        for (int b = 0; b < 2; ++b)
-#pragma unroll
-          for (int i = 0; i < 4; ++i) {
-            pf[rt][4 * b + i] = static_cast<_Float16>(__builtin_amdgcn_exp2f(s[b][rt][i]));
-          }
-        float sum = 0.f;
-#pragma unroll
-        for (int i = 0; i < 8; i += 2) sum = weight_sum((h2){pf[rt][i], pf[rt][i + 1]}, sum);
-        l[rt] += sum;
-      }
-      h8 vn[kAhead];
-      auto v_read = [&](int f) {  // (tile after tile, a tile's rests behind its values)
-        return t.v_frag(P::v_tile(vbase, f / kParts) + f % kParts * kPart, 0);
-      };
-#pragma unroll
-      for (int f = 0; f < kAhead; ++f) vn[f] = v_read(f);
+      for (int rt = 0; rt < RT; ++rt)
+        acc[rt][d] = __builtin_amdgcn_mfma_f32_16x16x32_f16(vf, pf[h][rt], acc[rt][d], 0, 0, 0);
+      if (f + kAhead < kTiles) vn[f % kAhead] = v_read(f + kAhead);
       __builtin_amdgcn_sched_barrier(0);
-#pragma unroll
-      for (int f = 0; f < DT * kParts; ++f) {
-        const h8 vf = vn[f % kAhead];
-        const int d = f / kParts;
-#pragma unroll
-        for (int rt = 0; rt < RT; ++rt)
-          acc[rt][d] = __builtin_amdgcn_mfma_f32_16x16x32_f16(vf, pf[rt], acc[rt][d], 0, 0, 0);
-        if (f + kAhead < DT * kParts) vn[f % kAhead] = v_read(f + kAhead);
-        __builtin_amdgcn_sched_barrier(0);
-      }
     }
   };
 
@@ -1029,7 +1037,7 @@ __global__ void __launch_bounds__(64 * kSlideRowWaves) slide_rows_kernel(const S
           if (st > 0) bar();  // nobody reads the first 32 keys any more
           if (turn_codes(it & 1, st, full, there)) *odds = 1;
           bar();  // everybody's keys are there
-          compute(step, st, koff, voff, full, there, std::true_type());
+          compute(step, st, koff, voff, full, there, std::true_type(), std::integral_constant<int, 1>());
         }
         step = next;
       }
@@ -1057,9 +1065,9 @@ __global__ void __launch_bounds__(64 * kSlideRowWaves) slide_rows_kernel(const S
       bar();  // everybody's copies of this step are here, and nobody reads the other buffer
       if (next < t.end) bring(next, rows, b ^ 2 * P::kStep);
 #pragma unroll 1
-      for (int st = 0; st < 2; ++st)
+      for (int st = 0; st < 2; st += kHalves)
         compute(step, st, koff + b + st * kPart, voff + b + st * kPart, full, there,
-                std::false_type());
+                std::false_type(), std::integral_constant<int, kHalves>());
       step = next;
     }
   }

@@ -23,6 +23,7 @@ BUDGETS = [
     ("sg_slide.hip", r"slide_few_kernelILi64ELi2E", 128),
     ("sg_slide.hip", r"slide_few_kernelILi64ELi1E", 96),
     ("sg_slide.hip", r"slide_rows_kernel", 256),
+    ("sg_slide.hip", r"slide_rows_kernelILi64E", 128),
     ("sg_slide.hip", r"attn_join_kernel", 128),
 ]
 
