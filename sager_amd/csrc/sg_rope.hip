@@ -106,7 +106,7 @@ __global__ void __launch_bounds__(kRopeThreads) rope_kernel(const RopeArgs a) {
   const int t = blockIdx.x, tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
   const int lanes = 1 << a.lanes_log2;
   const int e = (tid & (lanes - 1)) * 8;       // the thread's values of a row
-  const int per = kRopeThreads >> a.lanes_log2;  // rows at a time
+  const int per = blockDim.x >> a.lanes_log2;  // rows at a time
   const int rot = 2 * a.half;
   float* const mine = part[wave] + (lane & ~(lanes - 1)) * 8;  // the row's values
 
@@ -327,9 +327,12 @@ static int rope_launch(const T* q, const T* k, T* q_out, T* k_out, long long q_s
   a.mscale = mscale;
   // Few tokens' heads are spread over workgroups that each make the angles
   // (4 tokens of 18 heads of 256: 4.7 us on the device, 8.5 by one a token).
-  const int per = kRopeThreads >> a.lanes_log2;
+  // A wave does for a token of few values (50,140 tokens of two heads of 64: 32 us,
+  // two waves 47).
+  const int threads = a.n_rows << a.lanes_log2 <= 64 ? 64 : kRopeThreads;
+  const int per = threads >> a.lanes_log2;
   const int split = std::min((a.n_rows + per - 1) / per, std::max(1, kRopeGroups / n_tokens));
-  hipLaunchKernelGGL(rope_kernel<T>, dim3(n_tokens, split), dim3(kRopeThreads), 0,
+  hipLaunchKernelGGL(rope_kernel<T>, dim3(n_tokens, split), dim3(threads), 0,
                      static_cast<hipStream_t>(stream), a);
   return check_launch(nm);
 }
