@@ -63,6 +63,7 @@ struct SlideArgs : AttnArgs {
   const uint16_t *ks, *vs;  // scales of the quantised cache (kc, vc: its codes)
   int reach, sinks;
   int spread;  // how workgroups are mapped to row blocks
+  int turn_units;  // units, as far as the host knows
 };
 enum { kSpreadUnits, kSpreadTurns, kSpreadRuns };
 
@@ -124,10 +125,18 @@ struct SlidePart : Part<D> {
     this->grp = lane >> 4;
     const int id = blockIdx.x;
     if (sa.spread == kSpreadTurns) {
-      // Many row blocks that see all before them: over the XCDs in turn, the
-      // last rows, which see most, first.
-      this->unit = id / sa.row_blocks;
-      this->rb = sa.row_blocks - 1 - (id - this->unit * sa.row_blocks);
+      // Many row blocks that see all before them: over the XCDs in turn, the last
+      // rows of all units, which see most, first, so that short blocks fill up what
+      // long ones leave (4,096 tokens over none, 32 heads on 8 of 128: 159 us, unit
+      // after unit 258).
+      // (units that the host does not count on follow likewise)
+      const int turn = sa.turn_units, run = turn * sa.row_blocks;
+      const bool past = id >= run;
+      const int units = past ? max(sa.max_units - turn, 1) : turn, in = past ? id - run : id;
+      const int row = in / units;
+      this->unit = in - row * units + (past ? turn : 0);
+      this->rb = sa.row_blocks - 1 - row;
+      if (this->rb < 0) return false;  // (behind the last one)
     } else if (sa.spread == kSpreadRuns) {
       // That see a window: an XCD has neighbours, whose windows are the same keys
       // but for a few, and reads them once (4,096 tokens of 32 heads on 8 of 128 over
@@ -169,6 +178,16 @@ struct SlidePart : Part<D> {
     const int v1 = k == this->parts - 1 || from + part > count ? count : static_cast<int>(from + part);
     this->begin = v0 < v1 ? steps.skip(all.at(v0)) : 0;
     this->end = v0 < v1 ? min(all.at(v1 - 1) + 1, steps.high) : 0;
+    return true;
+  }
+  // A part of which the block's rows see no step: says so, and true, for the join.
+  __device__ __forceinline__ bool empty() const {
+    if (this->begin < this->end || this->parts == 1) return false;
+    const slide_p a = cold_slide();
+    const int in = threadIdx.x;
+    if (in < a->block_rows)
+      a->part_ml[(static_cast<long long>(this->unit) * a->row_blocks + this->rb) * a->block_rows + in] =
+          make_float2(0.f, 0.f);
     return true;
   }
   // Where the rows of a cached step's blocks of 16 keys begin, in values.
@@ -361,7 +380,7 @@ __global__ void __launch_bounds__(256, slide_waves(D, RT)) slide_few_kernel(cons
   extern __shared__ __attribute__((aligned(16))) unsigned char lds[];
   const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
   P t(a);
-  if (!t.start(lds)) return;
+  if (!t.start(lds) || t.empty()) return;
   const int lane = t.lane, col = t.col, grp = t.grp, row0 = t.rb * kRows;
   int* rise = reinterpret_cast<int*>(lds + L::kFlags);  // odd and even: 1 + the last step that moves
   float* mx = reinterpret_cast<float*>(lds + L::kMax);
@@ -770,7 +789,7 @@ __global__ void __launch_bounds__(64 * kSlideRowWaves) slide_rows_kernel(const S
   const int blk = wave & 3;
   const bool is_v = wave >= 4;
   P t(a);
-  if (!t.start(lds)) return;
+  if (!t.start(lds) || t.empty()) return;
   const int lane = t.lane, col = t.col, grp = t.grp;
   const int row0 = (t.rb * NW + wave) * 16 * RT;
   int* odds = reinterpret_cast<int*>(lds + L::kFlags);  // whether V had infinities or NaN
@@ -1084,9 +1103,11 @@ __global__ void __launch_bounds__(64 * kSlideRowWaves) slide_rows_kernel(const S
     }
     add_odds<D, Q8>(t, acc, 4 * grp, pos, up);
   }
+  int last_col = col;
+  asm("" : "+v"(last_col));  // (the rows made anew: registers)
 #pragma unroll
   for (int rt = 0; rt < RT; ++rt) {
-    const int r = row0 + rt * 16 + col;
+    const int r = row0 + rt * 16 + last_col;
     l[rt] += __shfl_xor(l[rt], 16);
     l[rt] += __shfl_xor(l[rt], 32);
     const float lt = a.parent && !seen[t.node_of(r)] ? 0.f : l[rt];  // 0: an absent node
@@ -1094,12 +1115,71 @@ __global__ void __launch_bounds__(64 * kSlideRowWaves) slide_rows_kernel(const S
   }
 }
 
+// The parts of many rows, joined as attn_join_kernel does it, which has a workgroup
+// for each row: here D / 4 lanes have a row and read its parts one after the
+// other, those in which it sees something (2,048 tokens of 16 heads of 256 in two
+// to four parts, with no cache: 98 us in all, 147 by a workgroup each).
+template <int D>
+__global__ void __launch_bounds__(256) slide_join_kernel(const AttnArgs a) {
+  constexpr int LP = D / 4, U = 4;  // lanes of a row, parts at once
+  const int per = a.max_window * a.n_heads;
+  const long long x = blockIdx.x * (256LL / LP) + threadIdx.x / LP;
+  const int seq = static_cast<int>(x / per);
+  if (seq >= a.n_seq) return;
+  const int rest = static_cast<int>(x - static_cast<long long>(seq) * per);
+  const int node = rest / a.n_heads, head = rest - node * a.n_heads;
+  const Window w = window_of(a.win_off, seq, a.n_tokens, a.max_window);
+  const int2 plan = a.seq_plan[seq];  // the first unit, the parts
+  if (node >= w.n || plan.y <= 1) return;
+  const int h = head / a.group, r = node * a.group + head - h * a.group;
+  const int rb = r / a.block_rows;
+  const long long at =
+      (static_cast<long long>(plan.x + h * plan.y) * a.row_blocks + rb) * a.block_rows + r -
+      rb * a.block_rows;
+  const long long step = static_cast<long long>(a.row_blocks) * a.block_rows;
+  const int c = threadIdx.x % LP * 4;
+  const float* po = a.part_o + at * D + c;
+  float m = -INFINITY, sum = 0.f;
+  f4 o = (f4){0.f, 0.f, 0.f, 0.f};
+  for (int s0 = 0; s0 < plan.y; s0 += U) {
+    f4 v[U];
+    float2 ml[U];
+#pragma unroll
+    for (int u = 0; u < U; ++u) ml[u] = a.part_ml[at + min(s0 + u, plan.y - 1) * step];
+    float top = m;
+#pragma unroll
+    for (int u = 0; u < U; ++u) {
+      if (s0 + u >= plan.y) ml[u].y = 0.f;
+      top = ml[u].y != 0.f ? fmaxf(top, ml[u].x) : top;
+      v[u] = (f4){0.f, 0.f, 0.f, 0.f};
+      if (ml[u].y != 0.f) v[u] = *reinterpret_cast<const f4*>(po + (s0 + u) * step * D);
+    }
+    const float f0 = m > -INFINITY ? __builtin_amdgcn_exp2f(m - top) : 0.f;
+    sum *= f0;
+    o *= f0;
+#pragma unroll
+    for (int u = 0; u < U; ++u) {
+      const float f = ml[u].y != 0.f ? __builtin_amdgcn_exp2f(ml[u].x - top) : 0.f;
+      sum += ml[u].y != 0.f ? ml[u].y * f : 0.f;
+#pragma unroll
+      for (int i = 0; i < 4; ++i) o[i] += ml[u].y != 0.f ? v[u][i] * f : 0.f;
+    }
+    m = top;
+  }
+  const float inv = sum != 0.f ? 1.f / sum : 0.f;
+  h4 z;
+#pragma unroll
+  for (int j = 0; j < 4; ++j) z[j] = static_cast<_Float16>(o[j] * inv);
+  const long long row = static_cast<long long>(w.off + node) * a.n_heads + head;
+  *reinterpret_cast<h4*>(a.out + row * D + c) = z;
+}
+
 // ---- host -----------------------------------------------------------------------
 
 // How a call is laid out: rows of a workgroup, the most units.
 struct SlideLayout {
   int block_rows, row_blocks, max_units, goal;
-  bool cut;
+  bool cut, by_rows;  // by_rows: how parts are joined
   int spread;
   int few[3];  // the most sequences that are cut for want of work, for two rounds, in few rows
   size_t plan_bytes, o_bytes, bytes;  // of the workspace
@@ -1110,20 +1190,22 @@ static SlideLayout slide_layout(int n_seq, int max_window, int max_len, int grou
   const long long rows = static_cast<long long>(max_window) * group;
   const long long units = static_cast<long long>(n_seq) * n_kv;
   // steps at the most: of a sequence, and of a block of 256 of its rows (a window
-  // that may be a tree lies in every block's reach)
-  auto steps = [&](long long nodes) {
-    const long long keys = static_cast<long long>(max_len) + max_window;
+  // that may be a tree lies in every block's reach); and over the blocks in the mean
+  auto steps = [&](long long before, long long nodes) {
+    const long long keys = static_cast<long long>(max_len) + before;
     const long long near = static_cast<long long>(reach) + nodes + sinks + 2 * kKeys;
     return ((keys < near ? keys : near) + kKeys - 1) / kKeys + 1;
   };
-  const long long most = steps(max_window);
-  const long long own = max_window <= kMaxWindow ? most : steps(256 / group + 1);
+  const bool chain = max_window > kMaxWindow;
+  const long long most = steps(max_window, max_window);
+  const long long own = chain ? steps(max_window, 256 / group + 1) : most;
+  const long long mean = chain ? steps(max_window / 2, 256 / group + 1) : most;
   // 256 rows read a step's keys once and keep the matrix cores busy, but 32 rows
   // spread little work further: by 256 as soon as each CU has two such steps (in
   // us, 32 rows and 256: 32 sequences of 64 nodes, 32 query heads on 8, over 300
   // keys of 128 quantised values 70 and 43, 4 of 32 nodes, 64 on 8, over 32,768
   // 494 and 322; 8 of 64 nodes that reach 128 keys back, 48 on 8, 24 and 32).
-  const long long wide_units = 2 * 256 / ((rows + 255) / 256 * own) + 1;
+  const long long wide_units = 2 * 256 / ((rows + 255) / 256 * mean) + 1;
   const bool wide = rows > 128 && units >= wide_units;
   l.block_rows = wide ? 256 : rows > 16 ? 32 : 16;
   l.row_blocks = static_cast<int>((rows + l.block_rows - 1) / l.block_rows);
@@ -1138,14 +1220,15 @@ static SlideLayout slide_layout(int n_seq, int max_window, int max_len, int grou
   const long long slots = 256 * each;
   const long long per = 32 * each >= l.row_blocks ? 32 * each / l.row_blocks * 8 : 8;
   // Less work than the card holds is cut into parts if that saves more steps than
-  // the parts' way through memory and the join cost, `join` of them; blocks that
-  // see few of their sequence's steps would get empty parts.  More than it holds,
-  // in blocks of few rows, is cut over long caches, so that a ragged batch ends
-  // together.  (28 sequences of up to 210 tokens, 56 query heads on 8 of 128, that
-  // reach 63 keys back: 340 us in parts, 88 whole; 600 batches of mixed shapes:
-  // half and twice `join` cost 2% and 1% more.)
-  const long long join = wide ? dim / 32 + 1 : 8;
-  const long long room = own > join ? slots - slots * join / own : 0;  // of blocks: below it
+  // the parts' way through memory and the join cost, `join` of them (of a chunk's
+  // blocks of 256 rows the last sees `own` steps, all together `mean` a block);
+  // blocks that see few of their sequence's steps would get empty parts.  More than
+  // it holds, in blocks of few rows, is cut over long caches, so that a ragged batch
+  // ends together.  (28 sequences of up to 210 tokens, 56 query heads on 8 of 128,
+  // that reach 63 keys back: 340 us in parts, 88 whole; 600 batches of mixed shapes:
+  // twice `join` costs 1 to 2% more.)
+  const long long join = wide ? dim / 64 + 1 : 8;
+  const long long room = own > join ? slots * (own - join) / (wide ? mean : own) : 0;  // of blocks: below it
   const bool rounds = blocks >= 2 * slots;
   l.cut = own * 2 >= most && (blocks < room || (!wide && blocks >= slots && most > 8));
   const long long a_seq = static_cast<long long>(n_kv) * l.row_blocks;
@@ -1156,7 +1239,10 @@ static SlideLayout slide_layout(int n_seq, int max_window, int max_len, int grou
   long long n = units;
   l.goal = 1;
   if (l.cut && wide) {
-    l.goal = static_cast<int>(slots / l.row_blocks);
+    // (as many as all CUs take, of the blocks that see something of a part; of four
+    // steps or more: 1,024 tokens as below 48 us, 68 with parts of two)
+    const long long goal = slots * own / mean / l.row_blocks, most_goal = units * own / 4;
+    l.goal = static_cast<int>(goal < most_goal ? goal : most_goal > units ? most_goal : units);
     n = l.goal + (n_seq <= 64 ? 0 : units);
   } else if (l.cut && !rounds) {
     n = (2 * units + per - 1) / per * per;
@@ -1166,6 +1252,8 @@ static SlideLayout slide_layout(int n_seq, int max_window, int max_len, int grou
     n = units + per;
     l.goal = static_cast<int>(per - ((per + 1023) >> 10));
   }
+  // many rows of few parts: a workgroup of the join has several rows, one after the other
+  l.by_rows = wide && l.goal < 8 * units;
   l.max_units = n > 0x7FFFFF00 ? 0x7FFFFF00 : static_cast<int>(n);
   const size_t part_rows =
       static_cast<size_t>((l.max_units + 7LL) / 8 * 8) * l.row_blocks * l.block_rows;
@@ -1176,7 +1264,7 @@ static SlideLayout slide_layout(int n_seq, int max_window, int max_len, int grou
 }
 
 template <int D, bool Q8>
-static int slide_launch(const SlideArgs& a, hipStream_t s, const char* nm) {
+static int slide_launch(const SlideArgs& a, bool by_rows, hipStream_t s, const char* nm) {
   const long long n = a.spread == kSpreadUnits ? (a.max_units + 7LL) / 8 * 8 : a.max_units;
   const dim3 grid(static_cast<unsigned>((n * a.row_blocks + 7) / 8 * 8));
   if (a.block_rows == 256)
@@ -1189,8 +1277,14 @@ static int slide_launch(const SlideArgs& a, hipStream_t s, const char* nm) {
     hipLaunchKernelGGL((slide_few_kernel<D, 1, Q8>), grid, dim3(256), (SlideFewLds<D, 1, Q8>::kBytes), s,
                        a);
   if (int st = check_launch(nm)) return st;
+  const long long join = static_cast<long long>(a.n_seq) * a.max_window * a.n_heads;
+  if (a.cut && by_rows) {
+    hipLaunchKernelGGL(slide_join_kernel<D>, dim3(static_cast<unsigned>((join * (D / 4) + 255) / 256)),
+                       dim3(256), 0, s, static_cast<const AttnArgs&>(a));
+    return check_launch(nm);
+  }
   if (a.cut) {
-    hipLaunchKernelGGL(attn_join_kernel<D>, dim3(a.n_seq * a.max_window * a.n_heads),
+    hipLaunchKernelGGL(attn_join_kernel<D>, dim3(static_cast<unsigned>(join)),
                        dim3(kJoinThreads<D>), 0, s, static_cast<const AttnArgs&>(a));
     return check_launch(nm);
   }
@@ -1313,13 +1407,14 @@ static int attn_slide(const uint16_t* q, const uint16_t* k, const uint16_t* v, l
   a.goal = l.goal;
   a.cut = l.cut;
   a.spread = l.spread;
+  a.turn_units = l.max_units / static_cast<int>(units) * static_cast<int>(units);
   a.scale_log2 = scale * kLog2e;
   a.reach = far;
   a.sinks = sinks;
   const hipStream_t s = static_cast<hipStream_t>(stream);
-  if (dim == 64) return slide_launch<64, kQ8>(a, s, nm);
-  if (dim == 128) return slide_launch<128, kQ8>(a, s, nm);
-  return slide_launch<256, kQ8>(a, s, nm);
+  if (dim == 64) return slide_launch<64, kQ8>(a, l.by_rows, s, nm);
+  if (dim == 128) return slide_launch<128, kQ8>(a, l.by_rows, s, nm);
+  return slide_launch<256, kQ8>(a, l.by_rows, s, nm);
 }
 
 }  // namespace sg

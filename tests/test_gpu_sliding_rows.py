@@ -12,33 +12,36 @@ pytestmark = pytest.mark.gpu
 
 
 def wide(c, max_len=None):
-    """Whether the call is laid out in blocks of 256 rows, and whether it may be cut."""
+    """Whether the call is laid out in blocks of 256 rows, whether it is cut, and into how many units."""
     T, heads, D = c["q"].shape
     n_kv, n_seq, window = c["k"].shape[1], len(c["off"]) - 1, c["max_window"]
     group = heads // n_kv
     max_len = c["max_len"] if max_len is None else max_len
 
-    def steps(nodes):
+    def steps(before, nodes):
         near = (c["reach"] or 1 << 31) + nodes + c["sinks"] + 128
-        return (min(max_len + window, near) + 63) // 64 + 1
+        return (min(max_len + before, near) + 63) // 64 + 1
 
-    own = steps(window) if window <= 64 else steps(256 // group + 1)
-    blocks = -(-window * group // 256)
-    join = D // 32 + 1
-    room = 256 - 256 * join // own if own > join else 0
-    return window * group > 128 and n_seq * n_kv * blocks * own >= 512 + own * blocks, \
-        own * 2 >= steps(window) and n_seq * n_kv * blocks < room
+    most = own = mean = steps(window, window)
+    if window > 64:
+        own, mean = steps(window, 256 // group + 1), steps(window // 2, 256 // group + 1)
+    row_blocks, units = -(-window * group // 256), n_seq * n_kv
+    join = D // 64 + 1
+    room = 256 * (own - join) // mean if own > join else 0
+    return window * group > 128 and units >= 512 // (row_blocks * mean) + 1, \
+        own * 2 >= most and units * row_blocks < room, \
+        max(units, min(256 * own // mean // row_blocks, units * own // 4))
 
 
 def whole(seed, sizes, lengths, *args, **kw):
     """With 600 empty sequences behind the first."""
     c = sl.case(seed, list(sizes) + [0] * 600, list(lengths) + [0] * 600, *args, **kw)
-    assert wide(c) == (True, False)
+    assert wide(c)[:2] == (True, False)
     return sl.check(c)
 
 
 def cut(c, max_len=10 ** 6):
-    assert wide(c, max_len) == (True, True)
+    assert wide(c, max_len)[:2] == (True, True)
     return sl.check(c, max_len)
 
 
@@ -72,6 +75,27 @@ def test_parts(q8, D, n_kv, group):
     cut(sl.case(D, [0] * 33 + [90] + [0] * 31 + [3], [0] * 33 + [900] + [0] * 31 + [2000], 1, group, D,
                 16, q8=q8, chain=True))
     cut(sl.case(D, [64] * 3, [1200, 3000, 0], n_kv, 8, D, 16, q8=q8, branch=2, reach=9000, sinks=4))
+
+
+@pytest.mark.parametrize("q8", [False, True])
+@pytest.mark.parametrize("D", [64, 128, 256])
+def test_few_parts_of_many_rows(q8, D):
+    """So few that a workgroup joins several rows; parts of which some blocks see nothing."""
+    for c in (sl.case(D, [150, 70, 1, 0, 149], [0, 900, 2000, 5, 64], 4, 2, D, 64, q8=q8, chain=True, pad=1),
+              sl.case(D, [64, 20, 0, 33, 1], [700, 65, 9, 0, 1500], 4, 8, D, 32, q8=q8, branch=2, absent=True)):
+        assert wide(c, 10 ** 6)[2] < 8 * 20
+        cut(c)
+    c = sl.case(D, [1000], [0], 2, 8, D, 16, q8=q8, chain=True)
+    assert wide(c) == (True, True, 8)
+    sl.check(c)
+
+
+@pytest.mark.parametrize("q8", [False, True])
+def test_more_units_than_the_host_counts_on(q8):
+    """Two sequences of 10 and 15 steps, 25 units of one step, in turn by their last rows."""
+    c = sl.case(4, [300, 270], [300, 640], 1, 8, 128, 32, q8=q8, chain=True, pad=2)
+    assert wide(c, 10 ** 6)[2] == 25
+    cut(c)
 
 
 @pytest.mark.parametrize("q8", [False, True])
