@@ -134,7 +134,8 @@ struct SlidePart : Part<D> {
       const bool past = id >= run;
       const int units = past ? max(sa.max_units - turn, 1) : turn, in = past ? id - run : id;
       const int row = in / units;
-      this->unit = in - row * units + (past ? turn : 0);
+      int k = in - row * units;
+      this->unit = k + (past ? turn : 0);
       this->rb = sa.row_blocks - 1 - row;
       if (this->rb < 0) return false;  // (behind the last one)
     } else if (sa.spread == kSpreadRuns) {
@@ -1211,7 +1212,6 @@ static SlideLayout slide_layout(int n_seq, int max_window, int max_len, int grou
   l.row_blocks = static_cast<int>((rows + l.block_rows - 1) / l.block_rows);
   const long long blocks = units * l.row_blocks;
   const bool near_only = reach / 2 < max_len / 2 + max_window / 2;
-  l.spread = l.row_blocks < 8 ? kSpreadUnits : near_only ? kSpreadRuns : kSpreadTurns;
   // workgroups that the card holds at once, and units of them (32 sequences of
   // one token and of five over 4,000 quantised ones, 8 kv heads of 128: 59.8 and
   // 69.4 us by 3 a CU, 62.0 and 80.0 by 4, 58.6 and 72.6 by 2; of 64: 41 us by
@@ -1231,6 +1231,13 @@ static SlideLayout slide_layout(int n_seq, int max_window, int max_len, int grou
   const long long room = own > join ? slots * (own - join) / (wide ? mean : own) : 0;  // of blocks: below it
   const bool rounds = blocks >= 2 * slots;
   l.cut = own * 2 >= most && (blocks < room || (!wide && blocks >= slots && most > 8));
+  // (blocks of 256 rows: as many parts as all CUs take, of the blocks that see something
+  // of a part; of four steps or more: 1,024 tokens over none, 16 heads on 2 of 256, 48
+  // us, 68 with parts of two)
+  const long long all_goal = slots * own / mean / l.row_blocks, most_goal = units * own / 4;
+  const long long wide_goal = all_goal < most_goal ? all_goal : most_goal > units ? most_goal : units;
+  if (wide && n_seq == 1 && wide_goal < 2 * units) l.cut = false;  // (it would not come to it)
+  l.spread = l.row_blocks < 8 ? kSpreadUnits : near_only && !l.cut ? kSpreadRuns : kSpreadTurns;
   const long long a_seq = static_cast<long long>(n_kv) * l.row_blocks;
   l.few[0] = static_cast<int>(room > 0 ? (room - 1) / a_seq : 0);
   l.few[1] = static_cast<int>((2 * slots - 1) / a_seq);
@@ -1239,10 +1246,7 @@ static SlideLayout slide_layout(int n_seq, int max_window, int max_len, int grou
   long long n = units;
   l.goal = 1;
   if (l.cut && wide) {
-    // (as many as all CUs take, of the blocks that see something of a part; of four
-    // steps or more: 1,024 tokens as below 48 us, 68 with parts of two)
-    const long long goal = slots * own / mean / l.row_blocks, most_goal = units * own / 4;
-    l.goal = static_cast<int>(goal < most_goal ? goal : most_goal > units ? most_goal : units);
+    l.goal = static_cast<int>(wide_goal);
     n = l.goal + (n_seq <= 64 ? 0 : units);
   } else if (l.cut && !rounds) {
     n = (2 * units + per - 1) / per * per;

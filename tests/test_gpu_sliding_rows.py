@@ -114,6 +114,8 @@ def test_many_row_blocks(q8, reach):
     c = sl.case(8, [300, 270], [129, 700], 1, 8, 128, 32, **kw)
     if reach == 0:
         cut(c)
+    else:
+        cut(sl.case(9, [300, 290, 0], [129, 17, 3], 4, 8, 128, 32, q8=q8, chain=True, reach=200, sinks=4), 129)
 
 
 @pytest.mark.parametrize("group", [8, 16])
