@@ -771,7 +771,7 @@ constexpr int kSlideRowWaves = 8, kSlideRowTiles = 2;  // 16-row tiles of a wave
 // the matrix cores, whose operands and scores are waited for by no more than two
 // waves a SIMD (4,096 tokens over 4,099 more, windows of 2,048: 16 heads on 2 of
 // 256 155 to 190 us, 890 to 730 TFLOP/s, quantised 280, as the products with the
-// cache are twice as many; 32 heads on 8 of 128 187 us and 250).
+// cache are twice as many; 32 heads on 8 of 128 187 to 210 us and 250 to 265).
 template <int D, bool Q8>
 __global__ void __launch_bounds__(64 * kSlideRowWaves) slide_rows_kernel(const SlideArgs a) {
   typedef SlidePart<D> P;
