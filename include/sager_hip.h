@@ -687,7 +687,8 @@ int sg_kv_read_q8(const sg_kv_cache_q8* cache, const int* first, const int* row_
  * that commit and append write, or is not a number.  The rest is as for
  * sg_attn_tree_f16.
  * Workspace: sg_attn_sliding_workspace_bytes of as many sequences or more, of
- * the same reach and sinks. */
+ * max_window and max_len as large or larger, and of the same heads, reach and
+ * sinks. */
 size_t sg_attn_sliding_workspace_bytes(int n_seq, int max_window, int max_len, int n_heads,
                                        int n_kv_heads, int head_dim, int reach, int sinks);
 int sg_attn_sliding_f16(const uint16_t* q, const uint16_t* k, const uint16_t* v, long long q_stride,

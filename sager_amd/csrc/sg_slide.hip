@@ -27,6 +27,8 @@
 // full such values are 0 in the product; if there were any, they are added at
 // the end to the rows that see them (what they are multiplied by does not
 // matter any more).
+#include <algorithm>
+#include <climits>
 #include <type_traits>
 
 #include "sg_attn.hpp"
@@ -1177,12 +1179,32 @@ __global__ void __launch_bounds__(256) slide_join_kernel(const AttnArgs a) {
 
 // ---- host -----------------------------------------------------------------------
 
+// Steps at the most: of `nodes` tokens in line that see each other and `before` of the window.
+static long long slide_steps(int max_len, int reach, int sinks, long long before, long long nodes) {
+  const long long keys = static_cast<long long>(max_len) + before;
+  const long long near = static_cast<long long>(reach) + nodes + sinks + 2 * kKeys;
+  return ((keys < near ? keys : near) + kKeys - 1) / kKeys + 1;
+}
+// Workgroups of few rows that a CU holds at once, and units of `row_blocks` of
+// them that the card does, an XCD's 32 CUs with whole ones (32 sequences of one
+// token and of five over 4,000 quantised ones, 8 kv heads of 128: 59.8 and 69.4
+// us by 3 a CU, 62.0 and 80.0 by 4, 58.6 and 72.6 by 2; of 64: 41 us by 4, 48 by
+// 2; four tokens over 131,071, 2 kv heads of 256: 43.8 by 2, 58.3 by 4).
+static int slide_few_each(int dim) { return dim == 256 ? 2 : dim == 128 ? 3 : 4; }
+static long long slide_units(int each, long long row_blocks) {
+  return 32 * each >= row_blocks ? 32 * each / row_blocks * 8 : 8;
+}
+static int slide_join_steps(int dim) { return dim / 64 + 1; }  // what a join of wide blocks costs
+constexpr int kFewJoinSteps = 8;                               // of blocks of few rows
+static size_t slide_plan_bytes(int n_seq) {
+  return (static_cast<size_t>(n_seq) * sizeof(int2) + 15) / 16 * 16;
+}
+
 // How a call is laid out: rows of a workgroup, the most units.
 struct SlideLayout {
   int block_rows, row_blocks, max_units, goal;
   bool cut, by_rows;  // by_rows: how parts are joined
   int spread;
-  int few[3];  // the most sequences that are cut for want of work, for two rounds, in few rows
   size_t plan_bytes, o_bytes, bytes;  // of the workspace
 };
 static SlideLayout slide_layout(int n_seq, int max_window, int max_len, int group, int n_kv, int dim,
@@ -1193,9 +1215,7 @@ static SlideLayout slide_layout(int n_seq, int max_window, int max_len, int grou
   // steps at the most: of a sequence, and of a block of 256 of its rows (a window
   // that may be a tree lies in every block's reach); and over the blocks in the mean
   auto steps = [&](long long before, long long nodes) {
-    const long long keys = static_cast<long long>(max_len) + before;
-    const long long near = static_cast<long long>(reach) + nodes + sinks + 2 * kKeys;
-    return ((keys < near ? keys : near) + kKeys - 1) / kKeys + 1;
+    return slide_steps(max_len, reach, sinks, before, nodes);
   };
   const bool chain = max_window > kMaxWindow;
   const long long most = steps(max_window, max_window);
@@ -1212,13 +1232,10 @@ static SlideLayout slide_layout(int n_seq, int max_window, int max_len, int grou
   l.row_blocks = static_cast<int>((rows + l.block_rows - 1) / l.block_rows);
   const long long blocks = units * l.row_blocks;
   const bool near_only = reach / 2 < max_len / 2 + max_window / 2;
-  // workgroups that the card holds at once, and units of them (32 sequences of
-  // one token and of five over 4,000 quantised ones, 8 kv heads of 128: 59.8 and
-  // 69.4 us by 3 a CU, 62.0 and 80.0 by 4, 58.6 and 72.6 by 2; of 64: 41 us by
-  // 4, 48 by 2; four tokens over 131,071, 2 kv heads of 256: 43.8 by 2, 58.3 by 4)
-  const int each = wide ? 1 : dim == 256 ? 2 : dim == 128 ? 3 : 4;
+  // workgroups that the card holds at once, and units of them
+  const int each = wide ? 1 : slide_few_each(dim);
   const long long slots = 256 * each;
-  const long long per = 32 * each >= l.row_blocks ? 32 * each / l.row_blocks * 8 : 8;
+  const long long per = slide_units(each, l.row_blocks);
   // Less work than the card holds is cut into parts if that saves more steps than
   // the parts' way through memory and the join cost, `join` of them (of a chunk's
   // blocks of 256 rows the last sees `own` steps, all together `mean` a block);
@@ -1227,10 +1244,10 @@ static SlideLayout slide_layout(int n_seq, int max_window, int max_len, int grou
   // ends together.  (28 sequences of up to 210 tokens, 56 query heads on 8 of 128,
   // that reach 63 keys back: 340 us in parts, 88 whole; 600 batches of mixed shapes:
   // twice `join` costs 1 to 2% more.)
-  const long long join = wide ? dim / 64 + 1 : 8;
+  const long long join = wide ? slide_join_steps(dim) : kFewJoinSteps;
   const long long room = own > join ? slots * (own - join) / (wide ? mean : own) : 0;  // of blocks: below it
   const bool rounds = blocks >= 2 * slots;
-  l.cut = own * 2 >= most && (blocks < room || (!wide && blocks >= slots && most > 8));
+  l.cut = own * 2 >= most && (blocks < room || (!wide && blocks >= slots && most > kFewJoinSteps));
   // (blocks of 256 rows: as many parts as all CUs take, of the blocks that see something
   // of a part; of four steps or more: 1,024 tokens over none, 16 heads on 2 of 256, 48
   // us, 68 with parts of two)
@@ -1238,11 +1255,6 @@ static SlideLayout slide_layout(int n_seq, int max_window, int max_len, int grou
   const long long wide_goal = all_goal < most_goal ? all_goal : most_goal > units ? most_goal : units;
   if (wide && n_seq == 1 && wide_goal < 2 * units) l.cut = false;  // (it would not come to it)
   l.spread = l.row_blocks < 8 ? kSpreadUnits : near_only && !l.cut ? kSpreadRuns : kSpreadTurns;
-  const long long a_seq = static_cast<long long>(n_kv) * l.row_blocks;
-  l.few[0] = static_cast<int>(room > 0 ? (room - 1) / a_seq : 0);
-  l.few[1] = static_cast<int>((2 * slots - 1) / a_seq);
-  const long long narrow = (wide_units - 1) / n_kv;  // the most sequences in blocks of few rows
-  l.few[2] = static_cast<int>(wide ? narrow : 0);
   long long n = units;
   l.goal = 1;
   if (l.cut && wide) {
@@ -1261,10 +1273,65 @@ static SlideLayout slide_layout(int n_seq, int max_window, int max_len, int grou
   l.max_units = n > 0x7FFFFF00 ? 0x7FFFFF00 : static_cast<int>(n);
   const size_t part_rows =
       static_cast<size_t>((l.max_units + 7LL) / 8 * 8) * l.row_blocks * l.block_rows;
-  l.plan_bytes = l.cut ? (static_cast<size_t>(n_seq) * sizeof(int2) + 15) / 16 * 16 : 0;
+  l.plan_bytes = l.cut ? slide_plan_bytes(n_seq) : 0;
   l.o_bytes = l.cut ? part_rows * dim * sizeof(float) : 0;
   l.bytes = l.plan_bytes + l.o_bytes + (l.cut ? part_rows * sizeof(float2) : 0);
   return l;
+}
+
+// Bytes that no layout of at most n_seq sequences, windows of max_window and caches of max_len
+// passes: a smaller call may be cut where a larger one is not, into more parts of more row blocks.
+// So all numbers of row blocks are gone through, each with the most units that slide_layout has of it.
+static size_t slide_workspace(int n_seq, int max_window, int max_len, int group, int n_kv, int dim,
+                              int reach, int sinks) {
+  const long long rows = static_cast<long long>(max_window) * group;
+  const long long near = std::min(max_window, kMaxWindow);  // of what may be a tree
+  auto steps = [&](int len, long long before, long long nodes) {
+    return slide_steps(len, reach, sinks, before, nodes);
+  };
+  long long part_rows = 0;
+  auto take = [&](long long units, long long row_blocks, int block_rows) {
+    part_rows = std::max(part_rows, (units + 7) / 8 * 8 * row_blocks * block_rows);
+  };
+  // Blocks of few rows.  Over 128 rows they have no more than 512 steps of 256 rows, those of
+  // the mean row over no cache at the least.
+  const long long in_line = std::max(max_window, 256 / group + 1);  // (a chain's block may count more)
+  if (steps(max_len, max_window, in_line) > kFewJoinSteps) {
+    const int each = slide_few_each(dim), block = rows > 16 ? 32 : 16;
+    for (long long rb = (group + block - 1) / block; rb <= (rows + block - 1) / block; ++rb) {
+      const long long least = (rb - 1) * block + 1, nodes = (least + group - 1) / group;
+      const long long per = slide_units(each, rb);
+      long long n = n_seq;
+      if (least > 128) {
+        long long mean = nodes > kMaxWindow ? LLONG_MAX : steps(0, nodes, nodes);
+        if (max_window > kMaxWindow) {
+          const long long w = std::max(nodes, kMaxWindow + 1LL);
+          mean = std::min(mean, steps(0, w / 2, 256 / group + 1));
+        }
+        n = std::min(n, 512 / ((least + 255) / 256 * mean) / n_kv);
+        if (n == 0) break;
+      }
+      const long long two = (2 * 256 * each - 1) / rb / n_kv;  // less than two rounds
+      if (const long long few = std::min(n, two)) take((2 * few * n_kv + per - 1) / per * per, rb, block);
+      if (n > two) take(n * n_kv + per, rb, block);
+    }
+  }
+  // Blocks of 256 rows: fewer than CUs times the last block's steps over the mean's, which is
+  // two at the most in a chain and one in what may be a tree.
+  for (long long rb = (group + 255) / 256; rows > 128 && rb <= (rows + 255) / 256; ++rb) {
+    const long long w = std::min<long long>(rb * 256 / group, max_window);
+    const long long quota = w > kMaxWindow ? 512 : 256;
+    long long own = steps(max_len, std::min(w, near), std::min(w, near));
+    if (w > kMaxWindow) own = std::max(own, steps(max_len, w, 256 / group + 1));
+    const long long n = std::min<long long>((quota - 1) / rb / n_kv, n_seq), units = n * n_kv;
+    if (n == 0) break;
+    const long long goal = std::min(quota / rb, std::max(units * own / 4, units));
+    if (own > slide_join_steps(dim) && (n > 1 || goal >= 2 * units))
+      take(goal + (n > 64 ? units : 0), rb, 256);
+  }
+  return part_rows == 0 ? 0
+                        : slide_plan_bytes(n_seq) +
+                              static_cast<size_t>(part_rows) * (dim * sizeof(float) + sizeof(float2));
 }
 
 template <int D, bool Q8>
@@ -1430,24 +1497,8 @@ size_t sg_attn_sliding_workspace_bytes(int n_seq, int max_window, int max_len, i
   if (n_seq <= 0 || max_window <= 0 || max_len < 0 || n_kv_heads <= 0 || n_heads <= 0 ||
       n_heads % n_kv_heads != 0 || reach < 0 || sinks < 0)
     return 0;
-  // Enough for every smaller batch too: within a way of cutting fewer sequences
-  // have no more units, but fewer may be cut where more are not.
-  const int group = n_heads / n_kv_heads, far = reach == 0 ? 0x7FFFFFFF : reach;
-  auto layout = [&](int n) {
-    return sg::slide_layout(n, max_window, max_len, group, n_kv_heads, head_dim, far, sinks);
-  };
-  size_t bytes = 0;
-  for (int n = n_seq; n > 0;) {
-    const sg::SlideLayout l = layout(n);
-    bytes = l.bytes > bytes ? l.bytes : bytes;
-    for (int i = 0; i < 2; ++i)
-      if (l.few[i] > 0 && l.few[i] < n) {
-        const size_t few = layout(l.few[i]).bytes;
-        bytes = few > bytes ? few : bytes;
-      }
-    n = l.few[2];
-  }
-  return bytes;
+  return sg::slide_workspace(n_seq, max_window, max_len, n_heads / n_kv_heads, n_kv_heads, head_dim,
+                             reach == 0 ? 0x7FFFFFFF : reach, sinks);
 }
 
 int sg_attn_sliding_f16(const uint16_t* q, const uint16_t* k, const uint16_t* v, long long q_stride,
