@@ -556,7 +556,8 @@ typedef struct sg_kv_cache {
  * their sum only).  max_len bounds the caches'
  * lengths for the choice of the launches; longer caches are right, but may
  * be slower.  Workspace: sg_attn_tree_workspace_bytes of as many sequences or
- * more (it may be 0 bytes); it belongs to one call at a time.  One launch, or
+ * more, of max_window and max_len as large or larger (it may be 0 bytes); it
+ * belongs to one call at a time.  One launch, or
  * two where the caches are cut into parts. */
 size_t sg_attn_tree_workspace_bytes(int n_seq, int max_window, int max_len, int n_heads,
                                     int n_kv_heads, int head_dim);

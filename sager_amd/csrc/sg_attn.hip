@@ -26,6 +26,8 @@
 // rounding, down to 2^-22 of the largest; below it 2^-33 of the largest, so
 // that smaller weights bring nothing (131,072 keys that all have just that
 // little together 2^-16).  l = sum p is fp32, of the unrounded p.
+#include <algorithm>
+
 #include "sg_attn.hpp"
 
 namespace sg {
@@ -637,17 +639,20 @@ size_t sg_attn_tree_workspace_bytes(int n_seq, int max_window, int max_len, int 
   if (n_seq <= 0 || max_window <= 0 || max_len < 0 || n_kv_heads <= 0 ||
       n_heads <= 0 || n_heads % n_kv_heads != 0)
     return 0;
-  // Enough for every smaller batch too: within a way of cutting fewer sequences
-  // have no more units, but fewer may be cut where more are not.
+  // Enough for every smaller call too: within a way of cutting fewer sequences
+  // have no more units, but fewer may be cut where more are not, and parts of
+  // fewer row blocks may be more of them.  (A shorter cache is cut no sooner.)
   const int group = n_heads / n_kv_heads;
-  const sg::Layout l = sg::attn_layout(n_seq, max_window, max_len, group, n_kv_heads, head_dim);
-  size_t bytes = l.bytes;
-  for (int few : l.few)
-    if (few > 0 && few < n_seq) {
-      const size_t b =
-          sg::attn_layout(few, max_window, max_len, group, n_kv_heads, head_dim).bytes;
-      bytes = b > bytes ? b : bytes;
-    }
+  auto layout = [&](int n, int window) {
+    return sg::attn_layout(n, window, max_len, group, n_kv_heads, head_dim);
+  };
+  size_t bytes = 0;
+  for (int window = std::min(max_window, sg::kMaxWindow); window > 0; --window) {
+    const sg::Layout l = layout(n_seq, window);
+    bytes = std::max(bytes, l.bytes);
+    for (int few : l.few)
+      if (few > 0 && few < n_seq) bytes = std::max(bytes, layout(few, window).bytes);
+  }
   return bytes;
 }
 

@@ -45,6 +45,12 @@ class Sliding:
         return int(re.search(r"needs (\d+) bytes", said)[1])
 
 
+class Tree(Sliding):
+    def __init__(self, lib, n_kv, group, D, *_):
+        super().__init__(lib, n_kv, group, D, 0, 0)
+        self.entry, self.size, self.more = lib.sg_attn_tree_f16, lib.sg_attn_tree_workspace_bytes, ()
+
+
 def spread(rng, most):  # from 1 on, over the logarithm
     return round(2 ** rng.uniform(0, math.log2(most)))
 
@@ -72,5 +78,20 @@ def test_sliding(lib, seed):
             less = spread(rng, most[0]), spread(rng, most[1]), spread(rng, most[2] + 1) - 1
             for call in (less, (less[0], most[1], less[2]), (most[0], less[1], most[2]),
                          (most[0], less[1], 0)):
+                assert c.need(*call, given) is None, (c.__dict__, most, call)
+                assert c.bytes(*call) <= given, (c.__dict__, most, call)
+
+
+@pytest.mark.parametrize("seed", range(8))
+def test_trees(lib, seed):
+    rng = random.Random(100 + seed)
+    for _ in range(1500):
+        c = Tree(lib, rng.choice([1, 2, 3, 4, 5, 7, 8, 16]), rng.choice([1, 2, 3, 4, 5, 7, 8, 16, 40]),
+                 rng.choice([64, 128, 256]))
+        most = spread(rng, 700), spread(rng, 64), spread(rng, 300000) - 1
+        given = c.bytes(*most)
+        for _ in range(12):
+            less = spread(rng, most[0]), spread(rng, most[1]), spread(rng, most[2] + 1) - 1
+            for call in (less, (most[0], less[1], most[2]), (most[0], most[1], less[2])):
                 assert c.need(*call, given) is None, (c.__dict__, most, call)
                 assert c.bytes(*call) <= given, (c.__dict__, most, call)
