@@ -1334,32 +1334,42 @@ static size_t slide_workspace(int n_seq, int max_window, int max_len, int group,
                               static_cast<size_t>(part_rows) * (dim * sizeof(float) + sizeof(float2));
 }
 
+// Workgroups of the launches, and their threads.
+static long long slide_grid(const SlideLayout& l) {
+  const long long n = l.spread == kSpreadUnits ? (l.max_units + 7LL) / 8 * 8 : l.max_units;
+  return (n * l.row_blocks + 7) / 8 * 8;
+}
+static int slide_threads(const SlideLayout& l) {
+  return l.block_rows == 256 ? 64 * kSlideRowWaves : 256;
+}
+static long long slide_join_groups(const SlideLayout& l, long long rows, int dim) {
+  return l.by_rows ? (rows * (dim / 4) + 255) / 256 : rows;
+}
+static int slide_join_threads(const SlideLayout& l, int dim) { return l.by_rows ? 256 : 2 * dim; }
+
 template <int D, bool Q8>
-static int slide_launch(const SlideArgs& a, bool by_rows, hipStream_t s, const char* nm) {
-  const long long n = a.spread == kSpreadUnits ? (a.max_units + 7LL) / 8 * 8 : a.max_units;
-  const dim3 grid(static_cast<unsigned>((n * a.row_blocks + 7) / 8 * 8));
+static int slide_launch(const SlideArgs& a, const SlideLayout& l, hipStream_t s, const char* nm) {
+  static_assert(kJoinThreads<D> == 2 * D, "the limit of the join's launch counts on it");
+  const dim3 grid(static_cast<unsigned>(slide_grid(l))), threads(slide_threads(l));
   if (a.block_rows == 256)
-    hipLaunchKernelGGL((slide_rows_kernel<D, Q8>), grid, dim3(64 * kSlideRowWaves),
+    hipLaunchKernelGGL((slide_rows_kernel<D, Q8>), grid, threads,
                        SlideRowsLds<D>::kBytes, s, a);
   else if (a.block_rows == 32)
-    hipLaunchKernelGGL((slide_few_kernel<D, 2, Q8>), grid, dim3(256), (SlideFewLds<D, 2, Q8>::kBytes), s,
+    hipLaunchKernelGGL((slide_few_kernel<D, 2, Q8>), grid, threads, (SlideFewLds<D, 2, Q8>::kBytes), s,
                        a);
   else
-    hipLaunchKernelGGL((slide_few_kernel<D, 1, Q8>), grid, dim3(256), (SlideFewLds<D, 1, Q8>::kBytes), s,
+    hipLaunchKernelGGL((slide_few_kernel<D, 1, Q8>), grid, threads, (SlideFewLds<D, 1, Q8>::kBytes), s,
                        a);
   if (int st = check_launch(nm)) return st;
-  const long long join = static_cast<long long>(a.n_seq) * a.max_window * a.n_heads;
-  if (a.cut && by_rows) {
-    hipLaunchKernelGGL(slide_join_kernel<D>, dim3(static_cast<unsigned>((join * (D / 4) + 255) / 256)),
-                       dim3(256), 0, s, static_cast<const AttnArgs&>(a));
-    return check_launch(nm);
-  }
-  if (a.cut) {
-    hipLaunchKernelGGL(attn_join_kernel<D>, dim3(static_cast<unsigned>(join)),
-                       dim3(kJoinThreads<D>), 0, s, static_cast<const AttnArgs&>(a));
-    return check_launch(nm);
-  }
-  return SG_OK;
+  if (!l.cut) return SG_OK;
+  const long long rows = static_cast<long long>(a.n_seq) * a.max_window * a.n_heads;
+  const dim3 groups(static_cast<unsigned>(slide_join_groups(l, rows, D)));
+  const dim3 of(slide_join_threads(l, D));
+  if (l.by_rows)
+    hipLaunchKernelGGL(slide_join_kernel<D>, groups, of, 0, s, static_cast<const AttnArgs&>(a));
+  else
+    hipLaunchKernelGGL(attn_join_kernel<D>, groups, of, 0, s, static_cast<const AttnArgs&>(a));
+  return check_launch(nm);
 }
 
 // What the cache is apart from its tables: whether out lies over it, and its layer.
@@ -1420,20 +1430,23 @@ static int attn_slide(const uint16_t* q, const uint16_t* k, const uint16_t* v, l
   // (a few tokens' rows are reached by 32-bit offsets)
   if (k_stride >= 1LL << 27 || v_stride >= 1LL << 27)
     return set_error(SG_ERR_UNSUPPORTED, "%s: a token stride of 2^27 or more", nm);
+  // each launch has less than 2^32 threads (windows of max_window count, whether they are there
+  // or not), each of which looks through the sequences; a window's rows are 32-bit
   const long long units = static_cast<long long>(n_seq) * n_kv;
-  const long long join = static_cast<long long>(n_seq) * max_window * n_heads;
   const long long rows = static_cast<long long>(max_window) * (n_heads / n_kv);
-  // a launch has less than 2^32 threads, two units to a kv head; rows are 32-bit
-  if (rows > 0x7FFFF000LL || units * (rows / 16 + 1) > 0x1FFFFF || join * 2 * dim > 0xFFFFFFFFLL)
+  if (rows > 0x7FFFF000LL || units > 0x1FFFFF)
+    return set_error(SG_ERR_UNSUPPORTED, "%s: too many sequences, or too long windows", nm);
+  const int far = reach == 0 ? 0x7FFFFFFF : reach;
+  const SlideLayout l =
+      slide_layout(n_seq, max_window, max_len, n_heads / n_kv, n_kv, dim, far, sinks);
+  if (slide_grid(l) > 0xFFFFFFFFLL / slide_threads(l) ||
+      (l.cut && slide_join_groups(l, units * rows, dim) > 0xFFFFFFFFLL / slide_join_threads(l, dim)))
     return set_error(SG_ERR_UNSUPPORTED, "%s: too many sequences, or too long windows", nm);
   const long long last = n_tokens - 1, n_out = static_cast<long long>(n_tokens) * n_heads * dim;
   if (overlap(out, n_out, q, last * q_stride + n_heads * dim) ||
       overlap(out, n_out, k, last * k_stride + n_kv * dim) ||
       overlap(out, n_out, v, last * v_stride + n_kv * dim))
     return set_error(SG_ERR_INVALID_ARGUMENT, "%s: out overlaps q, k or v", nm);
-  const int far = reach == 0 ? 0x7FFFFFFF : reach;
-  const SlideLayout l =
-      slide_layout(n_seq, max_window, max_len, n_heads / n_kv, n_kv, dim, far, sinks);
   if (l.bytes && (!ws || ws_bytes < l.bytes || reinterpret_cast<uintptr_t>(ws) % 16))
     return set_error(SG_ERR_INVALID_ARGUMENT, "%s: the workspace needs %zu bytes, 16-B aligned", nm,
                      l.bytes);
@@ -1483,9 +1496,9 @@ static int attn_slide(const uint16_t* q, const uint16_t* k, const uint16_t* v, l
   a.reach = far;
   a.sinks = sinks;
   const hipStream_t s = static_cast<hipStream_t>(stream);
-  if (dim == 64) return slide_launch<64, kQ8>(a, l.by_rows, s, nm);
-  if (dim == 128) return slide_launch<128, kQ8>(a, l.by_rows, s, nm);
-  return slide_launch<256, kQ8>(a, l.by_rows, s, nm);
+  if (dim == 64) return slide_launch<64, kQ8>(a, l, s, nm);
+  if (dim == 128) return slide_launch<128, kQ8>(a, l, s, nm);
+  return slide_launch<256, kQ8>(a, l, s, nm);
 }
 
 }  // namespace sg
