@@ -103,6 +103,24 @@ static inline int check_cache(const sg_kv_cache_q8* c, int n_seq, int n_tokens, 
   return SG_OK;
 }
 
+// Whether n ints lie over one of `layers` layers of `rows` rows of `width` values, `stride` apart
+// (width or more), `layer` from one layer to the next; what lies between rows is nobody's.
+template <typename T>
+static inline bool over_rows(const int* ints, long long n, const T* x, long long width,
+                             long long stride, long long rows, long long layer, int layers) {
+  for (int l = 0; ints && l < layers; ++l) {
+    const T* const base = x + l * layer;
+    if (!overlap(ints, n, base, (rows - 1) * stride + width)) continue;
+    const long long s = stride * static_cast<long long>(sizeof(T));
+    const long long w = width * static_cast<long long>(sizeof(T));
+    const long long from = static_cast<long long>(reinterpret_cast<uintptr_t>(ints)) -
+                           static_cast<long long>(reinterpret_cast<uintptr_t>(base));
+    const long long row = from < w ? 0 : (from - w) / s + 1;  // the first that ends behind them
+    if (row < rows && row * s < from + n * static_cast<long long>(sizeof(int))) return true;
+  }
+  return false;
+}
+
 // Values from a cache's first to its last layer's end.
 static inline long long cache_values(const sg_kv_cache_q8* c) {
   return (c->n_layers - 1) * c->layer_stride +

@@ -194,15 +194,14 @@ static int store_q8(const uint16_t* k, const uint16_t* v, long long k_stride, lo
     return set_error(SG_ERR_UNSUPPORTED, "%s: n_seq=%d n_layers=%d max_window=%d n_kv_heads=%d", nm,
                      n_seq, cache->n_layers, max_window, cache->n_kv_heads);
   // (a sequence's first workgroup writes its new length, the others read on)
-  const long long far = n_tokens - 1LL, layers = cache->n_layers - 1LL;
   const long long paths = static_cast<long long>(n_seq) * max_window;
   const long long pages = static_cast<long long>(n_seq) * cache->pages_per_seq;
   if (length_out &&
       (overlap(length_out, n_seq, cache->length, n_seq) || overlap(length_out, n_seq, n_path, n_seq) ||
        overlap(length_out, n_seq, path, paths) || overlap(length_out, n_seq, win_off, n_seq + 1LL) ||
        overlap(length_out, n_seq, cache->pages, pages) ||
-       overlap(length_out, n_seq, k, layers * k_layer_stride + far * k_stride + row) ||
-       overlap(length_out, n_seq, v, layers * v_layer_stride + far * v_stride + row)))
+       over_rows(length_out, n_seq, k, row, k_stride, n_tokens, k_layer_stride, cache->n_layers) ||
+       over_rows(length_out, n_seq, v, row, v_stride, n_tokens, v_layer_stride, cache->n_layers)))
     return set_error(SG_ERR_INVALID_ARGUMENT,
                      "%s: length_out overlaps the cache's lengths or pages, n_path, path, win_off, k "
                      "or v", nm);
