@@ -597,10 +597,10 @@ static int commit(const uint16_t* k, const uint16_t* v, long long k_stride, long
        overlap(length_out, n_seq, path, paths) || overlap(length_out, n_seq, win_off, n_seq + 1LL) ||
        overlap(length_out, n_seq, cache->pages, pages) ||
        over_rows(length_out, n_seq, k, row, k_stride, n_tokens, k_layer_stride, cache->n_layers) ||
-       over_rows(length_out, n_seq, v, row, v_stride, n_tokens, v_layer_stride, cache->n_layers)))
+       over_rows(length_out, n_seq, v, row, v_stride, n_tokens, v_layer_stride, cache->n_layers) ||
+       over_layers(length_out, n_seq, cache)))
     return set_error(SG_ERR_INVALID_ARGUMENT,
-                     "%s: length_out overlaps the cache's lengths or pages, n_path, path, win_off, k "
-                     "or v", nm);
+                     "%s: length_out overlaps the cache, n_path, path, win_off, k or v", nm);
   CommitArgs a;
   a.k = k;
   a.v = v;

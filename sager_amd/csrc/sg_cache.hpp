@@ -121,6 +121,21 @@ static inline bool over_rows(const int* ints, long long n, const T* x, long long
   return false;
 }
 
+// Whether n ints lie over one of a cache's layers.
+static inline bool over_layers(const int* ints, long long n, const sg_kv_cache* c) {
+  const long long m = static_cast<long long>(c->n_pages) * c->n_kv_heads * c->page_size * c->head_dim;
+  return over_rows(ints, n, c->k, m, m, 1, c->layer_stride, c->n_layers) ||
+         over_rows(ints, n, c->v, m, m, 1, c->layer_stride, c->n_layers);
+}
+static inline bool over_layers(const int* ints, long long n, const sg_kv_cache_q8* c) {
+  const long long m = static_cast<long long>(c->n_pages) * c->n_kv_heads * c->page_size * c->head_dim;
+  const long long s = m / kKvGroup, layer = c->layer_stride / kKvGroup;
+  return over_rows(ints, n, c->k, m, m, 1, c->layer_stride, c->n_layers) ||
+         over_rows(ints, n, c->v, m, m, 1, c->layer_stride, c->n_layers) ||
+         over_rows(ints, n, c->k_scale, s, s, 1, layer, c->n_layers) ||
+         over_rows(ints, n, c->v_scale, s, s, 1, layer, c->n_layers);
+}
+
 // Values from a cache's first to its last layer's end.
 static inline long long cache_values(const sg_kv_cache_q8* c) {
   return (c->n_layers - 1) * c->layer_stride +

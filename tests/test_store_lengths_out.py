@@ -1,4 +1,4 @@
-"""New lengths over what a store still reads are refused, in both caches, by path or of whole windows
+"""New lengths over what a store still reads or writes are refused, in both caches, by path or of whole windows
 (CPU: the calls are refused before anything is launched)."""
 import ctypes
 
@@ -43,4 +43,15 @@ def test_over_what_is_read(store, base):
         for t in range(T):
             row = ROOM * base + 2 * (layer * LAYER_LD + t * LD)
             for spot in (row, row + 2 * ROW - 4, row - 4 * N_SEQ + 4, row + ROW):
+                store(spot)
+
+
+def test_over_what_is_written(store, q8):
+    spans = [(1, LAYER, 1), (2, LAYER, 1), (3, LAYER // 32, 2), (4, LAYER // 32, 2)] if q8 else \
+        [(1, LAYER, 2), (2, LAYER, 2)]
+    for i, n, size in spans:
+        step = LAYER_AT // (LAYER // n) * size
+        for layer in range(LAYERS):
+            first = ROOM * i + layer * step
+            for spot in (first, first + n * size - 4, first - 4 * N_SEQ + 4, first + n * size // 2):
                 store(spot)
