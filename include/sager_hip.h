@@ -574,9 +574,10 @@ int sg_attn_tree_f16(const uint16_t* q, const uint16_t* k, const uint16_t* v, lo
  * node outside its window, and a token past the page table or on an absent
  * page, is left out, and so is every token of a cache whose length is less
  * than 0.  length_out[s] = length[s] + n_path[s] (NULL: not written; apart from
- * the cache's lengths and pages, n_path, path and win_off, which the launch
- * still reads).  k and v are not the cache's own memory, and two sequences do
- * not share the pages that are written. */
+ * the rows of k and v, the cache's lengths and pages, n_path, path and win_off,
+ * which the launch still reads, and from the cache's values).  k and v are not
+ * the cache's own memory, and two sequences do not share the pages that are
+ * written. */
 int sg_kv_commit_f16(const uint16_t* k, const uint16_t* v, long long k_stride, long long v_stride,
                      long long k_layer_stride, long long v_layer_stride, const sg_kv_cache* cache,
                      const int* win_off, const int* path, const int* n_path, int* length_out,
