@@ -686,8 +686,10 @@ int sg_kv_read_q8(const sg_kv_cache_q8* cache, const int* first, const int* row_
  * With a parent a window has at most 64 nodes; without one (chains) it may
  * have any number, a prompt's whole chunk.  A quantised value enters both
  * products as code * scale, not rounded; it has to be below 65,504, as all are
- * that commit and append write, or is not a number.  The rest is as for
- * sg_attn_tree_f16.
+ * that commit and append write, or is not a number.  The weights p are rounded
+ * to fp16 for the product with v, and their sum is that of the rounded ones (one
+ * of less than 2^-33 of the row's largest adds to neither).  The rest is as
+ * for sg_attn_tree_f16.
  * Workspace: sg_attn_sliding_workspace_bytes of as many sequences or more, of
  * max_window and max_len as large or larger, and of the same heads, reach and
  * sinks. */

@@ -28,8 +28,7 @@ struct AttnArgs {
   const int *pages, *length, *win_off, *parent;
   uint16_t* out;
   // Parts of cut units, by unit, row block and row: O, and mref (log2) and l.
-  // seq_plan: per sequence its first unit and the parts of its units; then the
-  // steps of a part.
+  // seq_plan: per sequence its first unit and the parts of its units.
   float* part_o;
   float2* part_ml;
   int2* seq_plan;

@@ -53,9 +53,13 @@ __device__ __forceinline__ void settle(T (&x)[N]) {
   for (int i = 0; i < N; ++i) asm volatile("" : "+v"(x[i]));
 }
 
-// Two weights more in a row's sum.  The sum is of the rounded weights, those that
-// the product with V is made with: what rounding a large weight takes from one it
-// then takes from the other.
+// Two weights more in a row's sum.  Weights are rounded to 16 bits, since the
+// matrix cores take such factors: 2^-11 of a weight at the most, as the output's
+// own rounding; in two parts they would double the second product.  The sum is of
+// the rounded weights, those that the product with V is made with: what rounding a
+// large weight takes from one it then takes from the other.  (Against 64 bits the
+// errors are 1.0 to 1.26 times those of 32-bit weights: 2.0e-4 to 2.6e-4 of the
+// outputs' size and 1.9e-4 to 2.1e-4, in batches of one token to a chunk of 4,096.)
 __device__ __forceinline__ float weight_sum(h2 p, float sum) {
   const h2 one = {static_cast<_Float16>(1.f), static_cast<_Float16>(1.f)};
   return __builtin_amdgcn_fdot2(p, one, sum, false);
@@ -770,10 +774,13 @@ constexpr int kSlideRowWaves = 8, kSlideRowTiles = 2;  // 16-row tiles of a wave
 // copied into one of two buffers while the other is computed on.  A step of
 // codes lies in half of the second buffer; 32 of its keys at a time are turned
 // into rounded values and rests of K and of V, which fill the first.  Bound by
-// the matrix cores, whose operands and scores are waited for by no more than two
-// waves a SIMD (4,096 tokens over 4,099 more, windows of 2,048: 16 heads on 2 of
-// 256 155 to 190 us, 890 to 730 TFLOP/s, quantised 280, as the products with the
-// cache are twice as many; 32 heads on 8 of 128 187 to 210 us and 250 to 265).
+// the matrix cores (36 % of the cycles) and the vector instructions between the
+// products (34 %), which no more than two waves a SIMD, for the registers' sake, do
+// in turn (4,096 tokens over 4,099 more, windows of 2,048: 16 heads on 2 of 256 155
+// to 190 us, 890 to 730 TFLOP/s, 32 heads on 8 of 128 187 to 210).  Where each CU
+// has one block the heaviest decides: without a cache the last, which sees twice the
+// mean; over a quantised one the first, which sees little else, at 1.5 times a
+// 16-bit step's time (280 us and 250 to 265 for the two chunks).
 template <int D, bool Q8>
 __global__ void __launch_bounds__(64 * kSlideRowWaves) slide_rows_kernel(const SlideArgs a) {
   typedef SlidePart<D> P;
@@ -1194,6 +1201,7 @@ static int slide_few_each(int dim) { return dim == 256 ? 2 : dim == 128 ? 3 : 4;
 static long long slide_units(int each, long long row_blocks) {
   return 32 * each >= row_blocks ? 32 * each / row_blocks * 8 : 8;
 }
+constexpr int kMostUnits = 0x1FFFFF;  // sequences times kv heads of a call
 static int slide_join_steps(int dim) { return dim / 64 + 1; }  // what a join of wide blocks costs
 constexpr int kFewJoinSteps = 8;                               // of blocks of few rows
 static size_t slide_plan_bytes(int n_seq) {
@@ -1284,6 +1292,7 @@ static SlideLayout slide_layout(int n_seq, int max_window, int max_len, int grou
 // So all numbers of row blocks are gone through, each with the most units that slide_layout has of it.
 static size_t slide_workspace(int n_seq, int max_window, int max_len, int group, int n_kv, int dim,
                               int reach, int sinks) {
+  n_seq = std::min(n_seq, kMostUnits / n_kv);
   const long long rows = static_cast<long long>(max_window) * group;
   const long long near = std::min(max_window, kMaxWindow);  // of what may be a tree
   auto steps = [&](int len, long long before, long long nodes) {
@@ -1434,7 +1443,7 @@ static int attn_slide(const uint16_t* q, const uint16_t* k, const uint16_t* v, l
   // or not), each of which looks through the sequences; a window's rows are 32-bit
   const long long units = static_cast<long long>(n_seq) * n_kv;
   const long long rows = static_cast<long long>(max_window) * (n_heads / n_kv);
-  if (rows > 0x7FFFF000LL || units > 0x1FFFFF)
+  if (rows > 0x7FFFF000LL || units > kMostUnits)
     return set_error(SG_ERR_UNSUPPORTED, "%s: too many sequences, or too long windows", nm);
   const int far = reach == 0 ? 0x7FFFFFFF : reach;
   const SlideLayout l =

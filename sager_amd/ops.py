@@ -931,7 +931,8 @@ class SlidingAttention(TreeAttention):
     """TreeAttention over a sliding window of `reach` positions (0: all) and
     the first `sinks` tokens, over a KvCache or a KvCacheQ8
     (sg_attn_sliding_f16 / _q8).  Without a parent (chains) windows may be
-    longer than 64 tokens: a prompt's chunk."""
+    longer than 64 tokens: a prompt's chunk.  The workspace serves smaller
+    objects of the same heads, reach and sinks too, one call after the other."""
 
     def __init__(self, n_heads, n_kv_heads, head_dim, max_tokens, max_seqs=1, max_window=1,
                  max_len=0, reach=0, sinks=0, device="cuda"):

@@ -95,3 +95,12 @@ def test_trees(lib, seed):
             for call in (less, (most[0], less[1], most[2]), (most[0], most[1], less[2])):
                 assert c.need(*call, given) is None, (c.__dict__, most, call)
                 assert c.bytes(*call) <= given, (c.__dict__, most, call)
+
+
+def test_sizes_past_all_calls(lib):
+    most = 0x7FFFFFFF
+    for heads, n_kv in ((1, 1), (1 << 20, 1 << 10), (most, most), (most, 1)):
+        assert lib.sg_attn_sliding_workspace_bytes(most, most, most, heads, n_kv, 256, 0, 0) >= 0
+    # as many sequences as a call takes
+    f = lib.sg_attn_sliding_workspace_bytes
+    assert f(most, 1, 10 ** 6, 2, 2, 64, 0, 0) == f(0x1FFFFF // 2, 1, 10 ** 6, 2, 2, 64, 0, 0) > 0
