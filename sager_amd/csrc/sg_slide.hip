@@ -1201,7 +1201,8 @@ static int slide_few_each(int dim) { return dim == 256 ? 2 : dim == 128 ? 3 : 4;
 static long long slide_units(int each, long long row_blocks) {
   return 32 * each >= row_blocks ? 32 * each / row_blocks * 8 : 8;
 }
-constexpr int kMostUnits = 0x1FFFFF;  // sequences times kv heads of a call
+constexpr int kMostUnits = 0x1FFFFF;    // sequences times kv heads of a call
+constexpr int kMostRows = 0x7FFFF000;   // tokens of a window times query heads of a kv head
 static int slide_join_steps(int dim) { return dim / 64 + 1; }  // what a join of wide blocks costs
 constexpr int kFewJoinSteps = 8;                               // of blocks of few rows
 static size_t slide_plan_bytes(int n_seq) {
@@ -1293,6 +1294,8 @@ static SlideLayout slide_layout(int n_seq, int max_window, int max_len, int grou
 static size_t slide_workspace(int n_seq, int max_window, int max_len, int group, int n_kv, int dim,
                               int reach, int sinks) {
   n_seq = std::min(n_seq, kMostUnits / n_kv);
+  max_window = std::min(max_window, kMostRows / group);
+  if (n_seq == 0 || max_window == 0) return 0;  // (no such call)
   const long long rows = static_cast<long long>(max_window) * group;
   const long long near = std::min(max_window, kMaxWindow);  // of what may be a tree
   auto steps = [&](int len, long long before, long long nodes) {
@@ -1443,7 +1446,7 @@ static int attn_slide(const uint16_t* q, const uint16_t* k, const uint16_t* v, l
   // or not), each of which looks through the sequences; a window's rows are 32-bit
   const long long units = static_cast<long long>(n_seq) * n_kv;
   const long long rows = static_cast<long long>(max_window) * (n_heads / n_kv);
-  if (rows > 0x7FFFF000LL || units > kMostUnits)
+  if (rows > kMostRows || units > kMostUnits)
     return set_error(SG_ERR_UNSUPPORTED, "%s: too many sequences, or too long windows", nm);
   const int far = reach == 0 ? 0x7FFFFFFF : reach;
   const SlideLayout l =
