@@ -66,8 +66,9 @@ __device__ __forceinline__ void quantise16(const u32x4 (&x)[2], u32x4& code, uin
 // a window's end leave at once, but there are many where one window is long and
 // others are short (1,091 tokens in five windows of up to 1,021, ten layers of 8
 // heads of 128: 68 MB in 19 us, 3.6 TB/s, four of five waves and some two fifths of
-// the vector instructions without a piece); else memory bounds long windows, and
-// four dependent rounds four tokens, 4.4 us.
+// the vector instructions without a piece; over the same buffers again and again
+// 15.6, as one window 13.7); else memory bounds long windows, and four dependent
+// rounds four tokens, 4.4 us.
 __global__ void __launch_bounds__(256) kv_store_q8_kernel(const StoreQ8Args a) {
   const int s = blockIdx.y, l0 = blockIdx.z * kStoreLayers;
   const Window w = window_of(a.win_off, s, a.n_tokens, a.max_window);
