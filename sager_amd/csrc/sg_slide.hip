@@ -780,7 +780,8 @@ constexpr int kSlideRowWaves = 8, kSlideRowTiles = 2;  // 16-row tiles of a wave
 // to 190 us, 890 to 730 TFLOP/s, 32 heads on 8 of 128 187 to 210).  Where each CU
 // has one block the heaviest decides: without a cache the last, which sees twice the
 // mean; over a quantised one the first, which sees little else, at 1.5 times a
-// 16-bit step's time (280 us and 250 to 265 for the two chunks).
+// 16-bit step's time (280 us for the heads of 256; those of 128, two blocks a CU,
+// 250 to 265).
 template <int D, bool Q8>
 __global__ void __launch_bounds__(64 * kSlideRowWaves) slide_rows_kernel(const SlideArgs a) {
   typedef SlidePart<D> P;
